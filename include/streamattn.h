@@ -453,6 +453,38 @@ int sta_pair_moments(const void* q, const void* k, const void* v, int dtype, int
                      int ld_qk, int ld_v, int degree, float scale, int chunk, int shift, int nsplit, float* low_num,
                      float* low_den, void* stream);
 
+/*
+ * Exact causal attention over a sliding window and the first tokens (sinks): row i of a sequence of `lengths[b]` rows
+ * (NULL: n) sees the keys j <= i with i - j < window or j < sinks.
+ *   q [batch][heads][n][d], k [batch][kv_heads][n][d], v [batch][kv_heads][n][dv], heads a multiple of kv_heads (query
+ *   head h reads key head h / (heads / kv_heads)); the last dimension is contiguous, strides [3][3] (host memory) gives
+ *   the element strides of batch, head and row of q, k and v (any values, 0 included).  d, dv <= 128; n <= 2^30.
+ *   out [batch][heads][n][dv] dense, 16-byte aligned, in dtype; rows at or behind a length are zero.
+ *   lse [batch][heads][n] fp32 (or NULL): log2 of every row's sum of weights, for the backward call.
+ *   window >= 1, sinks >= 0 (either may exceed n); scale any finite number.  Products of 16-bit inputs are exact, fp32
+ *   products and all sums and statistics fp32; the weights of 16-bit rows are rounded to 16 bits for the value sums.
+ *   A value that is infinite or NaN reaches the rows that see it and no others.
+ */
+int sta_window_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int heads,
+                         int kv_heads, int64_t n, int d, int dv, const int64_t* strides, float scale, int64_t window,
+                         int64_t sinks, const int32_t* lengths, void* out, float* lse, void* stream);
+
+/* Bytes of sta_window_attention_backward's workspace; -1 for arguments it refuses. */
+int64_t sta_window_backward_bytes(int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv, int64_t window,
+                                  int64_t sinks);
+
+/*
+ * Gradients of sta_window_attention: dq [batch][heads][n][d], dk [batch][kv_heads][n][d], dv [batch][kv_heads][n][dv],
+ * dense, 16-byte aligned, in dtype, from the gradient of out (strides [4][3]: q, k, v, grad), out and lse of the
+ * forward call.  Rows at or behind a length get zero gradients and give none.  Sums are taken in a fixed order:
+ * equal inputs give equal bits.  workspace: caller-allocated, 16-byte aligned (contents undefined before and after).
+ */
+int sta_window_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                  const float* lse, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
+                                  int d, int dv, const int64_t* strides, float scale, int64_t window, int64_t sinks,
+                                  const int32_t* lengths, void* dq, void* dk, void* dv_out, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
 /* Rows per block-attention tile and the moment chunk the library uses for a head dimension D (the
  * chunk argument of sta_block_attention is that chunk for sta_moments' partials, the query block for
  * sta_moments_ws' partials). */

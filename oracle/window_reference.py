@@ -1,0 +1,95 @@
+"""Plain float64 statements of the windowed attention, the head norm with rotation and the token cache, on the CPU, with
+bounds on how far a kernel may be from them.
+
+The bounds are first-order rounding analysis, element by element: u = eps / 2 of the element type for every rounding to
+it (the output, and the weights of 16-bit rows), 2^-24 for every fp32 operation of a sum."""
+
+import math
+
+import torch
+
+F24 = 2.0 ** -24
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def weight_step(dtype):
+    """Relative error of a weight as the value sums take it: 16-bit rows' weights are rounded to 16 bits."""
+    return 0.0 if dtype == torch.float32 else half_step(dtype)
+
+
+def visible(n, length, window, sinks):
+    i = torch.arange(n)[:, None]
+    j = torch.arange(n)[None]
+    return (j <= i) & ((i - j < window) | (j < sinks)) & (i < length)
+
+
+def window_attention(q, k, v, *, window, sinks, scale=None, lengths=None, grad=None):
+    """[B,H,N,D], [B,Hkv,N,D], [B,Hkv,N,Dv]: {"out": (value, bound)} in float64, with "dq", "dk", "dv" if grad is given."""
+    dt = q.dtype
+    u, w = half_step(dt), weight_step(dt)
+    b, h, n, d = q.shape
+    hk = k.shape[1]
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    q, k, v = q.double(), k.double(), v.double()
+    res = {name: [torch.zeros(*shape, dtype=torch.float64) for _ in range(2)]
+           for name, shape in (("out", (b, h, n, v.shape[3])), ("dq", q.shape), ("dk", k.shape), ("dv", v.shape))}
+    for bi in range(b):
+        length = n if lengths is None else max(0, min(n, int(lengths[bi])))
+        see = visible(n, length, window, sinks)
+        for hi in range(h):
+            kk, vv, qq = k[bi, hi * hk // h].clone(), v[bi, hi * hk // h].clone(), q[bi, hi].clone()
+            for x in (kk, vv, qq):
+                x[length:] = 0
+            x = (qq @ kk.T) * scale
+            size = (qq.abs() @ kk.abs().T) * abs(scale)
+            p = torch.where(see, x, -math.inf)
+            p = torch.where(see, torch.exp(p - p.amax(1, keepdim=True)), 0.0)
+            p = p / p.sum(1, keepdim=True).clamp_min(1e-300)
+            # relative error of an fp32 weight: its logit's dot product, the exponent's argument, the row's sum
+            ep = F24 * (2 * (d + 4) * torch.where(see, size, 0.0).amax(1, keepdim=True) + n + 32)
+            o = p @ vv
+            eo = u * o.abs() + (w + ep) * (p @ vv.abs()) + F24 * n * (p @ vv.abs())
+            res["out"][0][bi, hi], res["out"][1][bi, hi] = o, eo
+            if grad is None:
+                continue
+            go = grad[bi, hi].double().clone()
+            go[length:] = 0
+            dp = go @ vv.T
+            delta = (go * o).sum(1, keepdim=True)
+            # error of dp - delta: fp32 dot products, and the output as it was rounded
+            ed = (d + 32) * F24 * (go.abs() @ vv.abs().T) + (go.abs() * (eo + 2 * (d + 32) * F24 * o.abs())).sum(1, keepdim=True)
+            ds = p * (dp - delta) * scale
+            es = (w + ep) * ds.abs() + p * ed * abs(scale)
+            if dt == torch.float16:  # subnormal weights: half a step of 2^-24 over the power of two they carry
+                lift = 2.0 ** min(10, int(math.log2(max(1, min(window + sinks, n)))))
+                tiny = see * (2.0 ** -25 / lift)
+            else:
+                tiny = see * 0.0
+            dv, ev = p.T @ go, ((w + ep) * p + tiny).T @ go.abs()
+            dk, ek = ds.T @ qq, (es + tiny * abs(scale)).T @ qq.abs()
+            dq, eq = ds @ kk, (es + tiny * abs(scale)) @ kk.abs()
+            n_sum = F24 * n
+            res["dq"][0][bi, hi], res["dq"][1][bi, hi] = dq, eq + n_sum * (ds.abs() @ kk.abs())
+            for name, val, err, mag in (("dk", dk, ek, ds.abs().T @ qq.abs()), ("dv", dv, ev, p.T @ go.abs())):
+                res[name][0][bi, hi * hk // h] += val
+                res[name][1][bi, hi * hk // h] += err + n_sum * (h // hk) * mag
+    for name in ("dq", "dk", "dv"):
+        res[name][1].add_(u * res[name][0].abs())
+        if dt == torch.float16:
+            res[name][1].add_(2.0 ** -25)  # results below fp16's normal range
+    if dt == torch.float16:
+        res["out"][1].add_(2.0 ** -25)
+    return {name: tuple(x) for name, x in res.items() if grad is not None or name == "out"}
+
+
+def over(got, want):
+    """How many times over its bound the worst element is; infinite where finiteness differs."""
+    value, bound = want
+    got = got.detach().double().cpu()
+    if not torch.isfinite(got).all():
+        return math.inf
+    # 1e-30: elements with nothing to add up are zero on both sides
+    return float(((got - value).abs() / (bound * 1.05 + 1e-30)).max()) if got.numel() else 0.0

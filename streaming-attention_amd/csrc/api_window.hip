@@ -1,0 +1,169 @@
+// Entry points of the windowed attention (see include/streamattn.h): argument checks, the gradient's plan and the
+// choice of the compiled configuration.
+#include <cmath>
+
+#include "api_common.hpp"
+#include "window_attn.hip"
+
+using namespace sta_api;
+
+namespace sta_api {
+template <int P, int IN>
+int launch_window_forward(const sta::WinArgs& a, hipStream_t s);
+template <int P, int IN>
+int launch_window_backward(const sta::WinArgs& a, hipStream_t s);
+}  // namespace sta_api
+
+namespace {
+
+constexpr int kMaxWindowD = 128;
+constexpr int64_t kMaxWindowRows = int64_t(1) << 30;  // rows and their sums with a window stay in 32 bits
+
+int element_size(int dtype) { return dtype == STA_F32 ? 4 : 2; }
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+sta::WinRows rows_of(const void* p, const int64_t* strides, int dtype) {
+  sta::WinRows r;
+  r.p = p;
+  r.sb = strides[0];
+  r.sh = strides[1];
+  r.sn = strides[2];
+  const int64_t es = element_size(dtype);
+  r.aligned = aligned16(p) && r.sb * es % 16 == 0 && r.sh * es % 16 == 0 && r.sn * es % 16 == 0;
+  return r;
+}
+
+// The shape part of the arguments; STA_OK or what is wrong with it.
+int window_shape(sta::WinArgs& a, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv, float scale,
+                 int64_t window, int64_t sinks) {
+  if (batch < 1 || heads < 1 || kv_heads < 1 || n < 1 || d < 1 || dv < 1 || heads % kv_heads != 0)
+    return STA_ERR_SHAPE;
+  if (window < 1 || sinks < 0 || !std::isfinite(scale)) return STA_ERR_ARG;
+  if (d > kMaxWindowD || dv > kMaxWindowD || n > kMaxWindowRows || batch > 0x7fffffff) return STA_ERR_UNSUPPORTED;
+  a = sta::WinArgs{};
+  a.batch = static_cast<int>(batch);
+  a.heads = heads;
+  a.group = heads / kv_heads;
+  a.n = static_cast<int>(n);
+  a.d = d;
+  a.dv = dv;
+  a.window = static_cast<int>(window < n ? window : n);
+  a.sinks = static_cast<int>(sinks < n ? sinks : n);
+  a.scale = scale;
+  a.c = std::fabs(scale) * 1.44269504088896340736f;
+  a.tiles = static_cast<int>((n + sta::WIN_ROWS - 1) / sta::WIN_ROWS);
+  a.lift = a.drop = 1.f;
+  return STA_OK;
+}
+
+// How the rows behind the window of the sinks are dealt out: chunks of at least 256 rows, at most about two
+// workgroups a compute unit.
+void plan_sinks(sta::WinArgs& a) {
+  const int64_t behind = a.n - a.window;
+  if (a.sinks == 0 || behind <= 0) return;
+  const int64_t bkv = static_cast<int64_t>(a.batch) * (a.heads / a.group);
+  a.sink_rows = a.sinks;
+  a.sink_tiles = (a.sinks + sta::WIN_ROWS - 1) / sta::WIN_ROWS;
+  int64_t chunks = 512 / (bkv * a.sink_tiles);
+  if (chunks > (behind + 255) / 256) chunks = (behind + 255) / 256;
+  if (chunks < 1) chunks = 1;
+  const int64_t rows = ((behind + chunks - 1) / chunks + 31) / 32 * 32;
+  a.far_rows = static_cast<int>(rows);
+  a.far_chunks = static_cast<int>((behind + rows - 1) / rows);
+}
+
+int64_t delta_floats(const sta::WinArgs& a) {
+  return (static_cast<int64_t>(a.batch) * a.heads * a.n + 63) / 64 * 64;
+}
+
+int64_t part_floats(const sta::WinArgs& a) {
+  if (a.far_chunks == 0) return 0;
+  return static_cast<int64_t>(a.batch) * (a.heads / a.group) * (a.far_chunks + 1) * a.sink_rows * (a.d + a.dv);
+}
+
+template <int P>
+int by_type(bool backward, const sta::WinArgs& a, int dtype, hipStream_t s) {
+  if (dtype == STA_F32)
+    return backward ? launch_window_backward<P, sta::F32>(a, s) : launch_window_forward<P, sta::F32>(a, s);
+  if (dtype == STA_BF16)
+    return backward ? launch_window_backward<P, sta::BF16>(a, s) : launch_window_forward<P, sta::BF16>(a, s);
+  return backward ? launch_window_backward<P, sta::F16>(a, s) : launch_window_forward<P, sta::F16>(a, s);
+}
+
+int dispatch(bool backward, const sta::WinArgs& a, int dtype, void* stream) {
+  const int width = a.d > a.dv ? a.d : a.dv;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (width <= 32) return by_type<32>(backward, a, dtype, s);
+  if (width <= 64) return by_type<64>(backward, a, dtype, s);
+  if (width <= 96) return by_type<96>(backward, a, dtype, s);
+  return by_type<128>(backward, a, dtype, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sta_window_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int heads,
+                         int kv_heads, int64_t n, int d, int dv, const int64_t* strides, float scale, int64_t window,
+                         int64_t sinks, const int32_t* lengths, void* out, float* lse, void* stream) {
+  if (!q || !k || !v || !out || !strides || !aligned16(out)) return STA_ERR_ARG;
+  if (!dtype_ok(dtype)) return STA_ERR_DTYPE;
+  sta::WinArgs a;
+  if (const int st = window_shape(a, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
+  a.q = rows_of(q, strides, dtype);
+  a.k = rows_of(k, strides + 3, dtype);
+  a.v = rows_of(v, strides + 6, dtype);
+  a.lengths = lengths;
+  a.out = out;
+  a.lse = lse;
+  return dispatch(false, a, dtype, stream);
+}
+
+int64_t sta_window_backward_bytes(int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv, int64_t window,
+                                  int64_t sinks) {
+  sta::WinArgs a;
+  if (window_shape(a, batch, heads, kv_heads, n, d, dv, 1.f, window, sinks) != STA_OK) return -1;
+  plan_sinks(a);
+  return 4 * (delta_floats(a) + part_floats(a));
+}
+
+int sta_window_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
+                                  const float* lse, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
+                                  int d, int dv, const int64_t* strides, float scale, int64_t window, int64_t sinks,
+                                  const int32_t* lengths, void* dq, void* dk, void* dv_out, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  if (!grad || !q || !k || !v || !out || !lse || !strides || !dq || !dk || !dv_out || !workspace) return STA_ERR_ARG;
+  if (!aligned16(out) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv_out) || !aligned16(workspace))
+    return STA_ERR_ARG;
+  if (!dtype_ok(dtype)) return STA_ERR_DTYPE;
+  sta::WinArgs a;
+  if (const int st = window_shape(a, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
+  plan_sinks(a);
+  if (workspace_bytes < 4 * (delta_floats(a) + part_floats(a))) return STA_ERR_SCRATCH;
+  a.q = rows_of(q, strides, dtype);
+  a.k = rows_of(k, strides + 3, dtype);
+  a.v = rows_of(v, strides + 6, dtype);
+  a.go = rows_of(grad, strides + 9, dtype);
+  a.lengths = lengths;
+  a.out = const_cast<void*>(out);
+  a.lse = const_cast<float*>(lse);
+  a.delta = static_cast<float*>(workspace);
+  a.part = a.delta + delta_floats(a);
+  a.dq = dq;
+  a.dk = dk;
+  a.dv_out = dv_out;
+  if (dtype == STA_F16) {
+    // fp16 weights of long rows are subnormal (1 / 4096 has 10 bits left): they and their gradients are carried times
+    // a power of two near the number of keys, at most 2^10, so that weights near 1 times gradients up to 64 fit;
+    // rows beyond that come out infinite and are taken again in fp32
+    const int64_t keys = static_cast<int64_t>(a.window) + a.sinks < a.n ? a.window + a.sinks : a.n;
+    int e = 0;
+    while (e < 10 && (int64_t(2) << e) <= keys) ++e;
+    a.lift = std::ldexp(1.f, e);
+    a.drop = std::ldexp(1.f, -e);
+  }
+  return dispatch(true, a, dtype, stream);
+}
+
+}  // extern "C"

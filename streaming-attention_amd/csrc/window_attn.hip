@@ -1,0 +1,883 @@
+// Exact causal attention over a sliding window and a few first tokens (sinks), with its gradients.
+//
+// Row i of a sequence sees the keys V(i) = {j <= i : i - j < window or j < sinks}:
+//   p_ij = exp(s q_i.k_j - L_i), L_i = log sum_{j in V(i)} exp(s q_i.k_j),   o_i = sum_{j in V(i)} p_ij v_j
+//   dv_j = sum_i p_ij do_i,   D_i = do_i.o_i,   ds_ij = s p_ij (do_i.v_j - D_i)
+//   dq_i = sum_j ds_ij k_j,   dk_j = sum_i ds_ij q_i
+// Query heads share a key head in groups of heads / kv_heads; dk and dv are the sums over the group.  Rows at or
+// behind a sequence's length are no part of it: outputs and gradients there are zero, whatever the inputs hold.
+//
+// Matrix-core layout (v_mfma_f32_32x32x16 for 16-bit rows, 32x32x2_f32 eight times over the same operands for
+// fp32): lane l = 32 h + i holds A[i][8 h + j], B[8 h + j][i], j = 0..7, and D[8 (r / 4) + 4 h + r % 4][i] in
+// accumulator element r.  The logits are taken transposed where the next product contracts over keys (X^T = K Q^T: a
+// lane holds 16 keys of one row) and plain where it contracts over rows (X = Q K^T: 16 rows of one key), so that
+// the weights in accumulator elements 8 t .. 8 t + 7 are the B operand of the next product as they stand, for the
+// contraction order {4 h + 0..3, 8 + 4 h + 0..3} of 16 keys (rows); the A operand in that order is a transposed
+// read of the staged rows (ds_read_b64_tr_b16: 4 rows x 16 columns a 16-lane group; 32-bit reads for fp32).
+//
+// LDS rows are P elements wide without padding; 16-byte chunk c of row r sits at c ^ win_swizzle(r), which spreads
+// both 16 consecutive rows at one chunk (row reads) and 4 rows at 4 chunks (transposed reads) over all 64 banks.
+//
+// Hidden pairs are left out by selects, never by arithmetic on their logits.  A tile's products still multiply hidden
+// pairs' zero weights with their values, so an infinity or NaN in a value that some rows of a tile see would reach
+// those that do not: a result row that is not finite is taken again over its visible pairs alone (win_*_row).
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace sta {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef _Float16 win_half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 win_half2 __attribute__((ext_vector_type(2)));
+typedef short win_short4 __attribute__((ext_vector_type(4)));
+
+// rows of [batch][heads][n][width]: element strides; `aligned`: every row starts on 16 bytes
+struct WinRows {
+  const void* p;
+  int64_t sb, sh, sn;
+  int aligned;
+};
+
+struct WinArgs {
+  WinRows q, k, v, go;     // go: the output's gradient
+  int heads, group;        // query heads, query heads per key head
+  int batch, n, d, dv;
+  int window, sinks;       // 1 <= window <= n, 0 <= sinks <= n (the host clamps both to n)
+  float c;                 // |scale| log2(e): weights are exp2(c x - lse), x of queries with the scale's sign
+  float scale;             // the scale itself
+  const int* lengths;      // [batch] or null
+  void* out;               // [batch][heads][n][dv]
+  float* lse;              // [batch][heads][n]: log2 of the row's sum of weights, or null
+  float* delta;            // [batch][heads][n]: D_i
+  void *dq, *dk, *dv_out;  // [batch][heads][n][d], [batch][kv heads][n][d | dv]
+  int tiles;               // tiles of 128 rows (keys)
+  // gradients of sinks behind their window: rows [j + window, n) of the first sink_tiles key tiles, far_chunks
+  // workgroups a tile with far_rows rows each; sums part [batch kv_heads][far_chunks + 1][sink_rows][d + dv]
+  int sink_tiles, far_chunks, far_rows, sink_rows;
+  float* part;
+  float lift, drop;        // 2^e and 2^-e: the weights' scale in fp16 gradients
+};
+
+constexpr int WIN_ROWS = 128;
+
+template <int ES>
+__host__ __device__ constexpr int win_chunks(int p) { return p * ES / 16; }
+
+// see the top of the file; needs only bits 0..3 of the row
+template <int CH>
+__device__ __forceinline__ int win_swizzle(int row) {
+  if constexpr (CH % 16 == 0) return ((row & 3) << 2) | ((row >> 2) & 3);
+  if constexpr (CH % 8 == 0) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+  return (row >> 2) & 3;
+}
+
+template <int IN>
+struct WinFrag {  // 8 contraction elements of a lane
+  uint4 w[IN == F32 ? 2 : 1];
+};
+
+template <int IN>
+__device__ __forceinline__ void win_mma(floatx16& acc, const WinFrag<IN>& a, const WinFrag<IN>& b) {
+  if constexpr (IN == F32) {
+    const float* x = reinterpret_cast<const float*>(a.w);
+    const float* y = reinterpret_cast<const float*>(b.w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], acc, 0, 0, 0);
+  } else if constexpr (IN == F16) {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(win_half8, a.w[0]),
+                                                 __builtin_bit_cast(win_half8, b.w[0]), acc, 0, 0, 0);
+  } else {
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a.w[0]),
+                                                  __builtin_bit_cast(bf16x8, b.w[0]), acc, 0, 0, 0);
+  }
+}
+
+// accumulator elements 8 t .. 8 t + 7 as an operand (16 bits: each rounded to nearest even)
+template <int IN>
+__device__ __forceinline__ WinFrag<IN> win_operand(const floatx16& x, int t) {
+  WinFrag<IN> f;
+  if constexpr (IN == F32) {
+    f.w[0] = uint4{__float_as_uint(x[8 * t]), __float_as_uint(x[8 * t + 1]), __float_as_uint(x[8 * t + 2]),
+                   __float_as_uint(x[8 * t + 3])};
+    f.w[1] = uint4{__float_as_uint(x[8 * t + 4]), __float_as_uint(x[8 * t + 5]), __float_as_uint(x[8 * t + 6]),
+                   __float_as_uint(x[8 * t + 7])};
+  } else {
+    uint32_t u[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const floatx2 y = floatx2{x[8 * t + 2 * j], x[8 * t + 2 * j + 1]};
+      if constexpr (IN == F16)
+        u[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, win_half2));
+      else
+        u[j] = pk_bf16(y[0], y[1]);
+    }
+    f.w[0] = uint4{u[0], u[1], u[2], u[3]};
+  }
+  return f;
+}
+
+// 16 bytes at column `col` of a row, columns at or behind `width` zero
+template <int ES>
+__device__ __forceinline__ uint4 win_chunk(const void* row, int col, int width, int aligned) {
+  constexpr int E = 16 / ES;
+  const char* p = static_cast<const char*>(row) + static_cast<int64_t>(col) * ES;
+  if (aligned && col + E <= width) return *reinterpret_cast<const uint4*>(p);
+  uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (col + e < width) {
+      if constexpr (ES == 4)
+        u[e] = reinterpret_cast<const uint32_t*>(p)[e];
+      else
+        u[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
+    }
+  return uint4{u[0], u[1], u[2], u[3]};
+}
+
+template <int ES>
+__device__ __forceinline__ const char* win_row(const WinRows& t, int64_t b, int64_t h, int64_t row) {
+  return static_cast<const char*>(t.p) + (b * t.sb + h * t.sh + row * t.sn) * ES;
+}
+
+// Staging of ROWS rows of a tile by 256 threads: registers first (load), LDS when the tile before is done with (put)
+template <int P, int IN, int ROWS>
+struct WinStage {
+  static constexpr int ES = IN == F32 ? 4 : 2, E = 16 / ES, CH = win_chunks<ES>(P);
+  static constexpr int COUNT = (ROWS * CH + 255) / 256;
+  uint4 u[COUNT];
+  // rows [row0, row0 + ROWS) of head (b, h); rows at or behind `limit` and columns behind `width` are zero
+  __device__ __forceinline__ void load(const WinRows& t, int64_t b, int64_t h, int row0, int limit, int width) {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const int at = threadIdx.x + 256 * i, r = at / CH, c = at % CH;
+      u[i] = uint4{0u, 0u, 0u, 0u};
+      if ((ROWS * CH % 256 == 0 || at < ROWS * CH) && row0 + r < limit && c * E < width)
+        u[i] = win_chunk<ES>(win_row<ES>(t, b, h, row0 + r), c * E, width, t.aligned);
+    }
+  }
+  __device__ __forceinline__ void put(uint4* lds) const {
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) {
+      const int at = threadIdx.x + 256 * i, r = at / CH, c = at % CH;
+      if (ROWS * CH % 256 == 0 || at < ROWS * CH) lds[r * CH + (c ^ win_swizzle<CH>(r))] = u[i];
+    }
+  }
+};
+
+// A (or B) operand of 16 dimensions [16 s, 16 s + 16) of staged row r
+template <int P, int IN>
+__device__ __forceinline__ WinFrag<IN> win_read_row(const uint4* lds, int r, int s, int h) {
+  constexpr int CH = win_chunks<IN == F32 ? 4 : 2>(P);
+  WinFrag<IN> f;
+  const int x = win_swizzle<CH>(r);
+  if constexpr (IN == F32) {
+    f.w[0] = lds[r * CH + ((4 * s + 2 * h) ^ x)];
+    f.w[1] = lds[r * CH + ((4 * s + 2 * h + 1) ^ x)];
+  } else {
+    f.w[0] = lds[r * CH + ((2 * s + h) ^ x)];
+  }
+  return f;
+}
+
+// A operand of columns [32 mt, 32 mt + 32) over staged rows [r0, r0 + 16) (a multiple of 16) in the contraction order
+// of the accumulators
+template <int P, int IN>
+__device__ __forceinline__ WinFrag<IN> win_read_columns(const uint4* lds, int r0, int mt, int lane) {
+  constexpr int CH = win_chunks<IN == F32 ? 4 : 2>(P);
+  const int h = lane >> 5;
+  WinFrag<IN> f;
+  if constexpr (IN == F32) {
+    uint32_t u[8];
+    const int col = 32 * mt + (lane & 31);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = r0 + 8 * (j >> 2) + 4 * h + (j & 3);
+      u[j] = reinterpret_cast<const uint32_t*>(lds)[4 * (r * CH + ((col >> 2) ^ win_swizzle<CH>(r))) + (col & 3)];
+    }
+    f.w[0] = uint4{u[0], u[1], u[2], u[3]};
+    f.w[1] = uint4{u[4], u[5], u[6], u[7]};
+  } else {
+    const int col = 32 * mt + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    uint32_t u[4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r = r0 + 8 * t + 4 * h + ((lane & 15) >> 2);
+      const int at = 8 * (r * CH + ((col >> 3) ^ win_swizzle<CH>(r))) + (col & 7);
+      typedef __attribute__((address_space(3))) win_short4* lds_ptr;
+      const win_short4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_ptr)(reinterpret_cast<short*>(const_cast<uint4*>(lds)) + at));
+      const uint2 y = __builtin_bit_cast(uint2, x);
+      u[2 * t] = y.x;
+      u[2 * t + 1] = y.y;
+    }
+    f.w[0] = uint4{u[0], u[1], u[2], u[3]};
+  }
+  return f;
+}
+
+// 8 dimensions at column 16 s + 8 h of a row in memory, with the sign of the scale in `flip`
+template <int IN>
+__device__ __forceinline__ WinFrag<IN> win_load_row(const void* row, int s, int h, int width, int aligned,
+                                                    uint32_t flip) {
+  constexpr int ES = IN == F32 ? 4 : 2;
+  WinFrag<IN> f;
+#pragma unroll
+  for (int i = 0; i < (IN == F32 ? 2 : 1); ++i) {
+    const int col = 16 * s + 8 * h + 4 * i;
+    uint4 u = uint4{0u, 0u, 0u, 0u};
+    if (col < width) u = win_chunk<ES>(row, col, width, aligned);
+    f.w[i] = uint4{u.x ^ flip, u.y ^ flip, u.z ^ flip, u.w ^ flip};
+  }
+  return f;
+}
+
+__device__ __forceinline__ bool win_finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+// four values of a row at column col (a multiple of 4) of a dense [.., width] tensor
+template <int IN>
+__device__ __forceinline__ void win_store4(void* base, int64_t row_at, int col, int width, float a, float b, float c,
+                                           float d) {
+  const int64_t at = row_at + col;
+  if (col + 4 <= width && (width & 3) == 0) {
+    if constexpr (IN == F32) {
+      *reinterpret_cast<floatx4*>(static_cast<float*>(base) + at) = floatx4{a, b, c, d};
+    } else {
+      uint2 u;
+      if constexpr (IN == F16) {
+        u.x = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{a, b}), win_half2));
+        u.y = __builtin_bit_cast(uint32_t, __builtin_convertvector((floatx2{c, d}), win_half2));
+      } else {
+        u.x = pk_bf16(a, b);
+        u.y = pk_bf16(c, d);
+      }
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + at) = u;
+    }
+    return;
+  }
+  if (col < width) store_elem(base, at, IN, a);
+  if (col + 1 < width) store_elem(base, at + 1, IN, b);
+  if (col + 2 < width) store_elem(base, at + 2, IN, c);
+  if (col + 3 < width) store_elem(base, at + 3, IN, d);
+}
+
+__device__ __forceinline__ float win_wave_sum(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+  return x;
+}
+
+template <int IN>
+__device__ __forceinline__ float win_dot(const void* x, const void* y, int width) {
+  float s = 0.f;
+  for (int c = 0; c < width; ++c) s = fmaf(load_elem(x, c, IN), load_elem(y, c, IN), s);
+  return s;
+}
+
+__device__ __forceinline__ int win_length(const WinArgs& a, int b) {
+  if (!a.lengths) return a.n;
+  const int len = a.lengths[b];
+  return len < 0 ? 0 : (len > a.n ? a.n : len);
+}
+
+// Visible keys of row i in order: the sinks that the window has passed, then the window.
+struct WinKeys {
+  int sinks, first, count;
+  __device__ __forceinline__ WinKeys(const WinArgs& a, int i) {
+    first = i - a.window + 1 > 0 ? i - a.window + 1 : 0;
+    sinks = a.sinks < first ? a.sinks : first;
+    count = sinks + i - first + 1;
+  }
+  __device__ __forceinline__ int key(int t) const { return t < sinks ? t : first + t - sinks; }
+};
+
+// One row by one wave over its visible keys, in fp32 without matrix instructions.
+template <int IN>
+__device__ void win_forward_row(const WinArgs& a, int b, int h, int i) {
+  constexpr int ES = IN == F32 ? 4 : 2;
+  const int lane = threadIdx.x & 63;
+  const WinKeys keys(a, i);
+  const void* q = win_row<ES>(a.q, b, h, i);
+  float m = -__builtin_inff();
+  for (int t = lane; t < keys.count; t += 64)
+    m = fmaxf(m, a.scale * win_dot<IN>(q, win_row<ES>(a.k, b, h / a.group, keys.key(t)), a.d));
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float l = 0.f, acc[2] = {0.f, 0.f};
+  for (int t0 = 0; t0 < keys.count; t0 += 64) {
+    const int t = t0 + lane;
+    float p = 0.f;
+    if (t < keys.count)
+      p = expf(a.scale * win_dot<IN>(q, win_row<ES>(a.k, b, h / a.group, keys.key(t)), a.d) - m);
+    l += p;
+    for (int u = 0; u < 64 && t0 + u < keys.count; ++u) {
+      const float w = __shfl(p, u);
+      const void* v = win_row<ES>(a.v, b, h / a.group, keys.key(t0 + u));
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < a.dv) acc[e] = fmaf(w, load_elem(v, lane + 64 * e, IN), acc[e]);
+    }
+  }
+  l = win_wave_sum(l);
+  const int64_t row = (static_cast<int64_t>(b) * a.heads + h) * a.n + i;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + 64 * e < a.dv) store_elem(a.out, row * a.dv + lane + 64 * e, IN, acc[e] / l);
+  if (a.lse && lane == 0) a.lse[row] = m * 1.44269504f + log2f(l);
+}
+
+// Which (batch, query head, tile) a workgroup takes: the heads of a group and the neighbouring tiles of a head on one
+// XCD, whose L2 then holds the keys they share; the last tiles (most keys) first.
+__device__ __forceinline__ void win_place(const WinArgs& a, int& b, int& h, int& tile) {
+  int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int g = id % a.group;
+  id /= a.group;
+  tile = a.tiles - 1 - id % a.tiles;
+  id /= a.tiles;
+  const int kv = a.heads / a.group;
+  h = id % kv * a.group + g;
+  b = id / kv;
+}
+
+template <int IN>
+__host__ __device__ constexpr int win_keys() { return IN == F32 ? 32 : 64; }
+
+// One workgroup per 128 query rows of a head, 32 a wave; keys staged win_keys at a time, the next tile's rows in
+// registers while this one computes.
+template <int P, int IN>
+__global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forward_kernel(const WinArgs a) {
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN>(), NSUB = BK / 32, MT = P / 32;
+  __shared__ uint4 ks[BK * CH], vs[BK * CH];
+  int b, h, tile;
+  win_place(a, b, h, tile);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
+  const int len = win_length(a, b), hk = h / a.group;
+  const int r0 = tile * WIN_ROWS, w0 = r0 + 32 * wave, row = w0 + (lane & 31);
+  const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
+
+  floatx16 acc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
+  float m = -1e30f, l = 0.f;  // finite: exp2(m_old - m_new) is 0 or at most 1, never a NaN
+
+  if (r0 < len) {
+    WinFrag<IN> qf[P / 16];
+    const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
+    const char* qrow = win_row<ES>(a.q, b, h, row < len ? row : 0);
+#pragma unroll
+    for (int s = 0; s < P / 16; ++s) qf[s] = win_load_row<IN>(qrow, s, hh, row < len ? a.d : 0, a.q.aligned, flip);
+
+    const int last = (r0 + WIN_ROWS < len ? r0 + WIN_ROWS : len) - 1;
+    const int t_lo = (r0 - a.window + 1 > 0 ? r0 - a.window + 1 : 0) / BK;
+    int n_sink = (a.sinks + BK - 1) / BK;
+    if (n_sink > t_lo) n_sink = t_lo;
+    const int count = n_sink + last / BK - t_lo + 1;
+    WinStage<P, IN, BK> kst, vst;
+    auto first_key = [&](int it) { return (it < n_sink ? it : t_lo + it - n_sink) * BK; };
+    kst.load(a.k, b, hk, first_key(0), len, a.d);
+    vst.load(a.v, b, hk, first_key(0), len, a.dv);
+    for (int it = 0; it < count; ++it) {
+      __syncthreads();
+      kst.put(ks);
+      vst.put(vs);
+      __syncthreads();
+      const int key0 = first_key(it);
+      if (it + 1 < count) {
+        kst.load(a.k, b, hk, first_key(it + 1), len, a.d);
+        vst.load(a.v, b, hk, first_key(it + 1), len, a.dv);
+      }
+      // of the wave's rows, does one see one of the keys; do all see all of them
+      const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
+      if (!some) continue;
+      const bool all = key0 + BK - 1 <= w0 && (w0 + 31 - key0 < a.window || key0 + BK <= a.sinks);
+      floatx16 x[NSUB];
+#pragma unroll
+      for (int sub = 0; sub < NSUB; ++sub) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[sub][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < P / 16; ++s)
+          win_mma<IN>(x[sub], win_read_row<P, IN>(ks, 32 * sub + (lane & 31), s, hh), qf[s]);
+      }
+      auto seen = [&](int sub, int i) {
+        const int key = key0 + 32 * sub + 8 * (i >> 2) + 4 * hh + (i & 3);
+        return key <= row && (row - key < a.window || key < a.sinks);
+      };
+      float top = m;
+      if (all) {
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, x[sub][i]);
+      } else {
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, seen(sub, i) ? x[sub][i] : -1e30f);
+      }
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__any(top > m)) {
+        const float shrink = __builtin_amdgcn_exp2f((m - top) * a.c);
+        l *= shrink;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[mt][i] *= shrink;
+        m = top;
+      }
+      const float mc = m * a.c;
+#pragma unroll
+      for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[sub][i] = __builtin_amdgcn_exp2f(fmaf(x[sub][i], a.c, -mc));
+      if (!all) {
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[sub][i] = seen(sub, i) ? x[sub][i] : 0.f;
+      }
+#pragma unroll
+      for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l += x[sub][i];
+#pragma unroll
+      for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const WinFrag<IN> p = win_operand<IN>(x[sub], t);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            win_mma<IN>(acc[mt], win_read_columns<P, IN>(vs, 32 * sub + 16 * t, mt, lane), p);
+        }
+    }
+    l += __shfl_xor(l, 32);
+  }
+
+  const bool in = row < len;
+  float inv = 0.f;
+  int bad = 0;
+  if (in) {
+    inv = 1.f / l;
+    bad = !(l > 0.f && win_finite(l));
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bad |= !win_finite(acc[mt][i]);
+  }
+  bad |= __shfl_xor(bad, 32);
+  if (row < a.n && !bad) {
+    const int64_t at = (head_row + row) * a.dv;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = 32 * mt + 8 * r + 4 * hh;
+        if (col < a.dv)
+          win_store4<IN>(a.out, at, col, a.dv, in ? acc[mt][4 * r] * inv : 0.f, in ? acc[mt][4 * r + 1] * inv : 0.f,
+                         in ? acc[mt][4 * r + 2] * inv : 0.f, in ? acc[mt][4 * r + 3] * inv : 0.f);
+      }
+    if (a.lse && hh == 0) a.lse[head_row + row] = in ? m * a.c + __builtin_amdgcn_logf(l) : 0.f;
+  }
+  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1)
+    win_forward_row<IN>(a, b, h, w0 + __builtin_ctzll(todo));
+}
+
+// dq_i over the visible keys of row i by one wave; `delta` is D_i.
+template <int IN>
+__device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
+  constexpr int ES = IN == F32 ? 4 : 2;
+  const int lane = threadIdx.x & 63, hk = h / a.group;
+  const WinKeys keys(a, i);
+  const void* q = win_row<ES>(a.q, b, h, i);
+  const void* go = win_row<ES>(a.go, b, h, i);
+  const int64_t row = (static_cast<int64_t>(b) * a.heads + h) * a.n + i;
+  const float lse = a.lse[row];
+  float acc[2] = {0.f, 0.f};
+  for (int t0 = 0; t0 < keys.count; t0 += 64) {
+    const int t = t0 + lane;
+    float ds = 0.f;
+    if (t < keys.count) {
+      const int key = keys.key(t);
+      const float x = a.scale * win_dot<IN>(q, win_row<ES>(a.k, b, hk, key), a.d);
+      ds = exp2f(fmaf(x, 1.44269504f, -lse)) * (win_dot<IN>(go, win_row<ES>(a.v, b, hk, key), a.dv) - delta);
+    }
+    for (int u = 0; u < 64 && t0 + u < keys.count; ++u) {
+      const float w = __shfl(ds, u);
+      const void* k = win_row<ES>(a.k, b, hk, keys.key(t0 + u));
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < a.d) acc[e] = fmaf(w, load_elem(k, lane + 64 * e, IN), acc[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (lane + 64 * e < a.d) store_elem(a.dq, row * a.d + lane + 64 * e, IN, a.scale * acc[e]);
+}
+
+// dq and D: the forward kernel's walk over the keys with the rows' statistics given.
+template <int P, int IN>
+__global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const WinArgs a) {
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN>(), NSUB = BK / 32, MT = P / 32;
+  __shared__ uint4 ks[BK * CH], vs[BK * CH];
+  int b, h, tile;
+  win_place(a, b, h, tile);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
+  const int len = win_length(a, b), hk = h / a.group;
+  const int r0 = tile * WIN_ROWS, w0 = r0 + 32 * wave, row = w0 + (lane & 31);
+  const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
+  const bool in = row < len;
+
+  floatx16 acc[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
+  float delta = 0.f;
+
+  if (r0 < len) {
+    WinFrag<IN> qf[P / 16], gf[P / 16];
+    const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
+    const char* qrow = win_row<ES>(a.q, b, h, in ? row : 0);
+    const char* grow = win_row<ES>(a.go, b, h, in ? row : 0);
+    const char* orow = static_cast<const char*>(a.out) + (head_row + (in ? row : 0)) * a.dv * ES;
+    const int out_aligned = (a.dv * ES) % 16 == 0;
+#pragma unroll
+    for (int s = 0; s < P / 16; ++s) {
+      qf[s] = win_load_row<IN>(qrow, s, hh, in ? a.d : 0, a.q.aligned, flip);
+      gf[s] = win_load_row<IN>(grow, s, hh, in ? a.dv : 0, a.go.aligned, 0u);
+      const WinFrag<IN> o = win_load_row<IN>(orow, s, hh, in ? a.dv : 0, out_aligned, 0u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta = fmaf(load_elem(&gf[s], j, IN), load_elem(&o, j, IN), delta);
+    }
+    delta += __shfl_xor(delta, 32);
+    const float lse = in ? a.lse[head_row + row] : 0.f;
+    if (in && hh == 0) a.delta[head_row + row] = delta;
+
+    const int last = (r0 + WIN_ROWS < len ? r0 + WIN_ROWS : len) - 1;
+    const int t_lo = (r0 - a.window + 1 > 0 ? r0 - a.window + 1 : 0) / BK;
+    int n_sink = (a.sinks + BK - 1) / BK;
+    if (n_sink > t_lo) n_sink = t_lo;
+    const int count = n_sink + last / BK - t_lo + 1;
+    WinStage<P, IN, BK> kst, vst;
+    auto first_key = [&](int it) { return (it < n_sink ? it : t_lo + it - n_sink) * BK; };
+    kst.load(a.k, b, hk, first_key(0), len, a.d);
+    vst.load(a.v, b, hk, first_key(0), len, a.dv);
+    const float shift = __builtin_amdgcn_logf(a.lift) - lse;
+    for (int it = 0; it < count; ++it) {
+      __syncthreads();
+      kst.put(ks);
+      vst.put(vs);
+      __syncthreads();
+      const int key0 = first_key(it);
+      if (it + 1 < count) {
+        kst.load(a.k, b, hk, first_key(it + 1), len, a.d);
+        vst.load(a.v, b, hk, first_key(it + 1), len, a.dv);
+      }
+      const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
+      if (!some) continue;
+      const bool all = key0 + BK - 1 <= w0 && (w0 + 31 - key0 < a.window || key0 + BK <= a.sinks);
+#pragma unroll
+      for (int sub = 0; sub < NSUB; ++sub) {
+        floatx16 x, g;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < P / 16; ++s) {
+          win_mma<IN>(x, win_read_row<P, IN>(ks, 32 * sub + (lane & 31), s, hh), qf[s]);
+          win_mma<IN>(g, win_read_row<P, IN>(vs, 32 * sub + (lane & 31), s, hh), gf[s]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, shift)) * (g[i] - delta);
+        if (!all) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int key = key0 + 32 * sub + 8 * (i >> 2) + 4 * hh + (i & 3);
+            x[i] = key <= row && (row - key < a.window || key < a.sinks) ? x[i] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const WinFrag<IN> p = win_operand<IN>(x, t);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            win_mma<IN>(acc[mt], win_read_columns<P, IN>(ks, 32 * sub + 16 * t, mt, lane), p);
+        }
+      }
+    }
+  }
+
+  int bad = 0;
+  if (in) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) bad |= !win_finite(acc[mt][i]);
+  }
+  bad |= __shfl_xor(bad, 32);
+  if (row < a.n && !bad) {
+    const int64_t at = (head_row + row) * a.d;
+    const float f = a.scale * a.drop;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = 32 * mt + 8 * r + 4 * hh;
+        if (col < a.d)
+          win_store4<IN>(a.dq, at, col, a.d, in ? acc[mt][4 * r] * f : 0.f, in ? acc[mt][4 * r + 1] * f : 0.f,
+                         in ? acc[mt][4 * r + 2] * f : 0.f, in ? acc[mt][4 * r + 3] * f : 0.f);
+      }
+  }
+  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1) {
+    const int i = __builtin_ctzll(todo);
+    win_dq_row<IN>(a, b, h, w0 + i, __shfl(delta, i));
+  }
+}
+
+// dk_j and dv_j over the rows [lo, hi] of every head of the group, one wave; columns [lane, lane + 64] of both
+template <int IN>
+__device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, int hi, float (&dk)[2], float (&dv)[2]) {
+  constexpr int ES = IN == F32 ? 4 : 2;
+  const int lane = threadIdx.x & 63;
+  const void* k = win_row<ES>(a.k, b, hk, key);
+  const void* v = win_row<ES>(a.v, b, hk, key);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) dk[e] = dv[e] = 0.f;
+  for (int g = 0; g < a.group; ++g) {
+    const int h = hk * a.group + g;
+    const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
+    for (int i0 = lo; i0 <= hi; i0 += 64) {
+      const int i = i0 + lane;
+      float p = 0.f, ds = 0.f;
+      if (i <= hi) {
+        const float x = a.scale * win_dot<IN>(win_row<ES>(a.q, b, h, i), k, a.d);
+        p = exp2f(fmaf(x, 1.44269504f, -a.lse[head_row + i]));
+        ds = p * (win_dot<IN>(win_row<ES>(a.go, b, h, i), v, a.dv) - a.delta[head_row + i]);
+      }
+      for (int u = 0; u < 64 && i0 + u <= hi; ++u) {
+        const float pu = __shfl(p, u), du = __shfl(ds, u);
+        const void* q = win_row<ES>(a.q, b, h, i0 + u);
+        const void* go = win_row<ES>(a.go, b, h, i0 + u);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (lane + 64 * e < a.d) dk[e] = fmaf(du, load_elem(q, lane + 64 * e, IN), dk[e]);
+          if (lane + 64 * e < a.dv) dv[e] = fmaf(pu, load_elem(go, lane + 64 * e, IN), dv[e]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) dk[e] *= a.scale;
+}
+
+// dk and dv: one workgroup per 128 keys of a key head (32 a wave) walks over the rows that see them within the window,
+// for every head of the group; the rows behind the window of a sink go to workgroups of their own (far), whose
+// sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.
+template <int P, int IN>
+__global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = 32;
+  __shared__ uint4 qs[BQ * CH], gs[BQ * CH];
+  __shared__ floatx4 stat_lse[BQ / 4], stat_delta[BQ / 4];
+  const int kv = a.heads / a.group;
+  const int far_items = a.sink_tiles * a.far_chunks, items = far_items + a.tiles;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int item = id % items, bh = id / items, b = bh / kv, hk = bh % kv;
+  const bool far = item < far_items;
+  const int chunk = far ? item / a.sink_tiles : -1;
+  const int tile = far ? item % a.sink_tiles : item - far_items;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
+  const int len = win_length(a, b);
+  const int k0 = tile * WIN_ROWS, kw = k0 + 32 * wave, key = kw + (lane & 31);
+
+  // rows [lo, hi] to walk over
+  int lo, hi;
+  if (far) {
+    lo = a.window + chunk * a.far_rows;
+    hi = lo + a.far_rows - 1;
+    if (lo < k0 + a.window) lo = k0 + a.window;
+  } else {
+    lo = k0;
+    hi = k0 + WIN_ROWS - 1 < a.n - a.window ? k0 + WIN_ROWS - 1 + a.window - 1 : a.n - 1;
+  }
+  if (hi > len - 1) hi = len - 1;
+
+  floatx16 dk[MT], dv[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) dk[mt][i] = dv[mt][i] = 0.f;
+
+  if (lo <= hi) {
+    WinFrag<IN> kf[P / 16], vf[P / 16];
+    const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
+    const char* krow = win_row<ES>(a.k, b, hk, key < len ? key : 0);
+    const char* vrow = win_row<ES>(a.v, b, hk, key < len ? key : 0);
+#pragma unroll
+    for (int s = 0; s < P / 16; ++s) {
+      kf[s] = win_load_row<IN>(krow, s, hh, key < len ? a.d : 0, a.k.aligned, flip);
+      vf[s] = win_load_row<IN>(vrow, s, hh, key < len ? a.dv : 0, a.v.aligned, 0u);
+    }
+    const int t_lo = lo / BQ, per_head = hi / BQ - t_lo + 1, count = per_head * a.group;
+    const float lift = __builtin_amdgcn_logf(a.lift);
+    WinStage<P, IN, BQ> qst, gst;
+    float st_lse = 0.f, st_delta = 0.f;
+    auto load = [&](int it) {
+      const int h = hk * a.group + it / per_head, row0 = (t_lo + it % per_head) * BQ;
+      qst.load(a.q, b, h, row0, len, a.d);
+      gst.load(a.go, b, h, row0, len, a.dv);
+      const int row = row0 + (threadIdx.x & 31);
+      st_lse = st_delta = 0.f;
+      if (threadIdx.x < 32 && row < len) {
+        const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.n + row;
+        st_lse = a.lse[at];
+        st_delta = a.delta[at];
+      }
+    };
+    load(0);
+    for (int it = 0; it < count; ++it) {
+      __syncthreads();
+      qst.put(qs);
+      gst.put(gs);
+      if (threadIdx.x < 32) {
+        reinterpret_cast<float*>(stat_lse)[threadIdx.x] = st_lse;
+        reinterpret_cast<float*>(stat_delta)[threadIdx.x] = st_delta;
+      }
+      __syncthreads();
+      const int q0 = (t_lo + it % per_head) * BQ;
+      if (it + 1 < count) load(it + 1);
+      const bool some = far ? kw < a.sinks && q0 + BQ - 1 - kw >= a.window
+                            : q0 + BQ - 1 >= kw && q0 - (kw + 31) < a.window;
+      if (!some) continue;
+      const bool all = far ? kw + 32 <= a.sinks && q0 - (kw + 31) >= a.window && q0 >= lo && q0 + BQ - 1 <= hi
+                           : q0 >= kw + 31 && q0 + BQ - 1 - kw < a.window;
+      floatx16 x, g;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < P / 16; ++s) {
+        win_mma<IN>(x, win_read_row<P, IN>(qs, lane & 31, s, hh), kf[s]);
+        win_mma<IN>(g, win_read_row<P, IN>(gs, lane & 31, s, hh), vf[s]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const floatx4 lse = stat_lse[2 * r + hh], delta = stat_delta[2 * r + hh];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * r + e;
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, lift - lse[e]));
+          g[i] = p * (g[i] - delta[e]);
+          x[i] = p;
+        }
+      }
+      if (!all) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int row = q0 + 8 * (i >> 2) + 4 * hh + (i & 3);
+          const bool seen = far ? key < a.sinks && row - key >= a.window && row >= lo && row <= hi
+                                : row >= key && row - key < a.window;
+          x[i] = seen ? x[i] : 0.f;
+          g[i] = seen ? g[i] : 0.f;
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          win_mma<IN>(dv[mt], win_read_columns<P, IN>(gs, 16 * t, mt, lane), p);
+          win_mma<IN>(dk[mt], win_read_columns<P, IN>(qs, 16 * t, mt, lane), ds);
+        }
+      }
+    }
+  }
+
+  int bad = 0;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad |= !(win_finite(dk[mt][i]) && win_finite(dv[mt][i]));
+  bad = key < len ? bad : 0;
+  bad |= __shfl_xor(bad, 32);
+  // sums to be added to others' (the sinks of a call with rows behind their window)
+  const bool part = a.far_chunks > 0 && key < a.sink_rows;
+  const int64_t part_row = ((static_cast<int64_t>(bh) * (a.far_chunks + 1) + chunk + 1) * a.sink_rows + key) *
+                           (a.d + a.dv);
+  const int64_t out_row = static_cast<int64_t>(bh) * a.n + key;
+  const float f = a.scale * a.drop;
+  if (!bad && (part || (!far && key < a.n))) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = 32 * mt + 8 * r + 4 * hh;
+        if (part) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (col + e < a.d) a.part[part_row + col + e] = dk[mt][4 * r + e] * f;
+            if (col + e < a.dv) a.part[part_row + a.d + col + e] = dv[mt][4 * r + e] * a.drop;
+          }
+        } else {
+          if (col < a.d)
+            win_store4<IN>(a.dk, out_row * a.d, col, a.d, dk[mt][4 * r] * f, dk[mt][4 * r + 1] * f,
+                           dk[mt][4 * r + 2] * f, dk[mt][4 * r + 3] * f);
+          if (col < a.dv)
+            win_store4<IN>(a.dv_out, out_row * a.dv, col, a.dv, dv[mt][4 * r] * a.drop, dv[mt][4 * r + 1] * a.drop,
+                           dv[mt][4 * r + 2] * a.drop, dv[mt][4 * r + 3] * a.drop);
+        }
+      }
+  }
+  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1) {
+    const int j = kw + __builtin_ctzll(todo);
+    float sk[2], sv[2];
+    int from = lo, to = hi;
+    if (far) {
+      if (j >= a.sinks) continue;
+      if (from < j + a.window) from = j + a.window;
+    } else {
+      from = j;
+      if (j < a.n - a.window && to > j + a.window - 1) to = j + a.window - 1;
+    }
+    win_dkv_row<IN>(a, b, hk, j, from, to, sk, sv);
+    const bool pj = a.far_chunks > 0 && j < a.sink_rows;
+    const int64_t pr = ((static_cast<int64_t>(bh) * (a.far_chunks + 1) + chunk + 1) * a.sink_rows + j) * (a.d + a.dv);
+    const int64_t orow = static_cast<int64_t>(bh) * a.n + j;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int col = lane + 64 * e;
+      if (col < a.d) {
+        if (pj)
+          a.part[pr + col] = sk[e];
+        else
+          store_elem(a.dk, orow * a.d + col, IN, sk[e]);
+      }
+      if (col < a.dv) {
+        if (pj)
+          a.part[pr + a.d + col] = sv[e];
+        else
+          store_elem(a.dv_out, orow * a.dv + col, IN, sv[e]);
+      }
+    }
+  }
+}
+
+// dk and dv of the sinks: their tile's sums and the far chunks', in order.  One thread a column.
+template <int IN>
+__global__ __launch_bounds__(256) void window_sink_kernel(const WinArgs a) {
+  const int width = a.d + a.dv;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int64_t per = static_cast<int64_t>(a.sink_rows) * width;
+  const int64_t bh = at / per;
+  if (bh >= static_cast<int64_t>(a.batch) * (a.heads / a.group)) return;
+  const int64_t in = at % per;
+  float s = 0.f;
+  for (int c = 0; c <= a.far_chunks; ++c) s += a.part[(bh * (a.far_chunks + 1) + c) * per + in];
+  const int64_t row = bh * a.n + in / width;
+  const int col = static_cast<int>(in % width);
+  if (col < a.d)
+    store_elem(a.dk, row * a.d + col, IN, s);
+  else
+    store_elem(a.dv_out, row * a.dv + col - a.d, IN, s);
+}
+
+}  // namespace sta
