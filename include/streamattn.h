@@ -485,6 +485,40 @@ int sta_window_attention_backward(const void* grad, const void* q, const void* k
                                   const int32_t* lengths, void* dq, void* dk, void* dv_out, void* workspace,
                                   int64_t workspace_bytes, void* stream);
 
+/*
+ * RMS norm of every head's query and key rows and their position rotation in one pass (the rows that
+ * sta_window_attention takes): y = R(p) (x rsqrt(mean(x^2) + eps) w).
+ *   q [batch][heads][n][d], k [batch][kv_heads][n][d] in dtype, last dimension contiguous, strides [2][3] (host memory)
+ *   the element strides of batch, head and row; heads or kv_heads may be 0 (its pointers then are not used).  d <= 256;
+ *   batch n <= 2^30.
+ *   q_weight / k_weight [d] in weight_dtype, or NULL (1).
+ *   table [limit][rotary] fp32: cos then sin of the rotary / 2 angles of each position; the first `rotary` columns
+ *   (even, <= d; with 0 the table may be NULL) turn, in pairs (i, i + rotary / 2), or (2 i, 2 i + 1) if interleaved.
+ *   positions: int32 (positions_64 = 0) or int64, element strides position_stride_b, position_stride_n; NULL: the row's
+ *   index.  Rows at a position outside [0, limit) come out as NaN.
+ *   q_out / k_out dense, 16-byte aligned, in dtype.  All arithmetic is fp32, rounded once.
+ */
+int sta_head_rotary(const void* q, const void* k, int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int d,
+                    const int64_t* strides, const void* q_weight, const void* k_weight, int weight_dtype,
+                    const float* table, int64_t limit, int rotary, int interleaved, const void* positions,
+                    int positions_64, int64_t position_stride_b, int64_t position_stride_n, float eps, void* q_out,
+                    void* k_out, void* stream);
+
+/* Bytes of sta_head_rotary_backward's workspace; -1 for arguments it refuses. */
+int64_t sta_head_rotary_backward_bytes(int64_t batch, int heads, int kv_heads, int64_t n, int d);
+
+/*
+ * Gradients of sta_head_rotary from those of its results (strides [4][3]: q, k, q_grad, k_grad): dq, dk dense,
+ * 16-byte aligned, in dtype; dq_weight, dk_weight [d] in weight_dtype (or NULL).  Sums in a fixed order.
+ */
+int sta_head_rotary_backward(const void* q_grad, const void* k_grad, const void* q, const void* k, int dtype,
+                             int64_t batch, int heads, int kv_heads, int64_t n, int d, const int64_t* strides,
+                             const void* q_weight, const void* k_weight, int weight_dtype, const float* table,
+                             int64_t limit, int rotary, int interleaved, const void* positions, int positions_64,
+                             int64_t position_stride_b, int64_t position_stride_n, float eps, void* dq, void* dk,
+                             void* dq_weight, void* dk_weight, void* workspace, int64_t workspace_bytes,
+                             void* stream);
+
 /* Rows per block-attention tile and the moment chunk the library uses for a head dimension D (the
  * chunk argument of sta_block_attention is that chunk for sta_moments' partials, the query block for
  * sta_moments_ws' partials). */

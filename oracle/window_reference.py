@@ -93,3 +93,54 @@ def over(got, want):
         return math.inf
     # 1e-30: elements with nothing to add up are zero on both sides
     return float(((got - value).abs() / (bound * 1.05 + 1e-30)).max()) if got.numel() else 0.0
+
+
+def norm_rotary(x, w, cos, sin, *, eps, interleaved, grad=None):
+    """Rows [B,H,N,D] with cos and sin [B,N,R/2]: {"y": (value, bound)} in float64, with "dx" and "dw" if grad is given."""
+    dt = x.dtype
+    u = half_step(dt)
+    d = x.shape[-1]
+    x = x.double()
+    w = torch.ones(d, dtype=torch.float64) if w is None else w.double()
+    cos, sin = cos.double()[:, None], sin.double()[:, None]
+    pairs = cos.shape[-1]
+
+    def turn(h, sin):
+        a = h[..., 0:2 * pairs:2] if interleaved else h[..., :pairs]
+        b = h[..., 1:2 * pairs:2] if interleaved else h[..., pairs:2 * pairs]
+        y = h.clone()
+        parts = a * cos - b * sin, b * cos + a * sin
+        if interleaved:
+            y[..., 0:2 * pairs:2], y[..., 1:2 * pairs:2] = parts
+        else:
+            y[..., :pairs], y[..., pairs:2 * pairs] = parts
+        return y
+
+    def size(h):  # |a cos| + |b sin|
+        y = h.abs().clone()
+        a = y[..., 0:2 * pairs:2] if interleaved else y[..., :pairs]
+        b = y[..., 1:2 * pairs:2] if interleaved else y[..., pairs:2 * pairs]
+        parts = a * cos.abs() + b * sin.abs(), b * cos.abs() + a * sin.abs()
+        if interleaved:
+            y[..., 0:2 * pairs:2], y[..., 1:2 * pairs:2] = parts
+        else:
+            y[..., :pairs], y[..., pairs:2 * pairs] = parts
+        return y
+
+    inv = 1 / (x.square().mean(-1, keepdim=True) + eps).sqrt()
+    hat = x * inv
+    small = 2.0 ** -25 if dt == torch.float16 else 0.0
+    ops = F24 * (d + 12)  # the sum of squares' d operations and a dozen others
+    y = turn(hat * w, sin)
+    out = {"y": (y, u * y.abs() + ops * size(hat * w) + small)}
+    if grad is not None:
+        g = grad.double()
+        t, big = turn(g, -sin), size(g)
+        m = (t * w * hat).mean(-1, keepdim=True)
+        dx = inv * (t * w - hat * m)
+        err = ops * 2 * inv * (big * w.abs() + hat.abs() * (big * w.abs() * hat.abs()).mean(-1, keepdim=True))
+        out["dx"] = (dx, u * dx.abs() + err + small)
+        rows = x.numel() // d
+        dw = (t * hat).sum((0, 1, 2))
+        out["dw"] = (dw, F24 * (rows + d + 12) * (big * hat.abs()).sum((0, 1, 2)))
+    return out

@@ -171,6 +171,15 @@ _SIGNATURES = {
         _i32, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _c_p, _f32, _i64, _i64,
                _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # grad q k v out lse dtype .. lengths dq dk dv ws bytes stream
     ),
+    "sta_head_rotary": (
+        _i32, [_c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _c_p, _c_p, _c_p, _i32, _c_p, _i64, _i32, _i32, _c_p,
+               _i32, _i64, _i64, _f32, _c_p, _c_p, _c_p],  # .. weights type table limit rotary inter pos .. eps out out
+    ),
+    "sta_head_rotary_backward_bytes": (_i64, [_i64, _i32, _i32, _i64, _i32]),
+    "sta_head_rotary_backward": (
+        _i32, [_c_p, _c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _c_p, _c_p, _c_p, _i32, _c_p, _i64, _i32,
+               _i32, _c_p, _i32, _i64, _i64, _f32, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],
+    ),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -2,13 +2,13 @@
 
     python streaming-attention_amd/build_native.py
 
-The library is 112 objects compiled in parallel and linked into one shared object: api.hip (entry
+The library is 113 objects compiled in parallel and linked into one shared object: api.hip (entry
 points, compressor and decode kernels), launch_moments_ws.hip (the wave-specialised moment scan, per
 element size and column-tile count), launch_moments.hip (fp32 and split-bf16 products, 32 or 64
 columns), launch_accumulate.hip, and
 launch_block.hip and launch_flash.hip once per residual / flash kernel configuration (padded key
 width, value-column tiles, element size), launch_window.hip once per windowed-attention configuration
-(padded width, element type) with api_window.hip for its entry points.  Objects go to streaming-attention_amd/_build/.
+(padded width, element type) with api_window.hip for its entry points, api_rotary.hip.  Objects go to streaming-attention_amd/_build/.
 
 Packed-fp32 VALU instructions are disabled (-packed-fp32-ops): the kernels are written for the
 scalar fp32 and MFMA paths.
@@ -44,6 +44,7 @@ UNITS = tuple(("launch_moments_ws.hip", f"launch_moments_ws_{es}_{ct}", (f"-DSTA
     ("launch_window.hip", f"launch_window_{p}_{i}", (f"-DSTA_WIN_P={p}", f"-DSTA_WIN_IN={i}"))
     for p in (128, 96, 64, 32) for i in (0, 1, 2)) + (
     ("api_window.hip", "api_window", ()),
+    ("api_rotary.hip", "api_rotary", ()),
     ("api.hip", "api", ()),
 )
 OBJDIR = HERE / "_build"

@@ -23,8 +23,8 @@ int element_size(int dtype) { return dtype == STA_F32 ? 4 : 2; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-sta::WinRows rows_of(const void* p, const int64_t* strides, int dtype) {
-  sta::WinRows r;
+sta::Rows rows_of(const void* p, const int64_t* strides, int dtype) {
+  sta::Rows r;
   r.p = p;
   r.sb = strides[0];
   r.sh = strides[1];

@@ -23,7 +23,7 @@
 // those that do not: a result row that is not finite is taken again over its visible pairs alone (win_*_row).
 #include <type_traits>
 
-#include "common.hpp"
+#include "rows.hpp"
 
 namespace sta {
 
@@ -32,15 +32,8 @@ typedef _Float16 win_half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 win_half2 __attribute__((ext_vector_type(2)));
 typedef short win_short4 __attribute__((ext_vector_type(4)));
 
-// rows of [batch][heads][n][width]: element strides; `aligned`: every row starts on 16 bytes
-struct WinRows {
-  const void* p;
-  int64_t sb, sh, sn;
-  int aligned;
-};
-
 struct WinArgs {
-  WinRows q, k, v, go;     // go: the output's gradient
+  Rows q, k, v, go;     // go: the output's gradient
   int heads, group;        // query heads, query heads per key head
   int batch, n, d, dv;
   int window, sinks;       // 1 <= window <= n, 0 <= sinks <= n (the host clamps both to n)
@@ -117,29 +110,6 @@ __device__ __forceinline__ WinFrag<IN> win_operand(const floatx16& x, int t) {
   return f;
 }
 
-// 16 bytes at column `col` of a row, columns at or behind `width` zero
-template <int ES>
-__device__ __forceinline__ uint4 win_chunk(const void* row, int col, int width, int aligned) {
-  constexpr int E = 16 / ES;
-  const char* p = static_cast<const char*>(row) + static_cast<int64_t>(col) * ES;
-  if (aligned && col + E <= width) return *reinterpret_cast<const uint4*>(p);
-  uint32_t u[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (col + e < width) {
-      if constexpr (ES == 4)
-        u[e] = reinterpret_cast<const uint32_t*>(p)[e];
-      else
-        u[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
-    }
-  return uint4{u[0], u[1], u[2], u[3]};
-}
-
-template <int ES>
-__device__ __forceinline__ const char* win_row(const WinRows& t, int64_t b, int64_t h, int64_t row) {
-  return static_cast<const char*>(t.p) + (b * t.sb + h * t.sh + row * t.sn) * ES;
-}
-
 // Staging of ROWS rows of a tile by 256 threads: registers first (load), LDS when the tile before is done with (put)
 template <int P, int IN, int ROWS>
 struct WinStage {
@@ -147,13 +117,13 @@ struct WinStage {
   static constexpr int COUNT = (ROWS * CH + 255) / 256;
   uint4 u[COUNT];
   // rows [row0, row0 + ROWS) of head (b, h); rows at or behind `limit` and columns behind `width` are zero
-  __device__ __forceinline__ void load(const WinRows& t, int64_t b, int64_t h, int row0, int limit, int width) {
+  __device__ __forceinline__ void load(const Rows& t, int64_t b, int64_t h, int row0, int limit, int width) {
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       const int at = threadIdx.x + 256 * i, r = at / CH, c = at % CH;
       u[i] = uint4{0u, 0u, 0u, 0u};
       if ((ROWS * CH % 256 == 0 || at < ROWS * CH) && row0 + r < limit && c * E < width)
-        u[i] = win_chunk<ES>(win_row<ES>(t, b, h, row0 + r), c * E, width, t.aligned);
+        u[i] = rows_chunk<ES>(rows_at<ES>(t, b, h, row0 + r), c * E, width, t.aligned);
     }
   }
   __device__ __forceinline__ void put(uint4* lds) const {
@@ -226,7 +196,7 @@ __device__ __forceinline__ WinFrag<IN> win_load_row(const void* row, int s, int 
   for (int i = 0; i < (IN == F32 ? 2 : 1); ++i) {
     const int col = 16 * s + 8 * h + 4 * i;
     uint4 u = uint4{0u, 0u, 0u, 0u};
-    if (col < width) u = win_chunk<ES>(row, col, width, aligned);
+    if (col < width) u = rows_chunk<ES>(row, col, width, aligned);
     f.w[i] = uint4{u.x ^ flip, u.y ^ flip, u.z ^ flip, u.w ^ flip};
   }
   return f;
@@ -297,10 +267,10 @@ __device__ void win_forward_row(const WinArgs& a, int b, int h, int i) {
   constexpr int ES = IN == F32 ? 4 : 2;
   const int lane = threadIdx.x & 63;
   const WinKeys keys(a, i);
-  const void* q = win_row<ES>(a.q, b, h, i);
+  const void* q = rows_at<ES>(a.q, b, h, i);
   float m = -__builtin_inff();
   for (int t = lane; t < keys.count; t += 64)
-    m = fmaxf(m, a.scale * win_dot<IN>(q, win_row<ES>(a.k, b, h / a.group, keys.key(t)), a.d));
+    m = fmaxf(m, a.scale * win_dot<IN>(q, rows_at<ES>(a.k, b, h / a.group, keys.key(t)), a.d));
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
   float l = 0.f, acc[2] = {0.f, 0.f};
@@ -308,11 +278,11 @@ __device__ void win_forward_row(const WinArgs& a, int b, int h, int i) {
     const int t = t0 + lane;
     float p = 0.f;
     if (t < keys.count)
-      p = expf(a.scale * win_dot<IN>(q, win_row<ES>(a.k, b, h / a.group, keys.key(t)), a.d) - m);
+      p = expf(a.scale * win_dot<IN>(q, rows_at<ES>(a.k, b, h / a.group, keys.key(t)), a.d) - m);
     l += p;
     for (int u = 0; u < 64 && t0 + u < keys.count; ++u) {
       const float w = __shfl(p, u);
-      const void* v = win_row<ES>(a.v, b, h / a.group, keys.key(t0 + u));
+      const void* v = rows_at<ES>(a.v, b, h / a.group, keys.key(t0 + u));
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         if (lane + 64 * e < a.dv) acc[e] = fmaf(w, load_elem(v, lane + 64 * e, IN), acc[e]);
@@ -365,7 +335,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
   if (r0 < len) {
     WinFrag<IN> qf[P / 16];
     const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
-    const char* qrow = win_row<ES>(a.q, b, h, row < len ? row : 0);
+    const char* qrow = rows_at<ES>(a.q, b, h, row < len ? row : 0);
 #pragma unroll
     for (int s = 0; s < P / 16; ++s) qf[s] = win_load_row<IN>(qrow, s, hh, row < len ? a.d : 0, a.q.aligned, flip);
 
@@ -490,8 +460,8 @@ __device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
   constexpr int ES = IN == F32 ? 4 : 2;
   const int lane = threadIdx.x & 63, hk = h / a.group;
   const WinKeys keys(a, i);
-  const void* q = win_row<ES>(a.q, b, h, i);
-  const void* go = win_row<ES>(a.go, b, h, i);
+  const void* q = rows_at<ES>(a.q, b, h, i);
+  const void* go = rows_at<ES>(a.go, b, h, i);
   const int64_t row = (static_cast<int64_t>(b) * a.heads + h) * a.n + i;
   const float lse = a.lse[row];
   float acc[2] = {0.f, 0.f};
@@ -500,12 +470,12 @@ __device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
     float ds = 0.f;
     if (t < keys.count) {
       const int key = keys.key(t);
-      const float x = a.scale * win_dot<IN>(q, win_row<ES>(a.k, b, hk, key), a.d);
-      ds = exp2f(fmaf(x, 1.44269504f, -lse)) * (win_dot<IN>(go, win_row<ES>(a.v, b, hk, key), a.dv) - delta);
+      const float x = a.scale * win_dot<IN>(q, rows_at<ES>(a.k, b, hk, key), a.d);
+      ds = exp2f(fmaf(x, 1.44269504f, -lse)) * (win_dot<IN>(go, rows_at<ES>(a.v, b, hk, key), a.dv) - delta);
     }
     for (int u = 0; u < 64 && t0 + u < keys.count; ++u) {
       const float w = __shfl(ds, u);
-      const void* k = win_row<ES>(a.k, b, hk, keys.key(t0 + u));
+      const void* k = rows_at<ES>(a.k, b, hk, keys.key(t0 + u));
 #pragma unroll
       for (int e = 0; e < 2; ++e)
         if (lane + 64 * e < a.d) acc[e] = fmaf(w, load_elem(k, lane + 64 * e, IN), acc[e]);
@@ -539,8 +509,8 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
   if (r0 < len) {
     WinFrag<IN> qf[P / 16], gf[P / 16];
     const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
-    const char* qrow = win_row<ES>(a.q, b, h, in ? row : 0);
-    const char* grow = win_row<ES>(a.go, b, h, in ? row : 0);
+    const char* qrow = rows_at<ES>(a.q, b, h, in ? row : 0);
+    const char* grow = rows_at<ES>(a.go, b, h, in ? row : 0);
     const char* orow = static_cast<const char*>(a.out) + (head_row + (in ? row : 0)) * a.dv * ES;
     const int out_aligned = (a.dv * ES) % 16 == 0;
 #pragma unroll
@@ -640,8 +610,8 @@ template <int IN>
 __device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, int hi, float (&dk)[2], float (&dv)[2]) {
   constexpr int ES = IN == F32 ? 4 : 2;
   const int lane = threadIdx.x & 63;
-  const void* k = win_row<ES>(a.k, b, hk, key);
-  const void* v = win_row<ES>(a.v, b, hk, key);
+  const void* k = rows_at<ES>(a.k, b, hk, key);
+  const void* v = rows_at<ES>(a.v, b, hk, key);
 #pragma unroll
   for (int e = 0; e < 2; ++e) dk[e] = dv[e] = 0.f;
   for (int g = 0; g < a.group; ++g) {
@@ -651,14 +621,14 @@ __device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, in
       const int i = i0 + lane;
       float p = 0.f, ds = 0.f;
       if (i <= hi) {
-        const float x = a.scale * win_dot<IN>(win_row<ES>(a.q, b, h, i), k, a.d);
+        const float x = a.scale * win_dot<IN>(rows_at<ES>(a.q, b, h, i), k, a.d);
         p = exp2f(fmaf(x, 1.44269504f, -a.lse[head_row + i]));
-        ds = p * (win_dot<IN>(win_row<ES>(a.go, b, h, i), v, a.dv) - a.delta[head_row + i]);
+        ds = p * (win_dot<IN>(rows_at<ES>(a.go, b, h, i), v, a.dv) - a.delta[head_row + i]);
       }
       for (int u = 0; u < 64 && i0 + u <= hi; ++u) {
         const float pu = __shfl(p, u), du = __shfl(ds, u);
-        const void* q = win_row<ES>(a.q, b, h, i0 + u);
-        const void* go = win_row<ES>(a.go, b, h, i0 + u);
+        const void* q = rows_at<ES>(a.q, b, h, i0 + u);
+        const void* go = rows_at<ES>(a.go, b, h, i0 + u);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if (lane + 64 * e < a.d) dk[e] = fmaf(du, load_elem(q, lane + 64 * e, IN), dk[e]);
@@ -711,8 +681,8 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
   if (lo <= hi) {
     WinFrag<IN> kf[P / 16], vf[P / 16];
     const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
-    const char* krow = win_row<ES>(a.k, b, hk, key < len ? key : 0);
-    const char* vrow = win_row<ES>(a.v, b, hk, key < len ? key : 0);
+    const char* krow = rows_at<ES>(a.k, b, hk, key < len ? key : 0);
+    const char* vrow = rows_at<ES>(a.v, b, hk, key < len ? key : 0);
 #pragma unroll
     for (int s = 0; s < P / 16; ++s) {
       kf[s] = win_load_row<IN>(krow, s, hh, key < len ? a.d : 0, a.k.aligned, flip);
