@@ -40,6 +40,8 @@ extern "C" {
 #define STA_F16 2
 #define STA_F64 3 /* sta_compress_nodes only: float64 keys scored in fp64 against float64 draws */
 
+#define STA_STORAGE_FP4 3 /* sta_ring_*: the cache in 4-bit floats with a power of two for 32 columns */
+
 #define STA_PRODUCTS_FP32 0       /* matrix-core products in fp32                                 */
 #define STA_PRODUCTS_SPLIT_BF16 1 /* fp32 operands as bf16 hi + lo, three bf16 products            */
 
@@ -518,6 +520,54 @@ int sta_head_rotary_backward(const void* q_grad, const void* k_grad, const void*
                              int64_t position_stride_b, int64_t position_stride_n, float eps, void* dq, void* dk,
                              void* dq_weight, void* dk_weight, void* workspace, int64_t workspace_bytes,
                              void* stream);
+
+/*
+ * Token cache of windowed attention, for streams in lockstep: per stream and key head sinks + window slots; token
+ * p < sinks in slot p, the others in a ring, token p in slot sinks + (p - sinks) % window.  counts [streams][kv_heads]
+ * (device) is the number of tokens so far (equal over a stream's heads).
+ *   storage: the element type's own code, or STA_STORAGE_FP4: each block of 32 columns of a token as 4-bit floats
+ *   (0, 0.5, 1, 1.5, 2, 3, 4, 6 and signs; nearest, ties to the even code, larger values 6) times
+ *   2^(floor(log2(largest magnitude)) - 2) >= 2^-126; a block with a value that is not finite is NaN.
+ *   keys, values, key_exponents, value_exponents (the last two with STA_STORAGE_FP4 only, NULL otherwise): caller-owned
+ *   device buffers of sta_ring_layout's bytes [4], 16-byte aligned, zeroed before their first use; their layout is the
+ *   library's own (equal for equal arguments, so that they can be saved and loaded).
+ *   d, dv <= 128, sinks + window <= 2^30; heads a multiple of kv_heads.
+ */
+int sta_ring_layout(int dtype, int storage, int64_t streams, int kv_heads, int d, int dv, int64_t window,
+                    int64_t sinks, int64_t* bytes);
+
+/* Bytes of sta_ring_attention's workspace (0: none); -1 for arguments it refuses. */
+int64_t sta_ring_attention_bytes(int64_t streams, int heads, int kv_heads, int d, int dv, int64_t window,
+                                 int64_t sinks);
+
+/*
+ * out [streams][heads][dv] (dense, in dtype) = softmax attention of q [streams][heads][d] over the slots that hold a
+ * token, after the new tokens k [streams][kv_heads][d], v [..][dv] went in (both NULL: no new token); an empty cache
+ * gives 0.  strides [3][2] (host memory): element strides of stream and head of q, k and v.  workspace: caller-allocated,
+ * 16-byte aligned, of sta_ring_attention_bytes (contents undefined before and after).
+ */
+int sta_ring_attention(const void* q, const void* k, const void* v, int dtype, int storage, int64_t streams, int heads,
+                       int kv_heads, int d, int dv, const int64_t* strides, float scale, int64_t window,
+                       int64_t sinks, void* keys, void* values, void* key_exponents, void* value_exponents,
+                       int32_t* counts, void* out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Tokens k [streams][kv_heads][rows][d], v [..][dv] (strides [2][3]: stream, head, row) into the cache, of every stream
+ * the first take[stream] (device; NULL: rows) rows.
+ */
+int sta_ring_extend(const void* k, const void* v, int dtype, int storage, int64_t streams, int kv_heads, int64_t rows,
+                    int d, int dv, const int64_t* strides, int64_t window, int64_t sinks, const int32_t* take,
+                    void* keys, void* values, void* key_exponents, void* value_exponents, int32_t* counts,
+                    void* stream);
+
+/*
+ * The slots' contents: keys_out [streams][kv_heads][sinks + window][d], values_out [..][dv] in dtype (zero where no
+ * token is), positions [streams][sinks + window] (-1 there).
+ */
+int sta_ring_items(int dtype, int storage, int64_t streams, int kv_heads, int d, int dv, int64_t window,
+                   int64_t sinks, const void* keys, const void* values, const void* key_exponents,
+                   const void* value_exponents, const int32_t* counts, void* keys_out, void* values_out,
+                   int32_t* positions, void* stream);
 
 /* Rows per block-attention tile and the moment chunk the library uses for a head dimension D (the
  * chunk argument of sta_block_attention is that chunk for sta_moments' partials, the query block for

@@ -144,3 +144,67 @@ def norm_rotary(x, w, cos, sin, *, eps, interleaved, grad=None):
         dw = (t * hat).sum((0, 1, 2))
         out["dw"] = (dw, F24 * (rows + d + 12) * (big * hat.abs()).sum((0, 1, 2)))
     return out
+
+
+def as_held(x, storage):
+    """The float64 values that rows stand for in a cache: themselves, or 4-bit floats with a power of two for 32 columns."""
+    x = x.double()
+    if storage is None:
+        return x
+    grid = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+    y = torch.zeros_like(x)
+    for lo in range(0, x.shape[-1], 32):
+        z = x[..., lo:lo + 32]
+        top = z.abs().amax(-1, keepdim=True)
+        power = torch.floor(torch.log2(top.clamp_min(2.0 ** -140))) - 2
+        unit = 2.0 ** power.clamp_min(-126)
+        m = z.abs() / unit
+        code = torch.zeros_like(m, dtype=torch.long)
+        for i in range(7):  # the border between codes i and i + 1 belongs to the even one
+            mid = (grid[i] + grid[i + 1]) / 2
+            code += (m > mid) if i % 2 == 0 else (m >= mid)
+        v = torch.tensor(grid, dtype=torch.float64)[code] * unit * z.sign()
+        y[..., lo:lo + 32] = torch.where(torch.isfinite(top), v, math.nan)
+    return y
+
+
+class TokenCache:
+    """Per-token statement of the ring: a dict of positions a stream, every token held."""
+
+    def __init__(self, streams, window, sinks, storage):
+        self.window, self.sinks, self.storage = window, sinks, storage
+        self.held = [dict() for _ in range(streams)]
+        self.n = [0] * streams
+
+    def put(self, s, k, v):
+        p = self.n[s]
+        if p >= self.sinks + self.window:
+            self.held[s].pop(p - self.window, None)
+        self.held[s][p] = as_held(k, self.storage), as_held(v, self.storage)
+        self.n[s] = p + 1
+
+    def slot(self, p):
+        return p if p < self.sinks else self.sinks + (p - self.sinks) % self.window
+
+    def query(self, s, q, scale, dtype):
+        """(value, bound) [H, dv] of q [H, d]."""
+        u = half_step(dtype)
+        q = q.double()
+        if not self.held[s]:
+            return None
+        keys, values = (torch.stack([self.held[s][p][i] for p in sorted(self.held[s])], 1) for i in (0, 1))
+        g = q.shape[0] // keys.shape[0]
+        keys, values = keys.repeat_interleave(g, 0), values.repeat_interleave(g, 0)
+        x = (keys @ q[..., None])[..., 0] * scale
+        size = (keys.abs() @ q.abs()[..., None])[..., 0].amax(-1, keepdim=True) * abs(scale)
+        p = x.softmax(-1)
+        out, mag = (p[:, None] @ values)[:, 0], (p[:, None] @ values.abs())[:, 0]
+        # fp32 products and sums of d and n terms, three planes of 8 bits or more (2^-23), 16-bit rows' weights as two planes
+        # (2^-16 bf16; half a step of fp16's smallest, 2^-25, in units of the largest weight, of which n add up)
+        n, d = x.shape[-1], q.shape[-1]
+        planes = 2.0 ** -22 if dtype == torch.float32 else 2.0 ** -16
+        ep = F24 * (2 * (d + 8) * size + 2 * n + 64) + planes
+        bound = u * out.abs() + ep * mag
+        if dtype == torch.float16:
+            bound = bound + 2.0 ** -25 + 2.0 ** -25 * values.abs().sum(1)
+        return out, bound

@@ -26,6 +26,7 @@ STA_ERR_SCRATCH = 6
 
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 STA_F64 = 3  # sta_compress_nodes' float64 scoring
+STORAGE_FP4 = 3  # sta_ring_*: a cache in 4 bits
 PRODUCTS_FP32 = 0
 PRODUCTS_SPLIT_BF16 = 1
 
@@ -170,6 +171,19 @@ _SIGNATURES = {
     "sta_window_attention_backward": (
         _i32, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _c_p, _f32, _i64, _i64,
                _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # grad q k v out lse dtype .. lengths dq dk dv ws bytes stream
+    ),
+    "sta_ring_layout": (_i32, [_i32, _i32, _i64, _i32, _i32, _i32, _i64, _i64, _c_p]),
+    "sta_ring_attention_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i64, _i64]),
+    "sta_ring_attention": (
+        _i32, [_c_p, _c_p, _c_p, _i32, _i32, _i64, _i32, _i32, _i32, _i32, _c_p, _f32, _i64, _i64, _c_p, _c_p, _c_p,
+               _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # q k v types S H Hk d dv strides .. cache counts out ws bytes stream
+    ),
+    "sta_ring_extend": (
+        _i32, [_c_p, _c_p, _i32, _i32, _i64, _i32, _i64, _i32, _i32, _c_p, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p,
+               _c_p, _c_p],  # k v types S Hk rows d dv strides window sinks take cache counts stream
+    ),
+    "sta_ring_items": (
+        _i32, [_i32, _i32, _i64, _i32, _i32, _i32, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
     ),
     "sta_head_rotary": (
         _i32, [_c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _c_p, _c_p, _c_p, _i32, _c_p, _i64, _i32, _i32, _c_p,

@@ -2,13 +2,14 @@
 
     python streaming-attention_amd/build_native.py
 
-The library is 113 objects compiled in parallel and linked into one shared object: api.hip (entry
+The library is 138 objects compiled in parallel and linked into one shared object: api.hip (entry
 points, compressor and decode kernels), launch_moments_ws.hip (the wave-specialised moment scan, per
 element size and column-tile count), launch_moments.hip (fp32 and split-bf16 products, 32 or 64
 columns), launch_accumulate.hip, and
 launch_block.hip and launch_flash.hip once per residual / flash kernel configuration (padded key
 width, value-column tiles, element size), launch_window.hip once per windowed-attention configuration
-(padded width, element type) with api_window.hip for its entry points, api_rotary.hip.  Objects go to streaming-attention_amd/_build/.
+(padded width, element type) with api_window.hip for its entry points, launch_ring.hip once per token-cache configuration
+(storage, query type, key blocks) with api_ring.hip, and api_rotary.hip.  Objects go to streaming-attention_amd/_build/.
 
 Packed-fp32 VALU instructions are disabled (-packed-fp32-ops): the kernels are written for the
 scalar fp32 and MFMA paths.
@@ -42,8 +43,12 @@ UNITS = tuple(("launch_moments_ws.hip", f"launch_moments_ws_{es}_{ct}", (f"-DSTA
      (f"-DSTA_FLASH_DP={dp}", f"-DSTA_FLASH_DVT={dvt}", f"-DSTA_FLASH_ES={es}"))
     for dp in (128, 64, 32, 16) for dvt in (4, 2, 8, 1, 16) for es in (4, 2)) + tuple(
     ("launch_window.hip", f"launch_window_{p}_{i}", (f"-DSTA_WIN_P={p}", f"-DSTA_WIN_IN={i}"))
-    for p in (128, 96, 64, 32) for i in (0, 1, 2)) + (
+    for p in (128, 96, 64, 32) for i in (0, 1, 2)) + tuple(
+    ("launch_ring.hip", f"launch_ring_{st}{q}_{nbk}",
+     (f"-DSTA_RING_ST={st}", f"-DSTA_RING_Q={q}", f"-DSTA_RING_NBK={nbk}"))
+    for st, q in ((0, 0), (1, 1), (2, 2), (3, 0), (3, 1), (3, 2)) for nbk in (4, 3, 2, 1)) + (
     ("api_window.hip", "api_window", ()),
+    ("api_ring.hip", "api_ring", ()),
     ("api_rotary.hip", "api_rotary", ()),
     ("api.hip", "api", ()),
 )

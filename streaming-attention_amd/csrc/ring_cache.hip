@@ -1,0 +1,681 @@
+// The token cache of windowed attention and the single-token attention over it.
+//
+// A (stream, key head) holds sinks + window slots: token p < sinks sits in slot p, the others in a ring, token p in
+// slot sinks + (p - sinks) % window, so that after n tokens the first min(n, sinks + window) slots hold what the next
+// query sees, in an order that softmax does not mind.  counts[stream][head] is n.
+//
+// Slots lie in tiles of 32, each laid out in the order in which the matrix instructions take it (v_mfma_f32_16x16x32,
+// 16x16x4_f32 eight times for fp32), so that a wave loads operands straight from memory, in whole lines and without
+// LDS.  With lane l = 16 g + i:
+//   keys    [2 halves of 16 slots][d / 32][lane][8]: lane holds slot i of the half, dimensions 32 b + 8 g + 0..7
+//   values  [dv / 16][lane][8]: lane holds column 16 c + i of slots {4 g + 0..3, 16 + 4 g + 0..3}
+// X^T = K Q^T leaves lane (query i, g) with slots 4 g + 0..3 of each half: the B operand of O^T += V^T P^T as it stands.
+//
+// Storage in 4 bits (fp4): values in blocks of 32 columns of a token, each 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign,
+// times 2^(floor(log2(largest)) - 2), which one byte holds as an exponent (biased by 127; at least 2^-126).  Values
+// are rounded to the nearest, ties to the even code, above 6 down to 6; a block that holds a value that is not finite
+// is NaN as a whole (exponent byte 255 over zero codes: 0 times infinity).  Lane l's 8 elements are one 32-bit word:
+//   keys    [half][lane][d / 32], exponents [half][slot 16][d / 32 or next power of two]
+//   values  [lane][dv / 16],      exponents [g][8 slots of g][dv / 32 or next power of two]
+// The codes go through the matrix instructions unscaled (exact in 16 bits); a key block's power multiplies its part of
+// the logit, a value block's power the weight, both in fp32.
+//
+// fp32 queries over 4-bit keys are three bf16 planes (24 bits); weights are two 16-bit planes, three for fp32 queries:
+// the products keep the accuracy of the output's type, and a step is bound by reading the cache.
+#include "rows.hpp"
+
+namespace sta {
+
+constexpr int RING_F4 = 3;  // storage code beside the element types F32, BF16, F16
+
+struct RingArgs {
+  Rows q, k, v;  // q [streams][heads][d], the new tokens k, v [streams][kv][d | dv] (sn unused)
+  int streams, heads, kv, group, chunks;  // chunks: groups of 16 query heads of a key head
+  int d, dv, nbk, nbv;   // blocks of 32 columns
+  int sinks, window, slots, tiles;
+  float scale, c;        // c = |scale| log2(e)
+  uint8_t *keys, *values, *kexp, *vexp;
+  int* counts;           // [streams][kv]
+  int append, nsplit;
+  float* part;           // [streams][heads][nsplit][dv + 2]: sums, then maximum and sum of weights
+  void* out;             // [streams][heads][dv]
+};
+
+__host__ __device__ constexpr int ring_exps(int nb) { return nb < 3 ? nb : 4; }  // exponent bytes of a slot
+__host__ __device__ constexpr int64_t ring_tile_bytes(int nb, int storage) {
+  return storage == RING_F4 ? 512 * nb : 1024 * nb * (storage == F32 ? 4 : 2);
+}
+__host__ __device__ constexpr int64_t ring_exp_bytes(int nb, int storage) {
+  return storage == RING_F4 ? 32 * ring_exps(nb) : 0;
+}
+
+__device__ __forceinline__ int ring_slot(const RingArgs& a, int p) {
+  return p < a.sinks ? p : a.sinks + (p - a.sinks) % a.window;
+}
+
+// byte of dimension col (keys) or column col (values) of slot r of a tile, whole elements; for F4 the byte that
+// holds the code (low half for even elements of a lane)
+__device__ __forceinline__ int ring_key_at(int r, int col, int nb, int storage) {
+  const int half = r >> 4, b = col >> 5, g = (col >> 3) & 3, j = col & 7, lane = 16 * g + (r & 15);
+  if (storage == RING_F4) return ((half * 64 + lane) * nb + b) * 4 + (j >> 1);
+  return (((half * nb + b) * 64 + lane) * 8 + j) * (storage == F32 ? 4 : 2);
+}
+__device__ __forceinline__ int ring_value_at(int r, int col, int nb, int storage) {
+  const int g = (r >> 2) & 3, j = 4 * (r >> 4) + (r & 3), lane = 16 * g + (col & 15), ct = col >> 4;
+  if (storage == RING_F4) return (lane * 2 * nb + ct) * 4 + (j >> 1);
+  return ((ct * 64 + lane) * 8 + j) * (storage == F32 ? 4 : 2);
+}
+__device__ __forceinline__ int ring_value_exp_at(int r, int b, int nb) {
+  return (((r >> 2) & 3) * 8 + 4 * (r >> 4) + (r & 3)) * ring_exps(nb) + b;
+}
+
+__device__ __forceinline__ float ring_power(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// the exponent byte of a block whose largest magnitude has these bits
+__device__ __forceinline__ int ring_exponent(uint32_t largest) {
+  if (largest >= 0x7f800000u) return 255;
+  const int e = static_cast<int>(largest >> 23) - 2;
+  return e < 1 ? 1 : e;
+}
+// the 4-bit code of x in a block with exponent byte e
+__device__ __forceinline__ uint32_t ring_code(float x, int e) {
+  if (e == 255) return 0u;
+  const float y = x * __uint_as_float(static_cast<uint32_t>(254 - e) << 23), m = fabsf(y);
+  const uint32_t c = (m > 0.25f) + (m >= 0.75f) + (m > 1.25f) + (m >= 1.75f) + (m > 2.5f) + (m >= 3.5f) + (m > 5.f);
+  return y < 0.f ? c | 8u : c;
+}
+__device__ __forceinline__ float ring_decode(uint32_t code) {
+  const float m[8] = {0.f, 0.5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
+  const float x = m[code & 7u];
+  return code & 8u ? -x : x;
+}
+
+template <int N>
+__device__ __forceinline__ void ring_load(uint32_t (&w)[N], const uint8_t* p) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = u.x;
+      w[4 * i + 1] = u.y;
+      w[4 * i + 2] = u.z;
+      w[4 * i + 3] = u.w;
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 u = reinterpret_cast<const uint2*>(p)[i];
+      w[2 * i] = u.x;
+      w[2 * i + 1] = u.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+  }
+}
+
+// Operands of the products.  TYPE: F32 (8 floats a lane), BF16, F16 (8 16-bit values a lane).
+typedef _Float16 ring_half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 ring_half2 __attribute__((ext_vector_type(2)));
+
+template <int TYPE>
+struct RingFrag {
+  uint32_t w[TYPE == F32 ? 8 : 4];
+};
+
+template <int TYPE>
+__device__ __forceinline__ floatx4 ring_mma(const RingFrag<TYPE>& a, const RingFrag<TYPE>& b, floatx4 c) {
+  if constexpr (TYPE == F32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c = mfma4(__uint_as_float(a.w[j]), __uint_as_float(b.w[j]), c);
+    return c;
+  } else if constexpr (TYPE == F16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(ring_half8, a.w),
+                                                  __builtin_bit_cast(ring_half8, b.w), c, 0, 0, 0);
+  } else {
+    return mfma_bf16(__builtin_bit_cast(bf16x8, a.w), __builtin_bit_cast(bf16x8, b.w), c);
+  }
+}
+
+// 8 floats as NP planes, each the rounding of what the planes before it leave
+template <int TYPE, int NP>
+__device__ __forceinline__ void ring_planes(const float (&x)[8], RingFrag<TYPE> (&f)[NP]) {
+  if constexpr (TYPE == F32) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[0].w[j] = __float_as_uint(x[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a = x[2 * j], b = x[2 * j + 1];
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        if constexpr (TYPE == F16) {
+          const ring_half2 h = __builtin_convertvector((floatx2{a, b}), ring_half2);
+          f[p].w[j] = __builtin_bit_cast(uint32_t, h);
+          a -= static_cast<float>(h[0]);
+          b -= static_cast<float>(h[1]);
+        } else {
+          const uint32_t u = pk_bf16(a, b);
+          f[p].w[j] = u;
+          a -= __uint_as_float(u << 16);
+          b -= __uint_as_float(u & 0xffff0000u);
+        }
+      }
+    }
+  }
+}
+
+// 8 codes as 16-bit values
+template <int TYPE>
+__device__ __forceinline__ RingFrag<TYPE> ring_values(uint32_t codes) {
+  RingFrag<TYPE> f;
+  if constexpr (TYPE == F16) {
+    f.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 0));
+    f.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 1));
+    f.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 2));
+    f.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 3));
+  } else {
+    f.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 0));
+    f.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 1));
+    f.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 2));
+    f.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 3));
+  }
+  return f;
+}
+
+// One token into its slot, by a workgroup of at least 64 + 32 nbv threads (the caller's barrier follows).
+template <int ST, int Q>
+__device__ void ring_put(const RingArgs& a, int s, int hk, int slot) {
+  constexpr int ES = Q == F32 ? 4 : 2;
+  const int64_t tile = (static_cast<int64_t>(s) * a.kv + hk) * a.tiles + (slot >> 5);
+  const int r = slot & 31, t = threadIdx.x;
+  if (t < 4 * a.nbk) {
+    const char* row = rows_at<ES>(a.k, s, hk, 0);
+    const int col = 8 * t;  // block t / 4, g = t % 4
+    uint8_t* at = a.keys + tile * ring_tile_bytes(a.nbk, ST) + ring_key_at(r, col, a.nbk, ST);
+    if constexpr (ST == RING_F4) {
+      float x[8];
+      uint32_t top = 0u, codes = 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x[j] = col + j < a.d ? load_elem(row, col + j, Q) : 0.f;
+        top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+      }
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
+      const int e = ring_exponent(top);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) codes |= ring_code(x[j], e) << (4 * j);
+      *reinterpret_cast<uint32_t*>(at) = codes;
+      if ((t & 3) == 0)
+        a.kexp[tile * ring_exp_bytes(a.nbk, ST) + r * ring_exps(a.nbk) + (t >> 2)] = static_cast<uint8_t>(e);
+    } else {
+#pragma unroll
+      for (int i = 0; i < ES / 2; ++i)
+        reinterpret_cast<uint4*>(at)[i] = rows_chunk<ES>(row, col + (16 / ES) * i, a.d, a.k.aligned);
+    }
+  } else if (t >= 64 && t < 64 + 32 * a.nbv) {
+    const int col = t - 64;
+    const char* row = rows_at<ES>(a.v, s, hk, 0);
+    uint8_t* at = a.values + tile * ring_tile_bytes(a.nbv, ST) + ring_value_at(r, col, a.nbv, ST);
+    if constexpr (ST == RING_F4) {
+      const float x = col < a.dv ? load_elem(row, col, Q) : 0.f;
+      uint32_t top = __float_as_uint(x) & 0x7fffffffu;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
+      const int e = ring_exponent(top);
+      const uint32_t code = ring_code(x, e), old = *at;
+      *at = static_cast<uint8_t>(r & 1 ? (old & 0x0fu) | (code << 4) : (old & 0xf0u) | code);
+      if ((col & 31) == 0)
+        a.vexp[tile * ring_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, col >> 5, a.nbv)] = static_cast<uint8_t>(e);
+    } else if constexpr (ES == 4) {
+      *reinterpret_cast<uint32_t*>(at) = col < a.dv ? reinterpret_cast<const uint32_t*>(row)[col] : 0u;
+    } else {
+      *reinterpret_cast<uint16_t*>(at) = col < a.dv ? reinterpret_cast<const uint16_t*>(row)[col] : uint16_t(0);
+    }
+  }
+}
+
+// A tile's operands as they lie in memory, for one lane
+template <int NBK, int NBV, int ST>
+struct RingTile {
+  static constexpr int W = ST == RING_F4 ? 1 : (ST == F32 ? 8 : 4);  // words of 8 elements
+  uint32_t k[2][NBK * W], v[2 * NBV * W];
+  uint32_t ke[ST == RING_F4 ? 2 * ring_exps(NBK) : 1], ve[ST == RING_F4 ? 2 * ring_exps(NBV) : 1];
+
+  __device__ __forceinline__ void load(const RingArgs& a, int64_t tile, int lane) {
+    const uint8_t* kp = a.keys + tile * ring_tile_bytes(NBK, ST);
+    const uint8_t* vp = a.values + tile * ring_tile_bytes(NBV, ST);
+    if constexpr (ST == RING_F4) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) ring_load(k[half], kp + (half * 64 + lane) * NBK * 4);
+      ring_load(v, vp + lane * 2 * NBV * 4);
+      // 4 slots of each half; 8 slots of the values' order
+      uint32_t e[ring_exps(NBK)];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        ring_load(e, a.kexp + tile * ring_exp_bytes(NBK, ST) + (16 * half + 4 * (lane >> 4)) * ring_exps(NBK));
+#pragma unroll
+        for (int i = 0; i < ring_exps(NBK); ++i) ke[half * ring_exps(NBK) + i] = e[i];
+      }
+      ring_load(ve, a.vexp + tile * ring_exp_bytes(NBV, ST) + 8 * (lane >> 4) * ring_exps(NBV));
+    } else {
+      uint32_t w[W];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int b = 0; b < NBK; ++b) {
+          ring_load(w, kp + (((half * NBK + b) * 64 + lane) * W) * 4);
+#pragma unroll
+          for (int i = 0; i < W; ++i) k[half][b * W + i] = w[i];
+        }
+#pragma unroll
+      for (int ct = 0; ct < 2 * NBV; ++ct) {
+        ring_load(w, vp + ((ct * 64 + lane) * W) * 4);
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[ct * W + i] = w[i];
+      }
+    }
+  }
+};
+
+// byte i of slot r in words of NE bytes a slot
+template <int NE>
+__device__ __forceinline__ float ring_exp_of(const uint32_t* w, int r, int b) {
+  const int at = r * NE + b;
+  return ring_power((w[at >> 2] >> (8 * (at & 3))) & 0xffu);
+}
+
+template <int NBK, int NBV, int ST, int Q>
+__global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(const RingArgs a) {
+  constexpr int XT = ST == RING_F4 ? (Q == F16 ? F16 : BF16) : ST;  // type of the logits' products
+  constexpr int PT = ST == RING_F4 ? BF16 : ST;                     // and of the value sums'
+  constexpr int QP = ST == RING_F4 && Q == F32 ? 3 : 1;             // planes of the queries
+  constexpr int PP = ST == F32 ? 1 : (Q == F32 ? 3 : 2);            // and of the weights
+  constexpr int ES = Q == F32 ? 4 : 2, CT = 2 * NBV, W = RingTile<NBK, NBV, ST>::W;
+  constexpr int PITCH = 32 * NBV + 4;
+  __shared__ float red[4 * 16 * PITCH], red_m[4 * 16], red_l[4 * 16];
+  int id = blockIdx.x;
+  const int split = id % a.nsplit;
+  id /= a.nsplit;
+  const int chunk = id % a.chunks, sh = id / a.chunks;
+  const int s = sh / a.kv, hk = sh - s * a.kv;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+
+  const int n = a.counts[sh];
+  const int held = n + a.append < a.slots ? n + a.append : a.slots;
+  const int all = (held + 31) >> 5, per = (all + a.nsplit - 1) / a.nsplit;
+  const int t0 = split * per, t1 = t0 + per < all ? t0 + per : all;
+  if (a.append) {
+    const int slot = ring_slot(a, n);
+    if ((slot >> 5) >= t0 && (slot >> 5) < t1) ring_put<ST, Q>(a, s, hk, slot);
+    __syncthreads();
+  }
+
+  const int queries = min(16, a.group - 16 * chunk);
+  RingFrag<XT> qf[NBK][QP];
+  {
+    const bool in = li < queries;
+    const char* row = rows_at<ES>(a.q, s, hk * a.group + 16 * chunk + (in ? li : 0), 0);
+#pragma unroll
+    for (int b = 0; b < NBK; ++b) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int col = 32 * b + 8 * lg + j;
+        x[j] = in && col < a.d ? load_elem(row, col, Q) : 0.f;
+        if (a.scale < 0.f) x[j] = -x[j];
+      }
+      ring_planes<XT, QP>(x, qf[b]);
+    }
+  }
+
+  floatx4 acc[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) acc[ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m = -3.4028235e38f, l = 0.f;
+
+  const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
+  RingTile<NBK, NBV, ST> cur, next;
+  if (t0 + wave < t1) cur.load(a, tile0 + t0 + wave, lane);
+  for (int t = t0 + wave; t < t1; t += 4) {
+    if (t + 4 < t1) next.load(a, tile0 + t + 4, lane);
+    floatx4 x[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      x[half] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < NBK; ++b) {
+        if constexpr (ST == RING_F4) {
+          const RingFrag<XT> k = ring_values<XT>(cur.k[half][b]);
+          floatx4 y = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int p = QP - 1; p >= 0; --p) y = ring_mma<XT>(k, qf[b][p], y);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            x[half][r] = fmaf(y[r], ring_exp_of<ring_exps(NBK)>(cur.ke + half * ring_exps(NBK), r, b), x[half][r]);
+        } else {
+          RingFrag<XT> k;
+#pragma unroll
+          for (int i = 0; i < W; ++i) k.w[i] = cur.k[half][b * W + i];
+          x[half] = ring_mma<XT>(k, qf[b][0], x[half]);
+        }
+      }
+    }
+    // slots of this lane that hold a token
+    const int left = held - 32 * t - 4 * lg;
+    const bool whole = held - 32 * t >= 32;
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (!whole && 16 * (i >> 2) + (i & 3) >= left) x[i >> 2][i & 3] = -__builtin_inff();
+      top = fmaxf(top, x[i >> 2][i & 3]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    if (__any(top > m)) {
+      const float shrink = __builtin_amdgcn_exp2f((m - top) * a.c);
+      l *= shrink;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) acc[ct] *= shrink;
+      m = top;
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f((x[i >> 2][i & 3] - m) * a.c);
+      if (!whole && 16 * (i >> 2) + (i & 3) >= left) p[i] = 0.f;
+      l += p[i];
+    }
+    if constexpr (ST == RING_F4) {
+#pragma unroll
+      for (int b = 0; b < NBV; ++b) {
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float e = ring_exp_of<ring_exps(NBV)>(cur.ve, i, b);
+          if (!whole && 16 * (i >> 2) + (i & 3) >= left) e = 0.f;
+          y[i] = p[i] * e;
+        }
+        RingFrag<PT> pf[PP];
+        ring_planes<PT, PP>(y, pf);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const RingFrag<PT> v = ring_values<PT>(cur.v[2 * b + h]);
+#pragma unroll
+          for (int k = PP - 1; k >= 0; --k) acc[2 * b + h] = ring_mma<PT>(v, pf[k], acc[2 * b + h]);
+        }
+      }
+    } else {
+      RingFrag<PT> pf[PP];
+      ring_planes<PT, PP>(p, pf);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        RingFrag<PT> v;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v.w[i] = cur.v[ct * W + i];
+        if (!whole) {  // slots without a token: whatever they hold
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (16 * (i >> 2) + (i & 3) >= left) {
+              if constexpr (ST == F32)
+                v.w[i] = 0u;
+              else
+                v.w[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+            }
+        }
+#pragma unroll
+        for (int k = PP - 1; k >= 0; --k) acc[ct] = ring_mma<PT>(v, pf[k], acc[ct]);
+      }
+    }
+    cur = next;
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+
+  // the four waves' sums
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+    *reinterpret_cast<floatx4*>(&red[(wave * 16 + li) * PITCH + 16 * ct + 4 * lg]) = acc[ct];
+  if (lg == 0) {
+    red_m[wave * 16 + li] = m;
+    red_l[wave * 16 + li] = l;
+  }
+  __syncthreads();
+  for (int at = threadIdx.x; at < queries * a.dv; at += 256) {
+    const int i = at / a.dv, col = at - i * a.dv;
+    float top = red_m[i], sum = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, red_m[16 * w + i]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = __builtin_amdgcn_exp2f((red_m[16 * w + i] - top) * a.c);
+      sum = fmaf(f, red[(w * 16 + i) * PITCH + col], sum);
+      den = fmaf(f, red_l[16 * w + i], den);
+    }
+    const int64_t head = static_cast<int64_t>(s) * a.heads + hk * a.group + 16 * chunk + i;
+    if (a.nsplit == 1) {
+      store_elem(a.out, head * a.dv + col, Q, held ? sum / den : 0.f);
+    } else {
+      float* part = a.part + (head * a.nsplit + split) * (a.dv + 2);
+      part[col] = sum;
+      if (col == 0) {
+        part[a.dv] = top;
+        part[a.dv + 1] = den;
+      }
+    }
+  }
+  // every thread has read the count; other workgroups read it only where ring_join_kernel counts
+  if (a.append && a.nsplit == 1 && a.chunks == 1 && threadIdx.x == 0) a.counts[sh] = n + 1;
+}
+
+// The splits' sums of a query head, and the count of a step that several workgroups share.
+template <int Q>
+__global__ __launch_bounds__(128) void ring_join_kernel(const RingArgs a) {
+  const int64_t head = blockIdx.x;
+  const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads, sh = s * a.kv + h / a.group;
+  const int col = threadIdx.x;
+  if (a.nsplit > 1 && col < a.dv) {
+    const float* part = a.part + head * a.nsplit * (a.dv + 2);
+    float top = -3.4028235e38f, sum = 0.f, den = 0.f;
+    for (int i = 0; i < a.nsplit; ++i) top = fmaxf(top, part[i * (a.dv + 2) + a.dv]);
+    for (int i = 0; i < a.nsplit; ++i) {
+      const float* p = part + i * (a.dv + 2);
+      const float f = __builtin_amdgcn_exp2f((p[a.dv] - top) * a.c);
+      sum = fmaf(f, p[col], sum);
+      den = fmaf(f, p[a.dv + 1], den);
+    }
+    const bool empty = !a.append && a.counts[sh] == 0;
+    store_elem(a.out, head * a.dv + col, Q, empty ? 0.f : sum / den);
+  }
+  if (a.append && h % a.group == 0) {
+    __syncthreads();
+    if (col == 0) a.counts[sh] += 1;
+  }
+}
+
+struct RingFill {
+  RingArgs a;          // k, v: [streams][kv][rows][d | dv] with row strides
+  int rows;
+  const int* take;     // [streams] or null: rows of a stream that are tokens
+};
+
+// The token (an index into the call's rows) that slot gets from rows 0 .. take-1 after n tokens, or -1.
+__device__ __forceinline__ int ring_token(const RingArgs& a, int slot, int n, int take) {
+  const int64_t end = static_cast<int64_t>(n) + take;  // positions [n, end)
+  int64_t p = slot;
+  if (slot >= a.sinks) {
+    if (end - 1 < slot) return -1;
+    p = slot + (end - 1 - slot) / a.window * a.window;
+  }
+  return p >= n && p < end ? static_cast<int>(p - n) : -1;
+}
+
+__device__ __forceinline__ int ring_take(const RingFill& f, int s) {
+  const int t = f.take ? f.take[s] : f.rows;
+  return t < 0 ? 0 : (t > f.rows ? f.rows : t);
+}
+
+// A workgroup a tile of 32 slots: the last token that falls into each slot.
+template <int ST, int Q>
+__global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
+  constexpr int ES = Q == F32 ? 4 : 2;
+  const RingArgs& a = f.a;
+  __shared__ uint32_t vals[32 * 132];  // the tile's values (bits, or codes), 32 nbv + 1 a slot
+  __shared__ int token[32];
+  const int sh = blockIdx.x / a.tiles, tile = blockIdx.x - sh * a.tiles, s = sh / a.kv, hk = sh - s * a.kv;
+  const int n = a.counts[sh], take = ring_take(f, s);
+  if (threadIdx.x < 32) {
+    const int slot = 32 * tile + threadIdx.x;
+    token[threadIdx.x] = slot < a.slots ? ring_token(a, slot, n, take) : -1;
+  }
+  __syncthreads();
+  const int64_t at = static_cast<int64_t>(sh) * a.tiles + tile;
+  uint8_t* keys = a.keys + at * ring_tile_bytes(a.nbk, ST);
+  uint8_t* values = a.values + at * ring_tile_bytes(a.nbv, ST);
+  const int pitch = 32 * a.nbv + 1;
+  // 8 columns of a slot's key a thread, 4 neighbouring threads a block
+  for (int i = threadIdx.x; i < 32 * 4 * a.nbk; i += 256) {
+    const int r = i / (4 * a.nbk), u = i - r * 4 * a.nbk, col = 8 * u, p = token[r];
+    const char* row = rows_at<ES>(a.k, s, hk, p < 0 ? 0 : p);
+    uint8_t* to = keys + ring_key_at(r, col, a.nbk, ST);
+    if constexpr (ST == RING_F4) {
+      float x[8];
+      uint32_t top = 0u, codes = 0u;
+      constexpr int E = 16 / ES;
+#pragma unroll
+      for (int c = 0; c < 8 / E; ++c) {
+        float y[E];
+        rows_unpack<Q>(p < 0 ? uint4{0u, 0u, 0u, 0u} : rows_chunk<ES>(row, col + E * c, a.d, a.k.aligned), y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          x[E * c + e] = y[e];
+          top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
+        }
+      }
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
+      const int e = ring_exponent(top);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) codes |= ring_code(x[j], e) << (4 * j);
+      if (p >= 0) {
+        *reinterpret_cast<uint32_t*>(to) = codes;
+        if ((u & 3) == 0)
+          a.kexp[at * ring_exp_bytes(a.nbk, ST) + r * ring_exps(a.nbk) + (u >> 2)] = static_cast<uint8_t>(e);
+      }
+    } else if (p >= 0) {
+#pragma unroll
+      for (int c = 0; c < ES / 2; ++c)
+        reinterpret_cast<uint4*>(to)[c] = rows_chunk<ES>(row, col + (16 / ES) * c, a.d, a.k.aligned);
+    }
+  }
+  // values: the rows (codes) of the tile's slots, then 8 slots of a column a thread
+  for (int i = threadIdx.x; i < 32 * 4 * a.nbv; i += 256) {
+    const int r = i / (4 * a.nbv), u = i - r * 4 * a.nbv, col = 8 * u, p = token[r];
+    const char* row = rows_at<ES>(a.v, s, hk, p < 0 ? 0 : p);
+    constexpr int E = 16 / ES;
+    uint32_t* to = vals + r * pitch + col;
+    float x[8];
+    uint32_t top = 0u;
+#pragma unroll
+    for (int c = 0; c < 8 / E; ++c) {
+      const uint4 w = p < 0 ? uint4{0u, 0u, 0u, 0u} : rows_chunk<ES>(row, col + E * c, a.dv, a.v.aligned);
+      if constexpr (ST == RING_F4) {
+        float y[E];
+        rows_unpack<Q>(w, y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          x[E * c + e] = y[e];
+          top = max(top, __float_as_uint(y[e]) & 0x7fffffffu);
+        }
+      } else {
+        const uint32_t z[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < E; ++e) to[E * c + e] = ES == 4 ? z[e & 3] : (z[(e >> 1) & 3] >> (16 * (e & 1))) & 0xffffu;
+      }
+    }
+    if constexpr (ST == RING_F4) {
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
+      top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
+      const int e = ring_exponent(top);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) to[j] = ring_code(x[j], e);
+      if (p >= 0 && (u & 3) == 0)
+        a.vexp[at * ring_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, u >> 2, a.nbv)] = static_cast<uint8_t>(e);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * 2 * a.nbv; i += 256) {
+    const int lane = i & 63, ct = i >> 6, g = lane >> 4, col = 16 * ct + (lane & 15);
+    if constexpr (ST == RING_F4) {
+      uint32_t* to = reinterpret_cast<uint32_t*>(values + (lane * 2 * a.nbv + ct) * 4);
+      uint32_t w = *to;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = 16 * (j >> 2) + 4 * g + (j & 3);
+        if (token[r] >= 0) w = (w & ~(0xfu << (4 * j))) | (vals[r * pitch + col] << (4 * j));
+      }
+      *to = w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = 16 * (j >> 2) + 4 * g + (j & 3);
+        if (token[r] < 0) continue;
+        if constexpr (ST == F32)
+          reinterpret_cast<uint32_t*>(values)[(ct * 64 + lane) * 8 + j] = vals[r * pitch + col];
+        else
+          reinterpret_cast<uint16_t*>(values)[(ct * 64 + lane) * 8 + j] = static_cast<uint16_t>(vals[r * pitch + col]);
+      }
+    }
+  }
+}
+
+// counts += the tokens that ring_extend_kernel has put in
+__global__ __launch_bounds__(256) static void ring_count_kernel(const RingFill f) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < f.a.streams * f.a.kv) f.a.counts[i] += ring_take(f, i / f.a.kv);
+}
+
+// The slots' rows as they stand for: keys [streams][kv][slots][d], values [..][dv] in the element type, zero where no
+// token is; positions [streams][slots], -1 there.  A workgroup a tile.
+template <int ST, int Q>
+__global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void* keys, void* values, int* positions) {
+  const int sh = blockIdx.x / a.tiles, tile = blockIdx.x - sh * a.tiles, s = sh / a.kv, hk = sh - s * a.kv;
+  const int n = a.counts[sh];
+  const int64_t at = static_cast<int64_t>(sh) * a.tiles + tile;
+  const uint8_t* kp = a.keys + at * ring_tile_bytes(a.nbk, ST);
+  const uint8_t* vp = a.values + at * ring_tile_bytes(a.nbv, ST);
+  for (int i = threadIdx.x; i < 32 * (a.d + a.dv); i += 256) {
+    const int r = i / (a.d + a.dv), u = i - r * (a.d + a.dv), slot = 32 * tile + r;
+    if (slot >= a.slots) break;
+    const bool key = u < a.d;
+    const int col = key ? u : u - a.d;
+    float x = 0.f;
+    if (slot < n) {
+      const uint8_t* p = key ? kp + ring_key_at(r, col, a.nbk, ST) : vp + ring_value_at(r, col, a.nbv, ST);
+      if constexpr (ST == RING_F4) {
+        const uint32_t code = *p >> (4 * ((key ? col : r) & 1));
+        const uint32_t e = key ? a.kexp[at * ring_exp_bytes(a.nbk, ST) + r * ring_exps(a.nbk) + (col >> 5)]
+                               : a.vexp[at * ring_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, col >> 5, a.nbv)];
+        x = ring_decode(code & 15u) * ring_power(e);
+      } else {
+        x = load_elem(p, 0, ST);
+      }
+    }
+    const int64_t row = static_cast<int64_t>(sh) * a.slots + slot;
+    if (key)
+      store_elem(keys, row * a.d + col, Q, x);
+    else
+      store_elem(values, row * a.dv + col, Q, x);
+  }
+  if (hk == 0 && threadIdx.x < 32) {
+    const int slot = 32 * tile + threadIdx.x;
+    if (slot < a.slots) {
+      int p = -1;
+      if (slot < n) p = slot < a.sinks ? slot : slot + (n - 1 - slot) / a.window * a.window;
+      positions[static_cast<int64_t>(s) * a.slots + slot] = p;
+    }
+  }
+}
+
+}  // namespace sta

@@ -4,6 +4,8 @@ of the other modules: the same bounded state, exact weights, and no view of what
     sink_window_causal_attention   [N,D] or [B,H,N,D] sequences, differentiable in q, k and v
     sink_window_forward, sink_window_backward
                                    the two passes by themselves, for captured graphs and programs without autograd
+    SinkWindowStreamingAttention   its serving form: a cache of sinks and a ring of `window` tokens for streams in
+                                   lockstep, in the element type or in 4 bits, and one query a head at a time
 
 Row i sees the keys j <= i with i - j < window or j < sinks; window >= N is exact causal attention.  Key heads may be
 shared: k and v may have fewer heads than q (a divisor).  Computed by hand-written HIP kernels on the inputs'
@@ -14,7 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -22,7 +24,8 @@ import _native
 
 Tensor = torch.Tensor
 
-__all__ = ["sink_window_causal_attention", "sink_window_forward", "sink_window_backward"]
+__all__ = ["SinkWindowStreamingAttention", "sink_window_backward", "sink_window_causal_attention",
+           "sink_window_forward"]
 
 MAX_DIM = 128  # key and value widths of the kernels
 MAX_ROWS = 1 << 30
@@ -236,3 +239,201 @@ def sink_window_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Ten
     _check_gpu(q=q4, grad=grad, out=out, lse=lse)
     dq, dk, dv = _backward(grad, q4, k4, v4, out, lse, window, sinks, s, lengths)
     return (dq[0, 0], dk[0, 0], dv[0, 0]) if q.ndim == 2 else (dq, dk, dv)
+
+
+class SinkWindowStreamingAttention:
+    """Exact streaming attention over the last `window` tokens and the first `sinks` ones of every stream: a cache
+    of sinks + window tokens a stream and key head, whatever the streams' length.
+
+    `step(q, k, v)` takes one token of every stream: keys [S,Hkv,dim], values [S,Hkv,value_dim], queries [S,H,dim] ->
+    [S,H,value_dim], H a multiple of Hkv; `update` and `query` are its two halves, `extend` takes prompts in bulk and
+    `prefill` answers them too.  Queries see every token held, their own step's among them.
+
+    dtype (float32, bfloat16, float16) is that of inputs and outputs; storage None keeps the cache in it, "fp4" in 4
+    bits: blocks of 32 columns of a token as 4-bit floats (0, 0.5, 1, 1.5, 2, 3, 4, 6 and signs) times a power of two,
+    4.25 bits a value (a block with a value that is not finite becomes NaN).  Sums and softmax statistics are fp32.
+
+    Calls run on the device's current stream and may be captured into graphs (replays advance the state like
+    calls); calls on one object have to be ordered, by one stream or by events."""
+
+    def __init__(self, dim: int, value_dim: int, *, streams: int = 1, heads: int = 1, kv_heads: Optional[int] = None,
+                 window: int, sinks: int = 4, scale: Optional[float] = None,
+                 dtype: torch.dtype = torch.float32, storage: Optional[str] = None,
+                 device: Optional[Union[str, torch.device]] = None) -> None:
+        kv_heads = heads if kv_heads is None else kv_heads
+        if streams < 1 or heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise ValueError("streams and heads must be positive and heads a multiple of kv_heads")
+        if not 1 <= dim <= MAX_DIM or not 1 <= value_dim <= MAX_DIM:
+            raise ValueError(f"key and value widths must be 1 .. {MAX_DIM}, got {dim} and {value_dim}")
+        if window + sinks > MAX_ROWS:
+            raise ValueError(f"a cache of at most {MAX_ROWS} tokens is supported")
+        if dtype not in _native.DTYPE_CODES:
+            raise ValueError(f"dtype {dtype} is not supported (use float32, bfloat16 or float16)")
+        if storage not in (None, "fp4"):
+            raise ValueError("storage must be None or 'fp4'")
+        self.window, self.sinks = _check_tokens(window, sinks)
+        self.scale = _attention_scale(scale, dim)
+        self.dim, self.value_dim, self.streams, self.heads, self.kv_heads = dim, value_dim, streams, heads, kv_heads
+        self.dtype, self.storage = dtype, storage
+        dev = torch.device("cuda" if device is None else device)
+        if dev.type != "cuda":
+            raise ValueError(f"HIP kernels require a GPU (cuda/ROCm) device, got {dev}")
+        if not torch.cuda.is_available():
+            raise RuntimeError("streaming-attention HIP kernels need a ROCm GPU; none is visible")
+        self.device = torch.device("cuda", torch.cuda.current_device() if dev.index is None else dev.index)
+        self._code = _native.DTYPE_CODES[dtype]
+        self._store = self._code if storage is None else _native.STORAGE_FP4
+        sizes = (ctypes.c_int64 * 4)()
+        _native.check(_native.lib().sta_ring_layout(self._code, self._store, streams, kv_heads, dim, value_dim,
+                                                    self.window, self.sinks, sizes), "sta_ring_layout")
+        self._cache = [torch.zeros(n, device=self.device, dtype=torch.uint8) if n else None for n in sizes]
+        self._counts = torch.zeros((streams, kv_heads), device=self.device, dtype=torch.int32)
+        self._bytes = _native.lib().sta_ring_attention_bytes(streams, heads, kv_heads, dim, value_dim, self.window,
+                                                             self.sinks)
+        self._fresh = True
+
+    @property
+    def lengths(self) -> Tensor:
+        """int32 [S] on the device: tokens that each stream has taken (a view of the state)."""
+        return self._counts[:, 0]
+
+    def _rows(self, x: Tensor, want: Tuple[int, ...], what: str) -> Tensor:
+        if tuple(x.shape) != want:
+            raise ValueError(f"{what} must be {list(want)}, got {list(x.shape)}")
+        if x.dtype != self.dtype or x.device != self.device:
+            x = x.to(device=self.device, dtype=self.dtype)
+        return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+    def _attend(self, q: Tensor, k: Optional[Tensor], v: Optional[Tensor]) -> Tensor:
+        out = torch.empty((self.streams, self.heads, self.value_dim), device=self.device, dtype=self.dtype)
+        ws = torch.empty(self._bytes, device=self.device, dtype=torch.uint8) if self._bytes else None
+        none = (0, 0)
+        strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *(none if k is None else k.stride()[:2]),
+                                       *(none if v is None else v.stride()[:2]))
+        with torch.cuda.device(self.device):
+            st = _native.lib().sta_ring_attention(
+                q.data_ptr(), _native.ptr(k), _native.ptr(v), self._code, self._store, self.streams, self.heads,
+                self.kv_heads, self.dim, self.value_dim, strides, self.scale, self.window, self.sinks,
+                *(_native.ptr(x) for x in self._cache), self._counts.data_ptr(), out.data_ptr(), _native.ptr(ws),
+                self._bytes, _native.stream_handle(self.device))
+        _native.check(st, "sta_ring_attention")
+        return out
+
+    @torch.no_grad()
+    def step(self, query: Tensor, key: Tensor, value: Tensor) -> Tensor:
+        """One token of every stream into the cache, then one query a head: update(key, value); query(query)."""
+        q = self._rows(query, (self.streams, self.heads, self.dim), "query")
+        k = self._rows(key, (self.streams, self.kv_heads, self.dim), "key")
+        v = self._rows(value, (self.streams, self.kv_heads, self.value_dim), "value")
+        self._fresh = False
+        return self._attend(q, k, v)
+
+    @torch.no_grad()
+    def query(self, query: Tensor) -> Tensor:
+        """Attention of one query a head over the tokens held; zero for a stream that holds none."""
+        return self._attend(self._rows(query, (self.streams, self.heads, self.dim), "query"), None, None)
+
+    @torch.no_grad()
+    def update(self, key: Tensor, value: Tensor) -> None:
+        """One token of every stream into the cache."""
+        k = self._rows(key, (self.streams, self.kv_heads, self.dim), "key")
+        v = self._rows(value, (self.streams, self.kv_heads, self.value_dim), "value")
+        self._extend(k[:, :, None], v[:, :, None], None)
+
+    def _extend(self, k: Tensor, v: Tensor, counts: Optional[Tensor]) -> None:
+        self._fresh = False
+        if k.shape[2] == 0:
+            return
+        with torch.cuda.device(self.device):
+            st = _native.lib().sta_ring_extend(
+                k.data_ptr(), v.data_ptr(), self._code, self._store, self.streams, self.kv_heads, k.shape[2], self.dim,
+                self.value_dim, _strides(k, v), self.window, self.sinks, _native.ptr(counts),
+                *(_native.ptr(x) for x in self._cache), self._counts.data_ptr(), _native.stream_handle(self.device))
+        _native.check(st, "sta_ring_extend")
+
+    def _prompt(self, keys: Tensor, values: Tensor, counts: Optional[Tensor]):
+        rows = keys.shape[2] if keys.ndim == 4 else 0
+        if rows > MAX_ROWS:
+            raise ValueError(f"at most {MAX_ROWS} rows at a time are supported")
+        k = self._rows(keys, (self.streams, self.kv_heads, rows, self.dim), "keys")
+        v = self._rows(values, (self.streams, self.kv_heads, rows, self.value_dim), "values")
+        if counts is not None:
+            counts = _check_lengths(counts, self.streams)
+            if counts.device != self.device:
+                raise ValueError("counts must be on the object's device")
+        return k, v, counts
+
+    @torch.no_grad()
+    def extend(self, keys: Tensor, values: Tensor, *, counts: Optional[Tensor] = None) -> None:
+        """update() with the rows of keys [S,Hkv,P,dim] and values [S,Hkv,P,value_dim] in bulk; counts: int32 [S] on
+        the device, the rows of every stream that are tokens (None: all P; values outside 0 .. P are taken as the
+        nearest of them)."""
+        self._extend(*self._prompt(keys, values, counts))
+
+    @torch.no_grad()
+    def prefill(self, q: Tensor, k: Tensor, v: Tensor, *, counts: Optional[Tensor] = None) -> Tensor:
+        """Outputs [S,H,P,value_dim] of a prompt's rows (sink_window_causal_attention, on the rows as given), leaving
+        the state after it.  Only on a fresh state."""
+        if not self._fresh:
+            raise ValueError("prefill starts from an empty state; use step() / extend() afterwards")
+        k, v, counts = self._prompt(k, v, counts)
+        q = self._rows(q, (self.streams, self.heads, k.shape[2], self.dim), "q")
+        out = sink_window_causal_attention(q, k, v, window=self.window, sinks=self.sinks, scale=self.scale,
+                                           lengths=counts)
+        self._extend(k, v, counts)
+        return out
+
+    @torch.no_grad()
+    def reset(self, streams: Optional[Sequence[int]] = None) -> None:
+        """Forgets every token of all streams, or of the given ones (new sequences start there)."""
+        if streams is None:
+            self._counts.zero_()
+            self._fresh = True
+            return
+        for i in streams:
+            if not 0 <= i < self.streams:
+                raise ValueError(f"there is no stream {i}")
+            self._counts[i].zero_()
+
+    @torch.no_grad()
+    def items(self) -> Tuple[Tensor, Tensor, Tensor]:
+        """(keys [S,Hkv,sinks + window,dim], values [S,Hkv,sinks + window,value_dim], positions int32
+        [S,sinks + window]) as the cache holds them, in the order of its slots; zero and -1 where no token is."""
+        slots = self.sinks + self.window
+        keys = torch.empty((self.streams, self.kv_heads, slots, self.dim), device=self.device, dtype=self.dtype)
+        values = torch.empty((self.streams, self.kv_heads, slots, self.value_dim), device=self.device, dtype=self.dtype)
+        positions = torch.empty((self.streams, slots), device=self.device, dtype=torch.int32)
+        with torch.cuda.device(self.device):
+            st = _native.lib().sta_ring_items(
+                self._code, self._store, self.streams, self.kv_heads, self.dim, self.value_dim, self.window, self.sinks,
+                *(_native.ptr(x) for x in self._cache), self._counts.data_ptr(), keys.data_ptr(), values.data_ptr(),
+                positions.data_ptr(), _native.stream_handle(self.device))
+        _native.check(st, "sta_ring_items")
+        return keys, values, positions
+
+    def state_size_bytes(self) -> int:
+        """Device bytes of the cache."""
+        return sum(x.numel() for x in self._cache if x is not None) + 4 * self._counts.numel()
+
+    def state_dict_settings(self) -> dict:
+        return {"dim": self.dim, "value_dim": self.value_dim, "streams": self.streams, "heads": self.heads,
+                "kv_heads": self.kv_heads, "window": self.window, "sinks": self.sinks, "scale": self.scale,
+                "dtype": str(self.dtype), "storage": self.storage}
+
+    def state_dict(self) -> dict:
+        """The state for a later resume: plain tensors on the host and Python scalars."""
+        return {"attention": self.state_dict_settings(), "counts": self._counts.cpu(),
+                "cache": [None if x is None else x.cpu() for x in self._cache]}
+
+    def load_state_dict(self, state: dict) -> None:
+        """Resume from state_dict() of an object built with the same settings (the device may differ)."""
+        mine = self.state_dict_settings()
+        if state["attention"] != mine:
+            raise ValueError(f"state settings {state['attention']} do not match this object's {mine}")
+        for x, y in zip((self._counts, *self._cache), (state["counts"], *state["cache"])):
+            if (x is None) != (y is None) or (x is not None and (x.shape != y.shape or x.dtype != y.dtype)):
+                raise ValueError("the state's tensors do not match this object's")
+        for x, y in zip((self._counts, *self._cache), (state["counts"], *state["cache"])):
+            if x is not None:
+                x.copy_(y)
+        self._fresh = not bool(state["counts"].any())
