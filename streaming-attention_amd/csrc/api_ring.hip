@@ -52,11 +52,15 @@ int ring_shape(sta::RingArgs& a, int64_t streams, int heads, int kv_heads, int d
   return STA_OK;
 }
 
-// Workgroups that share a key head's slots: enough for four a compute unit (256), each with at least 8 tiles of 32 slots.
+// Workgroups that share a key head's slots.  A compute unit holds 2 to 4 at a time and the card has 256: up to 1536 keep
+// them busy to the end (64 x 8 key heads of 32772 tokens in 4 bits: 2 workgroups a head 397 us, 3 388, 4 392).  Each has
+// at least 16 tiles of 32 slots: shorter ones cost the second launch more than they save the first (one key head of
+// 65552: 257 workgroups 7.6 + 6.4 us, 128 8.2 + 4.2; 260 tokens in one 8.0, in two 6.3 + 2.5).
 int splits_of(const sta::RingArgs& a) {
   const int64_t blocks = static_cast<int64_t>(a.streams) * a.kv * a.chunks;
-  int64_t want = 1024 / blocks;
-  if (want > (a.tiles + 7) / 8) want = (a.tiles + 7) / 8;
+  int64_t want = 1536 / blocks;
+  if (want > a.tiles / 16) want = a.tiles / 16;
+  if (want > sta::RING_SPLITS) want = sta::RING_SPLITS;
   return static_cast<int>(want < 1 ? 1 : want);
 }
 
@@ -99,8 +103,8 @@ int sta_ring_layout(int dtype, int storage, int64_t streams, int kv_heads, int d
   const int64_t tiles = static_cast<int64_t>(a.streams) * a.kv * a.tiles;
   bytes[0] = tiles * sta::ring_tile_bytes(a.nbk, storage);
   bytes[1] = tiles * sta::ring_tile_bytes(a.nbv, storage);
-  bytes[2] = tiles * sta::ring_exp_bytes(a.nbk, storage);
-  bytes[3] = tiles * sta::ring_exp_bytes(a.nbv, storage);
+  bytes[2] = tiles * sta::ring_key_exp_bytes(a.nbk, storage);
+  bytes[3] = tiles * sta::ring_value_exp_bytes(a.nbv, storage);
   return STA_OK;
 }
 

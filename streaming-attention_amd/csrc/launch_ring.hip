@@ -23,7 +23,7 @@ int launch_ring(const sta::RingArgs& a, hipStream_t s) {
     default: hipLaunchKernelGGL((sta::ring_attention_kernel<NBK, 4, ST, Q>), g, dim3(256), 0, s, a);
   }
   if (a.nsplit > 1 || (a.append && a.chunks > 1))
-    hipLaunchKernelGGL((sta::ring_join_kernel<Q>), dim3(static_cast<unsigned>(heads)), dim3(128), 0, s, a);
+    hipLaunchKernelGGL((sta::ring_join_kernel<Q>), dim3(static_cast<unsigned>(heads)), dim3(512), 0, s, a);
   return check_launch();
 }
 

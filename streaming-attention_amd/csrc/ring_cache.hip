@@ -14,14 +14,15 @@
 // Storage in 4 bits (fp4): values in blocks of 32 columns of a token, each 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign,
 // times 2^(floor(log2(largest)) - 2), which one byte holds as an exponent (biased by 127; at least 2^-126).  Values
 // are rounded to the nearest, ties to the even code, above 6 down to 6; a block that holds a value that is not finite
-// is NaN as a whole (exponent byte 255 over zero codes: 0 times infinity).  Lane l's 8 elements are one 32-bit word:
-//   keys    [half][lane][d / 32], exponents [half][slot 16][d / 32 or next power of two]
-//   values  [lane][dv / 16],      exponents [g][8 slots of g][dv / 32 or next power of two]
-// The codes go through the matrix instructions unscaled (exact in 16 bits); a key block's power multiplies its part of
-// the logit, a value block's power the weight, both in fp32.
-//
-// fp32 queries over 4-bit keys are three bf16 planes (24 bits); weights are two 16-bit planes, three for fp32 queries:
-// the products keep the accuracy of the output's type, and a step is bound by reading the cache.
+// is NaN as a whole (exponent byte 255, which the conversion turns into NaN whatever the code).
+//   keys    [half][lane][d / 32] words of 8 codes, exponents [slot 16][half][d / 32 or next power of two]
+//   values  [lane][dv / 32][8 slots] bytes, columns 32 b + i and 32 b + 16 + i of a slot in the halves of a byte (so that
+//           both take one exponent in one conversion, and a token writes whole bytes), exponents [g][dv / 32][8 slots]
+// Codes become bf16 with their powers (exact); queries of more than 8 bits and the weights are carried as bf16 planes (fp16
+// queries 2, fp32 3; weights 2, 3 for fp32), of 16-bit caches as 2 planes of their type: the products keep the accuracy
+// of the output's type, and a step is bound by reading the cache.
+#include <type_traits>
+
 #include "rows.hpp"
 
 namespace sta {
@@ -45,16 +46,19 @@ __host__ __device__ constexpr int ring_exps(int nb) { return nb < 3 ? nb : 4; } 
 __host__ __device__ constexpr int64_t ring_tile_bytes(int nb, int storage) {
   return storage == RING_F4 ? 512 * nb : 1024 * nb * (storage == F32 ? 4 : 2);
 }
-__host__ __device__ constexpr int64_t ring_exp_bytes(int nb, int storage) {
+__host__ __device__ constexpr int64_t ring_key_exp_bytes(int nb, int storage) {
   return storage == RING_F4 ? 32 * ring_exps(nb) : 0;
+}
+__host__ __device__ constexpr int64_t ring_value_exp_bytes(int nb, int storage) {
+  return storage == RING_F4 ? 32 * nb : 0;
 }
 
 __device__ __forceinline__ int ring_slot(const RingArgs& a, int p) {
   return p < a.sinks ? p : a.sinks + (p - a.sinks) % a.window;
 }
 
-// byte of dimension col (keys) or column col (values) of slot r of a tile, whole elements; for F4 the byte that
-// holds the code (low half for even elements of a lane)
+// byte of dimension col (keys) or column col (values) of slot r of a tile; of 4-bit caches the byte that holds the
+// code (keys: low half for even dimensions, values: for the first 16 columns of a block)
 __device__ __forceinline__ int ring_key_at(int r, int col, int nb, int storage) {
   const int half = r >> 4, b = col >> 5, g = (col >> 3) & 3, j = col & 7, lane = 16 * g + (r & 15);
   if (storage == RING_F4) return ((half * 64 + lane) * nb + b) * 4 + (j >> 1);
@@ -62,11 +66,14 @@ __device__ __forceinline__ int ring_key_at(int r, int col, int nb, int storage) 
 }
 __device__ __forceinline__ int ring_value_at(int r, int col, int nb, int storage) {
   const int g = (r >> 2) & 3, j = 4 * (r >> 4) + (r & 3), lane = 16 * g + (col & 15), ct = col >> 4;
-  if (storage == RING_F4) return (lane * 2 * nb + ct) * 4 + (j >> 1);
+  if (storage == RING_F4) return (lane * nb + (ct >> 1)) * 8 + j;
   return ((ct * 64 + lane) * 8 + j) * (storage == F32 ? 4 : 2);
 }
+__device__ __forceinline__ int ring_key_exp_at(int r, int b, int nb) {
+  return ((r & 15) * 2 + (r >> 4)) * ring_exps(nb) + b;
+}
 __device__ __forceinline__ int ring_value_exp_at(int r, int b, int nb) {
-  return (((r >> 2) & 3) * 8 + 4 * (r >> 4) + (r & 3)) * ring_exps(nb) + b;
+  return (((r >> 2) & 3) * nb + b) * 8 + 4 * (r >> 4) + (r & 3);
 }
 
 __device__ __forceinline__ float ring_power(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -90,27 +97,29 @@ __device__ __forceinline__ float ring_decode(uint32_t code) {
   return code & 8u ? -x : x;
 }
 
+// N words in the widest loads that N allows, past the caches' usual policy: a step reads each tile once (reading 2 GiB
+// 7.0 TB/s that way, 6.4 with plain loads)
 template <int N>
 __device__ __forceinline__ void ring_load(uint32_t (&w)[N], const uint8_t* p) {
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  typedef uint32_t u2 __attribute__((ext_vector_type(2)));
   if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-      w[4 * i] = u.x;
-      w[4 * i + 1] = u.y;
-      w[4 * i + 2] = u.z;
-      w[4 * i + 3] = u.w;
+      const u4 u = __builtin_nontemporal_load(reinterpret_cast<const u4*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[4 * i + j] = u[j];
     }
   } else if constexpr (N % 2 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 2; ++i) {
-      const uint2 u = reinterpret_cast<const uint2*>(p)[i];
-      w[2 * i] = u.x;
-      w[2 * i + 1] = u.y;
+      const u2 u = __builtin_nontemporal_load(reinterpret_cast<const u2*>(p) + i);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) w[2 * i + j] = u[j];
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    for (int i = 0; i < N; ++i) w[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(p) + i);
   }
 }
 
@@ -165,22 +174,29 @@ __device__ __forceinline__ void ring_planes(const float (&x)[8], RingFrag<TYPE> 
   }
 }
 
-// 8 codes as 16-bit values
-template <int TYPE>
-__device__ __forceinline__ RingFrag<TYPE> ring_values(uint32_t codes) {
-  RingFrag<TYPE> f;
-  if constexpr (TYPE == F16) {
-    f.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 0));
-    f.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 1));
-    f.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 2));
-    f.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, 1.f, 3));
-  } else {
-    f.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 0));
-    f.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 1));
-    f.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 2));
-    f.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, 1.f, 3));
-  }
+// 8 codes as bf16 values times one power
+__device__ __forceinline__ RingFrag<BF16> ring_key_values(uint32_t codes, float power) {
+  RingFrag<BF16> f;
+  f.w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 0));
+  f.w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 1));
+  f.w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 2));
+  f.w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power, 3));
   return f;
+}
+
+// 4 slots' pairs of columns (a byte each) times their powers, and the two columns' words of 4 slots each
+__device__ __forceinline__ void ring_value_words(uint32_t codes, const float (&power)[4], uint32_t (&first)[2],
+                                                 uint32_t (&second)[2]) {
+  uint32_t r[4];
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power[0], 0));
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power[1], 1));
+  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power[2], 2));
+  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, power[3], 3));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    first[i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x05040100u);
+    second[i] = __builtin_amdgcn_perm(r[2 * i + 1], r[2 * i], 0x07060302u);
+  }
 }
 
 // One token into its slot, by a workgroup of at least 64 + 32 nbv threads (the caller's barrier follows).
@@ -208,30 +224,32 @@ __device__ void ring_put(const RingArgs& a, int s, int hk, int slot) {
       for (int j = 0; j < 8; ++j) codes |= ring_code(x[j], e) << (4 * j);
       *reinterpret_cast<uint32_t*>(at) = codes;
       if ((t & 3) == 0)
-        a.kexp[tile * ring_exp_bytes(a.nbk, ST) + r * ring_exps(a.nbk) + (t >> 2)] = static_cast<uint8_t>(e);
+        a.kexp[tile * ring_key_exp_bytes(a.nbk, ST) + ring_key_exp_at(r, t >> 2, a.nbk)] = static_cast<uint8_t>(e);
     } else {
 #pragma unroll
       for (int i = 0; i < ES / 2; ++i)
         reinterpret_cast<uint4*>(at)[i] = rows_chunk<ES>(row, col + (16 / ES) * i, a.d, a.k.aligned);
     }
-  } else if (t >= 64 && t < 64 + 32 * a.nbv) {
-    const int col = t - 64;
+  } else if (t >= 64 && t < 64 + (ST == RING_F4 ? 16 : 32) * a.nbv) {
     const char* row = rows_at<ES>(a.v, s, hk, 0);
-    uint8_t* at = a.values + tile * ring_tile_bytes(a.nbv, ST) + ring_value_at(r, col, a.nbv, ST);
+    uint8_t* values = a.values + tile * ring_tile_bytes(a.nbv, ST);
     if constexpr (ST == RING_F4) {
-      const float x = col < a.dv ? load_elem(row, col, Q) : 0.f;
-      uint32_t top = __float_as_uint(x) & 0x7fffffffu;
+      const int b = (t - 64) >> 4, c0 = 32 * b + (t & 15), c1 = c0 + 16;
+      const float x0 = c0 < a.dv ? load_elem(row, c0, Q) : 0.f, x1 = c1 < a.dv ? load_elem(row, c1, Q) : 0.f;
+      uint32_t top = max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
+      for (int o = 8; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
       const int e = ring_exponent(top);
-      const uint32_t code = ring_code(x, e), old = *at;
-      *at = static_cast<uint8_t>(r & 1 ? (old & 0x0fu) | (code << 4) : (old & 0xf0u) | code);
-      if ((col & 31) == 0)
-        a.vexp[tile * ring_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, col >> 5, a.nbv)] = static_cast<uint8_t>(e);
-    } else if constexpr (ES == 4) {
-      *reinterpret_cast<uint32_t*>(at) = col < a.dv ? reinterpret_cast<const uint32_t*>(row)[col] : 0u;
+      values[ring_value_at(r, c0, a.nbv, ST)] = static_cast<uint8_t>(ring_code(x0, e) | ring_code(x1, e) << 4);
+      if ((t & 15) == 0)
+        a.vexp[tile * ring_value_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, b, a.nbv)] = static_cast<uint8_t>(e);
     } else {
-      *reinterpret_cast<uint16_t*>(at) = col < a.dv ? reinterpret_cast<const uint16_t*>(row)[col] : uint16_t(0);
+      const int col = t - 64;
+      uint8_t* at = values + ring_value_at(r, col, a.nbv, ST);
+      if constexpr (ES == 4)
+        *reinterpret_cast<uint32_t*>(at) = col < a.dv ? reinterpret_cast<const uint32_t*>(row)[col] : 0u;
+      else
+        *reinterpret_cast<uint16_t*>(at) = col < a.dv ? reinterpret_cast<const uint16_t*>(row)[col] : uint16_t(0);
     }
   }
 }
@@ -241,7 +259,8 @@ template <int NBK, int NBV, int ST>
 struct RingTile {
   static constexpr int W = ST == RING_F4 ? 1 : (ST == F32 ? 8 : 4);  // words of 8 elements
   uint32_t k[2][NBK * W], v[2 * NBV * W];
-  uint32_t ke[ST == RING_F4 ? 2 * ring_exps(NBK) : 1], ve[ST == RING_F4 ? 2 * ring_exps(NBV) : 1];
+  static constexpr int KE = ring_exps(NBK) == 4 ? 2 : 1;  // words of a slot pair's exponents
+  uint32_t ke[KE], ve[2 * NBV];
 
   __device__ __forceinline__ void load(const RingArgs& a, int64_t tile, int lane) {
     const uint8_t* kp = a.keys + tile * ring_tile_bytes(NBK, ST);
@@ -250,15 +269,12 @@ struct RingTile {
 #pragma unroll
       for (int half = 0; half < 2; ++half) ring_load(k[half], kp + (half * 64 + lane) * NBK * 4);
       ring_load(v, vp + lane * 2 * NBV * 4);
-      // 4 slots of each half; 8 slots of the values' order
-      uint32_t e[ring_exps(NBK)];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        ring_load(e, a.kexp + tile * ring_exp_bytes(NBK, ST) + (16 * half + 4 * (lane >> 4)) * ring_exps(NBK));
-#pragma unroll
-        for (int i = 0; i < ring_exps(NBK); ++i) ke[half * ring_exps(NBK) + i] = e[i];
-      }
-      ring_load(ve, a.vexp + tile * ring_exp_bytes(NBV, ST) + 8 * (lane >> 4) * ring_exps(NBV));
+      const uint8_t* ep = a.kexp + tile * ring_key_exp_bytes(NBK, ST) + (lane & 15) * 2 * ring_exps(NBK);
+      if constexpr (NBK == 1)
+        ke[0] = *reinterpret_cast<const uint16_t*>(ep);
+      else
+        ring_load(ke, ep);
+      ring_load(ve, a.vexp + tile * ring_value_exp_bytes(NBV, ST) + (lane >> 4) * 8 * NBV);
     } else {
       uint32_t w[W];
 #pragma unroll
@@ -279,19 +295,22 @@ struct RingTile {
   }
 };
 
-// byte i of slot r in words of NE bytes a slot
-template <int NE>
-__device__ __forceinline__ float ring_exp_of(const uint32_t* w, int r, int b) {
-  const int at = r * NE + b;
-  return ring_power((w[at >> 2] >> (8 * (at & 3))) & 0xffu);
+// the power of two in byte i of exponent words
+__device__ __forceinline__ float ring_power_of(const uint32_t* w, int i) {
+  return ring_power((w[i >> 2] >> (8 * (i & 3))) & 0xffu);
 }
 
+// A workgroup a share of a key head's tiles, its four waves every fourth tile, joined through LDS at the end.  The
+// matrix instructions have 16 columns for the query heads of a key head; with fewer they idle, which costs nothing: bound
+// by reading the cache, for 4 bits nearly as much by the conversions (285 VALU instructions a tile of 128 + 128 columns,
+// 69 % of the cycles at 4.7 TB/s).  64 x 32 heads x 4100 tokens of 64 + 64 bf16 (2.15 GB): 345 us, 6.2 TB/s; 64 x 8 key
+// heads x 32772 tokens of 128 + 128 in 4 bits (2.28 GB): 388 us, 5.9 TB/s (558 us with the exponents multiplied into
+// logits and weights, 480 with a check for the last tile in every tile); plain reads reach 7.0 TB/s.
 template <int NBK, int NBV, int ST, int Q>
 __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(const RingArgs a) {
-  constexpr int XT = ST == RING_F4 ? (Q == F16 ? F16 : BF16) : ST;  // type of the logits' products
-  constexpr int PT = ST == RING_F4 ? BF16 : ST;                     // and of the value sums'
-  constexpr int QP = ST == RING_F4 && Q == F32 ? 3 : 1;             // planes of the queries
-  constexpr int PP = ST == F32 ? 1 : (Q == F32 ? 3 : 2);            // and of the weights
+  constexpr int XT = ST == RING_F4 ? BF16 : ST;                                   // type of the products
+  constexpr int QP = ST == RING_F4 ? (Q == F32 ? 3 : (Q == F16 ? 2 : 1)) : 1;     // planes of the queries
+  constexpr int PP = ST == F32 ? 1 : (Q == F32 ? 3 : 2);                          // and of the weights
   constexpr int ES = Q == F32 ? 4 : 2, CT = 2 * NBV, W = RingTile<NBK, NBV, ST>::W;
   constexpr int PITCH = 32 * NBV + 4;
   __shared__ float red[4 * 16 * PITCH], red_m[4 * 16], red_l[4 * 16];
@@ -300,7 +319,7 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
   id /= a.nsplit;
   const int chunk = id % a.chunks, sh = id / a.chunks;
   const int s = sh / a.kv, hk = sh - s * a.kv;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, li = lane & 15, lg = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
 
   const int n = a.counts[sh];
   const int held = n + a.append < a.slots ? n + a.append : a.slots;
@@ -319,12 +338,14 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
     const char* row = rows_at<ES>(a.q, s, hk * a.group + 16 * chunk + (in ? li : 0), 0);
 #pragma unroll
     for (int b = 0; b < NBK; ++b) {
+      constexpr int E = 16 / ES;
       float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int col = 32 * b + 8 * lg + j;
-        x[j] = in && col < a.d ? load_elem(row, col, Q) : 0.f;
-        if (a.scale < 0.f) x[j] = -x[j];
+      for (int i = 0; i < 8 / E; ++i) {
+        float y[E];
+        rows_unpack<Q>(rows_chunk<ES>(row, 32 * b + 8 * lg + E * i, in ? a.d : 0, a.q.aligned), y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[E * i + e] = a.scale < 0.f ? -y[e] : y[e];
       }
       ring_planes<XT, QP>(x, qf[b]);
     }
@@ -333,13 +354,13 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
   floatx4 acc[CT];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) acc[ct] = floatx4{0.f, 0.f, 0.f, 0.f};
-  float m = -3.4028235e38f, l = 0.f;
+  float m = -3.4028235e38f, limit = m, l = 0.f;
+  const float room = 8.f / a.c;
 
   const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
-  RingTile<NBK, NBV, ST> cur, next;
-  if (t0 + wave < t1) cur.load(a, tile0 + t0 + wave, lane);
-  for (int t = t0 + wave; t < t1; t += 4) {
-    if (t + 4 < t1) next.load(a, tile0 + t + 4, lane);
+  // a tile's part of the sums; PART: not all of its slots hold a token
+  auto take = [&](const RingTile<NBK, NBV, ST>& cur, int t, auto part) {
+    constexpr bool PART = decltype(part)::value;
     floatx4 x[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -347,13 +368,9 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
 #pragma unroll
       for (int b = 0; b < NBK; ++b) {
         if constexpr (ST == RING_F4) {
-          const RingFrag<XT> k = ring_values<XT>(cur.k[half][b]);
-          floatx4 y = floatx4{0.f, 0.f, 0.f, 0.f};
+          const RingFrag<XT> k = ring_key_values(cur.k[half][b], ring_power_of(cur.ke, half * ring_exps(NBK) + b));
 #pragma unroll
-          for (int p = QP - 1; p >= 0; --p) y = ring_mma<XT>(k, qf[b][p], y);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            x[half][r] = fmaf(y[r], ring_exp_of<ring_exps(NBK)>(cur.ke + half * ring_exps(NBK), r, b), x[half][r]);
+          for (int p = QP - 1; p >= 0; --p) x[half] = ring_mma<XT>(k, qf[b][p], x[half]);
         } else {
           RingFrag<XT> k;
 #pragma unroll
@@ -364,57 +381,64 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
     }
     // slots of this lane that hold a token
     const int left = held - 32 * t - 4 * lg;
-    const bool whole = held - 32 * t >= 32;
     float top = m;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (!whole && 16 * (i >> 2) + (i & 3) >= left) x[i >> 2][i & 3] = -__builtin_inff();
+      if (PART && 16 * (i >> 2) + (i & 3) >= left) x[i >> 2][i & 3] = -__builtin_inff();
       top = fmaxf(top, x[i >> 2][i & 3]);
     }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__any(top > m)) {
+    // the maximum moves, for all lanes of a query at once, when a weight would exceed 2^8
+    if (__any(top > limit)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
       const float shrink = __builtin_amdgcn_exp2f((m - top) * a.c);
       l *= shrink;
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) acc[ct] *= shrink;
       m = top;
+      limit = top + room;
     }
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       p[i] = __builtin_amdgcn_exp2f((x[i >> 2][i & 3] - m) * a.c);
-      if (!whole && 16 * (i >> 2) + (i & 3) >= left) p[i] = 0.f;
+      if (PART && 16 * (i >> 2) + (i & 3) >= left) p[i] = 0.f;
       l += p[i];
     }
+    RingFrag<XT> pf[PP];
+    ring_planes<XT, PP>(p, pf);
     if constexpr (ST == RING_F4) {
 #pragma unroll
       for (int b = 0; b < NBV; ++b) {
-        float y[8];
+        RingFrag<XT> v[2];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float e = ring_exp_of<ring_exps(NBV)>(cur.ve, i, b);
-          if (!whole && 16 * (i >> 2) + (i & 3) >= left) e = 0.f;
-          y[i] = p[i] * e;
+        for (int half = 0; half < 2; ++half) {
+          float power[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            power[i] = ring_power_of(cur.ve, 8 * b + 4 * half + i);
+            if (PART && 16 * half + i >= left) power[i] = 0.f;  // a slot without a token, whatever it holds
+          }
+          uint32_t first[2], second[2];
+          ring_value_words(cur.v[2 * b + half], power, first, second);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            v[0].w[2 * half + i] = first[i];
+            v[1].w[2 * half + i] = second[i];
+          }
         }
-        RingFrag<PT> pf[PP];
-        ring_planes<PT, PP>(y, pf);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const RingFrag<PT> v = ring_values<PT>(cur.v[2 * b + h]);
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int k = PP - 1; k >= 0; --k) acc[2 * b + h] = ring_mma<PT>(v, pf[k], acc[2 * b + h]);
-        }
+          for (int k = PP - 1; k >= 0; --k) acc[2 * b + h] = ring_mma<XT>(v[h], pf[k], acc[2 * b + h]);
       }
     } else {
-      RingFrag<PT> pf[PP];
-      ring_planes<PT, PP>(p, pf);
 #pragma unroll
       for (int ct = 0; ct < CT; ++ct) {
-        RingFrag<PT> v;
+        RingFrag<XT> v;
 #pragma unroll
         for (int i = 0; i < W; ++i) v.w[i] = cur.v[ct * W + i];
-        if (!whole) {  // slots without a token: whatever they hold
+        if constexpr (PART) {  // slots without a token: whatever they hold
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (16 * (i >> 2) + (i & 3) >= left) {
@@ -425,10 +449,29 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
             }
         }
 #pragma unroll
-        for (int k = PP - 1; k >= 0; --k) acc[ct] = ring_mma<PT>(v, pf[k], acc[ct]);
+        for (int k = PP - 1; k >= 0; --k) acc[ct] = ring_mma<XT>(v, pf[k], acc[ct]);
       }
     }
-    cur = next;
+  };
+  // whole tiles, one ahead in registers, the two buffers in turn; then the last tile if it is not whole
+  {
+    const int end = t1 < (held >> 5) ? t1 : held >> 5;
+    RingTile<NBK, NBV, ST> even, odd;
+    int t = t0 + wave;
+    if (t < end) even.load(a, tile0 + t, lane);
+    while (t < end) {
+      if (t + 4 < end) odd.load(a, tile0 + t + 4, lane);
+      take(even, t, std::false_type{});
+      t += 4;
+      if (t >= end) break;
+      if (t + 4 < end) even.load(a, tile0 + t + 4, lane);
+      take(odd, t, std::false_type{});
+      t += 4;
+    }
+    if (t < t1) {
+      even.load(a, tile0 + t, lane);
+      take(even, t, std::true_type{});
+    }
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
@@ -469,29 +512,52 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
   if (a.append && a.nsplit == 1 && a.chunks == 1 && threadIdx.x == 0) a.counts[sh] = n + 1;
 }
 
-// The splits' sums of a query head, and the count of a step that several workgroups share.
+// The splits' sums of a query head, 4 groups of 128 threads (a column each) over the splits, and the count of a step
+// that several workgroups share.  Bound by latency: 8 heads x 257 splits of 80 columns 6.4 us (113 us with one thread a
+// column over all splits, each load waiting for the one before), 128 splits 4.2 us.
+constexpr int RING_SPLITS = 1024;
 template <int Q>
-__global__ __launch_bounds__(128) void ring_join_kernel(const RingArgs a) {
+__global__ __launch_bounds__(512) void ring_join_kernel(const RingArgs a) {
+  __shared__ float weight[RING_SPLITS], red[4 * 128], wave_red[8];
   const int64_t head = blockIdx.x;
   const int s = blockIdx.x / a.heads, h = blockIdx.x - s * a.heads, sh = s * a.kv + h / a.group;
-  const int col = threadIdx.x;
-  if (a.nsplit > 1 && col < a.dv) {
-    const float* part = a.part + head * a.nsplit * (a.dv + 2);
-    float top = -3.4028235e38f, sum = 0.f, den = 0.f;
-    for (int i = 0; i < a.nsplit; ++i) top = fmaxf(top, part[i * (a.dv + 2) + a.dv]);
-    for (int i = 0; i < a.nsplit; ++i) {
-      const float* p = part + i * (a.dv + 2);
-      const float f = __builtin_amdgcn_exp2f((p[a.dv] - top) * a.c);
-      sum = fmaf(f, p[col], sum);
-      den = fmaf(f, p[a.dv + 1], den);
+  const int col = threadIdx.x & 127, group = threadIdx.x >> 7, wave = threadIdx.x >> 6;
+  if (a.nsplit > 1) {
+    const int pitch = a.dv + 2;
+    const float* part = a.part + head * a.nsplit * pitch;
+    float top = -3.4028235e38f, den = 0.f;
+    for (int i = threadIdx.x; i < a.nsplit; i += 512) {
+      weight[i] = part[i * pitch + a.dv];
+      top = fmaxf(top, weight[i]);
     }
-    const bool empty = !a.append && a.counts[sh] == 0;
-    store_elem(a.out, head * a.dv + col, Q, empty ? 0.f : sum / den);
-  }
-  if (a.append && h % a.group == 0) {
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) wave_red[wave] = top;
     __syncthreads();
-    if (col == 0) a.counts[sh] += 1;
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, wave_red[i]);
+    for (int i = threadIdx.x; i < a.nsplit; i += 512) {
+      const float f = __builtin_amdgcn_exp2f((weight[i] - top) * a.c);
+      weight[i] = f;
+      den = fmaf(f, part[i * pitch + a.dv + 1], den);
+    }
+    for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) wave_red[wave] = den;
+    float sum = 0.f;
+    if (col < a.dv) {
+#pragma unroll 8
+      for (int i = group; i < a.nsplit; i += 4) sum = fmaf(weight[i], part[i * pitch + col], sum);
+    }
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    if (threadIdx.x < a.dv) {
+      den = 0.f;
+      for (int i = 0; i < 8; ++i) den += wave_red[i];
+      sum = red[threadIdx.x] + red[128 + threadIdx.x] + red[256 + threadIdx.x] + red[384 + threadIdx.x];
+      const bool empty = !a.append && a.counts[sh] == 0;
+      store_elem(a.out, head * a.dv + threadIdx.x, Q, empty ? 0.f : sum / den);
+    }
   }
+  if (a.append && h % a.group == 0 && threadIdx.x == 0) a.counts[sh] += 1;
 }
 
 struct RingFill {
@@ -561,7 +627,7 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
       if (p >= 0) {
         *reinterpret_cast<uint32_t*>(to) = codes;
         if ((u & 3) == 0)
-          a.kexp[at * ring_exp_bytes(a.nbk, ST) + r * ring_exps(a.nbk) + (u >> 2)] = static_cast<uint8_t>(e);
+          a.kexp[at * ring_key_exp_bytes(a.nbk, ST) + ring_key_exp_at(r, u >> 2, a.nbk)] = static_cast<uint8_t>(e);
       }
     } else if (p >= 0) {
 #pragma unroll
@@ -601,31 +667,44 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) to[j] = ring_code(x[j], e);
       if (p >= 0 && (u & 3) == 0)
-        a.vexp[at * ring_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, u >> 2, a.nbv)] = static_cast<uint8_t>(e);
+        a.vexp[at * ring_value_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, u >> 2, a.nbv)] = static_cast<uint8_t>(e);
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 64 * 2 * a.nbv; i += 256) {
-    const int lane = i & 63, ct = i >> 6, g = lane >> 4, col = 16 * ct + (lane & 15);
-    if constexpr (ST == RING_F4) {
-      uint32_t* to = reinterpret_cast<uint32_t*>(values + (lane * 2 * a.nbv + ct) * 4);
-      uint32_t w = *to;
+  for (int i = threadIdx.x; i < 64 * (ST == RING_F4 ? a.nbv : 2 * a.nbv); i += 256) {
+    const int lane = i & 63, ct = i >> 6, g = lane >> 4;
+    const int col = ST == RING_F4 ? 32 * ct + (lane & 15) : 16 * ct + (lane & 15);
+    uint32_t w[8];
+    bool all = true;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = 16 * (j >> 2) + 4 * g + (j & 3);
-        if (token[r] >= 0) w = (w & ~(0xfu << (4 * j))) | (vals[r * pitch + col] << (4 * j));
+    for (int j = 0; j < 8; ++j) {
+      const int r = 16 * (j >> 2) + 4 * g + (j & 3);
+      w[j] = vals[r * pitch + col];
+      if constexpr (ST == RING_F4) w[j] |= vals[r * pitch + col + 16] << 4;
+      all = all && token[r] >= 0;
+    }
+    uint8_t* to = values + (ST == RING_F4 ? (lane * a.nbv + ct) * 8 : (ct * 64 + lane) * 8 * (ST == F32 ? 4 : 2));
+    if (all) {
+      if constexpr (ST == RING_F4) {
+        *reinterpret_cast<uint2*>(to) = uint2{w[0] | w[1] << 8 | w[2] << 16 | w[3] << 24,
+                                              w[4] | w[5] << 8 | w[6] << 16 | w[7] << 24};
+      } else if constexpr (ST == F32) {
+        reinterpret_cast<uint4*>(to)[0] = uint4{w[0], w[1], w[2], w[3]};
+        reinterpret_cast<uint4*>(to)[1] = uint4{w[4], w[5], w[6], w[7]};
+      } else {
+        *reinterpret_cast<uint4*>(to) = uint4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
       }
-      *to = w;
-    } else {
+      continue;
+    }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int r = 16 * (j >> 2) + 4 * g + (j & 3);
-        if (token[r] < 0) continue;
-        if constexpr (ST == F32)
-          reinterpret_cast<uint32_t*>(values)[(ct * 64 + lane) * 8 + j] = vals[r * pitch + col];
-        else
-          reinterpret_cast<uint16_t*>(values)[(ct * 64 + lane) * 8 + j] = static_cast<uint16_t>(vals[r * pitch + col]);
-      }
+    for (int j = 0; j < 8; ++j) {
+      if (token[16 * (j >> 2) + 4 * g + (j & 3)] < 0) continue;
+      if constexpr (ST == RING_F4)
+        to[j] = static_cast<uint8_t>(w[j]);
+      else if constexpr (ST == F32)
+        reinterpret_cast<uint32_t*>(to)[j] = w[j];
+      else
+        reinterpret_cast<uint16_t*>(to)[j] = static_cast<uint16_t>(w[j]);
     }
   }
 }
@@ -637,44 +716,76 @@ __global__ __launch_bounds__(256) static void ring_count_kernel(const RingFill f
 }
 
 // The slots' rows as they stand for: keys [streams][kv][slots][d], values [..][dv] in the element type, zero where no
-// token is; positions [streams][slots], -1 there.  A workgroup a tile.
+// token is; positions [streams][slots], -1 there.  A workgroup a tile: the tile's words in their order into LDS rows, then
+// whole rows out.
 template <int ST, int Q>
 __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void* keys, void* values, int* positions) {
+  constexpr int PITCH = 129;
+  __shared__ uint32_t rows[32 * PITCH];  // values: floats (4-bit), or the elements' bits
   const int sh = blockIdx.x / a.tiles, tile = blockIdx.x - sh * a.tiles, s = sh / a.kv, hk = sh - s * a.kv;
   const int n = a.counts[sh];
   const int64_t at = static_cast<int64_t>(sh) * a.tiles + tile;
   const uint8_t* kp = a.keys + at * ring_tile_bytes(a.nbk, ST);
   const uint8_t* vp = a.values + at * ring_tile_bytes(a.nbv, ST);
-  for (int i = threadIdx.x; i < 32 * (a.d + a.dv); i += 256) {
-    const int r = i / (a.d + a.dv), u = i - r * (a.d + a.dv), slot = 32 * tile + r;
-    if (slot >= a.slots) break;
-    const bool key = u < a.d;
-    const int col = key ? u : u - a.d;
-    float x = 0.f;
-    if (slot < n) {
-      const uint8_t* p = key ? kp + ring_key_at(r, col, a.nbk, ST) : vp + ring_value_at(r, col, a.nbv, ST);
+  const int live = min(32, a.slots - 32 * tile);  // slots of the tile
+  auto elem = [&](const uint8_t* p, int e) -> uint32_t {
+    if constexpr (ST == F32) return reinterpret_cast<const uint32_t*>(p)[e];
+    return reinterpret_cast<const uint16_t*>(p)[e];
+  };
+  auto store_rows = [&](void* out, int width) {
+    const int64_t base = (static_cast<int64_t>(sh) * a.slots + 32 * tile) * width;
+    for (int i = threadIdx.x; i < live * width; i += 256) {
+      const int r = i / width, col = i - r * width;
+      const uint32_t w = 32 * tile + r < n ? rows[r * PITCH + col] : 0u;
+      if constexpr (ST == RING_F4)
+        store_elem(out, base + i, Q, __uint_as_float(w));
+      else if constexpr (ST == F32)
+        static_cast<uint32_t*>(out)[base + i] = w;
+      else
+        static_cast<uint16_t*>(out)[base + i] = static_cast<uint16_t>(w);
+    }
+  };
+  for (int i = threadIdx.x; i < 128 * a.nbk; i += 256) {  // 8 dimensions of a slot a thread, in the cache's order
+    const int lane = i & 63, u = i >> 6, half = u / a.nbk, b = u - half * a.nbk;
+    const int r = 16 * half + (lane & 15), col = 32 * b + 8 * (lane >> 4);
+    if constexpr (ST == RING_F4) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(kp)[(half * 64 + lane) * a.nbk + b];
+      const float e = ring_power(a.kexp[at * ring_key_exp_bytes(a.nbk, ST) + ring_key_exp_at(r, b, a.nbk)]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        rows[r * PITCH + col + j] = __float_as_uint(ring_decode((w >> (4 * j)) & 15u) * e);
+    } else {
+      const uint8_t* p = kp + (u * 64 + lane) * 8 * (ST == F32 ? 4 : 2);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) rows[r * PITCH + col + j] = elem(p, j);
+    }
+  }
+  __syncthreads();
+  store_rows(keys, a.d);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 64 * (ST == RING_F4 ? a.nbv : 2 * a.nbv); i += 256) {  // 8 slots of a column a thread
+    const int lane = i & 63, ct = i >> 6, g = lane >> 4;
+    const int col = ST == RING_F4 ? 32 * ct + (lane & 15) : 16 * ct + (lane & 15);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int r = 16 * (j >> 2) + 4 * g + (j & 3);
       if constexpr (ST == RING_F4) {
-        const uint32_t code = *p >> (4 * ((key ? col : r) & 1));
-        const uint32_t e = key ? a.kexp[at * ring_exp_bytes(a.nbk, ST) + r * ring_exps(a.nbk) + (col >> 5)]
-                               : a.vexp[at * ring_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, col >> 5, a.nbv)];
-        x = ring_decode(code & 15u) * ring_power(e);
+        const uint32_t w = vp[(lane * a.nbv + ct) * 8 + j];
+        const float e = ring_power(a.vexp[at * ring_value_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, ct, a.nbv)]);
+        rows[r * PITCH + col] = __float_as_uint(ring_decode(w & 15u) * e);
+        rows[r * PITCH + col + 16] = __float_as_uint(ring_decode(w >> 4) * e);
       } else {
-        x = load_elem(p, 0, ST);
+        rows[r * PITCH + col] = elem(vp + (ct * 64 + lane) * 8 * (ST == F32 ? 4 : 2), j);
       }
     }
-    const int64_t row = static_cast<int64_t>(sh) * a.slots + slot;
-    if (key)
-      store_elem(keys, row * a.d + col, Q, x);
-    else
-      store_elem(values, row * a.dv + col, Q, x);
   }
-  if (hk == 0 && threadIdx.x < 32) {
+  __syncthreads();
+  store_rows(values, a.dv);
+  if (hk == 0 && static_cast<int>(threadIdx.x) < live) {
     const int slot = 32 * tile + threadIdx.x;
-    if (slot < a.slots) {
-      int p = -1;
-      if (slot < n) p = slot < a.sinks ? slot : slot + (n - 1 - slot) / a.window * a.window;
-      positions[static_cast<int64_t>(s) * a.slots + slot] = p;
-    }
+    int p = -1;
+    if (slot < n) p = slot < a.sinks ? slot : slot + (n - 1 - slot) / a.window * a.window;
+    positions[static_cast<int64_t>(s) * a.slots + slot] = p;
   }
 }
 

@@ -320,7 +320,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
   __shared__ uint4 ks[BK * CH], vs[BK * CH];
   int b, h, tile;
   win_place(a, b, h, tile);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int len = win_length(a, b), hk = h / a.group;
   const int r0 = tile * WIN_ROWS, w0 = r0 + 32 * wave, row = w0 + (lane & 31);
   const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
@@ -493,7 +493,7 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
   __shared__ uint4 ks[BK * CH], vs[BK * CH];
   int b, h, tile;
   win_place(a, b, h, tile);
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int len = win_length(a, b), hk = h / a.group;
   const int r0 = tile * WIN_ROWS, w0 = r0 + 32 * wave, row = w0 + (lane & 31);
   const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
@@ -656,7 +656,7 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
   const bool far = item < far_items;
   const int chunk = far ? item / a.sink_tiles : -1;
   const int tile = far ? item % a.sink_tiles : item - far_items;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, hh = lane >> 5;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int len = win_length(a, b);
   const int k0 = tile * WIN_ROWS, kw = k0 + 32 * wave, key = kw + (lane & 31);
 

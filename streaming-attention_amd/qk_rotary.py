@@ -9,14 +9,13 @@ Computed by hand-written HIP kernels on the inputs' ROCm device and its current 
 
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import Optional, Tuple, Union
 
 import torch
 
 import _native
-from sink_window_attention import _check_gpu, _refuse_capture
+from sink_window_attention import _check_gpu, _on, _refuse_capture, _strides
 
 Tensor = torch.Tensor
 
@@ -83,7 +82,7 @@ class _Call:
                 self.pos_strides = tuple(positions.stride())
         else:
             self.pos_strides = (0, 0)
-        _check_gpu(q=q, k=k, table=table, q_weight=q_weight, k_weight=k_weight, positions=positions)
+        _check_gpu(q, k, table, q_weight, k_weight, positions)
         self.table = table.contiguous()
         self.positions, self.eps, self.interleaved = positions, float(eps), bool(interleaved)
         self.weight_code = _native.DTYPE_CODES[weights[0].dtype if weights else q.dtype]
@@ -110,7 +109,7 @@ class _Call:
         yq = torch.empty((b, h, n, d), device=q.device, dtype=q.dtype)
         yk = torch.empty((b, hk, n, d), device=q.device, dtype=q.dtype)
         if b * n and h + hk:
-            with torch.cuda.device(q.device):
+            with _on(q.device):
                 st = _native.lib().sta_head_rotary(
                     q.data_ptr(), k.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, hk, n, d, _strides(q, k),
                     *self.tail(qw, kw), yq.data_ptr(), yk.data_ptr(), _native.stream_handle(q.device))
@@ -130,7 +129,7 @@ class _Call:
             lib = _native.lib()
             nbytes = lib.sta_head_rotary_backward_bytes(b, h, hk, n, d)
             ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-            with torch.cuda.device(q.device):
+            with _on(q.device):
                 st = lib.sta_head_rotary_backward(
                     gq.data_ptr(), gk.data_ptr(), q.data_ptr(), k.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, hk,
                     n, d, _strides(q, k, gq, gk), *self.tail(qw, kw), dq.data_ptr(), dk.data_ptr(),
@@ -143,27 +142,20 @@ def _walkable(x: Tensor) -> Tensor:
     return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
 
 
-def _strides(*tensors: Tensor):
-    flat = [s for x in tensors for s in x.stride()[:3]]
-    return (ctypes.c_int64 * len(flat))(*flat)
-
-
 class _NormRotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, table, positions, eps, interleaved, call):
+    def forward(ctx, q, k, q_weight, k_weight, table, positions, call):
         _refuse_capture()
         ctx.save_for_backward(q, k, q_weight, k_weight, table, positions)
-        ctx.settings = eps, interleaved
+        ctx.call = call
         return call.forward(q, k, q_weight, k_weight)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         _refuse_capture()
-        q, k, q_weight, k_weight, table, positions = ctx.saved_tensors
-        eps, interleaved = ctx.settings
-        call = _Call(q, k, table, q_weight, k_weight, positions, eps, interleaved)
-        return (*call.backward(gq, gk, q, k, q_weight, k_weight), None, None, None, None, None)
+        q, k, q_weight, k_weight, _, _ = ctx.saved_tensors  # table and positions: checked to be as they were
+        return (*ctx.call.backward(gq, gk, q, k, q_weight, k_weight), None, None, None)
 
 
 def qk_norm_rotary(q: Tensor, k: Tensor, table: Tensor, *, q_weight: Optional[Tensor] = None,
@@ -180,9 +172,8 @@ def qk_norm_rotary(q: Tensor, k: Tensor, table: Tensor, *, q_weight: Optional[Te
     graph (RuntimeError); qk_norm_rotary_backward can."""
     call = _Call(q, k, table, q_weight, k_weight, positions, eps, interleaved)
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
-        return _NormRotary.apply(q, k, q_weight, k_weight, table, positions, eps, interleaved, call)
-    with torch.no_grad():
-        return call.forward(q, k, q_weight, k_weight)
+        return _NormRotary.apply(q, k, q_weight, k_weight, table, positions, call)
+    return call.forward(q, k, q_weight, k_weight)
 
 
 @torch.no_grad()
@@ -197,5 +188,5 @@ def qk_norm_rotary_backward(q_grad: Tensor, k_grad: Tensor, q: Tensor, k: Tensor
     if q_grad.dtype != q.dtype or k_grad.dtype != q.dtype:
         raise ValueError("gradients must have q's dtype")
     call = _Call(q, k, table, q_weight, k_weight, positions, eps, interleaved)
-    _check_gpu(q=q, q_grad=q_grad, k_grad=k_grad)
+    _check_gpu(q, q_grad, k_grad)
     return call.backward(q_grad, k_grad, q, k, q_weight, k_weight)

@@ -14,6 +14,7 @@ ROCm device and its current stream; there is no CPU path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from typing import Optional, Sequence, Tuple, Union
@@ -49,16 +50,13 @@ def _check_tokens(window: int, sinks: int) -> Tuple[int, int]:
     return min(window, MAX_ROWS), min(sinks, MAX_ROWS)
 
 
-def _check_gpu(**tensors: Optional[Tensor]) -> None:
-    dev = None
-    for name, x in tensors.items():
-        if x is None:
-            continue
-        if not x.is_cuda:
-            raise ValueError(f"HIP kernels require GPU (cuda/ROCm) tensors: {name} is on {x.device}")
-        if dev is not None and x.device != dev:
-            raise ValueError("all tensors must be on one device")
-        dev = x.device
+def _check_gpu(*tensors: Optional[Tensor]) -> None:
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"HIP kernels require GPU (cuda/ROCm) tensors, got one on {dev}")
+    for x in tensors:
+        if x is not None and x.device != dev:
+            raise ValueError(f"all tensors must be on one device, got {x.device} and {dev}")
 
 
 def _check_dtype(*tensors: Tensor) -> None:
@@ -108,9 +106,21 @@ def _dense(x: Tensor) -> Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+_STRIDES = {n: ctypes.c_int64 * n for n in (6, 9, 12)}
+
+
 def _strides(*tensors: Tensor):
+    """The element strides of batch, head and row of every tensor, for the C ABI."""
     flat = [s for x in tensors for s in x.stride()[:3]]
-    return (ctypes.c_int64 * len(flat))(*flat)
+    return _STRIDES[len(flat)](*flat)
+
+
+_here = contextlib.nullcontext()
+
+
+def _on(device: torch.device):
+    """The device as the current one (nothing to do where it is: 5 us of a small call's host time)."""
+    return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: float, lengths: Optional[Tensor],
@@ -122,7 +132,7 @@ def _forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: fl
     if out.numel() == 0:
         return out, lse
     q, k, v = _rows(q), _rows(k), _rows(v)
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         st = _native.lib().sta_window_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, k.shape[1], n, d, dv,
             _strides(q, k, v), scale, window, sinks, _native.ptr(lengths), out.data_ptr(), _native.ptr(lse),
@@ -142,7 +152,7 @@ def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: T
         return dq, dk.zero_(), dvo.zero_()
     grad, q, k, v, out, lse = _rows(grad), _rows(q), _rows(k), _rows(v), _dense(out), lse.contiguous()
     lib = _native.lib()
-    with torch.cuda.device(q.device):
+    with _on(q.device):
         nbytes = lib.sta_window_backward_bytes(b, h, hk, n, d, dv, window, sinks)
         if nbytes < 0:
             raise _native.NativeError("sta_window_backward_bytes refused the shape")
@@ -187,7 +197,7 @@ def _checked(q, k, v, window, sinks, scale, lengths):
     q4, k4, v4 = _heads_first(q, k, v)
     _check_dtype(q4, k4, v4)
     lengths = _check_lengths(lengths, q4.shape[0])
-    _check_gpu(q=q4, k=k4, v=v4, lengths=lengths)
+    _check_gpu(q4, k4, v4, lengths)
     return q4, k4, v4, window, sinks, _attention_scale(scale, q4.shape[3]), lengths
 
 
@@ -236,7 +246,7 @@ def sink_window_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Ten
     _check_dtype(q4, grad, out)
     if lse.dtype != torch.float32:
         raise ValueError("lse must be float32")
-    _check_gpu(q=q4, grad=grad, out=out, lse=lse)
+    _check_gpu(q4, grad, out, lse)
     dq, dk, dv = _backward(grad, q4, k4, v4, out, lse, window, sinks, s, lengths)
     return (dq[0, 0], dk[0, 0], dv[0, 0]) if q.ndim == 2 else (dq, dk, dv)
 
@@ -288,6 +298,7 @@ class SinkWindowStreamingAttention:
                                                     self.window, self.sinks, sizes), "sta_ring_layout")
         self._cache = [torch.zeros(n, device=self.device, dtype=torch.uint8) if n else None for n in sizes]
         self._counts = torch.zeros((streams, kv_heads), device=self.device, dtype=torch.int32)
+        self._state = (*(_native.ptr(x) for x in self._cache), self._counts.data_ptr())
         self._bytes = _native.lib().sta_ring_attention_bytes(streams, heads, kv_heads, dim, value_dim, self.window,
                                                              self.sinks)
         self._fresh = True
@@ -308,18 +319,16 @@ class SinkWindowStreamingAttention:
         out = torch.empty((self.streams, self.heads, self.value_dim), device=self.device, dtype=self.dtype)
         ws = torch.empty(self._bytes, device=self.device, dtype=torch.uint8) if self._bytes else None
         none = (0, 0)
-        strides = (ctypes.c_int64 * 6)(*q.stride()[:2], *(none if k is None else k.stride()[:2]),
-                                       *(none if v is None else v.stride()[:2]))
-        with torch.cuda.device(self.device):
+        strides = _STRIDES[6](*q.stride()[:2], *(none if k is None else k.stride()[:2]),
+                              *(none if v is None else v.stride()[:2]))
+        with _on(self.device):
             st = _native.lib().sta_ring_attention(
                 q.data_ptr(), _native.ptr(k), _native.ptr(v), self._code, self._store, self.streams, self.heads,
                 self.kv_heads, self.dim, self.value_dim, strides, self.scale, self.window, self.sinks,
-                *(_native.ptr(x) for x in self._cache), self._counts.data_ptr(), out.data_ptr(), _native.ptr(ws),
-                self._bytes, _native.stream_handle(self.device))
+                *self._state, out.data_ptr(), _native.ptr(ws), self._bytes, _native.stream_handle(self.device))
         _native.check(st, "sta_ring_attention")
         return out
 
-    @torch.no_grad()
     def step(self, query: Tensor, key: Tensor, value: Tensor) -> Tensor:
         """One token of every stream into the cache, then one query a head: update(key, value); query(query)."""
         q = self._rows(query, (self.streams, self.heads, self.dim), "query")
@@ -328,7 +337,6 @@ class SinkWindowStreamingAttention:
         self._fresh = False
         return self._attend(q, k, v)
 
-    @torch.no_grad()
     def query(self, query: Tensor) -> Tensor:
         """Attention of one query a head over the tokens held; zero for a stream that holds none."""
         return self._attend(self._rows(query, (self.streams, self.heads, self.dim), "query"), None, None)
@@ -344,11 +352,11 @@ class SinkWindowStreamingAttention:
         self._fresh = False
         if k.shape[2] == 0:
             return
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             st = _native.lib().sta_ring_extend(
                 k.data_ptr(), v.data_ptr(), self._code, self._store, self.streams, self.kv_heads, k.shape[2], self.dim,
                 self.value_dim, _strides(k, v), self.window, self.sinks, _native.ptr(counts),
-                *(_native.ptr(x) for x in self._cache), self._counts.data_ptr(), _native.stream_handle(self.device))
+                *self._state, _native.stream_handle(self.device))
         _native.check(st, "sta_ring_extend")
 
     def _prompt(self, keys: Tensor, values: Tensor, counts: Optional[Tensor]):
@@ -403,11 +411,11 @@ class SinkWindowStreamingAttention:
         keys = torch.empty((self.streams, self.kv_heads, slots, self.dim), device=self.device, dtype=self.dtype)
         values = torch.empty((self.streams, self.kv_heads, slots, self.value_dim), device=self.device, dtype=self.dtype)
         positions = torch.empty((self.streams, slots), device=self.device, dtype=torch.int32)
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             st = _native.lib().sta_ring_items(
                 self._code, self._store, self.streams, self.kv_heads, self.dim, self.value_dim, self.window, self.sinks,
-                *(_native.ptr(x) for x in self._cache), self._counts.data_ptr(), keys.data_ptr(), values.data_ptr(),
-                positions.data_ptr(), _native.stream_handle(self.device))
+                *self._state, keys.data_ptr(), values.data_ptr(), positions.data_ptr(),
+                _native.stream_handle(self.device))
         _native.check(st, "sta_ring_items")
         return keys, values, positions
 

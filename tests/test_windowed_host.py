@@ -53,8 +53,7 @@ def test_scales_must_be_finite():
 def test_differentiable_calls_refuse_capture(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     for f, args in ((swa._SinkWindow, (x(1, 1, 4, 8).requires_grad_(), x(1, 1, 4, 8), x(1, 1, 4, 8), 2, 0, 1.0, None)),
-                    (qkr._NormRotary, (x(1, 1, 4, 8).requires_grad_(), x(1, 1, 4, 8), None, None, x(4, 8), None, 1e-6,
-                                       False, None))):
+                    (qkr._NormRotary, (x(1, 1, 4, 8).requires_grad_(), x(1, 1, 4, 8), None, None, x(4, 8), None, None))):
         with pytest.raises(RuntimeError, match="captured"):
             f.apply(*args)
 
