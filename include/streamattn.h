@@ -460,7 +460,8 @@ int sta_pair_moments(const void* q, const void* k, const void* v, int dtype, int
  * (NULL: n) sees the keys j <= i with i - j < window or j < sinks.
  *   q [batch][heads][n][d], k [batch][kv_heads][n][d], v [batch][kv_heads][n][dv], heads a multiple of kv_heads (query
  *   head h reads key head h / (heads / kv_heads)); the last dimension is contiguous, strides [3][3] (host memory) gives
- *   the element strides of batch, head and row of q, k and v (any values, 0 included).  d, dv <= 128; n <= 2^30.
+ *   the element strides of batch, head and row of q, k and v (0 included; rows up to 2^24 bytes apart; no alignment
+ *   beyond the element's).  d, dv at most 128 and rows of at least 16 bytes; n <= 2^30.
  *   out [batch][heads][n][dv] dense, 16-byte aligned, in dtype; rows at or behind a length are zero.
  *   lse [batch][heads][n] fp32 (or NULL): log2 of every row's sum of weights, for the backward call.
  *   window >= 1, sinks >= 0 (either may exceed n); scale any finite number.  Products of 16-bit inputs are exact, fp32
@@ -472,8 +473,8 @@ int sta_window_attention(const void* q, const void* k, const void* v, int dtype,
                          int64_t sinks, const int32_t* lengths, void* out, float* lse, void* stream);
 
 /* Bytes of sta_window_attention_backward's workspace; -1 for arguments it refuses. */
-int64_t sta_window_backward_bytes(int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv, int64_t window,
-                                  int64_t sinks);
+int64_t sta_window_backward_bytes(int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv,
+                                  int64_t window, int64_t sinks);
 
 /*
  * Gradients of sta_window_attention: dq [batch][heads][n][d], dk [batch][kv_heads][n][d], dv [batch][kv_heads][n][dv],

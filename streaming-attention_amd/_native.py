@@ -167,7 +167,7 @@ _SIGNATURES = {
         _i32, [_c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _c_p, _f32, _i64, _i64, _c_p, _c_p, _c_p,
                _c_p],  # q k v dtype batch heads kv_heads n d dv strides scale window sinks lengths out lse stream
     ),
-    "sta_window_backward_bytes": (_i64, [_i64, _i32, _i32, _i64, _i32, _i32, _i64, _i64]),
+    "sta_window_backward_bytes": (_i64, [_i32, _i64, _i32, _i32, _i64, _i32, _i32, _i64, _i64]),
     "sta_window_attention_backward": (
         _i32, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _c_p, _f32, _i64, _i64,
                _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # grad q k v out lse dtype .. lengths dq dk dv ws bytes stream

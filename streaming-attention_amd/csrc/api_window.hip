@@ -23,24 +23,26 @@ int element_size(int dtype) { return dtype == STA_F32 ? 4 : 2; }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-sta::Rows rows_of(const void* p, const int64_t* strides, int dtype) {
-  sta::Rows r;
-  r.p = p;
-  r.sb = strides[0];
-  r.sh = strides[1];
-  r.sn = strides[2];
-  const int64_t es = element_size(dtype);
-  r.aligned = aligned16(p) && r.sb * es % 16 == 0 && r.sh * es % 16 == 0 && r.sn * es % 16 == 0;
-  return r;
+sta::Rows rows_of(const void* p, const int64_t* strides) { return sta::Rows{p, strides[0], strides[1], strides[2], 0}; }
+
+// a tile's rows are reached by 32-bit offsets from its first
+bool strides_ok(const int64_t* strides, int tensors, int dtype) {
+  for (int i = 0; i < tensors; ++i) {
+    const int64_t sn = strides[3 * i + 2];
+    if (sn < 0 || sn > (int64_t(1) << 24) / element_size(dtype)) return false;
+  }
+  return true;
 }
 
 // The shape part of the arguments; STA_OK or what is wrong with it.
-int window_shape(sta::WinArgs& a, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv, float scale,
-                 int64_t window, int64_t sinks) {
+int window_shape(sta::WinArgs& a, int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv,
+                 float scale, int64_t window, int64_t sinks) {
+  if (!dtype_ok(dtype)) return STA_ERR_DTYPE;
+  const int es = element_size(dtype);
   if (batch < 1 || heads < 1 || kv_heads < 1 || n < 1 || d < 1 || dv < 1 || heads % kv_heads != 0)
     return STA_ERR_SHAPE;
   if (window < 1 || sinks < 0 || !std::isfinite(scale)) return STA_ERR_ARG;
-  if (d > kMaxWindowD || dv > kMaxWindowD || n > kMaxWindowRows || batch > 0x7fffffff) return STA_ERR_UNSUPPORTED;
+  if (d > kMaxWindowD || dv > kMaxWindowD || d * es < 16 || dv * es < 16 || n > kMaxWindowRows || batch > 0x7fffffff) return STA_ERR_UNSUPPORTED;
   a = sta::WinArgs{};
   a.batch = static_cast<int>(batch);
   a.heads = heads;
@@ -51,7 +53,8 @@ int window_shape(sta::WinArgs& a, int64_t batch, int heads, int kv_heads, int64_
   a.window = static_cast<int>(window < n ? window : n);
   a.sinks = static_cast<int>(sinks < n ? sinks : n);
   a.scale = scale;
-  a.c = std::fabs(scale) * 1.44269504088896340736f;
+  // above 0: a hidden pair's logit, -inf, stays one times c
+  a.c = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-37f);
   a.tiles = static_cast<int>((n + sta::WIN_ROWS - 1) / sta::WIN_ROWS);
   a.lift = a.drop = 1.f;
   return STA_OK;
@@ -108,22 +111,22 @@ int sta_window_attention(const void* q, const void* k, const void* v, int dtype,
                          int kv_heads, int64_t n, int d, int dv, const int64_t* strides, float scale, int64_t window,
                          int64_t sinks, const int32_t* lengths, void* out, float* lse, void* stream) {
   if (!q || !k || !v || !out || !strides || !aligned16(out)) return STA_ERR_ARG;
-  if (!dtype_ok(dtype)) return STA_ERR_DTYPE;
   sta::WinArgs a;
-  if (const int st = window_shape(a, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
-  a.q = rows_of(q, strides, dtype);
-  a.k = rows_of(k, strides + 3, dtype);
-  a.v = rows_of(v, strides + 6, dtype);
+  if (const int st = window_shape(a, dtype, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
+  if (!strides_ok(strides, 3, dtype)) return STA_ERR_UNSUPPORTED;
+  a.q = rows_of(q, strides);
+  a.k = rows_of(k, strides + 3);
+  a.v = rows_of(v, strides + 6);
   a.lengths = lengths;
   a.out = out;
   a.lse = lse;
   return dispatch(false, a, dtype, stream);
 }
 
-int64_t sta_window_backward_bytes(int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv, int64_t window,
-                                  int64_t sinks) {
+int64_t sta_window_backward_bytes(int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv,
+                                  int64_t window, int64_t sinks) {
   sta::WinArgs a;
-  if (window_shape(a, batch, heads, kv_heads, n, d, dv, 1.f, window, sinks) != STA_OK) return -1;
+  if (window_shape(a, dtype, batch, heads, kv_heads, n, d, dv, 1.f, window, sinks) != STA_OK) return -1;
   plan_sinks(a);
   return 4 * (delta_floats(a) + part_floats(a));
 }
@@ -136,15 +139,15 @@ int sta_window_attention_backward(const void* grad, const void* q, const void* k
   if (!grad || !q || !k || !v || !out || !lse || !strides || !dq || !dk || !dv_out || !workspace) return STA_ERR_ARG;
   if (!aligned16(out) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv_out) || !aligned16(workspace))
     return STA_ERR_ARG;
-  if (!dtype_ok(dtype)) return STA_ERR_DTYPE;
   sta::WinArgs a;
-  if (const int st = window_shape(a, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
+  if (const int st = window_shape(a, dtype, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
   plan_sinks(a);
   if (workspace_bytes < 4 * (delta_floats(a) + part_floats(a))) return STA_ERR_SCRATCH;
-  a.q = rows_of(q, strides, dtype);
-  a.k = rows_of(k, strides + 3, dtype);
-  a.v = rows_of(v, strides + 6, dtype);
-  a.go = rows_of(grad, strides + 9, dtype);
+  if (!strides_ok(strides, 4, dtype)) return STA_ERR_UNSUPPORTED;
+  a.q = rows_of(q, strides);
+  a.k = rows_of(k, strides + 3);
+  a.v = rows_of(v, strides + 6);
+  a.go = rows_of(grad, strides + 9);
   a.lengths = lengths;
   a.out = const_cast<void*>(out);
   a.lse = const_cast<float*>(lse);

@@ -228,7 +228,7 @@ __device__ void ring_put(const RingArgs& a, int s, int hk, int slot) {
     } else {
 #pragma unroll
       for (int i = 0; i < ES / 2; ++i)
-        reinterpret_cast<uint4*>(at)[i] = rows_chunk<ES>(row, col + (16 / ES) * i, a.d, a.k.aligned);
+        reinterpret_cast<uint4*>(at)[i] = rows_chunk<ES>(row, col + (16 / ES) * i, a.d);
     }
   } else if (t >= 64 && t < 64 + (ST == RING_F4 ? 16 : 32) * a.nbv) {
     const char* row = rows_at<ES>(a.v, s, hk, 0);
@@ -343,9 +343,9 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
 #pragma unroll
       for (int i = 0; i < 8 / E; ++i) {
         float y[E];
-        rows_unpack<Q>(rows_chunk<ES>(row, 32 * b + 8 * lg + E * i, in ? a.d : 0, a.q.aligned), y);
+        rows_unpack<Q>(rows_chunk<ES>(row, 32 * b + 8 * lg + E * i, a.d), y);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[E * i + e] = a.scale < 0.f ? -y[e] : y[e];
+        for (int e = 0; e < E; ++e) x[E * i + e] = in ? (a.scale < 0.f ? -y[e] : y[e]) : 0.f;
       }
       ring_planes<XT, QP>(x, qf[b]);
     }
@@ -612,7 +612,7 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
 #pragma unroll
       for (int c = 0; c < 8 / E; ++c) {
         float y[E];
-        rows_unpack<Q>(p < 0 ? uint4{0u, 0u, 0u, 0u} : rows_chunk<ES>(row, col + E * c, a.d, a.k.aligned), y);
+        rows_unpack<Q>(p < 0 ? uint4{0u, 0u, 0u, 0u} : rows_chunk<ES>(row, col + E * c, a.d), y);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           x[E * c + e] = y[e];
@@ -632,7 +632,7 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
     } else if (p >= 0) {
 #pragma unroll
       for (int c = 0; c < ES / 2; ++c)
-        reinterpret_cast<uint4*>(to)[c] = rows_chunk<ES>(row, col + (16 / ES) * c, a.d, a.k.aligned);
+        reinterpret_cast<uint4*>(to)[c] = rows_chunk<ES>(row, col + (16 / ES) * c, a.d);
     }
   }
   // values: the rows (codes) of the tile's slots, then 8 slots of a column a thread
@@ -645,7 +645,7 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
     uint32_t top = 0u;
 #pragma unroll
     for (int c = 0; c < 8 / E; ++c) {
-      const uint4 w = p < 0 ? uint4{0u, 0u, 0u, 0u} : rows_chunk<ES>(row, col + E * c, a.dv, a.v.aligned);
+      const uint4 w = p < 0 ? uint4{0u, 0u, 0u, 0u} : rows_chunk<ES>(row, col + E * c, a.dv);
       if constexpr (ST == RING_F4) {
         float y[E];
         rows_unpack<Q>(w, y);

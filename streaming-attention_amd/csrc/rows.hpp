@@ -16,20 +16,50 @@ __device__ __forceinline__ const char* rows_at(const Rows& t, int64_t b, int64_t
   return static_cast<const char*>(t.p) + (b * t.sb + h * t.sh + row * t.sn) * ES;
 }
 
-// 16 bytes at column `col` of a row, columns at or behind `width` zero
+// 16 bytes at any element's address (gfx950 reads them in one load whatever the alignment)
+__device__ __forceinline__ uint4 rows_load16(const char* p) {
+  uint4 u;
+  __builtin_memcpy(&u, p, 16);
+  return u;
+}
+
+// u moved down by `bytes` (0 .. 15), zeros coming in above
+__device__ __forceinline__ uint4 rows_shift(const uint4& u, int bytes) {
+  uint64_t lo = u.x | static_cast<uint64_t>(u.y) << 32, hi = u.z | static_cast<uint64_t>(u.w) << 32;
+  if (bytes & 8) {
+    lo = hi;
+    hi = 0;
+  }
+  const int s = 8 * (bytes & 7);
+  lo = s ? (lo >> s) | (hi << (64 - s)) : lo;
+  hi >>= s;
+  return uint4{static_cast<uint32_t>(lo), static_cast<uint32_t>(lo >> 32), static_cast<uint32_t>(hi),
+               static_cast<uint32_t>(hi >> 32)};
+}
+
+// 16 bytes at column `col` of a row of at least 16 bytes, columns at or behind `width` zero: where the unit reaches over
+// the row's end, the row's last 16 bytes, moved into place
 template <int ES>
-__device__ __forceinline__ uint4 rows_chunk(const void* row, int col, int width, int aligned) {
+__device__ __forceinline__ uint4 rows_unit(const char* row, int col, int width) {
   constexpr int E = 16 / ES;
-  const char* p = static_cast<const char*>(row) + static_cast<int64_t>(col) * ES;
-  if (aligned && col + E <= width) return *reinterpret_cast<const uint4*>(p);
+  uint4 u = rows_load16(row + min(col, width - E) * ES);
+  if (width % E) u = rows_shift(u, max(0, col + E - width) * ES & 15);
+  return col < width ? u : uint4{0u, 0u, 0u, 0u};
+}
+
+// the same of a row of any width
+template <int ES>
+__device__ __forceinline__ uint4 rows_chunk(const char* row, int col, int width) {
+  constexpr int E = 16 / ES;
+  if (width >= E) return rows_unit<ES>(row, col, width);
   uint32_t u[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int e = 0; e < E; ++e)
     if (col + e < width) {
       if constexpr (ES == 4)
-        u[e] = reinterpret_cast<const uint32_t*>(p)[e];
+        u[e] = reinterpret_cast<const uint32_t*>(row)[col + e];
       else
-        u[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(p)[e]) << (16 * (e & 1));
+        u[e / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(row)[col + e]) << (16 * (e & 1));
     }
   return uint4{u[0], u[1], u[2], u[3]};
 }

@@ -110,27 +110,57 @@ __device__ __forceinline__ WinFrag<IN> win_operand(const floatx16& x, int t) {
   return f;
 }
 
-// Staging of ROWS rows of a tile by 256 threads: registers first (load), LDS when the tile before is done with (put)
+// Staging of ROWS rows of a tile by 256 threads: registers first (load), LDS when the tile before is done with (put).
+// The loads are free of branches, so that they stay in flight while a tile computes: rows behind the last are read as the
+// last one and a row's last 16 bytes in the place of a unit that would reach over its end; put zeroes the ones and
+// moves the others into place.
 template <int P, int IN, int ROWS>
 struct WinStage {
   static constexpr int ES = IN == F32 ? 4 : 2, E = 16 / ES, CH = win_chunks<ES>(P);
   static constexpr int COUNT = (ROWS * CH + 255) / 256;
   uint4 u[COUNT];
-  // rows [row0, row0 + ROWS) of head (b, h); rows at or behind `limit` and columns behind `width` are zero
-  __device__ __forceinline__ void load(const Rows& t, int64_t b, int64_t h, int row0, int limit, int width) {
+  uint32_t at[COUNT];  // bytes from the tile's first row (the host keeps 64 rows below 2^31 bytes)
+  int pitch, width;
+
+  __device__ __forceinline__ void init(const Rows& t, int w) {
+    pitch = static_cast<int>(t.sn) * ES;
+    width = w;
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
-      const int at = threadIdx.x + 256 * i, r = at / CH, c = at % CH;
-      u[i] = uint4{0u, 0u, 0u, 0u};
-      if ((ROWS * CH % 256 == 0 || at < ROWS * CH) && row0 + r < limit && c * E < width)
-        u[i] = rows_chunk<ES>(rows_at<ES>(t, b, h, row0 + r), c * E, width, t.aligned);
+      const int x = threadIdx.x + 256 * i;
+      at[i] = min(x / CH, ROWS - 1) * pitch + min(x % CH * E, width - E) * ES;
     }
   }
-  __device__ __forceinline__ void put(uint4* lds) const {
+  // the tile at `row`, `left` >= 1 of its rows being there; a row has at least 16 bytes
+  __device__ __forceinline__ void load(const char* row, int left) {
+    if (left >= ROWS) {
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-      const int at = threadIdx.x + 256 * i, r = at / CH, c = at % CH;
-      if (ROWS * CH % 256 == 0 || at < ROWS * CH) lds[r * CH + (c ^ win_swizzle<CH>(r))] = u[i];
+      for (int i = 0; i < COUNT; ++i) u[i] = rows_load16(row + at[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) {
+        const int r = min((threadIdx.x + 256 * i) / CH, ROWS - 1);
+        u[i] = rows_load16(row + (at[i] - static_cast<uint32_t>(max(0, r - left + 1) * pitch)));
+      }
+    }
+  }
+  __device__ __forceinline__ void put(uint4* lds, int left) const {
+    auto to = [&](int i, const uint4& x) {
+      const int k = threadIdx.x + 256 * i, r = k / CH, c = k % CH;
+      if (ROWS * CH % 256 == 0 || k < ROWS * CH) lds[r * CH + (c ^ win_swizzle<CH>(r))] = x;
+    };
+    if (left >= ROWS && width == P) {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) to(i, u[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i) {
+        const int k = threadIdx.x + 256 * i, r = k / CH, c = k % CH;
+        uint4 x = u[i];
+        if (width % E) x = rows_shift(x, max(0, c * E + E - width) * ES & 15);
+        const bool in = r < left && c * E < width;
+        to(i, uint4{in ? x.x : 0u, in ? x.y : 0u, in ? x.z : 0u, in ? x.w : 0u});
+      }
     }
   }
 };
@@ -186,20 +216,25 @@ __device__ __forceinline__ WinFrag<IN> win_read_columns(const uint4* lds, int r0
   return f;
 }
 
-// 8 dimensions at column 16 s + 8 h of a row in memory, with the sign of the scale in `flip`
+// 8 dimensions at column 16 s + 8 h of a row in memory (none of a row of width 0), with the sign of the scale in `flip`
 template <int IN>
-__device__ __forceinline__ WinFrag<IN> win_load_row(const void* row, int s, int h, int width, int aligned,
-                                                    uint32_t flip) {
+__device__ __forceinline__ WinFrag<IN> win_load_row(const char* row, int s, int h, int width, uint32_t flip) {
   constexpr int ES = IN == F32 ? 4 : 2;
   WinFrag<IN> f;
 #pragma unroll
   for (int i = 0; i < (IN == F32 ? 2 : 1); ++i) {
-    const int col = 16 * s + 8 * h + 4 * i;
-    uint4 u = uint4{0u, 0u, 0u, 0u};
-    if (col < width) u = rows_chunk<ES>(row, col, width, aligned);
+    const uint4 u = rows_unit<ES>(row, 16 * s + 8 * h + 4 * i, width);
     f.w[i] = uint4{u.x ^ flip, u.y ^ flip, u.z ^ flip, u.w ^ flip};
   }
   return f;
+}
+
+// Keeps the operands of a lane whose row is one; others are zero.
+template <int IN>
+__device__ __forceinline__ void win_keep(WinFrag<IN>& f, bool row) {
+#pragma unroll
+  for (int i = 0; i < (IN == F32 ? 2 : 1); ++i)
+    f.w[i] = uint4{row ? f.w[i].x : 0u, row ? f.w[i].y : 0u, row ? f.w[i].z : 0u, row ? f.w[i].w : 0u};
 }
 
 __device__ __forceinline__ bool win_finite(float x) { return fabsf(x) < __builtin_inff(); }
@@ -330,14 +365,18 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
-  float m = -1e30f, l = 0.f;  // finite: exp2(m_old - m_new) is 0 or at most 1, never a NaN
+  float m = -1e30f, limit = m, l = 0.f;  // finite: exp2(m_old - m_new) is 0 or at most 1, never a NaN
+  const float room = 8.f / a.c;
 
   if (r0 < len) {
     WinFrag<IN> qf[P / 16];
     const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
     const char* qrow = rows_at<ES>(a.q, b, h, row < len ? row : 0);
 #pragma unroll
-    for (int s = 0; s < P / 16; ++s) qf[s] = win_load_row<IN>(qrow, s, hh, row < len ? a.d : 0, a.q.aligned, flip);
+    for (int s = 0; s < P / 16; ++s) {
+      qf[s] = win_load_row<IN>(qrow, s, hh, a.d, flip);
+      win_keep<IN>(qf[s], row < len);
+    }
 
     const int last = (r0 + WIN_ROWS < len ? r0 + WIN_ROWS : len) - 1;
     const int t_lo = (r0 - a.window + 1 > 0 ? r0 - a.window + 1 : 0) / BK;
@@ -346,49 +385,57 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
     const int count = n_sink + last / BK - t_lo + 1;
     WinStage<P, IN, BK> kst, vst;
     auto first_key = [&](int it) { return (it < n_sink ? it : t_lo + it - n_sink) * BK; };
-    kst.load(a.k, b, hk, first_key(0), len, a.d);
-    vst.load(a.v, b, hk, first_key(0), len, a.dv);
+    kst.init(a.k, a.d);
+    vst.init(a.v, a.dv);
+    auto load = [&](int it) {
+      const int row = first_key(it);
+      kst.load(rows_at<ES>(a.k, b, hk, row), len - row);
+      vst.load(rows_at<ES>(a.v, b, hk, row), len - row);
+    };
+    load(0);
     for (int it = 0; it < count; ++it) {
       __syncthreads();
-      kst.put(ks);
-      vst.put(vs);
-      __syncthreads();
       const int key0 = first_key(it);
-      if (it + 1 < count) {
-        kst.load(a.k, b, hk, first_key(it + 1), len, a.d);
-        vst.load(a.v, b, hk, first_key(it + 1), len, a.dv);
-      }
+      kst.put(ks, len - key0);
+      vst.put(vs, len - key0);
+      __syncthreads();
+      if (it + 1 < count) load(it + 1);
       // of the wave's rows, does one see one of the keys; do all see all of them
       const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
       if (!some) continue;
       const bool all = key0 + BK - 1 <= w0 && (w0 + 31 - key0 < a.window || key0 + BK <= a.sinks);
       floatx16 x[NSUB];
 #pragma unroll
-      for (int sub = 0; sub < NSUB; ++sub) {
+      for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[sub][i] = 0.f;
 #pragma unroll
-        for (int s = 0; s < P / 16; ++s)
+      for (int s = 0; s < P / 16; ++s)
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub)
           win_mma<IN>(x[sub], win_read_row<P, IN>(ks, 32 * sub + (lane & 31), s, hh), qf[s]);
+      if (!all) {
+        // key <= row within the window in one comparison; of the sinks those up to the row
+        const int ahead = row - key0 - 4 * hh, sinks = min(a.sinks, row + 1) - key0 - 4 * hh;
+        const bool far = key0 < a.sinks;
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int k = 32 * sub + 8 * (i >> 2) + (i & 3);
+            bool seen = static_cast<uint32_t>(ahead - k) < static_cast<uint32_t>(a.window);
+            if (far) seen = seen | (k < sinks);
+            x[sub][i] = seen ? x[sub][i] : -__builtin_inff();
+          }
       }
-      auto seen = [&](int sub, int i) {
-        const int key = key0 + 32 * sub + 8 * (i >> 2) + 4 * hh + (i & 3);
-        return key <= row && (row - key < a.window || key < a.sinks);
-      };
       float top = m;
-      if (all) {
 #pragma unroll
-        for (int sub = 0; sub < NSUB; ++sub)
+      for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, x[sub][i]);
-      } else {
-#pragma unroll
-        for (int sub = 0; sub < NSUB; ++sub)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, seen(sub, i) ? x[sub][i] : -1e30f);
-      }
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (__any(top > m)) {
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, x[sub][i]);
+      // the maximum moves, for both lanes of a row at once, when a weight would exceed 2^8
+      if (__any(top > limit)) {
+        top = fmaxf(top, __shfl_xor(top, 32));
         const float shrink = __builtin_amdgcn_exp2f((m - top) * a.c);
         l *= shrink;
 #pragma unroll
@@ -396,18 +443,13 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[mt][i] *= shrink;
         m = top;
+        limit = m + room;
       }
       const float mc = m * a.c;
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[sub][i] = __builtin_amdgcn_exp2f(fmaf(x[sub][i], a.c, -mc));
-      if (!all) {
-#pragma unroll
-        for (int sub = 0; sub < NSUB; ++sub)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[sub][i] = seen(sub, i) ? x[sub][i] : 0.f;
-      }
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
@@ -512,12 +554,14 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
     const char* qrow = rows_at<ES>(a.q, b, h, in ? row : 0);
     const char* grow = rows_at<ES>(a.go, b, h, in ? row : 0);
     const char* orow = static_cast<const char*>(a.out) + (head_row + (in ? row : 0)) * a.dv * ES;
-    const int out_aligned = (a.dv * ES) % 16 == 0;
 #pragma unroll
     for (int s = 0; s < P / 16; ++s) {
-      qf[s] = win_load_row<IN>(qrow, s, hh, in ? a.d : 0, a.q.aligned, flip);
-      gf[s] = win_load_row<IN>(grow, s, hh, in ? a.dv : 0, a.go.aligned, 0u);
-      const WinFrag<IN> o = win_load_row<IN>(orow, s, hh, in ? a.dv : 0, out_aligned, 0u);
+      qf[s] = win_load_row<IN>(qrow, s, hh, a.d, flip);
+      gf[s] = win_load_row<IN>(grow, s, hh, a.dv, 0u);
+      WinFrag<IN> o = win_load_row<IN>(orow, s, hh, a.dv, 0u);
+      win_keep<IN>(qf[s], in);
+      win_keep<IN>(gf[s], in);
+      win_keep<IN>(o, in);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf(load_elem(&gf[s], j, IN), load_elem(&o, j, IN), delta);
     }
@@ -532,19 +576,22 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
     const int count = n_sink + last / BK - t_lo + 1;
     WinStage<P, IN, BK> kst, vst;
     auto first_key = [&](int it) { return (it < n_sink ? it : t_lo + it - n_sink) * BK; };
-    kst.load(a.k, b, hk, first_key(0), len, a.d);
-    vst.load(a.v, b, hk, first_key(0), len, a.dv);
+    kst.init(a.k, a.d);
+    vst.init(a.v, a.dv);
+    auto load = [&](int it) {
+      const int row = first_key(it);
+      kst.load(rows_at<ES>(a.k, b, hk, row), len - row);
+      vst.load(rows_at<ES>(a.v, b, hk, row), len - row);
+    };
+    load(0);
     const float shift = __builtin_amdgcn_logf(a.lift) - lse;
     for (int it = 0; it < count; ++it) {
       __syncthreads();
-      kst.put(ks);
-      vst.put(vs);
-      __syncthreads();
       const int key0 = first_key(it);
-      if (it + 1 < count) {
-        kst.load(a.k, b, hk, first_key(it + 1), len, a.d);
-        vst.load(a.v, b, hk, first_key(it + 1), len, a.dv);
-      }
+      kst.put(ks, len - key0);
+      vst.put(vs, len - key0);
+      __syncthreads();
+      if (it + 1 < count) load(it + 1);
       const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
       if (!some) continue;
       const bool all = key0 + BK - 1 <= w0 && (w0 + 31 - key0 < a.window || key0 + BK <= a.sinks);
@@ -561,10 +608,14 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, shift)) * (g[i] - delta);
         if (!all) {
+          const int ahead = row - key0 - 4 * hh, sinks = min(a.sinks, row + 1) - key0 - 4 * hh;
+          const bool far = key0 < a.sinks;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int key = key0 + 32 * sub + 8 * (i >> 2) + 4 * hh + (i & 3);
-            x[i] = key <= row && (row - key < a.window || key < a.sinks) ? x[i] : 0.f;
+            const int k = 32 * sub + 8 * (i >> 2) + (i & 3);
+            bool seen = static_cast<uint32_t>(ahead - k) < static_cast<uint32_t>(a.window);
+            if (far) seen = seen | (k < sinks);
+            x[i] = seen ? x[i] : 0.f;
           }
         }
 #pragma unroll
@@ -685,17 +736,21 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
     const char* vrow = rows_at<ES>(a.v, b, hk, key < len ? key : 0);
 #pragma unroll
     for (int s = 0; s < P / 16; ++s) {
-      kf[s] = win_load_row<IN>(krow, s, hh, key < len ? a.d : 0, a.k.aligned, flip);
-      vf[s] = win_load_row<IN>(vrow, s, hh, key < len ? a.dv : 0, a.v.aligned, 0u);
+      kf[s] = win_load_row<IN>(krow, s, hh, a.d, flip);
+      vf[s] = win_load_row<IN>(vrow, s, hh, a.dv, 0u);
+      win_keep<IN>(kf[s], key < len);
+      win_keep<IN>(vf[s], key < len);
     }
     const int t_lo = lo / BQ, per_head = hi / BQ - t_lo + 1, count = per_head * a.group;
     const float lift = __builtin_amdgcn_logf(a.lift);
     WinStage<P, IN, BQ> qst, gst;
+    qst.init(a.q, a.d);
+    gst.init(a.go, a.dv);
     float st_lse = 0.f, st_delta = 0.f;
     auto load = [&](int it) {
       const int h = hk * a.group + it / per_head, row0 = (t_lo + it % per_head) * BQ;
-      qst.load(a.q, b, h, row0, len, a.d);
-      gst.load(a.go, b, h, row0, len, a.dv);
+      qst.load(rows_at<ES>(a.q, b, h, row0), len - row0);
+      gst.load(rows_at<ES>(a.go, b, h, row0), len - row0);
       const int row = row0 + (threadIdx.x & 31);
       st_lse = st_delta = 0.f;
       if (threadIdx.x < 32 && row < len) {
@@ -707,14 +762,14 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
     load(0);
     for (int it = 0; it < count; ++it) {
       __syncthreads();
-      qst.put(qs);
-      gst.put(gs);
+      const int q0 = (t_lo + it % per_head) * BQ;
+      qst.put(qs, len - q0);
+      gst.put(gs, len - q0);
       if (threadIdx.x < 32) {
         reinterpret_cast<float*>(stat_lse)[threadIdx.x] = st_lse;
         reinterpret_cast<float*>(stat_delta)[threadIdx.x] = st_delta;
       }
       __syncthreads();
-      const int q0 = (t_lo + it % per_head) * BQ;
       if (it + 1 < count) load(it + 1);
       const bool some = far ? kw < a.sinks && q0 + BQ - 1 - kw >= a.window
                             : q0 + BQ - 1 >= kw && q0 - (kw + 31) < a.window;
@@ -741,11 +796,13 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
         }
       }
       if (!all) {
+        const int ahead = q0 + 4 * hh - key;  // of row q0 + 4 hh
+        const int first = lo - q0 - 4 * hh, last = key < a.sinks ? hi - q0 - 4 * hh : -1;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const int row = q0 + 8 * (i >> 2) + 4 * hh + (i & 3);
-          const bool seen = far ? key < a.sinks && row - key >= a.window && row >= lo && row <= hi
-                                : row >= key && row - key < a.window;
+          const int r = 8 * (i >> 2) + (i & 3);
+          bool seen = static_cast<uint32_t>(ahead + r) < static_cast<uint32_t>(a.window);
+          if (far) seen = (ahead + r >= a.window) & (r >= first) & (r <= last);
           x[i] = seen ? x[i] : 0.f;
           g[i] = seen ? g[i] : 0.f;
         }

@@ -96,8 +96,10 @@ def _check_lengths(lengths: Optional[Tensor], batch: int) -> Optional[Tensor]:
 
 
 def _rows(x: Tensor) -> Tensor:
-    """x itself where the kernels can walk its rows (contiguous last dimension), else a dense copy."""
-    return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
+    """x itself where the kernels can walk its rows (contiguous last dimension, rows at most 2^24 bytes apart), else a
+    dense copy."""
+    near = x.stride(2) * x.element_size() <= 1 << 24
+    return x if near and (x.stride(3) == 1 or x.shape[3] == 1) else x.contiguous()
 
 
 def _dense(x: Tensor) -> Tensor:
@@ -123,6 +125,12 @@ def _on(device: torch.device):
     return _here if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
+def _widen(x: Tensor) -> Tensor:
+    """x with zero columns up to the 16 bytes that the kernels' rows have at least."""
+    short = 16 // x.element_size() - x.shape[3]
+    return torch.nn.functional.pad(x, (0, short)) if short > 0 else x
+
+
 def _forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: float, lengths: Optional[Tensor],
              with_lse: bool) -> Tuple[Tensor, Optional[Tensor]]:
     b, h, n, d = q.shape
@@ -131,6 +139,9 @@ def _forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: fl
     lse = torch.empty((b, h, n), device=q.device, dtype=torch.float32) if with_lse else None
     if out.numel() == 0:
         return out, lse
+    if min(d, dv) * q.element_size() < 16:
+        wide, lse = _forward(_widen(q), _widen(k), _widen(v), window, sinks, scale, lengths, with_lse)
+        return out.copy_(wide[..., :dv]), lse
     q, k, v = _rows(q), _rows(k), _rows(v)
     with _on(q.device):
         st = _native.lib().sta_window_attention(
@@ -150,10 +161,13 @@ def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: T
     dvo = torch.empty((b, hk, n, dv), device=q.device, dtype=q.dtype)
     if dq.numel() == 0:
         return dq, dk.zero_(), dvo.zero_()
+    if min(d, dv) * q.element_size() < 16:
+        wide = _backward(*(_widen(x) for x in (grad, q, k, v, out)), lse, window, sinks, scale, lengths)
+        return dq.copy_(wide[0][..., :d]), dk.copy_(wide[1][..., :d]), dvo.copy_(wide[2][..., :dv])
     grad, q, k, v, out, lse = _rows(grad), _rows(q), _rows(k), _rows(v), _dense(out), lse.contiguous()
     lib = _native.lib()
     with _on(q.device):
-        nbytes = lib.sta_window_backward_bytes(b, h, hk, n, d, dv, window, sinks)
+        nbytes = lib.sta_window_backward_bytes(_native.DTYPE_CODES[q.dtype], b, h, hk, n, d, dv, window, sinks)
         if nbytes < 0:
             raise _native.NativeError("sta_window_backward_bytes refused the shape")
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)

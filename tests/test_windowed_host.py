@@ -123,12 +123,13 @@ def test_library_refuses_without_touching_a_device():
     for kw, want in [(dict(q=None), E.STA_ERR_ARG), (dict(out=None), E.STA_ERR_ARG), (dict(out=8), E.STA_ERR_ARG),
                      (dict(s=None), E.STA_ERR_ARG), (dict(dt=3), E.STA_ERR_DTYPE), (dict(b=0), E.STA_ERR_SHAPE),
                      (dict(h=3, hk=2), E.STA_ERR_SHAPE), (dict(n=0), E.STA_ERR_SHAPE), (dict(d=129), E.STA_ERR_UNSUPPORTED),
-                     (dict(dv=129), E.STA_ERR_UNSUPPORTED), (dict(n=(1 << 30) + 1), E.STA_ERR_UNSUPPORTED),
+                     (dict(dv=129), E.STA_ERR_UNSUPPORTED), (dict(d=3), E.STA_ERR_UNSUPPORTED),
+                     (dict(dt=1, dv=7), E.STA_ERR_UNSUPPORTED), (dict(n=(1 << 30) + 1), E.STA_ERR_UNSUPPORTED),
                      (dict(w=0), E.STA_ERR_ARG), (dict(sinks=-1), E.STA_ERR_ARG), (dict(scale=math.inf), E.STA_ERR_ARG),
                      (dict(b=1 << 31), E.STA_ERR_UNSUPPORTED), (dict(b=1 << 30, n=1 << 20), E.STA_ERR_SHAPE)]:
         assert fwd(**kw) == want, kw
-    assert lib.sta_window_backward_bytes(1, 2, 1, 8, 8, 8, 0, 1) == -1
-    need = lib.sta_window_backward_bytes(1, 2, 1, 1000, 8, 8, 100, 4)
+    assert lib.sta_window_backward_bytes(0, 1, 2, 1, 8, 8, 8, 0, 1) == -1
+    need = lib.sta_window_backward_bytes(0, 1, 2, 1, 1000, 8, 8, 100, 4)
     assert need >= 4 * 2 * 1000
     back = [16] * 6 + [0, 1, 2, 1, 1000, 8, 8, st, 1.0, 100, 4, None, 16, 16, 16, 16]
     assert lib.sta_window_attention_backward(*back, need - 1, None) == E.STA_ERR_SCRATCH
