@@ -27,7 +27,13 @@ int launch_window_backward(const sta::WinArgs& a, hipStream_t s) {
   const int64_t grid_s = (bkv * a.sink_rows * (a.d + a.dv) + 255) / 256;
   if (grid_q <= 0 || grid_q > 0x7fffffff || grid_k > 0x7fffffff || grid_s > 0x7fffffff) return STA_ERR_SHAPE;
   hipLaunchKernelGGL((sta::window_dq_kernel<P, IN>), dim3(static_cast<unsigned>(grid_q)), dim3(256), 0, s, a);
-  hipLaunchKernelGGL((sta::window_dkv_kernel<P, IN>), dim3(static_cast<unsigned>(grid_k)), dim3(256), 0, s, a);
+  constexpr int lds = sta::win_dkv_lds<P, IN>();
+  if constexpr (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&sta::window_dkv_kernel<P, IN>),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return hip_status(e);
+  }
+  hipLaunchKernelGGL((sta::window_dkv_kernel<P, IN>), dim3(static_cast<unsigned>(grid_k)), dim3(256), lds, s, a);
   if (a.far_chunks > 0)
     hipLaunchKernelGGL((sta::window_sink_kernel<IN>), dim3(static_cast<unsigned>(grid_s)), dim3(256), 0, s, a);
   return check_launch();

@@ -237,6 +237,8 @@ __device__ __forceinline__ void win_keep(WinFrag<IN>& f, bool row) {
     f.w[i] = uint4{row ? f.w[i].x : 0u, row ? f.w[i].y : 0u, row ? f.w[i].z : 0u, row ? f.w[i].w : 0u};
 }
 
+__device__ __forceinline__ void win_pin(floatx16& x) { asm volatile("" : "+a"(x)); }
+
 __device__ __forceinline__ bool win_finite(float x) { return fabsf(x) < __builtin_inff(); }
 
 // four values of a row at column col (a multiple of 4) of a dense [.., width] tensor
@@ -692,14 +694,24 @@ __device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, in
   for (int e = 0; e < 2; ++e) dk[e] *= a.scale;
 }
 
+// Rows that window_dkv_kernel stages at a time, and its LDS: two stages of query and gradient rows, then their
+// statistics.
+template <int IN>
+__host__ __device__ constexpr int win_rows() { return IN == F32 ? 32 : 64; }
+template <int P, int IN>
+__host__ __device__ constexpr int win_dkv_lds() {
+  return 2 * (2 * win_rows<IN>() * P * (IN == F32 ? 4 : 2) + 2 * win_rows<IN>() * 4);
+}
+
 // dk and dv: one workgroup per 128 keys of a key head (32 a wave) walks over the rows that see them within the window,
 // for every head of the group; the rows behind the window of a sink go to workgroups of their own (far), whose
 // sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.
 template <int P, int IN>
 __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
-  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = 32;
-  __shared__ uint4 qs[BQ * CH], gs[BQ * CH];
-  __shared__ floatx4 stat_lse[BQ / 4], stat_delta[BQ / 4];
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_rows<IN>(), NSUB = BQ / 32;
+  constexpr int STAGE = 2 * BQ * CH;  // 16-byte units of a stage
+  extern __shared__ uint4 win_lds[];
+  float* const stats = reinterpret_cast<float*>(win_lds + 2 * STAGE);  // [stage][lse, delta][BQ]
   const int kv = a.heads / a.group;
   const int far_items = a.sink_tiles * a.far_chunks, items = far_items + a.tiles;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
@@ -741,79 +753,129 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
       win_keep<IN>(kf[s], key < len);
       win_keep<IN>(vf[s], key < len);
     }
-    const int t_lo = lo / BQ, per_head = hi / BQ - t_lo + 1, count = per_head * a.group;
+    const int first = lo / BQ * BQ, count = (hi / BQ - lo / BQ + 1) * a.group;
     const float lift = __builtin_amdgcn_logf(a.lift);
     WinStage<P, IN, BQ> qst, gst;
     qst.init(a.q, a.d);
     gst.init(a.go, a.dv);
-    float st_lse = 0.f, st_delta = 0.f;
-    auto load = [&](int it) {
-      const int h = hk * a.group + it / per_head, row0 = (t_lo + it % per_head) * BQ;
-      qst.load(rows_at<ES>(a.q, b, h, row0), len - row0);
-      gst.load(rows_at<ES>(a.go, b, h, row0), len - row0);
-      const int row = row0 + (threadIdx.x & 31);
-      st_lse = st_delta = 0.f;
-      if (threadIdx.x < 32 && row < len) {
-        const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.n + row;
-        st_lse = a.lse[at];
-        st_delta = a.delta[at];
+    float stat = 0.f;
+    // the tile to be loaded next, the one in registers, the one to be computed
+    int load_row = first, load_head = hk * a.group, put_row = first, row0 = first;
+    auto load = [&]() {
+      qst.load(rows_at<ES>(a.q, b, load_head, load_row), len - load_row);
+      gst.load(rows_at<ES>(a.go, b, load_head, load_row), len - load_row);
+      if (threadIdx.x < 2 * BQ) {
+        const int row = load_row + threadIdx.x % BQ;
+        const float* from = static_cast<int>(threadIdx.x) < BQ ? a.lse : a.delta;
+        stat = row < len ? from[(static_cast<int64_t>(b) * a.heads + load_head) * a.n + row] : 0.f;
+      }
+      load_row += BQ;
+      if (load_row > hi) {
+        load_row = first;
+        ++load_head;
       }
     };
-    load(0);
+    auto put = [&](int stage) {
+      qst.put(win_lds + stage * STAGE, len - put_row);
+      gst.put(win_lds + stage * STAGE + BQ * CH, len - put_row);
+      if (threadIdx.x < 2 * BQ) stats[stage * 2 * BQ + threadIdx.x] = stat;
+      put_row = put_row + BQ > hi ? first : put_row + BQ;
+    };
+    load();
+    put(0);
+    if (count > 1) load();
     for (int it = 0; it < count; ++it) {
-      __syncthreads();
-      const int q0 = (t_lo + it % per_head) * BQ;
-      qst.put(qs, len - q0);
-      gst.put(gs, len - q0);
-      if (threadIdx.x < 32) {
-        reinterpret_cast<float*>(stat_lse)[threadIdx.x] = st_lse;
-        reinterpret_cast<float*>(stat_delta)[threadIdx.x] = st_delta;
+      // the accumulators stay in accumulation registers (the compiler else moves all of them there and back)
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        win_pin(dk[mt]);
+        win_pin(dv[mt]);
       }
       __syncthreads();
-      if (it + 1 < count) load(it + 1);
+      if (it + 1 < count) put((it + 1) & 1);
+      if (it + 2 < count) load();
+      const uint4 *qs = win_lds + (it & 1) * STAGE, *gs = qs + BQ * CH;
+      const floatx4* st = reinterpret_cast<const floatx4*>(stats + (it & 1) * 2 * BQ);
+      const int q0 = row0;
+      row0 = row0 + BQ > hi ? first : row0 + BQ;
       const bool some = far ? kw < a.sinks && q0 + BQ - 1 - kw >= a.window
                             : q0 + BQ - 1 >= kw && q0 - (kw + 31) < a.window;
       if (!some) continue;
       const bool all = far ? kw + 32 <= a.sinks && q0 - (kw + 31) >= a.window && q0 >= lo && q0 + BQ - 1 <= hi
                            : q0 >= kw + 31 && q0 + BQ - 1 - kw < a.window;
-      floatx16 x, g;
+#pragma unroll 1
+      for (int sub = 0; sub < NSUB; ++sub) {
+        // every operand is read well before its product: a compute unit holds one wave a SIMD, which has nothing else to
+        // do while it waits
+        WinFrag<IN> qa[P / 16], ga[P / 16], qc[MT], gc[MT];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
-#pragma unroll
-      for (int s = 0; s < P / 16; ++s) {
-        win_mma<IN>(x, win_read_row<P, IN>(qs, lane & 31, s, hh), kf[s]);
-        win_mma<IN>(g, win_read_row<P, IN>(gs, lane & 31, s, hh), vf[s]);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const floatx4 lse = stat_lse[2 * r + hh], delta = stat_delta[2 * r + hh];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = 4 * r + e;
-          const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, lift - lse[e]));
-          g[i] = p * (g[i] - delta[e]);
-          x[i] = p;
+        for (int s = 0; s < P / 16; ++s) {
+          qa[s] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
+          ga[s] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
         }
-      }
-      if (!all) {
-        const int ahead = q0 + 4 * hh - key;  // of row q0 + 4 hh
-        const int first = lo - q0 - 4 * hh, last = key < a.sinks ? hi - q0 - 4 * hh : -1;
+        __builtin_amdgcn_sched_barrier(0);
+        floatx16 x, g;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int r = 8 * (i >> 2) + (i & 3);
-          bool seen = static_cast<uint32_t>(ahead + r) < static_cast<uint32_t>(a.window);
-          if (far) seen = (ahead + r >= a.window) & (r >= first) & (r <= last);
-          x[i] = seen ? x[i] : 0.f;
-          g[i] = seen ? g[i] : 0.f;
+        for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < P / 16; ++s) {
+          win_mma<IN>(x, qa[s], kf[s]);
+          win_mma<IN>(g, ga[s], vf[s]);
         }
-      }
+        floatx4 lse[4], delta[4];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
+        for (int r = 0; r < 4; ++r) {
+          lse[r] = st[8 * sub + 2 * r + hh];
+          delta[r] = st[BQ / 4 + 8 * sub + 2 * r + hh];
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          win_mma<IN>(dv[mt], win_read_columns<P, IN>(gs, 16 * t, mt, lane), p);
-          win_mma<IN>(dk[mt], win_read_columns<P, IN>(qs, 16 * t, mt, lane), ds);
+          gc[mt] = win_read_columns<P, IN>(gs, 32 * sub, mt, lane);
+          qc[mt] = win_read_columns<P, IN>(qs, 32 * sub, mt, lane);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, lift - lse[i >> 2][i & 3]));
+          g[i] = p * (g[i] - delta[i >> 2][i & 3]);
+          x[i] = p;
+        }
+        if (!all) {
+          const int base = q0 + 32 * sub + 4 * hh, ahead = base - key;
+          const int from = lo - base, last = key < a.sinks ? hi - base : -1;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int r = 8 * (i >> 2) + (i & 3);
+            bool seen = static_cast<uint32_t>(ahead + r) < static_cast<uint32_t>(a.window);
+            if (far) seen = (ahead + r >= a.window) & (r >= from) & (r <= last);
+            x[i] = seen ? x[i] : 0.f;
+            g[i] = seen ? g[i] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
+          WinFrag<IN> gn[MT], qn[MT];
+          if (t == 0) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              gn[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16, mt, lane);
+              qn[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16, mt, lane);
+            }
+          }
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            win_mma<IN>(dv[mt], gc[mt], p);
+            win_mma<IN>(dk[mt], qc[mt], ds);
+          }
+          if (t == 0) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              gc[mt] = gn[mt];
+              qc[mt] = qn[mt];
+            }
+          }
         }
       }
     }
