@@ -34,6 +34,12 @@ bool strides_ok(const int64_t* strides, int tensors, int dtype) {
   return true;
 }
 
+#ifndef WIN_SHARE
+#define WIN_SHARE 512
+#endif
+#ifndef WIN_KSHARE
+#define WIN_KSHARE 256
+#endif
 // The shape part of the arguments; STA_OK or what is wrong with it.
 int window_shape(sta::WinArgs& a, int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv,
                  float scale, int64_t window, int64_t sinks) {
@@ -55,7 +61,11 @@ int window_shape(sta::WinArgs& a, int dtype, int64_t batch, int heads, int kv_he
   a.scale = scale;
   // above 0: a hidden pair's logit, -inf, stays one times c
   a.c = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-37f);
-  a.tiles = static_cast<int>((n + sta::WIN_ROWS - 1) / sta::WIN_ROWS);
+  const int64_t wide = (n + sta::WIN_ROWS - 1) / sta::WIN_ROWS;
+  a.share = batch * heads * wide < WIN_SHARE;
+  a.key_share = batch * kv_heads * wide < WIN_KSHARE;
+  a.tiles = static_cast<int>(a.share ? (n + 31) / 32 : wide);
+  a.key_tiles = static_cast<int>(a.key_share ? (n + 31) / 32 : wide);
   a.lift = a.drop = 1.f;
   return STA_OK;
 }
@@ -67,13 +77,14 @@ void plan_sinks(sta::WinArgs& a) {
   if (a.sinks == 0 || behind <= 0) return;
   const int64_t bkv = static_cast<int64_t>(a.batch) * (a.heads / a.group);
   a.sink_rows = a.sinks;
-  a.sink_tiles = (a.sinks + sta::WIN_ROWS - 1) / sta::WIN_ROWS;
+  const int rows = a.key_share ? 32 : sta::WIN_ROWS;
+  a.sink_tiles = (a.sinks + rows - 1) / rows;
   int64_t chunks = 512 / (bkv * a.sink_tiles);
   if (chunks > (behind + 255) / 256) chunks = (behind + 255) / 256;
   if (chunks < 1) chunks = 1;
-  const int64_t rows = ((behind + chunks - 1) / chunks + 31) / 32 * 32;
-  a.far_rows = static_cast<int>(rows);
-  a.far_chunks = static_cast<int>((behind + rows - 1) / rows);
+  const int64_t chunk = ((behind + chunks - 1) / chunks + 31) / 32 * 32;
+  a.far_rows = static_cast<int>(chunk);
+  a.far_chunks = static_cast<int>((behind + chunk - 1) / chunk);
 }
 
 int64_t delta_floats(const sta::WinArgs& a) {

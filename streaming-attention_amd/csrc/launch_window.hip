@@ -10,12 +10,23 @@
 
 namespace sta_api {
 
+template <typename Kernel>
+static int launch(Kernel kernel, int64_t grid, int lds, const sta::WinArgs& a, hipStream_t s) {
+  if (grid <= 0 || grid > 0x7fffffff) return STA_ERR_SHAPE;
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return hip_status(e);
+  }
+  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), lds, s, a);
+  return check_launch();
+}
+
 template <int P, int IN>
 int launch_window_forward(const sta::WinArgs& a, hipStream_t s) {
   const int64_t grid = static_cast<int64_t>(a.batch) * a.heads * a.tiles;
-  if (grid <= 0 || grid > 0x7fffffff) return STA_ERR_SHAPE;
-  hipLaunchKernelGGL((sta::window_forward_kernel<P, IN>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
-  return check_launch();
+  if (a.share) return launch(sta::window_forward_kernel<P, IN, true>, grid, sta::win_lds_bytes<P, IN, true>(), a, s);
+  return launch(sta::window_forward_kernel<P, IN, false>, grid, sta::win_lds_bytes<P, IN, false>(), a, s);
 }
 
 // D and dq, then dk and dv, then the sums of the sinks
@@ -23,20 +34,16 @@ template <int P, int IN>
 int launch_window_backward(const sta::WinArgs& a, hipStream_t s) {
   const int64_t bkv = static_cast<int64_t>(a.batch) * (a.heads / a.group);
   const int64_t grid_q = static_cast<int64_t>(a.batch) * a.heads * a.tiles;
-  const int64_t grid_k = bkv * (a.tiles + static_cast<int64_t>(a.sink_tiles) * a.far_chunks);
+  const int64_t grid_k = bkv * (a.key_tiles + static_cast<int64_t>(a.sink_tiles) * a.far_chunks);
   const int64_t grid_s = (bkv * a.sink_rows * (a.d + a.dv) + 255) / 256;
-  if (grid_q <= 0 || grid_q > 0x7fffffff || grid_k > 0x7fffffff || grid_s > 0x7fffffff) return STA_ERR_SHAPE;
-  hipLaunchKernelGGL((sta::window_dq_kernel<P, IN>), dim3(static_cast<unsigned>(grid_q)), dim3(256), 0, s, a);
-  constexpr int lds = sta::win_dkv_lds<P, IN>();
-  if constexpr (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(&sta::window_dkv_kernel<P, IN>),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return hip_status(e);
-  }
-  hipLaunchKernelGGL((sta::window_dkv_kernel<P, IN>), dim3(static_cast<unsigned>(grid_k)), dim3(256), lds, s, a);
-  if (a.far_chunks > 0)
-    hipLaunchKernelGGL((sta::window_sink_kernel<IN>), dim3(static_cast<unsigned>(grid_s)), dim3(256), 0, s, a);
-  return check_launch();
+  if (grid_k > 0x7fffffff || grid_s > 0x7fffffff) return STA_ERR_SHAPE;
+  int st = a.share ? launch(sta::window_dq_kernel<P, IN, true>, grid_q, sta::win_lds_bytes<P, IN, true>(), a, s)
+                   : launch(sta::window_dq_kernel<P, IN, false>, grid_q, sta::win_lds_bytes<P, IN, false>(), a, s);
+  if (st != STA_OK) return st;
+  st = a.key_share ? launch(sta::window_dkv_kernel<P, IN, true>, grid_k, sta::win_dkv_lds<P, IN, true>(), a, s)
+                   : launch(sta::window_dkv_kernel<P, IN, false>, grid_k, sta::win_dkv_lds<P, IN, false>(), a, s);
+  if (st != STA_OK || a.far_chunks == 0) return st;
+  return launch(sta::window_sink_kernel<IN>, grid_s, 0, a, s);
 }
 
 template int launch_window_forward<STA_WIN_P, STA_WIN_IN>(const sta::WinArgs&, hipStream_t);

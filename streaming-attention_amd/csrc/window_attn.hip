@@ -44,7 +44,8 @@ struct WinArgs {
   float* lse;              // [batch][heads][n]: log2 of the row's sum of weights, or null
   float* delta;            // [batch][heads][n]: D_i
   void *dq, *dk, *dv_out;  // [batch][heads][n][d], [batch][kv heads][n][d | dv]
-  int tiles;               // tiles of 128 rows (keys)
+  int share, key_share;    // tiles of 32 rows (keys) instead of 128, see win_rows
+  int tiles, key_tiles;
   // gradients of sinks behind their window: rows [j + window, n) of the first sink_tiles key tiles, far_chunks
   // workgroups a tile with far_rows rows each; sums part [batch kv_heads][far_chunks + 1][sink_rows][d + dv]
   int sink_tiles, far_chunks, far_rows, sink_rows;
@@ -110,44 +111,43 @@ __device__ __forceinline__ WinFrag<IN> win_operand(const floatx16& x, int t) {
   return f;
 }
 
-// Staging of ROWS rows of a tile by 256 threads: registers first (load), LDS when the tile before is done with (put).
+// Staging of ROWS rows of a tile by a workgroup (256 threads) or a wave: registers first (load), LDS when the tile before is done with (put).
 // The loads are free of branches, so that they stay in flight while a tile computes: rows behind the last are read as the
 // last one and a row's last 16 bytes in the place of a unit that would reach over its end; put zeroes the ones and
 // moves the others into place.
-template <int P, int IN, int ROWS>
+template <int P, int IN, int ROWS, int THREADS>
 struct WinStage {
   static constexpr int ES = IN == F32 ? 4 : 2, E = 16 / ES, CH = win_chunks<ES>(P);
-  static constexpr int COUNT = (ROWS * CH + 255) / 256;
+  static constexpr int COUNT = (ROWS * CH + THREADS - 1) / THREADS;
+  static constexpr bool EVEN = THREADS % CH == 0;  // a thread's units lie in one column, THREADS / CH rows apart
   uint4 u[COUNT];
-  uint32_t at[COUNT];  // bytes from the tile's first row (the host keeps 64 rows below 2^31 bytes)
+  uint32_t at[EVEN ? 1 : COUNT];  // bytes from the tile's first row (the host keeps 64 rows below 2^31 bytes)
   int pitch, width;
 
+  __device__ __forceinline__ static int unit(int i) { return (threadIdx.x % THREADS) + THREADS * i; }
   __device__ __forceinline__ void init(const Rows& t, int w) {
     pitch = static_cast<int>(t.sn) * ES;
     width = w;
 #pragma unroll
-    for (int i = 0; i < COUNT; ++i) {
-      const int x = threadIdx.x + 256 * i;
+    for (int i = 0; i < (EVEN ? 1 : COUNT); ++i) {
+      const int x = unit(i);
       at[i] = min(x / CH, ROWS - 1) * pitch + min(x % CH * E, width - E) * ES;
     }
   }
   // the tile at `row`, `left` >= 1 of its rows being there; a row has at least 16 bytes
   __device__ __forceinline__ void load(const char* row, int left) {
-    if (left >= ROWS) {
 #pragma unroll
-      for (int i = 0; i < COUNT; ++i) u[i] = rows_load16(row + at[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < COUNT; ++i) {
-        const int r = min((threadIdx.x + 256 * i) / CH, ROWS - 1);
-        u[i] = rows_load16(row + (at[i] - static_cast<uint32_t>(max(0, r - left + 1) * pitch)));
-      }
+    for (int i = 0; i < COUNT; ++i) {
+      const char* from = EVEN ? row + static_cast<int64_t>(i * (THREADS / CH)) * pitch : row;
+      uint32_t off = at[EVEN ? 0 : i];
+      if (left < ROWS) off -= static_cast<uint32_t>(max(0, min(unit(i) / CH, ROWS - 1) - left + 1) * pitch);
+      u[i] = rows_load16(from + static_cast<int32_t>(off));
     }
   }
   __device__ __forceinline__ void put(uint4* lds, int left) const {
     auto to = [&](int i, const uint4& x) {
-      const int k = threadIdx.x + 256 * i, r = k / CH, c = k % CH;
-      if (ROWS * CH % 256 == 0 || k < ROWS * CH) lds[r * CH + (c ^ win_swizzle<CH>(r))] = x;
+      const int k = unit(i), r = k / CH, c = k % CH;
+      if (ROWS * CH % THREADS == 0 || k < ROWS * CH) lds[r * CH + (c ^ win_swizzle<CH>(r))] = x;
     };
     if (left >= ROWS && width == P) {
 #pragma unroll
@@ -155,7 +155,7 @@ struct WinStage {
     } else {
 #pragma unroll
       for (int i = 0; i < COUNT; ++i) {
-        const int k = threadIdx.x + 256 * i, r = k / CH, c = k % CH;
+        const int k = unit(i), r = k / CH, c = k % CH;
         uint4 x = u[i];
         if (width % E) x = rows_shift(x, max(0, c * E + E - width) * ES & 15);
         const bool in = r < left && c * E < width;
@@ -333,6 +333,51 @@ __device__ void win_forward_row(const WinArgs& a, int b, int h, int i) {
   if (a.lse && lane == 0) a.lse[row] = m * 1.44269504f + log2f(l);
 }
 
+// Two ways to deal out a head's rows.  Wide: 128 rows (keys) a workgroup, 32 a wave, which share the staged tiles of the
+// other side.  Shared, for grids that would leave compute units idle: 32 rows a workgroup, whose four waves stage and
+// take every fourth tile of the other side by themselves and are joined through LDS: four times the workgroups, each a
+// quarter as long.
+template <bool SHARE>
+__host__ __device__ constexpr int win_rows() { return SHARE ? 32 : WIN_ROWS; }
+// whether a tile's rows are loaded while the one before computes: not where a wave would hold 128 registers of them
+template <int P, int IN, bool SHARE>
+__host__ __device__ constexpr bool win_ahead() { return !(SHARE && IN == F32 && P > 64); }
+template <bool SHARE>
+__device__ __forceinline__ void win_sync() {
+  if constexpr (SHARE) {  // a wave's LDS accesses are in order; the fences keep the compiler's order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  } else {
+    __syncthreads();
+  }
+}
+
+// The accumulators of the four waves in LDS, [wave][32 rows][P + 4], and their sums with weights f: 4 columns (a
+// multiple of 4 from col) of row threadIdx.x / 8
+template <int P>
+__host__ __device__ constexpr int win_join_floats() { return 4 * 32 * (P + 4); }
+template <int P>
+__device__ __forceinline__ void win_join_put(float* red, const floatx16 (&acc)[P / 32], int wave, int lane) {
+#pragma unroll
+  for (int mt = 0; mt < P / 32; ++mt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<floatx4*>(&red[(wave * 32 + (lane & 31)) * (P + 4) + 32 * mt + 8 * r + 4 * (lane >> 5)]) =
+          floatx4{acc[mt][4 * r], acc[mt][4 * r + 1], acc[mt][4 * r + 2], acc[mt][4 * r + 3]};
+}
+template <int P>
+__device__ __forceinline__ floatx4 win_join_get(const float* red, int col, const float (&f)[4]) {
+  floatx4 s = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    s += *reinterpret_cast<const floatx4*>(&red[(w * 32 + threadIdx.x / 8) * (P + 4) + col]) * f[w];
+  return s;
+}
+__device__ __forceinline__ int win_bad4(const floatx4& x) {
+  return !(win_finite(x[0]) && win_finite(x[1]) && win_finite(x[2]) && win_finite(x[3]));
+}
+
 // Which (batch, query head, tile) a workgroup takes: the heads of a group and the neighbouring tiles of a head on one
 // XCD, whose L2 then holds the keys they share; the last tiles (most keys) first.
 __device__ __forceinline__ void win_place(const WinArgs& a, int& b, int& h, int& tile) {
@@ -346,20 +391,30 @@ __device__ __forceinline__ void win_place(const WinArgs& a, int& b, int& h, int&
   b = id / kv;
 }
 
-template <int IN>
-__host__ __device__ constexpr int win_keys() { return IN == F32 ? 32 : 64; }
+template <int IN, bool SHARE>
+__host__ __device__ constexpr int win_keys() { return IN == F32 || SHARE ? 32 : 64; }
+// LDS of the forward and the dq kernel
+template <int P, int IN, bool SHARE>
+__host__ __device__ constexpr int win_lds_bytes() {
+  const int stage = 2 * win_keys<IN, SHARE>() * P * (IN == F32 ? 4 : 2);
+  if (!SHARE) return stage;
+  const int join = 4 * (win_join_floats<P>() + 2 * 4 * 32);
+  return 4 * stage > join ? 4 * stage : join;
+}
 
-// One workgroup per 128 query rows of a head, 32 a wave; keys staged win_keys at a time, the next tile's rows in
-// registers while this one computes.
-template <int P, int IN>
+// Row tiles: keys staged win_keys at a time, the next tile's rows in registers while this one computes.
+template <int P, int IN, bool SHARE>
 __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forward_kernel(const WinArgs a) {
-  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN>(), NSUB = BK / 32, MT = P / 32;
-  __shared__ uint4 ks[BK * CH], vs[BK * CH];
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
+                MT = P / 32, STEP = SHARE ? 4 : 1;
+  constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
+  extern __shared__ uint4 win_lds[];
   int b, h, tile;
   win_place(a, b, h, tile);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
+  uint4 *const ks = win_lds + (SHARE ? wave * 2 * BK * CH : 0), *const vs = ks + BK * CH;
   const int len = win_length(a, b), hk = h / a.group;
-  const int r0 = tile * WIN_ROWS, w0 = r0 + 32 * wave, row = w0 + (lane & 31);
+  const int r0 = tile * win_rows<SHARE>(), w0 = r0 + (SHARE ? 0 : 32 * wave), row = w0 + (lane & 31);
   const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
 
   floatx16 acc[MT];
@@ -380,12 +435,12 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       win_keep<IN>(qf[s], row < len);
     }
 
-    const int last = (r0 + WIN_ROWS < len ? r0 + WIN_ROWS : len) - 1;
+    const int last = (r0 + win_rows<SHARE>() < len ? r0 + win_rows<SHARE>() : len) - 1;
     const int t_lo = (r0 - a.window + 1 > 0 ? r0 - a.window + 1 : 0) / BK;
     int n_sink = (a.sinks + BK - 1) / BK;
     if (n_sink > t_lo) n_sink = t_lo;
     const int count = n_sink + last / BK - t_lo + 1;
-    WinStage<P, IN, BK> kst, vst;
+    WinStage<P, IN, BK, SHARE ? 64 : 256> kst, vst;
     auto first_key = [&](int it) { return (it < n_sink ? it : t_lo + it - n_sink) * BK; };
     kst.init(a.k, a.d);
     vst.init(a.v, a.dv);
@@ -394,14 +449,16 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       kst.load(rows_at<ES>(a.k, b, hk, row), len - row);
       vst.load(rows_at<ES>(a.v, b, hk, row), len - row);
     };
-    load(0);
-    for (int it = 0; it < count; ++it) {
-      __syncthreads();
+    const int start = SHARE ? wave : 0;
+    if (AHEAD && start < count) load(start);
+    for (int it = start; it < count; it += STEP) {
+      if (!AHEAD) load(it);
+      win_sync<SHARE>();
       const int key0 = first_key(it);
       kst.put(ks, len - key0);
       vst.put(vs, len - key0);
-      __syncthreads();
-      if (it + 1 < count) load(it + 1);
+      win_sync<SHARE>();
+      if (AHEAD && it + STEP < count) load(it + STEP);
       // of the wave's rows, does one see one of the keys; do all see all of them
       const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
       if (!some) continue;
@@ -469,6 +526,52 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
     l += __shfl_xor(l, 32);
   }
 
+  if constexpr (SHARE) {
+    float *red = reinterpret_cast<float*>(win_lds), *red_m = red + win_join_floats<P>(), *red_l = red_m + 4 * 32;
+    __syncthreads();
+    win_join_put<P>(red, acc, wave, lane);
+    if (hh == 0) {
+      red_m[32 * wave + lane] = m;
+      red_l[32 * wave + lane] = l;
+    }
+    __syncthreads();
+    const int r = threadIdx.x / 8, at_row = r0 + r;
+    float top = red_m[r], den = 0.f, f[4];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, red_m[32 * w + r]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = __builtin_amdgcn_exp2f((red_m[32 * w + r] - top) * a.c);
+      den = fmaf(f[w], red_l[32 * w + r], den);
+    }
+    const bool in = at_row < len;
+    const float inv = in ? 1.f / den : 0.f;
+    floatx4 o[MT];
+    int bad = !(den > 0.f && win_finite(den));
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      o[j] = win_join_get<P>(red, 32 * j + 4 * (threadIdx.x & 7), f);
+      bad |= win_bad4(o[j]);
+    }
+    bad = in ? bad : 0;
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) bad |= __shfl_xor(bad, x);
+    if (at_row < a.n && !bad) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const int col = 32 * j + 4 * (threadIdx.x & 7);
+        if (col < a.dv)
+          win_store4<IN>(a.out, (head_row + at_row) * a.dv, col, a.dv, in ? o[j][0] * inv : 0.f, in ? o[j][1] * inv : 0.f,
+                         in ? o[j][2] * inv : 0.f, in ? o[j][3] * inv : 0.f);
+      }
+      if (a.lse && (threadIdx.x & 7) == 0)
+        a.lse[head_row + at_row] = in ? top * a.c + __builtin_amdgcn_logf(den) : 0.f;
+    }
+    for (uint64_t todo = __ballot(bad) & 0x0101010101010101ull; todo; todo &= todo - 1)
+      win_forward_row<IN>(a, b, h, r0 + 8 * wave + __builtin_ctzll(todo) / 8);
+    return;
+  }
+
   const bool in = row < len;
   float inv = 0.f;
   int bad = 0;
@@ -531,15 +634,18 @@ __device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
 }
 
 // dq and D: the forward kernel's walk over the keys with the rows' statistics given.
-template <int P, int IN>
-__global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const WinArgs a) {
-  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN>(), NSUB = BK / 32, MT = P / 32;
-  __shared__ uint4 ks[BK * CH], vs[BK * CH];
+template <int P, int IN, bool SHARE>
+__global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : 2) void window_dq_kernel(const WinArgs a) {
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
+                MT = P / 32, STEP = SHARE ? 4 : 1;
+  constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
+  extern __shared__ uint4 win_lds[];
   int b, h, tile;
   win_place(a, b, h, tile);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
+  uint4 *const ks = win_lds + (SHARE ? wave * 2 * BK * CH : 0), *const vs = ks + BK * CH;
   const int len = win_length(a, b), hk = h / a.group;
-  const int r0 = tile * WIN_ROWS, w0 = r0 + 32 * wave, row = w0 + (lane & 31);
+  const int r0 = tile * win_rows<SHARE>(), w0 = r0 + (SHARE ? 0 : 32 * wave), row = w0 + (lane & 31);
   const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
   const bool in = row < len;
 
@@ -569,14 +675,14 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
     }
     delta += __shfl_xor(delta, 32);
     const float lse = in ? a.lse[head_row + row] : 0.f;
-    if (in && hh == 0) a.delta[head_row + row] = delta;
+    if (in && hh == 0 && (!SHARE || wave == 0)) a.delta[head_row + row] = delta;
 
-    const int last = (r0 + WIN_ROWS < len ? r0 + WIN_ROWS : len) - 1;
+    const int last = (r0 + win_rows<SHARE>() < len ? r0 + win_rows<SHARE>() : len) - 1;
     const int t_lo = (r0 - a.window + 1 > 0 ? r0 - a.window + 1 : 0) / BK;
     int n_sink = (a.sinks + BK - 1) / BK;
     if (n_sink > t_lo) n_sink = t_lo;
     const int count = n_sink + last / BK - t_lo + 1;
-    WinStage<P, IN, BK> kst, vst;
+    WinStage<P, IN, BK, SHARE ? 64 : 256> kst, vst;
     auto first_key = [&](int it) { return (it < n_sink ? it : t_lo + it - n_sink) * BK; };
     kst.init(a.k, a.d);
     vst.init(a.v, a.dv);
@@ -585,15 +691,17 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
       kst.load(rows_at<ES>(a.k, b, hk, row), len - row);
       vst.load(rows_at<ES>(a.v, b, hk, row), len - row);
     };
-    load(0);
+    const int start = SHARE ? wave : 0;
+    if (AHEAD && start < count) load(start);
     const float shift = __builtin_amdgcn_logf(a.lift) - lse;
-    for (int it = 0; it < count; ++it) {
-      __syncthreads();
+    for (int it = start; it < count; it += STEP) {
+      if (!AHEAD) load(it);
+      win_sync<SHARE>();
       const int key0 = first_key(it);
       kst.put(ks, len - key0);
       vst.put(vs, len - key0);
-      __syncthreads();
-      if (it + 1 < count) load(it + 1);
+      win_sync<SHARE>();
+      if (AHEAD && it + STEP < count) load(it + STEP);
       const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
       if (!some) continue;
       const bool all = key0 + BK - 1 <= w0 && (w0 + 31 - key0 < a.window || key0 + BK <= a.sinks);
@@ -629,6 +737,40 @@ __global__ __launch_bounds__(256, IN == F32 ? 1 : 2) void window_dq_kernel(const
         }
       }
     }
+  }
+
+  if constexpr (SHARE) {
+    float* red = reinterpret_cast<float*>(win_lds);
+    const float one[4] = {1.f, 1.f, 1.f, 1.f}, f = a.scale * a.drop;
+    __syncthreads();
+    win_join_put<P>(red, acc, wave, lane);
+    __syncthreads();
+    const int at_row = r0 + threadIdx.x / 8;
+    floatx4 o[MT];
+    int bad = 0;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      o[j] = win_join_get<P>(red, 32 * j + 4 * (threadIdx.x & 7), one);
+      bad |= win_bad4(o[j]);
+    }
+    bad = at_row < len ? bad : 0;
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) bad |= __shfl_xor(bad, x);
+    if (at_row < a.n && !bad) {
+      const bool real = at_row < len;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const int col = 32 * j + 4 * (threadIdx.x & 7);
+        if (col < a.d)
+          win_store4<IN>(a.dq, (head_row + at_row) * a.d, col, a.d, real ? o[j][0] * f : 0.f, real ? o[j][1] * f : 0.f,
+                         real ? o[j][2] * f : 0.f, real ? o[j][3] * f : 0.f);
+      }
+    }
+    for (uint64_t todo = __ballot(bad) & 0x0101010101010101ull; todo; todo &= todo - 1) {
+      const int r = 8 * wave + __builtin_ctzll(todo) / 8;
+      win_dq_row<IN>(a, b, h, r0 + r, __shfl(delta, r));
+    }
+    return;
   }
 
   int bad = 0;
@@ -694,26 +836,30 @@ __device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, in
   for (int e = 0; e < 2; ++e) dk[e] *= a.scale;
 }
 
-// Rows that window_dkv_kernel stages at a time, and its LDS: two stages of query and gradient rows, then their
-// statistics.
-template <int IN>
-__host__ __device__ constexpr int win_rows() { return IN == F32 ? 32 : 64; }
-template <int P, int IN>
+// Rows that window_dkv_kernel stages at a time, and its LDS: two stages of query and gradient rows and their statistics
+// (shared: one stage a wave).
+template <int IN, bool SHARE>
+__host__ __device__ constexpr int win_staged_rows() { return IN == F32 || SHARE ? 32 : 64; }
+template <int P, int IN, bool SHARE>
 __host__ __device__ constexpr int win_dkv_lds() {
-  return 2 * (2 * win_rows<IN>() * P * (IN == F32 ? 4 : 2) + 2 * win_rows<IN>() * 4);
+  const int rows = win_staged_rows<IN, SHARE>(), stage = 2 * rows * P * (IN == F32 ? 4 : 2) + 2 * rows * 4;
+  if (!SHARE) return 2 * stage;
+  return 4 * stage > 4 * win_join_floats<P>() ? 4 * stage : 4 * win_join_floats<P>();
 }
 
 // dk and dv: one workgroup per 128 keys of a key head (32 a wave) walks over the rows that see them within the window,
 // for every head of the group; the rows behind the window of a sink go to workgroups of their own (far), whose
 // sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.
-template <int P, int IN>
+template <int P, int IN, bool SHARE>
 __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
-  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_rows<IN>(), NSUB = BQ / 32;
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_staged_rows<IN, SHARE>(),
+                NSUB = BQ / 32, TILE = win_rows<SHARE>(), THREADS = SHARE ? 64 : 256;
   constexpr int STAGE = 2 * BQ * CH;  // 16-byte units of a stage
   extern __shared__ uint4 win_lds[];
-  float* const stats = reinterpret_cast<float*>(win_lds + 2 * STAGE);  // [stage][lse, delta][BQ]
+  constexpr int STAGES = SHARE ? 4 : 2;  // of the waves, or of two tiles
+  float* const stats = reinterpret_cast<float*>(win_lds + STAGES * STAGE);  // [stage][lse, delta][BQ]
   const int kv = a.heads / a.group;
-  const int far_items = a.sink_tiles * a.far_chunks, items = far_items + a.tiles;
+  const int far_items = a.sink_tiles * a.far_chunks, items = far_items + a.key_tiles;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
   const int item = id % items, bh = id / items, b = bh / kv, hk = bh % kv;
   const bool far = item < far_items;
@@ -721,7 +867,7 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
   const int tile = far ? item % a.sink_tiles : item - far_items;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int len = win_length(a, b);
-  const int k0 = tile * WIN_ROWS, kw = k0 + 32 * wave, key = kw + (lane & 31);
+  const int k0 = tile * TILE, kw = k0 + (SHARE ? 0 : 32 * wave), key = kw + (lane & 31);
 
   // rows [lo, hi] to walk over
   int lo, hi;
@@ -731,7 +877,7 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
     if (lo < k0 + a.window) lo = k0 + a.window;
   } else {
     lo = k0;
-    hi = k0 + WIN_ROWS - 1 < a.n - a.window ? k0 + WIN_ROWS - 1 + a.window - 1 : a.n - 1;
+    hi = k0 + TILE - 1 < a.n - a.window ? k0 + TILE - 1 + a.window - 1 : a.n - 1;
   }
   if (hi > len - 1) hi = len - 1;
 
@@ -753,51 +899,58 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
       win_keep<IN>(kf[s], key < len);
       win_keep<IN>(vf[s], key < len);
     }
-    const int first = lo / BQ * BQ, count = (hi / BQ - lo / BQ + 1) * a.group;
+    const int first = lo / BQ * BQ, per_head = hi / BQ - lo / BQ + 1, count = per_head * a.group;
     const float lift = __builtin_amdgcn_logf(a.lift);
-    WinStage<P, IN, BQ> qst, gst;
+    WinStage<P, IN, BQ, THREADS> qst, gst;
     qst.init(a.q, a.d);
     gst.init(a.go, a.dv);
     float stat = 0.f;
-    // the tile to be loaded next, the one in registers, the one to be computed
-    int load_row = first, load_head = hk * a.group, put_row = first, row0 = first;
-    auto load = [&]() {
-      qst.load(rows_at<ES>(a.q, b, load_head, load_row), len - load_row);
-      gst.load(rows_at<ES>(a.go, b, load_head, load_row), len - load_row);
-      if (threadIdx.x < 2 * BQ) {
-        const int row = load_row + threadIdx.x % BQ;
-        const float* from = static_cast<int>(threadIdx.x) < BQ ? a.lse : a.delta;
-        stat = row < len ? from[(static_cast<int64_t>(b) * a.heads + load_head) * a.n + row] : 0.f;
-      }
-      load_row += BQ;
-      if (load_row > hi) {
-        load_row = first;
-        ++load_head;
+    const int self = threadIdx.x % THREADS;
+    auto row_of = [&](int it) { return first + it % per_head * BQ; };
+    auto load = [&](int it) {
+      const int row0 = row_of(it), h = hk * a.group + it / per_head;
+      qst.load(rows_at<ES>(a.q, b, h, row0), len - row0);
+      gst.load(rows_at<ES>(a.go, b, h, row0), len - row0);
+      if (self < 2 * BQ) {
+        const int row = row0 + self % BQ;
+        const float* from = self < BQ ? a.lse : a.delta;
+        stat = row < len ? from[(static_cast<int64_t>(b) * a.heads + h) * a.n + row] : 0.f;
       }
     };
-    auto put = [&](int stage) {
-      qst.put(win_lds + stage * STAGE, len - put_row);
-      gst.put(win_lds + stage * STAGE + BQ * CH, len - put_row);
-      if (threadIdx.x < 2 * BQ) stats[stage * 2 * BQ + threadIdx.x] = stat;
-      put_row = put_row + BQ > hi ? first : put_row + BQ;
+    auto put = [&](int it, int stage) {
+      qst.put(win_lds + stage * STAGE, len - row_of(it));
+      gst.put(win_lds + stage * STAGE + BQ * CH, len - row_of(it));
+      if (self < 2 * BQ) stats[stage * 2 * BQ + self] = stat;
     };
-    load();
-    put(0);
-    if (count > 1) load();
-    for (int it = 0; it < count; ++it) {
+    const int start = SHARE ? wave : 0, step = SHARE ? 4 : 1;
+    constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
+    if (AHEAD && start < count) load(start);
+    if constexpr (!SHARE) {
+      put(0, 0);
+      if (count > 1) load(1);
+    }
+    for (int it = start; it < count; it += step) {
       // the accumulators stay in accumulation registers (the compiler else moves all of them there and back)
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         win_pin(dk[mt]);
         win_pin(dv[mt]);
       }
-      __syncthreads();
-      if (it + 1 < count) put((it + 1) & 1);
-      if (it + 2 < count) load();
-      const uint4 *qs = win_lds + (it & 1) * STAGE, *gs = qs + BQ * CH;
-      const floatx4* st = reinterpret_cast<const floatx4*>(stats + (it & 1) * 2 * BQ);
-      const int q0 = row0;
-      row0 = row0 + BQ > hi ? first : row0 + BQ;
+      int stage = wave;
+      if (!AHEAD) load(it);
+      win_sync<SHARE>();
+      if constexpr (SHARE) {
+        put(it, wave);
+        win_sync<SHARE>();
+        if (AHEAD && it + step < count) load(it + step);
+      } else {  // stage `it` is written, the other one read
+        stage = it & 1;
+        if (it + 1 < count) put(it + 1, stage ^ 1);
+        if (it + 2 < count) load(it + 2);
+      }
+      const uint4 *qs = win_lds + stage * STAGE, *gs = qs + BQ * CH;
+      const floatx4* st = reinterpret_cast<const floatx4*>(stats + stage * 2 * BQ);
+      const int q0 = row_of(it);
       const bool some = far ? kw < a.sinks && q0 + BQ - 1 - kw >= a.window
                             : q0 + BQ - 1 >= kw && q0 - (kw + 31) < a.window;
       if (!some) continue;
@@ -807,20 +960,28 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
       for (int sub = 0; sub < NSUB; ++sub) {
         // every operand is read well before its product: a compute unit holds one wave a SIMD, which has nothing else to
         // do while it waits
-        WinFrag<IN> qa[P / 16], ga[P / 16], qc[MT], gc[MT];
-#pragma unroll
-        for (int s = 0; s < P / 16; ++s) {
-          qa[s] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
-          ga[s] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        // (fp32 products take eight times as long as their operands' reads: those are read as they come)
+        constexpr bool EARLY = IN != F32;
+        WinFrag<IN> qa[EARLY ? P / 16 : 1], ga[EARLY ? P / 16 : 1], qc[MT], gc[MT];
         floatx16 x, g;
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
+        if constexpr (EARLY) {
+#pragma unroll
+          for (int s = 0; s < P / 16; ++s) {
+            qa[s] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
+            ga[s] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
 #pragma unroll
         for (int s = 0; s < P / 16; ++s) {
-          win_mma<IN>(x, qa[s], kf[s]);
-          win_mma<IN>(g, ga[s], vf[s]);
+          if constexpr (!EARLY) {
+            qa[0] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
+            ga[0] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
+          }
+          win_mma<IN>(x, qa[EARLY ? s : 0], kf[s]);
+          win_mma<IN>(g, ga[EARLY ? s : 0], vf[s]);
         }
         floatx4 lse[4], delta[4];
 #pragma unroll
@@ -828,12 +989,14 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
           lse[r] = st[8 * sub + 2 * r + hh];
           delta[r] = st[BQ / 4 + 8 * sub + 2 * r + hh];
         }
+        if constexpr (EARLY) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          gc[mt] = win_read_columns<P, IN>(gs, 32 * sub, mt, lane);
-          qc[mt] = win_read_columns<P, IN>(qs, 32 * sub, mt, lane);
+          for (int mt = 0; mt < MT; ++mt) {
+            gc[mt] = win_read_columns<P, IN>(gs, 32 * sub, mt, lane);
+            qc[mt] = win_read_columns<P, IN>(qs, 32 * sub, mt, lane);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, lift - lse[i >> 2][i & 3]));
@@ -855,25 +1018,33 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
-          WinFrag<IN> gn[MT], qn[MT];
-          if (t == 0) {
+          WinFrag<IN> gn[EARLY ? MT : 1], qn[EARLY ? MT : 1];
+          if constexpr (EARLY) {
+            if (t == 0) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              gn[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16, mt, lane);
-              qn[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16, mt, lane);
+              for (int mt = 0; mt < MT; ++mt) {
+                gn[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16, mt, lane);
+                qn[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16, mt, lane);
+              }
             }
+            __builtin_amdgcn_sched_barrier(0);
           }
-          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
+            if constexpr (!EARLY) {
+              gc[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16 * t, mt, lane);
+              qc[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16 * t, mt, lane);
+            }
             win_mma<IN>(dv[mt], gc[mt], p);
             win_mma<IN>(dk[mt], qc[mt], ds);
           }
-          if (t == 0) {
+          if constexpr (EARLY) {
+            if (t == 0) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              gc[mt] = gn[mt];
-              qc[mt] = qn[mt];
+              for (int mt = 0; mt < MT; ++mt) {
+                gc[mt] = gn[mt];
+                qc[mt] = qn[mt];
+              }
             }
           }
         }
@@ -881,55 +1052,40 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
     }
   }
 
-  int bad = 0;
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bad |= !(win_finite(dk[mt][i]) && win_finite(dv[mt][i]));
-  bad = key < len ? bad : 0;
-  bad |= __shfl_xor(bad, 32);
   // sums to be added to others' (the sinks of a call with rows behind their window)
-  const bool part = a.far_chunks > 0 && key < a.sink_rows;
-  const int64_t part_row = ((static_cast<int64_t>(bh) * (a.far_chunks + 1) + chunk + 1) * a.sink_rows + key) *
-                           (a.d + a.dv);
-  const int64_t out_row = static_cast<int64_t>(bh) * a.n + key;
   const float f = a.scale * a.drop;
-  if (!bad && (part || (!far && key < a.n))) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int col = 32 * mt + 8 * r + 4 * hh;
-        if (part) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (col + e < a.d) a.part[part_row + col + e] = dk[mt][4 * r + e] * f;
-            if (col + e < a.dv) a.part[part_row + a.d + col + e] = dv[mt][4 * r + e] * a.drop;
-          }
-        } else {
-          if (col < a.d)
-            win_store4<IN>(a.dk, out_row * a.d, col, a.d, dk[mt][4 * r] * f, dk[mt][4 * r + 1] * f,
-                           dk[mt][4 * r + 2] * f, dk[mt][4 * r + 3] * f);
-          if (col < a.dv)
-            win_store4<IN>(a.dv_out, out_row * a.dv, col, a.dv, dv[mt][4 * r] * a.drop, dv[mt][4 * r + 1] * a.drop,
-                           dv[mt][4 * r + 2] * a.drop, dv[mt][4 * r + 3] * a.drop);
-        }
-      }
-  }
-  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1) {
-    const int j = kw + __builtin_ctzll(todo);
+  auto part_at = [&](int j) {
+    return ((static_cast<int64_t>(bh) * (a.far_chunks + 1) + chunk + 1) * a.sink_rows + j) * (a.d + a.dv);
+  };
+  auto is_part = [&](int j) { return a.far_chunks > 0 && j < a.sink_rows; };
+  // 4 columns of key j's dk (value 0) or dv (1), where this workgroup has any to give
+  auto store4 = [&](int j, int value, int col, float x0, float x1, float x2, float x3) {
+    const int width = value ? a.dv : a.d;
+    if (col >= width) return;
+    if (is_part(j)) {
+      float* to = a.part + part_at(j) + (value ? a.d : 0);
+      to[col] = x0;
+      if (col + 1 < width) to[col + 1] = x1;
+      if (col + 2 < width) to[col + 2] = x2;
+      if (col + 3 < width) to[col + 3] = x3;
+    } else if (!far && j < a.n) {
+      win_store4<IN>(value ? a.dv_out : a.dk, (static_cast<int64_t>(bh) * a.n + j) * width, col, width, x0, x1, x2, x3);
+    }
+  };
+  // key j over its visible rows again, by a wave
+  auto again = [&](int j) {
     float sk[2], sv[2];
     int from = lo, to = hi;
     if (far) {
-      if (j >= a.sinks) continue;
+      if (j >= a.sinks) return;
       if (from < j + a.window) from = j + a.window;
     } else {
       from = j;
       if (j < a.n - a.window && to > j + a.window - 1) to = j + a.window - 1;
     }
     win_dkv_row<IN>(a, b, hk, j, from, to, sk, sv);
-    const bool pj = a.far_chunks > 0 && j < a.sink_rows;
-    const int64_t pr = ((static_cast<int64_t>(bh) * (a.far_chunks + 1) + chunk + 1) * a.sink_rows + j) * (a.d + a.dv);
+    const bool pj = is_part(j);
+    const int64_t pr = part_at(j);
     const int64_t orow = static_cast<int64_t>(bh) * a.n + j;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -947,7 +1103,59 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
           store_elem(a.dv_out, orow * a.dv + col, IN, sv[e]);
       }
     }
+    };
+  if constexpr (SHARE) {
+    float* red = reinterpret_cast<float*>(win_lds);
+    const float one[4] = {1.f, 1.f, 1.f, 1.f};
+    const int j = k0 + threadIdx.x / 8;
+    floatx4 o[2][MT];
+    int bad = 0;
+#pragma unroll
+    for (int value = 0; value < 2; ++value) {
+      __syncthreads();
+      win_join_put<P>(red, value ? dv : dk, wave, lane);
+      __syncthreads();
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        o[value][mt] = win_join_get<P>(red, 32 * mt + 4 * (threadIdx.x & 7), one);
+        bad |= win_bad4(o[value][mt]);
+      }
+    }
+    bad = j < len ? bad : 0;
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) bad |= __shfl_xor(bad, x);
+    if (!bad) {
+#pragma unroll
+      for (int value = 0; value < 2; ++value)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const floatx4 y = o[value][mt] * (value ? a.drop : f);
+          store4(j, value, 32 * mt + 4 * (threadIdx.x & 7), y[0], y[1], y[2], y[3]);
+        }
+    }
+    for (uint64_t todo = __ballot(bad) & 0x0101010101010101ull; todo; todo &= todo - 1)
+      again(k0 + 8 * wave + __builtin_ctzll(todo) / 8);
+    return;
   }
+  int bad = 0;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) bad |= !(win_finite(dk[mt][i]) && win_finite(dv[mt][i]));
+  bad = key < len ? bad : 0;
+  bad |= __shfl_xor(bad, 32);
+  if (!bad) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = 32 * mt + 8 * r + 4 * hh;
+        store4(key, 0, col, dk[mt][4 * r] * f, dk[mt][4 * r + 1] * f, dk[mt][4 * r + 2] * f, dk[mt][4 * r + 3] * f);
+        store4(key, 1, col, dv[mt][4 * r] * a.drop, dv[mt][4 * r + 1] * a.drop, dv[mt][4 * r + 2] * a.drop,
+               dv[mt][4 * r + 3] * a.drop);
+      }
+  }
+  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1) again(kw + __builtin_ctzll(todo));
 }
 
 // dk and dv of the sinks: their tile's sums and the far chunks', in order.  One thread a column.

@@ -60,6 +60,48 @@ def test_outputs_and_gradients(b, h, hk, n, d, dv, window, sinks, lengths, dtype
     check(run(q, k, v, go, **kw), ref.window_attention(q, k, v, grad=go, **kw))
 
 
+WIDE = [  # many heads: tiles of 128 rows
+    (4, 32, 32, 400, 64, 64, 100, 4, None),
+    (2, 32, 16, 1030, 32, 32, 1100, 0, None),
+    (8, 24, 8, 513, 40, 72, 33, 140, [513, 0, 1, 512, 128, 129, 300, 511]),
+    (4, 32, 32, 300, 128, 100, 90, 5, [300, 131, 299, 64]),
+    (4, 64, 32, 257, 96, 96, 64, 3, None),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,hk,n,d,dv,window,sinks,lengths", WIDE)
+def test_many_heads(b, h, hk, n, d, dv, window, sinks, lengths, dtype):
+    q, k, v, go = make(b, h, hk, n, d, dv, dtype)
+    kw = dict(window=window, sinks=sinks, lengths=lengths)
+    check(run(q, k, v, go, **kw), ref.window_attention(q, k, v, grad=go, **kw))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_heads_hide_infinities(dtype):
+    """test_hidden_infinities_stay_hidden on tiles of 128 rows: one key's value, one row's gradient."""
+    b, h, n, window, sinks = 8, 32, 300, 40, 3
+    q, k, v, go = make(b, h, h, n, 32, 32, dtype, seed=5)
+    kw = dict(window=window, sinks=sinks)
+    want = ref.window_attention(q, k, v, grad=go, **kw)
+    see = ref.visible(n, n, window, sinks)
+    v2, g2 = v.clone(), go.clone()
+    v2[3, 7, 100, 5] = math.inf
+    g2[4, 9, 200, 2] = math.nan
+    got = {name: x.cpu() for name, x in run(q, k, v2, g2, **kw).items()}
+    rows, keys = see[:, 100], (see & see[:, 100][:, None]).any(0)
+    assert not torch.isfinite(got["out"][3, 7, 100, 5]) and not torch.isfinite(got["dv"][4, 9, 190, 2])
+    for name in ("out", "dq"):
+        assert ref.over(got[name][3, 7][~rows], tuple(t[3, 7][~rows] for t in want[name])) <= 1.0
+        other = torch.arange(n) != 200
+        assert ref.over(got[name][4, 9][other], tuple(t[4, 9][other] for t in want[name])) <= 1.0
+    for name in ("dk", "dv"):
+        assert ref.over(got[name][3, 7][~keys], tuple(t[3, 7][~keys] for t in want[name])) <= 1.0
+        assert ref.over(got[name][4, 9][~see[200]], tuple(t[4, 9][~see[200]] for t in want[name])) <= 1.0
+    for name in want:
+        assert ref.over(got[name][5], tuple(t[5] for t in want[name])) <= 1.0
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 4.0])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_scales(dtype, scale):
