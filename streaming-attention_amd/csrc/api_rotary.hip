@@ -167,8 +167,8 @@ int sta_head_rotary_backward(const void* q_grad, const void* k_grad, const void*
   hipStream_t s = static_cast<hipStream_t>(stream);
   launch_typed<true>(a, p, dtype, s);
   if (a.part[0] || a.part[1])
-    hipLaunchKernelGGL(sta::head_rotary_weight_kernel, dim3((d + 7) / 8, 2), dim3(256), 0, s, a.part[0], a.part[1],
-                       rows[0], rows[1], d, dq_weight, dk_weight, weight_dtype, weight_dtype);
+    hipLaunchKernelGGL(sta::head_rotary_weight_kernel, dim3((d + 3) / 4, 2), dim3(256), 0, s, a.part[0], a.part[1],
+                       rows[0], rows[1], d, dq_weight, dk_weight, weight_dtype);
   return check_launch();
 }
 

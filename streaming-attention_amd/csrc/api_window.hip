@@ -34,12 +34,18 @@ bool strides_ok(const int64_t* strides, int tensors, int dtype) {
   return true;
 }
 
-#ifndef WIN_SHARE
-#define WIN_SHARE 512
-#endif
-#ifndef WIN_KSHARE
-#define WIN_KSHARE 256
-#endif
+// The number of 128-row tiles below which the waves of a workgroup share 32 rows instead (the card has 256 compute
+// units).  Long windows gain more, short ones pay for staging a tile's keys four times; fp32 products take 16 times as
+// long, so balance counts for more.  Wide / shared, forward + gradients, 2048 rows a head:
+//   bf16, d = 64, window 256: 64 tiles 20+44 / 19+33 us, 192 19+64 / 18+64, 256 19+62 / 19+71; window 2048: 128 38+113 /
+//   21+58, 256 38+114 / 27+98, 512 51+182 / 45+192; d = 128: 128 55+177 / 33+98, 256 55+180 / 45+193, 512 76+275 / 87+380;
+//   fp32, d = 64, window 256: 256 41+177 / 42+174, 512 67+303 / 78+325; window 2048: 256 162+534 / 99+348, 768 397+1203 /
+//   285+1035
+int64_t share_below(int es, int64_t window) {
+  if (es == 4) return window >= 1024 ? 1024 : 448;
+  return window >= 1024 ? 256 : 144;
+}
+
 // The shape part of the arguments; STA_OK or what is wrong with it.
 int window_shape(sta::WinArgs& a, int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv,
                  float scale, int64_t window, int64_t sinks) {
@@ -62,8 +68,8 @@ int window_shape(sta::WinArgs& a, int dtype, int64_t batch, int heads, int kv_he
   // above 0: a hidden pair's logit, -inf, stays one times c
   a.c = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-37f);
   const int64_t wide = (n + sta::WIN_ROWS - 1) / sta::WIN_ROWS;
-  a.share = batch * heads * wide < WIN_SHARE;
-  a.key_share = batch * kv_heads * wide < WIN_KSHARE;
+  a.share = batch * heads * wide < share_below(es, a.window);
+  a.key_share = batch * kv_heads * wide < share_below(es, a.window);
   a.tiles = static_cast<int>(a.share ? (n + 31) / 32 : wide);
   a.key_tiles = static_cast<int>(a.key_share ? (n + 31) / 32 : wide);
   a.lift = a.drop = 1.f;

@@ -136,12 +136,18 @@ struct WinStage {
   }
   // the tile at `row`, `left` >= 1 of its rows being there; a row has at least 16 bytes
   __device__ __forceinline__ void load(const char* row, int left) {
+    uint32_t off[COUNT];
+#pragma unroll
+    for (int i = 0; i < COUNT; ++i) off[i] = at[EVEN ? 0 : i];
+    if (left < ROWS) {
+#pragma unroll
+      for (int i = 0; i < COUNT; ++i)
+        off[i] -= static_cast<uint32_t>(max(0, min(unit(i) / CH, ROWS - 1) - left + 1) * pitch);
+    }
 #pragma unroll
     for (int i = 0; i < COUNT; ++i) {
       const char* from = EVEN ? row + static_cast<int64_t>(i * (THREADS / CH)) * pitch : row;
-      uint32_t off = at[EVEN ? 0 : i];
-      if (left < ROWS) off -= static_cast<uint32_t>(max(0, min(unit(i) / CH, ROWS - 1) - left + 1) * pitch);
-      u[i] = rows_load16(from + static_cast<int32_t>(off));
+      u[i] = rows_load16(from + static_cast<int32_t>(off[i]));
     }
   }
   __device__ __forceinline__ void put(uint4* lds, int left) const {
