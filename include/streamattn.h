@@ -562,8 +562,8 @@ int sta_ring_extend(const void* k, const void* v, int dtype, int storage, int64_
                     void* stream);
 
 /*
- * The slots' contents: keys_out [streams][kv_heads][sinks + window][d], values_out [..][dv] in dtype (zero where no
- * token is), positions [streams][sinks + window] (-1 there).
+ * The slots' contents: keys_out [streams][kv_heads][sinks + window][d], values_out [..][dv] in dtype (16-byte aligned;
+ * zero where no token is), positions [streams][sinks + window] (-1 there).
  */
 int sta_ring_items(int dtype, int storage, int64_t streams, int kv_heads, int d, int dv, int64_t window,
                    int64_t sinks, const void* keys, const void* values, const void* key_exponents,

@@ -189,7 +189,8 @@ int sta_ring_items(int dtype, int storage, int64_t streams, int kv_heads, int d,
                    int64_t sinks, const void* keys, const void* values, const void* key_exponents,
                    const void* value_exponents, const int32_t* counts, void* keys_out, void* values_out,
                    int32_t* positions, void* stream) {
-  if (!counts || !keys_out || !values_out || !positions) return STA_ERR_ARG;
+  if (!counts || !keys_out || !values_out || !positions || !aligned16(keys_out) || !aligned16(values_out))
+    return STA_ERR_ARG;
   if (!dtype_ok(dtype) || !storage_ok(storage, dtype)) return STA_ERR_DTYPE;
   if (!cache_ok(keys, values, key_exponents, value_exponents, storage)) return STA_ERR_ARG;
   sta::RingArgs a;

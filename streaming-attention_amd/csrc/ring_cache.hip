@@ -595,7 +595,7 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
     const int slot = 32 * tile + threadIdx.x;
     token[threadIdx.x] = slot < a.slots ? ring_token(a, slot, n, take) : -1;
   }
-  __syncthreads();
+  if (!__syncthreads_or(threadIdx.x < 32 && token[threadIdx.x] >= 0)) return;  // no token falls into this tile
   const int64_t at = static_cast<int64_t>(sh) * a.tiles + tile;
   uint8_t* keys = a.keys + at * ring_tile_bytes(a.nbk, ST);
   uint8_t* values = a.values + at * ring_tile_bytes(a.nbv, ST);
@@ -728,12 +728,38 @@ __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void*
   const uint8_t* kp = a.keys + at * ring_tile_bytes(a.nbk, ST);
   const uint8_t* vp = a.values + at * ring_tile_bytes(a.nbv, ST);
   const int live = min(32, a.slots - 32 * tile);  // slots of the tile
+  const bool some = 32 * tile < n;                // one of them holds a token
   auto elem = [&](const uint8_t* p, int e) -> uint32_t {
     if constexpr (ST == F32) return reinterpret_cast<const uint32_t*>(p)[e];
     return reinterpret_cast<const uint16_t*>(p)[e];
   };
   auto store_rows = [&](void* out, int width) {
+    constexpr int ES = Q == F32 ? 4 : 2, E = 16 / ES;
     const int64_t base = (static_cast<int64_t>(sh) * a.slots + 32 * tile) * width;
+    if (width % E == 0) {  // 16 bytes a thread
+      const int units = width / E;
+      for (int i = threadIdx.x; i < live * units; i += 256) {
+        const int r = i / units, col = (i - r * units) * E;
+        const bool held = 32 * tile + r < n;
+        uint4 w;
+        if constexpr (ST == RING_F4) {
+          float f[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] = held ? __uint_as_float(rows[r * PITCH + col + e]) : 0.f;
+          w = rows_pack<Q>(f);
+        } else {
+          uint32_t f[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) f[e] = held ? rows[r * PITCH + col + e] : 0u;
+          if constexpr (ES == 4)
+            w = uint4{f[0], f[1], f[2], f[3]};
+          else
+            w = uint4{f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16};
+        }
+        reinterpret_cast<uint4*>(static_cast<char*>(out) + base * ES)[i] = w;
+      }
+      return;
+    }
     for (int i = threadIdx.x; i < live * width; i += 256) {
       const int r = i / width, col = i - r * width;
       const uint32_t w = 32 * tile + r < n ? rows[r * PITCH + col] : 0u;
@@ -745,7 +771,7 @@ __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void*
         static_cast<uint16_t*>(out)[base + i] = static_cast<uint16_t>(w);
     }
   };
-  for (int i = threadIdx.x; i < 128 * a.nbk; i += 256) {  // 8 dimensions of a slot a thread, in the cache's order
+  for (int i = threadIdx.x; some && i < 128 * a.nbk; i += 256) {  // 8 dimensions of a slot a thread, in the cache's order
     const int lane = i & 63, u = i >> 6, half = u / a.nbk, b = u - half * a.nbk;
     const int r = 16 * half + (lane & 15), col = 32 * b + 8 * (lane >> 4);
     if constexpr (ST == RING_F4) {
@@ -763,7 +789,7 @@ __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void*
   __syncthreads();
   store_rows(keys, a.d);
   __syncthreads();
-  for (int i = threadIdx.x; i < 64 * (ST == RING_F4 ? a.nbv : 2 * a.nbv); i += 256) {  // 8 slots of a column a thread
+  for (int i = threadIdx.x; some && i < 64 * (ST == RING_F4 ? a.nbv : 2 * a.nbv); i += 256) {  // 8 slots of a column a thread
     const int lane = i & 63, ct = i >> 6, g = lane >> 4;
     const int col = ST == RING_F4 ? 32 * ct + (lane & 15) : 16 * ct + (lane & 15);
 #pragma unroll
