@@ -84,12 +84,19 @@ __device__ __forceinline__ int ring_exponent(uint32_t largest) {
   const int e = static_cast<int>(largest >> 23) - 2;
   return e < 1 ? 1 : e;
 }
-// the 4-bit code of x in a block with exponent byte e
-__device__ __forceinline__ uint32_t ring_code(float x, int e) {
+// the 4-bit codes of two values in a block with exponent byte e: rounded to the nearest, ties to even, 6 at most
+__device__ __forceinline__ uint32_t ring_codes(float x, float y, int e) {
   if (e == 255) return 0u;
-  const float y = x * __uint_as_float(static_cast<uint32_t>(254 - e) << 23), m = fabsf(y);
-  const uint32_t c = (m > 0.25f) + (m >= 0.75f) + (m > 1.25f) + (m >= 1.75f) + (m > 2.5f) + (m >= 3.5f) + (m > 5.f);
-  return y < 0.f ? c | 8u : c;
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x, y, ring_power(e), 0);
+}
+// and of eight, in order
+__device__ __forceinline__ uint32_t ring_codes(const float (&x)[8], int e) {
+  if (e == 255) return 0u;
+  const float power = ring_power(e);
+  uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], power, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], power, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], power, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], power, 3);
 }
 __device__ __forceinline__ float ring_decode(uint32_t code) {
   const float m[8] = {0.f, 0.5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
@@ -211,7 +218,7 @@ __device__ void ring_put(const RingArgs& a, int s, int hk, int slot) {
     uint8_t* at = a.keys + tile * ring_tile_bytes(a.nbk, ST) + ring_key_at(r, col, a.nbk, ST);
     if constexpr (ST == RING_F4) {
       float x[8];
-      uint32_t top = 0u, codes = 0u;
+      uint32_t top = 0u;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         x[j] = col + j < a.d ? load_elem(row, col + j, Q) : 0.f;
@@ -220,9 +227,7 @@ __device__ void ring_put(const RingArgs& a, int s, int hk, int slot) {
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
       const int e = ring_exponent(top);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) codes |= ring_code(x[j], e) << (4 * j);
-      *reinterpret_cast<uint32_t*>(at) = codes;
+      *reinterpret_cast<uint32_t*>(at) = ring_codes(x, e);
       if ((t & 3) == 0)
         a.kexp[tile * ring_key_exp_bytes(a.nbk, ST) + ring_key_exp_at(r, t >> 2, a.nbk)] = static_cast<uint8_t>(e);
     } else {
@@ -240,7 +245,7 @@ __device__ void ring_put(const RingArgs& a, int s, int hk, int slot) {
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), o)));
       const int e = ring_exponent(top);
-      values[ring_value_at(r, c0, a.nbv, ST)] = static_cast<uint8_t>(ring_code(x0, e) | ring_code(x1, e) << 4);
+      values[ring_value_at(r, c0, a.nbv, ST)] = static_cast<uint8_t>(ring_codes(x0, x1, e));
       if ((t & 15) == 0)
         a.vexp[tile * ring_value_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, b, a.nbv)] = static_cast<uint8_t>(e);
     } else {
@@ -607,7 +612,7 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
     uint8_t* to = keys + ring_key_at(r, col, a.nbk, ST);
     if constexpr (ST == RING_F4) {
       float x[8];
-      uint32_t top = 0u, codes = 0u;
+      uint32_t top = 0u;
       constexpr int E = 16 / ES;
 #pragma unroll
       for (int c = 0; c < 8 / E; ++c) {
@@ -622,10 +627,8 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
       const int e = ring_exponent(top);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) codes |= ring_code(x[j], e) << (4 * j);
       if (p >= 0) {
-        *reinterpret_cast<uint32_t*>(to) = codes;
+        *reinterpret_cast<uint32_t*>(to) = ring_codes(x, e);
         if ((u & 3) == 0)
           a.kexp[at * ring_key_exp_bytes(a.nbk, ST) + ring_key_exp_at(r, u >> 2, a.nbk)] = static_cast<uint8_t>(e);
       }
@@ -664,8 +667,9 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 1)));
       top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 2)));
       const int e = ring_exponent(top);
+      const uint32_t codes = ring_codes(x, e);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) to[j] = ring_code(x[j], e);
+      for (int j = 0; j < 8; ++j) to[j] = (codes >> (4 * j)) & 15u;
       if (p >= 0 && (u & 3) == 0)
         a.vexp[at * ring_value_exp_bytes(a.nbv, ST) + ring_value_exp_at(r, u >> 2, a.nbv)] = static_cast<uint8_t>(e);
     }
