@@ -1174,6 +1174,7 @@ __global__ __launch_bounds__(256) void window_sink_kernel(const WinArgs a) {
   if (bh >= static_cast<int64_t>(a.batch) * (a.heads / a.group)) return;
   const int64_t in = at % per;
   float s = 0.f;
+#pragma unroll 8
   for (int c = 0; c <= a.far_chunks; ++c) s += a.part[(bh * (a.far_chunks + 1) + c) * per + in];
   const int64_t row = bh * a.n + in / width;
   const int col = static_cast<int>(in % width);

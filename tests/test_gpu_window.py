@@ -49,6 +49,8 @@ CASES = [  # b h hk n d dv window sinks lengths
     (1, 1, 1, 700, 96, 80, 128, 33, [650]),
     (1, 1, 1, 1030, 32, 64, 200, 4, None),
     (2, 1, 1, 260, 5, 3, 17, 129, [260, 131]),
+    (1, 2, 2, 1400, 64, 64, 100, 4, None),
+    (2, 8, 2, 700, 33, 40, 64, 70, [700, 333]),
 ]
 
 
