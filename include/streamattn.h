@@ -525,7 +525,8 @@ int sta_head_rotary_backward(const void* q_grad, const void* k_grad, const void*
 /*
  * Token cache of windowed attention, for streams in lockstep: per stream and key head sinks + window slots; token
  * p < sinks in slot p, the others in a ring, token p in slot sinks + (p - sinks) % window.  counts [streams][kv_heads]
- * (device) is the number of tokens so far (equal over a stream's heads).
+ * (device) is the number of tokens so far (equal over a stream's heads); one that would pass 2^31 - 1 goes back by whole
+ * windows (the slots keep their turn), a negative one is taken as 0.
  *   storage: the element type's own code, or STA_STORAGE_FP4: each block of 32 columns of a token as 4-bit floats
  *   (0, 0.5, 1, 1.5, 2, 3, 4, 6 and signs; nearest, ties to the even code, larger values 6) times
  *   2^(floor(log2(largest magnitude)) - 2) >= 2^-126; a block with a value that is not finite is NaN.

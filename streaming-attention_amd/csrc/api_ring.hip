@@ -64,6 +64,15 @@ int splits_of(const sta::RingArgs& a) {
   return static_cast<int>(want < 1 ? 1 : want);
 }
 
+// A workgroup a tile of the cache, in rows of 2^20 (a million tokens of 512 key heads are 2^24 tiles, whose threads one
+// dimension of a launch does not take).
+bool tile_grid(const sta::RingArgs& a, dim3& g) {
+  const int64_t tiles = static_cast<int64_t>(a.streams) * a.kv * a.tiles, x = tiles < 1 << 20 ? tiles : 1 << 20;
+  const int64_t y = (tiles + x - 1) / x;
+  g = dim3(static_cast<unsigned>(x), static_cast<unsigned>(y));
+  return y <= 65535;
+}
+
 template <int ST, int Q>
 int by_keys(const sta::RingArgs& a, hipStream_t s) {
   switch (a.nbk) {
@@ -137,7 +146,8 @@ int sta_ring_attention(const void* q, const void* k, const void* v, int dtype, i
     a.v = rows_of(v, vs, es);
   }
   a.scale = scale;
-  a.c = std::fabs(scale) * 1.44269504088896340736f;
+  // above 0: what a wave without tiles has, -3e38, stays far below a logit times c
+  a.c = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-37f);
   a.keys = static_cast<uint8_t*>(keys);
   a.values = static_cast<uint8_t*>(values);
   a.kexp = static_cast<uint8_t*>(key_exponents);
@@ -158,8 +168,7 @@ int sta_ring_extend(const void* k, const void* v, int dtype, int storage, int64_
   if (!cache_ok(keys, values, key_exponents, value_exponents, storage)) return STA_ERR_ARG;
   sta::RingFill f{};
   if (const int st = ring_shape(f.a, streams, kv_heads, kv_heads, d, dv, window, sinks)) return st;
-  const int64_t grid = static_cast<int64_t>(f.a.streams) * f.a.kv * f.a.tiles;
-  if (rows < 1 || grid > 0x7fffffff) return STA_ERR_SHAPE;
+  if (rows < 1) return STA_ERR_SHAPE;
   if (rows > kMaxRingSlots) return STA_ERR_UNSUPPORTED;
   const int es = dtype == STA_F32 ? 4 : 2;
   f.a.k = rows_of(k, strides, es);
@@ -171,7 +180,8 @@ int sta_ring_extend(const void* k, const void* v, int dtype, int storage, int64_
   f.a.counts = counts;
   f.rows = static_cast<int>(rows);
   f.take = take;
-  const dim3 g(static_cast<unsigned>(grid));
+  dim3 g;
+  if (!tile_grid(f.a, g)) return STA_ERR_SHAPE;
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define STA_RING_EXTEND(ST, Q) hipLaunchKernelGGL((sta::ring_extend_kernel<ST, Q>), g, dim3(256), 0, s, f)
   if (storage == sta::RING_F4 && dtype == STA_F32) STA_RING_EXTEND(sta::RING_F4, sta::F32);
@@ -195,14 +205,13 @@ int sta_ring_items(int dtype, int storage, int64_t streams, int kv_heads, int d,
   if (!cache_ok(keys, values, key_exponents, value_exponents, storage)) return STA_ERR_ARG;
   sta::RingArgs a;
   if (const int st = ring_shape(a, streams, kv_heads, kv_heads, d, dv, window, sinks)) return st;
-  const int64_t grid = static_cast<int64_t>(a.streams) * a.kv * a.tiles;
-  if (grid > 0x7fffffff) return STA_ERR_SHAPE;
   a.keys = static_cast<uint8_t*>(const_cast<void*>(keys));
   a.values = static_cast<uint8_t*>(const_cast<void*>(values));
   a.kexp = static_cast<uint8_t*>(const_cast<void*>(key_exponents));
   a.vexp = static_cast<uint8_t*>(const_cast<void*>(value_exponents));
   a.counts = const_cast<int32_t*>(counts);
-  const dim3 g(static_cast<unsigned>(grid));
+  dim3 g;
+  if (!tile_grid(a, g)) return STA_ERR_SHAPE;
   hipStream_t s = static_cast<hipStream_t>(stream);
 #define STA_RING_ITEMS(ST, Q) \
   hipLaunchKernelGGL((sta::ring_items_kernel<ST, Q>), g, dim3(256), 0, s, a, keys_out, values_out, positions)

@@ -14,7 +14,8 @@ template <int ST, int Q, int NBK>
 int launch_ring(const sta::RingArgs& a, hipStream_t s) {
   const int64_t grid = static_cast<int64_t>(a.streams) * a.kv * a.chunks * a.nsplit;
   const int64_t heads = static_cast<int64_t>(a.streams) * a.heads;
-  if (grid <= 0 || grid > 0x7fffffff || heads > 0x7fffffff) return STA_ERR_SHAPE;
+  const bool join = a.nsplit > 1 || (a.append && a.chunks > 1);  // 512 threads a head
+  if (grid <= 0 || grid > sta::MAX_GROUPS || (join && heads > sta::MAX_GROUPS / 2)) return STA_ERR_SHAPE;
   const dim3 g(static_cast<unsigned>(grid));
   switch (a.nbv) {
     case 1: hipLaunchKernelGGL((sta::ring_attention_kernel<NBK, 1, ST, Q>), g, dim3(256), 0, s, a); break;
@@ -22,7 +23,7 @@ int launch_ring(const sta::RingArgs& a, hipStream_t s) {
     case 3: hipLaunchKernelGGL((sta::ring_attention_kernel<NBK, 3, ST, Q>), g, dim3(256), 0, s, a); break;
     default: hipLaunchKernelGGL((sta::ring_attention_kernel<NBK, 4, ST, Q>), g, dim3(256), 0, s, a);
   }
-  if (a.nsplit > 1 || (a.append && a.chunks > 1))
+  if (join)
     hipLaunchKernelGGL((sta::ring_join_kernel<Q>), dim3(static_cast<unsigned>(heads)), dim3(512), 0, s, a);
   return check_launch();
 }

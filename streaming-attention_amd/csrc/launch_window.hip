@@ -12,7 +12,7 @@ namespace sta_api {
 
 template <typename Kernel>
 static int launch(Kernel kernel, int64_t grid, int lds, const sta::WinArgs& a, hipStream_t s) {
-  if (grid <= 0 || grid > 0x7fffffff) return STA_ERR_SHAPE;
+  if (grid <= 0 || grid > sta::MAX_GROUPS) return STA_ERR_SHAPE;
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
@@ -36,7 +36,7 @@ int launch_window_backward(const sta::WinArgs& a, hipStream_t s) {
   const int64_t grid_q = static_cast<int64_t>(a.batch) * a.heads * a.tiles;
   const int64_t grid_k = bkv * (a.key_tiles + static_cast<int64_t>(a.sink_tiles) * a.far_chunks);
   const int64_t grid_s = (bkv * a.sink_rows * (a.d + a.dv) + 255) / 256;
-  if (grid_k > 0x7fffffff || grid_s > 0x7fffffff) return STA_ERR_SHAPE;
+  if (grid_q > sta::MAX_GROUPS || grid_k > sta::MAX_GROUPS || grid_s > sta::MAX_GROUPS) return STA_ERR_SHAPE;
   int st = a.share ? launch(sta::window_dq_kernel<P, IN, true>, grid_q, sta::win_lds_bytes<P, IN, true>(), a, s)
                    : launch(sta::window_dq_kernel<P, IN, false>, grid_q, sta::win_lds_bytes<P, IN, false>(), a, s);
   if (st != STA_OK) return st;

@@ -57,6 +57,28 @@ __device__ __forceinline__ int ring_slot(const RingArgs& a, int p) {
   return p < a.sinks ? p : a.sinks + (p - a.sinks) % a.window;
 }
 
+// tokens that a key head has taken
+__device__ __forceinline__ int ring_count(const RingArgs& a, int sh) {
+  const int n = a.counts[sh];
+  return n < 0 ? 0 : n;
+}
+// The count after `take` more tokens.  One that would pass 31 bits goes back by whole windows: the slots keep their turn
+// (window and sinks + window are at most 2^30, so it stays above them).
+__device__ __forceinline__ int ring_after(const RingArgs& a, int n, int take) {
+  constexpr int64_t most = 0x7fffffff;
+  int64_t end = static_cast<int64_t>(n) + take;
+  if (end > most) end -= (end - most + a.window - 1) / a.window * a.window;
+  return static_cast<int>(end);
+}
+
+// the key head and tile of a workgroup of a launch over tiles
+__device__ __forceinline__ bool ring_place(const RingArgs& a, int& sh, int& tile) {
+  const int64_t id = static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x;
+  sh = static_cast<int>(id / a.tiles);
+  tile = static_cast<int>(id - static_cast<int64_t>(sh) * a.tiles);
+  return sh < a.streams * a.kv;
+}
+
 // byte of dimension col (keys) or column col (values) of slot r of a tile; of 4-bit caches the byte that holds the
 // code (keys: low half for even dimensions, values: for the first 16 columns of a block)
 __device__ __forceinline__ int ring_key_at(int r, int col, int nb, int storage) {
@@ -326,8 +348,8 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
   const int s = sh / a.kv, hk = sh - s * a.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
 
-  const int n = a.counts[sh];
-  const int held = n + a.append < a.slots ? n + a.append : a.slots;
+  const int n = ring_count(a, sh);
+  const int held = n < a.slots - a.append ? n + a.append : a.slots;
   const int all = (held + 31) >> 5, per = (all + a.nsplit - 1) / a.nsplit;
   const int t0 = split * per, t1 = t0 + per < all ? t0 + per : all;
   if (a.append) {
@@ -514,7 +536,7 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
     }
   }
   // every thread has read the count; other workgroups read it only where ring_join_kernel counts
-  if (a.append && a.nsplit == 1 && a.chunks == 1 && threadIdx.x == 0) a.counts[sh] = n + 1;
+  if (a.append && a.nsplit == 1 && a.chunks == 1 && threadIdx.x == 0) a.counts[sh] = ring_after(a, n, 1);
 }
 
 // The splits' sums of a query head, 4 groups of 128 threads (a column each) over the splits, and the count of a step
@@ -558,11 +580,11 @@ __global__ __launch_bounds__(512) void ring_join_kernel(const RingArgs a) {
       den = 0.f;
       for (int i = 0; i < 8; ++i) den += wave_red[i];
       sum = red[threadIdx.x] + red[128 + threadIdx.x] + red[256 + threadIdx.x] + red[384 + threadIdx.x];
-      const bool empty = !a.append && a.counts[sh] == 0;
+      const bool empty = !a.append && ring_count(a, sh) == 0;
       store_elem(a.out, head * a.dv + threadIdx.x, Q, empty ? 0.f : sum / den);
     }
   }
-  if (a.append && h % a.group == 0 && threadIdx.x == 0) a.counts[sh] += 1;
+  if (a.append && h % a.group == 0 && threadIdx.x == 0) a.counts[sh] = ring_after(a, ring_count(a, sh), 1);
 }
 
 struct RingFill {
@@ -594,8 +616,9 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
   const RingArgs& a = f.a;
   __shared__ uint32_t vals[32 * 132];  // the tile's values (bits, or codes), 32 nbv + 1 a slot
   __shared__ int token[32];
-  const int sh = blockIdx.x / a.tiles, tile = blockIdx.x - sh * a.tiles, s = sh / a.kv, hk = sh - s * a.kv;
-  const int n = a.counts[sh], take = ring_take(f, s);
+  int sh, tile;
+  if (!ring_place(a, sh, tile)) return;
+  const int s = sh / a.kv, hk = sh - s * a.kv, n = ring_count(a, sh), take = ring_take(f, s);
   if (threadIdx.x < 32) {
     const int slot = 32 * tile + threadIdx.x;
     token[threadIdx.x] = slot < a.slots ? ring_token(a, slot, n, take) : -1;
@@ -716,7 +739,7 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
 // counts += the tokens that ring_extend_kernel has put in
 __global__ __launch_bounds__(256) static void ring_count_kernel(const RingFill f) {
   const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < f.a.streams * f.a.kv) f.a.counts[i] += ring_take(f, i / f.a.kv);
+  if (i < f.a.streams * f.a.kv) f.a.counts[i] = ring_after(f.a, ring_count(f.a, i), ring_take(f, i / f.a.kv));
 }
 
 // The slots' rows as they stand for: keys [streams][kv][slots][d], values [..][dv] in the element type, zero where no
@@ -726,8 +749,9 @@ template <int ST, int Q>
 __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void* keys, void* values, int* positions) {
   constexpr int PITCH = 129;
   __shared__ uint32_t rows[32 * PITCH];  // values: floats (4-bit), or the elements' bits
-  const int sh = blockIdx.x / a.tiles, tile = blockIdx.x - sh * a.tiles, s = sh / a.kv, hk = sh - s * a.kv;
-  const int n = a.counts[sh];
+  int sh, tile;
+  if (!ring_place(a, sh, tile)) return;
+  const int s = sh / a.kv, hk = sh - s * a.kv, n = ring_count(a, sh);
   const int64_t at = static_cast<int64_t>(sh) * a.tiles + tile;
   const uint8_t* kp = a.keys + at * ring_tile_bytes(a.nbk, ST);
   const uint8_t* vp = a.values + at * ring_tile_bytes(a.nbv, ST);

@@ -4,6 +4,9 @@
 
 namespace sta {
 
+// workgroups of 256 threads in one dimension of a launch, whose threads have to stay below 2^32
+constexpr int64_t MAX_GROUPS = (int64_t(1) << 24) - 1;
+
 // element strides; `aligned`: every row starts on 16 bytes
 struct Rows {
   const void* p;

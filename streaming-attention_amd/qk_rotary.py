@@ -168,9 +168,11 @@ def qk_norm_rotary(q: Tensor, k: Tensor, table: Tensor, *, q_weight: Optional[Te
     q [B,H,N,D] and k [B,Hkv,N,D] (any strides), [N,D] each, or one token of every stream, [S,H,D] and [S,Hkv,D];
     float32, bfloat16 or float16, D up to 256.  Weights [D] in that dtype or float32 (None: 1).
     positions: int32 or int64, [N] or [B,N] ([S] for [S,H,D]); None: 0 .. N-1.  A position outside the table makes its
-    rows (and gradients) NaN.  The results are dense in q's dtype.  Differentiable calls cannot be captured into a
-    graph (RuntimeError); qk_norm_rotary_backward can."""
+    rows (and gradients) NaN; the table takes no gradient.  The results are dense in q's dtype.  Differentiable calls
+    cannot be captured into a graph (RuntimeError); qk_norm_rotary_backward can."""
     call = _Call(q, k, table, q_weight, k_weight, positions, eps, interleaved)
+    if torch.is_grad_enabled() and table.requires_grad:
+        raise ValueError("table takes no gradient: pass table.detach()")
     if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight)):
         return _NormRotary.apply(q, k, q_weight, k_weight, table, positions, call)
     return call.forward(q, k, q_weight, k_weight)

@@ -99,7 +99,9 @@ def _rows(x: Tensor) -> Tensor:
     """x itself where the kernels can walk its rows (contiguous last dimension, rows at most 2^24 bytes apart), else a
     dense copy."""
     near = x.stride(2) * x.element_size() <= 1 << 24
-    return x if near and (x.stride(3) == 1 or x.shape[3] == 1) else x.contiguous()
+    if near and (x.stride(3) == 1 or x.shape[3] == 1):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)  # strides of dimensions of one element too
 
 
 def _dense(x: Tensor) -> Tensor:
@@ -221,8 +223,9 @@ def sink_window_causal_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int
     ones, for [N,D] and [B,H,N,D] tensors (any strides); differentiable in q, k and v.
 
     q [B,H,N,D], k [B,Hkv,N,D], v [B,Hkv,N,Dv], H a multiple of Hkv; float32, bfloat16 or float16, widths up to 128.
-    scale: 1/sqrt(D) when None.  lengths: int32 [B] on the device, the rows of every sequence of a padded batch;
-    output rows behind them are zero and take no part in the gradients, whatever the padding holds.
+    scale: 1/sqrt(D) when None.  lengths: int32 [B] on the device, the rows of every sequence of a padded batch
+    (values outside 0 .. N are taken as the nearest of them); output rows behind them are zero and take no part in the
+    gradients, whatever the padding holds.
     The output has q's dtype.  Differentiable calls cannot be captured into a graph (RuntimeError); use
     sink_window_forward and sink_window_backward there."""
     q4, k4, v4, window, sinks, s, lengths = _checked(q, k, v, window, sinks, scale, lengths)
@@ -276,6 +279,7 @@ class SinkWindowStreamingAttention:
     dtype (float32, bfloat16, float16) is that of inputs and outputs; storage None keeps the cache in it, "fp4" in 4
     bits: blocks of 32 columns of a token as 4-bit floats (0, 0.5, 1, 1.5, 2, 3, 4, 6 and signs) times a power of two,
     4.25 bits a value (a block with a value that is not finite becomes NaN).  Sums and softmax statistics are fp32.
+    A token held with an infinity or NaN makes the outputs that it reaches NaN or infinite until it leaves.
 
     Calls run on the device's current stream and may be captured into graphs (replays advance the state like
     calls); calls on one object have to be ordered, by one stream or by events."""
@@ -289,13 +293,13 @@ class SinkWindowStreamingAttention:
             raise ValueError("streams and heads must be positive and heads a multiple of kv_heads")
         if not 1 <= dim <= MAX_DIM or not 1 <= value_dim <= MAX_DIM:
             raise ValueError(f"key and value widths must be 1 .. {MAX_DIM}, got {dim} and {value_dim}")
+        self.window, self.sinks = _check_tokens(window, sinks)
         if window + sinks > MAX_ROWS:
             raise ValueError(f"a cache of at most {MAX_ROWS} tokens is supported")
         if dtype not in _native.DTYPE_CODES:
             raise ValueError(f"dtype {dtype} is not supported (use float32, bfloat16 or float16)")
         if storage not in (None, "fp4"):
             raise ValueError("storage must be None or 'fp4'")
-        self.window, self.sinks = _check_tokens(window, sinks)
         self.scale = _attention_scale(scale, dim)
         self.dim, self.value_dim, self.streams, self.heads, self.kv_heads = dim, value_dim, streams, heads, kv_heads
         self.dtype, self.storage = dtype, storage
@@ -319,7 +323,8 @@ class SinkWindowStreamingAttention:
 
     @property
     def lengths(self) -> Tensor:
-        """int32 [S] on the device: tokens that each stream has taken (a view of the state)."""
+        """int32 [S] on the device: tokens that each stream has taken, a view of the state to be read only.  A count
+        that would pass 2^31 - 1 goes back by whole windows; outputs do not depend on that."""
         return self._counts[:, 0]
 
     def _rows(self, x: Tensor, want: Tuple[int, ...], what: str) -> Tensor:
@@ -363,9 +368,9 @@ class SinkWindowStreamingAttention:
         self._extend(k[:, :, None], v[:, :, None], None)
 
     def _extend(self, k: Tensor, v: Tensor, counts: Optional[Tensor]) -> None:
-        self._fresh = False
         if k.shape[2] == 0:
             return
+        self._fresh = False
         with _on(self.device):
             st = _native.lib().sta_ring_extend(
                 k.data_ptr(), v.data_ptr(), self._code, self._store, self.streams, self.kv_heads, k.shape[2], self.dim,
@@ -412,9 +417,11 @@ class SinkWindowStreamingAttention:
             self._counts.zero_()
             self._fresh = True
             return
+        streams = list(streams)
         for i in streams:
             if not 0 <= i < self.streams:
                 raise ValueError(f"there is no stream {i}")
+        for i in streams:
             self._counts[i].zero_()
 
     @torch.no_grad()
@@ -452,9 +459,13 @@ class SinkWindowStreamingAttention:
         mine = self.state_dict_settings()
         if state["attention"] != mine:
             raise ValueError(f"state settings {state['attention']} do not match this object's {mine}")
+        if len(state["cache"]) != len(self._cache):
+            raise ValueError("the state's tensors do not match this object's")
         for x, y in zip((self._counts, *self._cache), (state["counts"], *state["cache"])):
             if (x is None) != (y is None) or (x is not None and (x.shape != y.shape or x.dtype != y.dtype)):
                 raise ValueError("the state's tensors do not match this object's")
+        if bool((state["counts"] < 0).any()):
+            raise ValueError("the state's counts must not be negative")
         for x, y in zip((self._counts, *self._cache), (state["counts"], *state["cache"])):
             if x is not None:
                 x.copy_(y)

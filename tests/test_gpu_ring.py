@@ -227,3 +227,66 @@ def test_state_round_trip(storage):
     assert torch.equal(a.step(q, k, v), b.step(q, k, v))
     for x, y in zip(a.items(), b.items()):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("storage", STORAGE)
+def test_counts_past_31_bits(storage):
+    """A stream's count goes back by whole windows where it would pass 2^31 - 1, and nothing else changes."""
+    g = torch.Generator().manual_seed(6)
+    shape = (2, 34, 2, 32, 32, 37, 3, torch.bfloat16, storage)  # 17 query heads a key head: counted by the second launch
+    for step in (True, False):
+        a, _ = build(*shape)
+        b, _ = build(*shape)
+        k, v = rand(g, torch.bfloat16, 2, 2, 60, 32).to(DEV), rand(g, torch.bfloat16, 2, 2, 60, 32).to(DEV)
+        a.extend(k, v)
+        state = a.state_dict()
+        state["counts"] += (2 ** 31 - 3 - 60) // 37 * 37
+        b.load_state_dict(state)
+        for _ in range(80):
+            q, k, v = (rand(g, torch.bfloat16, 2, h, 32).to(DEV) for h in (34, 2, 2))
+            if step:
+                assert torch.equal(a.step(q, k, v), b.step(q, k, v))
+            else:
+                for x in (a, b):
+                    x.update(k, v)
+                assert torch.equal(a.query(q), b.query(q))
+        n = b.lengths.cpu()
+        assert torch.all(n >= 40) and torch.all((n - a.lengths.cpu()) % 37 == 0)
+        for x, y in zip(a.items()[:2], b.items()[:2]):
+            assert torch.equal(x, y)
+
+
+def test_state_refusals():
+    a, _ = build(2, 1, 1, 8, 8, 4, 0, torch.float32, None)
+    a.extend(torch.ones(2, 1, 3, 8), torch.ones(2, 1, 3, 8))
+    state = a.state_dict()
+    for wrong in (dict(counts=state["counts"] - 4), dict(cache=state["cache"][:2]), dict(counts=state["counts"][:1])):
+        with pytest.raises(ValueError):
+            a.load_state_dict(dict(state, **wrong))
+    with pytest.raises(ValueError, match="no stream"):
+        a.reset([0, 2])
+    assert a.lengths.tolist() == [3, 3]
+
+
+def test_more_tiles_than_one_row_of_a_launch():
+    """2^20 + 3 tiles of slots: the last ones are filled and read like the first."""
+    window = (1 << 25) + 77
+    a, _ = build(1, 1, 1, 8, 8, window, 2, torch.bfloat16, "fp4")
+    a._counts.fill_(1 << 25)
+    k = (torch.arange(70 * 8).remainder(3) + 1).bfloat16().reshape(1, 1, 70, 8).to(DEV)
+    a.extend(k, -k)
+    keys, values, positions = a.items()
+    at = slice(1 << 25, (1 << 25) + 70)
+    assert torch.equal(keys[:, :, at], k) and torch.equal(values[:, :, at], -k)
+    assert positions[0, at].tolist() == list(range(at.start, at.stop)) and not (positions[0, at.stop:] + 1).any()
+    assert not keys[:, :, :at.start].any() and not keys[:, :, at.stop:].any()
+
+
+def test_scale_zero_of_huge_logits():
+    """Every token held weighs the same, also in tiles that only some waves have."""
+    a, _ = build(1, 1, 1, 32, 32, 40, 0, torch.float32, None, scale=0.0)
+    k, v = torch.full((1, 1, 35, 32), 1e18), torch.arange(35.0)[None, None, :, None].expand(1, 1, 35, 32)
+    a.extend(k, v)
+    out = a.query(torch.full((1, 1, 32), 1e18)).cpu()
+    # 35 weights of 1: the sum is exact, the quotient 17 too
+    assert torch.equal(out, torch.full((1, 1, 32), 17.0))

@@ -295,3 +295,18 @@ def test_empty_batches():
         assert out.shape == shape
         out.sum().backward()
         assert x.grad.shape == shape
+
+
+def test_row_strides_of_single_rows():
+    """The stride of a dimension of one element is never walked, however far it reaches."""
+    q, k, v, go = make(2, 2, 1, 1, 32, 32, torch.bfloat16)
+    want = run(q, k, v, go, window=3, sinks=0)
+
+    def far(x):
+        x = x.to(DEV)
+        return x.as_strided(x.shape, (x.stride(0), x.stride(1), 1 << 25, 1))
+
+    out, lse = swa.sink_window_forward(far(q), far(k), far(v), window=3, sinks=0)
+    got = (out, *swa.sink_window_backward(far(go), far(q), far(k), far(v), out, lse, window=3, sinks=0))
+    for x, y in zip(got, want.values()):
+        assert torch.equal(x.cpu(), y.cpu())

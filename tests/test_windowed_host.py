@@ -101,6 +101,12 @@ def test_rotary_refuses(q, k, kw, message):
         qkr.qk_norm_rotary(q, k, table, **kw)
 
 
+def test_rotary_table_takes_no_gradient(monkeypatch):
+    monkeypatch.setattr(qkr, "_check_gpu", lambda *a: None)
+    with pytest.raises(ValueError, match="table takes no gradient"):
+        qkr.qk_norm_rotary(x(3, 8), x(3, 8), x(4, 8).requires_grad_())
+
+
 def test_rotary_table():
     t = qkr.rotary_table(100, 8, base=100.0)
     assert t.shape == (100, 8) and t.dtype == torch.float32
@@ -126,7 +132,8 @@ def test_library_refuses_without_touching_a_device():
                      (dict(dv=129), E.STA_ERR_UNSUPPORTED), (dict(d=3), E.STA_ERR_UNSUPPORTED),
                      (dict(dt=1, dv=7), E.STA_ERR_UNSUPPORTED), (dict(n=(1 << 30) + 1), E.STA_ERR_UNSUPPORTED),
                      (dict(w=0), E.STA_ERR_ARG), (dict(sinks=-1), E.STA_ERR_ARG), (dict(scale=math.inf), E.STA_ERR_ARG),
-                     (dict(b=1 << 31), E.STA_ERR_UNSUPPORTED), (dict(b=1 << 30, n=1 << 20), E.STA_ERR_SHAPE)]:
+                     (dict(b=1 << 31), E.STA_ERR_UNSUPPORTED), (dict(b=1 << 30, n=1 << 20), E.STA_ERR_SHAPE),
+                     (dict(b=1 << 23, n=1), E.STA_ERR_SHAPE)]:  # 2^24 workgroups
         assert fwd(**kw) == want, kw
     assert lib.sta_window_backward_bytes(0, 1, 2, 1, 8, 8, 8, 0, 1) == -1
     need = lib.sta_window_backward_bytes(0, 1, 2, 1, 1000, 8, 8, 100, 4)
@@ -134,6 +141,8 @@ def test_library_refuses_without_touching_a_device():
     back = [16] * 6 + [0, 1, 2, 1, 1000, 8, 8, st, 1.0, 100, 4, None, 16, 16, 16, 16]
     assert lib.sta_window_attention_backward(*back, need - 1, None) == E.STA_ERR_SCRATCH
     assert lib.sta_window_attention_backward(None, *back[1:], need, None) == E.STA_ERR_ARG
+    wide = [16] * 6 + [0, 1 << 23, 2, 1, 1, 8, 8, st, 1.0, 100, 4, None, 16, 16, 16, 16]
+    assert lib.sta_window_attention_backward(*wide, 1 << 40, None) == E.STA_ERR_SHAPE
 
     rot = dict(q=16, k=16, dt=0, b=1, h=2, hk=1, n=8, d=8, s=st, qw=None, kw=None, wt=0, table=16, limit=8, r=8, i=0,
                pos=None, p64=0, psb=0, psn=0, eps=1e-6, qo=16, ko=16)
@@ -159,7 +168,7 @@ def test_library_refuses_without_touching_a_device():
     for kw, want in [(dict(q=None), E.STA_ERR_ARG), (dict(k=None), E.STA_ERR_ARG), (dict(counts=None), E.STA_ERR_ARG),
                      (dict(ek=None), E.STA_ERR_ARG), (dict(ck=8), E.STA_ERR_ARG), (dict(store=2), E.STA_ERR_DTYPE),
                      (dict(h=3, hk=2), E.STA_ERR_SHAPE), (dict(w=0), E.STA_ERR_ARG), (dict(scale=math.nan), E.STA_ERR_ARG),
-                     (dict(), E.STA_ERR_SCRATCH)]:
+                     (dict(), E.STA_ERR_SCRATCH), (dict(s=1 << 24, w=4), E.STA_ERR_SHAPE)]:
         a = dict(ring, **kw)
         assert lib.sta_ring_attention(*a.values(), None) == want, kw
     fill = dict(k=16, v=16, dt=1, store=1, s=1, hk=1, rows=4, d=8, dv=8, st=st, w=4, sinks=1, take=None, ck=16, cv=16,
