@@ -846,24 +846,24 @@ __device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, in
 // (shared: one stage a wave).
 template <int IN, bool SHARE>
 __host__ __device__ constexpr int win_staged_rows() { return IN == F32 || SHARE ? 32 : 64; }
-template <int P, int IN, bool SHARE>
+template <int P, int IN, bool SHARE, bool PIPE>
 __host__ __device__ constexpr int win_dkv_lds() {
   const int rows = win_staged_rows<IN, SHARE>(), stage = 2 * rows * P * (IN == F32 ? 4 : 2) + 2 * rows * 4;
-  if (!SHARE) return 2 * stage;
+  if (!SHARE) return (PIPE ? 3 : 2) * stage;
   return 4 * stage > 4 * win_join_floats<P>() ? 4 * stage : 4 * win_join_floats<P>();
 }
 
 // dk and dv: one workgroup per 128 keys of a key head (32 a wave) walks over the rows that see them within the window,
 // for every head of the group; the rows behind the window of a sink go to workgroups of their own (far), whose
 // sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.
-template <int P, int IN, bool SHARE>
+template <int P, int IN, bool SHARE, bool PIPE>
 __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_staged_rows<IN, SHARE>(),
                 NSUB = BQ / 32, TILE = win_rows<SHARE>(), THREADS = SHARE ? 64 : 256;
   constexpr int STAGE = 2 * BQ * CH;  // 16-byte units of a stage
   extern __shared__ uint4 win_lds[];
-  constexpr int STAGES = SHARE ? 4 : 2;  // of the waves, or of two tiles
-  float* const stats = reinterpret_cast<float*>(win_lds + STAGES * STAGE);  // [stage][lse, delta][BQ]
+  constexpr int STAGES = SHARE ? 4 : (PIPE ? 3 : 2);  // of the waves, or of tiles
+  float* const stats = reinterpret_cast<float*>(win_lds + STAGES * STAGE);  // [stage][lift - lse, delta][BQ]
   const int kv = a.heads / a.group;
   const int far_items = a.sink_tiles * a.far_chunks, items = far_items + a.key_tiles;
   const int id = xcd_remap(blockIdx.x, gridDim.x);
@@ -907,149 +907,336 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
     }
     const int first = lo / BQ * BQ, per_head = hi / BQ - lo / BQ + 1, count = per_head * a.group;
     const float lift = __builtin_amdgcn_logf(a.lift);
-    WinStage<P, IN, BQ, THREADS> qst, gst;
-    qst.init(a.q, a.d);
-    gst.init(a.go, a.dv);
-    float stat = 0.f;
-    const int self = threadIdx.x % THREADS;
-    auto row_of = [&](int it) { return first + it % per_head * BQ; };
-    auto load = [&](int it) {
-      const int row0 = row_of(it), h = hk * a.group + it / per_head;
-      qst.load(rows_at<ES>(a.q, b, h, row0), len - row0);
-      gst.load(rows_at<ES>(a.go, b, h, row0), len - row0);
-      if (self < 2 * BQ) {
-        const int row = row0 + self % BQ;
-        const float* from = self < BQ ? a.lse : a.delta;
-        stat = row < len ? from[(static_cast<int64_t>(b) * a.heads + h) * a.n + row] : 0.f;
+    // hidden pairs' weights and gradients
+    auto hide = [&](floatx16& x, floatx16& g, int base) {
+      const int ahead = base - key, from = lo - base, last = key < a.sinks ? hi - base : -1;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = 8 * (i >> 2) + (i & 3);
+        bool seen = static_cast<uint32_t>(ahead + r) < static_cast<uint32_t>(a.window);
+        if (far) seen = (ahead + r >= a.window) & (r >= from) & (r <= last);
+        x[i] = seen ? x[i] : 0.f;
+        g[i] = seen ? g[i] : 0.f;
       }
     };
-    auto put = [&](int it, int stage) {
-      qst.put(win_lds + stage * STAGE, len - row_of(it));
-      gst.put(win_lds + stage * STAGE + BQ * CH, len - row_of(it));
-      if (self < 2 * BQ) stats[stage * 2 * BQ + self] = stat;
+    // of the wave's keys, does none or do all see each of the rows [q0, q0 + rows)
+    auto none = [&](int q0, int rows) {
+      return far ? kw >= a.sinks || q0 + rows - 1 - kw < a.window : q0 + rows - 1 < kw || q0 - (kw + 31) >= a.window;
     };
-    const int start = SHARE ? wave : 0, step = SHARE ? 4 : 1;
-    constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
-    if (AHEAD && start < count) load(start);
-    if constexpr (!SHARE) {
-      put(0, 0);
-      if (count > 1) load(1);
-    }
-    for (int it = start; it < count; it += step) {
-      // the accumulators stay in accumulation registers (the compiler else moves all of them there and back)
+    auto whole = [&](int q0, int rows) {
+      return far ? kw + 32 <= a.sinks && q0 - (kw + 31) >= a.window && q0 >= lo && q0 + rows - 1 <= hi
+                 : q0 >= kw + 31 && q0 + rows - 1 - kw < a.window;
+    };
+    if constexpr (PIPE) {
+      // One wave a SIMD has nothing else to do while it waits, so its own matrix and vector instructions are interleaved:
+      // the products of the next 32 rows' logits with the weights of these, the next tiles' way into LDS with the
+      // sums.  Three stages: tile `it` and the next are written, the third is being written.  Rows behind the last
+      // are read as the last one, their weights are exp2(-inf).
+      constexpr int U = BQ * CH / 256;  // 16-byte units of a tensor's tile a thread
+      static_assert(U == MT && NSUB == 2);
+      uint4 uq[U], ug[U];
+      uint32_t to[U], off[2][U];
+      const int pitch_q = static_cast<int>(a.q.sn) * ES, pitch_g = static_cast<int>(a.go.sn) * ES;
+      const int srow = threadIdx.x % BQ;
+      const bool of_lse = threadIdx.x % (2 * BQ) < BQ;
+      float stat;
+      int next = 0, lrow = first, lhead = hk * a.group;  // the tile to be read, its first row and head
+      bool cut = true;                                   // off is not that of whole tiles
+      const char *qp, *gp;
+      const float* sp;
+      bool srow_in;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        win_pin(dk[mt]);
-        win_pin(dv[mt]);
+      for (int i = 0; i < U; ++i) {
+        const int k = threadIdx.x + 256 * i, row = k / CH;
+        to[i] = row * CH + ((k % CH) ^ win_swizzle<CH>(row));
       }
-      int stage = wave;
-      if (!AHEAD) load(it);
-      win_sync<SHARE>();
-      if constexpr (SHARE) {
-        put(it, wave);
-        win_sync<SHARE>();
-        if (AHEAD && it + step < count) load(it + step);
-      } else {  // stage `it` is written, the other one read
-        stage = it & 1;
-        if (it + 1 < count) put(it + 1, stage ^ 1);
-        if (it + 2 < count) load(it + 2);
+      auto aim = [&]() {
+        const int left = len - lrow;
+        if (cut || left < BQ) {
+          cut = left < BQ;
+#pragma unroll
+          for (int i = 0; i < U; ++i) {
+            const int k = threadIdx.x + 256 * i, row = min(k / CH, left - 1);
+            off[0][i] = row * pitch_q + k % CH * 16;
+            off[1][i] = row * pitch_g + k % CH * 16;
+          }
+        }
+        qp = rows_at<ES>(a.q, b, lhead, lrow);
+        gp = rows_at<ES>(a.go, b, lhead, lrow);
+        sp = (of_lse ? a.lse : a.delta) + (static_cast<int64_t>(b) * a.heads + lhead) * a.n + min(lrow + srow, len - 1);
+        srow_in = lrow + srow < len;
+        // the tile after; behind the last one, that again
+        if (++next < count) {
+          lrow += BQ;
+          if (lrow > hi) {
+            lrow = first;
+            ++lhead;
+          }
+        }
+      };
+      auto read = [&](int i) {
+        uq[i] = rows_load16(qp + off[0][i]);
+        ug[i] = rows_load16(gp + off[1][i]);
+        if (i == 0) stat = *sp;
+      };
+      bool stat_in;
+      auto write = [&](int i, int st) {
+        win_lds[st * STAGE + to[i]] = uq[i];
+        win_lds[st * STAGE + BQ * CH + to[i]] = ug[i];
+        if (i == 0) {
+          const float x = of_lse ? lift - stat : stat;
+          stats[st * 2 * BQ + threadIdx.x % (2 * BQ)] = stat_in ? x : (of_lse ? -__builtin_inff() : 0.f);
+        }
+      };
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        aim();
+#pragma unroll
+        for (int i = 0; i < U; ++i) read(i);
+        stat_in = srow_in;
+        if (j < 2) {
+#pragma unroll
+          for (int i = 0; i < U; ++i) write(i, j);
+        }
       }
-      const uint4 *qs = win_lds + stage * STAGE, *gs = qs + BQ * CH;
-      const floatx4* st = reinterpret_cast<const floatx4*>(stats + stage * 2 * BQ);
-      const int q0 = row_of(it);
-      const bool some = far ? kw < a.sinks && q0 + BQ - 1 - kw >= a.window
-                            : q0 + BQ - 1 >= kw && q0 - (kw + 31) < a.window;
-      if (!some) continue;
-      const bool all = far ? kw + 32 <= a.sinks && q0 - (kw + 31) >= a.window && q0 >= lo && q0 + BQ - 1 <= hi
-                           : q0 >= kw + 31 && q0 + BQ - 1 - kw < a.window;
-#pragma unroll 1
-      for (int sub = 0; sub < NSUB; ++sub) {
-        // every operand is read well before its product: a compute unit holds one wave a SIMD, which has nothing else to
-        // do while it waits
-        // (fp32 products take eight times as long as their operands' reads: those are read as they come)
-        constexpr bool EARLY = IN != F32;
-        WinFrag<IN> qa[EARLY ? P / 16 : 1], ga[EARLY ? P / 16 : 1], qc[MT], gc[MT];
-        floatx16 x, g;
+      int stage = 0;
+      auto rows_of_stage = [&](int st) { return win_lds + st * STAGE; };
+      floatx16 x[2], g[2];
+      __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
-        if constexpr (EARLY) {
+      for (int i = 0; i < 16; ++i) x[0][i] = g[0][i] = 0.f;
 #pragma unroll
-          for (int s = 0; s < P / 16; ++s) {
-            qa[s] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
-            ga[s] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
+      for (int s = 0; s < P / 16; ++s) {
+        win_mma<IN>(x[0], win_read_row<P, IN>(win_lds, lane & 31, s, hh), kf[s]);
+        win_mma<IN>(g[0], win_read_row<P, IN>(win_lds + BQ * CH, lane & 31, s, hh), vf[s]);
+      }
+      int q0 = first;
+      for (int it = 0; it < count; ++it) {
+        if (it) __syncthreads();
+        const int after = stage == 2 ? 0 : stage + 1, third = after == 2 ? 0 : after + 1;
+        aim();
+        const uint4 *qs = rows_of_stage(stage), *gs = qs + BQ * CH;
+        const floatx4* st = reinterpret_cast<const floatx4*>(stats + stage * 2 * BQ);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          win_pin(dk[mt]);
+          win_pin(dv[mt]);
+        }
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
+          floatx16 &x0 = x[sub], &g0 = g[sub], &x1 = x[sub ^ 1], &g1 = g[sub ^ 1];
+          // the rows after these (behind the last tile: of whatever the stage holds, not used)
+          const uint4 *nq = sub ? rows_of_stage(after) : qs, *ng = nq + BQ * CH;
+          const int nrow = 32 * (sub ^ 1) + (lane & 31);
+          floatx4 shift[4], delta[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            shift[r] = st[8 * sub + 2 * r + hh];
+            delta[r] = st[BQ / 4 + 8 * sub + 2 * r + hh];
+          }
+          constexpr int STEPS = P / 16, LEAD = 2;
+          WinFrag<IN> qa[STEPS], ga[STEPS], qc[2][MT], gc[2][MT];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x1[i] = g1[i] = 0.f;
+#pragma unroll
+          for (int s = 0; s < LEAD; ++s) {
+            qa[s] = win_read_row<P, IN>(nq, nrow, s, hh);
+            ga[s] = win_read_row<P, IN>(ng, nrow, s, hh);
           }
           __builtin_amdgcn_sched_barrier(0);
-        }
+          auto weigh = [&](int i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(x0[i], a.c, shift[i >> 2][i & 3]));
+            g0[i] = p * (g0[i] - delta[i >> 2][i & 3]);
+            x0[i] = p;
+          };
 #pragma unroll
-        for (int s = 0; s < P / 16; ++s) {
-          if constexpr (!EARLY) {
-            qa[0] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
-            ga[0] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
+          for (int s = 0; s < STEPS; ++s) {
+            if (s + LEAD < STEPS) {
+              qa[s + LEAD] = win_read_row<P, IN>(nq, nrow, s + LEAD, hh);
+              ga[s + LEAD] = win_read_row<P, IN>(ng, nrow, s + LEAD, hh);
+            } else if (s + 1 < STEPS) {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) gc[0][mt] = win_read_columns<P, IN>(gs, 32 * sub, mt, lane);
+            } else {
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) qc[0][mt] = win_read_columns<P, IN>(qs, 32 * sub, mt, lane);
+            }
+            win_mma<IN>(x1, qa[s], kf[s]);
+            const int from = 16 * s / STEPS, to = 16 * (s + 1) / STEPS, half = (from + to) / 2;
+#pragma unroll
+            for (int i = from; i < half; ++i) weigh(i);
+            __builtin_amdgcn_sched_barrier(0);
+            win_mma<IN>(g1, ga[s], vf[s]);
+#pragma unroll
+            for (int i = half; i < to; ++i) weigh(i);
+            __builtin_amdgcn_sched_barrier(0);
           }
-          win_mma<IN>(x, qa[EARLY ? s : 0], kf[s]);
-          win_mma<IN>(g, ga[EARLY ? s : 0], vf[s]);
-        }
-        floatx4 lse[4], delta[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          lse[r] = st[8 * sub + 2 * r + hh];
-          delta[r] = st[BQ / 4 + 8 * sub + 2 * r + hh];
-        }
-        if constexpr (EARLY) {
+          asm volatile("" : "+v"(x0), "+v"(g0));
+          if (!whole(q0 + 32 * sub, 32)) hide(x0, g0, q0 + 32 * sub + 4 * hh);
+          WinFrag<IN> p[2], ds[2];
+          p[0] = win_operand<IN>(x0, 0);
+          ds[0] = win_operand<IN>(g0, 0);
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            gc[mt] = win_read_columns<P, IN>(gs, 32 * sub, mt, lane);
-            qc[mt] = win_read_columns<P, IN>(qs, 32 * sub, mt, lane);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, lift - lse[i >> 2][i & 3]));
-          g[i] = p * (g[i] - delta[i >> 2][i & 3]);
-          x[i] = p;
-        }
-        if (!all) {
-          const int base = q0 + 32 * sub + 4 * hh, ahead = base - key;
-          const int from = lo - base, last = key < a.sinks ? hi - base : -1;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int r = 8 * (i >> 2) + (i & 3);
-            bool seen = static_cast<uint32_t>(ahead + r) < static_cast<uint32_t>(a.window);
-            if (far) seen = (ahead + r >= a.window) & (r >= from) & (r <= last);
-            x[i] = seen ? x[i] : 0.f;
-            g[i] = seen ? g[i] : 0.f;
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
-          WinFrag<IN> gn[EARLY ? MT : 1], qn[EARLY ? MT : 1];
-          if constexpr (EARLY) {
-            if (t == 0) {
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                gn[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16, mt, lane);
-                qn[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16, mt, lane);
-              }
+            gc[1][mt] = win_read_columns<P, IN>(gs, 32 * sub + 16, mt, lane);
+            qc[1][mt] = win_read_columns<P, IN>(qs, 32 * sub + 16, mt, lane);
+            win_mma<IN>(dv[mt], gc[0][mt], p[0]);
+            win_mma<IN>(dk[mt], qc[0][mt], ds[0]);
+            if (mt == 0) {
+              p[1] = win_operand<IN>(x0, 1);
+              ds[1] = win_operand<IN>(g0, 1);
             }
             __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            if constexpr (!EARLY) {
-              gc[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16 * t, mt, lane);
-              qc[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16 * t, mt, lane);
+            win_mma<IN>(dv[mt], gc[1][mt], p[1]);
+            win_mma<IN>(dk[mt], qc[1][mt], ds[1]);
+            if (sub == 0) {
+              write(mt, third);
+              read(mt);
             }
-            win_mma<IN>(dv[mt], gc[mt], p);
-            win_mma<IN>(dk[mt], qc[mt], ds);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          if (sub == 0) stat_in = srow_in;
+        }
+        stage = after;
+        q0 += BQ;
+        if (q0 > hi) q0 = first;
+      }
+    } else {
+      WinStage<P, IN, BQ, THREADS> qst, gst;
+      qst.init(a.q, a.d);
+      gst.init(a.go, a.dv);
+      float stat = 0.f;
+      const int self = threadIdx.x % THREADS;
+      auto row_of = [&](int it) { return first + it % per_head * BQ; };
+      auto load = [&](int it) {
+        const int row0 = row_of(it), h = hk * a.group + it / per_head;
+        qst.load(rows_at<ES>(a.q, b, h, row0), len - row0);
+        gst.load(rows_at<ES>(a.go, b, h, row0), len - row0);
+        if (self < 2 * BQ) {
+          const int row = row0 + self % BQ;
+          const float* from = self < BQ ? a.lse : a.delta;
+          stat = row < len ? from[(static_cast<int64_t>(b) * a.heads + h) * a.n + row] : 0.f;
+          if (self < BQ) stat = lift - stat;
+        }
+      };
+      auto put = [&](int it, int stage) {
+        qst.put(win_lds + stage * STAGE, len - row_of(it));
+        gst.put(win_lds + stage * STAGE + BQ * CH, len - row_of(it));
+        if (self < 2 * BQ) stats[stage * 2 * BQ + self] = stat;
+      };
+      const int start = SHARE ? wave : 0, step = SHARE ? 4 : 1;
+      constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
+      if (AHEAD && start < count) load(start);
+      if constexpr (!SHARE) {
+        put(0, 0);
+        if (count > 1) load(1);
+      }
+      for (int it = start; it < count; it += step) {
+        // the accumulators stay in accumulation registers (the compiler else moves all of them there and back)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          win_pin(dk[mt]);
+          win_pin(dv[mt]);
+        }
+        int stage = wave;
+        if (!AHEAD) load(it);
+        win_sync<SHARE>();
+        if constexpr (SHARE) {
+          put(it, wave);
+          win_sync<SHARE>();
+          if (AHEAD && it + step < count) load(it + step);
+        } else {  // stage `it` is written, the other one read
+          stage = it & 1;
+          if (it + 1 < count) put(it + 1, stage ^ 1);
+          if (it + 2 < count) load(it + 2);
+        }
+        const uint4 *qs = win_lds + stage * STAGE, *gs = qs + BQ * CH;
+        const floatx4* st = reinterpret_cast<const floatx4*>(stats + stage * 2 * BQ);
+        const int q0 = row_of(it);
+        if (none(q0, BQ)) continue;
+        const bool all = whole(q0, BQ);
+#pragma unroll 1
+        for (int sub = 0; sub < NSUB; ++sub) {
+          // every operand is read well before its product: a compute unit holds one wave a SIMD, which has nothing else to
+          // do while it waits
+          // (fp32 products take eight times as long as their operands' reads: those are read as they come)
+          constexpr bool EARLY = IN != F32;
+          WinFrag<IN> qa[EARLY ? P / 16 : 1], ga[EARLY ? P / 16 : 1], qc[MT], gc[MT];
+          floatx16 x, g;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = g[i] = 0.f;
+          if constexpr (EARLY) {
+#pragma unroll
+            for (int s = 0; s < P / 16; ++s) {
+              qa[s] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
+              ga[s] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int s = 0; s < P / 16; ++s) {
+            if constexpr (!EARLY) {
+              qa[0] = win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh);
+              ga[0] = win_read_row<P, IN>(gs, 32 * sub + (lane & 31), s, hh);
+            }
+            win_mma<IN>(x, qa[EARLY ? s : 0], kf[s]);
+            win_mma<IN>(g, ga[EARLY ? s : 0], vf[s]);
+          }
+          floatx4 shift[4], delta[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            shift[r] = st[8 * sub + 2 * r + hh];
+            delta[r] = st[BQ / 4 + 8 * sub + 2 * r + hh];
           }
           if constexpr (EARLY) {
-            if (t == 0) {
 #pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                gc[mt] = gn[mt];
-                qc[mt] = qn[mt];
+            for (int mt = 0; mt < MT; ++mt) {
+              gc[mt] = win_read_columns<P, IN>(gs, 32 * sub, mt, lane);
+              qc[mt] = win_read_columns<P, IN>(qs, 32 * sub, mt, lane);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, shift[i >> 2][i & 3]));
+            g[i] = p * (g[i] - delta[i >> 2][i & 3]);
+            x[i] = p;
+          }
+          if (!all) hide(x, g, q0 + 32 * sub + 4 * hh);
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
+            WinFrag<IN> gn[EARLY ? MT : 1], qn[EARLY ? MT : 1];
+            if constexpr (EARLY) {
+              if (t == 0) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  gn[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16, mt, lane);
+                  qn[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16, mt, lane);
+                }
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              if constexpr (!EARLY) {
+                gc[mt] = win_read_columns<P, IN>(gs, 32 * sub + 16 * t, mt, lane);
+                qc[mt] = win_read_columns<P, IN>(qs, 32 * sub + 16 * t, mt, lane);
+              }
+              win_mma<IN>(dv[mt], gc[mt], p);
+              win_mma<IN>(dk[mt], qc[mt], ds);
+            }
+            if constexpr (EARLY) {
+              if (t == 0) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                  gc[mt] = gn[mt];
+                  qc[mt] = qn[mt];
+                }
               }
             }
           }
