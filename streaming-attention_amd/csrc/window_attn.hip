@@ -1034,7 +1034,7 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
             shift[r] = st[8 * sub + 2 * r + hh];
             delta[r] = st[BQ / 4 + 8 * sub + 2 * r + hh];
           }
-          constexpr int STEPS = P / 16, LEAD = 2;
+          constexpr int STEPS = P / 16, LEAD = STEPS < 3 ? STEPS : 3;
           WinFrag<IN> qa[STEPS], ga[STEPS], qc[2][MT], gc[2][MT];
 #pragma unroll
           for (int i = 0; i < 16; ++i) x1[i] = g1[i] = 0.f;
@@ -1054,10 +1054,12 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
             if (s + LEAD < STEPS) {
               qa[s + LEAD] = win_read_row<P, IN>(nq, nrow, s + LEAD, hh);
               ga[s + LEAD] = win_read_row<P, IN>(ng, nrow, s + LEAD, hh);
-            } else if (s + 1 < STEPS) {
+            }
+            if (s == STEPS - 2) {
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) gc[0][mt] = win_read_columns<P, IN>(gs, 32 * sub, mt, lane);
-            } else {
+            }
+            if (s == STEPS - 1) {
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) qc[0][mt] = win_read_columns<P, IN>(qs, 32 * sub, mt, lane);
             }
