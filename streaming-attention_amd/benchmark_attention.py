@@ -12,6 +12,9 @@ Differences from the reference, all in how numbers are obtained, not in what is 
   * the state-size columns come from the per-token size formula (state_size_trace /
     coreset_item_trace, equal to the reference's per-token update loop, benchmark_attention.py:107-136)
     instead of replaying every token through the streaming object.
+
+With --window W (and --sinks S) a row also has exact attention over the last W tokens and the first S ones, the other
+way to a bounded state: its columns follow the others in the table and the CSV, which are unchanged without it.
 """
 
 from __future__ import annotations
@@ -31,6 +34,7 @@ if str(_HERE) not in sys.path:
 
 from _cli_util import fmt_bytes, pick_device, wall_ms  # noqa: E402
 from fast_article_attention import _make_data, _resolve_dtype  # noqa: E402
+from sink_window_attention import sink_window_causal_attention  # noqa: E402
 from streaming_taylor_coreset_attention import (  # noqa: E402
     article_causal_attention,
     classical_causal_attention,
@@ -44,6 +48,9 @@ COLUMNS = ("n", "d", "dv", "degree", "block_size", "compressor", "data", "radius
            "rel_l2", "max_abs", "mean_abs", "classical_median_ms", "classical_best_ms", "article_median_ms",
            "article_best_ms", "article_final_state_bytes", "article_max_state_bytes", "article_max_coreset_items",
            "classical_kv_bytes", "classical_naive_scores_bytes")
+# and of --window
+WINDOW_COLUMNS = ("window", "sinks", "window_rel_l2", "window_max_abs", "window_mean_abs", "window_median_ms",
+                  "window_best_ms", "window_state_bytes")
 
 
 def state_bytes(n: int, d: int, dv: int, *, degree: int, block_size: int, compressor: str, elem: int):
@@ -82,7 +89,19 @@ def run_one(args: argparse.Namespace, n: int) -> Dict[str, object]:
     row.update(n=n, d=args.d, dv=args.dv, degree=args.degree, block_size=args.block_size, compressor=args.compressor,
                data=args.data, radius=args.radius, scale=scale, device=str(device),
                dtype=str(dtype).replace("torch.", ""))
-    return {c: row[c] for c in COLUMNS}
+    if args.window is None:
+        return {c: row[c] for c in COLUMNS}
+    kw = dict(window=args.window, sinks=args.sinks, scale=scale)
+    on_gpu = [x.to(gpu) for x in (q, k, v)]
+    diff = sink_window_causal_attention(*on_gpu, **kw).to(exact.device)
+    row["window_rel_l2"] = safe_relative_l2(diff, exact)
+    diff = (diff.float() - exact.float()).abs()
+    row["window_max_abs"], row["window_mean_abs"] = diff.max().item(), diff.mean().item()
+    row["window_median_ms"], row["window_best_ms"] = wall_ms(
+        lambda: sink_window_causal_attention(*on_gpu, **kw), args.repeats, gpu)
+    row.update(window=args.window, sinks=args.sinks,
+               window_state_bytes=min(n, args.window + args.sinks) * (args.d + args.dv) * elem)
+    return {c: row[c] for c in COLUMNS + WINDOW_COLUMNS}
 
 
 def print_table(rows: List[Dict[str, object]]) -> None:
@@ -92,6 +111,10 @@ def print_table(rows: List[Dict[str, object]]) -> None:
             ("article_state", lambda r: fmt_bytes(int(r["article_max_state_bytes"]))),
             ("score_matrix", lambda r: fmt_bytes(int(r["classical_naive_scores_bytes"]))),
             ("coreset_items", lambda r: str(r["article_max_coreset_items"]))]
+    if rows and "window" in rows[0]:
+        cols += [("window_rel_l2", lambda r: f"{r['window_rel_l2']:.4g}"),
+                 ("window_ms", lambda r: f"{r['window_median_ms']:.3f}"),
+                 ("window_state", lambda r: fmt_bytes(int(r["window_state_bytes"])))]
     print("\n" + " | ".join(h for h, _ in cols))
     print(" | ".join("---" for _ in cols))
     for r in rows:
@@ -102,7 +125,7 @@ def print_table(rows: List[Dict[str, object]]) -> None:
 def write_csv(path: pathlib.Path, rows: List[Dict[str, object]]) -> None:
     path.parent.mkdir(parents=True, exist_ok=True)
     with path.open("w", newline="") as fh:
-        w = csv.DictWriter(fh, fieldnames=list(COLUMNS))
+        w = csv.DictWriter(fh, fieldnames=list(rows[0]) if rows else list(COLUMNS))
         w.writeheader()
         w.writerows(rows)
 
@@ -123,6 +146,8 @@ def parser() -> argparse.ArgumentParser:
     p.add_argument("--dtype", default="float32")
     p.add_argument("--repeats", type=int, default=3)
     p.add_argument("--seed", type=int, default=0)
+    p.add_argument("--window", type=int, default=None, help="Also exact attention over a window of this many tokens")
+    p.add_argument("--sinks", type=int, default=4, help="... and this many first tokens (with --window)")
     p.add_argument("--csv", type=pathlib.Path, default=None)
     return p
 

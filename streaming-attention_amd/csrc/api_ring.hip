@@ -18,11 +18,7 @@ constexpr int64_t kMaxRingSlots = int64_t(1) << 30;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-sta::Rows rows_of(const void* p, const int64_t* strides, int es) {
-  sta::Rows r{p, strides[0], strides[1], strides[2], 0};
-  r.aligned = aligned16(p) && r.sb * es % 16 == 0 && r.sh * es % 16 == 0 && r.sn * es % 16 == 0;
-  return r;
-}
+sta::Rows rows_of(const void* p, const int64_t* strides) { return sta::Rows{p, strides[0], strides[1], strides[2], 0}; }
 
 // storage: the element type's own code, or 4 bits
 bool storage_ok(int storage, int dtype) { return storage == dtype || storage == sta::RING_F4; }
@@ -136,14 +132,13 @@ int sta_ring_attention(const void* q, const void* k, const void* v, int dtype, i
   if (const int st = ring_shape(a, streams, heads, kv_heads, d, dv, window, sinks)) return st;
   const int64_t need = sta_ring_attention_bytes(streams, heads, kv_heads, d, dv, window, sinks);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return STA_ERR_SCRATCH;
-  const int es = dtype == STA_F32 ? 4 : 2;
   const int64_t qs[3] = {strides[0], strides[1], 0}, ks[3] = {strides[2], strides[3], 0},
                 vs[3] = {strides[4], strides[5], 0};
-  a.q = rows_of(q, qs, es);
+  a.q = rows_of(q, qs);
   a.append = k != nullptr;
   if (a.append) {
-    a.k = rows_of(k, ks, es);
-    a.v = rows_of(v, vs, es);
+    a.k = rows_of(k, ks);
+    a.v = rows_of(v, vs);
   }
   a.scale = scale;
   // above 0: what a wave without tiles has, -3e38, stays far below a logit times c
@@ -170,9 +165,8 @@ int sta_ring_extend(const void* k, const void* v, int dtype, int storage, int64_
   if (const int st = ring_shape(f.a, streams, kv_heads, kv_heads, d, dv, window, sinks)) return st;
   if (rows < 1) return STA_ERR_SHAPE;
   if (rows > kMaxRingSlots) return STA_ERR_UNSUPPORTED;
-  const int es = dtype == STA_F32 ? 4 : 2;
-  f.a.k = rows_of(k, strides, es);
-  f.a.v = rows_of(v, strides + 3, es);
+  f.a.k = rows_of(k, strides);
+  f.a.v = rows_of(v, strides + 3);
   f.a.keys = static_cast<uint8_t*>(keys);
   f.a.values = static_cast<uint8_t*>(values);
   f.a.kexp = static_cast<uint8_t*>(key_exponents);

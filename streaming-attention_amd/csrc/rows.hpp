@@ -1,4 +1,4 @@
-// Rows of strided [batch][heads][n][width] tensors, read in units of 16 bytes where they are aligned.
+// Rows of strided [batch][heads][n][width] tensors, read in units of 16 bytes.
 #pragma once
 #include "common.hpp"
 
@@ -7,7 +7,7 @@ namespace sta {
 // workgroups of 256 threads in one dimension of a launch, whose threads have to stay below 2^32
 constexpr int64_t MAX_GROUPS = (int64_t(1) << 24) - 1;
 
-// element strides; `aligned`: every row starts on 16 bytes
+// element strides; `aligned`: every row starts on 16 bytes (set for the kernels that ask for it)
 struct Rows {
   const void* p;
   int64_t sb, sh, sn;

@@ -408,7 +408,13 @@ __host__ __device__ constexpr int win_lds_bytes() {
   return 4 * stage > join ? 4 * stage : join;
 }
 
-// Row tiles: keys staged win_keys at a time, the next tile's rows in registers while this one computes.
+// Row tiles: keys staged win_keys at a time, the next tile's rows in registers while this one computes, softmax in one
+// pass.  The weights of 16-bit rows enter the second product rounded to their type (half a step each, errors that
+// average over the keys and end below the output's own rounding); their sum is taken before that, in fp32.
+// Measured, bf16: 32 heads of 16384 rows, 128 wide, window 4096: 1.04 ms, 925 TFLOP/s, bound by the products (a large
+// matrix product reaches 1180).  8 x 16 heads of 4096 rows, 64 wide, window 1024: 0.20 ms, 600 TFLOP/s, bound by the vector
+// unit: a tile of 64 keys takes 16 products (512 cycles of the matrix unit) but 32 exponentials, a quarter of the rate,
+// and about 150 other instructions (1100 cycles); 4 waves a SIMD instead of 3 change nothing.
 template <int P, int IN, bool SHARE>
 __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forward_kernel(const WinArgs a) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
@@ -639,7 +645,9 @@ __device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
     if (lane + 64 * e < a.d) store_elem(a.dq, row * a.d + lane + 64 * e, IN, a.scale * acc[e]);
 }
 
-// dq and D: the forward kernel's walk over the keys with the rows' statistics given.
+// dq and D: the forward kernel's walk over the keys with the rows' statistics given.  ds is rounded to the rows' type for
+// its product with the keys like the weights of the forward kernel.  32 heads of 16384 rows, 128 wide, window 4096,
+// bf16: 1.45 ms, three products at 995 TFLOP/s, bound by them.
 template <int P, int IN, bool SHARE>
 __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : 2) void window_dq_kernel(const WinArgs a) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
@@ -855,7 +863,15 @@ __host__ __device__ constexpr int win_dkv_lds() {
 
 // dk and dv: one workgroup per 128 keys of a key head (32 a wave) walks over the rows that see them within the window,
 // for every head of the group; the rows behind the window of a sink go to workgroups of their own (far), whose
-// sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.
+// sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.  p and ds are rounded to
+// the rows' type for their products like the weights of the forward kernel.
+// dk and dv of 32 keys of 128 columns take 128 registers a lane and the keys' operands 64, so a compute unit holds one wave
+// a SIMD.  PIPE (16-bit rows that fill their padded width): that wave's instructions are laid out by hand, see below;
+// without it the operands are at least read ahead.  32 heads of 16384 rows over 8 key heads, 128 wide, window 4096, bf16:
+// 2.37 ms, four products at 810 TFLOP/s (3.03 ms without PIPE; operands read two steps ahead 2.48, three 2.37, four
+// 2.33; dk and dv in kernels of their own, 5 products but two waves a SIMD, 3.45); 48 heads of 2048 rows, 64 wide,
+// window 2048: 205 us with dq (233 without PIPE).  What is left: about 300 instructions a wave issues for 32 rows, one
+// at a time, against 1024 cycles of the matrix unit.
 template <int P, int IN, bool SHARE, bool PIPE>
 __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_staged_rows<IN, SHARE>(),
@@ -930,8 +946,9 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
     if constexpr (PIPE) {
       // One wave a SIMD has nothing else to do while it waits, so its own matrix and vector instructions are interleaved:
       // the products of the next 32 rows' logits with the weights of these, the next tiles' way into LDS with the
-      // sums.  Three stages: tile `it` and the next are written, the third is being written.  Rows behind the last
-      // are read as the last one, their weights are exp2(-inf).
+      // sums (the barriers of the schedule keep that order).  Three stages: tile `it` and the next are written, the third is
+      // being written; one __syncthreads a tile.  Rows behind the last are read as the last one, their weights are
+      // exp2(-inf).  No tile is left out for a wave that sees none of it: the others' barrier waits for it anyway.
       constexpr int U = BQ * CH / 256;  // 16-byte units of a tensor's tile a thread
       static_assert(U == MT && NSUB == 2);
       uint4 uq[U], ug[U];

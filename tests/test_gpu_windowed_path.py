@@ -6,6 +6,7 @@ import math
 import pytest
 import torch
 
+import benchmark_attention as bench_mod
 import qk_rotary as qkr
 import sink_window_attention as swa
 import window_reference as ref
@@ -119,3 +120,21 @@ def test_two_objects_and_streams():
     for i in range(20):
         assert torch.equal(outs[0][i], a1.step(q[i], k[i], k[19 - i]))
         assert torch.equal(outs[1][i], b1.step(q[i], k[i], k[19 - i]))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_benchmark_command(tmp_path, capsys, dtype):
+    """--window adds its columns behind the others, which stay as they are without it; a window as long as the sequence
+    is exact attention."""
+    plain = bench_mod.main(["--sweep-n", "96", "--repeats", "1", "--csv", str(tmp_path / "a.csv"), "--dtype", dtype])
+    assert list(plain[0]) == list(bench_mod.COLUMNS) and "window" not in capsys.readouterr().out
+    rows = bench_mod.main(["--sweep-n", "96", "300", "--repeats", "1", "--csv", str(tmp_path / "b.csv"), "--dtype", dtype,
+                           "--window", "100", "--sinks", "3"])
+    assert capsys.readouterr().out.splitlines()[1].endswith("coreset_items | window_rel_l2 | window_ms | window_state")
+    header, *lines = (tmp_path / "b.csv").read_text().splitlines()
+    assert header == ",".join(bench_mod.COLUMNS + bench_mod.WINDOW_COLUMNS) and len(lines) == 2
+    elem = 4 if dtype == "float32" else 2
+    assert [r["window_state_bytes"] for r in rows] == [96 * 64 * elem, 103 * 64 * elem]
+    # both round their outputs once (and 16-bit weights once more), the fp32 ones sum 96 products
+    assert rows[0]["window_rel_l2"] <= (1e-5 if dtype == "float32" else 4 * 2.0 ** -8)
+    assert rows[1]["window_rel_l2"] > rows[0]["window_rel_l2"] and rows[1]["window_best_ms"] > 0
