@@ -1270,10 +1270,12 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
     return ((static_cast<int64_t>(bh) * (a.far_chunks + 1) + chunk + 1) * a.sink_rows + j) * (a.d + a.dv);
   };
   auto is_part = [&](int j) { return a.far_chunks > 0 && j < a.sink_rows; };
-  // 4 columns of key j's dk (value 0) or dv (1), where this workgroup has any to give
+  // 4 columns of key j's dk (value 0) or dv (1), where this workgroup has any to give; zero behind the last key (a zero
+  // weight times a row that is not finite may have left a NaN there)
   auto store4 = [&](int j, int value, int col, float x0, float x1, float x2, float x3) {
     const int width = value ? a.dv : a.d;
     if (col >= width) return;
+    if (j >= len) x0 = x1 = x2 = x3 = 0.f;
     if (is_part(j)) {
       float* to = a.part + part_at(j) + (value ? a.d : 0);
       to[col] = x0;

@@ -310,3 +310,58 @@ def test_row_strides_of_single_rows():
     got = (out, *swa.sink_window_backward(far(go), far(q), far(k), far(v), out, lse, window=3, sinks=0))
     for x, y in zip(got, want.values()):
         assert torch.equal(x.cpu(), y.cpu())
+
+
+FULL = [  # many heads whose widths fill their padded ones
+    (4, 64, 32, 300, 128, 128, 70, 5, [300, 131, 1, 64]),
+    (2, 64, 64, 520, 128, 128, 600, 0, None),
+    (6, 32, 32, 257, 64, 64, 30, 140, [257, 129, 128, 65, 0, 200]),
+    (2, 48, 48, 400, 64, 64, 399, 1, [400, 399]),
+    (4, 64, 64, 129, 32, 32, 1, 0, None),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,hk,n,d,dv,window,sinks,lengths", FULL)
+def test_many_heads_of_full_width(b, h, hk, n, d, dv, window, sinks, lengths, dtype):
+    q, k, v, go = make(b, h, hk, n, d, dv, dtype, seed=11)
+    kw = dict(window=window, sinks=sinks, lengths=lengths)
+    check(run(q, k, v, go, **kw), ref.window_attention(q, k, v, grad=go, **kw))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_many_heads_never_read_padding(dtype, d):
+    q, k, v, go = make(4, 64, 32, 200, d, d, dtype, seed=12)
+    kw = dict(window=64, sinks=4, lengths=[70, 131, 0, 199])
+    clean = run(q, k, v, go, **kw)
+    for x in (q, k, v, go):
+        for i, length in enumerate(kw["lengths"]):
+            x[i, :, length:] = math.nan
+    got = run(q, k, v, go, **kw)
+    for name in clean:
+        assert torch.equal(got[name], clean[name]), name
+        for i, length in enumerate(kw["lengths"]):
+            assert not got[name][i, :, length:].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_heads_last_row_of_a_length(dtype):
+    """A query and a gradient that are not finite in a sequence's last row reach what that row sees alone."""
+    b, h, n, window, sinks, length = 4, 64, 200, 40, 3, 135
+    q, k, v, go = make(b, h, h, n, 64, 64, dtype, seed=13)
+    kw = dict(window=window, sinks=sinks, lengths=[length] * b)
+    want = ref.window_attention(q, k, v, grad=go, **kw)
+    see = ref.visible(n, n, window, sinks)[length - 1]
+    q2, g2 = q.clone(), go.clone()
+    q2[1, 5, length - 1, 7] = math.inf
+    g2[2, 6, length - 1, 2] = math.nan
+    got = {name: x.cpu() for name, x in run(q2, k, v, g2, **kw).items()}
+    rows = torch.arange(n) != length - 1
+    for i, head in ((1, 5), (2, 6)):
+        for name in ("out", "dq"):
+            assert ref.over(got[name][i, head][rows], tuple(t[i, head][rows] for t in want[name])) <= 1.0
+        for name in ("dk", "dv"):
+            assert ref.over(got[name][i, head][~see], tuple(t[i, head][~see] for t in want[name])) <= 1.0
+    for name in want:
+        assert ref.over(got[name][0], tuple(t[0] for t in want[name])) <= 1.0
