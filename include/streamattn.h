@@ -463,6 +463,7 @@ int sta_pair_moments(const void* q, const void* k, const void* v, int dtype, int
  *   the element strides of batch, head and row of q, k and v (0 included; rows up to 2^24 bytes apart; no alignment
  *   beyond the element's).  d, dv at most 128 and rows of at least 16 bytes; n <= 2^30.
  *   out [batch][heads][n][dv] dense, 16-byte aligned, in dtype; rows at or behind a length are zero.
+ *   rest (or NULL; not written for fp32): like out, what out's rounding left, for the backward call.
  *   lse [batch][heads][n] fp32 (or NULL): log2 of every row's sum of weights, for the backward call.
  *   window >= 1, sinks >= 0 (either may exceed n); scale any finite number.  Products of 16-bit inputs are exact, fp32
  *   products and all sums and statistics fp32; the weights of 16-bit rows are rounded to 16 bits for the value sums.
@@ -470,7 +471,7 @@ int sta_pair_moments(const void* q, const void* k, const void* v, int dtype, int
  */
 int sta_window_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int heads,
                          int kv_heads, int64_t n, int d, int dv, const int64_t* strides, float scale, int64_t window,
-                         int64_t sinks, const int32_t* lengths, void* out, float* lse, void* stream);
+                         int64_t sinks, const int32_t* lengths, void* out, void* rest, float* lse, void* stream);
 
 /* Bytes of sta_window_attention_backward's workspace; -1 for arguments it refuses. */
 int64_t sta_window_backward_bytes(int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int d, int dv,
@@ -478,12 +479,12 @@ int64_t sta_window_backward_bytes(int dtype, int64_t batch, int heads, int kv_he
 
 /*
  * Gradients of sta_window_attention: dq [batch][heads][n][d], dk [batch][kv_heads][n][d], dv [batch][kv_heads][n][dv],
- * dense, 16-byte aligned, in dtype, from the gradient of out (strides [4][3]: q, k, v, grad), out and lse of the
- * forward call.  Rows at or behind a length get zero gradients and give none.  Sums are taken in a fixed order:
+ * dense, 16-byte aligned, in dtype, from the gradient of out (strides [4][3]: q, k, v, grad), out, rest (or NULL: the
+ * rounding of out then shows in dq and dk) and lse of the forward call.  Rows at or behind a length get zero gradients and give none.  Sums are taken in a fixed order:
  * equal inputs give equal bits.  workspace: caller-allocated, 16-byte aligned (contents undefined before and after).
  */
 int sta_window_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
-                                  const float* lse, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
+                                  const void* rest, const float* lse, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
                                   int d, int dv, const int64_t* strides, float scale, int64_t window, int64_t sinks,
                                   const int32_t* lengths, void* dq, void* dk, void* dv_out, void* workspace,
                                   int64_t workspace_bytes, void* stream);

@@ -165,12 +165,12 @@ _SIGNATURES = {
     "sta_selftest_mfma": (_i32, [_c_p, _c_p, _c_p]),
     "sta_window_attention": (
         _i32, [_c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _c_p, _f32, _i64, _i64, _c_p, _c_p, _c_p,
-               _c_p],  # q k v dtype batch heads kv_heads n d dv strides scale window sinks lengths out lse stream
+               _c_p, _c_p],  # q k v dtype batch heads kv_heads n d dv strides scale window sinks lengths out rest lse stream
     ),
     "sta_window_backward_bytes": (_i64, [_i32, _i64, _i32, _i32, _i64, _i32, _i32, _i64, _i64]),
     "sta_window_attention_backward": (
-        _i32, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _c_p, _f32, _i64, _i64,
-               _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # grad q k v out lse dtype .. lengths dq dk dv ws bytes stream
+        _i32, [_c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _i32, _c_p, _f32, _i64, _i64,
+               _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # grad q k v out rest lse dtype .. lengths dq dk dv ws bytes stream
     ),
     "sta_ring_layout": (_i32, [_i32, _i32, _i64, _i32, _i32, _i32, _i64, _i64, _c_p]),
     "sta_ring_attention_bytes": (_i64, [_i64, _i32, _i32, _i32, _i32, _i64, _i64]),

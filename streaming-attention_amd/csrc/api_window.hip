@@ -126,8 +126,8 @@ extern "C" {
 
 int sta_window_attention(const void* q, const void* k, const void* v, int dtype, int64_t batch, int heads,
                          int kv_heads, int64_t n, int d, int dv, const int64_t* strides, float scale, int64_t window,
-                         int64_t sinks, const int32_t* lengths, void* out, float* lse, void* stream) {
-  if (!q || !k || !v || !out || !strides || !aligned16(out)) return STA_ERR_ARG;
+                         int64_t sinks, const int32_t* lengths, void* out, void* rest, float* lse, void* stream) {
+  if (!q || !k || !v || !out || !strides || !aligned16(out) || !aligned16(rest)) return STA_ERR_ARG;
   sta::WinArgs a;
   if (const int st = window_shape(a, dtype, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
   if (!strides_ok(strides, 3, dtype)) return STA_ERR_UNSUPPORTED;
@@ -136,6 +136,7 @@ int sta_window_attention(const void* q, const void* k, const void* v, int dtype,
   a.v = rows_of(v, strides + 6);
   a.lengths = lengths;
   a.out = out;
+  a.rest = rest;
   a.lse = lse;
   return dispatch(false, a, dtype, stream);
 }
@@ -149,12 +150,12 @@ int64_t sta_window_backward_bytes(int dtype, int64_t batch, int heads, int kv_he
 }
 
 int sta_window_attention_backward(const void* grad, const void* q, const void* k, const void* v, const void* out,
-                                  const float* lse, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
+                                  const void* rest, const float* lse, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
                                   int d, int dv, const int64_t* strides, float scale, int64_t window, int64_t sinks,
                                   const int32_t* lengths, void* dq, void* dk, void* dv_out, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
   if (!grad || !q || !k || !v || !out || !lse || !strides || !dq || !dk || !dv_out || !workspace) return STA_ERR_ARG;
-  if (!aligned16(out) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv_out) || !aligned16(workspace))
+  if (!aligned16(out) || !aligned16(rest) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv_out) || !aligned16(workspace))
     return STA_ERR_ARG;
   sta::WinArgs a;
   if (const int st = window_shape(a, dtype, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
@@ -167,6 +168,7 @@ int sta_window_attention_backward(const void* grad, const void* q, const void* k
   a.go = rows_of(grad, strides + 9);
   a.lengths = lengths;
   a.out = const_cast<void*>(out);
+  a.rest = const_cast<void*>(rest);
   a.lse = const_cast<float*>(lse);
   a.delta = static_cast<float*>(workspace);
   a.part = a.delta + delta_floats(a);

@@ -41,6 +41,7 @@ struct WinArgs {
   float scale;             // the scale itself
   const int* lengths;      // [batch] or null
   void* out;               // [batch][heads][n][dv]
+  void* rest;              // [batch][heads][n][dv]: what the rounding of out left, rounded; or null
   float* lse;              // [batch][heads][n]: log2 of the row's sum of weights, or null
   float* delta;            // [batch][heads][n]: D_i
   void *dq, *dk, *dv_out;  // [batch][heads][n][d], [batch][kv heads][n][d | dv]
@@ -280,6 +281,28 @@ __device__ __forceinline__ float win_wave_sum(float x) {
   return x;
 }
 
+// what the rounding of x to the rows' type leaves (0 of an infinity or NaN)
+template <int IN>
+__device__ __forceinline__ float win_rest(float x) {
+  float y;
+  if constexpr (IN == F16)
+    y = static_cast<float>(static_cast<_Float16>(x));
+  else
+    y = __uint_as_float(pk_bf16(x, 0.f) << 16);
+  return win_finite(y) ? x - y : 0.f;
+}
+
+// four values of a row of out, and of what their rounding leaves
+template <int IN>
+__device__ __forceinline__ void win_store_out(const WinArgs& a, int64_t row_at, int col, float x0, float x1, float x2,
+                                              float x3) {
+  win_store4<IN>(a.out, row_at, col, a.dv, x0, x1, x2, x3);
+  if constexpr (IN != F32) {
+    if (a.rest)
+      win_store4<IN>(a.rest, row_at, col, a.dv, win_rest<IN>(x0), win_rest<IN>(x1), win_rest<IN>(x2), win_rest<IN>(x3));
+  }
+}
+
 template <int IN>
 __device__ __forceinline__ float win_dot(const void* x, const void* y, int width) {
   float s = 0.f;
@@ -335,7 +358,12 @@ __device__ void win_forward_row(const WinArgs& a, int b, int h, int i) {
   const int64_t row = (static_cast<int64_t>(b) * a.heads + h) * a.n + i;
 #pragma unroll
   for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.dv) store_elem(a.out, row * a.dv + lane + 64 * e, IN, acc[e] / l);
+    if (lane + 64 * e < a.dv) {
+      store_elem(a.out, row * a.dv + lane + 64 * e, IN, acc[e] / l);
+      if constexpr (IN != F32) {
+        if (a.rest) store_elem(a.rest, row * a.dv + lane + 64 * e, IN, win_rest<IN>(acc[e] / l));
+      }
+    }
   if (a.lse && lane == 0) a.lse[row] = m * 1.44269504f + log2f(l);
 }
 
@@ -573,8 +601,8 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       for (int j = 0; j < MT; ++j) {
         const int col = 32 * j + 4 * (threadIdx.x & 7);
         if (col < a.dv)
-          win_store4<IN>(a.out, (head_row + at_row) * a.dv, col, a.dv, in ? o[j][0] * inv : 0.f, in ? o[j][1] * inv : 0.f,
-                         in ? o[j][2] * inv : 0.f, in ? o[j][3] * inv : 0.f);
+          win_store_out<IN>(a, (head_row + at_row) * a.dv, col, in ? o[j][0] * inv : 0.f, in ? o[j][1] * inv : 0.f,
+                            in ? o[j][2] * inv : 0.f, in ? o[j][3] * inv : 0.f);
       }
       if (a.lse && (threadIdx.x & 7) == 0)
         a.lse[head_row + at_row] = in ? top * a.c + __builtin_amdgcn_logf(den) : 0.f;
@@ -604,8 +632,8 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       for (int r = 0; r < 4; ++r) {
         const int col = 32 * mt + 8 * r + 4 * hh;
         if (col < a.dv)
-          win_store4<IN>(a.out, at, col, a.dv, in ? acc[mt][4 * r] * inv : 0.f, in ? acc[mt][4 * r + 1] * inv : 0.f,
-                         in ? acc[mt][4 * r + 2] * inv : 0.f, in ? acc[mt][4 * r + 3] * inv : 0.f);
+          win_store_out<IN>(a, at, col, in ? acc[mt][4 * r] * inv : 0.f, in ? acc[mt][4 * r + 1] * inv : 0.f,
+                            in ? acc[mt][4 * r + 2] * inv : 0.f, in ? acc[mt][4 * r + 3] * inv : 0.f);
       }
     if (a.lse && hh == 0) a.lse[head_row + row] = in ? m * a.c + __builtin_amdgcn_logf(l) : 0.f;
   }
@@ -645,7 +673,9 @@ __device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
     if (lane + 64 * e < a.d) store_elem(a.dq, row * a.d + lane + 64 * e, IN, a.scale * acc[e]);
 }
 
-// dq and D: the forward kernel's walk over the keys with the rows' statistics given.  ds is rounded to the rows' type for
+// dq and D: the forward kernel's walk over the keys with the rows' statistics given.  D of a rounded out is off by do.(out -
+// o), the same for all keys of a row, which adds about a tenth to the gradients' rounding errors (a third with windows of 16
+// keys); with what the rounding left (rest) it is not.  ds is rounded to the rows' type for
 // its product with the keys like the weights of the forward kernel.  32 heads of 16384 rows, 128 wide, window 4096,
 // bf16: 1.45 ms, three products at 995 TFLOP/s, bound by them.
 template <int P, int IN, bool SHARE>
@@ -675,7 +705,8 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : 2) void w
     const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
     const char* qrow = rows_at<ES>(a.q, b, h, in ? row : 0);
     const char* grow = rows_at<ES>(a.go, b, h, in ? row : 0);
-    const char* orow = static_cast<const char*>(a.out) + (head_row + (in ? row : 0)) * a.dv * ES;
+    const int64_t orow_at = (head_row + (in ? row : 0)) * a.dv * ES;
+    const char* orow = static_cast<const char*>(a.out) + orow_at;
 #pragma unroll
     for (int s = 0; s < P / 16; ++s) {
       qf[s] = win_load_row<IN>(qrow, s, hh, a.d, flip);
@@ -686,6 +717,14 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : 2) void w
       win_keep<IN>(o, in);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta = fmaf(load_elem(&gf[s], j, IN), load_elem(&o, j, IN), delta);
+      if constexpr (IN != F32) {
+        if (a.rest) {
+          o = win_load_row<IN>(static_cast<const char*>(a.rest) + orow_at, s, hh, a.dv, 0u);
+          win_keep<IN>(o, in);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) delta = fmaf(load_elem(&gf[s], j, IN), load_elem(&o, j, IN), delta);
+        }
+      }
     }
     delta += __shfl_xor(delta, 32);
     const float lse = in ? a.lse[head_row + row] : 0.f;

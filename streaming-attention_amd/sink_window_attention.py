@@ -134,28 +134,29 @@ def _widen(x: Tensor) -> Tensor:
 
 
 def _forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: float, lengths: Optional[Tensor],
-             with_lse: bool) -> Tuple[Tensor, Optional[Tensor]]:
+             with_lse: bool, with_rest: bool) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
     b, h, n, d = q.shape
     dv = v.shape[3]
     out = torch.empty((b, h, n, dv), device=q.device, dtype=q.dtype)
+    rest = torch.empty_like(out) if with_rest and q.dtype != torch.float32 else None
     lse = torch.empty((b, h, n), device=q.device, dtype=torch.float32) if with_lse else None
     if out.numel() == 0:
-        return out, lse
+        return out, rest, lse
     if min(d, dv) * q.element_size() < 16:
-        wide, lse = _forward(_widen(q), _widen(k), _widen(v), window, sinks, scale, lengths, with_lse)
-        return out.copy_(wide[..., :dv]), lse
+        wide = _forward(_widen(q), _widen(k), _widen(v), window, sinks, scale, lengths, with_lse, with_rest)
+        return out.copy_(wide[0][..., :dv]), None if rest is None else rest.copy_(wide[1][..., :dv]), wide[2]
     q, k, v = _rows(q), _rows(k), _rows(v)
     with _on(q.device):
         st = _native.lib().sta_window_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, k.shape[1], n, d, dv,
-            _strides(q, k, v), scale, window, sinks, _native.ptr(lengths), out.data_ptr(), _native.ptr(lse),
-            _native.stream_handle(q.device))
+            _strides(q, k, v), scale, window, sinks, _native.ptr(lengths), out.data_ptr(), _native.ptr(rest),
+            _native.ptr(lse), _native.stream_handle(q.device))
     _native.check(st, "sta_window_attention")
-    return out, lse
+    return out, rest, lse
 
 
-def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, window: int, sinks: int,
-              scale: float, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
+def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, rest: Optional[Tensor], lse: Tensor,
+              window: int, sinks: int, scale: float, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
     b, h, n, d = q.shape
     hk, dv = k.shape[1], v.shape[3]
     dq = torch.empty((b, h, n, d), device=q.device, dtype=q.dtype)
@@ -164,9 +165,11 @@ def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: T
     if dq.numel() == 0:
         return dq, dk.zero_(), dvo.zero_()
     if min(d, dv) * q.element_size() < 16:
-        wide = _backward(*(_widen(x) for x in (grad, q, k, v, out)), lse, window, sinks, scale, lengths)
+        wide = _backward(*(_widen(x) for x in (grad, q, k, v, out)), None if rest is None else _widen(rest), lse, window,
+                         sinks, scale, lengths)
         return dq.copy_(wide[0][..., :d]), dk.copy_(wide[1][..., :d]), dvo.copy_(wide[2][..., :dv])
     grad, q, k, v, out, lse = _rows(grad), _rows(q), _rows(k), _rows(v), _dense(out), lse.contiguous()
+    rest = None if rest is None else _dense(rest)
     lib = _native.lib()
     with _on(q.device):
         nbytes = lib.sta_window_backward_bytes(_native.DTYPE_CODES[q.dtype], b, h, hk, n, d, dv, window, sinks)
@@ -174,7 +177,7 @@ def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: T
             raise _native.NativeError("sta_window_backward_bytes refused the shape")
         ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
         st = lib.sta_window_attention_backward(
-            grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _native.ptr(rest), lse.data_ptr(),
             _native.DTYPE_CODES[q.dtype], b, h, hk, n, d, dv, _strides(q, k, v, grad), scale, window, sinks,
             _native.ptr(lengths), dq.data_ptr(), dk.data_ptr(), dvo.data_ptr(), ws.data_ptr(), nbytes,
             _native.stream_handle(q.device))
@@ -194,8 +197,8 @@ class _SinkWindow(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, lengths):
         _refuse_capture()
-        out, lse = _forward(q, k, v, window, sinks, scale, lengths, True)
-        ctx.save_for_backward(q, k, v, out, lse, lengths)
+        out, rest, lse = _forward(q, k, v, window, sinks, scale, lengths, True, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, lengths)
         ctx.settings = window, sinks, scale
         return out
 
@@ -203,8 +206,8 @@ class _SinkWindow(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         _refuse_capture()
-        q, k, v, out, lse, lengths = ctx.saved_tensors
-        dq, dk, dv = _backward(grad, q, k, v, out, lse, *ctx.settings, lengths)
+        q, k, v, out, rest, lse, lengths = ctx.saved_tensors
+        dq, dk, dv = _backward(grad, q, k, v, out, rest, lse, *ctx.settings, lengths)
         return dq, dk, dv, None, None, None, None
 
 
@@ -226,45 +229,53 @@ def sink_window_causal_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int
     scale: 1/sqrt(D) when None.  lengths: int32 [B] on the device, the rows of every sequence of a padded batch
     (values outside 0 .. N are taken as the nearest of them); output rows behind them are zero and take no part in the
     gradients, whatever the padding holds.
-    The output has q's dtype.  Differentiable calls cannot be captured into a graph (RuntimeError); use
-    sink_window_forward and sink_window_backward there."""
+    The output has q's dtype; with gradients a 16-bit call also keeps what the output's rounding left.  Differentiable
+    calls cannot be captured into a graph (RuntimeError); use sink_window_forward and sink_window_backward there."""
     q4, k4, v4, window, sinks, s, lengths = _checked(q, k, v, window, sinks, scale, lengths)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         out = _SinkWindow.apply(q4, k4, v4, window, sinks, s, lengths)
     else:
-        out = _forward(q4, k4, v4, window, sinks, s, lengths, False)[0]
+        out = _forward(q4, k4, v4, window, sinks, s, lengths, False, False)[0]
     return out[0, 0] if q.ndim == 2 else out
 
 
 @torch.no_grad()
 def sink_window_forward(q: Tensor, k: Tensor, v: Tensor, *, window: int, sinks: int = 4,
-                        scale: Optional[float] = None, lengths: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+                        scale: Optional[float] = None, lengths: Optional[Tensor] = None,
+                        with_rest: bool = False) -> Tuple[Tensor, ...]:
     """sink_window_causal_attention's output and its row statistics [B,H,N] ([N] for [N,D] tensors): log2 of every
-    row's sum of weights, float32, as sink_window_backward takes them.  May be captured into a graph."""
+    row's sum of weights, float32, as sink_window_backward takes them.  with_rest: also what the output's rounding left,
+    like the output (None for float32), which keeps that rounding out of the gradients.  May be captured into a graph."""
     q4, k4, v4, window, sinks, s, lengths = _checked(q, k, v, window, sinks, scale, lengths)
-    out, lse = _forward(q4, k4, v4, window, sinks, s, lengths, True)
-    return (out[0, 0], lse[0, 0]) if q.ndim == 2 else (out, lse)
+    out, rest, lse = _forward(q4, k4, v4, window, sinks, s, lengths, True, with_rest)
+    if q.ndim == 2:
+        out, rest, lse = out[0, 0], None if rest is None else rest[0, 0], lse[0, 0]
+    return (out, lse, rest) if with_rest else (out, lse)
 
 
 @torch.no_grad()
 def sink_window_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, lse: Tensor, *, window: int,
-                         sinks: int = 4, scale: Optional[float] = None,
-                         lengths: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+                         sinks: int = 4, scale: Optional[float] = None, lengths: Optional[Tensor] = None,
+                         rest: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """(dq, dk, dv) of sink_window_causal_attention for the output's gradient `grad`, from the inputs and results of
-    sink_window_forward with the same settings.  May be captured into a graph."""
+    sink_window_forward with the same settings (rest: its third result, if it was asked for).  May be captured into a
+    graph."""
     q4, k4, v4, window, sinks, s, lengths = _checked(q, k, v, window, sinks, scale, lengths)
     if q.ndim == 2:
         if grad.ndim != 2 or out.ndim != 2 or lse.ndim != 1:
             raise ValueError("for [N,D] inputs grad and out must be [N,Dv] and lse [N]")
         grad, out, lse = grad[None, None], out[None, None], lse[None, None]
+        rest = None if rest is None else rest[None, None]
     want = (*q4.shape[:3], v4.shape[3])
     if tuple(grad.shape) != want or tuple(out.shape) != want or tuple(lse.shape) != want[:3]:
         raise ValueError(f"grad and out must be {want} and lse {want[:3]}")
     _check_dtype(q4, grad, out)
+    if rest is not None and (q4.dtype == torch.float32 or rest.shape != out.shape or rest.dtype != out.dtype):
+        raise ValueError("rest must be like out, and None for float32")
     if lse.dtype != torch.float32:
         raise ValueError("lse must be float32")
-    _check_gpu(q4, grad, out, lse)
-    dq, dk, dv = _backward(grad, q4, k4, v4, out, lse, window, sinks, s, lengths)
+    _check_gpu(q4, grad, out, lse, rest)
+    dq, dk, dv = _backward(grad, q4, k4, v4, out, rest, lse, window, sinks, s, lengths)
     return (dq[0, 0], dk[0, 0], dv[0, 0]) if q.ndim == 2 else (dq, dk, dv)
 
 

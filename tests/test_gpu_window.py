@@ -365,3 +365,32 @@ def test_many_heads_last_row_of_a_length(dtype):
             assert ref.over(got[name][i, head][~see], tuple(t[i, head][~see] for t in want[name])) <= 1.0
     for name in want:
         assert ref.over(got[name][0], tuple(t[0] for t in want[name])) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("b,h,hk,n,d,dv,window,lengths", [(1, 2, 1, 500, 64, 48, 16, None), (2, 3, 3, 200, 93, 33, 40, [200, 77]),
+                                                          (4, 64, 64, 300, 64, 64, 20, None), (1, 1, 1, 70, 5, 3, 9, None)])
+def test_rest_of_the_output(b, h, hk, n, d, dv, window, lengths, dtype):
+    """What the output's rounding left is at most half a step of it; with it the gradients lose that rounding."""
+    q, k, v, go = make(b, h, hk, n, d, dv, dtype, seed=14)
+    want = ref.window_attention(q, k, v, grad=go, window=window, sinks=2, lengths=lengths)
+    kw = dict(window=window, sinks=2, lengths=None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=DEV))
+    x = [t.to(DEV) for t in (q, k, v)]
+    out, lse, rest = swa.sink_window_forward(*x, with_rest=True, **kw)
+    assert torch.equal(out, swa.sink_window_forward(*x, **kw)[0])
+    # half a step, or half the smallest step of the type
+    smallest = torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+    half = (out.abs().double() * torch.finfo(dtype).eps / 2).clamp_min(smallest / 2)
+    assert rest.dtype == dtype and torch.all(rest.double().abs() <= half * (1 + torch.finfo(dtype).eps) + smallest)
+    with_rest = swa.sink_window_backward(go.to(DEV), *x, out, lse, rest=rest, **kw)
+    without = swa.sink_window_backward(go.to(DEV), *x, out, lse, **kw)
+    grads = dict(zip(("dq", "dk", "dv"), with_rest))
+    check(grads, {name: want[name] for name in grads})
+    for name, a, b_ in zip(("dq", "dk"), with_rest, without):
+        error = [(t.cpu().double() - want[name][0]).norm() for t in (a, b_)]
+        assert error[0] < error[1], (name, error)
+    assert torch.equal(with_rest[2], without[2])
+    # the differentiable call keeps it
+    got = run(q, k, v, go, window=window, sinks=2, lengths=lengths)
+    for name in grads:
+        assert torch.equal(got[name], grads[name])

@@ -123,10 +123,10 @@ def test_library_refuses_without_touching_a_device():
     st = (ctypes.c_int64 * 12)(*([64] * 12))
     E = _native
 
-    def fwd(q=16, k=16, v=16, dt=0, b=1, h=2, hk=1, n=8, d=8, dv=8, s=st, scale=1.0, w=4, sinks=1, out=16):
-        return lib.sta_window_attention(q, k, v, dt, b, h, hk, n, d, dv, s, scale, w, sinks, None, out, None, None)
+    def fwd(q=16, k=16, v=16, dt=0, b=1, h=2, hk=1, n=8, d=8, dv=8, s=st, scale=1.0, w=4, sinks=1, out=16, rest=None):
+        return lib.sta_window_attention(q, k, v, dt, b, h, hk, n, d, dv, s, scale, w, sinks, None, out, rest, None, None)
 
-    for kw, want in [(dict(q=None), E.STA_ERR_ARG), (dict(out=None), E.STA_ERR_ARG), (dict(out=8), E.STA_ERR_ARG),
+    for kw, want in [(dict(q=None), E.STA_ERR_ARG), (dict(out=None), E.STA_ERR_ARG), (dict(out=8), E.STA_ERR_ARG), (dict(rest=8), E.STA_ERR_ARG),
                      (dict(s=None), E.STA_ERR_ARG), (dict(dt=3), E.STA_ERR_DTYPE), (dict(b=0), E.STA_ERR_SHAPE),
                      (dict(h=3, hk=2), E.STA_ERR_SHAPE), (dict(n=0), E.STA_ERR_SHAPE), (dict(d=129), E.STA_ERR_UNSUPPORTED),
                      (dict(dv=129), E.STA_ERR_UNSUPPORTED), (dict(d=3), E.STA_ERR_UNSUPPORTED),
@@ -138,10 +138,10 @@ def test_library_refuses_without_touching_a_device():
     assert lib.sta_window_backward_bytes(0, 1, 2, 1, 8, 8, 8, 0, 1) == -1
     need = lib.sta_window_backward_bytes(0, 1, 2, 1, 1000, 8, 8, 100, 4)
     assert need >= 4 * 2 * 1000
-    back = [16] * 6 + [0, 1, 2, 1, 1000, 8, 8, st, 1.0, 100, 4, None, 16, 16, 16, 16]
+    back = [16] * 5 + [None, 16, 0, 1, 2, 1, 1000, 8, 8, st, 1.0, 100, 4, None, 16, 16, 16, 16]
     assert lib.sta_window_attention_backward(*back, need - 1, None) == E.STA_ERR_SCRATCH
     assert lib.sta_window_attention_backward(None, *back[1:], need, None) == E.STA_ERR_ARG
-    wide = [16] * 6 + [0, 1 << 23, 2, 1, 1, 8, 8, st, 1.0, 100, 4, None, 16, 16, 16, 16]
+    wide = [16] * 5 + [None, 16, 0, 1 << 23, 2, 1, 1, 8, 8, st, 1.0, 100, 4, None, 16, 16, 16, 16]
     assert lib.sta_window_attention_backward(*wide, 1 << 40, None) == E.STA_ERR_SHAPE
 
     rot = dict(q=16, k=16, dt=0, b=1, h=2, hk=1, n=8, d=8, s=st, qw=None, kw=None, wt=0, table=16, limit=8, r=8, i=0,
@@ -231,3 +231,11 @@ def test_held_values():
     row = torch.tensor([4.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 5.1, -0.3, 7.9])
     assert ref.as_held(row, "fp4").tolist() == [4.0, 0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0, 6.0, -0.5, 6.0]
     assert ref.as_held(row * 2.0 ** 20, "fp4").tolist() == [x * 2.0 ** 20 for x in ref.as_held(row, "fp4").tolist()]
+
+
+@pytest.mark.parametrize("dtype,rest", [(torch.float32, x(3, 8)), (torch.float16, x(3, 8)), (torch.float16, x(3, 7, dtype=torch.float16))])
+def test_backward_refuses_another_rest(monkeypatch, dtype, rest):
+    monkeypatch.setattr(swa, "_check_gpu", lambda *a: None)
+    t = x(3, 8, dtype=dtype)
+    with pytest.raises(ValueError, match="rest must be like out"):
+        swa.sink_window_backward(t, t, t, t, t, x(3), window=2, rest=rest)
