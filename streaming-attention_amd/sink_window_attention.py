@@ -194,10 +194,17 @@ def _refuse_capture() -> None:
 
 
 class _SinkWindow(torch.autograd.Function):
+    """[N,D] tensors become [1,1,N,D] in here: the gradients of views taken outside are launches of their own (100 us of
+    a small training step)."""
+
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, scale, lengths):
         _refuse_capture()
-        out, rest, lse = _forward(q, k, v, window, sinks, scale, lengths, True, True)
+        ctx.flat = q.ndim == 2
+        q4, k4, v4 = (q[None, None], k[None, None], v[None, None]) if ctx.flat else (q, k, v)
+        out, rest, lse = _forward(q4, k4, v4, window, sinks, scale, lengths, True, True)
+        if ctx.flat:
+            out = out[0, 0]
         ctx.save_for_backward(q, k, v, out, rest, lse, lengths)
         ctx.settings = window, sinks, scale
         return out
@@ -207,8 +214,12 @@ class _SinkWindow(torch.autograd.Function):
     def backward(ctx, grad):
         _refuse_capture()
         q, k, v, out, rest, lse, lengths = ctx.saved_tensors
-        dq, dk, dv = _backward(grad, q, k, v, out, rest, lse, *ctx.settings, lengths)
-        return dq, dk, dv, None, None, None, None
+        if ctx.flat:
+            grad, q, k, v, out = (x[None, None] for x in (grad, q, k, v, out))
+        grads = _backward(grad, q, k, v, out, rest, lse, *ctx.settings, lengths)
+        if ctx.flat:
+            grads = (x[0, 0] for x in grads)
+        return *grads, None, None, None, None
 
 
 def _checked(q, k, v, window, sinks, scale, lengths):
@@ -233,9 +244,8 @@ def sink_window_causal_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int
     calls cannot be captured into a graph (RuntimeError); use sink_window_forward and sink_window_backward there."""
     q4, k4, v4, window, sinks, s, lengths = _checked(q, k, v, window, sinks, scale, lengths)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out = _SinkWindow.apply(q4, k4, v4, window, sinks, s, lengths)
-    else:
-        out = _forward(q4, k4, v4, window, sinks, s, lengths, False, False)[0]
+        return _SinkWindow.apply(q, k, v, window, sinks, s, lengths)
+    out = _forward(q4, k4, v4, window, sinks, s, lengths, False, False)[0]
     return out[0, 0] if q.ndim == 2 else out
 
 
