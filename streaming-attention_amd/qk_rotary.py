@@ -15,7 +15,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 import _native
-from sink_window_attention import _check_gpu, _on, _refuse_capture, _strides
+from sink_window_attention import _check_gpu, _differentiable_once, _like, _on, _refuse_capture, _strides
 
 Tensor = torch.Tensor
 
@@ -106,8 +106,7 @@ class _Call:
         b, h, hk, n, d = self.shape
         q, k = _walkable(self.rows(q)), _walkable(self.rows(k))
         qw, kw = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-        yq = torch.empty((b, h, n, d), device=q.device, dtype=q.dtype)
-        yk = torch.empty((b, hk, n, d), device=q.device, dtype=q.dtype)
+        yq, yk = _like(q), _like(k)
         if b * n and h + hk:
             with _on(q.device):
                 st = _native.lib().sta_head_rotary(
@@ -120,15 +119,14 @@ class _Call:
         b, h, hk, n, d = self.shape
         q, k, gq, gk = (_walkable(self.rows(x)) for x in (q, k, gq, gk))
         qw, kw = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
-        dq = torch.empty((b, h, n, d), device=q.device, dtype=q.dtype)
-        dk = torch.empty((b, hk, n, d), device=q.device, dtype=q.dtype)
+        dq, dk = _like(q), _like(k)
         empty = not (b * n and h + hk)
         dw = [None if w is None else (torch.zeros_like(w) if empty or not heads else torch.empty_like(w))
               for w, heads in ((qw, h), (kw, hk))]
         if not empty:
             lib = _native.lib()
             nbytes = lib.sta_head_rotary_backward_bytes(b, h, hk, n, d)
-            ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+            ws = q.new_empty(nbytes, dtype=torch.uint8)
             with _on(q.device):
                 st = lib.sta_head_rotary_backward(
                     gq.data_ptr(), gk.data_ptr(), q.data_ptr(), k.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, hk,
@@ -151,7 +149,7 @@ class _NormRotary(torch.autograd.Function):
         return call.forward(q, k, q_weight, k_weight)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, gq, gk):
         _refuse_capture()
         q, k, q_weight, k_weight, _, _ = ctx.saved_tensors  # table and positions: checked to be as they were

@@ -110,6 +110,11 @@ def _dense(x: Tensor) -> Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+def _like(x: Tensor) -> Tensor:
+    """A dense tensor like x, its values not set (half the host time of torch.empty)."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 _STRIDES = {n: ctypes.c_int64 * n for n in (6, 9, 12)}
 
 
@@ -137,9 +142,9 @@ def _forward(q: Tensor, k: Tensor, v: Tensor, window: int, sinks: int, scale: fl
              with_lse: bool, with_rest: bool) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor]]:
     b, h, n, d = q.shape
     dv = v.shape[3]
-    out = torch.empty((b, h, n, dv), device=q.device, dtype=q.dtype)
-    rest = torch.empty_like(out) if with_rest and q.dtype != torch.float32 else None
-    lse = torch.empty((b, h, n), device=q.device, dtype=torch.float32) if with_lse else None
+    out = _like(q) if d == dv else q.new_empty((b, h, n, dv))
+    rest = _like(out) if with_rest and q.dtype != torch.float32 else None
+    lse = q.new_empty((b, h, n), dtype=torch.float32) if with_lse else None
     if out.numel() == 0:
         return out, rest, lse
     if min(d, dv) * q.element_size() < 16:
@@ -159,9 +164,7 @@ def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, rest: 
               window: int, sinks: int, scale: float, lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor, Tensor]:
     b, h, n, d = q.shape
     hk, dv = k.shape[1], v.shape[3]
-    dq = torch.empty((b, h, n, d), device=q.device, dtype=q.dtype)
-    dk = torch.empty((b, hk, n, d), device=q.device, dtype=q.dtype)
-    dvo = torch.empty((b, hk, n, dv), device=q.device, dtype=q.dtype)
+    dq, dk, dvo = _like(q), _like(k), _like(v)
     if dq.numel() == 0:
         return dq, dk.zero_(), dvo.zero_()
     if min(d, dv) * q.element_size() < 16:
@@ -175,7 +178,7 @@ def _backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Tensor, rest: 
         nbytes = lib.sta_window_backward_bytes(_native.DTYPE_CODES[q.dtype], b, h, hk, n, d, dv, window, sinks)
         if nbytes < 0:
             raise _native.NativeError("sta_window_backward_bytes refused the shape")
-        ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+        ws = q.new_empty(nbytes, dtype=torch.uint8)
         st = lib.sta_window_attention_backward(
             grad.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _native.ptr(rest), lse.data_ptr(),
             _native.DTYPE_CODES[q.dtype], b, h, hk, n, d, dv, _strides(q, k, v, grad), scale, window, sinks,
@@ -191,6 +194,12 @@ def _refuse_capture() -> None:
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("differentiable calls cannot be captured into a graph: call the forward and backward "
                            "functions by themselves, or run under torch.no_grad()")
+
+
+def _differentiable_once(backward):
+    """once_differentiable where a graph of the gradients is asked for; without one its wrapping costs 5 us a call."""
+    once = torch.autograd.function.once_differentiable(backward)
+    return lambda ctx, *grads: once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
 
 class _SinkWindow(torch.autograd.Function):
@@ -210,7 +219,7 @@ class _SinkWindow(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_differentiable_once
     def backward(ctx, grad):
         _refuse_capture()
         q, k, v, out, rest, lse, lengths = ctx.saved_tensors
@@ -338,6 +347,9 @@ class SinkWindowStreamingAttention:
         self._cache = [torch.zeros(n, device=self.device, dtype=torch.uint8) if n else None for n in sizes]
         self._counts = torch.zeros((streams, kv_heads), device=self.device, dtype=torch.int32)
         self._state = (*(_native.ptr(x) for x in self._cache), self._counts.data_ptr())
+        self._shapes = {"query": (streams, heads, dim), "key": (streams, kv_heads, dim),
+                        "value": (streams, kv_heads, value_dim)}
+        self._dense = _STRIDES[6](heads * dim, dim, kv_heads * dim, dim, kv_heads * value_dim, value_dim)
         self._bytes = _native.lib().sta_ring_attention_bytes(streams, heads, kv_heads, dim, value_dim, self.window,
                                                              self.sinks)
         self._fresh = True
@@ -349,18 +361,21 @@ class SinkWindowStreamingAttention:
         return self._counts[:, 0]
 
     def _rows(self, x: Tensor, want: Tuple[int, ...], what: str) -> Tensor:
-        if tuple(x.shape) != want:
+        if x.shape != want:
             raise ValueError(f"{what} must be {list(want)}, got {list(x.shape)}")
         if x.dtype != self.dtype or x.device != self.device:
             x = x.to(device=self.device, dtype=self.dtype)
-        return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+        return x if x.is_contiguous() or x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
     def _attend(self, q: Tensor, k: Optional[Tensor], v: Optional[Tensor]) -> Tensor:
-        out = torch.empty((self.streams, self.heads, self.value_dim), device=self.device, dtype=self.dtype)
-        ws = torch.empty(self._bytes, device=self.device, dtype=torch.uint8) if self._bytes else None
-        none = (0, 0)
-        strides = _STRIDES[6](*q.stride()[:2], *(none if k is None else k.stride()[:2]),
-                              *(none if v is None else v.stride()[:2]))
+        out = _like(q) if self.dim == self.value_dim else q.new_empty((self.streams, self.heads, self.value_dim))
+        ws = q.new_empty(self._bytes, dtype=torch.uint8) if self._bytes else None
+        if q.is_contiguous() and (k is None or (k.is_contiguous() and v.is_contiguous())):
+            strides = self._dense
+        else:
+            none = (0, 0)
+            strides = _STRIDES[6](*q.stride()[:2], *(none if k is None else k.stride()[:2]),
+                                  *(none if v is None else v.stride()[:2]))
         with _on(self.device):
             st = _native.lib().sta_ring_attention(
                 q.data_ptr(), _native.ptr(k), _native.ptr(v), self._code, self._store, self.streams, self.heads,
@@ -371,21 +386,22 @@ class SinkWindowStreamingAttention:
 
     def step(self, query: Tensor, key: Tensor, value: Tensor) -> Tensor:
         """One token of every stream into the cache, then one query a head: update(key, value); query(query)."""
-        q = self._rows(query, (self.streams, self.heads, self.dim), "query")
-        k = self._rows(key, (self.streams, self.kv_heads, self.dim), "key")
-        v = self._rows(value, (self.streams, self.kv_heads, self.value_dim), "value")
+        shapes = self._shapes
+        q = self._rows(query, shapes["query"], "query")
+        k = self._rows(key, shapes["key"], "key")
+        v = self._rows(value, shapes["value"], "value")
         self._fresh = False
         return self._attend(q, k, v)
 
     def query(self, query: Tensor) -> Tensor:
         """Attention of one query a head over the tokens held; zero for a stream that holds none."""
-        return self._attend(self._rows(query, (self.streams, self.heads, self.dim), "query"), None, None)
+        return self._attend(self._rows(query, self._shapes["query"], "query"), None, None)
 
     @torch.no_grad()
     def update(self, key: Tensor, value: Tensor) -> None:
         """One token of every stream into the cache."""
-        k = self._rows(key, (self.streams, self.kv_heads, self.dim), "key")
-        v = self._rows(value, (self.streams, self.kv_heads, self.value_dim), "value")
+        k = self._rows(key, self._shapes["key"], "key")
+        v = self._rows(value, self._shapes["value"], "value")
         self._extend(k[:, :, None], v[:, :, None], None)
 
     def _extend(self, k: Tensor, v: Tensor, counts: Optional[Tensor]) -> None:

@@ -138,3 +138,15 @@ def test_benchmark_command(tmp_path, capsys, dtype):
     # both round their outputs once (and 16-bit weights once more), the fp32 ones sum 96 products
     assert rows[0]["window_rel_l2"] <= (1e-5 if dtype == "float32" else 4 * 2.0 ** -8)
     assert rows[1]["window_rel_l2"] > rows[0]["window_rel_l2"] and rows[1]["window_best_ms"] > 0
+
+
+def test_second_derivatives_are_refused():
+    """A graph of the gradients may be asked for; a derivative of them is an error and not a silent zero."""
+    q, k, v = (torch.randn(1, 2, 40, 32, device=DEV).requires_grad_() for _ in range(3))
+    table = qkr.rotary_table(64, 32, device=DEV)
+    for out in (swa.sink_window_causal_attention(q, k, v, window=8), qkr.qk_norm_rotary(q, k, table)[0]):
+        plain = torch.autograd.grad(out.square().sum(), q, retain_graph=True)[0]
+        dq = torch.autograd.grad(out.square().sum(), q, create_graph=True)[0]
+        assert torch.equal(plain, dq)
+        with pytest.raises(RuntimeError, match="differentiate twice"):
+            dq.sum().backward()
