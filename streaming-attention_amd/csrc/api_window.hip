@@ -34,16 +34,20 @@ bool strides_ok(const int64_t* strides, int tensors, int dtype) {
   return true;
 }
 
-// The number of 128-row tiles below which the waves of a workgroup share 32 rows instead (the card has 256 compute
-// units).  Long windows gain more, short ones pay for staging a tile's keys four times; fp32 products take 16 times as
-// long, so balance counts for more.  Wide / shared, forward + gradients, 2048 rows a head:
-//   bf16, d = 64, window 256: 64 tiles 20+44 / 19+33 us, 192 19+64 / 18+64, 256 19+62 / 19+71; window 2048: 128 38+113 /
-//   21+58, 256 38+114 / 27+98, 512 51+182 / 45+192; d = 128: 128 55+177 / 33+98, 256 55+180 / 45+193, 512 76+275 / 87+380;
-//   fp32, d = 64, window 256: 256 41+177 / 42+174, 512 67+303 / 78+325; window 2048: 256 162+534 / 99+348, 768 397+1203 /
-//   285+1035
-int64_t share_below(int es, int64_t window) {
+// The number of 128-row tiles (128-key tiles for dk and dv) below which the waves of a workgroup share 32 rows instead (the
+// card has 256 compute units).  Long windows gain more, short ones pay for staging a tile four times; shared tiles of 128
+// columns leave one wave a SIMD, as those of dk and dv always do; fp32 products take 16 times as long, so balance counts for
+// more.  Wide / shared in us, 2048 rows a head (tiles: 16 a head):
+//   16 bits, window 1024: out d = 64, 256 tiles 26 / 21, 384 33 / 29, 512 34 / 38; dq 256 31 / 29, 384 41 / 40;
+//     d = 96, out 256 33 / 32, 384 42 / 43; dq 384 56 / 52; d = 128, out + dq 128 86 / 66, 160 87 / 92, 192 88 / 105
+//   window 256: out + dq d = 64, 128 33 / 23, 160 33 / 31, 192 32 / 31, 256 32 / 35; d = 128, 128 45 / 39, 160 46 / 59
+//   dk, dv: window 1024, d = 64, 128 39 / 33, 160 40 / 47; d = 128, 128 55 / 51, 160 56 / 71; window 256, 64 tiles
+//     23 / 19 and 31 / 31, 128 23 / 28 and 32 / 41
+//   fp32, d = 64, all of them: window 256, 256 tiles 218 / 216, 512 370 / 403; window 2048, 256 696 / 447, 768 1600 / 1320
+int64_t share_below(int es, int width, int64_t window, bool keys) {
   if (es == 4) return window >= 1024 ? 1024 : 448;
-  return window >= 1024 ? 256 : 144;
+  if (keys) return window >= 1024 ? 144 : 96;
+  return window >= 1024 && width <= 96 ? 448 : 160;
 }
 
 // The shape part of the arguments; STA_OK or what is wrong with it.
@@ -68,8 +72,9 @@ int window_shape(sta::WinArgs& a, int dtype, int64_t batch, int heads, int kv_he
   // above 0: a hidden pair's logit, -inf, stays one times c
   a.c = std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-37f);
   const int64_t wide = (n + sta::WIN_ROWS - 1) / sta::WIN_ROWS;
-  a.share = batch * heads * wide < share_below(es, a.window);
-  a.key_share = batch * kv_heads * wide < share_below(es, a.window);
+  const int width = d > dv ? d : dv;
+  a.share = batch * heads * wide < share_below(es, width, a.window, false);
+  a.key_share = batch * kv_heads * wide < share_below(es, width, a.window, true);
   a.tiles = static_cast<int>(a.share ? (n + 31) / 32 : wide);
   a.key_tiles = static_cast<int>(a.key_share ? (n + 31) / 32 : wide);
   a.lift = a.drop = 1.f;
