@@ -15,7 +15,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 import _native
-from sink_window_attention import _check_gpu, _differentiable_once, _like, _on, _refuse_capture, _strides
+from sink_window_attention import _STRIDES, _check_gpu, _differentiable_once, _like, _on, _refuse_capture, _strides
 
 Tensor = torch.Tensor
 
@@ -47,15 +47,14 @@ class _Call:
         if q.ndim != k.ndim or q.ndim not in (2, 3, 4):
             raise ValueError("q and k must be [N,D], [S,H,D] or [B,H,N,D]")
         self.ndim = q.ndim
-        q, k = self.rows(q), self.rows(k)
-        b, h, n, d = q.shape
-        if k.shape[0] != b or k.shape[2:] != (n, d):
+        (b, h, n, d), (kb, hk, kn, kd) = self.shape_of(q), self.shape_of(k)
+        if kb != b or kn != n or kd != d:
             raise ValueError(f"k must match q but for its heads, got {tuple(k.shape)} and {tuple(q.shape)}")
         if q.dtype not in _native.DTYPE_CODES or k.dtype != q.dtype:
             raise ValueError("q and k must have one dtype of float32, bfloat16 and float16")
         if not 1 <= d <= MAX_DIM:
             raise ValueError(f"head widths must be 1 .. {MAX_DIM}, got {d}")
-        if h > MAX_HEADS or k.shape[1] > MAX_HEADS or b * n > MAX_ROWS:
+        if h > MAX_HEADS or hk > MAX_HEADS or b * n > MAX_ROWS:
             raise ValueError(f"at most {MAX_HEADS} heads and {MAX_ROWS} rows of a head are supported")
         if table.ndim != 2 or table.dtype != torch.float32 or table.shape[1] % 2 or table.shape[1] > d:
             raise ValueError(f"table must be float32 [limit, rotary_dim], rotary_dim even and at most {d}")
@@ -86,14 +85,22 @@ class _Call:
         self.table = table.contiguous()
         self.positions, self.eps, self.interleaved = positions, float(eps), bool(interleaved)
         self.weight_code = _native.DTYPE_CODES[weights[0].dtype if weights else q.dtype]
-        self.shape = (b, h, k.shape[1], n, d)
+        self.shape = (b, h, hk, n, d)
 
-    def rows(self, x: Tensor) -> Tensor:
-        """x as [B,H,N,D]."""
-        return x[None, None] if x.ndim == 2 else (x[:, :, None] if x.ndim == 3 else x)
+    def shape_of(self, x: Tensor) -> Tuple[int, int, int, int]:
+        """x's shape as [B,H,N,D]."""
+        s = x.shape
+        return s if self.ndim == 4 else ((1, 1, *s) if self.ndim == 2 else (s[0], s[1], 1, s[2]))
 
-    def back(self, x: Tensor) -> Tensor:
-        return x[0, 0] if self.ndim == 2 else (x[:, :, 0] if self.ndim == 3 else x)
+    def strides(self, *tensors: Tensor):
+        """The element strides of batch, head and row of every tensor, for the C ABI."""
+        if self.ndim == 4:
+            return _strides(*tensors)
+        flat = ()
+        for x in tensors:
+            s = x.stride()
+            flat += (0, 0, s[0]) if self.ndim == 2 else (s[0], s[1], 0)
+        return _STRIDES[len(flat)](*flat)
 
     def tail(self, q_weight, k_weight):
         b, h, hk, n, d = self.shape
@@ -104,20 +111,20 @@ class _Call:
 
     def forward(self, q, k, q_weight, k_weight):
         b, h, hk, n, d = self.shape
-        q, k = _walkable(self.rows(q)), _walkable(self.rows(k))
+        q, k = _walkable(q), _walkable(k)
         qw, kw = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
         yq, yk = _like(q), _like(k)
         if b * n and h + hk:
             with _on(q.device):
                 st = _native.lib().sta_head_rotary(
-                    q.data_ptr(), k.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, hk, n, d, _strides(q, k),
+                    q.data_ptr(), k.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, hk, n, d, self.strides(q, k),
                     *self.tail(qw, kw), yq.data_ptr(), yk.data_ptr(), _native.stream_handle(q.device))
             _native.check(st, "sta_head_rotary")
-        return self.back(yq), self.back(yk)
+        return yq, yk
 
     def backward(self, gq, gk, q, k, q_weight, k_weight):
         b, h, hk, n, d = self.shape
-        q, k, gq, gk = (_walkable(self.rows(x)) for x in (q, k, gq, gk))
+        q, k, gq, gk = _walkable(q), _walkable(k), _walkable(gq), _walkable(gk)
         qw, kw = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
         dq, dk = _like(q), _like(k)
         empty = not (b * n and h + hk)
@@ -130,14 +137,14 @@ class _Call:
             with _on(q.device):
                 st = lib.sta_head_rotary_backward(
                     gq.data_ptr(), gk.data_ptr(), q.data_ptr(), k.data_ptr(), _native.DTYPE_CODES[q.dtype], b, h, hk,
-                    n, d, _strides(q, k, gq, gk), *self.tail(qw, kw), dq.data_ptr(), dk.data_ptr(),
+                    n, d, self.strides(q, k, gq, gk), *self.tail(qw, kw), dq.data_ptr(), dk.data_ptr(),
                     _native.ptr(dw[0]), _native.ptr(dw[1]), ws.data_ptr(), nbytes, _native.stream_handle(q.device))
             _native.check(st, "sta_head_rotary_backward")
-        return self.back(dq), self.back(dk), dw[0], dw[1]
+        return dq, dk, dw[0], dw[1]
 
 
 def _walkable(x: Tensor) -> Tensor:
-    return x if x.stride(3) == 1 or x.shape[3] == 1 else x.contiguous()
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
 class _NormRotary(torch.autograd.Function):

@@ -40,9 +40,10 @@ def _attention_scale(scale: Optional[float], dim: int) -> float:
 
 
 def _check_tokens(window: int, sinks: int) -> Tuple[int, int]:
-    for name, x in (("window", window), ("sinks", sinks)):
-        if isinstance(x, bool) or not isinstance(x, int):
-            raise ValueError(f"{name} must be an int, got {x!r}")
+    if type(window) is not int or type(sinks) is not int:
+        for name, x in (("window", window), ("sinks", sinks)):
+            if isinstance(x, bool) or not isinstance(x, int):
+                raise ValueError(f"{name} must be an int, got {x!r}")
     if window < 1:
         raise ValueError("window must be at least 1")
     if sinks < 0:
@@ -63,8 +64,14 @@ def _check_dtype(*tensors: Tensor) -> None:
     t = tensors[0].dtype
     if t not in _native.DTYPE_CODES:
         raise ValueError(f"dtype {t} is not supported (use float32, bfloat16 or float16)")
-    if any(x.dtype != t for x in tensors):
-        raise ValueError("all of q, k and v (and their gradients) must have one dtype")
+    for x in tensors:
+        if x.dtype != t:
+            raise ValueError("all of q, k and v (and their gradients) must have one dtype")
+
+
+def _four(x: Tensor) -> Tensor:
+    """[N,D] as [1,1,N,D]."""
+    return x.view(1, 1, *x.shape)
 
 
 def _heads_first(q: Tensor, k: Tensor, v: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
@@ -72,16 +79,16 @@ def _heads_first(q: Tensor, k: Tensor, v: Tensor) -> Tuple[Tensor, Tensor, Tenso
     if q.ndim != k.ndim or q.ndim != v.ndim or q.ndim not in (2, 4):
         raise ValueError("q/k/v must be [N,D] or [B,H,N,D]")
     if q.ndim == 2:
-        q, k, v = q[None, None], k[None, None], v[None, None]
-    b, h, n, d = q.shape
-    if k.shape[0] != b or k.shape[2:] != (n, d):
+        q, k, v = _four(q), _four(k), _four(v)
+    (b, h, n, d), (kb, hk, kn, kd), (vb, vh, vn, dv) = q.shape, k.shape, v.shape
+    if kb != b or kn != n or kd != d:
         raise ValueError(f"k must be [B,Hkv,N,D] like q [B,H,N,D], got {tuple(k.shape)} and {tuple(q.shape)}")
-    if v.shape[:3] != k.shape[:3]:
+    if vb != kb or vh != hk or vn != kn:
         raise ValueError(f"v must be [B,Hkv,N,Dv] like k, got {tuple(v.shape)} and {tuple(k.shape)}")
-    if h != k.shape[1] and (k.shape[1] == 0 or h % k.shape[1] != 0):
-        raise ValueError(f"the query heads ({h}) must be a multiple of the key heads ({k.shape[1]})")
-    if not 1 <= d <= MAX_DIM or not 1 <= v.shape[3] <= MAX_DIM:
-        raise ValueError(f"key and value widths must be 1 .. {MAX_DIM}, got {d} and {v.shape[3]}")
+    if h != hk and (hk == 0 or h % hk != 0):
+        raise ValueError(f"the query heads ({h}) must be a multiple of the key heads ({hk})")
+    if not 1 <= d <= MAX_DIM or not 1 <= dv <= MAX_DIM:
+        raise ValueError(f"key and value widths must be 1 .. {MAX_DIM}, got {d} and {dv}")
     if n > MAX_ROWS:
         raise ValueError(f"sequences of at most {MAX_ROWS} rows are supported")
     return q, k, v
@@ -98,8 +105,8 @@ def _check_lengths(lengths: Optional[Tensor], batch: int) -> Optional[Tensor]:
 def _rows(x: Tensor) -> Tensor:
     """x itself where the kernels can walk its rows (contiguous last dimension, rows at most 2^24 bytes apart), else a
     dense copy."""
-    near = x.stride(2) * x.element_size() <= 1 << 24
-    if near and (x.stride(3) == 1 or x.shape[3] == 1):
+    strides = x.stride()
+    if strides[2] * x.element_size() <= 1 << 24 and (strides[3] == 1 or x.shape[3] == 1):
         return x
     return x.clone(memory_format=torch.contiguous_format)  # strides of dimensions of one element too
 
@@ -120,7 +127,9 @@ _STRIDES = {n: ctypes.c_int64 * n for n in (6, 9, 12)}
 
 def _strides(*tensors: Tensor):
     """The element strides of batch, head and row of every tensor, for the C ABI."""
-    flat = [s for x in tensors for s in x.stride()[:3]]
+    flat = ()
+    for x in tensors:
+        flat += x.stride()[:3]
     return _STRIDES[len(flat)](*flat)
 
 
@@ -210,10 +219,10 @@ class _SinkWindow(torch.autograd.Function):
     def forward(ctx, q, k, v, window, sinks, scale, lengths):
         _refuse_capture()
         ctx.flat = q.ndim == 2
-        q4, k4, v4 = (q[None, None], k[None, None], v[None, None]) if ctx.flat else (q, k, v)
+        q4, k4, v4 = (_four(q), _four(k), _four(v)) if ctx.flat else (q, k, v)
         out, rest, lse = _forward(q4, k4, v4, window, sinks, scale, lengths, True, True)
         if ctx.flat:
-            out = out[0, 0]
+            out = out.view(out.shape[2:])
         ctx.save_for_backward(q, k, v, out, rest, lse, lengths)
         ctx.settings = window, sinks, scale
         return out
@@ -224,10 +233,10 @@ class _SinkWindow(torch.autograd.Function):
         _refuse_capture()
         q, k, v, out, rest, lse, lengths = ctx.saved_tensors
         if ctx.flat:
-            grad, q, k, v, out = (x[None, None] for x in (grad, q, k, v, out))
+            grad, q, k, v, out = (_four(x) for x in (grad, q, k, v, out))
         grads = _backward(grad, q, k, v, out, rest, lse, *ctx.settings, lengths)
         if ctx.flat:
-            grads = (x[0, 0] for x in grads)
+            grads = (x.view(x.shape[2:]) for x in grads)
         return *grads, None, None, None, None
 
 
