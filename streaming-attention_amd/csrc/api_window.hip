@@ -36,17 +36,17 @@ bool strides_ok(const int64_t* strides, int tensors, int dtype) {
 
 // The number of 128-row tiles (128-key tiles for dk and dv) below which the waves of a workgroup share 32 rows instead (the
 // card has 256 compute units).  Long windows gain more, short ones pay for staging a tile four times; shared tiles of 128
-// columns leave one wave a SIMD, as those of dk and dv always do; fp32 products take 16 times as long, so balance counts for
+// columns leave one wave a SIMD, as those of dk and dv do above 64; fp32 products take 16 times as long, so balance counts for
 // more.  Wide / shared in us, 2048 rows a head (tiles: 16 a head):
 //   16 bits, window 1024: out d = 64, 256 tiles 26 / 21, 384 33 / 29, 512 34 / 38; dq 256 31 / 29, 384 41 / 40;
 //     d = 96, out 256 33 / 32, 384 42 / 43; dq 384 56 / 52; d = 128, out + dq 128 86 / 66, 160 87 / 92, 192 88 / 105
 //   window 256: out + dq d = 64, 128 33 / 23, 160 33 / 31, 192 32 / 31, 256 32 / 35; d = 128, 128 45 / 39, 160 46 / 59
-//   dk, dv: window 1024, d = 64, 128 39 / 33, 160 40 / 47; d = 128, 128 55 / 51, 160 56 / 71; window 256, 64 tiles
-//     23 / 19 and 31 / 31, 128 23 / 28 and 32 / 41
+//   dk, dv: d = 64, window 1024, 256 47 / 40, 384 56 / 56, window 256, 256 29 / 29, 384 43 / 39; d = 128, window 1024, 128
+//     55 / 51, 160 56 / 71, window 256, 64 31 / 31, 128 31 / 41
 //   fp32, d = 64, all of them: window 256, 256 tiles 218 / 216, 512 370 / 403; window 2048, 256 696 / 447, 768 1600 / 1320
 int64_t share_below(int es, int width, int64_t window, bool keys) {
   if (es == 4) return window >= 1024 ? 1024 : 448;
-  if (keys) return window >= 1024 ? 144 : 96;
+  if (keys) return width <= 64 ? 448 : (window >= 1024 ? 144 : 96);
   return window >= 1024 && width <= 96 ? 448 : 160;
 }
 

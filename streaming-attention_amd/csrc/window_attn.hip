@@ -244,7 +244,15 @@ __device__ __forceinline__ void win_keep(WinFrag<IN>& f, bool row) {
     f.w[i] = uint4{row ? f.w[i].x : 0u, row ? f.w[i].y : 0u, row ? f.w[i].z : 0u, row ? f.w[i].w : 0u};
 }
 
-__device__ __forceinline__ void win_pin(floatx16& x) { asm volatile("" : "+a"(x)); }
+// waves a SIMD of window_dkv_kernel
+template <int P, int IN>
+__host__ __device__ constexpr int win_dkv_waves() { return IN != F32 && P <= 64 ? 2 : 1; }
+
+// keeps x in accumulation registers, where a kernel has both kinds (the compiler else moves sums there and back)
+template <bool PIN>
+__device__ __forceinline__ void win_pin(floatx16& x) {
+  if constexpr (PIN) asm volatile("" : "+a"(x));
+}
 
 __device__ __forceinline__ bool win_finite(float x) { return fabsf(x) < __builtin_inff(); }
 
@@ -905,17 +913,20 @@ __host__ __device__ constexpr int win_dkv_lds() {
 // sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.  p and ds are rounded to
 // the rows' type for their products like the weights of the forward kernel.
 // dk and dv of 32 keys of 128 columns take 128 registers a lane and the keys' operands 64, so a compute unit holds one wave
-// a SIMD.  PIPE (16-bit rows that fill their padded width): that wave's instructions are laid out by hand, see below;
-// without it the operands are at least read ahead.  32 heads of 16384 rows over 8 key heads, 128 wide, window 4096, bf16:
-// 2.37 ms, four products at 810 TFLOP/s (3.03 ms without PIPE; operands read two steps ahead 2.48, three 2.37, four
-// 2.33; dk and dv in kernels of their own, 5 products but two waves a SIMD, 3.45); 48 heads of 2048 rows, 64 wide,
-// window 2048: 205 us with dq (233 without PIPE).  What is left: about 300 instructions a wave issues for 32 rows, one
-// at a time, against 1024 cycles of the matrix unit.
+// a SIMD above 64 columns.  PIPE (16-bit rows that fill a padded width of 96 or 128): that wave's instructions are laid
+// out by hand, see below; without it the operands are at least read ahead.  32 heads of 16384 rows over 8 key heads, 128 wide,
+// window 4096, bf16: 2.37 ms, four products at 810 TFLOP/s (3.03 ms without PIPE; operands read two steps ahead 2.48, three
+// 2.37, four 2.33; dk and dv in kernels of their own, 5 products but two waves a SIMD, 3.45).  What is left: about 300
+// instructions a wave issues for 32 rows, one at a time, against 1024 cycles of the matrix unit.
+// Up to 64 columns two waves a SIMD fill each other's waits better than PIPE does: 8 x 16 heads of 4096 rows, 64 wide, window
+// 1024, 515 us (PIPE with one wave 722, with two, which spill, 714); 32 heads of 16384 over 8 key heads, window 4096, 1.36
+// ms (1.73); 32 wide 265 us (314); 96 wide the other way round: 4 x 16 heads over 4 key heads 359 us with PIPE, 411 with two waves.
 template <int P, int IN, bool SHARE, bool PIPE>
-__global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
+__global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kernel(const WinArgs a) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_staged_rows<IN, SHARE>(),
                 NSUB = BQ / 32, TILE = win_rows<SHARE>(), THREADS = SHARE ? 64 : 256;
   constexpr int STAGE = 2 * BQ * CH;  // 16-byte units of a stage
+  constexpr int WAVES = win_dkv_waves<P, IN>();
   extern __shared__ uint4 win_lds[];
   constexpr int STAGES = SHARE ? 4 : (PIPE ? 3 : 2);  // of the waves, or of tiles
   float* const stats = reinterpret_cast<float*>(win_lds + STAGES * STAGE);  // [stage][lift - lse, delta][BQ]
@@ -1075,8 +1086,8 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
         const floatx4* st = reinterpret_cast<const floatx4*>(stats + stage * 2 * BQ);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          win_pin(dk[mt]);
-          win_pin(dv[mt]);
+          win_pin<WAVES == 1>(dk[mt]);
+          win_pin<WAVES == 1>(dv[mt]);
         }
 #pragma unroll
         for (int sub = 0; sub < 2; ++sub) {
@@ -1194,11 +1205,10 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
         if (count > 1) load(1);
       }
       for (int it = start; it < count; it += step) {
-        // the accumulators stay in accumulation registers (the compiler else moves all of them there and back)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          win_pin(dk[mt]);
-          win_pin(dv[mt]);
+          win_pin<WAVES == 1>(dk[mt]);
+          win_pin<WAVES == 1>(dv[mt]);
         }
         int stage = wave;
         if (!AHEAD) load(it);
@@ -1219,10 +1229,9 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(const WinArgs a) {
         const bool all = whole(q0, BQ);
 #pragma unroll 1
         for (int sub = 0; sub < NSUB; ++sub) {
-          // every operand is read well before its product: a compute unit holds one wave a SIMD, which has nothing else to
-          // do while it waits
-          // (fp32 products take eight times as long as their operands' reads: those are read as they come)
-          constexpr bool EARLY = IN != F32;
+          // one wave a SIMD: every operand is read well before its product, there is nothing else to do while it waits (fp32
+          // products take eight times as long as their operands' reads: those are read as they come)
+          constexpr bool EARLY = IN != F32 && WAVES == 1;
           WinFrag<IN> qa[EARLY ? P / 16 : 1], ga[EARLY ? P / 16 : 1], qc[MT], gc[MT];
           floatx16 x, g;
 #pragma unroll
