@@ -40,13 +40,13 @@ int launch_window_backward(const sta::WinArgs& a, hipStream_t s) {
   int st = a.share ? launch(sta::window_dq_kernel<P, IN, true>, grid_q, sta::win_lds_bytes<P, IN, true>(), a, s)
                    : launch(sta::window_dq_kernel<P, IN, false>, grid_q, sta::win_lds_bytes<P, IN, false>(), a, s);
   if (st != STA_OK) return st;
-  constexpr bool PIPE = IN != sta::F32 && sta::win_dkv_waves<P, IN>() == 1;
+  constexpr bool FULL = sta::win_pipe<P, IN, false>();
   if (a.key_share)
-    st = launch(sta::window_dkv_kernel<P, IN, true, false>, grid_k, sta::win_dkv_lds<P, IN, true, false>(), a, s);
-  else if (PIPE && a.d == P && a.dv == P)
-    st = launch(sta::window_dkv_kernel<P, IN, false, PIPE>, grid_k, sta::win_dkv_lds<P, IN, false, PIPE>(), a, s);
+    st = launch(sta::window_dkv_kernel<P, IN, true, false>, grid_k, sta::win_dkv_lds<P, IN, true>(), a, s);
+  else if (FULL && a.d == P && a.dv == P)
+    st = launch(sta::window_dkv_kernel<P, IN, false, FULL>, grid_k, sta::win_dkv_lds<P, IN, false>(), a, s);
   else
-    st = launch(sta::window_dkv_kernel<P, IN, false, false>, grid_k, sta::win_dkv_lds<P, IN, false, false>(), a, s);
+    st = launch(sta::window_dkv_kernel<P, IN, false, false>, grid_k, sta::win_dkv_lds<P, IN, false>(), a, s);
   if (st != STA_OK || a.far_chunks == 0) return st;
   return launch(sta::window_sink_kernel<IN>, grid_s, 0, a, s);
 }

@@ -247,6 +247,9 @@ __device__ __forceinline__ void win_keep(WinFrag<IN>& f, bool row) {
 // waves a SIMD of window_dkv_kernel
 template <int P, int IN>
 __host__ __device__ constexpr int win_dkv_waves() { return IN != F32 && P <= 64 ? 2 : 1; }
+// whether its instructions are laid out by hand
+template <int P, int IN, bool SHARE>
+__host__ __device__ constexpr bool win_pipe() { return !SHARE && IN != F32 && win_dkv_waves<P, IN>() == 1; }
 
 // keeps x in accumulation registers, where a kernel has both kinds (the compiler else moves sums there and back)
 template <bool PIN>
@@ -901,10 +904,10 @@ __device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, in
 // (shared: one stage a wave).
 template <int IN, bool SHARE>
 __host__ __device__ constexpr int win_staged_rows() { return IN == F32 || SHARE ? 32 : 64; }
-template <int P, int IN, bool SHARE, bool PIPE>
+template <int P, int IN, bool SHARE>
 __host__ __device__ constexpr int win_dkv_lds() {
   const int rows = win_staged_rows<IN, SHARE>(), stage = 2 * rows * P * (IN == F32 ? 4 : 2) + 2 * rows * 4;
-  if (!SHARE) return (PIPE ? 3 : 2) * stage;
+  if (!SHARE) return (win_pipe<P, IN, SHARE>() ? 3 : 2) * stage;
   return 4 * stage > 4 * win_join_floats<P>() ? 4 * stage : 4 * win_join_floats<P>();
 }
 
@@ -913,20 +916,23 @@ __host__ __device__ constexpr int win_dkv_lds() {
 // sums, like those of the sinks' own tiles, are added by window_sink_kernel in their order.  p and ds are rounded to
 // the rows' type for their products like the weights of the forward kernel.
 // dk and dv of 32 keys of 128 columns take 128 registers a lane and the keys' operands 64, so a compute unit holds one wave
-// a SIMD above 64 columns.  PIPE (16-bit rows that fill a padded width of 96 or 128): that wave's instructions are laid
-// out by hand, see below; without it the operands are at least read ahead.  32 heads of 16384 rows over 8 key heads, 128 wide,
-// window 4096, bf16: 2.37 ms, four products at 810 TFLOP/s (3.03 ms without PIPE; operands read two steps ahead 2.48, three
+// a SIMD above 64 columns.  PIPE (16-bit rows): that wave's instructions are laid out by hand, see below; without it (SHARE) the
+// operands are at least read ahead.  32 heads of 16384 rows over 8 key heads, 128 wide,
+// window 4096, bf16: 2.37 ms, four products at 810 TFLOP/s (3.03 ms without PIPE; 93 wide, 4 x 16 heads of 4096 rows, window
+// 1024, with dq 841 us, 923 without; operands read two steps ahead 2.48, three
 // 2.37, four 2.33; dk and dv in kernels of their own, 5 products but two waves a SIMD, 3.45).  What is left: about 300
 // instructions a wave issues for 32 rows, one at a time, against 1024 cycles of the matrix unit.
 // Up to 64 columns two waves a SIMD fill each other's waits better than PIPE does: 8 x 16 heads of 4096 rows, 64 wide, window
 // 1024, 515 us (PIPE with one wave 722, with two, which spill, 714); 32 heads of 16384 over 8 key heads, window 4096, 1.36
 // ms (1.73); 32 wide 265 us (314); 96 wide the other way round: 4 x 16 heads over 4 key heads 359 us with PIPE, 411 with two waves.
-template <int P, int IN, bool SHARE, bool PIPE>
+// FULL: both widths are the padded one (with PIPE).
+template <int P, int IN, bool SHARE, bool FULL>
 __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kernel(const WinArgs a) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_staged_rows<IN, SHARE>(),
                 NSUB = BQ / 32, TILE = win_rows<SHARE>(), THREADS = SHARE ? 64 : 256;
   constexpr int STAGE = 2 * BQ * CH;  // 16-byte units of a stage
   constexpr int WAVES = win_dkv_waves<P, IN>();
+  constexpr bool PIPE = win_pipe<P, IN, SHARE>();
   extern __shared__ uint4 win_lds[];
   constexpr int STAGES = SHARE ? 4 : (PIPE ? 3 : 2);  // of the waves, or of tiles
   float* const stats = reinterpret_cast<float*>(win_lds + STAGES * STAGE);  // [stage][lift - lse, delta][BQ]
@@ -999,7 +1005,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
       // sums (the barriers of the schedule keep that order).  Three stages: tile `it` and the next are written, the third is
       // being written; one __syncthreads a tile.  Rows behind the last are read as the last one, their weights are
       // exp2(-inf).  No tile is left out for a wave that sees none of it: the others' barrier waits for it anyway.
-      constexpr int U = BQ * CH / 256;  // 16-byte units of a tensor's tile a thread
+      constexpr int U = BQ * CH / 256, E = 16 / ES;  // 16-byte units of a tensor's tile a thread, their elements
       static_assert(U == MT && NSUB == 2);
       uint4 uq[U], ug[U];
       uint32_t to[U], off[2][U];
@@ -1024,8 +1030,8 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
 #pragma unroll
           for (int i = 0; i < U; ++i) {
             const int k = threadIdx.x + 256 * i, row = min(k / CH, left - 1);
-            off[0][i] = row * pitch_q + k % CH * 16;
-            off[1][i] = row * pitch_g + k % CH * 16;
+            off[0][i] = row * pitch_q + (FULL ? k % CH * E : min(k % CH * E, a.d - E)) * ES;
+            off[1][i] = row * pitch_g + (FULL ? k % CH * E : min(k % CH * E, a.dv - E)) * ES;
           }
         }
         qp = rows_at<ES>(a.q, b, lhead, lrow);
@@ -1047,14 +1053,29 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
         if (i == 0) stat = *sp;
       };
       bool stat_in;
+      // a unit into its place: a row's last one moved down where it reaches over the end, none behind it
+      auto place = [&](int at, uint4 x, int col, int width) {
+        if (width % E) x = rows_shift(x, max(0, col + E - width) * ES & 15);
+        if (col < width) win_lds[at] = x;
+      };
       auto write = [&](int i, int st) {
-        win_lds[st * STAGE + to[i]] = uq[i];
-        win_lds[st * STAGE + BQ * CH + to[i]] = ug[i];
+        if constexpr (FULL) {
+          win_lds[st * STAGE + to[i]] = uq[i];
+          win_lds[st * STAGE + BQ * CH + to[i]] = ug[i];
+        } else {
+          const int col = (threadIdx.x + 256 * i) % CH * E;
+          place(st * STAGE + to[i], uq[i], col, a.d);
+          place(st * STAGE + BQ * CH + to[i], ug[i], col, a.dv);
+        }
         if (i == 0) {
           const float x = of_lse ? lift - stat : stat;
           stats[st * 2 * BQ + threadIdx.x % (2 * BQ)] = stat_in ? x : (of_lse ? -__builtin_inff() : 0.f);
         }
       };
+      if constexpr (!FULL) {  // the columns behind the widths
+        for (int i = threadIdx.x; i < 3 * STAGE; i += 256) win_lds[i] = uint4{0u, 0u, 0u, 0u};
+        __syncthreads();
+      }
 #pragma unroll
       for (int j = 0; j < 3; ++j) {
         aim();
