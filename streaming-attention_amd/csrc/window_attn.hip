@@ -688,9 +688,10 @@ __device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
 // o), the same for all keys of a row, which adds about a tenth to the gradients' rounding errors (a third with windows of 16
 // keys); with what the rounding left (rest) it is not.  ds is rounded to the rows' type for
 // its product with the keys like the weights of the forward kernel.  32 heads of 16384 rows, 128 wide, window 4096,
-// bf16: 1.45 ms, three products at 995 TFLOP/s, bound by them.
+// bf16: 1.45 ms, three products at 995 TFLOP/s, bound by them; 8 x 16 heads of 4096 rows, 64 wide, window 1024: 291 us with
+// three waves a SIMD (one register less a lane than the compiler takes by itself), 316 with two.
 template <int P, int IN, bool SHARE>
-__global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : 2) void window_dq_kernel(const WinArgs a) {
+__global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 && !SHARE ? 3 : 2)) void window_dq_kernel(const WinArgs a) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
                 MT = P / 32, STEP = SHARE ? 4 : 1;
   constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
