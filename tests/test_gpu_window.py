@@ -394,3 +394,13 @@ def test_rest_of_the_output(b, h, hk, n, d, dv, window, lengths, dtype):
     got = run(q, k, v, go, window=window, sinks=2, lengths=lengths)
     for name in grads:
         assert torch.equal(got[name], grads[name])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sinks", [1, 33, 64, 65])
+@pytest.mark.parametrize("d,dv", [(64, 64), (128, 96)])
+def test_sinks_of_many_heads_behind_short_windows(d, dv, sinks, dtype):
+    """Rows behind the window of the sinks, in their own launch and in the keys' one; lengths that end before and in them."""
+    q, k, v, go = make(3, 64, 64, 500, d, dv, dtype, seed=15)
+    kw = dict(window=20, sinks=sinks, lengths=[500, 19, 83])
+    check(run(q, k, v, go, **kw), ref.window_attention(q, k, v, grad=go, **kw))
