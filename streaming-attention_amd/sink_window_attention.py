@@ -373,8 +373,8 @@ class SinkWindowStreamingAttention:
         if x.shape != want:
             raise ValueError(f"{what} must be {list(want)}, got {list(x.shape)}")
         if x.dtype != self.dtype or x.device != self.device:
-            x = x.to(device=self.device, dtype=self.dtype)
-        return x if x.is_contiguous() or x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+            x = x.detach().to(device=self.device, dtype=self.dtype)
+        return x if x.is_contiguous() or x.stride(-1) == 1 or x.shape[-1] == 1 else x.detach().contiguous()
 
     def _attend(self, q: Tensor, k: Optional[Tensor], v: Optional[Tensor]) -> Tensor:
         out = _like(q) if self.dim == self.value_dim else q.new_empty((self.streams, self.heads, self.value_dim))
@@ -406,7 +406,6 @@ class SinkWindowStreamingAttention:
         """Attention of one query a head over the tokens held; zero for a stream that holds none."""
         return self._attend(self._rows(query, self._shapes["query"], "query"), None, None)
 
-    @torch.no_grad()
     def update(self, key: Tensor, value: Tensor) -> None:
         """One token of every stream into the cache."""
         k = self._rows(key, self._shapes["key"], "key")
@@ -436,7 +435,6 @@ class SinkWindowStreamingAttention:
                 raise ValueError("counts must be on the object's device")
         return k, v, counts
 
-    @torch.no_grad()
     def extend(self, keys: Tensor, values: Tensor, *, counts: Optional[Tensor] = None) -> None:
         """update() with the rows of keys [S,Hkv,P,dim] and values [S,Hkv,P,value_dim] in bulk; counts: int32 [S] on
         the device, the rows of every stream that are tokens (None: all P; values outside 0 .. P are taken as the
@@ -456,7 +454,6 @@ class SinkWindowStreamingAttention:
         self._extend(k, v, counts)
         return out
 
-    @torch.no_grad()
     def reset(self, streams: Optional[Sequence[int]] = None) -> None:
         """Forgets every token of all streams, or of the given ones (new sequences start there)."""
         if streams is None:
@@ -470,14 +467,14 @@ class SinkWindowStreamingAttention:
         for i in streams:
             self._counts[i].zero_()
 
-    @torch.no_grad()
     def items(self) -> Tuple[Tensor, Tensor, Tensor]:
         """(keys [S,Hkv,sinks + window,dim], values [S,Hkv,sinks + window,value_dim], positions int32
         [S,sinks + window]) as the cache holds them, in the order of its slots; zero and -1 where no token is."""
         slots = self.sinks + self.window
-        keys = torch.empty((self.streams, self.kv_heads, slots, self.dim), device=self.device, dtype=self.dtype)
-        values = torch.empty((self.streams, self.kv_heads, slots, self.value_dim), device=self.device, dtype=self.dtype)
-        positions = torch.empty((self.streams, slots), device=self.device, dtype=torch.int32)
+        positions = self._counts.new_empty((self.streams, slots))
+        keys = positions.new_empty((self.streams, self.kv_heads, slots, self.dim), dtype=self.dtype)
+        values = (_like(keys) if self.dim == self.value_dim else
+                  keys.new_empty((self.streams, self.kv_heads, slots, self.value_dim)))
         with _on(self.device):
             st = _native.lib().sta_ring_items(
                 self._code, self._store, self.streams, self.kv_heads, self.dim, self.value_dim, self.window, self.sinks,
