@@ -404,3 +404,16 @@ def test_sinks_of_many_heads_behind_short_windows(d, dv, sinks, dtype):
     q, k, v, go = make(3, 64, 64, 500, d, dv, dtype, seed=15)
     kw = dict(window=20, sinks=sinks, lengths=[500, 19, 83])
     check(run(q, k, v, go, **kw), ref.window_attention(q, k, v, grad=go, **kw))
+
+
+def test_single_sequences_in_autograd():
+    """[N,D] leaves of any strides, one of them used twice, under a gradient that is one expanded number."""
+    base = torch.randn(48, 200, generator=torch.Generator().manual_seed(16)).to(DEV)
+    x, v = base[:32].t().requires_grad_(), base[32:].t().requires_grad_()  # 200 rows, columns 200 elements apart
+    out = swa.sink_window_causal_attention(x, x, v, window=30, sinks=2)
+    dx, dv = torch.autograd.grad(out.sum(), (x, v))
+    y, w = (t.detach().contiguous()[None, None] for t in (x, v))
+    o, lse = swa.sink_window_forward(y, y, w, window=30, sinks=2)
+    dq, dk, dw = swa.sink_window_backward(torch.ones_like(o), y, y, w, o, lse, window=30, sinks=2)
+    assert out.shape == (200, 16) and dx.shape == x.shape and dv.shape == v.shape
+    assert torch.equal(out, o[0, 0]) and torch.equal(dx, (dq + dk)[0, 0]) and torch.equal(dv, dw[0, 0])
