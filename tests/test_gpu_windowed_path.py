@@ -2,6 +2,7 @@
 into the cache, and token after token from there; and a training step through all of it."""
 
 import math
+import threading
 
 import pytest
 import torch
@@ -150,3 +151,83 @@ def test_second_derivatives_are_refused():
         assert torch.equal(plain, dq)
         with pytest.raises(RuntimeError, match="differentiate twice"):
             dq.sum().backward()
+
+
+@pytest.mark.parametrize("storage", [None, "fp4"])
+def test_two_captured_objects(storage):
+    """Steps of two objects in graphs of their own, both with split queries, replayed in turn and on two streams at once."""
+    g = torch.Generator().manual_seed(31)
+    size = dict(streams=1, heads=4, kv_heads=1, window=3000, sinks=4, dtype=torch.bfloat16, storage=storage, device=DEV)
+    objects, eager, graphs, inputs, outs = [], [], [], [], []
+    for i in range(2):
+        pair = [swa.SinkWindowStreamingAttention(64, 48, **size) for _ in range(2)]
+        k, v = (torch.randn(1, 1, 2990, d, generator=g).bfloat16().to(DEV) for d in (64, 48))
+        for a in pair:
+            a.extend(k, v)
+        x = [torch.zeros(1, h, d, dtype=torch.bfloat16, device=DEV) for h, d in ((4, 64), (1, 64), (1, 48))]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(pair[0].step(*x))
+        objects.append(pair[0])
+        eager.append(pair[1])
+        graphs.append(graph)
+        inputs.append(x)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for n in range(20):
+        for x in inputs:
+            for t in x:
+                t.copy_(torch.randn(t.shape, generator=g))
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i if n % 2 else 0]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], eager[i].step(*inputs[i])), (n, i)
+    for a, b in zip(objects, eager):
+        for x, y in zip(a.items(), b.items()):
+            assert torch.equal(x, y)
+
+
+def test_calls_from_two_threads():
+    """Forward and backward passes of two threads at once, each on a stream of its own, give what they give alone."""
+    def inputs(i):
+        g = torch.Generator().manual_seed(40 + i)
+        return [torch.randn(2, 4, 300 + 77 * i, 64, generator=g).to(DEV, (torch.bfloat16, torch.float32)[i]) for _ in range(4)]
+
+    table = qkr.rotary_table(512, 64, device=DEV)
+
+    def work(q, k, v, go):
+        q, k, v = (t.clone().requires_grad_() for t in (q, k, v))
+        x, y = qkr.qk_norm_rotary(q, k, table)
+        out = swa.sink_window_causal_attention(x, y, v, window=50)
+        return [t.detach() for t in (out, *torch.autograd.grad(out, (q, k, v), go))]
+
+    data = [inputs(i) for i in range(2)]
+    alone = [work(*x) for x in data]
+    torch.cuda.synchronize()
+    results, failures = [[], []], []
+
+    def run(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    results[i].append(work(*data[i]))
+            stream.synchronize()
+        except Exception as e:  # reported in the test's own thread
+            failures.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(results[i]) == 10
+        for got in results[i]:
+            for x, y in zip(got, alone[i]):
+                assert torch.equal(x, y)
