@@ -417,3 +417,24 @@ def test_single_sequences_in_autograd():
     dq, dk, dw = swa.sink_window_backward(torch.ones_like(o), y, y, w, o, lse, window=30, sinks=2)
     assert out.shape == (200, 16) and dx.shape == x.shape and dv.shape == v.shape
     assert torch.equal(out, o[0, 0]) and torch.equal(dx, (dq + dk)[0, 0]) and torch.equal(dv, dw[0, 0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_captured_passes_of_many_wide_heads(dtype):
+    """The largest workgroups' passes captured as their first call of the process may be, replayed with eager work between."""
+    q, k, v, go = (t.to(DEV) for t in make(2, 64, 32, 260, 128, 128, dtype, seed=17))
+    kw = dict(window=33, sinks=3)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out, lse, rest = swa.sink_window_forward(q, k, v, with_rest=True, **kw)
+        grads = swa.sink_window_backward(go, q, k, v, out, lse, rest=rest, **kw)
+    for i in range(4):
+        for t in (q, k, v, go):
+            t.copy_(t.roll(i + 1, 1) * 0.9)
+        graph.replay()
+        o, l, r = swa.sink_window_forward(q, k, v, with_rest=True, **kw)
+        want = (o, l, *swa.sink_window_backward(go, q, k, v, o, l, rest=r, **kw))
+        torch.cuda.synchronize()
+        for x, y in zip((out, lse, *grads), want):
+            assert torch.equal(x, y), i

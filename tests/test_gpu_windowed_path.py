@@ -231,3 +231,21 @@ def test_calls_from_two_threads():
         for got in results[i]:
             for x, y in zip(got, alone[i]):
                 assert torch.equal(x, y)
+
+
+def test_lengths_outside_the_rows():
+    """Lengths and counts outside 0 .. N are taken as the nearest of them."""
+    g = torch.Generator().manual_seed(50)
+    q, k, v, go = (torch.randn(3, 2, 150, 32, generator=g).to(DEV) for _ in range(4))
+    far = torch.tensor([-7, 2 ** 31 - 1, 151], dtype=torch.int32, device=DEV)
+    near = torch.tensor([0, 150, 150], dtype=torch.int32, device=DEV)
+    got, want = [], []
+    for lengths, to in ((far, got), (near, want)):
+        out, lse = swa.sink_window_forward(q, k, v, window=20, sinks=2, lengths=lengths)
+        to += [out, lse, *swa.sink_window_backward(go, q, k, v, out, lse, window=20, sinks=2, lengths=lengths)]
+        a = swa.SinkWindowStreamingAttention(32, 32, streams=3, heads=2, window=20, sinks=2, device=DEV)
+        to.append(a.prefill(q, k, v, counts=lengths))
+        to += [a.lengths, *a.items(), a.step(q[:, :, 0], k[:, :, 0], v[:, :, 0])]
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    assert got[0][0].count_nonzero() == 0 and got[6].tolist() == [1, 151, 151]  # a view: the step counts
