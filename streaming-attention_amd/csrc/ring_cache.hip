@@ -784,7 +784,8 @@ __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void*
           else
             w = uint4{f[0] | f[1] << 16, f[2] | f[3] << 16, f[4] | f[5] << 16, f[6] | f[7] << 16};
         }
-        reinterpret_cast<uint4*>(static_cast<char*>(out) + base * ES)[i] = w;
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));  // past the caches: 16 x 8 heads of 4100 x 64 40 -> 37.5 us
+        __builtin_nontemporal_store(u4{w.x, w.y, w.z, w.w}, reinterpret_cast<u4*>(static_cast<char*>(out) + base * ES) + i);
       }
       return;
     }
