@@ -81,16 +81,19 @@ int window_shape(sta::WinArgs& a, int dtype, int64_t batch, int heads, int kv_he
   return STA_OK;
 }
 
-// How the rows behind the window of the sinks are dealt out: chunks of at least 256 rows, at most about two
-// workgroups a compute unit.
-void plan_sinks(sta::WinArgs& a) {
+// How the rows behind the window of the sinks are dealt out: as many workgroups as the card holds at a time (256 compute
+// units, two each of 16-bit rows up to 64 columns), chunks of at least 256 rows.  Backward, window 256, 4 sinks: 8 x 16 heads of
+// 4096 x 64, 256 workgroups 450 us, 512 442, 1024 456, 2048 464; 2 x 16 heads of 4096 x 128, 256 227, 512 238; chunks of at
+// least 64 rows, 4 query heads of one key head of 32768 x 64, window 512, 186 us, of 256 158.
+void plan_sinks(sta::WinArgs& a, int es) {
   const int64_t behind = a.n - a.window;
   if (a.sinks == 0 || behind <= 0) return;
   const int64_t bkv = static_cast<int64_t>(a.batch) * (a.heads / a.group);
   a.sink_rows = a.sinks;
   const int rows = a.key_share ? 32 : sta::WIN_ROWS;
   a.sink_tiles = (a.sinks + rows - 1) / rows;
-  int64_t chunks = 512 / (bkv * a.sink_tiles);
+  const int64_t room = es == 2 && a.d <= 64 && a.dv <= 64 ? 512 : 256;
+  int64_t chunks = room / (bkv * a.sink_tiles);
   if (chunks > (behind + 255) / 256) chunks = (behind + 255) / 256;
   if (chunks < 1) chunks = 1;
   const int64_t chunk = ((behind + chunks - 1) / chunks + 31) / 32 * 32;
@@ -150,7 +153,7 @@ int64_t sta_window_backward_bytes(int dtype, int64_t batch, int heads, int kv_he
                                   int64_t window, int64_t sinks) {
   sta::WinArgs a;
   if (window_shape(a, dtype, batch, heads, kv_heads, n, d, dv, 1.f, window, sinks) != STA_OK) return -1;
-  plan_sinks(a);
+  plan_sinks(a, element_size(dtype));
   return 4 * (delta_floats(a) + part_floats(a));
 }
 
@@ -164,7 +167,7 @@ int sta_window_attention_backward(const void* grad, const void* q, const void* k
     return STA_ERR_ARG;
   sta::WinArgs a;
   if (const int st = window_shape(a, dtype, batch, heads, kv_heads, n, d, dv, scale, window, sinks)) return st;
-  plan_sinks(a);
+  plan_sinks(a, element_size(dtype));
   if (workspace_bytes < 4 * (delta_floats(a) + part_floats(a))) return STA_ERR_SCRATCH;
   if (!strides_ok(strides, 4, dtype)) return STA_ERR_UNSUPPORTED;
   a.q = rows_of(q, strides);

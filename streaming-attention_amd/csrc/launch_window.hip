@@ -29,16 +29,17 @@ int launch_window_forward(const sta::WinArgs& a, hipStream_t s) {
   return launch(sta::window_forward_kernel<P, IN, false>, grid, sta::win_lds_bytes<P, IN, false>(), a, s);
 }
 
-// D and dq, then dk and dv, then the sums of the sinks.  The rows behind the window of up to 64 sinks go to workgroups whose
+// D and dq, then dk and dv, then the sums of the sinks.  The rows behind the window of up to 32 sinks go to workgroups whose
 // waves share 32 of them, in a launch of their own: in tiles of 128 keys they take as many steps for 4 keys as for 128
-// (backward with 4 sinks, 8 x 16 heads of 4096 rows, 64 wide: window 256 452 -> 415 us, window 1024 833 -> 819).  Below a
-// sixteenth of the steps that launch costs what it saves (32 heads of 16384 rows, 128 wide, window 4096 3744 -> 3788 us).
+// (backward, 8 x 16 heads of 4096 rows, 64 wide, window 256: 4 sinks 484 -> 442 us, 32 425 -> 412, 64 419 -> 420; 2 x 16 heads,
+// 128 wide, 64 sinks 255 -> 268).  Below a sixteenth of the steps that launch costs what it saves (32 heads of 16384 rows, 128
+// wide, window 4096 3744 -> 3788 us).
 template <int P, int IN>
 int launch_window_backward(const sta::WinArgs& a, hipStream_t s) {
   const int64_t bkv = static_cast<int64_t>(a.batch) * (a.heads / a.group);
   const int64_t grid_q = static_cast<int64_t>(a.batch) * a.heads * a.tiles;
   const int64_t behind = a.n - a.window, steps = static_cast<int64_t>(a.key_tiles) * (a.window + sta::WIN_ROWS);
-  const bool apart = !a.key_share && a.far_chunks > 0 && a.sinks <= 64 && 16 * behind > steps;
+  const bool apart = !a.key_share && a.far_chunks > 0 && a.sinks <= 32 && 16 * behind > steps;
   sta::WinArgs keys = a, far = a;
   if (apart) {
     keys.sink_tiles = 0;
