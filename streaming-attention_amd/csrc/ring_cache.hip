@@ -382,7 +382,10 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) acc[ct] = floatx4{0.f, 0.f, 0.f, 0.f};
   float m = -3.4028235e38f, limit = m, l = 0.f;
-  const float room = 8.f / a.c;
+  // fp16 weights are carried times 2^11, at most 2^15: below 2^-14 fp16 holds steps of 2^-24 only, of which a long cache has
+  // many; so a weight loses at most 2^-36 of the largest
+  constexpr bool LIFT = XT == F16;
+  const float room = (LIFT ? 4.f : 8.f) / a.c;
 
   const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
   // a tile's part of the sums; PART: not all of its slots hold a token
@@ -414,7 +417,7 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
       if (PART && 16 * (i >> 2) + (i & 3) >= left) x[i >> 2][i & 3] = -__builtin_inff();
       top = fmaxf(top, x[i >> 2][i & 3]);
     }
-    // the maximum moves, for all lanes of a query at once, when a weight would exceed 2^8
+    // the maximum moves, for all lanes of a query at once, when a weight would exceed 2^8 (fp16: 2^4)
     if (__any(top > limit)) {
       top = fmaxf(top, __shfl_xor(top, 16));
       top = fmaxf(top, __shfl_xor(top, 32));
@@ -428,7 +431,8 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void ring_attention_kernel(
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f((x[i >> 2][i & 3] - m) * a.c);
+      const float y = x[i >> 2][i & 3] - m;
+      p[i] = __builtin_amdgcn_exp2f(LIFT ? fmaf(y, a.c, 11.f) : y * a.c);
       if (PART && 16 * (i >> 2) + (i & 3) >= left) p[i] = 0.f;
       l += p[i];
     }

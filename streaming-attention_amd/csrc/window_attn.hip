@@ -447,6 +447,15 @@ __host__ __device__ constexpr int win_lds_bytes() {
   return 4 * stage > join ? 4 * stage : join;
 }
 
+// The forward kernel's weights relative to the running maximum: at most 2^room, before it moves, and carried times 2^lift.
+// fp16 ends at 2^16, and below 2^-14 it holds steps of 2^-24 only: with 2^11 a weight loses at most 2^-36 of the row's largest,
+// less than the output's rounding for up to 2^24 keys (2^-25 as they are: any number of keys of weight 2^-26 next to one
+// of weight 1 would be lost).
+template <int IN>
+__host__ __device__ constexpr float win_weight_room() { return IN == F16 ? 4.f : 8.f; }
+template <int IN>
+__host__ __device__ constexpr float win_weight_lift() { return IN == F16 ? 11.f : 0.f; }
+
 // Row tiles: keys staged win_keys at a time, the next tile's rows in registers while this one computes, softmax in one
 // pass.  The weights of 16-bit rows enter the second product rounded to their type (half a step each, errors that
 // average over the keys and end below the output's own rounding); their sum is taken before that, in fp32.
@@ -474,7 +483,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
   float m = -1e30f, limit = m, l = 0.f;  // finite: exp2(m_old - m_new) is 0 or at most 1, never a NaN
-  const float room = 8.f / a.c;
+  const float room = win_weight_room<IN>() / a.c;
 
   if (r0 < len) {
     WinFrag<IN> qf[P / 16];
@@ -543,7 +552,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, x[sub][i]);
-      // the maximum moves, for both lanes of a row at once, when a weight would exceed 2^8
+      // the maximum moves, for both lanes of a row at once, when a weight would exceed 2^room
       if (__any(top > limit)) {
         top = fmaxf(top, __shfl_xor(top, 32));
         const float shrink = __builtin_amdgcn_exp2f((m - top) * a.c);
@@ -555,7 +564,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
         m = top;
         limit = m + room;
       }
-      const float mc = m * a.c;
+      const float mc = m * a.c - win_weight_lift<IN>();
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
@@ -616,7 +625,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
                             in ? o[j][2] * inv : 0.f, in ? o[j][3] * inv : 0.f);
       }
       if (a.lse && (threadIdx.x & 7) == 0)
-        a.lse[head_row + at_row] = in ? top * a.c + __builtin_amdgcn_logf(den) : 0.f;
+        a.lse[head_row + at_row] = in ? top * a.c - win_weight_lift<IN>() + __builtin_amdgcn_logf(den) : 0.f;
     }
     for (uint64_t todo = __ballot(bad) & 0x0101010101010101ull; todo; todo &= todo - 1)
       win_forward_row<IN>(a, b, h, r0 + 8 * wave + __builtin_ctzll(todo) / 8);
@@ -646,7 +655,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
           win_store_out<IN>(a, at, col, in ? acc[mt][4 * r] * inv : 0.f, in ? acc[mt][4 * r + 1] * inv : 0.f,
                             in ? acc[mt][4 * r + 2] * inv : 0.f, in ? acc[mt][4 * r + 3] * inv : 0.f);
       }
-    if (a.lse && hh == 0) a.lse[head_row + row] = in ? m * a.c + __builtin_amdgcn_logf(l) : 0.f;
+    if (a.lse && hh == 0) a.lse[head_row + row] = in ? m * a.c - win_weight_lift<IN>() + __builtin_amdgcn_logf(l) : 0.f;
   }
   for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1)
     win_forward_row<IN>(a, b, h, w0 + __builtin_ctzll(todo));
