@@ -15,7 +15,8 @@ from typing import Optional, Tuple, Union
 import torch
 
 import _native
-from sink_window_attention import _STRIDES, _check_gpu, _differentiable_once, _like, _on, _refuse_capture, _strides
+from sink_window_attention import (_STRIDES, _check_gpu, _differentiable_once, _like, _on, _refuse_capture, _refuse_tangents,
+                                   _strides)
 
 Tensor = torch.Tensor
 
@@ -44,6 +45,7 @@ class _Call:
     """The checked arguments of a call, as the kernels take them."""
 
     def __init__(self, q, k, table, q_weight, k_weight, positions, eps, interleaved):
+        _refuse_tangents(q, k, table, q_weight, k_weight)
         if q.ndim != k.ndim or q.ndim not in (2, 3, 4):
             raise ValueError("q and k must be [N,D], [S,H,D] or [B,H,N,D]")
         self.ndim = q.ndim
@@ -174,7 +176,8 @@ def qk_norm_rotary(q: Tensor, k: Tensor, table: Tensor, *, q_weight: Optional[Te
     float32, bfloat16 or float16, D up to 256.  Weights [D] in that dtype or float32 (None: 1).
     positions: int32 or int64, [N] or [B,N] ([S] for [S,H,D]); None: 0 .. N-1.  A position outside the table makes its
     rows (and gradients) NaN; the table takes no gradient.  The results are dense in q's dtype.  Differentiable calls
-    cannot be captured into a graph (RuntimeError); qk_norm_rotary_backward can."""
+    cannot be captured into a graph (RuntimeError); qk_norm_rotary_backward can.  Second and forward-mode derivatives are
+    refused (RuntimeError)."""
     call = _Call(q, k, table, q_weight, k_weight, positions, eps, interleaved)
     if torch.is_grad_enabled() and table.requires_grad:
         raise ValueError("table takes no gradient: pass table.detach()")
@@ -195,5 +198,6 @@ def qk_norm_rotary_backward(q_grad: Tensor, k_grad: Tensor, q: Tensor, k: Tensor
     if q_grad.dtype != q.dtype or k_grad.dtype != q.dtype:
         raise ValueError("gradients must have q's dtype")
     call = _Call(q, k, table, q_weight, k_weight, positions, eps, interleaved)
+    _refuse_tangents(q_grad, k_grad)
     _check_gpu(q, q_grad, k_grad)
     return call.backward(q_grad, k_grad, q, k, q_weight, k_weight)

@@ -20,6 +20,7 @@ import math
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 import _native
 
@@ -205,6 +206,13 @@ def _refuse_capture() -> None:
                            "functions by themselves, or run under torch.no_grad()")
 
 
+def _refuse_tangents(*tensors: Optional[Tensor]) -> None:
+    """The operators have no forward-mode derivative; a result without one would be taken for a constant."""
+    for x in tensors:
+        if x is not None and forward_ad.unpack_dual(x).tangent is not None:
+            raise RuntimeError("forward-mode derivatives are not supported: use the backward pass")
+
+
 def _differentiable_once(backward):
     """once_differentiable where a graph of the gradients is asked for; without one its wrapping costs 5 us a call."""
     once = torch.autograd.function.once_differentiable(backward)
@@ -242,6 +250,7 @@ class _SinkWindow(torch.autograd.Function):
 
 def _checked(q, k, v, window, sinks, scale, lengths):
     window, sinks = _check_tokens(window, sinks)
+    _refuse_tangents(q, k, v)
     q4, k4, v4 = _heads_first(q, k, v)
     _check_dtype(q4, k4, v4)
     lengths = _check_lengths(lengths, q4.shape[0])
@@ -259,7 +268,8 @@ def sink_window_causal_attention(q: Tensor, k: Tensor, v: Tensor, *, window: int
     (values outside 0 .. N are taken as the nearest of them); output rows behind them are zero and take no part in the
     gradients, whatever the padding holds.
     The output has q's dtype; with gradients a 16-bit call also keeps what the output's rounding left.  Differentiable
-    calls cannot be captured into a graph (RuntimeError); use sink_window_forward and sink_window_backward there."""
+    calls cannot be captured into a graph (RuntimeError); use sink_window_forward and sink_window_backward there.  Second
+    and forward-mode derivatives are refused (RuntimeError)."""
     q4, k4, v4, window, sinks, s, lengths = _checked(q, k, v, window, sinks, scale, lengths)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _SinkWindow.apply(q, k, v, window, sinks, s, lengths)
@@ -298,6 +308,7 @@ def sink_window_backward(grad: Tensor, q: Tensor, k: Tensor, v: Tensor, out: Ten
     if tuple(grad.shape) != want or tuple(out.shape) != want or tuple(lse.shape) != want[:3]:
         raise ValueError(f"grad and out must be {want} and lse {want[:3]}")
     _check_dtype(q4, grad, out)
+    _refuse_tangents(grad, out, lse, rest)
     if rest is not None and (q4.dtype == torch.float32 or rest.shape != out.shape or rest.dtype != out.dtype):
         raise ValueError("rest must be like out, and None for float32")
     if lse.dtype != torch.float32:
@@ -321,7 +332,7 @@ class SinkWindowStreamingAttention:
     A token held with an infinity or NaN makes the outputs that it reaches NaN or infinite until it leaves.
 
     Calls run on the device's current stream and may be captured into graphs (replays advance the state like
-    calls); calls on one object have to be ordered, by one stream or by events."""
+    calls); calls on one object have to be ordered, by one stream or by events.  Results take no part in derivatives."""
 
     def __init__(self, dim: int, value_dim: int, *, streams: int = 1, heads: int = 1, kv_heads: Optional[int] = None,
                  window: int, sinks: int = 4, scale: Optional[float] = None,
