@@ -372,7 +372,7 @@ class SinkWindowStreamingAttention:
         self._dense = _STRIDES[6](heads * dim, dim, kv_heads * dim, dim, kv_heads * value_dim, value_dim)
         self._bytes = _native.lib().sta_ring_attention_bytes(streams, heads, kv_heads, dim, value_dim, self.window,
                                                              self.sinks)
-        self._fresh = True
+        self._used = False  # a call has changed the state, or has been captured to
 
     @property
     def lengths(self) -> Tensor:
@@ -410,7 +410,7 @@ class SinkWindowStreamingAttention:
         q = self._rows(query, shapes["query"], "query")
         k = self._rows(key, shapes["key"], "key")
         v = self._rows(value, shapes["value"], "value")
-        self._fresh = False
+        self._used = True
         return self._attend(q, k, v)
 
     def query(self, query: Tensor) -> Tensor:
@@ -426,7 +426,7 @@ class SinkWindowStreamingAttention:
     def _extend(self, k: Tensor, v: Tensor, counts: Optional[Tensor]) -> None:
         if k.shape[2] == 0:
             return
-        self._fresh = False
+        self._used = True
         with _on(self.device):
             st = _native.lib().sta_ring_extend(
                 k.data_ptr(), v.data_ptr(), self._code, self._store, self.streams, self.kv_heads, k.shape[2], self.dim,
@@ -455,13 +455,19 @@ class SinkWindowStreamingAttention:
     @torch.no_grad()
     def prefill(self, q: Tensor, k: Tensor, v: Tensor, *, counts: Optional[Tensor] = None) -> Tensor:
         """Outputs [S,H,P,value_dim] of a prompt's rows (sink_window_causal_attention, on the rows as given), leaving
-        the state after it.  Only on a fresh state."""
-        if not self._fresh:
+        the state after it.  Only on an empty state: on an object that has been used the call waits for the device to
+        see that it is.  A captured call cannot see that; it empties the state itself, so that every replay starts there."""
+        with _on(self.device):
+            captured = torch.cuda.is_current_stream_capturing()
+        # the device's counts decide: replays of captured calls change them unseen
+        if not captured and self._used and bool(self._counts.any()):
             raise ValueError("prefill starts from an empty state; use step() / extend() afterwards")
         k, v, counts = self._prompt(k, v, counts)
         q = self._rows(q, (self.streams, self.heads, k.shape[2], self.dim), "q")
         out = sink_window_causal_attention(q, k, v, window=self.window, sinks=self.sinks, scale=self.scale,
                                            lengths=counts)
+        if captured:
+            self._counts.zero_()
         self._extend(k, v, counts)
         return out
 
@@ -469,7 +475,6 @@ class SinkWindowStreamingAttention:
         """Forgets every token of all streams, or of the given ones (new sequences start there)."""
         if streams is None:
             self._counts.zero_()
-            self._fresh = True
             return
         streams = list(streams)
         for i in streams:
@@ -523,4 +528,4 @@ class SinkWindowStreamingAttention:
         for x, y in zip((self._counts, *self._cache), (state["counts"], *state["cache"])):
             if x is not None:
                 x.copy_(y)
-        self._fresh = not bool(state["counts"].any())
+        self._used = True
