@@ -24,7 +24,7 @@ import csv
 import math
 import pathlib
 import sys
-from typing import Dict, List
+from typing import Dict, List, Optional
 
 import torch
 
@@ -33,8 +33,9 @@ if str(_HERE) not in sys.path:
     sys.path.insert(0, str(_HERE))
 
 from _cli_util import fmt_bytes, pick_device, wall_ms  # noqa: E402
+from _native import DTYPE_CODES  # noqa: E402
 from fast_article_attention import _make_data, _resolve_dtype  # noqa: E402
-from sink_window_attention import sink_window_causal_attention  # noqa: E402
+from sink_window_attention import MAX_DIM, sink_window_causal_attention  # noqa: E402
 from streaming_taylor_coreset_attention import (  # noqa: E402
     article_causal_attention,
     classical_causal_attention,
@@ -152,8 +153,27 @@ def parser() -> argparse.ArgumentParser:
     return p
 
 
+def check_window(args: argparse.Namespace) -> Optional[str]:
+    """What --window cannot take; asked before the first row is measured."""
+    if args.window is None:
+        return None
+    if args.window < 1 or args.sinks < 0:
+        return "--window must be at least 1 and --sinks non-negative"
+    if not (1 <= args.d <= MAX_DIM and 1 <= args.dv <= MAX_DIM):
+        return f"--window takes --d and --dv of 1 to {MAX_DIM}"
+    if _resolve_dtype(args.dtype) not in DTYPE_CODES:
+        return "--window takes float32, bfloat16 and float16"
+    if args.scale is not None and not math.isfinite(args.scale):
+        return "--window takes a finite --scale"
+    return None
+
+
 def main(argv=None) -> List[Dict[str, object]]:
-    args = parser().parse_args(argv)
+    p = parser()
+    args = p.parse_args(argv)
+    wrong = check_window(args)
+    if wrong:
+        p.error(wrong)
     rows = [run_one(args, n) for n in args.sweep_n]
     print_table(rows)
     if args.csv is not None:
