@@ -185,8 +185,8 @@ int sta_window_attention_backward(const void* grad, const void* q, const void* k
   a.dv_out = dv_out;
   if (dtype == STA_F16) {
     // fp16 weights of long rows are subnormal (1 / 4096 has 10 bits left): they and their gradients are carried times
-    // a power of two near the number of keys, at most 2^10, so that weights near 1 times gradients up to 64 fit;
-    // rows beyond that come out infinite and are taken again in fp32
+    // a power of two near the number of keys, at most 2^10; the gradients of rows and keys for which that is too much
+    // are lowered from there (win_lower)
     const int64_t keys = static_cast<int64_t>(a.window) + a.sinks < a.n ? a.window + a.sinks : a.n;
     int e = 0;
     while (e < 10 && (int64_t(2) << e) <= keys) ++e;

@@ -257,6 +257,24 @@ __device__ __forceinline__ void win_pin(floatx16& x) {
   if constexpr (PIN) asm volatile("" : "+a"(x));
 }
 
+// fp16's gradients of logits, p (do.v - D), are carried times a power of two: at first the weights' `lift`, and where one of a
+// row (dq; of a key: dk) would pass 65504 a lower one for that row alone, from there on, with what was summed before
+// lowered too.  Then the largest is between 2^11 and 2^12, so what the others lose below fp16's normal range is at most 2^-36
+// of it.  (With the lift alone such rows and keys came out infinite and were taken again one by one: 8 x 16 heads of 4096 x 64,
+// window 1024, unit normal gradients times 1 / 64 / 1024: 0.78 / 13.8 / 338 ms; so 0.79 / 0.75 / 0.80.)
+// The factor by which operands up to `big` are lowered; infinities stay.
+__device__ __forceinline__ float win_lower(float big) {
+  const uint32_t e = __float_as_uint(big) >> 23;
+  return big > 65504.f && e < 255u ? __uint_as_float((265u - e) << 23) : 1.f;
+}
+// the largest magnitude of a lane's elements (NaN left out)
+__device__ __forceinline__ float win_largest(const floatx16& x) {
+  float big = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) big = fmaxf(big, fabsf(x[i]));
+  return big;
+}
+
 __device__ __forceinline__ bool win_finite(float x) { return fabsf(x) < __builtin_inff(); }
 
 // four values of a row at column col (a multiple of 4) of a dense [.., width] tensor
@@ -719,7 +737,7 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
-  float delta = 0.f;
+  float delta = 0.f, drop = a.drop;
 
   if (r0 < len) {
     WinFrag<IN> qf[P / 16], gf[P / 16];
@@ -767,7 +785,7 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
     };
     const int start = SHARE ? wave : 0;
     if (AHEAD && start < count) load(start);
-    const float shift = __builtin_amdgcn_logf(a.lift) - lse;
+    float shift = __builtin_amdgcn_logf(a.lift) - lse;
     for (int it = start; it < count; it += STEP) {
       if (!AHEAD) load(it);
       win_sync<SHARE>();
@@ -802,6 +820,21 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
             x[i] = seen ? x[i] : 0.f;
           }
         }
+        if constexpr (IN == F16) {
+          float big = win_largest(x);
+          if (__any(big > 65504.f)) {
+            big = fmaxf(big, __shfl_xor(big, 32));
+            const float f = win_lower(big);
+            drop /= f;
+            shift += __builtin_amdgcn_logf(f);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] *= f;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[mt][i] *= f;
+          }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const WinFrag<IN> p = win_operand<IN>(x, t);
@@ -814,17 +847,23 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
   }
 
   if constexpr (SHARE) {
-    float* red = reinterpret_cast<float*>(win_lds);
-    const float one[4] = {1.f, 1.f, 1.f, 1.f}, f = a.scale * a.drop;
+    float *red = reinterpret_cast<float*>(win_lds), *red_d = red + win_join_floats<P>();
+    float weight[4] = {1.f, 1.f, 1.f, 1.f};
     __syncthreads();
     win_join_put<P>(red, acc, wave, lane);
+    if (IN == F16 && hh == 0) red_d[32 * wave + lane] = drop;
     __syncthreads();
+    if constexpr (IN == F16) {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) weight[w] = red_d[32 * w + threadIdx.x / 8];
+    }
+    const float f = a.scale;
     const int at_row = r0 + threadIdx.x / 8;
     floatx4 o[MT];
     int bad = 0;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
-      o[j] = win_join_get<P>(red, 32 * j + 4 * (threadIdx.x & 7), one);
+      o[j] = win_join_get<P>(red, 32 * j + 4 * (threadIdx.x & 7), weight);
       bad |= win_bad4(o[j]);
     }
     bad = at_row < len ? bad : 0;
@@ -857,7 +896,7 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
   bad |= __shfl_xor(bad, 32);
   if (row < a.n && !bad) {
     const int64_t at = (head_row + row) * a.d;
-    const float f = a.scale * a.drop;
+    const float f = a.scale * drop;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -918,7 +957,8 @@ template <int P, int IN, bool SHARE>
 __host__ __device__ constexpr int win_dkv_lds() {
   const int rows = win_staged_rows<IN, SHARE>(), stage = 2 * rows * P * (IN == F32 ? 4 : 2) + 2 * rows * 4;
   if (!SHARE) return (win_pipe<P, IN, SHARE>() ? 3 : 2) * stage;
-  return 4 * stage > 4 * win_join_floats<P>() ? 4 * stage : 4 * win_join_floats<P>();
+  const int join = 4 * (win_join_floats<P>() + 4 * 32);
+  return 4 * stage > join ? 4 * stage : join;
 }
 
 // dk and dv: one workgroup per 128 keys of a key head (32 a wave) walks over the rows that see them within the window,
@@ -974,6 +1014,33 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) dk[mt][i] = dv[mt][i] = 0.f;
+  // by what the key's gradients of logits are lowered (see win_lower), and what they are looked at above: 65504, or any once one
+  // of the wave's keys has been lowered
+  float lower = 1.f, limit = 65504.f;
+  // g as it fits
+  auto fit = [&](floatx16& g) {
+    if constexpr (IN == F16) {
+      if (__any(win_largest(g) > limit)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g[i] *= lower;
+        float big = win_largest(g);
+        big = fmaxf(big, __shfl_xor(big, 32));
+        const float f = win_lower(big);
+        if (!__any(f < 1.f)) return;
+        lower *= f;
+        limit = -1.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g[i] *= f;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          win_pin<WAVES == 1>(dk[mt]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) dk[mt][i] *= f;
+          win_pin<WAVES == 1>(dk[mt]);
+        }
+      }
+    }
+  };
 
   if (lo <= hi) {
     WinFrag<IN> kf[P / 16], vf[P / 16];
@@ -1173,6 +1240,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
           }
           asm volatile("" : "+v"(x0), "+v"(g0));
           if (!whole(q0 + 32 * sub, 32)) hide(x0, g0, q0 + 32 * sub + 4 * hh);
+          fit(g0);
           WinFrag<IN> p[2], ds[2];
           p[0] = win_operand<IN>(x0, 0);
           ds[0] = win_operand<IN>(g0, 0);
@@ -1305,6 +1373,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
             x[i] = p;
           }
           if (!all) hide(x, g, q0 + 32 * sub + 4 * hh);
+          fit(g);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
@@ -1344,7 +1413,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
   }
 
   // sums to be added to others' (the sinks of a call with rows behind their window)
-  const float f = a.scale * a.drop;
+  const float f = a.scale * a.drop / (SHARE ? 1.f : lower);
   auto part_at = [&](int j) {
     return ((static_cast<int64_t>(bh) * (a.far_chunks + 1) + chunk + 1) * a.sink_rows + j) * (a.d + a.dv);
   };
@@ -1398,8 +1467,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
     }
     };
   if constexpr (SHARE) {
-    float* red = reinterpret_cast<float*>(win_lds);
-    const float one[4] = {1.f, 1.f, 1.f, 1.f};
+    float *red = reinterpret_cast<float*>(win_lds), *red_f = red + win_join_floats<P>();
     const int j = k0 + threadIdx.x / 8;
     floatx4 o[2][MT];
     int bad = 0;
@@ -1407,10 +1475,16 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
     for (int value = 0; value < 2; ++value) {
       __syncthreads();
       win_join_put<P>(red, value ? dv : dk, wave, lane);
+      if (IN == F16 && value == 0 && hh == 0) red_f[32 * wave + lane] = 1.f / lower;
       __syncthreads();
+      float weight[4] = {1.f, 1.f, 1.f, 1.f};
+      if constexpr (IN == F16) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) weight[w] = value ? 1.f : red_f[32 * w + threadIdx.x / 8];
+      }
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        o[value][mt] = win_join_get<P>(red, 32 * mt + 4 * (threadIdx.x & 7), one);
+        o[value][mt] = win_join_get<P>(red, 32 * mt + 4 * (threadIdx.x & 7), weight);
         bad |= win_bad4(o[value][mt]);
       }
     }
