@@ -20,7 +20,8 @@
 //
 // Hidden pairs are left out by selects, never by arithmetic on their logits.  A tile's products still multiply hidden
 // pairs' zero weights with their values, so an infinity or NaN in a value that some rows of a tile see would reach
-// those that do not: a result row that is not finite is taken again over its visible pairs alone (win_*_row).
+// those that do not: a workgroup with a result that is not finite goes over its tiles once more, taking the partly visible ones
+// pair by pair (win_add_seen), and stores that result from there.
 #include <type_traits>
 
 #include "rows.hpp"
@@ -223,6 +224,47 @@ __device__ __forceinline__ WinFrag<IN> win_read_columns(const uint4* lds, int r0
   return f;
 }
 
+// acc += weights times values of 32 staged rows from r0 (a multiple of 32), over the seen pairs alone: bit i of a lane's `seen`
+// stands for its element i, whose row win_mma's layout gives.  By vector instructions, row after row, which only results that
+// are not finite ask for: backward, bf16, one NaN in the gradient of 32 heads of 16384 x 128, window 4096, 11 ms (4.2 without it; 900
+// with rows and keys taken alone by a wave each), a gradient that is NaN throughout of 8 x 16 heads of 4096 x 64, window 1024, 2.8
+// ms (0.87; 344).
+template <int P, int IN>
+__device__ __forceinline__ void win_add_seen(floatx16 (&acc)[P / 32], const floatx16& weights, uint32_t seen, const uint4* lds,
+                                             int r0, int lane) {
+  constexpr int ES = IN == F32 ? 4 : 2, E = 16 / ES, CH = win_chunks<ES>(P);
+  floatx16 w = weights;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = r0 + 8 * (i >> 2) + 4 * half + (i & 3), from = (lane & 31) + 32 * half;
+      const float p = __shfl(w[0], from);
+      const bool in = __shfl(static_cast<int>(seen), from) & 1;
+#pragma unroll
+      for (int mt = 0; mt < P / 32; ++mt) {
+        // the columns of the lane's accumulator elements, four neighbours at a time
+        uint32_t v[4][ES];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int col = 32 * mt + 8 * c + 4 * (lane >> 5);
+          const uint4* unit = lds + r * CH + ((col / E) ^ win_swizzle<CH>(r));
+          __builtin_memcpy(v[c], __builtin_assume_aligned(reinterpret_cast<const char*>(unit) + col % E * ES, 4 * ES), 4 * ES);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float x = load_elem(v[e >> 2], e & 3, IN);
+          acc[mt][e] = in ? fmaf(p, x, acc[mt][e]) : acc[mt][e];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 15; ++j) w[j] = w[j + 1];
+    seen >>= 1;
+  }
+}
+
 // 8 dimensions at column 16 s + 8 h of a row in memory (none of a row of width 0), with the sign of the scale in `flip`
 template <int IN>
 __device__ __forceinline__ WinFrag<IN> win_load_row(const char* row, int s, int h, int width, uint32_t flip) {
@@ -246,7 +288,7 @@ __device__ __forceinline__ void win_keep(WinFrag<IN>& f, bool row) {
 
 // waves a SIMD of window_dkv_kernel
 template <int P, int IN>
-__host__ __device__ constexpr int win_dkv_waves() { return IN != F32 && P <= 64 ? 2 : 1; }
+__host__ __device__ constexpr int win_dkv_waves() { return IN != F32 && P <= 64 ? (P > 32 ? 2 : 3) : 1; }
 // whether its instructions are laid out by hand
 template <int P, int IN, bool SHARE>
 __host__ __device__ constexpr bool win_pipe() { return !SHARE && IN != F32 && win_dkv_waves<P, IN>() == 1; }
@@ -304,12 +346,6 @@ __device__ __forceinline__ void win_store4(void* base, int64_t row_at, int col, 
   if (col + 3 < width) store_elem(base, at + 3, IN, d);
 }
 
-__device__ __forceinline__ float win_wave_sum(float x) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
-  return x;
-}
-
 // what the rounding of x to the rows' type leaves (0 of an infinity or NaN)
 template <int IN>
 __device__ __forceinline__ float win_rest(float x) {
@@ -332,68 +368,10 @@ __device__ __forceinline__ void win_store_out(const WinArgs& a, int64_t row_at, 
   }
 }
 
-template <int IN>
-__device__ __forceinline__ float win_dot(const void* x, const void* y, int width) {
-  float s = 0.f;
-  for (int c = 0; c < width; ++c) s = fmaf(load_elem(x, c, IN), load_elem(y, c, IN), s);
-  return s;
-}
-
 __device__ __forceinline__ int win_length(const WinArgs& a, int b) {
   if (!a.lengths) return a.n;
   const int len = a.lengths[b];
   return len < 0 ? 0 : (len > a.n ? a.n : len);
-}
-
-// Visible keys of row i in order: the sinks that the window has passed, then the window.
-struct WinKeys {
-  int sinks, first, count;
-  __device__ __forceinline__ WinKeys(const WinArgs& a, int i) {
-    first = i - a.window + 1 > 0 ? i - a.window + 1 : 0;
-    sinks = a.sinks < first ? a.sinks : first;
-    count = sinks + i - first + 1;
-  }
-  __device__ __forceinline__ int key(int t) const { return t < sinks ? t : first + t - sinks; }
-};
-
-// One row by one wave over its visible keys, in fp32 without matrix instructions.
-template <int IN>
-__device__ void win_forward_row(const WinArgs& a, int b, int h, int i) {
-  constexpr int ES = IN == F32 ? 4 : 2;
-  const int lane = threadIdx.x & 63;
-  const WinKeys keys(a, i);
-  const void* q = rows_at<ES>(a.q, b, h, i);
-  float m = -__builtin_inff();
-  for (int t = lane; t < keys.count; t += 64)
-    m = fmaxf(m, a.scale * win_dot<IN>(q, rows_at<ES>(a.k, b, h / a.group, keys.key(t)), a.d));
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-  float l = 0.f, acc[2] = {0.f, 0.f};
-  for (int t0 = 0; t0 < keys.count; t0 += 64) {
-    const int t = t0 + lane;
-    float p = 0.f;
-    if (t < keys.count)
-      p = expf(a.scale * win_dot<IN>(q, rows_at<ES>(a.k, b, h / a.group, keys.key(t)), a.d) - m);
-    l += p;
-    for (int u = 0; u < 64 && t0 + u < keys.count; ++u) {
-      const float w = __shfl(p, u);
-      const void* v = rows_at<ES>(a.v, b, h / a.group, keys.key(t0 + u));
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < a.dv) acc[e] = fmaf(w, load_elem(v, lane + 64 * e, IN), acc[e]);
-    }
-  }
-  l = win_wave_sum(l);
-  const int64_t row = (static_cast<int64_t>(b) * a.heads + h) * a.n + i;
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.dv) {
-      store_elem(a.out, row * a.dv + lane + 64 * e, IN, acc[e] / l);
-      if constexpr (IN != F32) {
-        if (a.rest) store_elem(a.rest, row * a.dv + lane + 64 * e, IN, win_rest<IN>(acc[e] / l));
-      }
-    }
-  if (a.lse && lane == 0) a.lse[row] = m * 1.44269504f + log2f(l);
 }
 
 // Two ways to deal out a head's rows.  Wide: 128 rows (keys) a workgroup, 32 a wave, which share the staged tiles of the
@@ -441,6 +419,19 @@ __device__ __forceinline__ int win_bad4(const floatx4& x) {
   return !(win_finite(x[0]) && win_finite(x[1]) && win_finite(x[2]) && win_finite(x[3]));
 }
 
+// Results that are finite are stored by a first pass over the tiles, the others by a second, careful one, which every thread of
+// the workgroup takes if one result is not.  A pass is told which lanes' results were left, and tells.  It costs the first
+// pass up to 4 % (registers, a barrier at its end).
+template <typename Pass>
+__device__ __forceinline__ void win_passes(Pass pass) {
+  __shared__ int more;
+  if (threadIdx.x == 0) more = 0;  // a barrier lies between this and a result
+  const int bad = pass(std::false_type{}, 0);
+  if (__any(bad)) more = 1;
+  __syncthreads();
+  if (more) pass(std::true_type{}, bad);
+}
+
 // Which (batch, query head, tile) a workgroup takes: the heads of a group and the neighbouring tiles of a head on one
 // XCD, whose L2 then holds the keys they share; the last tiles (most keys) first.
 __device__ __forceinline__ void win_place(const WinArgs& a, int& b, int& h, int& tile) {
@@ -454,6 +445,16 @@ __device__ __forceinline__ void win_place(const WinArgs& a, int& b, int& h, int&
   b = id / kv;
 }
 
+// waves a SIMD of the forward and the dq kernel: what their first pass has room for (the second one may spill)
+template <int P, int IN, bool SHARE>
+__host__ __device__ constexpr int win_row_waves() {
+  return P > 64 ? (IN == F32 ? 1 : 2) : (IN == F32 && SHARE ? 2 : (P == 64 ? 3 : 4));
+}
+template <int P, int IN, bool SHARE>
+__host__ __device__ constexpr int win_dq_waves() {
+  if (IN == F32) return P > 64 || (SHARE && P > 32) ? 1 : (P > 32 || SHARE ? 2 : 3);
+  return SHARE && P > 96 ? 1 : (SHARE || P > 64 ? 2 : (P > 32 ? 3 : 4));
+}
 template <int IN, bool SHARE>
 __host__ __device__ constexpr int win_keys() { return IN == F32 || SHARE ? 32 : 64; }
 // LDS of the forward and the dq kernel
@@ -481,11 +482,10 @@ __host__ __device__ constexpr float win_weight_lift() { return IN == F16 ? 11.f 
 // matrix product reaches 1180).  8 x 16 heads of 4096 rows, 64 wide, window 1024: 0.20 ms, 600 TFLOP/s, bound by the vector
 // unit: a tile of 64 keys takes 16 products (512 cycles of the matrix unit) but 32 exponentials, a quarter of the rate,
 // and about 150 other instructions (1100 cycles); 4 waves a SIMD instead of 3 change nothing.
-template <int P, int IN, bool SHARE>
-__global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forward_kernel(const WinArgs a) {
+template <int P, int IN, bool SHARE, bool CAREFUL>
+__device__ __forceinline__ int window_forward_pass(const WinArgs& a, int again) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
                 MT = P / 32, STEP = SHARE ? 4 : 1;
-  constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
   extern __shared__ uint4 win_lds[];
   int b, h, tile;
   win_place(a, b, h, tile);
@@ -495,12 +495,15 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
   const int r0 = tile * win_rows<SHARE>(), w0 = r0 + (SHARE ? 0 : 32 * wave), row = w0 + (lane & 31);
   const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
 
+  constexpr bool AHEAD = !CAREFUL && win_ahead<P, IN, SHARE>();
+  int bad = 0;
   floatx16 acc[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
-  float m = -1e30f, limit = m, l = 0.f;  // finite: exp2(m_old - m_new) is 0 or at most 1, never a NaN
+  // finite: exp2(m_old - m_new) is 0 or at most 1, never a NaN; rows whose logits are all below have no weights, and are bad
+  float m = CAREFUL ? -3.4e38f : -1e30f, limit = m, l = 0.f;
   const float room = win_weight_room<IN>() / a.c;
 
   if (r0 < len) {
@@ -540,7 +543,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       // of the wave's rows, does one see one of the keys; do all see all of them
       const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
       if (!some) continue;
-      const bool all = key0 + BK - 1 <= w0 && (w0 + 31 - key0 < a.window || key0 + BK <= a.sinks);
+      const bool all = (key0 + BK - 1 <= w0) & ((w0 + 31 - key0 < a.window) | (key0 + BK <= a.sinks));
       floatx16 x[NSUB];
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub)
@@ -551,6 +554,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
 #pragma unroll
         for (int sub = 0; sub < NSUB; ++sub)
           win_mma<IN>(x[sub], win_read_row<P, IN>(ks, 32 * sub + (lane & 31), s, hh), qf[s]);
+      uint32_t pairs[NSUB] = {};
       if (!all) {
         // key <= row within the window in one comparison; of the sinks those up to the row
         const int ahead = row - key0 - 4 * hh, sinks = min(a.sinks, row + 1) - key0 - 4 * hh;
@@ -563,6 +567,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
             bool seen = static_cast<uint32_t>(ahead - k) < static_cast<uint32_t>(a.window);
             if (far) seen = seen | (k < sinks);
             x[sub][i] = seen ? x[sub][i] : -__builtin_inff();
+            if constexpr (CAREFUL) pairs[sub] |= static_cast<uint32_t>(seen) << i;
           }
       }
       float top = m;
@@ -586,11 +591,22 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[sub][i] = __builtin_amdgcn_exp2f(fmaf(x[sub][i], a.c, -mc));
+        for (int i = 0; i < 16; ++i) {
+          // a product m c of more than 2^31 is off by more than an exponent holds: such rows are bad too
+          if constexpr (CAREFUL)
+            x[sub][i] = __builtin_amdgcn_exp2f(fmaf(x[sub][i] - m, a.c, win_weight_lift<IN>()));
+          else
+            x[sub][i] = __builtin_amdgcn_exp2f(fmaf(x[sub][i], a.c, -mc));
+        }
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
         for (int i = 0; i < 16; ++i) l += x[sub][i];
+      if (CAREFUL && !all) {
+#pragma unroll
+        for (int sub = 0; sub < NSUB; ++sub) win_add_seen<P, IN>(acc, x[sub], pairs[sub], vs, 32 * sub, lane);
+        continue;
+      }
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub)
 #pragma unroll
@@ -623,9 +639,10 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       den = fmaf(f[w], red_l[32 * w + r], den);
     }
     const bool in = at_row < len;
+    if (CAREFUL && !(den > 0.f)) den = __builtin_nanf("");  // no logit above -inf
     const float inv = in ? 1.f / den : 0.f;
     floatx4 o[MT];
-    int bad = !(den > 0.f && win_finite(den));
+    bad = !(den > 0.f && win_finite(den));
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       o[j] = win_join_get<P>(red, 32 * j + 4 * (threadIdx.x & 7), f);
@@ -634,7 +651,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
     bad = in ? bad : 0;
 #pragma unroll
     for (int x = 1; x < 8; x <<= 1) bad |= __shfl_xor(bad, x);
-    if (at_row < a.n && !bad) {
+    if (at_row < a.n && (CAREFUL ? again : !bad)) {
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
         const int col = 32 * j + 4 * (threadIdx.x & 7);
@@ -645,15 +662,13 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       if (a.lse && (threadIdx.x & 7) == 0)
         a.lse[head_row + at_row] = in ? top * a.c - win_weight_lift<IN>() + __builtin_amdgcn_logf(den) : 0.f;
     }
-    for (uint64_t todo = __ballot(bad) & 0x0101010101010101ull; todo; todo &= todo - 1)
-      win_forward_row<IN>(a, b, h, r0 + 8 * wave + __builtin_ctzll(todo) / 8);
-    return;
+    return bad;
   }
 
   const bool in = row < len;
   float inv = 0.f;
-  int bad = 0;
   if (in) {
+    if (CAREFUL && !(l > 0.f)) l = __builtin_nanf("");
     inv = 1.f / l;
     bad = !(l > 0.f && win_finite(l));
 #pragma unroll
@@ -662,7 +677,7 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       for (int i = 0; i < 16; ++i) bad |= !win_finite(acc[mt][i]);
   }
   bad |= __shfl_xor(bad, 32);
-  if (row < a.n && !bad) {
+  if (row < a.n && (CAREFUL ? again : !bad)) {
     const int64_t at = (head_row + row) * a.dv;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -675,40 +690,12 @@ __global__ __launch_bounds__(256, IN == F32 && P > 64 ? 1 : 2) void window_forwa
       }
     if (a.lse && hh == 0) a.lse[head_row + row] = in ? m * a.c - win_weight_lift<IN>() + __builtin_amdgcn_logf(l) : 0.f;
   }
-  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1)
-    win_forward_row<IN>(a, b, h, w0 + __builtin_ctzll(todo));
+  return bad;
 }
 
-// dq_i over the visible keys of row i by one wave; `delta` is D_i.
-template <int IN>
-__device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
-  constexpr int ES = IN == F32 ? 4 : 2;
-  const int lane = threadIdx.x & 63, hk = h / a.group;
-  const WinKeys keys(a, i);
-  const void* q = rows_at<ES>(a.q, b, h, i);
-  const void* go = rows_at<ES>(a.go, b, h, i);
-  const int64_t row = (static_cast<int64_t>(b) * a.heads + h) * a.n + i;
-  const float lse = a.lse[row];
-  float acc[2] = {0.f, 0.f};
-  for (int t0 = 0; t0 < keys.count; t0 += 64) {
-    const int t = t0 + lane;
-    float ds = 0.f;
-    if (t < keys.count) {
-      const int key = keys.key(t);
-      const float x = a.scale * win_dot<IN>(q, rows_at<ES>(a.k, b, hk, key), a.d);
-      ds = exp2f(fmaf(x, 1.44269504f, -lse)) * (win_dot<IN>(go, rows_at<ES>(a.v, b, hk, key), a.dv) - delta);
-    }
-    for (int u = 0; u < 64 && t0 + u < keys.count; ++u) {
-      const float w = __shfl(ds, u);
-      const void* k = rows_at<ES>(a.k, b, hk, keys.key(t0 + u));
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < a.d) acc[e] = fmaf(w, load_elem(k, lane + 64 * e, IN), acc[e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 2; ++e)
-    if (lane + 64 * e < a.d) store_elem(a.dq, row * a.d + lane + 64 * e, IN, a.scale * acc[e]);
+template <int P, int IN, bool SHARE>
+__global__ __launch_bounds__(256, (win_row_waves<P, IN, SHARE>())) void window_forward_kernel(const WinArgs a) {
+  win_passes([&](auto second, int again) { return window_forward_pass<P, IN, SHARE, decltype(second)::value>(a, again); });
 }
 
 // dq and D: the forward kernel's walk over the keys with the rows' statistics given.  D of a rounded out is off by do.(out -
@@ -717,11 +704,10 @@ __device__ void win_dq_row(const WinArgs& a, int b, int h, int i, float delta) {
 // its product with the keys like the weights of the forward kernel.  32 heads of 16384 rows, 128 wide, window 4096,
 // bf16: 1.45 ms, three products at 995 TFLOP/s, bound by them; 8 x 16 heads of 4096 rows, 64 wide, window 1024: 291 us with
 // three waves a SIMD (one register less a lane than the compiler takes by itself), 316 with two.
-template <int P, int IN, bool SHARE>
-__global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 && !SHARE ? 3 : 2)) void window_dq_kernel(const WinArgs a) {
+template <int P, int IN, bool SHARE, bool CAREFUL>
+__device__ __forceinline__ int window_dq_pass(const WinArgs& a, int again) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
                 MT = P / 32, STEP = SHARE ? 4 : 1;
-  constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
   extern __shared__ uint4 win_lds[];
   int b, h, tile;
   win_place(a, b, h, tile);
@@ -732,12 +718,15 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
   const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
   const bool in = row < len;
 
+  constexpr bool AHEAD = !CAREFUL && win_ahead<P, IN, SHARE>();
+  int bad = 0;
   floatx16 acc[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
   float delta = 0.f, drop = a.drop;
+  bool lost = false;  // the row's statistics are NaN, and with them all of its gradient
 
   if (r0 < len) {
     WinFrag<IN> qf[P / 16], gf[P / 16];
@@ -767,6 +756,7 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
     }
     delta += __shfl_xor(delta, 32);
     const float lse = in ? a.lse[head_row + row] : 0.f;
+    lost = delta != delta || lse != lse;
     if (in && hh == 0 && (!SHARE || wave == 0)) a.delta[head_row + row] = delta;
 
     const int last = (r0 + win_rows<SHARE>() < len ? r0 + win_rows<SHARE>() : len) - 1;
@@ -796,7 +786,7 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
       if (AHEAD && it + STEP < count) load(it + STEP);
       const bool some = key0 <= w0 + 31 && w0 < len && (w0 - (key0 + BK - 1) < a.window || key0 < a.sinks);
       if (!some) continue;
-      const bool all = key0 + BK - 1 <= w0 && (w0 + 31 - key0 < a.window || key0 + BK <= a.sinks);
+      const bool all = (key0 + BK - 1 <= w0) & ((w0 + 31 - key0 < a.window) | (key0 + BK <= a.sinks));
 #pragma unroll
       for (int sub = 0; sub < NSUB; ++sub) {
         floatx16 x, g;
@@ -809,6 +799,7 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = __builtin_amdgcn_exp2f(fmaf(x[i], a.c, shift)) * (g[i] - delta);
+        uint32_t pairs = 0;
         if (!all) {
           const int ahead = row - key0 - 4 * hh, sinks = min(a.sinks, row + 1) - key0 - 4 * hh;
           const bool far = key0 < a.sinks;
@@ -818,6 +809,7 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
             bool seen = static_cast<uint32_t>(ahead - k) < static_cast<uint32_t>(a.window);
             if (far) seen = seen | (k < sinks);
             x[i] = seen ? x[i] : 0.f;
+            if constexpr (CAREFUL) pairs |= static_cast<uint32_t>(seen) << i;
           }
         }
         if constexpr (IN == F16) {
@@ -834,6 +826,10 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
 #pragma unroll
               for (int i = 0; i < 16; ++i) acc[mt][i] *= f;
           }
+        }
+        if (CAREFUL && !all) {
+          win_add_seen<P, IN>(acc, x, pairs, ks, 32 * sub, lane);
+          continue;
         }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -857,19 +853,19 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
 #pragma unroll
       for (int w = 0; w < 4; ++w) weight[w] = red_d[32 * w + threadIdx.x / 8];
     }
-    const float f = a.scale;
     const int at_row = r0 + threadIdx.x / 8;
+    lost = __shfl(static_cast<int>(lost), threadIdx.x / 8);
+    const float f = lost ? __builtin_nanf("") : a.scale;
     floatx4 o[MT];
-    int bad = 0;
 #pragma unroll
     for (int j = 0; j < MT; ++j) {
       o[j] = win_join_get<P>(red, 32 * j + 4 * (threadIdx.x & 7), weight);
       bad |= win_bad4(o[j]);
     }
-    bad = at_row < len ? bad : 0;
+    bad = at_row < len && !lost ? bad : 0;
 #pragma unroll
     for (int x = 1; x < 8; x <<= 1) bad |= __shfl_xor(bad, x);
-    if (at_row < a.n && !bad) {
+    if (at_row < a.n && (CAREFUL ? again : !bad)) {
       const bool real = at_row < len;
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
@@ -879,24 +875,19 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
                          real ? o[j][2] * f : 0.f, real ? o[j][3] * f : 0.f);
       }
     }
-    for (uint64_t todo = __ballot(bad) & 0x0101010101010101ull; todo; todo &= todo - 1) {
-      const int r = 8 * wave + __builtin_ctzll(todo) / 8;
-      win_dq_row<IN>(a, b, h, r0 + r, __shfl(delta, r));
-    }
-    return;
+    return bad;
   }
 
-  int bad = 0;
-  if (in) {
+  if (in && !lost) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) bad |= !win_finite(acc[mt][i]);
   }
   bad |= __shfl_xor(bad, 32);
-  if (row < a.n && !bad) {
+  if (row < a.n && (CAREFUL ? again : !bad)) {
     const int64_t at = (head_row + row) * a.d;
-    const float f = a.scale * drop;
+    const float f = lost ? __builtin_nanf("") : a.scale * drop;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -907,46 +898,12 @@ __global__ __launch_bounds__(256, IN == F32 || (SHARE && P > 96) ? 1 : (P == 64 
                          in ? acc[mt][4 * r + 2] * f : 0.f, in ? acc[mt][4 * r + 3] * f : 0.f);
       }
   }
-  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1) {
-    const int i = __builtin_ctzll(todo);
-    win_dq_row<IN>(a, b, h, w0 + i, __shfl(delta, i));
-  }
+  return bad;
 }
 
-// dk_j and dv_j over the rows [lo, hi] of every head of the group, one wave; columns [lane, lane + 64] of both
-template <int IN>
-__device__ void win_dkv_row(const WinArgs& a, int b, int hk, int key, int lo, int hi, float (&dk)[2], float (&dv)[2]) {
-  constexpr int ES = IN == F32 ? 4 : 2;
-  const int lane = threadIdx.x & 63;
-  const void* k = rows_at<ES>(a.k, b, hk, key);
-  const void* v = rows_at<ES>(a.v, b, hk, key);
-#pragma unroll
-  for (int e = 0; e < 2; ++e) dk[e] = dv[e] = 0.f;
-  for (int g = 0; g < a.group; ++g) {
-    const int h = hk * a.group + g;
-    const int64_t head_row = (static_cast<int64_t>(b) * a.heads + h) * a.n;
-    for (int i0 = lo; i0 <= hi; i0 += 64) {
-      const int i = i0 + lane;
-      float p = 0.f, ds = 0.f;
-      if (i <= hi) {
-        const float x = a.scale * win_dot<IN>(rows_at<ES>(a.q, b, h, i), k, a.d);
-        p = exp2f(fmaf(x, 1.44269504f, -a.lse[head_row + i]));
-        ds = p * (win_dot<IN>(rows_at<ES>(a.go, b, h, i), v, a.dv) - a.delta[head_row + i]);
-      }
-      for (int u = 0; u < 64 && i0 + u <= hi; ++u) {
-        const float pu = __shfl(p, u), du = __shfl(ds, u);
-        const void* q = rows_at<ES>(a.q, b, h, i0 + u);
-        const void* go = rows_at<ES>(a.go, b, h, i0 + u);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          if (lane + 64 * e < a.d) dk[e] = fmaf(du, load_elem(q, lane + 64 * e, IN), dk[e]);
-          if (lane + 64 * e < a.dv) dv[e] = fmaf(pu, load_elem(go, lane + 64 * e, IN), dv[e]);
-        }
-      }
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) dk[e] *= a.scale;
+template <int P, int IN, bool SHARE>
+__global__ __launch_bounds__(256, (win_dq_waves<P, IN, SHARE>())) void window_dq_kernel(const WinArgs a) {
+  win_passes([&](auto second, int again) { return window_dq_pass<P, IN, SHARE, decltype(second)::value>(a, again); });
 }
 
 // Rows that window_dkv_kernel stages at a time, and its LDS: two stages of query and gradient rows and their statistics
@@ -976,8 +933,8 @@ __host__ __device__ constexpr int win_dkv_lds() {
 // 1024, 515 us (PIPE with one wave 722, with two, which spill, 714); 32 heads of 16384 over 8 key heads, window 4096, 1.36
 // ms (1.73); 32 wide 265 us (314); 96 wide the other way round: 4 x 16 heads over 4 key heads 359 us with PIPE, 411 with two waves.
 // FULL: both widths are the padded one (with PIPE).
-template <int P, int IN, bool SHARE, bool FULL>
-__global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kernel(const WinArgs a) {
+template <int P, int IN, bool SHARE, bool FULL, bool CAREFUL>
+__device__ __forceinline__ int window_dkv_pass(const WinArgs& a, int again) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), MT = P / 32, BQ = win_staged_rows<IN, SHARE>(),
                 NSUB = BQ / 32, TILE = win_rows<SHARE>(), THREADS = SHARE ? 64 : 256;
   constexpr int STAGE = 2 * BQ * CH;  // 16-byte units of a stage
@@ -1009,6 +966,8 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
   }
   if (hi > len - 1) hi = len - 1;
 
+  constexpr bool AHEAD = !SHARE || (!CAREFUL && win_ahead<P, IN, SHARE>());
+  int bad = 0;
   floatx16 dk[MT], dv[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
@@ -1056,6 +1015,11 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
     }
     const int first = lo / BQ * BQ, per_head = hi / BQ - lo / BQ + 1, count = per_head * a.group;
     const float lift = __builtin_amdgcn_logf(a.lift);
+    // does the lane's key take part in row i here
+    auto sees = [&](int i) {
+      if (far) return i - key >= a.window && i >= lo && i <= hi && key < a.sinks;
+      return static_cast<uint32_t>(i - key) < static_cast<uint32_t>(a.window);
+    };
     // hidden pairs' weights and gradients
     auto hide = [&](floatx16& x, floatx16& g, int base) {
       const int ahead = base - key, from = lo - base, last = key < a.sinks ? hi - base : -1;
@@ -1073,17 +1037,18 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
       return far ? kw >= a.sinks || q0 + rows - 1 - kw < a.window : q0 + rows - 1 < kw || q0 - (kw + 31) >= a.window;
     };
     auto whole = [&](int q0, int rows) {
-      return far ? kw + 32 <= a.sinks && q0 - (kw + 31) >= a.window && q0 >= lo && q0 + rows - 1 <= hi
-                 : q0 >= kw + 31 && q0 + rows - 1 - kw < a.window;
+      const bool behind = (kw + 32 <= a.sinks) & (q0 - (kw + 31) >= a.window) & (q0 >= lo) & (q0 + rows - 1 <= hi);
+      const bool within = (q0 >= kw + 31) & (q0 + rows - 1 - kw < a.window);
+      return far ? behind : within;
     };
-    if constexpr (PIPE) {
+    if constexpr (PIPE && !CAREFUL) {
       // One wave a SIMD has nothing else to do while it waits, so its own matrix and vector instructions are interleaved:
       // the products of the next 32 rows' logits with the weights of these, the next tiles' way into LDS with the
       // sums (the barriers of the schedule keep that order).  Three stages: tile `it` and the next are written, the third is
       // being written; one __syncthreads a tile.  Rows behind the last are read as the last one, their weights are
       // exp2(-inf).  No tile is left out for a wave that sees none of it: the others' barrier waits for it anyway.
-      constexpr int U = BQ * CH / 256, E = 16 / ES;  // 16-byte units of a tensor's tile a thread, their elements
-      static_assert(U == MT && NSUB == 2);
+      constexpr int U = MT, E = 16 / ES;  // 16-byte units of a tensor's tile a thread, their elements
+      static_assert(!PIPE || (U == BQ * CH / 256 && NSUB == 2));
       uint4 uq[U], ug[U];
       uint32_t to[U], off[2][U];
       const int pitch_q = static_cast<int>(a.q.sn) * ES, pitch_g = static_cast<int>(a.go.sn) * ES;
@@ -1239,7 +1204,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
             __builtin_amdgcn_sched_barrier(0);
           }
           asm volatile("" : "+v"(x0), "+v"(g0));
-          if (!whole(q0 + 32 * sub, 32)) hide(x0, g0, q0 + 32 * sub + 4 * hh);
+          if (__builtin_expect(!whole(q0 + 32 * sub, 32), 0)) hide(x0, g0, q0 + 32 * sub + 4 * hh);
           fit(g0);
           WinFrag<IN> p[2], ds[2];
           p[0] = win_operand<IN>(x0, 0);
@@ -1297,7 +1262,6 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
         if (self < 2 * BQ) stats[stage * 2 * BQ + self] = stat;
       };
       const int start = SHARE ? wave : 0, step = SHARE ? 4 : 1;
-      constexpr bool AHEAD = win_ahead<P, IN, SHARE>();
       if (AHEAD && start < count) load(start);
       if constexpr (!SHARE) {
         put(0, 0);
@@ -1330,7 +1294,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
         for (int sub = 0; sub < NSUB; ++sub) {
           // one wave a SIMD: every operand is read well before its product, there is nothing else to do while it waits (fp32
           // products take eight times as long as their operands' reads: those are read as they come)
-          constexpr bool EARLY = IN != F32 && WAVES == 1;
+          constexpr bool EARLY = IN != F32 && WAVES == 1 && !CAREFUL;
           WinFrag<IN> qa[EARLY ? P / 16 : 1], ga[EARLY ? P / 16 : 1], qc[MT], gc[MT];
           floatx16 x, g;
 #pragma unroll
@@ -1374,6 +1338,14 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
           }
           if (!all) hide(x, g, q0 + 32 * sub + 4 * hh);
           fit(g);
+          if (CAREFUL && !all) {
+            uint32_t pairs = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pairs |= static_cast<uint32_t>(sees(q0 + 32 * sub + 4 * hh + 8 * (i >> 2) + (i & 3))) << i;
+            win_add_seen<P, IN>(dv, x, pairs, gs, 32 * sub, lane);
+            win_add_seen<P, IN>(dk, g, pairs, qs, 32 * sub, lane);
+            continue;
+          }
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             const WinFrag<IN> p = win_operand<IN>(x, t), ds = win_operand<IN>(g, t);
@@ -1434,43 +1406,10 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
       win_store4<IN>(value ? a.dv_out : a.dk, (static_cast<int64_t>(bh) * a.n + j) * width, col, width, x0, x1, x2, x3);
     }
   };
-  // key j over its visible rows again, by a wave
-  auto again = [&](int j) {
-    float sk[2], sv[2];
-    int from = lo, to = hi;
-    if (far) {
-      if (j >= a.sinks) return;
-      if (from < j + a.window) from = j + a.window;
-    } else {
-      from = j;
-      if (j < a.n - a.window && to > j + a.window - 1) to = j + a.window - 1;
-    }
-    win_dkv_row<IN>(a, b, hk, j, from, to, sk, sv);
-    const bool pj = is_part(j);
-    const int64_t pr = part_at(j);
-    const int64_t orow = static_cast<int64_t>(bh) * a.n + j;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int col = lane + 64 * e;
-      if (col < a.d) {
-        if (pj)
-          a.part[pr + col] = sk[e];
-        else
-          store_elem(a.dk, orow * a.d + col, IN, sk[e]);
-      }
-      if (col < a.dv) {
-        if (pj)
-          a.part[pr + a.d + col] = sv[e];
-        else
-          store_elem(a.dv_out, orow * a.dv + col, IN, sv[e]);
-      }
-    }
-    };
   if constexpr (SHARE) {
     float *red = reinterpret_cast<float*>(win_lds), *red_f = red + win_join_floats<P>();
     const int j = k0 + threadIdx.x / 8;
     floatx4 o[2][MT];
-    int bad = 0;
 #pragma unroll
     for (int value = 0; value < 2; ++value) {
       __syncthreads();
@@ -1491,7 +1430,7 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
     bad = j < len ? bad : 0;
 #pragma unroll
     for (int x = 1; x < 8; x <<= 1) bad |= __shfl_xor(bad, x);
-    if (!bad) {
+    if (CAREFUL ? again : !bad) {
 #pragma unroll
       for (int value = 0; value < 2; ++value)
 #pragma unroll
@@ -1500,18 +1439,16 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
           store4(j, value, 32 * mt + 4 * (threadIdx.x & 7), y[0], y[1], y[2], y[3]);
         }
     }
-    for (uint64_t todo = __ballot(bad) & 0x0101010101010101ull; todo; todo &= todo - 1)
-      again(k0 + 8 * wave + __builtin_ctzll(todo) / 8);
-    return;
+    return bad;
   }
-  int bad = 0;
+
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) bad |= !(win_finite(dk[mt][i]) && win_finite(dv[mt][i]));
   bad = key < len ? bad : 0;
   bad |= __shfl_xor(bad, 32);
-  if (!bad) {
+  if (CAREFUL ? again : !bad) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -1522,7 +1459,12 @@ __global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kern
                dv[mt][4 * r + 3] * a.drop);
       }
   }
-  for (uint64_t todo = __ballot(bad) & 0xffffffffull; todo; todo &= todo - 1) again(kw + __builtin_ctzll(todo));
+  return bad;
+}
+
+template <int P, int IN, bool SHARE, bool FULL>
+__global__ __launch_bounds__(256, (win_dkv_waves<P, IN>())) void window_dkv_kernel(const WinArgs a) {
+  win_passes([&](auto second, int again) { return window_dkv_pass<P, IN, SHARE, FULL, decltype(second)::value>(a, again); });
 }
 
 // dk and dv of the sinks: their tile's sums and the far chunks', in order.  One thread a column.
