@@ -34,6 +34,9 @@ struct RotArgs {
   float* part[2];       // backward: sums of dw [segs gridDim.x][d]
 };
 
+// 2^-70: the squares of 256 of fp32's largest values times it stay in fp32
+constexpr float ROT_SMALL = 8.470329472543003e-22f;
+
 __device__ __forceinline__ int64_t rot_position(const RotArgs& a, int b, int n) {
   if (!a.positions) return n;
   const int64_t at = b * a.pos_sb + n * a.pos_sn;
@@ -123,7 +126,17 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(const RotArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
       for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-      const float inv = 1.f / sqrtf(fmaf(ss, a.inv_d, a.eps));
+      float inv = 1.f / sqrtf(fmaf(ss, a.inv_d, a.eps));
+      if (!(ss < __builtin_inff())) {  // squares past fp32: of the row times a power of two
+        ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float ya = xa[e] * ROT_SMALL, yb = xb[e] * ROT_SMALL;
+          ss = fmaf(ya, ya, fmaf(yb, yb, ss));
+        }
+        for (int o = a.lanes >> 1; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+        inv = ROT_SMALL / sqrtf(fmaf(ss, a.inv_d, a.eps * ROT_SMALL * ROT_SMALL));
+      }
       float ya[E], yb[E];
       auto turn = [&](const float (&fa)[E], const float (&fb)[E], float sign) {
         if constexpr (INTER) {
@@ -244,7 +257,14 @@ __global__ __launch_bounds__(256) void head_rotary_any_kernel(const RotArgs a) {
         ss = fmaf(x[k], x[k], ss);
       }
       for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-      const float inv = 1.f / sqrtf(fmaf(ss, a.inv_d, a.eps));
+      float inv = 1.f / sqrtf(fmaf(ss, a.inv_d, a.eps));
+      if (!(ss < __builtin_inff())) {
+        ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < C; ++k) ss = fmaf(x[k] * ROT_SMALL, x[k] * ROT_SMALL, ss);
+        for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+        inv = ROT_SMALL / sqrtf(fmaf(ss, a.inv_d, a.eps * ROT_SMALL * ROT_SMALL));
+      }
       if constexpr (!BACK) {
 #pragma unroll
         for (int k = 0; k < C; ++k)
