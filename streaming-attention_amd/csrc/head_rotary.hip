@@ -138,21 +138,23 @@ __global__ __launch_bounds__(256) void head_rotary_kernel(const RotArgs a) {
         inv = ROT_SMALL / sqrtf(fmaf(ss, a.inv_d, a.eps * ROT_SMALL * ROT_SMALL));
       }
       float ya[E], yb[E];
+      // (a column that does not turn takes nothing of its neighbour, not even 0 times an infinity)
       auto turn = [&](const float (&fa)[E], const float (&fb)[E], float sign) {
         if constexpr (INTER) {
 #pragma unroll
           for (int i = 0; i < E / 2; ++i) {
             const float sa = sign * s[i], sb = sign * s[E / 2 + i];
-            ya[2 * i] = fa[2 * i] * c[i] - fa[2 * i + 1] * sa;
-            ya[2 * i + 1] = fa[2 * i + 1] * c[i] + fa[2 * i] * sa;
-            yb[2 * i] = fb[2 * i] * c[E / 2 + i] - fb[2 * i + 1] * sb;
-            yb[2 * i + 1] = fb[2 * i + 1] * c[E / 2 + i] + fb[2 * i] * sb;
+            const bool ta = ca / 2 + i < pairs, tb = cb / 2 + i < pairs;
+            ya[2 * i] = fa[2 * i] * c[i] - (ta ? fa[2 * i + 1] * sa : 0.f);
+            ya[2 * i + 1] = fa[2 * i + 1] * c[i] + (ta ? fa[2 * i] * sa : 0.f);
+            yb[2 * i] = fb[2 * i] * c[E / 2 + i] - (tb ? fb[2 * i + 1] * sb : 0.f);
+            yb[2 * i + 1] = fb[2 * i + 1] * c[E / 2 + i] + (tb ? fb[2 * i] * sb : 0.f);
           }
         } else {
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            ya[e] = fa[e] * c[e] - fb[e] * (sign * s[e]);
-            yb[e] = fb[e] * c[e] + fa[e] * (sign * s[e]);
+            ya[e] = fa[e] * c[e] - (u < turning ? fb[e] * (sign * s[e]) : 0.f);
+            yb[e] = fb[e] * c[e] + (u < turning ? fa[e] * (sign * s[e]) : 0.f);
           }
         }
       };
