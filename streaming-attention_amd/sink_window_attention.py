@@ -208,6 +208,8 @@ def _refuse_capture() -> None:
 
 def _refuse_tangents(*tensors: Optional[Tensor]) -> None:
     """The operators have no forward-mode derivative; a result without one would be taken for a constant."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no tangents anywhere (five tensors' looks take 0.7 us)
+        return
     for x in tensors:
         if x is not None and forward_ad.unpack_dual(x).tangent is not None:
             raise RuntimeError("forward-mode derivatives are not supported: use the backward pass")
