@@ -13,7 +13,7 @@ namespace sta_api {
 template <typename Kernel>
 static int launch(Kernel kernel, int64_t grid, int lds, const sta::WinArgs& a, hipStream_t s) {
   if (grid <= 0 || grid > sta::MAX_GROUPS) return STA_ERR_SHAPE;
-  if (lds > 64 * 1024) {
+  if (lds > 64 * 1024 - 16) {  // with the kernels' own few bytes past 64 KB
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                              hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return hip_status(e);
