@@ -226,8 +226,8 @@ __device__ __forceinline__ WinFrag<IN> win_read_columns(const uint4* lds, int r0
 
 // acc += weights times values of 32 staged rows from r0 (a multiple of 32), over the seen pairs alone: bit i of a lane's `seen`
 // stands for its element i, whose row win_mma's layout gives.  By vector instructions, row after row, which only results that
-// are not finite ask for: backward, bf16, one NaN in the gradient of 32 heads of 16384 x 128, window 4096, 11 ms (4.2 without it; 900
-// with rows and keys taken alone by a wave each), a gradient that is NaN throughout of 8 x 16 heads of 4096 x 64, window 1024, 2.8
+// are not finite ask for: backward, bf16, one NaN in the gradient of 32 heads of 16384 x 128, window 4096, 10 ms (4.2 without it; 900
+// with rows and keys taken alone by a wave each), a gradient that is NaN throughout of 8 x 16 heads of 4096 x 64, window 1024, 2.5
 // ms (0.87; 344).
 template <int P, int IN>
 __device__ __forceinline__ void win_add_seen(floatx16 (&acc)[P / 32], const floatx16& weights, uint32_t seen, const uint4* lds,
@@ -251,10 +251,9 @@ __device__ __forceinline__ void win_add_seen(floatx16 (&acc)[P / 32], const floa
           const uint4* unit = lds + r * CH + ((col / E) ^ win_swizzle<CH>(r));
           __builtin_memcpy(v[c], __builtin_assume_aligned(reinterpret_cast<const char*>(unit) + col % E * ES, 4 * ES), 4 * ES);
         }
+        if (in) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float x = load_elem(v[e >> 2], e & 3, IN);
-          acc[mt][e] = in ? fmaf(p, x, acc[mt][e]) : acc[mt][e];
+          for (int e = 0; e < 16; ++e) acc[mt][e] = fmaf(p, load_elem(v[e >> 2], e & 3, IN), acc[mt][e]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -478,7 +477,7 @@ __host__ __device__ constexpr float win_weight_lift() { return IN == F16 ? 11.f 
 // Row tiles: keys staged win_keys at a time, the next tile's rows in registers while this one computes, softmax in one
 // pass.  The weights of 16-bit rows enter the second product rounded to their type (half a step each, errors that
 // average over the keys and end below the output's own rounding); their sum is taken before that, in fp32.
-// Measured, bf16: 32 heads of 16384 rows, 128 wide, window 4096: 1.04 ms, 925 TFLOP/s, bound by the products (a large
+// Measured, bf16: 32 heads of 16384 rows, 128 wide, window 4096: 1.10 ms, 880 TFLOP/s, bound by the products (a large
 // matrix product reaches 1180).  8 x 16 heads of 4096 rows, 64 wide, window 1024: 0.20 ms, 600 TFLOP/s, bound by the vector
 // unit: a tile of 64 keys takes 16 products (512 cycles of the matrix unit) but 32 exponentials, a quarter of the rate,
 // and about 150 other instructions (1100 cycles); 4 waves a SIMD instead of 3 change nothing.
@@ -702,7 +701,7 @@ __global__ __launch_bounds__(256, (win_row_waves<P, IN, SHARE>())) void window_f
 // o), the same for all keys of a row, which adds about a tenth to the gradients' rounding errors (a third with windows of 16
 // keys); with what the rounding left (rest) it is not.  ds is rounded to the rows' type for
 // its product with the keys like the weights of the forward kernel.  32 heads of 16384 rows, 128 wide, window 4096,
-// bf16: 1.45 ms, three products at 995 TFLOP/s, bound by them; 8 x 16 heads of 4096 rows, 64 wide, window 1024: 291 us with
+// bf16: 1.48 ms, three products at 975 TFLOP/s, bound by them; 8 x 16 heads of 4096 rows, 64 wide, window 1024: 291 us with
 // three waves a SIMD (one register less a lane than the compiler takes by itself), 316 with two.
 template <int P, int IN, bool SHARE, bool CAREFUL>
 __device__ __forceinline__ int window_dq_pass(const WinArgs& a, int again) {
@@ -925,9 +924,9 @@ __host__ __device__ constexpr int win_dkv_lds() {
 // dk and dv of 32 keys of 128 columns take 128 registers a lane and the keys' operands 64, so a compute unit holds one wave
 // a SIMD above 64 columns.  PIPE (16-bit rows): that wave's instructions are laid out by hand, see below; without it (SHARE) the
 // operands are at least read ahead.  32 heads of 16384 rows over 8 key heads, 128 wide,
-// window 4096, bf16: 2.37 ms, four products at 810 TFLOP/s (3.03 ms without PIPE; 93 wide, 4 x 16 heads of 4096 rows, window
-// 1024, with dq 841 us, 923 without; operands read two steps ahead 2.48, three
-// 2.37, four 2.33; dk and dv in kernels of their own, 5 products but two waves a SIMD, 3.45).  What is left: about 300
+// window 4096, bf16: 2.44 ms, four products at 790 TFLOP/s (before it had a second pass 2.37, and 3.03 without PIPE; operands
+// read two steps ahead 2.48, three 2.37, four 2.33; dk and dv in kernels of their own, 5 products but two waves a SIMD, 3.45; 93
+// wide, 4 x 16 heads of 4096 rows, window 1024, with dq 841 us, 923 without PIPE).  What is left: about 300
 // instructions a wave issues for 32 rows, one at a time, against 1024 cycles of the matrix unit.
 // Up to 64 columns two waves a SIMD fill each other's waits better than PIPE does: 8 x 16 heads of 4096 rows, 64 wide, window
 // 1024, 515 us (PIPE with one wave 722, with two, which spill, 714); 32 heads of 16384 over 8 key heads, window 4096, 1.36
