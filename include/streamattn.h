@@ -572,6 +572,102 @@ int sta_ring_items(int dtype, int storage, int64_t streams, int kv_heads, int d,
                    const void* value_exponents, const int32_t* counts, void* keys_out, void* values_out,
                    int32_t* positions, void* stream);
 
+/*
+ * Attention of the newest rows of a batch over a prefix that its sequences share and over each one's own tokens.
+ * Sequence b has lengths[b] own tokens (NULL: m; values outside 0 .. m are taken as the nearest of them), and its last
+ * counts[b] of them (NULL: n; at most lengths[b]) have their queries in rows 0 .. counts[b] - 1 of q.  Row i sees the
+ * prefix whole and the own tokens up to its own, lengths[b] - counts[b] + i.
+ *   q [batch][heads][n][d], k [batch][kv_heads][m][d], v [..][dv], prefix_k [sets][kv_heads][p][d], prefix_v [..][dv]:
+ *   sequence b reads prefix b / (batch / sets) (batch a multiple of sets), of which the first prefix_lengths[set] rows
+ *   (NULL: p) count; p may be 0.  strides [5][3] (host memory): element strides of batch (set), head and row of q, k, v,
+ *   prefix_k and prefix_v; the last dimension is contiguous, rows at most 2^24 bytes apart, no alignment beyond the
+ *   element's.  d, dv at most 128, rows of at least 16 bytes, n, m, p <= 2^30.
+ *   out [batch][heads][n][dv] dense, 16-byte aligned; lse [batch][heads][n] fp32 or NULL: log2 of a row's sum of weights;
+ *   rows behind counts are 0 in both.  Products of 16-bit inputs are exact, sums and statistics fp32, weights of 16-bit rows
+ *   rounded to 16 bits for the value sums.  A value that is infinite or NaN reaches the rows that see it and no others.
+ *   workspace: caller-allocated, 16-byte aligned, of sta_prefix_attention_bytes (-1: arguments it refuses).
+ */
+int64_t sta_prefix_attention_bytes(int dtype, int64_t batch, int heads, int kv_heads, int64_t sets, int64_t n, int64_t m,
+                                   int64_t p, int d, int dv);
+int sta_prefix_attention(const void* q, const void* k, const void* v, const void* prefix_k, const void* prefix_v, int dtype,
+                         int64_t batch, int heads, int kv_heads, int64_t sets, int64_t n, int64_t m, int64_t p, int d,
+                         int dv, const int64_t* strides, float scale, const int32_t* lengths, const int32_t* counts,
+                         const int32_t* prefix_lengths, void* out, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
+ * The attention weights that own tokens receive: weights [batch][kv_heads][m] fp32, the sum over the rows that see a
+ * token and the query heads of its key head of exp2(log2(e) scale q.k - lse); 0 behind lengths.  q, k, lengths, counts and
+ * the rows' view as sta_prefix_attention (strides [2][3]); lse [batch][heads][n] as it gives them (with a prefix: its share
+ * is missing from the weights), or NULL: computed here, over the own tokens.  A row whose lse is infinite or NaN makes the
+ * weights of the tokens that it sees NaN.  Sums in a fixed order.
+ */
+int64_t sta_received_attention_bytes(int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int64_t m, int d,
+                                     int with_lse);
+int sta_received_attention(const void* q, const void* k, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
+                           int64_t m, int d, const int64_t* strides, float scale, const int32_t* lengths,
+                           const int32_t* counts, const float* lse, float* weights, void* workspace,
+                           int64_t workspace_bytes, void* stream);
+
+/*
+ * Token cache that keeps the most attended tokens, for streams in lockstep: per stream and key head the last `recent`
+ * tokens, token p in slot p % (recent + 1), and in `kept` slots behind them older ones.  Token n sends token n - recent out
+ * of the ring: into the next kept slot while there is one, else into the kept slot of the lowest weight (of equal ones the
+ * first) unless its own is lower.
+ *   keys, values: caller-owned device buffers of sta_heavy_layout's sizes [0] and [1] bytes, 16-byte aligned, zeroed before
+ *   their first use; their layout is the library's own (equal for equal arguments, so that they can be saved and loaded).
+ *   counts int64 [streams][kv_heads]: tokens so far (at first 0); weights fp32 and positions int64 [streams][kv_heads][pitch],
+ *   pitch = sizes[2]: the slots' weights and tokens (0 and -1 where none is, and behind the slots); lowest [..][2]: the lowest
+ *   kept weight and its slot, the library's own form (at first all bits set).  weights and positions 16-byte aligned.
+ *   dtype: that of the cache and of all rows.  d, dv <= 128, recent, kept >= 1, recent + kept <= 2^30, at most 512 query
+ *   heads of a key head.
+ */
+int sta_heavy_layout(int dtype, int64_t streams, int kv_heads, int d, int dv, int64_t recent, int64_t kept,
+                     int64_t* sizes);
+
+/* Bytes of sta_heavy_attention's workspace; -1 for arguments it refuses.  sets, p: of the prefix (p 0: none). */
+int64_t sta_heavy_attention_bytes(int dtype, int64_t streams, int heads, int kv_heads, int d, int dv, int64_t recent,
+                                  int64_t kept, int64_t sets, int64_t p);
+
+/*
+ * out [streams][heads][dv] (dense) = softmax attention of q [streams][heads][d] over the tokens held, after the new tokens k
+ * [streams][kv_heads][d], v [..][dv] went in (both NULL: no new token), and over a prefix that the streams of a set share;
+ * nothing to see gives 0.  Each token's weight grows by the softmax weights that it gets from the query heads of its key
+ * head (increments that are not finite are left out).  strides [3][2] (host memory): element strides of stream and head
+ * of q, k and v.  prefix_k [sets][kv_heads][p][d], prefix_v [..][dv], prefix_strides [2][3], prefix_lengths: as
+ * sta_prefix_attention (rows of at least 16 bytes then), p 0: none.  workspace: caller-allocated, 16-byte aligned, of
+ * sta_heavy_attention_bytes (contents undefined before and after).
+ */
+int sta_heavy_attention(const void* q, const void* k, const void* v, int dtype, int64_t streams, int heads, int kv_heads,
+                        int d, int dv, const int64_t* strides, float scale, int64_t recent, int64_t kept,
+                        const void* prefix_k, const void* prefix_v, int64_t sets, int64_t p,
+                        const int64_t* prefix_strides, const int32_t* prefix_lengths, void* keys, void* values,
+                        int64_t* counts, float* weights, int64_t* positions, uint64_t* lowest, void* out,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* One token k [streams][kv_heads][d], v [..][dv] of every stream into the cache (strides [2][2]). */
+int sta_heavy_update(const void* k, const void* v, int dtype, int64_t streams, int kv_heads, int d, int dv,
+                     const int64_t* strides, int64_t recent, int64_t kept, void* keys, void* values, int64_t* counts,
+                     float* weights, int64_t* positions, uint64_t* lowest, void* stream);
+
+/*
+ * Streams begin anew from prompts k [streams][kv_heads][rows][d], v [..][dv] (strides [2][3]: stream, head, row) whose tokens
+ * have the weights given [streams][kv_heads][rows] (dense; NaN counts as 0): the last `recent` of the first take[stream]
+ * (device; NULL: rows) rows, and of the others the `kept` of the largest weights, of equal ones the first, in their
+ * order.  A stream whose take is 0 or less keeps what it holds.  workspace: sta_heavy_start_bytes, 16-byte aligned.
+ */
+int64_t sta_heavy_start_bytes(int64_t streams, int kv_heads, int64_t recent, int64_t kept);
+int sta_heavy_start(const void* k, const void* v, const float* given, int dtype, int64_t streams, int kv_heads, int64_t rows,
+                    int d, int dv, const int64_t* strides, int64_t recent, int64_t kept, const int32_t* take, void* keys,
+                    void* values, int64_t* counts, float* weights, int64_t* positions, uint64_t* lowest,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The slots' rows: keys_out [streams][kv_heads][recent + 1 + kept][d], values_out [..][dv] (16-byte aligned; zero where no
+ * token is). */
+int sta_heavy_items(int dtype, int64_t streams, int kv_heads, int d, int dv, int64_t recent, int64_t kept,
+                    const void* keys, const void* values, const int64_t* positions, void* keys_out, void* values_out,
+                    void* stream);
+
 /* Rows per block-attention tile and the moment chunk the library uses for a head dimension D (the
  * chunk argument of sta_block_attention is that chunk for sta_moments' partials, the query block for
  * sta_moments_ws' partials). */

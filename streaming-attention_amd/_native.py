@@ -185,6 +185,31 @@ _SIGNATURES = {
     "sta_ring_items": (
         _i32, [_i32, _i32, _i64, _i32, _i32, _i32, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
     ),
+    "sta_prefix_attention_bytes": (_i64, [_i32, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32]),
+    "sta_prefix_attention": (
+        _i32, [_c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i64, _i64, _i64, _i32, _i32, _c_p, _f32, _c_p,
+               _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # q k v pk pv type B H Hk sets n m p d dv strides .. ws bytes stream
+    ),
+    "sta_received_attention_bytes": (_i64, [_i32, _i64, _i32, _i32, _i64, _i64, _i32, _i32]),
+    "sta_received_attention": (
+        _i32, [_c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i64, _i32, _c_p, _f32, _c_p, _c_p, _c_p, _c_p, _c_p, _i64,
+               _c_p],  # q k type B H Hk n m d strides scale lengths counts lse weights ws bytes stream
+    ),
+    "sta_heavy_layout": (_i32, [_i32, _i64, _i32, _i32, _i32, _i64, _i64, _c_p]),
+    "sta_heavy_attention_bytes": (_i64, [_i32, _i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _i64]),
+    "sta_heavy_attention": (
+        _i32, [_c_p, _c_p, _c_p, _i32, _i64, _i32, _i32, _i32, _i32, _c_p, _f32, _i64, _i64, _c_p, _c_p, _i64, _i64, _c_p,
+               _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _i64, _c_p],  # q k v .. prefix .. state out ws bytes stream
+    ),
+    "sta_heavy_update": (
+        _i32, [_c_p, _c_p, _i32, _i64, _i32, _i32, _i32, _c_p, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "sta_heavy_start_bytes": (_i64, [_i64, _i32, _i64, _i64]),
+    "sta_heavy_start": (
+        _i32, [_c_p, _c_p, _c_p, _i32, _i64, _i32, _i64, _i32, _i32, _c_p, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
+               _c_p, _c_p, _i64, _c_p],  # k v weights type S Hk rows d dv strides recent kept take state ws bytes stream
+    ),
+    "sta_heavy_items": (_i32, [_i32, _i64, _i32, _i32, _i32, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
     "sta_head_rotary": (
         _i32, [_c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _c_p, _c_p, _c_p, _i32, _c_p, _i64, _i32, _i32, _c_p,
                _i32, _i64, _i64, _f32, _c_p, _c_p, _c_p],  # .. weights type table limit rotary inter pos .. eps out out

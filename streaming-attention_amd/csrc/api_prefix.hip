@@ -1,0 +1,144 @@
+// Entry points of the attention over a shared prefix and of the received weights (see include/streamattn.h): argument
+// checks, plans, launches.
+#include "prefix_plan.hpp"
+
+using namespace sta_api;
+
+namespace {
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <int IN>
+void join(const sta::PrefixArgs& a, dim3 grid, hipStream_t s) {
+  hipLaunchKernelGGL((sta::prefix_join_kernel<IN>), grid, dim3(128), 0, s, a);
+}
+
+// The partials of every row; a row is a workgroup, in rows of 2^20 of them.
+int join_rows(const sta::PrefixArgs& a, int dtype, hipStream_t s) {
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.n, x = rows < 1 << 20 ? rows : 1 << 20;
+  const int64_t y = ceil_div(rows, x);
+  if (y > 65535) return STA_ERR_SHAPE;
+  const dim3 g(static_cast<unsigned>(x), static_cast<unsigned>(y));
+  if (dtype == STA_F32) join<sta::F32>(a, g, s);
+  else if (dtype == STA_BF16) join<sta::BF16>(a, g, s);
+  else join<sta::F16>(a, g, s);
+  return check_launch();
+}
+
+// How the received weights are dealt out: tiles of 128 keys, and workgroups that share a tile's rows where there are
+// fewer than 1024 tiles (four workgroups a compute unit).
+void plan_received(sta::ReceivedArgs& w) {
+  const sta::PrefixArgs& a = w.a;
+  w.tiles = static_cast<int>(ceil_div(a.m, sta::WIN_ROWS));
+  int64_t want = 1024 / (static_cast<int64_t>(a.batch) * a.kv * w.tiles);
+  const int64_t most = static_cast<int64_t>(a.group) * ceil_div(a.n, 64);
+  if (want > most) want = most;
+  w.nsplit = static_cast<int>(want < 1 ? 1 : want);
+}
+
+int64_t received_sum_bytes(const sta::ReceivedArgs& w) {
+  return w.nsplit == 1 ? 0 : 4 * ceil_div(static_cast<int64_t>(w.nsplit) * w.a.batch * w.a.kv * w.a.m, 4) * 4;
+}
+int64_t received_lse_bytes(const sta::PrefixArgs& a) {
+  return 4 * ceil_div(static_cast<int64_t>(a.batch) * a.heads * a.n, 4) * 4;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t sta_prefix_attention_bytes(int dtype, int64_t batch, int heads, int kv_heads, int64_t sets, int64_t n, int64_t m,
+                                   int64_t p, int d, int dv) {
+  sta::PrefixArgs a;
+  if (prefix_shape(a, dtype, batch, heads, kv_heads, sets, n, m, p, d, dv, 1.f) != STA_OK || m < 1 || dv < 1) return -1;
+  return prefix_part_bytes(a, plan_prefix(a, true).parts);
+}
+
+int sta_prefix_attention(const void* q, const void* k, const void* v, const void* prefix_k, const void* prefix_v, int dtype,
+                         int64_t batch, int heads, int kv_heads, int64_t sets, int64_t n, int64_t m, int64_t p, int d,
+                         int dv, const int64_t* strides, float scale, const int32_t* lengths, const int32_t* counts,
+                         const int32_t* prefix_lengths, void* out, float* lse, void* workspace,
+                         int64_t workspace_bytes, void* stream) {
+  if (!q || !k || !v || !out || !strides || (p > 0 && (!prefix_k || !prefix_v))) return STA_ERR_ARG;
+  sta::PrefixArgs a;
+  if (const int st = prefix_shape(a, dtype, batch, heads, kv_heads, sets, n, m, p, d, dv, scale)) return st;
+  if (m < 1 || dv < 1) return STA_ERR_SHAPE;
+  if (!aligned16(out)) return STA_ERR_ARG;
+  if (!prefix_strides_ok(strides, p > 0 ? 5 : 3, dtype)) return STA_ERR_UNSUPPORTED;
+  const PrefixPlan plan = plan_prefix(a, true);
+  const int64_t need = prefix_part_bytes(a, plan.parts);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return STA_ERR_SCRATCH;
+  a.q = prefix_rows_of(q, strides);
+  a.k = prefix_rows_of(k, strides + 3);
+  a.v = prefix_rows_of(v, strides + 6);
+  if (p > 0) {
+    a.pk = prefix_rows_of(prefix_k, strides + 9);
+    a.pv = prefix_rows_of(prefix_v, strides + 12);
+  }
+  a.lengths = lengths;
+  a.counts = counts;
+  a.prefix_lengths = prefix_lengths;
+  a.out = out;
+  a.lse = lse;
+  a.part = static_cast<float*>(workspace);
+  a.parts = plan.parts;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int st = run_prefix(a, plan, dtype, 1, s);
+  return st == STA_OK && plan.parts ? join_rows(a, dtype, s) : st;
+}
+
+int64_t sta_received_attention_bytes(int dtype, int64_t batch, int heads, int kv_heads, int64_t n, int64_t m, int d,
+                                     int with_lse) {
+  sta::ReceivedArgs w{};
+  if (prefix_shape(w.a, dtype, batch, heads, kv_heads, batch, n, m, 0, d, 0, 1.f) != STA_OK || m < 1) return -1;
+  plan_received(w);
+  int64_t bytes = received_sum_bytes(w);
+  if (!with_lse) bytes += received_lse_bytes(w.a) + prefix_part_bytes(w.a, plan_prefix(w.a, true).parts);
+  return bytes;
+}
+
+int sta_received_attention(const void* q, const void* k, int dtype, int64_t batch, int heads, int kv_heads, int64_t n,
+                           int64_t m, int d, const int64_t* strides, float scale, const int32_t* lengths,
+                           const int32_t* counts, const float* lse, float* weights, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
+  if (!q || !k || !weights || !strides) return STA_ERR_ARG;
+  sta::ReceivedArgs w{};
+  sta::PrefixArgs& a = w.a;
+  if (const int st = prefix_shape(a, dtype, batch, heads, kv_heads, batch, n, m, 0, d, 0, scale)) return st;
+  if (m < 1) return STA_ERR_SHAPE;
+  if (!prefix_strides_ok(strides, 2, dtype)) return STA_ERR_UNSUPPORTED;
+  const int64_t need = sta_received_attention_bytes(dtype, batch, heads, kv_heads, n, m, d, lse != nullptr);
+  if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return STA_ERR_SCRATCH;
+  a.q = prefix_rows_of(q, strides);
+  a.k = prefix_rows_of(k, strides + 3);
+  a.lengths = lengths;
+  a.counts = counts;
+  plan_received(w);
+  char* room = static_cast<char*>(workspace);
+  w.sums = reinterpret_cast<float*>(room);
+  room += received_sum_bytes(w);
+  w.weights = weights;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (lse) {
+    a.lse = const_cast<float*>(lse);
+  } else {
+    a.lse = reinterpret_cast<float*>(room);
+    room += received_lse_bytes(a);
+    const PrefixPlan plan = plan_prefix(a, true);
+    a.part = reinterpret_cast<float*>(room);
+    a.parts = plan.parts;
+    int st = run_prefix(a, plan, dtype, 0, s);
+    if (st == STA_OK && plan.parts) st = join_rows(a, dtype, s);
+    if (st != STA_OK) return st;
+  }
+  const int st = prefix_by_type(dtype, d, [&](auto width, auto in) {
+    return launch_received<decltype(width)::value, decltype(in)::value>(w, s);
+  });
+  if (st != STA_OK || w.nsplit == 1) return st;
+  const int64_t groups = ceil_div(static_cast<int64_t>(a.batch) * a.kv * a.m, 256);
+  if (groups > sta::MAX_GROUPS) return STA_ERR_SHAPE;
+  hipLaunchKernelGGL(sta::received_join_kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, w);
+  return check_launch();
+}
+
+}  // extern "C"

@@ -1,0 +1,639 @@
+// The cache that keeps the most attended tokens, and the single-token attention over it.
+//
+// A (stream, key head) holds the last `recent` tokens in a ring of recent + 1 slots, token p in slot p % (recent + 1), and
+// in `kept` slots behind them older ones, each slot with its position and its weight W, the attention weights that the
+// token has received.  Token n of a stream sends token n - recent out of the ring: into the next kept slot while there
+// is one, else into the kept slot of the lowest W (of equal ones the first) unless its own W is lower.  The ring's one
+// slot more than it holds lets the token that leaves be read from its slot while the new one is written: the slot is
+// empty from then on until the next token takes it.
+//   p_hj = exp(s q_h.k_j - L_h), L_h = log of the sum over the tokens held (and the rows of a shared prefix),
+//   o_h = sum_j p_hj v_j,   W_j += sum over the query heads of the key head of p_hj
+// Increments that are not finite are left out, so that a token held with an infinity or NaN does not make its
+// neighbours' weights NaN, and itself leaves in the end.
+//
+// Keys and values lie as in the token cache of windowed attention (ring_cache.hip).  The slot of the lowest W is part of
+// the state: whoever changes weights looks for it, in the pass that it makes over them anyway, so that a step knows it
+// without one.  Two entries take turns (by the parity of the count that they are for), since workgroups of a step that
+// read one may run beside another that clears the other.
+#include "prefix_attn.hip"
+#include "ring_cache.hip"
+
+namespace sta {
+
+struct HeavyArgs {
+  RingArgs r;            // q, new tokens, sizes, cache, part, out; counts unused
+  int recent, kept, ring, pitch;  // ring = recent + 1; pitch: slots of a row of weights and positions, whole tiles
+  int64_t* counts;       // [streams][kv]: tokens so far
+  float* weights;        // [streams][kv][pitch]
+  int64_t* positions;    // [streams][kv][pitch], -1: no token
+  unsigned long long* lowest;  // [streams][kv][2]: order of the lowest weight of the kept slots, and the slot
+  float* logits;         // [streams][heads][pitch]: this step's, times nothing
+  struct HeavyMove* moves;  // [streams][kv], of steps that several workgroups share
+  const float* prefix;   // [streams][heads][prefix_parts][dv + 2]: a shared prefix's partials
+  int prefix_parts;
+  int alone;             // a workgroup has a key head to itself and finishes it: one split, up to 16 query heads, no prefix
+};
+
+// What a step does to the slots of a key head.
+struct HeavyMove {
+  int64_t n;             // tokens before it
+  int from, to;          // the slot that a token leaves (-1: none), the kept slot that it takes (-1: it is forgotten)
+  int slot;              // of the new token (-1: none comes)
+  int hole;              // the empty slot of a full ring (-1: none)
+  int held;              // slots [0, held) but the hole hold a token
+  float weight;          // of the token that leaves its slot
+};
+
+// weights in the order of unsigned numbers (none is NaN)
+__device__ __forceinline__ uint32_t heavy_order(float w) {
+  const uint32_t u = __float_as_uint(w);
+  return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ unsigned long long heavy_key(float w, int slot) {
+  return static_cast<unsigned long long>(heavy_order(w)) << 32 | static_cast<uint32_t>(slot);
+}
+constexpr unsigned long long HEAVY_NONE = ~0ull;
+
+__device__ __forceinline__ unsigned long long heavy_min(unsigned long long a, unsigned long long b) { return a < b ? a : b; }
+// the least of a workgroup's keys, for every thread (a barrier before red is used again is the caller's)
+template <int THREADS>
+__device__ __forceinline__ unsigned long long heavy_least(unsigned long long x, unsigned long long* red) {
+  for (int o = 32; o > 0; o >>= 1) {
+    const unsigned long long y = static_cast<unsigned long long>(__shfl_xor(static_cast<long long>(x), o));
+    x = heavy_min(x, y);
+  }
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  for (int i = 0; i < THREADS / 64; ++i) x = heavy_min(x, red[i]);
+  return x;
+}
+
+__device__ __forceinline__ HeavyMove heavy_move(const HeavyArgs& a, int sh, bool append) {
+  HeavyMove m;
+  const int64_t n = a.counts[sh];
+  m.n = n < 0 ? 0 : n;
+  const int64_t after = m.n + (append ? 1 : 0), gone = m.n - a.recent;
+  m.from = m.to = m.slot = m.hole = -1;
+  m.weight = 0.f;
+  if (append) {
+    m.slot = static_cast<int>(m.n % a.ring);
+    if (gone >= 0) {
+      m.from = static_cast<int>(gone % a.ring);
+      m.weight = a.weights[static_cast<int64_t>(sh) * a.pitch + m.from];
+      if (gone < a.kept) {
+        m.to = a.ring + static_cast<int>(gone);
+      } else {
+        const unsigned long long low = a.lowest[2 * static_cast<int64_t>(sh) + (m.n & 1)];
+        const int slot = static_cast<int>(low & 0xffffffffu);
+        if (heavy_order(m.weight) >= static_cast<uint32_t>(low >> 32) && slot >= a.ring && slot < a.r.slots) m.to = slot;
+      }
+    }
+  }
+  const int64_t older = after - a.recent;
+  if (older > 0) {
+    m.hole = static_cast<int>((older - 1) % a.ring);
+    m.held = a.ring + static_cast<int>(older < a.kept ? older : a.kept);
+  } else {
+    m.held = static_cast<int>(after);
+  }
+  return m;
+}
+
+// The token that leaves the ring into its kept slot, by a workgroup of at least 64 + 32 nbv threads; the caller's barrier
+// follows.  Its old slot is nobody's to write in this step.
+template <int ST>
+__device__ __forceinline__ void heavy_keep(const RingArgs& a, int sh, int from, int to) {
+  constexpr int ES = ST == F32 ? 4 : 2;
+  const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
+  const int t = threadIdx.x;
+  if (t < 4 * a.nbk) {
+    const uint8_t* x = a.keys + (tile0 + (from >> 5)) * ring_tile_bytes(a.nbk, ST) + ring_key_at(from & 31, 8 * t, a.nbk, ST);
+    uint8_t* y = a.keys + (tile0 + (to >> 5)) * ring_tile_bytes(a.nbk, ST) + ring_key_at(to & 31, 8 * t, a.nbk, ST);
+#pragma unroll
+    for (int i = 0; i < ES / 2; ++i) reinterpret_cast<uint4*>(y)[i] = reinterpret_cast<const uint4*>(x)[i];
+  } else if (t >= 64 && t < 64 + 32 * a.nbv) {
+    const uint8_t* x =
+        a.values + (tile0 + (from >> 5)) * ring_tile_bytes(a.nbv, ST) + ring_value_at(from & 31, t - 64, a.nbv, ST);
+    uint8_t* y = a.values + (tile0 + (to >> 5)) * ring_tile_bytes(a.nbv, ST) + ring_value_at(to & 31, t - 64, a.nbv, ST);
+    if constexpr (ES == 4)
+      *reinterpret_cast<uint32_t*>(y) = *reinterpret_cast<const uint32_t*>(x);
+    else
+      *reinterpret_cast<uint16_t*>(y) = *reinterpret_cast<const uint16_t*>(x);
+  }
+}
+
+// A slot's weight and position after the step, before its query adds to the weight.
+__device__ __forceinline__ float heavy_base(const HeavyMove& m, int slot, float w) {
+  if (slot == m.to) return m.weight;
+  return slot == m.slot || slot == m.hole ? 0.f : w;
+}
+
+// The increments of slots 4 at, .. + 3 from `queries` heads' logits, and what they do to the lowest kept weight; stat: the
+// heads' maxima, and their sums' inverses behind them.
+template <int ST>
+__device__ __forceinline__ unsigned long long heavy_grow(const HeavyArgs& a, const HeavyMove& m, int sh, int at,
+                                                         const float* logits, int queries, const float* stat, int pitch) {
+  constexpr float lift = win_weight_lift<ST>();
+  float* row = a.weights + static_cast<int64_t>(sh) * a.pitch + 4 * at;
+  const floatx4 w = *reinterpret_cast<const floatx4*>(row);
+  floatx4 grown = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < queries; ++i) {
+    const floatx4 x = *reinterpret_cast<const floatx4*>(logits + static_cast<int64_t>(i) * a.pitch + 4 * at);
+    const float top = stat[i], inv = stat[pitch + i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(x[j] - top, a.r.c, lift)) * inv;
+      grown[j] += win_finite(p) ? p : 0.f;
+    }
+  }
+  unsigned long long low = HEAVY_NONE;
+  floatx4 y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int slot = 4 * at + j;
+    const bool in = slot < m.held && slot != m.hole;
+    y[j] = in ? heavy_base(m, slot, w[j]) + grown[j] : 0.f;
+    if (in && slot >= a.ring) low = heavy_min(low, heavy_key(y[j], slot));
+  }
+  *reinterpret_cast<floatx4*>(row) = y;
+  return low;
+}
+
+// positions of the slots that a step changes
+__device__ __forceinline__ void heavy_positions(const HeavyArgs& a, const HeavyMove& m, int sh) {
+  int64_t* row = a.positions + static_cast<int64_t>(sh) * a.pitch;
+  if (m.to >= 0) row[m.to] = m.n - a.recent;
+  if (m.from >= 0) row[m.from] = -1;
+  if (m.slot >= 0) row[m.slot] = m.n;
+}
+
+// The walk of ring_attention_kernel over the slots that hold a token, with the logits put down for the weights' growth.  A
+// workgroup that is alone with a key head finishes it: outputs, weights, the next lowest one; else heavy_join_kernel does.
+template <int NBK, int NBV, int ST>
+__global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel(const HeavyArgs h) {
+  const RingArgs& a = h.r;
+  constexpr int PP = ST == F32 ? 1 : 2;  // planes of the weights, see ring_cache.hip
+  constexpr int ES = ST == F32 ? 4 : 2, CT = 2 * NBV, W = RingTile<NBK, NBV, ST>::W;
+  constexpr int PITCH = 32 * NBV + 4;
+  __shared__ float red[4 * 16 * PITCH], red_m[4 * 16], red_l[4 * 16], stat[2 * 16];
+  __shared__ unsigned long long red_low[4];
+  int id = blockIdx.x;
+  const int split = id % a.nsplit;
+  id /= a.nsplit;
+  const int chunk = id % a.chunks, sh = id / a.chunks;
+  const int s = sh / a.kv, hk = sh - s * a.kv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
+
+  const HeavyMove move = heavy_move(h, sh, a.append);
+  const bool alone = h.alone;
+  const int all = (move.held + 31) >> 5, per = (all + a.nsplit - 1) / a.nsplit;
+  const int t0 = split * per, t1 = t0 + per < all ? t0 + per : all;
+  if (a.append) {
+    if (move.to >= 0 && (move.to >> 5) >= t0 && (move.to >> 5) < t1) heavy_keep<ST>(a, sh, move.from, move.to);
+    if ((move.slot >> 5) >= t0 && (move.slot >> 5) < t1) ring_put<ST, ST>(a, s, hk, move.slot);
+    __syncthreads();
+  }
+  if (!alone && split == 0 && chunk == 0 && threadIdx.x == 0) {
+    h.moves[sh] = move;
+    h.lowest[2 * static_cast<int64_t>(sh) + ((move.n + a.append) & 1)] = HEAVY_NONE;
+  }
+
+  const int queries = min(16, a.group - 16 * chunk);
+  const int64_t head0 = static_cast<int64_t>(s) * a.heads + hk * a.group + 16 * chunk;
+  RingFrag<ST> qf[NBK];
+  {
+    const bool in = li < queries;
+    const char* row = rows_at<ES>(a.q, s, hk * a.group + 16 * chunk + (in ? li : 0), 0);
+#pragma unroll
+    for (int b = 0; b < NBK; ++b) {
+      constexpr int E = 16 / ES;
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8 / E; ++i) {
+        float y[E];
+        rows_unpack<ST>(rows_chunk<ES>(row, 32 * b + 8 * lg + E * i, a.d), y);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[E * i + e] = in ? (a.scale < 0.f ? -y[e] : y[e]) : 0.f;
+      }
+      RingFrag<ST> planes[1];
+      ring_planes<ST, 1>(x, planes);
+      qf[b] = planes[0];
+    }
+  }
+
+  floatx4 acc[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) acc[ct] = floatx4{0.f, 0.f, 0.f, 0.f};
+  float m = -3.4028235e38f, limit = m, l = 0.f;
+  constexpr float lift = win_weight_lift<ST>();  // fp16 weights, see ring_cache.hip
+  const float room = win_weight_room<ST>() / a.c;
+
+  const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
+  float* const logits = h.logits + (head0 + li) * h.pitch + 4 * lg;
+  // a tile's part of the sums; PART: not all of its slots hold a token
+  auto take = [&](const RingTile<NBK, NBV, ST>& cur, int t, auto part) {
+    constexpr bool PART = decltype(part)::value;
+    floatx4 x[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      x[half] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int b = 0; b < NBK; ++b) {
+        RingFrag<ST> k;
+#pragma unroll
+        for (int i = 0; i < W; ++i) k.w[i] = cur.k[half][b * W + i];
+        x[half] = ring_mma<ST>(k, qf[b], x[half]);
+      }
+    }
+    // this lane's slots that hold a token: below `left`, but `hole`
+    const int left = move.held - 32 * t - 4 * lg, hole = move.hole - 32 * t - 4 * lg;
+    auto out = [&](int i) {
+      const int at = 16 * (i >> 2) + (i & 3);
+      return at >= left || at == hole;
+    };
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (PART && out(i)) x[i >> 2][i & 3] = -__builtin_inff();
+      top = fmaxf(top, x[i >> 2][i & 3]);
+    }
+    if (li < queries) {
+      *reinterpret_cast<floatx4*>(logits + 32 * t) = x[0];
+      *reinterpret_cast<floatx4*>(logits + 32 * t + 16) = x[1];
+    }
+    // the maximum moves, for all lanes of a query at once, when a weight would exceed 2^room
+    if (__any(top > limit)) {
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float shrink = __builtin_amdgcn_exp2f((m - top) * a.c);
+      l *= shrink;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) acc[ct] *= shrink;
+      m = top;
+      limit = top + room;
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3] - m, a.c, lift));
+      if (PART && out(i)) p[i] = 0.f;
+      l += p[i];
+    }
+    RingFrag<ST> pf[PP];
+    ring_planes<ST, PP>(p, pf);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      RingFrag<ST> v;
+#pragma unroll
+      for (int i = 0; i < W; ++i) v.w[i] = cur.v[ct * W + i];
+      if constexpr (PART) {  // slots without a token: whatever they hold
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (out(i)) {
+            if constexpr (ST == F32)
+              v.w[i] = 0u;
+            else
+              v.w[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+          }
+      }
+#pragma unroll
+      for (int k = PP - 1; k >= 0; --k) acc[ct] = ring_mma<ST>(v, pf[k], acc[ct]);
+    }
+  };
+  // whole tiles, one ahead in registers, the two buffers in turn; then the hole's tile, and the last if it is not whole
+  {
+    const int whole_end = t1 < (move.held >> 5) ? t1 : move.held >> 5;
+    const int hole_tile = move.hole >= 0 ? move.hole >> 5 : -1;
+    const bool skip = hole_tile >= t0 && hole_tile < whole_end;
+    const int end = whole_end - (skip ? 1 : 0);
+    auto tile = [&](int i) { return i + (skip && i >= hole_tile ? 1 : 0); };
+    RingTile<NBK, NBV, ST> even, odd;
+    int t = t0 + wave;
+    if (t < end) even.load(a, tile0 + tile(t), lane);
+    while (t < end) {
+      if (t + 4 < end) odd.load(a, tile0 + tile(t + 4), lane);
+      take(even, tile(t), std::false_type{});
+      t += 4;
+      if (t >= end) break;
+      if (t + 4 < end) even.load(a, tile0 + tile(t + 4), lane);
+      take(odd, tile(t), std::false_type{});
+      t += 4;
+    }
+    const int last = t0 <= whole_end && whole_end < t1 ? whole_end : -1;
+    const int mine = wave == 3 ? (hole_tile >= t0 && hole_tile < t1 ? hole_tile : -1) : (wave == 2 && last != hole_tile ? last : -1);
+    if (mine >= 0) {
+      even.load(a, tile0 + mine, lane);
+      take(even, mine, std::true_type{});
+    }
+  }
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+
+  // the four waves' sums
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+    *reinterpret_cast<floatx4*>(&red[(wave * 16 + li) * PITCH + 16 * ct + 4 * lg]) = acc[ct];
+  if (lg == 0) {
+    red_m[wave * 16 + li] = prefix_top(m, l);
+    red_l[wave * 16 + li] = l;
+  }
+  __syncthreads();
+  for (int at = threadIdx.x; at < queries * a.dv; at += 256) {
+    const int i = at / a.dv, col = at - i * a.dv;
+    float top = red_m[i], sum = 0.f, den = 0.f;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, red_m[16 * w + i]);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float lw = red_l[16 * w + i], f = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f((red_m[16 * w + i] - top) * a.c);
+      if (lw != 0.f) sum = fmaf(f, red[(w * 16 + i) * PITCH + col], sum);
+      den = fmaf(f, lw, den);
+    }
+    if (alone) {
+      store_elem(a.out, (head0 + i) * a.dv + col, ST, move.held ? sum / den : 0.f);
+      if (col == 0) {
+        stat[i] = top;
+        stat[16 + i] = 1.f / den;
+      }
+    } else {
+      float* part = a.part + ((head0 + i) * a.nsplit + split) * (a.dv + 2);
+      part[col] = sum;
+      if (col == 0) {
+        part[a.dv] = prefix_top(top, den);
+        part[a.dv + 1] = den;
+      }
+    }
+  }
+  if (!alone) return;
+  __syncthreads();  // the logits of all waves, too
+  unsigned long long low = HEAVY_NONE;
+  for (int at = threadIdx.x; 4 * at < move.held; at += 256)
+    low = heavy_min(low, heavy_grow<ST>(h, move, sh, at, h.logits + head0 * h.pitch, queries, stat, 16));
+  low = heavy_least<256>(low, red_low);
+  if (threadIdx.x == 0) {
+    heavy_positions(h, move, sh);
+    h.lowest[2 * static_cast<int64_t>(sh) + ((move.n + a.append) & 1)] = low;
+    h.counts[sh] = move.n + a.append;
+  }
+}
+
+// Steps that several workgroups share: outputs, 4 groups of 128 threads (a column each) over the partials of a query head,
+// then in workgroups of their own the weights, 2048 slots of a key head each.
+constexpr int HEAVY_SPLITS = 1024, HEAVY_SLOTS = 2048, HEAVY_HEADS = 512;
+template <int ST>
+__global__ __launch_bounds__(512) void heavy_join_kernel(const HeavyArgs h, int outputs, int ranges) {
+  const RingArgs& a = h.r;
+  __shared__ float weight[HEAVY_SPLITS], red[4 * 128], wave_red[8], stat[2 * HEAVY_HEADS];
+  __shared__ unsigned long long red_low[8];
+  const int pitch = a.dv + 2, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int total = a.nsplit + h.prefix_parts;
+  auto partial = [&](int64_t head, int j) {
+    return j < a.nsplit ? a.part + (head * a.nsplit + j) * pitch : h.prefix + (head * h.prefix_parts + j - a.nsplit) * pitch;
+  };
+  if (static_cast<int>(blockIdx.x) < outputs) {
+    const int64_t head = blockIdx.x;
+    const int s = blockIdx.x / a.heads, hh = blockIdx.x - s * a.heads, sh = s * a.kv + hh / a.group;
+    const int col = threadIdx.x & 127, group = threadIdx.x >> 7;
+    float top = -__builtin_inff(), den = 0.f;
+    for (int i = threadIdx.x; i < total; i += 512) top = fmaxf(top, partial(head, i)[a.dv]);
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if (lane == 0) wave_red[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, wave_red[i]);
+    for (int i = threadIdx.x; i < total; i += 512) {
+      const float* part = partial(head, i);
+      const float li = part[a.dv + 1], f = li == 0.f ? 0.f : __builtin_amdgcn_exp2f((part[a.dv] - top) * a.c);
+      weight[i] = f;
+      den = fmaf(f, li, den);
+    }
+    for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
+    __syncthreads();
+    if (lane == 0) wave_red[wave] = den;
+    float sum = 0.f;
+    if (col < a.dv) {
+#pragma unroll 8
+      for (int i = group; i < total; i += 4) sum = fmaf(weight[i], partial(head, i)[col], sum);
+    }
+    red[threadIdx.x] = sum;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < a.dv) {
+      den = 0.f;
+      for (int i = 0; i < 8; ++i) den += wave_red[i];
+      sum = red[threadIdx.x] + red[128 + threadIdx.x] + red[256 + threadIdx.x] + red[384 + threadIdx.x];
+      const bool some = h.moves[sh].held || den != 0.f;
+      store_elem(a.out, head * a.dv + threadIdx.x, ST, some ? sum / den : 0.f);
+    }
+    return;
+  }
+  const int id = blockIdx.x - outputs, sh = id / ranges, range = id - sh * ranges;
+  const HeavyMove move = h.moves[sh];
+  const int s = sh / a.kv, hk = sh - s * a.kv;
+  const int64_t head0 = static_cast<int64_t>(s) * a.heads + hk * a.group;
+  unsigned long long low = HEAVY_NONE;
+  if (range * HEAVY_SLOTS < move.held) {
+    for (int i = wave; i < a.group; i += 8) {  // a wave a head: its maximum and sum
+      float top = -__builtin_inff(), den = 0.f;
+      for (int j = lane; j < total; j += 64) top = fmaxf(top, partial(head0 + i, j)[a.dv]);
+      for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+      for (int j = lane; j < total; j += 64) {
+        const float* part = partial(head0 + i, j);
+        const float lj = part[a.dv + 1];
+        den = fmaf(lj == 0.f ? 0.f : __builtin_amdgcn_exp2f((part[a.dv] - top) * a.c), lj, den);
+      }
+      for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
+      if (lane == 0) {
+        stat[i] = top;
+        stat[HEAVY_HEADS + i] = 1.f / den;
+      }
+    }
+    __syncthreads();
+    const int at = range * (HEAVY_SLOTS / 4) + threadIdx.x;
+    if (4 * at < move.held)
+      low = heavy_grow<ST>(h, move, sh, at, h.logits + head0 * h.pitch, a.group, stat, HEAVY_HEADS);
+  }
+  low = heavy_least<512>(low, red_low);
+  if (threadIdx.x == 0) {
+    if (low != HEAVY_NONE) atomicMin(&h.lowest[2 * static_cast<int64_t>(sh) + ((move.n + a.append) & 1)], low);
+    if (range == 0) {
+      heavy_positions(h, move, sh);
+      h.counts[sh] = move.n + a.append;
+    }
+  }
+}
+
+// One token of every stream into the cache, without a query: a workgroup a key head.
+template <int ST>
+__global__ __launch_bounds__(256) void heavy_update_kernel(const HeavyArgs h) {
+  const RingArgs& a = h.r;
+  __shared__ unsigned long long red_low[4];
+  const int sh = blockIdx.x, s = sh / a.kv, hk = sh - s * a.kv;
+  const HeavyMove move = heavy_move(h, sh, true);
+  if (move.to >= 0) heavy_keep<ST>(a, sh, move.from, move.to);
+  ring_put<ST, ST>(a, s, hk, move.slot);
+  float* row = h.weights + static_cast<int64_t>(sh) * h.pitch;
+  unsigned long long low = HEAVY_NONE;
+  for (int slot = h.ring + threadIdx.x; slot < move.held; slot += 256)
+    low = heavy_min(low, heavy_key(heavy_base(move, slot, row[slot]), slot));
+  low = heavy_least<256>(low, red_low);  // with a barrier: every thread has read the count and its weights
+  if (threadIdx.x == 0) {
+    if (move.to >= 0) row[move.to] = move.weight;
+    if (move.from >= 0) row[move.from] = 0.f;
+    row[move.slot] = 0.f;
+    heavy_positions(h, move, sh);
+    h.lowest[2 * static_cast<int64_t>(sh) + ((move.n + 1) & 1)] = low;
+    h.counts[sh] = move.n + 1;
+  }
+}
+
+struct HeavyFill {
+  HeavyArgs h;           // r.k, r.v: [streams][kv][rows][d | dv]
+  int rows;
+  const int* take;       // [streams] or null: rows of a stream that are tokens; a stream with none keeps what it holds
+  const float* given;    // [streams][kv][rows]: the rows' weights
+  int* token;            // [streams][kv][pitch]: the row of every slot, or -1
+};
+
+__device__ __forceinline__ int heavy_take(const HeavyFill& f, int s) {
+  const int t = f.take ? f.take[s] : f.rows;
+  return t < 0 ? 0 : (t > f.rows ? f.rows : t);
+}
+// a weight as the cache takes it: NaN and -0 as 0
+__device__ __forceinline__ float heavy_given(float w) { return w == w ? w + 0.f : 0.f; }
+
+// Which rows stay, by a workgroup of 1024 threads a key head: the last `recent`, and of the others the `kept` of the
+// largest weights, of equal ones the first.  Four passes over the weights find the smallest that stays, 8 bits of its
+// order at a time (the highest byte first, among those that agree with it so far); one more puts the rows that stay down in
+// their order.
+__global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFill f) {
+  const HeavyArgs& h = f.h;
+  __shared__ int bins[256], wave_sum[2][16], chosen[2];
+  __shared__ unsigned long long red_low[16];
+  const int sh = blockIdx.x, s = sh / h.r.kv, n = heavy_take(f, s), t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  if (n == 0) return;
+  const float* given = f.given + static_cast<int64_t>(sh) * f.rows;
+  int* token = f.token + static_cast<int64_t>(sh) * h.pitch;
+  float* weights = h.weights + static_cast<int64_t>(sh) * h.pitch;
+  int64_t* positions = h.positions + static_cast<int64_t>(sh) * h.pitch;
+  const int older = n > h.recent ? n - h.recent : 0;
+
+  uint32_t least = 0u;  // the order of the smallest weight that stays
+  int equal = 0x7fffffff;  // how many of those equal to it stay
+  if (older > h.kept) {
+    int want = h.kept;  // among those that agree so far
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      if (t < 256) bins[t] = 0;
+      __syncthreads();
+      const uint32_t high = shift == 24 ? 0u : least >> (shift + 8);
+      for (int i = t; i < older; i += 1024) {
+        const uint32_t u = heavy_order(heavy_given(given[i]));
+        if (shift == 24 || u >> (shift + 8) == high) atomicAdd(&bins[(u >> shift) & 255u], 1);
+      }
+      __syncthreads();
+      // the highest byte with `want` at or above it: sums from above, 4 bins a lane of the first wave
+      if (wave == 0) {
+        int part[4], sum = 0;
+        for (int j = 0; j < 4; ++j) {
+          part[j] = bins[255 - 4 * lane - j];
+          sum += part[j];
+        }
+        int before = sum;
+        for (int o = 1; o < 64; o <<= 1) {
+          const int y = __shfl_up(before, o);
+          if (lane >= o) before += y;
+        }
+        before -= sum;
+        for (int j = 0; j < 4; ++j) {
+          if (before < want && before + part[j] >= want) {
+            chosen[0] = 255 - 4 * lane - j;
+            chosen[1] = want - before;
+          }
+          before += part[j];
+        }
+      }
+      __syncthreads();
+      least |= static_cast<uint32_t>(chosen[0]) << shift;
+      want = chosen[1];
+      __syncthreads();
+    }
+    equal = want;
+  }
+  // the rows that stay, in their order
+  unsigned long long low = HEAVY_NONE;
+  int taken = 0, ties = 0;
+  for (int i0 = 0; i0 < older; i0 += 1024) {
+    const int i = i0 + t;
+    const float w = i < older ? heavy_given(given[i]) : 0.f;
+    const uint32_t u = heavy_order(w);
+    const bool tie = i < older && u == least && equal != 0x7fffffff;
+    const unsigned long long ballot = __ballot(tie), below = (1ull << lane) - 1ull;
+    if (lane == 0) wave_sum[0][wave] = __popcll(ballot);
+    __syncthreads();
+    int rank = ties + __popcll(ballot & below), all = 0;
+    for (int j = 0; j < 16; ++j) {
+      if (j < wave) rank += wave_sum[0][j];
+      all += wave_sum[0][j];
+    }
+    ties += all;
+    const bool stays = i < older && (equal == 0x7fffffff || u > least || (tie && rank < equal));
+    const unsigned long long kept = __ballot(stays);
+    if (lane == 0) wave_sum[1][wave] = __popcll(kept);
+    __syncthreads();
+    int at = taken + __popcll(kept & below);
+    all = 0;
+    for (int j = 0; j < 16; ++j) {
+      if (j < wave) at += wave_sum[1][j];
+      all += wave_sum[1][j];
+    }
+    taken += all;
+    if (stays) {
+      const int slot = h.ring + at;
+      token[slot] = i;
+      weights[slot] = w;
+      positions[slot] = i;
+      low = heavy_min(low, heavy_key(w, slot));
+    }
+  }
+  for (int slot = h.ring + taken + t; slot < h.pitch; slot += 1024) {
+    token[slot] = -1;
+    weights[slot] = 0.f;
+    positions[slot] = -1;
+  }
+  for (int slot = t; slot < h.ring; slot += 1024) {
+    const int p = n - 1 - static_cast<int>((static_cast<int64_t>(n) - 1 - slot + h.ring) % h.ring);
+    const bool in = p >= 0 && p >= older;
+    token[slot] = in ? p : -1;
+    weights[slot] = in ? heavy_given(given[p]) : 0.f;
+    positions[slot] = in ? p : -1;
+  }
+  low = heavy_least<1024>(low, red_low);
+  if (t == 0) {
+    h.lowest[2 * static_cast<int64_t>(sh) + (n & 1)] = low;
+    h.counts[sh] = n;
+  }
+}
+
+// The rows that stay into their slots: a workgroup a tile.
+template <int ST>
+__global__ __launch_bounds__(256) void heavy_fill_kernel(const HeavyFill f) {
+  const RingArgs& a = f.h.r;
+  __shared__ int token[32];
+  int sh, tile;
+  if (!ring_place(a, sh, tile)) return;
+  const int s = sh / a.kv, hk = sh - s * a.kv;
+  if (heavy_take(f, s) == 0) return;
+  if (threadIdx.x < 32) token[threadIdx.x] = f.token[static_cast<int64_t>(sh) * f.h.pitch + 32 * tile + threadIdx.x];
+  if (!__syncthreads_or(threadIdx.x < 32 && token[threadIdx.x] >= 0)) return;
+  ring_fill<ST, ST>(a, s, hk, tile, token);
+}
+
+// The slots' rows as they are.
+template <int ST>
+__global__ __launch_bounds__(256) void heavy_items_kernel(const HeavyArgs h, void* keys, void* values) {
+  int sh, tile;
+  if (!ring_place(h.r, sh, tile)) return;
+  const int64_t* positions = h.positions + static_cast<int64_t>(sh) * h.pitch + 32 * tile;
+  const bool some = __syncthreads_or(threadIdx.x < 32 && positions[threadIdx.x] >= 0);
+  ring_rows_out<ST, ST>(h.r, sh, tile, some, [&](int r) { return positions[r] >= 0; }, keys, values);
+}
+
+}  // namespace sta

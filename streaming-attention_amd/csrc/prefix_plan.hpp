@@ -1,0 +1,145 @@
+// How the rows and keys of an attention over a shared prefix are dealt out, for the entry points that launch it.
+#pragma once
+
+#include "api_common.hpp"
+#include "prefix_attn.hip"
+
+namespace sta_api {
+
+template <int P, int IN>
+int launch_prefix(const sta::PrefixArgs& a, const sta::PrefixWalk& w, int share, int values, hipStream_t s);
+template <int P, int IN>
+int launch_received(const sta::ReceivedArgs& w, hipStream_t s);
+
+constexpr int kMaxPrefixD = 128;
+constexpr int64_t kMaxPrefixRows = int64_t(1) << 30;
+constexpr int kMaxPrefixParts = 256;  // prefix_join_kernel's weights
+
+// The walks of a call: one over prefix and own tokens together, or two, whose partials are joined.
+struct PrefixPlan {
+  int walks;
+  sta::PrefixWalk walk[2];
+  int share[2];
+  int parts;        // 0: one workgroup finishes a row
+};
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// One walk over `keys` keys of units of `rows` rows: the tile and the number of workgroups that share a tile's keys.
+// Up to 32 rows: one tile of 32 whose waves share the keys.  The card holds 512 workgroups at a time (256 compute units,
+// two each of 128 columns); a share has at least 256 keys.
+inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows, int64_t keys) {
+  share = rows <= 32;
+  w.tiles = static_cast<int>(ceil_div(rows, share ? 32 : sta::WIN_ROWS));
+  int64_t want = 512 / (units * w.tiles);
+  const int64_t most = ceil_div(keys, 256);
+  if (want > most) want = most;
+  if (want > kMaxPrefixParts / 2) want = kMaxPrefixParts / 2;
+  w.nsplit = static_cast<int>(want < 1 ? 1 : want);
+}
+
+// own: the sequences' own tokens take part.  The sequences of a set lie in one tile for the prefix where each has fewer rows
+// than a tile.
+inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, bool own) {
+  PrefixPlan p{};
+  const int64_t rows = static_cast<int64_t>(a.n) * a.group, units = static_cast<int64_t>(a.batch) * a.kv;
+  const bool packed = a.p > 0 && (!own || (a.per_set > 1 && rows < sta::WIN_ROWS));
+  if (packed) {
+    p.walks = own ? 2 : 1;
+    p.walk[0].span = a.per_set;
+    p.walk[0].prefix = 1;
+    deal_out(p.walk[0], p.share[0], static_cast<int64_t>(a.sets) * a.kv, rows * a.per_set, a.p);
+    p.parts = p.walk[0].nsplit;
+    if (own) {
+      p.walk[1].span = 1;
+      p.walk[1].own = 1;
+      p.walk[1].first = p.parts;
+      deal_out(p.walk[1], p.share[1], units, rows, a.m);
+      p.parts += p.walk[1].nsplit;
+    }
+    return p;
+  }
+  p.walks = 1;
+  p.walk[0].span = 1;
+  p.walk[0].prefix = a.p > 0;
+  p.walk[0].own = 1;
+  deal_out(p.walk[0], p.share[0], units, rows, static_cast<int64_t>(a.p) + a.m);
+  p.parts = p.walk[0].nsplit > 1 ? p.walk[0].nsplit : 0;
+  return p;
+}
+
+inline int64_t prefix_part_bytes(const sta::PrefixArgs& a, int parts) {
+  return 4 * static_cast<int64_t>(a.batch) * a.heads * a.n * parts * (a.dv + 2);
+}
+
+// The shape part of the arguments; d and dv padded are the caller's.
+inline int prefix_shape(sta::PrefixArgs& a, int dtype, int64_t batch, int heads, int kv_heads, int64_t sets, int64_t n,
+                        int64_t m, int64_t p, int d, int dv, float scale) {
+  if (!dtype_ok(dtype)) return STA_ERR_DTYPE;
+  const int es = dtype == STA_F32 ? 4 : 2;
+  if (batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || sets < 1 || batch % sets || n < 1 || m < 0 || p < 0 ||
+      d < 1 || dv < 0)
+    return STA_ERR_SHAPE;
+  if (!(scale == scale && scale - scale == 0.f)) return STA_ERR_ARG;  // finite
+  if (d > kMaxPrefixD || dv > kMaxPrefixD || d * es < 16 || (dv && dv * es < 16) || n > kMaxPrefixRows ||
+      m > kMaxPrefixRows || p > kMaxPrefixRows || batch > 0x7fffffff / heads ||
+      static_cast<int64_t>(batch / sets) * n > kMaxPrefixRows / (heads / kv_heads))
+    return STA_ERR_UNSUPPORTED;
+  a = sta::PrefixArgs{};
+  a.batch = static_cast<int>(batch);
+  a.heads = heads;
+  a.kv = kv_heads;
+  a.group = heads / kv_heads;
+  a.sets = static_cast<int>(sets);
+  a.per_set = static_cast<int>(batch / sets);
+  a.n = static_cast<int>(n);
+  a.m = static_cast<int>(m);
+  a.p = static_cast<int>(p);
+  a.d = d;
+  a.dv = dv;
+  a.scale = scale;
+  const float c = (scale < 0.f ? -scale : scale) * 1.44269504088896340736f;
+  a.c = c > 1e-37f ? c : 1e-37f;  // above 0: a hidden pair's logit, -inf, stays one times c
+  return STA_OK;
+}
+
+// a tile's rows are reached by 32-bit offsets from its first
+inline bool prefix_strides_ok(const int64_t* strides, int tensors, int dtype) {
+  for (int i = 0; i < tensors; ++i) {
+    const int64_t sn = strides[3 * i + 2];
+    if (sn < 0 || sn > (int64_t(1) << 24) / (dtype == STA_F32 ? 4 : 2)) return false;
+  }
+  return true;
+}
+
+inline sta::Rows prefix_rows_of(const void* p, const int64_t* strides) {
+  return sta::Rows{p, strides[0], strides[1], strides[2], 0};
+}
+
+template <typename Call>
+int prefix_by_type(int dtype, int width, Call call) {
+#define STA_PREFIX_CASE(P)                                                                                 \
+  if (width <= P) {                                                                                        \
+    if (dtype == STA_F32) return call(std::integral_constant<int, P>{}, std::integral_constant<int, sta::F32>{});   \
+    if (dtype == STA_BF16) return call(std::integral_constant<int, P>{}, std::integral_constant<int, sta::BF16>{}); \
+    return call(std::integral_constant<int, P>{}, std::integral_constant<int, sta::F16>{});                \
+  }
+  STA_PREFIX_CASE(32)
+  STA_PREFIX_CASE(64)
+  STA_PREFIX_CASE(96)
+  STA_PREFIX_CASE(128)
+#undef STA_PREFIX_CASE
+  return STA_ERR_UNSUPPORTED;
+}
+
+// the walks of a plan
+inline int run_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int dtype, int values, hipStream_t s) {
+  return prefix_by_type(dtype, values && a.dv > a.d ? a.dv : a.d, [&](auto width, auto in) {
+    int st = STA_OK;
+    for (int i = 0; i < p.walks && st == STA_OK; ++i)
+      st = launch_prefix<decltype(width)::value, decltype(in)::value>(a, p.walk[i], p.share[i], values, s);
+    return st;
+  });
+}
+
+}  // namespace sta_api

@@ -21,6 +21,7 @@
 // Codes become bf16 with their powers (exact); queries of more than 8 bits and the weights are carried as bf16 planes (fp16
 // queries 2, fp32 3; weights 2, 3 for fp32), of 16-bit caches as 2 planes of their type: the products keep the accuracy
 // of the output's type, and a step is bound by reading the cache.
+#pragma once
 #include <type_traits>
 
 #include "rows.hpp"
@@ -613,21 +614,12 @@ __device__ __forceinline__ int ring_take(const RingFill& f, int s) {
   return t < 0 ? 0 : (t > f.rows ? f.rows : t);
 }
 
-// A workgroup a tile of 32 slots: the last token that falls into each slot.
+// The rows token[0 .. 31] (-1: none) of a stream's key head into the slots of a tile, by a workgroup of 256 threads.
 template <int ST, int Q>
-__global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
+__device__ __forceinline__ void ring_fill(const RingArgs& a, int s, int hk, int tile, const int* token) {
   constexpr int ES = Q == F32 ? 4 : 2;
-  const RingArgs& a = f.a;
   __shared__ uint32_t vals[32 * 132];  // the tile's values (bits, or codes), 32 nbv + 1 a slot
-  __shared__ int token[32];
-  int sh, tile;
-  if (!ring_place(a, sh, tile)) return;
-  const int s = sh / a.kv, hk = sh - s * a.kv, n = ring_count(a, sh), take = ring_take(f, s);
-  if (threadIdx.x < 32) {
-    const int slot = 32 * tile + threadIdx.x;
-    token[threadIdx.x] = slot < a.slots ? ring_token(a, slot, n, take) : -1;
-  }
-  if (!__syncthreads_or(threadIdx.x < 32 && token[threadIdx.x] >= 0)) return;  // no token falls into this tile
+  const int sh = s * a.kv + hk;
   const int64_t at = static_cast<int64_t>(sh) * a.tiles + tile;
   uint8_t* keys = a.keys + at * ring_tile_bytes(a.nbk, ST);
   uint8_t* values = a.values + at * ring_tile_bytes(a.nbv, ST);
@@ -740,27 +732,40 @@ __global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
   }
 }
 
+// A workgroup a tile of 32 slots: the last token that falls into each slot.
+template <int ST, int Q>
+__global__ __launch_bounds__(256) void ring_extend_kernel(const RingFill f) {
+  const RingArgs& a = f.a;
+  __shared__ int token[32];
+  int sh, tile;
+  if (!ring_place(a, sh, tile)) return;
+  const int s = sh / a.kv, hk = sh - s * a.kv, n = ring_count(a, sh), take = ring_take(f, s);
+  if (threadIdx.x < 32) {
+    const int slot = 32 * tile + threadIdx.x;
+    token[threadIdx.x] = slot < a.slots ? ring_token(a, slot, n, take) : -1;
+  }
+  if (!__syncthreads_or(threadIdx.x < 32 && token[threadIdx.x] >= 0)) return;  // no token falls into this tile
+  ring_fill<ST, Q>(a, s, hk, tile, token);
+}
+
 // counts += the tokens that ring_extend_kernel has put in
 __global__ __launch_bounds__(256) static void ring_count_kernel(const RingFill f) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   if (i < f.a.streams * f.a.kv) f.a.counts[i] = ring_after(f.a, ring_count(f.a, i), ring_take(f, i / f.a.kv));
 }
 
-// The slots' rows as they stand for: keys [streams][kv][slots][d], values [..][dv] in the element type, zero where no
-// token is; positions [streams][slots], -1 there.  A workgroup a tile: the tile's words in their order into LDS rows, then
-// whole rows out.
-template <int ST, int Q>
-__global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void* keys, void* values, int* positions) {
+// A tile's rows as they stand for: keys [streams][kv][slots][d], values [..][dv] in the element type, zero where no
+// token is (`there` of a slot of the tile; `some`: one of them holds a token).  A workgroup of 256 threads: the tile's words
+// in their order into LDS rows, then whole rows out.
+template <int ST, int Q, typename There>
+__device__ __forceinline__ void ring_rows_out(const RingArgs& a, int sh, int tile, bool some, There there, void* keys,
+                                              void* values) {
   constexpr int PITCH = 129;
   __shared__ uint32_t rows[32 * PITCH];  // values: floats (4-bit), or the elements' bits
-  int sh, tile;
-  if (!ring_place(a, sh, tile)) return;
-  const int s = sh / a.kv, hk = sh - s * a.kv, n = ring_count(a, sh);
   const int64_t at = static_cast<int64_t>(sh) * a.tiles + tile;
   const uint8_t* kp = a.keys + at * ring_tile_bytes(a.nbk, ST);
   const uint8_t* vp = a.values + at * ring_tile_bytes(a.nbv, ST);
   const int live = min(32, a.slots - 32 * tile);  // slots of the tile
-  const bool some = 32 * tile < n;                // one of them holds a token
   auto elem = [&](const uint8_t* p, int e) -> uint32_t {
     if constexpr (ST == F32) return reinterpret_cast<const uint32_t*>(p)[e];
     return reinterpret_cast<const uint16_t*>(p)[e];
@@ -772,7 +777,7 @@ __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void*
       const int units = width / E;
       for (int i = threadIdx.x; i < live * units; i += 256) {
         const int r = i / units, col = (i - r * units) * E;
-        const bool held = 32 * tile + r < n;
+        const bool held = there(r);
         uint4 w;
         if constexpr (ST == RING_F4) {
           float f[E];
@@ -795,7 +800,7 @@ __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void*
     }
     for (int i = threadIdx.x; i < live * width; i += 256) {
       const int r = i / width, col = i - r * width;
-      const uint32_t w = 32 * tile + r < n ? rows[r * PITCH + col] : 0u;
+      const uint32_t w = there(r) ? rows[r * PITCH + col] : 0u;
       if constexpr (ST == RING_F4)
         store_elem(out, base + i, Q, __uint_as_float(w));
       else if constexpr (ST == F32)
@@ -840,7 +845,16 @@ __global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void*
   }
   __syncthreads();
   store_rows(values, a.dv);
-  if (hk == 0 && static_cast<int>(threadIdx.x) < live) {
+}
+
+// The slots' rows, and positions [streams][slots], -1 where no token is.
+template <int ST, int Q>
+__global__ __launch_bounds__(256) void ring_items_kernel(const RingArgs a, void* keys, void* values, int* positions) {
+  int sh, tile;
+  if (!ring_place(a, sh, tile)) return;
+  const int s = sh / a.kv, hk = sh - s * a.kv, n = ring_count(a, sh);
+  ring_rows_out<ST, Q>(a, sh, tile, 32 * tile < n, [&](int r) { return 32 * tile + r < n; }, keys, values);
+  if (hk == 0 && static_cast<int>(threadIdx.x) < min(32, a.slots - 32 * tile)) {
     const int slot = 32 * tile + threadIdx.x;
     int p = -1;
     if (slot < n) p = slot < a.sinks ? slot : slot + (n - 1 - slot) / a.window * a.window;

@@ -22,6 +22,7 @@
 // pairs' zero weights with their values, so an infinity or NaN in a value that some rows of a tile see would reach
 // those that do not: a workgroup with a result that is not finite goes over its tiles once more, taking the partly visible ones
 // pair by pair (win_add_seen), and stores that result from there.
+#pragma once
 #include <type_traits>
 
 #include "rows.hpp"

@@ -95,11 +95,11 @@ def _heads_first(q: Tensor, k: Tensor, v: Tensor) -> Tuple[Tensor, Tensor, Tenso
     return q, k, v
 
 
-def _check_lengths(lengths: Optional[Tensor], batch: int) -> Optional[Tensor]:
+def _check_lengths(lengths: Optional[Tensor], batch: int, name: str = "lengths") -> Optional[Tensor]:
     if lengths is None:
         return None
     if lengths.dtype != torch.int32 or tuple(lengths.shape) != (batch,):
-        raise ValueError(f"lengths must be an int32 tensor [{batch}]")
+        raise ValueError(f"{name} must be an int32 tensor [{batch}]")
     return lengths.contiguous()
 
 
