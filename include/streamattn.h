@@ -662,11 +662,11 @@ int sta_heavy_start(const void* k, const void* v, const float* given, int dtype,
                     void* values, int64_t* counts, float* weights, int64_t* positions, uint64_t* lowest,
                     void* workspace, int64_t workspace_bytes, void* stream);
 
-/* The slots' rows: keys_out [streams][kv_heads][recent + 1 + kept][d], values_out [..][dv] (16-byte aligned; zero where no
- * token is). */
+/* The slots: keys_out [streams][kv_heads][recent + 1 + kept][d], values_out [..][dv] (16-byte aligned; zero where no token
+ * is), weights_out, positions_out [streams][kv_heads][recent + 1 + kept]. */
 int sta_heavy_items(int dtype, int64_t streams, int kv_heads, int d, int dv, int64_t recent, int64_t kept,
-                    const void* keys, const void* values, const int64_t* positions, void* keys_out, void* values_out,
-                    void* stream);
+                    const void* keys, const void* values, const float* weights, const int64_t* positions,
+                    void* keys_out, void* values_out, float* weights_out, int64_t* positions_out, void* stream);
 
 /* Rows per block-attention tile and the moment chunk the library uses for a head dimension D (the
  * chunk argument of sta_block_attention is that chunk for sta_moments' partials, the query block for

@@ -209,7 +209,7 @@ _SIGNATURES = {
         _i32, [_c_p, _c_p, _c_p, _i32, _i64, _i32, _i64, _i32, _i32, _c_p, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p,
                _c_p, _c_p, _i64, _c_p],  # k v weights type S Hk rows d dv strides recent kept take state ws bytes stream
     ),
-    "sta_heavy_items": (_i32, [_i32, _i64, _i32, _i32, _i32, _i64, _i64, _c_p, _c_p, _c_p, _c_p, _c_p, _c_p]),
+    "sta_heavy_items": (_i32, [_i32, _i64, _i32, _i32, _i32, _i64, _i64, *[_c_p] * 9]),
     "sta_head_rotary": (
         _i32, [_c_p, _c_p, _i32, _i64, _i32, _i32, _i64, _i32, _c_p, _c_p, _c_p, _i32, _c_p, _i64, _i32, _i32, _c_p,
                _i32, _i64, _i64, _f32, _c_p, _c_p, _c_p],  # .. weights type table limit rotary inter pos .. eps out out

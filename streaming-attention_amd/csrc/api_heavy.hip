@@ -3,7 +3,7 @@
 #include <cmath>
 
 #include "heavy_cache.hip"
-#include "prefix_plan.hpp"
+#include "prefix_dispatch.hpp"
 
 using namespace sta_api;
 
@@ -47,6 +47,7 @@ int heavy_shape(sta::HeavyArgs& h, int dtype, int64_t streams, int heads, int kv
   a.tiles = (a.slots + 31) / 32;
   a.nsplit = 1;
   h.pitch = 32 * a.tiles;
+  h.part_pitch = (dv + 3) / 4 * 4;
   return STA_OK;
 }
 
@@ -76,10 +77,10 @@ Workspace workspace_of(const sta::HeavyArgs& h, const sta::PrefixArgs* p, int pr
   const sta::RingArgs& a = h.r;
   const int64_t heads = static_cast<int64_t>(a.streams) * a.heads;
   Workspace w{};
-  w.logits = 4 * heads * h.pitch;
+  w.logits = h.local ? 0 : 4 * heads * h.pitch;
   if (h.alone) return w;
   w.moves = static_cast<int64_t>(sizeof(sta::HeavyMove)) * a.streams * a.kv;
-  w.part = round16(4 * heads * a.nsplit * (a.dv + 2));
+  w.part = round16(4 * heads * a.nsplit * h.part_pitch) + round16(8 * heads * a.nsplit);
   if (p) w.prefix = prefix_part_bytes(*p, prefix_parts);
   return w;
 }
@@ -87,6 +88,8 @@ void plan_heavy(sta::HeavyArgs& h, int prefix_parts) {
   h.r.nsplit = splits_of(h.r);
   h.prefix_parts = prefix_parts;
   h.alone = h.r.nsplit == 1 && h.r.chunks == 1 && prefix_parts == 0;
+  // two workgroups a compute unit with the logits in LDS, and the kernel's own kilobyte
+  h.local = h.alone && sta::heavy_lds_bytes(h.r.group, h.r.nbv, h.pitch, true) <= 79 * 1024;
 }
 
 template <int ST>
@@ -198,20 +201,21 @@ int sta_heavy_attention(const void* q, const void* k, const void* v, int dtype, 
   }
   plan_heavy(h, plan.parts);
   const Workspace w = workspace_of(h, p > 0 ? &x : nullptr, plan.parts);
-  if (!workspace || !aligned16(workspace) || workspace_bytes < w.total()) return STA_ERR_SCRATCH;
+  if (w.total() > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < w.total())) return STA_ERR_SCRATCH;
   char* room = static_cast<char*>(workspace);
   h.logits = reinterpret_cast<float*>(room);
   h.moves = reinterpret_cast<sta::HeavyMove*>(room + w.logits);
   a.part = reinterpret_cast<float*>(room + w.logits + w.moves);
-  h.prefix = reinterpret_cast<float*>(room + w.logits + w.moves + w.part);
+  h.stat = a.part + round16(4 * static_cast<int64_t>(a.streams) * a.heads * a.nsplit * h.part_pitch) / 4;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (p > 0) {
     x.q = rows_of(q, strides[0], strides[1], 0);
     x.pk = prefix_rows_of(prefix_k, prefix_strides);
     x.pv = prefix_rows_of(prefix_v, prefix_strides + 3);
     x.prefix_lengths = prefix_lengths;
-    x.part = const_cast<float*>(h.prefix);
-    x.parts = plan.parts;
+    set_parts(x, room + w.logits + w.moves + w.part, plan.parts);
+    h.prefix = x.part;
+    h.prefix_stat = x.stat;
     if (const int st = run_prefix(x, plan, dtype, 1, s)) return st;
   }
   int st = STA_OK;
@@ -272,21 +276,23 @@ int sta_heavy_start(const void* k, const void* v, const float* given, int dtype,
 }
 
 int sta_heavy_items(int dtype, int64_t streams, int kv_heads, int d, int dv, int64_t recent, int64_t kept,
-                    const void* keys, const void* values, const int64_t* positions, void* keys_out, void* values_out,
-                    void* stream) {
-  if (!keys || !values || !positions || !keys_out || !values_out || !aligned16(keys) || !aligned16(values) ||
-      !aligned16(keys_out) || !aligned16(values_out))
+                    const void* keys, const void* values, const float* weights, const int64_t* positions,
+                    void* keys_out, void* values_out, float* weights_out, int64_t* positions_out, void* stream) {
+  if (!keys || !values || !weights || !positions || !keys_out || !values_out || !weights_out || !positions_out ||
+      !aligned16(keys) || !aligned16(values) || !aligned16(keys_out) || !aligned16(values_out))
     return STA_ERR_ARG;
   sta::HeavyArgs h;
   if (const int st = heavy_shape(h, dtype, streams, kv_heads, kv_heads, d, dv, recent, kept)) return st;
   h.r.keys = static_cast<uint8_t*>(const_cast<void*>(keys));
   h.r.values = static_cast<uint8_t*>(const_cast<void*>(values));
+  h.weights = const_cast<float*>(weights);
   h.positions = const_cast<int64_t*>(positions);
+  const sta::HeavyItems to{keys_out, values_out, positions_out, weights_out};
   dim3 g;
   if (!tile_grid(h.r, g)) return STA_ERR_SHAPE;
   hipStream_t s = static_cast<hipStream_t>(stream);
   by_type(dtype, [&](auto t) {
-    hipLaunchKernelGGL((sta::heavy_items_kernel<decltype(t)::value>), g, dim3(256), 0, s, h, keys_out, values_out);
+    hipLaunchKernelGGL((sta::heavy_items_kernel<decltype(t)::value>), g, dim3(256), 0, s, h, to);
   });
   return check_launch();
 }

@@ -1,6 +1,6 @@
 // Entry points of the attention over a shared prefix and of the received weights (see include/streamattn.h): argument
 // checks, plans, launches.
-#include "prefix_plan.hpp"
+#include "prefix_dispatch.hpp"
 
 using namespace sta_api;
 
@@ -25,13 +25,22 @@ int join_rows(const sta::PrefixArgs& a, int dtype, hipStream_t s) {
   return check_launch();
 }
 
-// How the received weights are dealt out: tiles of 128 keys, and workgroups that share a tile's rows where there are
-// fewer than 1024 tiles (four workgroups a compute unit).
-void plan_received(sta::ReceivedArgs& w) {
+// How the received weights are dealt out.  Few rows: 2048 workgroups (eight a compute unit), whose waves have four blocks
+// of keys at least.  Many: a workgroup a tile of keys, and where that leaves fewer than 4096 several that share its rows, of
+// which the first tiles have most, 16 row tiles at least.
+void plan_received(sta::ReceivedArgs& w, int dtype) {
   const sta::PrefixArgs& a = w.a;
-  w.tiles = static_cast<int>(ceil_div(a.m, sta::WIN_ROWS));
-  int64_t want = 1024 / (static_cast<int64_t>(a.batch) * a.kv * w.tiles);
-  const int64_t most = static_cast<int64_t>(a.group) * ceil_div(a.n, 64);
+  const int64_t units = static_cast<int64_t>(a.batch) * a.kv, rows = static_cast<int64_t>(a.n) * a.group;
+  w.few = rows <= sta::RECEIVED_FEW;
+  w.nsplit = 1;
+  if (w.few) {
+    const int64_t want = ceil_div(2048, units), most = ceil_div(a.m, 4 * 4 * 32);
+    w.tiles = static_cast<int>(want < most ? want : most);
+    return;
+  }
+  w.tiles = static_cast<int>(ceil_div(a.m, dtype == STA_F32 ? 128 : 256));
+  int64_t want = 4096 / (units * w.tiles);
+  const int64_t most = ceil_div(a.group * ceil_div(a.n, 64), 16);
   if (want > most) want = most;
   w.nsplit = static_cast<int>(want < 1 ? 1 : want);
 }
@@ -80,8 +89,7 @@ int sta_prefix_attention(const void* q, const void* k, const void* v, const void
   a.prefix_lengths = prefix_lengths;
   a.out = out;
   a.lse = lse;
-  a.part = static_cast<float*>(workspace);
-  a.parts = plan.parts;
+  set_parts(a, workspace, plan.parts);
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int st = run_prefix(a, plan, dtype, 1, s);
   return st == STA_OK && plan.parts ? join_rows(a, dtype, s) : st;
@@ -91,7 +99,7 @@ int64_t sta_received_attention_bytes(int dtype, int64_t batch, int heads, int kv
                                      int with_lse) {
   sta::ReceivedArgs w{};
   if (prefix_shape(w.a, dtype, batch, heads, kv_heads, batch, n, m, 0, d, 0, 1.f) != STA_OK || m < 1) return -1;
-  plan_received(w);
+  plan_received(w, dtype);
   int64_t bytes = received_sum_bytes(w);
   if (!with_lse) bytes += received_lse_bytes(w.a) + prefix_part_bytes(w.a, plan_prefix(w.a, true).parts);
   return bytes;
@@ -113,7 +121,7 @@ int sta_received_attention(const void* q, const void* k, int dtype, int64_t batc
   a.k = prefix_rows_of(k, strides + 3);
   a.lengths = lengths;
   a.counts = counts;
-  plan_received(w);
+  plan_received(w, dtype);
   char* room = static_cast<char*>(workspace);
   w.sums = reinterpret_cast<float*>(room);
   room += received_sum_bytes(w);
@@ -125,8 +133,7 @@ int sta_received_attention(const void* q, const void* k, int dtype, int64_t batc
     a.lse = reinterpret_cast<float*>(room);
     room += received_lse_bytes(a);
     const PrefixPlan plan = plan_prefix(a, true);
-    a.part = reinterpret_cast<float*>(room);
-    a.parts = plan.parts;
+    set_parts(a, room, plan.parts);
     int st = run_prefix(a, plan, dtype, 0, s);
     if (st == STA_OK && plan.parts) st = join_rows(a, dtype, s);
     if (st != STA_OK) return st;

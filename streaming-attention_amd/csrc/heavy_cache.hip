@@ -27,11 +27,15 @@ struct HeavyArgs {
   float* weights;        // [streams][kv][pitch]
   int64_t* positions;    // [streams][kv][pitch], -1: no token
   unsigned long long* lowest;  // [streams][kv][2]: order of the lowest weight of the kept slots, and the slot
-  float* logits;         // [streams][heads][pitch]: this step's, times nothing
+  float* logits;         // [streams][heads][pitch]: this step's; unused by workgroups that keep them in LDS
   struct HeavyMove* moves;  // [streams][kv], of steps that several workgroups share
-  const float* prefix;   // [streams][heads][prefix_parts][dv + 2]: a shared prefix's partials
-  int prefix_parts;
+  // partials, of splits (r.part: sums) and of a shared prefix: sums [streams][heads][parts][part_pitch], maximum and sum of
+  // weights [streams][heads][parts][2]
+  float* stat;
+  const float *prefix, *prefix_stat;
+  int prefix_parts, part_pitch;
   int alone;             // a workgroup has a key head to itself and finishes it: one split, up to 16 query heads, no prefix
+  int local;             // such a workgroup keeps the logits in LDS
 };
 
 // What a step does to the slots of a key head.
@@ -128,18 +132,19 @@ __device__ __forceinline__ float heavy_base(const HeavyMove& m, int slot, float 
   return slot == m.slot || slot == m.hole ? 0.f : w;
 }
 
-// The increments of slots 4 at, .. + 3 from `queries` heads' logits, and what they do to the lowest kept weight; stat: the
-// heads' maxima, and their sums' inverses behind them.
-template <int ST>
+// The increments of slots 4 at, .. + 3 from `queries` heads' logits (`pitch` floats each), and what they do to the lowest
+// kept weight; stat: the heads' maxima, and their sums' inverses `stats` behind them.
+template <int ST, typename Logits>
 __device__ __forceinline__ unsigned long long heavy_grow(const HeavyArgs& a, const HeavyMove& m, int sh, int at,
-                                                         const float* logits, int queries, const float* stat, int pitch) {
+                                                         Logits logits, int64_t pitch, int queries, const float* stat,
+                                                         int stats) {
   constexpr float lift = win_weight_lift<ST>();
   float* row = a.weights + static_cast<int64_t>(sh) * a.pitch + 4 * at;
   const floatx4 w = *reinterpret_cast<const floatx4*>(row);
   floatx4 grown = floatx4{0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < queries; ++i) {
-    const floatx4 x = *reinterpret_cast<const floatx4*>(logits + static_cast<int64_t>(i) * a.pitch + 4 * at);
-    const float top = stat[i], inv = stat[pitch + i];
+    const floatx4 x = *reinterpret_cast<const floatx4*>(logits + i * pitch + 4 * at);
+    const float top = stat[i], inv = stat[stats + i];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float p = __builtin_amdgcn_exp2f(fmaf(x[j] - top, a.r.c, lift)) * inv;
@@ -167,6 +172,15 @@ __device__ __forceinline__ void heavy_positions(const HeavyArgs& a, const HeavyM
   if (m.slot >= 0) row[m.slot] = m.n;
 }
 
+__host__ __device__ constexpr int heavy_red_pitch(int nbv) { return 32 * nbv + 4; }
+// rows of logits in LDS, four banks apart
+__host__ __device__ constexpr int heavy_kept_pitch(int pitch) { return pitch + 4; }
+// dynamic LDS of a workgroup of heavy_attention_kernel
+__host__ __device__ constexpr int64_t heavy_lds_bytes(int group, int nbv, int pitch, bool local) {
+  const int64_t rows = group < 16 ? group : 16;
+  return 4 * rows * (4 * heavy_red_pitch(nbv) + (local ? heavy_kept_pitch(pitch) : 0));
+}
+
 // The walk of ring_attention_kernel over the slots that hold a token, with the logits put down for the weights' growth.  A
 // workgroup that is alone with a key head finishes it: outputs, weights, the next lowest one; else heavy_join_kernel does.
 template <int NBK, int NBV, int ST>
@@ -174,8 +188,9 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   const RingArgs& a = h.r;
   constexpr int PP = ST == F32 ? 1 : 2;  // planes of the weights, see ring_cache.hip
   constexpr int ES = ST == F32 ? 4 : 2, CT = 2 * NBV, W = RingTile<NBK, NBV, ST>::W;
-  constexpr int PITCH = 32 * NBV + 4;
-  __shared__ float red[4 * 16 * PITCH], red_m[4 * 16], red_l[4 * 16], stat[2 * 16];
+  constexpr int PITCH = heavy_red_pitch(NBV);
+  extern __shared__ float heavy_lds[];  // [4][queries][PITCH] for the waves' sums, then the logits if they are kept here
+  __shared__ float red_m[4 * 16], red_l[4 * 16], stat[2 * 16];
   __shared__ unsigned long long red_low[4];
   int id = blockIdx.x;
   const int split = id % a.nsplit;
@@ -183,11 +198,28 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   const int chunk = id % a.chunks, sh = id / a.chunks;
   const int s = sh / a.kv, hk = sh - s * a.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, lg = lane >> 4;
+  const int rows = min(16, a.group);  // of red
+  float *const red = heavy_lds, *const kept = heavy_lds + 4 * rows * PITCH;
+  const int kept_pitch = heavy_kept_pitch(h.pitch);
 
   const HeavyMove move = heavy_move(h, sh, a.append);
   const bool alone = h.alone;
   const int all = (move.held + 31) >> 5, per = (all + a.nsplit - 1) / a.nsplit;
-  const int t0 = split * per, t1 = t0 + per < all ? t0 + per : all;
+  const int t0 = split * per, t1 = t0 + per < all ? t0 + per : all, count = t1 - t0;
+  const int hole_tile = move.hole >= 0 ? move.hole >> 5 : -1;
+  const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
+  // Key heads begin at different tiles of their share: caches of equal lengths, walked in step, would else ask the same
+  // memory channels at a time.
+  const int turn = count > 0 ? (sh * 29) % count : 0;
+  auto tile = [&](int i) {
+    const int t = i + turn;
+    return t0 + (t < count ? t : t - count);
+  };
+  // a wave's first tile, before the new token is in if it does not go there
+  RingTile<NBK, NBV, ST> even;
+  const int first = wave < count ? tile(wave) : -1;
+  const bool early = first >= 0 && first != move.to >> 5 && first != move.slot >> 5;
+  if (early) even.load(a, tile0 + first, lane);
   if (a.append) {
     if (move.to >= 0 && (move.to >> 5) >= t0 && (move.to >> 5) < t1) heavy_keep<ST>(a, sh, move.from, move.to);
     if ((move.slot >> 5) >= t0 && (move.slot >> 5) < t1) ring_put<ST, ST>(a, s, hk, move.slot);
@@ -228,11 +260,9 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   constexpr float lift = win_weight_lift<ST>();  // fp16 weights, see ring_cache.hip
   const float room = win_weight_room<ST>() / a.c;
 
-  const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
   float* const logits = h.logits + (head0 + li) * h.pitch + 4 * lg;
-  // a tile's part of the sums; PART: not all of its slots hold a token
-  auto take = [&](const RingTile<NBK, NBV, ST>& cur, int t, auto part) {
-    constexpr bool PART = decltype(part)::value;
+  // a tile's part of the sums
+  auto take = [&](RingTile<NBK, NBV, ST>& cur, int t) {
     floatx4 x[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
@@ -245,21 +275,37 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
         x[half] = ring_mma<ST>(k, qf[b], x[half]);
       }
     }
-    // this lane's slots that hold a token: below `left`, but `hole`
-    const int left = move.held - 32 * t - 4 * lg, hole = move.hole - 32 * t - 4 * lg;
-    auto out = [&](int i) {
-      const int at = 16 * (i >> 2) + (i & 3);
-      return at >= left || at == hole;
-    };
+    // not all of the tile's slots hold a token: this lane's do below `left`, but `hole`
+    if (t == hole_tile || 32 * t + 32 > move.held) {
+      const int left = move.held - 32 * t - 4 * lg, hole = move.hole - 32 * t - 4 * lg;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = 16 * (i >> 2) + (i & 3);
+        const bool out = at >= left || at == hole;
+        x[i >> 2][i & 3] = out ? -__builtin_inff() : x[i >> 2][i & 3];
+        // values: whatever the slot holds
+        const uint32_t keep = out ? 0u : 0xffffffffu;
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) {
+          if constexpr (ST == F32)
+            cur.v[ct * W + i] &= keep;
+          else
+            cur.v[ct * W + (i >> 1)] &= i & 1 ? keep | 0x0000ffffu : keep | 0xffff0000u;
+        }
+      }
+    }
     float top = m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (PART && out(i)) x[i >> 2][i & 3] = -__builtin_inff();
-      top = fmaxf(top, x[i >> 2][i & 3]);
-    }
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, x[i >> 2][i & 3]);
     if (li < queries) {
-      *reinterpret_cast<floatx4*>(logits + 32 * t) = x[0];
-      *reinterpret_cast<floatx4*>(logits + 32 * t + 16) = x[1];
+      if (h.local) {
+        float* to = kept + li * kept_pitch + 4 * lg + 32 * t;
+        *reinterpret_cast<floatx4*>(to) = x[0];
+        *reinterpret_cast<floatx4*>(to + 16) = x[1];
+      } else {
+        *reinterpret_cast<floatx4*>(logits + 32 * t) = x[0];
+        *reinterpret_cast<floatx4*>(logits + 32 * t + 16) = x[1];
+      }
     }
     // the maximum moves, for all lanes of a query at once, when a weight would exceed 2^room
     if (__any(top > limit)) {
@@ -276,7 +322,6 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       p[i] = __builtin_amdgcn_exp2f(fmaf(x[i >> 2][i & 3] - m, a.c, lift));
-      if (PART && out(i)) p[i] = 0.f;
       l += p[i];
     }
     RingFrag<ST> pf[PP];
@@ -286,44 +331,23 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
       RingFrag<ST> v;
 #pragma unroll
       for (int i = 0; i < W; ++i) v.w[i] = cur.v[ct * W + i];
-      if constexpr (PART) {  // slots without a token: whatever they hold
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (out(i)) {
-            if constexpr (ST == F32)
-              v.w[i] = 0u;
-            else
-              v.w[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
-          }
-      }
 #pragma unroll
       for (int k = PP - 1; k >= 0; --k) acc[ct] = ring_mma<ST>(v, pf[k], acc[ct]);
     }
   };
-  // whole tiles, one ahead in registers, the two buffers in turn; then the hole's tile, and the last if it is not whole
+  // every fourth tile a wave, one ahead in registers, the two buffers in turn
   {
-    const int whole_end = t1 < (move.held >> 5) ? t1 : move.held >> 5;
-    const int hole_tile = move.hole >= 0 ? move.hole >> 5 : -1;
-    const bool skip = hole_tile >= t0 && hole_tile < whole_end;
-    const int end = whole_end - (skip ? 1 : 0);
-    auto tile = [&](int i) { return i + (skip && i >= hole_tile ? 1 : 0); };
-    RingTile<NBK, NBV, ST> even, odd;
-    int t = t0 + wave;
-    if (t < end) even.load(a, tile0 + tile(t), lane);
-    while (t < end) {
-      if (t + 4 < end) odd.load(a, tile0 + tile(t + 4), lane);
-      take(even, tile(t), std::false_type{});
-      t += 4;
-      if (t >= end) break;
-      if (t + 4 < end) even.load(a, tile0 + tile(t + 4), lane);
-      take(odd, tile(t), std::false_type{});
-      t += 4;
-    }
-    const int last = t0 <= whole_end && whole_end < t1 ? whole_end : -1;
-    const int mine = wave == 3 ? (hole_tile >= t0 && hole_tile < t1 ? hole_tile : -1) : (wave == 2 && last != hole_tile ? last : -1);
-    if (mine >= 0) {
-      even.load(a, tile0 + mine, lane);
-      take(even, mine, std::true_type{});
+    RingTile<NBK, NBV, ST> odd;
+    int i = wave;
+    if (i < count && !early) even.load(a, tile0 + tile(i), lane);
+    while (i < count) {
+      if (i + 4 < count) odd.load(a, tile0 + tile(i + 4), lane);
+      take(even, tile(i));
+      i += 4;
+      if (i >= count) break;
+      if (i + 4 < count) even.load(a, tile0 + tile(i + 4), lane);
+      take(odd, tile(i));
+      i += 4;
     }
   }
   l += __shfl_xor(l, 16);
@@ -332,7 +356,7 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   // the four waves' sums
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
-    *reinterpret_cast<floatx4*>(&red[(wave * 16 + li) * PITCH + 16 * ct + 4 * lg]) = acc[ct];
+    if (li < queries) *reinterpret_cast<floatx4*>(&red[(wave * rows + li) * PITCH + 16 * ct + 4 * lg]) = acc[ct];
   if (lg == 0) {
     red_m[wave * 16 + li] = prefix_top(m, l);
     red_l[wave * 16 + li] = l;
@@ -346,7 +370,7 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       const float lw = red_l[16 * w + i], f = lw == 0.f ? 0.f : __builtin_amdgcn_exp2f((red_m[16 * w + i] - top) * a.c);
-      if (lw != 0.f) sum = fmaf(f, red[(w * 16 + i) * PITCH + col], sum);
+      if (lw != 0.f) sum = fmaf(f, red[(w * rows + i) * PITCH + col], sum);
       den = fmaf(f, lw, den);
     }
     if (alone) {
@@ -356,19 +380,21 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
         stat[16 + i] = 1.f / den;
       }
     } else {
-      float* part = a.part + ((head0 + i) * a.nsplit + split) * (a.dv + 2);
-      part[col] = sum;
-      if (col == 0) {
-        part[a.dv] = prefix_top(top, den);
-        part[a.dv + 1] = den;
-      }
+      const int64_t part = (head0 + i) * a.nsplit + split;
+      a.part[part * h.part_pitch + col] = sum;
+      if (col == 0) *reinterpret_cast<floatx2*>(h.stat + 2 * part) = floatx2{prefix_top(top, den), den};
     }
   }
   if (!alone) return;
   __syncthreads();  // the logits of all waves, too
   unsigned long long low = HEAVY_NONE;
-  for (int at = threadIdx.x; 4 * at < move.held; at += 256)
-    low = heavy_min(low, heavy_grow<ST>(h, move, sh, at, h.logits + head0 * h.pitch, queries, stat, 16));
+  for (int at = threadIdx.x; 4 * at < move.held; at += 256) {
+    if (h.local)
+      low = heavy_min(low, heavy_grow<ST>(h, move, sh, at, static_cast<const float*>(kept), kept_pitch, queries, stat, 16));
+    else
+      low = heavy_min(low, heavy_grow<ST>(h, move, sh, at, static_cast<const float*>(h.logits + head0 * h.pitch), h.pitch,
+                                          queries, stat, 16));
+  }
   low = heavy_least<256>(low, red_low);
   if (threadIdx.x == 0) {
     heavy_positions(h, move, sh);
@@ -383,45 +409,58 @@ constexpr int HEAVY_SPLITS = 1024, HEAVY_SLOTS = 2048, HEAVY_HEADS = 512;
 template <int ST>
 __global__ __launch_bounds__(512) void heavy_join_kernel(const HeavyArgs h, int outputs, int ranges) {
   const RingArgs& a = h.r;
+  constexpr int AHEAD = 16;
   __shared__ float weight[HEAVY_SPLITS], red[4 * 128], wave_red[8], stat[2 * HEAVY_HEADS];
   __shared__ unsigned long long red_low[8];
-  const int pitch = a.dv + 2, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const int total = a.nsplit + h.prefix_parts;
-  auto partial = [&](int64_t head, int j) {
-    return j < a.nsplit ? a.part + (head * a.nsplit + j) * pitch : h.prefix + (head * h.prefix_parts + j - a.nsplit) * pitch;
+  // maximum and sum of weights of a head's partial, and a column of its sums; partials behind the last have none
+  auto stat_of = [&](int64_t head, int j) {
+    const float* at = j < a.nsplit ? h.stat + 2 * (head * a.nsplit + j) : h.prefix_stat + 2 * (head * h.prefix_parts + j - a.nsplit);
+    return j < total ? *reinterpret_cast<const floatx2*>(at) : floatx2{-__builtin_inff(), 0.f};
+  };
+  auto sum_of = [&](int64_t head, int j, int col) {
+    return j < a.nsplit ? a.part[(head * a.nsplit + j) * h.part_pitch + col]
+                        : h.prefix[(head * h.prefix_parts + j - a.nsplit) * h.part_pitch + col];
   };
   if (static_cast<int>(blockIdx.x) < outputs) {
     const int64_t head = blockIdx.x;
     const int s = blockIdx.x / a.heads, hh = blockIdx.x - s * a.heads, sh = s * a.kv + hh / a.group;
-    const int col = threadIdx.x & 127, group = threadIdx.x >> 7;
-    float top = -__builtin_inff(), den = 0.f;
-    for (int i = threadIdx.x; i < total; i += 512) top = fmaxf(top, partial(head, i)[a.dv]);
+    const int col = t & 127, group = t >> 7;
+    // the partials' loads are under way before their weights are known
+    float ahead[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) ahead[i] = col < a.dv && group + 4 * i < total ? sum_of(head, group + 4 * i, col) : 0.f;
+    const floatx2 mine[2] = {stat_of(head, t), stat_of(head, t + 512)};
+    const int held = h.moves[sh].held;
+    float top = fmaxf(mine[0][0], mine[1][0]), den = 0.f;
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     if (lane == 0) wave_red[wave] = top;
     __syncthreads();
     for (int i = 0; i < 8; ++i) top = fmaxf(top, wave_red[i]);
-    for (int i = threadIdx.x; i < total; i += 512) {
-      const float* part = partial(head, i);
-      const float li = part[a.dv + 1], f = li == 0.f ? 0.f : __builtin_amdgcn_exp2f((part[a.dv] - top) * a.c);
-      weight[i] = f;
-      den = fmaf(f, li, den);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float f = mine[k][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f((mine[k][0] - top) * a.c);
+      weight[t + 512 * k] = f;
+      den = fmaf(f, mine[k][1], den);
     }
     for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
     __syncthreads();
     if (lane == 0) wave_red[wave] = den;
     float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) sum = fmaf(weight[group + 4 * i], ahead[i], sum);
     if (col < a.dv) {
 #pragma unroll 8
-      for (int i = group; i < total; i += 4) sum = fmaf(weight[i], partial(head, i)[col], sum);
+      for (int i = group + 4 * AHEAD; i < total; i += 4) sum = fmaf(weight[i], sum_of(head, i, col), sum);
     }
-    red[threadIdx.x] = sum;
+    red[t] = sum;
     __syncthreads();
-    if (static_cast<int>(threadIdx.x) < a.dv) {
+    if (t < a.dv) {
       den = 0.f;
       for (int i = 0; i < 8; ++i) den += wave_red[i];
-      sum = red[threadIdx.x] + red[128 + threadIdx.x] + red[256 + threadIdx.x] + red[384 + threadIdx.x];
-      const bool some = h.moves[sh].held || den != 0.f;
-      store_elem(a.out, head * a.dv + threadIdx.x, ST, some ? sum / den : 0.f);
+      sum = red[t] + red[128 + t] + red[256 + t] + red[384 + t];
+      store_elem(a.out, head * a.dv + t, ST, held || den != 0.f ? sum / den : 0.f);
     }
     return;
   }
@@ -433,23 +472,27 @@ __global__ __launch_bounds__(512) void heavy_join_kernel(const HeavyArgs h, int 
   if (range * HEAVY_SLOTS < move.held) {
     for (int i = wave; i < a.group; i += 8) {  // a wave a head: its maximum and sum
       float top = -__builtin_inff(), den = 0.f;
-      for (int j = lane; j < total; j += 64) top = fmaxf(top, partial(head0 + i, j)[a.dv]);
-      for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
       for (int j = lane; j < total; j += 64) {
-        const float* part = partial(head0 + i, j);
-        const float lj = part[a.dv + 1];
-        den = fmaf(lj == 0.f ? 0.f : __builtin_amdgcn_exp2f((part[a.dv] - top) * a.c), lj, den);
+        const floatx2 x = stat_of(head0 + i, j);
+        const float up = fmaxf(top, x[0]);
+        den = (den == 0.f ? 0.f : den * __builtin_amdgcn_exp2f((top - up) * a.c)) +
+              (x[1] == 0.f ? 0.f : x[1] * __builtin_amdgcn_exp2f((x[0] - up) * a.c));
+        top = up;
       }
+      float up = top;
+      for (int o = 32; o > 0; o >>= 1) up = fmaxf(up, __shfl_xor(up, o));
+      den = den == 0.f ? 0.f : den * __builtin_amdgcn_exp2f((top - up) * a.c);
       for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
       if (lane == 0) {
-        stat[i] = top;
+        stat[i] = up;
         stat[HEAVY_HEADS + i] = 1.f / den;
       }
     }
     __syncthreads();
     const int at = range * (HEAVY_SLOTS / 4) + threadIdx.x;
     if (4 * at < move.held)
-      low = heavy_grow<ST>(h, move, sh, at, h.logits + head0 * h.pitch, a.group, stat, HEAVY_HEADS);
+      low = heavy_grow<ST>(h, move, sh, at, static_cast<const float*>(h.logits + head0 * h.pitch), h.pitch, a.group, stat,
+                           HEAVY_HEADS);
   }
   low = heavy_least<512>(low, red_low);
   if (threadIdx.x == 0) {
@@ -501,12 +544,14 @@ __device__ __forceinline__ int heavy_take(const HeavyFill& f, int s) {
 __device__ __forceinline__ float heavy_given(float w) { return w == w ? w + 0.f : 0.f; }
 
 // Which rows stay, by a workgroup of 1024 threads a key head: the last `recent`, and of the others the `kept` of the
-// largest weights, of equal ones the first.  Four passes over the weights find the smallest that stays, 8 bits of its
-// order at a time (the highest byte first, among those that agree with it so far); one more puts the rows that stay down in
-// their order.
+// largest weights, of equal ones the first.  Three passes over the weights find the smallest that stays, 11 bits of its
+// order at a time (the highest first, among those that agree with it so far): the weights of a prompt lie within a few powers
+// of two, so that bins of 8 bits, the sign and 7 of the exponent's, would all be added to in one place.  One more pass puts the
+// rows that stay down in their order.  The first 16384 weights are held in registers.  16 x 8 key heads of 8192 rows: 20 us.
 __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFill f) {
   const HeavyArgs& h = f.h;
-  __shared__ int bins[256], wave_sum[2][16], chosen[2];
+  constexpr int HOLD = 16, BINS = 2048;
+  __shared__ int bins[BINS], wave_sum[2][16], chosen[2];
   __shared__ unsigned long long red_low[16];
   const int sh = blockIdx.x, s = sh / h.r.kv, n = heavy_take(f, s), t = threadIdx.x, lane = t & 63, wave = t >> 6;
   if (n == 0) return;
@@ -515,43 +560,49 @@ __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFi
   float* weights = h.weights + static_cast<int64_t>(sh) * h.pitch;
   int64_t* positions = h.positions + static_cast<int64_t>(sh) * h.pitch;
   const int older = n > h.recent ? n - h.recent : 0;
+  float hold[HOLD];
+#pragma unroll
+  for (int j = 0; j < HOLD; ++j) hold[j] = t + 1024 * j < older ? heavy_given(given[t + 1024 * j]) : 0.f;
 
   uint32_t least = 0u;  // the order of the smallest weight that stays
   int equal = 0x7fffffff;  // how many of those equal to it stay
   if (older > h.kept) {
     int want = h.kept;  // among those that agree so far
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (t < 256) bins[t] = 0;
+    for (int shift = 21; shift >= -1; shift -= 11) {
+      const int low = shift < 0 ? 0 : shift, bits = shift < 0 ? 10 : 11;  // 11 + 11 + 10 bits
+      const uint32_t mask = (1u << bits) - 1u;
+      bins[t] = bins[t + 1024] = 0;
       __syncthreads();
-      const uint32_t high = shift == 24 ? 0u : least >> (shift + 8);
-      for (int i = t; i < older; i += 1024) {
-        const uint32_t u = heavy_order(heavy_given(given[i]));
-        if (shift == 24 || u >> (shift + 8) == high) atomicAdd(&bins[(u >> shift) & 255u], 1);
+      auto put = [&](float w) {
+        const uint32_t u = heavy_order(w);
+        if (low + bits == 32 || u >> (low + bits) == least >> (low + bits)) atomicAdd(&bins[(u >> low) & mask], 1);
+      };
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j)
+        if (t + 1024 * j < older) put(hold[j]);
+      for (int i = t + 1024 * HOLD; i < older; i += 1024) put(heavy_given(given[i]));
+      __syncthreads();
+      // the highest bin with `want` at or above it: sums from above, two bins a thread
+      const int first = BINS - 1 - 2 * t, part[2] = {bins[first], bins[first - 1]};
+      int before = part[0] + part[1];
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(before, o);
+        if (lane >= o) before += y;
+      }
+      if (lane == 63) wave_sum[0][wave] = before;
+      __syncthreads();
+      before -= part[0] + part[1];
+      for (int j = 0; j < wave; ++j) before += wave_sum[0][j];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (before < want && before + part[j] >= want) {
+          chosen[0] = first - j;
+          chosen[1] = want - before;
+        }
+        before += part[j];
       }
       __syncthreads();
-      // the highest byte with `want` at or above it: sums from above, 4 bins a lane of the first wave
-      if (wave == 0) {
-        int part[4], sum = 0;
-        for (int j = 0; j < 4; ++j) {
-          part[j] = bins[255 - 4 * lane - j];
-          sum += part[j];
-        }
-        int before = sum;
-        for (int o = 1; o < 64; o <<= 1) {
-          const int y = __shfl_up(before, o);
-          if (lane >= o) before += y;
-        }
-        before -= sum;
-        for (int j = 0; j < 4; ++j) {
-          if (before < want && before + part[j] >= want) {
-            chosen[0] = 255 - 4 * lane - j;
-            chosen[1] = want - before;
-          }
-          before += part[j];
-        }
-      }
-      __syncthreads();
-      least |= static_cast<uint32_t>(chosen[0]) << shift;
+      least |= static_cast<uint32_t>(chosen[0]) << low;
       want = chosen[1];
       __syncthreads();
     }
@@ -560,9 +611,7 @@ __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFi
   // the rows that stay, in their order
   unsigned long long low = HEAVY_NONE;
   int taken = 0, ties = 0;
-  for (int i0 = 0; i0 < older; i0 += 1024) {
-    const int i = i0 + t;
-    const float w = i < older ? heavy_given(given[i]) : 0.f;
+  auto place = [&](int i, float w) {
     const uint32_t u = heavy_order(w);
     const bool tie = i < older && u == least && equal != 0x7fffffff;
     const unsigned long long ballot = __ballot(tie), below = (1ull << lane) - 1ull;
@@ -592,7 +641,11 @@ __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFi
       positions[slot] = i;
       low = heavy_min(low, heavy_key(w, slot));
     }
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < HOLD; ++j)
+    if (1024 * j < older) place(1024 * j + t, hold[j]);
+  for (int i0 = 1024 * HOLD; i0 < older; i0 += 1024) place(i0 + t, i0 + t < older ? heavy_given(given[i0 + t]) : 0.f);
   for (int slot = h.ring + taken + t; slot < h.pitch; slot += 1024) {
     token[slot] = -1;
     weights[slot] = 0.f;
@@ -626,14 +679,29 @@ __global__ __launch_bounds__(256) void heavy_fill_kernel(const HeavyFill f) {
   ring_fill<ST, ST>(a, s, hk, tile, token);
 }
 
-// The slots' rows as they are.
+// The slots as they are: rows, positions and weights.
+struct HeavyItems {
+  void *keys, *values;   // [streams][kv][slots][d | dv]
+  int64_t* positions;    // [streams][kv][slots]
+  float* weights;
+};
 template <int ST>
-__global__ __launch_bounds__(256) void heavy_items_kernel(const HeavyArgs h, void* keys, void* values) {
+__global__ __launch_bounds__(256) void heavy_items_kernel(const HeavyArgs h, const HeavyItems to) {
   int sh, tile;
   if (!ring_place(h.r, sh, tile)) return;
-  const int64_t* positions = h.positions + static_cast<int64_t>(sh) * h.pitch + 32 * tile;
-  const bool some = __syncthreads_or(threadIdx.x < 32 && positions[threadIdx.x] >= 0);
-  ring_rows_out<ST, ST>(h.r, sh, tile, some, [&](int r) { return positions[r] >= 0; }, keys, values);
+  const int64_t at = static_cast<int64_t>(sh) * h.pitch + 32 * tile;
+  __shared__ int there[32];
+  if (threadIdx.x < 32) {
+    const int64_t p = h.positions[at + threadIdx.x];
+    there[threadIdx.x] = p >= 0;
+    if (32 * tile + static_cast<int>(threadIdx.x) < h.r.slots) {
+      const int64_t slot = static_cast<int64_t>(sh) * h.r.slots + 32 * tile + threadIdx.x;
+      to.positions[slot] = p;
+      to.weights[slot] = h.weights[at + threadIdx.x];
+    }
+  }
+  const bool some = __syncthreads_or(threadIdx.x < 32 && there[threadIdx.x]);
+  ring_rows_out<ST, ST>(h.r, sh, tile, some, [&](int r) { return there[r] != 0; }, to.keys, to.values);
 }
 
 }  // namespace sta

@@ -19,12 +19,21 @@ int launch_heavy(const sta::HeavyArgs& h, hipStream_t s) {
   const int64_t join = outputs + static_cast<int64_t>(a.streams) * a.kv * ranges;
   if (grid <= 0 || grid > sta::MAX_GROUPS || (!h.alone && join > sta::MAX_GROUPS / 2)) return STA_ERR_SHAPE;
   const dim3 g(static_cast<unsigned>(grid));
-  switch (a.nbv) {
-    case 1: hipLaunchKernelGGL((sta::heavy_attention_kernel<NBK, 1, ST>), g, dim3(256), 0, s, h); break;
-    case 2: hipLaunchKernelGGL((sta::heavy_attention_kernel<NBK, 2, ST>), g, dim3(256), 0, s, h); break;
-    case 3: hipLaunchKernelGGL((sta::heavy_attention_kernel<NBK, 3, ST>), g, dim3(256), 0, s, h); break;
-    default: hipLaunchKernelGGL((sta::heavy_attention_kernel<NBK, 4, ST>), g, dim3(256), 0, s, h);
-  }
+  const int lds = static_cast<int>(sta::heavy_lds_bytes(a.group, a.nbv, h.pitch, h.local));
+  auto launch = [&](auto kernel) {
+    if (lds > 64 * 1024 - 1024) {  // with the kernel's own arrays past 64 KB
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e != hipSuccess) return hip_status(e);
+    }
+    hipLaunchKernelGGL(kernel, g, dim3(256), lds, s, h);
+    return check_launch();
+  };
+  const int st = a.nbv == 1   ? launch(sta::heavy_attention_kernel<NBK, 1, ST>)
+                 : a.nbv == 2 ? launch(sta::heavy_attention_kernel<NBK, 2, ST>)
+                 : a.nbv == 3 ? launch(sta::heavy_attention_kernel<NBK, 3, ST>)
+                              : launch(sta::heavy_attention_kernel<NBK, 4, ST>);
+  if (st != STA_OK) return st;
   if (!h.alone)
     hipLaunchKernelGGL((sta::heavy_join_kernel<ST>), dim3(static_cast<unsigned>(join)), dim3(512), 0, s, h,
                        static_cast<int>(outputs), static_cast<int>(ranges));

@@ -1,8 +1,7 @@
 // Launches of the attention over a shared prefix and of the received weights for one configuration.  The build compiles
 // this unit once per padded width P (32, 64, 96, 128; keys and values both) and element type IN (0 fp32, 1 bf16, 2 fp16),
 // given as -DSTA_PREFIX_P= and -DSTA_PREFIX_IN=.
-#include "api_common.hpp"
-#include "prefix_attn.hip"
+#include "prefix_plan.hpp"
 
 #if !defined(STA_PREFIX_P) || !defined(STA_PREFIX_IN)
 #error "launch_prefix.hip is compiled with -DSTA_PREFIX_P= -DSTA_PREFIX_IN="
@@ -10,38 +9,61 @@
 
 namespace sta_api {
 
-// The rows of one walk: finished, or their partials.  values 0: statistics alone.
+// The walks of a plan; values 0: statistics alone (one walk).
 template <int P, int IN>
-int launch_prefix(const sta::PrefixArgs& a, const sta::PrefixWalk& w, int share, int values, hipStream_t s) {
-  const int64_t grid = static_cast<int64_t>(a.kv) * (a.batch / w.span) * w.tiles * w.nsplit;
-  if (grid <= 0 || grid > sta::MAX_GROUPS) return STA_ERR_SHAPE;
-  auto launch = [&](auto kernel, int lds) {
+int launch_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int values, hipStream_t s) {
+  int64_t grid[2] = {0, 0};
+  for (int i = 0; i < p.walks; ++i)
+    grid[i] = static_cast<int64_t>(a.kv) * (a.batch / p.walk[i].span) * p.walk[i].tiles * p.walk[i].nsplit;
+  if (grid[0] <= 0 || grid[0] + grid[1] > sta::MAX_GROUPS) return STA_ERR_SHAPE;
+  const dim3 g(static_cast<unsigned>(grid[0] + grid[1]));
+  auto launch = [&](auto kernel, int lds, auto... args) {
     if (lds > 64 * 1024 - 16) {  // with the kernels' own few bytes past 64 KB
       const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
       if (e != hipSuccess) return hip_status(e);
     }
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(256), lds, s, a, w);
+    hipLaunchKernelGGL(kernel, g, dim3(256), lds, s, a, args...);
     return check_launch();
   };
-  constexpr int wide = sta::win_lds_bytes<P, IN, false>(), shared = sta::win_lds_bytes<P, IN, true>();
-  if (values) {
-    return share ? launch(sta::prefix_attention_kernel<P, IN, true, true>, shared)
-                 : launch(sta::prefix_attention_kernel<P, IN, false, true>, wide);
+  constexpr int shared = sta::win_lds_bytes<P, IN, true>(), rows = 4 * sta::win_join_floats<P>();
+  const int stage = sta::win_lds_bytes<P, IN, false>(), wide = a.parts && values && rows > stage ? rows : stage;
+  if (p.walks == 2) {
+    const int both = wide > shared ? wide : shared;
+    const int ga = static_cast<int>(grid[0]), gb = static_cast<int>(grid[1]);
+    if (p.share[0] && p.share[1])
+      return launch(sta::prefix_walks_kernel<P, IN, true, true>, shared, p.walk[0], p.walk[1], ga, gb);
+    if (p.share[1]) return launch(sta::prefix_walks_kernel<P, IN, false, true>, both, p.walk[0], p.walk[1], ga, gb);
+    return launch(sta::prefix_walks_kernel<P, IN, false, false>, wide, p.walk[0], p.walk[1], ga, gb);
   }
-  return share ? launch(sta::prefix_attention_kernel<P, IN, true, false>, shared)
-               : launch(sta::prefix_attention_kernel<P, IN, false, false>, wide);
+  if (values) {
+    return p.share[0] ? launch(sta::prefix_attention_kernel<P, IN, true, true>, shared, p.walk[0])
+                      : launch(sta::prefix_attention_kernel<P, IN, false, true>, wide, p.walk[0]);
+  }
+  return p.share[0] ? launch(sta::prefix_attention_kernel<P, IN, true, false>, shared, p.walk[0])
+                    : launch(sta::prefix_attention_kernel<P, IN, false, false>, wide, p.walk[0]);
 }
 
 template <int P, int IN>
 int launch_received(const sta::ReceivedArgs& w, hipStream_t s) {
   const int64_t grid = static_cast<int64_t>(w.a.kv) * w.a.batch * w.tiles * w.nsplit;
   if (grid <= 0 || grid > sta::MAX_GROUPS) return STA_ERR_SHAPE;
-  hipLaunchKernelGGL((sta::received_kernel<P, IN>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, w);
+  const dim3 g(static_cast<unsigned>(grid));
+  if (w.few) {
+    const int lds = sta::received_few_bytes<P, IN>((w.a.n * w.a.group + 31) / 32 * 32);
+    if (lds > 64 * 1024) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sta::received_few_kernel<P, IN>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+      if (e != hipSuccess) return hip_status(e);
+    }
+    hipLaunchKernelGGL((sta::received_few_kernel<P, IN>), g, dim3(256), lds, s, w);
+  } else {
+    hipLaunchKernelGGL((sta::received_kernel<P, IN>), g, dim3(256), 0, s, w);
+  }
   return check_launch();
 }
 
-template int launch_prefix<STA_PREFIX_P, STA_PREFIX_IN>(const sta::PrefixArgs&, const sta::PrefixWalk&, int, int, hipStream_t);
+template int launch_prefix<STA_PREFIX_P, STA_PREFIX_IN>(const sta::PrefixArgs&, const PrefixPlan&, int, hipStream_t);
 template int launch_received<STA_PREFIX_P, STA_PREFIX_IN>(const sta::ReceivedArgs&, hipStream_t);
 
 }  // namespace sta_api

@@ -24,8 +24,9 @@ struct PrefixArgs {
   const int *lengths, *counts, *prefix_lengths;  // [batch], [batch], [sets], or null
   void* out;             // [batch][heads][n][dv]
   float* lse;            // [batch][heads][n]: log2 of the row's sum of weights, or null
-  float* part;           // [batch][heads][n][parts][dv + 2]: sums, then maximum and sum of weights
-  int parts;             // 0: rows are finished by one workgroup
+  float* part;           // [batch][heads][n][parts][pitch]: sums, on 16 bytes
+  float* stat;           // [batch][heads][n][parts][2]: maximum and sum of weights
+  int parts, pitch;      // parts 0: rows are finished by one workgroup; pitch: dv in whole units of 4
 };
 
 // One launch: which rows lie together, what they see, how their keys are dealt out.
@@ -52,13 +53,21 @@ __device__ __forceinline__ int prefix_rows(const PrefixArgs& a, int set) {
 // a partial of a row without weights: a maximum of -inf
 __device__ __forceinline__ float prefix_top(float m, float l) { return l == 0.f ? -__builtin_inff() : m; }
 
+// log2 of a row's sum of weights.  The sum's power of two goes into the whole number, so that the logarithm is taken near 1
+// and rounds at its size there: of a sum of 2^13 it is off by up to 1e-6, much the same for neighbouring rows, so that it
+// stays in the sums over them (received weights of 16384 rows: errors of 2.9e-7, so 5e-8).
+template <int IN>
+__device__ __forceinline__ float prefix_lse(float top, float den, float c) {
+  const int e = __builtin_amdgcn_frexp_expf(den);
+  return fmaf(top, c, static_cast<float>(e) - win_weight_lift<IN>()) + __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(den));
+}
+
 template <int P, int IN, bool SHARE, bool VALUES, bool CAREFUL>
-__device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk& w, int again) {
+__device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk& w, int id, int again) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
                 MT = P / 32, STEP = SHARE ? 4 : 1;
   extern __shared__ uint4 win_lds[];
   // the tiles of a unit, then the units of a key head next to each other: they read the same keys
-  int id = xcd_remap(blockIdx.x, gridDim.x);
   const int tile = w.tiles - 1 - id % w.tiles;
   id /= w.tiles;
   const int split = id % w.nsplit;
@@ -113,10 +122,11 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
   }
   const bool any = w.own ? own_end > 0 : r0 < w.span * per;
   const int tiles_p = any ? (rows_p + BK - 1) / BK : 0, all_tiles = tiles_p + (own_end + BK - 1) / BK;
-  const int share = (all_tiles + w.nsplit - 1) / w.nsplit;
-  const int t0 = split * share, t1 = t0 + share < all_tiles ? t0 + share : all_tiles;
+  // Every nsplit-th tile: workgroups that walk in step are at neighbouring rows, and not at round distances, which would
+  // ask the same memory channels at a time.
+  const int own_first = (split + w.nsplit - tiles_p % w.nsplit) % w.nsplit;  // of the own tokens' tiles
 
-  if (t0 < t1) {
+  if (split < all_tiles) {
     WinFrag<IN> qf[P / 16];
     const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
     const char* qrow = rows_at<ES>(a.q, mine.b, mine.h, mine.i);
@@ -126,10 +136,11 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
       win_keep<IN>(qf[s], mine.live);
     }
 #pragma unroll 1
-    for (int seg = t0 < tiles_p ? 0 : 1; seg < (t1 > tiles_p ? 2 : 1); ++seg) {
+    for (int seg = 0; seg < 2; ++seg) {
       const Rows kr = seg ? a.k : a.pk, vr = seg ? a.v : a.pv;
       const int rb = seg ? b0 : b0 / a.per_set, end = seg ? own_end : rows_p;
-      const int lo = seg ? (t0 > tiles_p ? t0 - tiles_p : 0) : t0, hi = seg ? t1 - tiles_p : (t1 < tiles_p ? t1 : tiles_p);
+      const int lo = seg ? own_first : split, hi = seg ? all_tiles - tiles_p : tiles_p, step = STEP * w.nsplit;
+      if (lo >= hi) continue;
       // the last key that a lane's row, the wave's first and its last one see
       const int lim = seg ? mine.lim : rows_p - 1;
       const int lim_lo = seg ? base + w0 / a.group : rows_p - 1;
@@ -142,16 +153,16 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
         kst.load(rows_at<ES>(kr, rb, hk, row), end - row);
         if constexpr (VALUES) vst.load(rows_at<ES>(vr, rb, hk, row), end - row);
       };
-      const int start = lo + (SHARE ? wave : 0);
+      const int start = lo + (SHARE ? wave * w.nsplit : 0);
       if (AHEAD && start < hi) load(start);
-      for (int it = start; it < hi; it += STEP) {
+      for (int it = start; it < hi; it += step) {
         if (!AHEAD) load(it);
         win_sync<SHARE>();
         const int key0 = it * BK;
         kst.put(ks, end - key0);
         if constexpr (VALUES) vst.put(vs, end - key0);
         win_sync<SHARE>();
-        if (AHEAD && it + STEP < hi) load(it + STEP);
+        if (AHEAD && it + step < hi) load(it + step);
         if (key0 > lim_hi) continue;
         const bool all = key0 + BK - 1 <= lim_lo;
         floatx16 x[NSUB];
@@ -206,10 +217,14 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
             else
               x[sub][i] = __builtin_amdgcn_exp2f(fmaf(x[sub][i], a.c, -mc));
           }
+        // a tile's weights first: long rows' sums lose less
 #pragma unroll
-        for (int sub = 0; sub < NSUB; ++sub)
+        for (int sub = 0; sub < NSUB; ++sub) {
+          float sum = x[sub][0];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) l += x[sub][i];
+          for (int i = 1; i < 16; ++i) sum += x[sub][i];
+          l += sum;
+        }
         if constexpr (VALUES) {
           if (CAREFUL && !all) {
 #pragma unroll
@@ -231,32 +246,24 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
     l += __shfl_xor(l, 32);
   }
 
-  // four sums of a row at column col, its maximum and sum of weights
-  auto store4 = [&](const Place& x, int col, float inv, float y0, float y1, float y2, float y3) {
-    if (col >= a.dv) return;
-    if (a.parts) {
-      float* to = a.part + (x.at * a.parts + w.first + split) * (a.dv + 2) + col;
-      to[0] = y0;
-      if (col + 1 < a.dv) to[1] = y1;
-      if (col + 2 < a.dv) to[2] = y2;
-      if (col + 3 < a.dv) to[3] = y3;
-    } else {
-      win_store4<IN>(a.out, x.at * a.dv, col, a.dv, x.live ? y0 * inv : 0.f, x.live ? y1 * inv : 0.f,
-                     x.live ? y2 * inv : 0.f, x.live ? y3 * inv : 0.f);
-    }
+  // four sums of a row at column col (below dv), its maximum and sum of weights
+  auto store4 = [&](const Place& x, int col, float inv, const floatx4& y) {
+    if (a.parts)
+      *reinterpret_cast<floatx4*>(a.part + (x.at * a.parts + w.first + split) * a.pitch + col) = y;
+    else
+      win_store4<IN>(a.out, x.at * a.dv, col, a.dv, x.live ? y[0] * inv : 0.f, x.live ? y[1] * inv : 0.f,
+                     x.live ? y[2] * inv : 0.f, x.live ? y[3] * inv : 0.f);
   };
   auto store_sums = [&](const Place& x, float top, float den) {
     if (a.parts) {
-      float* to = a.part + (x.at * a.parts + w.first + split) * (a.dv + 2) + a.dv;
-      to[0] = prefix_top(top, den);
-      to[1] = den;
+      *reinterpret_cast<floatx2*>(a.stat + (x.at * a.parts + w.first + split) * 2) = floatx2{prefix_top(top, den), den};
     } else if (a.lse) {
-      a.lse[x.at] = x.live ? top * a.c - win_weight_lift<IN>() + __builtin_amdgcn_logf(den) : 0.f;
+      a.lse[x.at] = x.live ? prefix_lse<IN>(top, den, a.c) : 0.f;
     }
   };
   // a sum of weights that is not finite, or none though the row sees a key of the workgroup's share
   auto wrong = [&](const Place& x, float den) {
-    const bool sees = t0 < tiles_p || (t0 < t1 && (t0 - tiles_p) * BK <= x.lim);
+    const bool sees = split < tiles_p || (split < all_tiles && own_first * BK <= x.lim);
     return !win_finite(den) || (sees && !(den > 0.f));
   };
 
@@ -297,8 +304,10 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
     if (x.in && (CAREFUL ? again : !bad)) {
       if constexpr (VALUES) {
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
-          store4(x, 32 * j + 4 * (threadIdx.x & 7), inv, o[j][0], o[j][1], o[j][2], o[j][3]);
+        for (int j = 0; j < MT; ++j) {
+          const int col = 32 * j + 4 * (threadIdx.x & 7);
+          if (col < a.dv) store4(x, col, inv, o[j]);
+        }
       }
       if ((threadIdx.x & 7) == 0) store_sums(x, top, den);
     }
@@ -318,162 +327,354 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
     }
   }
   bad |= __shfl_xor(bad, 32);
-  if (mine.in && (CAREFUL ? again : !bad)) {
-    if constexpr (VALUES) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          store4(mine, 32 * mt + 8 * r + 4 * hh, inv, acc[mt][4 * r], acc[mt][4 * r + 1], acc[mt][4 * r + 2],
-                 acc[mt][4 * r + 3]);
+  const bool store = mine.in && (CAREFUL ? again : !bad);
+  if (VALUES && a.parts) {
+    // Partials by whole rows, through LDS: stored from the lanes that have them, 16 bytes here and there, they cost as much
+    // as eight tiles of keys (64 x 32 heads over 32768 rows, 32 shares: 77 us, so 56)
+    float* red = reinterpret_cast<float*>(win_lds);
+    __syncthreads();
+    win_join_put<P>(red, acc, wave, lane);
+    win_sync<true>();
+    constexpr int UNITS = P / 4;
+#pragma unroll 4
+    for (int i = 0; i < UNITS / 2; ++i) {
+      const int unit = 64 * i + lane, r = unit / UNITS, col = 4 * (unit % UNITS);
+      const int lo = __shfl(static_cast<int>(mine.at), r), hi = __shfl(static_cast<int>(mine.at >> 32), r);
+      const bool row = __shfl(static_cast<int>(store), r);
+      Place x = mine;
+      x.at = static_cast<int64_t>(hi) << 32 | static_cast<uint32_t>(lo);
+      if (row && col < a.dv) store4(x, col, 1.f, *reinterpret_cast<floatx4*>(&red[(wave * 32 + r) * (P + 4) + col]));
     }
-    if (hh == 0) store_sums(mine, m, l);
+  } else if (VALUES && store) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int col = 32 * mt + 8 * r + 4 * hh;
+        if (col < a.dv)
+          store4(mine, col, inv, floatx4{acc[mt][4 * r], acc[mt][4 * r + 1], acc[mt][4 * r + 2], acc[mt][4 * r + 3]});
+      }
   }
+  if (store && hh == 0) store_sums(mine, m, l);
   return bad;
 }
 
 template <int P, int IN, bool SHARE, bool VALUES>
 __global__ __launch_bounds__(256, (win_row_waves<P, IN, SHARE>())) void prefix_attention_kernel(const PrefixArgs a,
                                                                                                const PrefixWalk w) {
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
   win_passes([&](auto second, int again) {
-    return prefix_pass<P, IN, SHARE, VALUES, decltype(second)::value>(a, w, again);
+    return prefix_pass<P, IN, SHARE, VALUES, decltype(second)::value>(a, w, id, again);
   });
 }
 
-// The partials of a row: a workgroup of 128 threads a row, a thread a column.
+// Both walks of a batch of few rows in one launch: that over the prefix is bound by products and by latency, that over the
+// own tokens by memory.  64 x 32 heads, 128 wide, 32768 shared and up to 1024 own rows: 56 and 32 us one after the other, 78
+// together, with the prefix's workgroups first (98 with the two in turn).
+template <int P, int IN, bool SHARE_A, bool SHARE_B>
+__global__ __launch_bounds__(256, (win_row_waves<P, IN, SHARE_B>() < win_row_waves<P, IN, SHARE_A>()
+                                       ? win_row_waves<P, IN, SHARE_B>()
+                                       : win_row_waves<P, IN, SHARE_A>())) void
+prefix_walks_kernel(const PrefixArgs a, const PrefixWalk wa, const PrefixWalk wb, int grid_a, int grid_b) {
+  // each walk's neighbours on one XCD, the first walk's workgroups before the second's
+  const int xcds = grid_a % 8 == 0 && grid_b % 8 == 0 ? 8 : 1, xcd = blockIdx.x % xcds, slot = blockIdx.x / xcds;
+  const int ga = grid_a / xcds, gb = grid_b / xcds;
+  const bool first = slot < ga;
+  if (first) {
+    const int id = xcd * ga + slot;
+    win_passes([&](auto second, int again) {
+      return prefix_pass<P, IN, SHARE_A, true, decltype(second)::value>(a, wa, id, again);
+    });
+  } else {
+    const int id = xcd * gb + slot - ga;
+    win_passes([&](auto second, int again) {
+      return prefix_pass<P, IN, SHARE_B, true, decltype(second)::value>(a, wb, id, again);
+    });
+  }
+}
+
+// The partials of a row: a workgroup of 128 threads a row, a thread a column.  Bound by latency, so that the partials' loads
+// are under way before their weights are known.
 template <int IN>
 __global__ __launch_bounds__(128) void prefix_join_kernel(const PrefixArgs a) {
   __shared__ float weight[256], red[2];
+  constexpr int AHEAD = 32;
   const int64_t row = blockIdx.x + static_cast<int64_t>(blockIdx.y) * gridDim.x;
   if (row >= static_cast<int64_t>(a.batch) * a.heads * a.n) return;
-  const int b = static_cast<int>(row / (static_cast<int64_t>(a.heads) * a.n)), i = static_cast<int>(row % a.n);
+  const int t = threadIdx.x, b = static_cast<int>(row / (static_cast<int64_t>(a.heads) * a.n)), i = static_cast<int>(row % a.n);
   const int length = prefix_length(a, b);
-  const bool live = i < prefix_count(a, b, length);
-  const int pitch = a.dv + 2;
-  const float* part = a.part + row * a.parts * pitch;
-  if (live) {
-    float top = -__builtin_inff(), den = 0.f;
-    for (int j = threadIdx.x; j < a.parts; j += 128) top = fmaxf(top, part[j * pitch + a.dv]);
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = fmaxf(red[0], red[1]);
-    __syncthreads();
-    for (int j = threadIdx.x; j < a.parts; j += 128) {
-      const float lj = part[j * pitch + a.dv + 1];
-      const float f = lj == 0.f ? 0.f : __builtin_amdgcn_exp2f((part[j * pitch + a.dv] - top) * a.c);
-      weight[j] = f;
-      den = fmaf(f, lj, den);
-    }
-    for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = den;
-    __syncthreads();
-    den = red[0] + red[1];
-    if (!(den > 0.f)) den = __builtin_nanf("");
-    if (static_cast<int>(threadIdx.x) < a.dv && a.out) {
-      float sum = 0.f;
-#pragma unroll 8
-      for (int j = 0; j < a.parts; ++j) sum = fmaf(weight[j], part[j * pitch + threadIdx.x], sum);
-      store_elem(a.out, row * a.dv + threadIdx.x, IN, sum / den);
-    }
-    if (threadIdx.x == 0 && a.lse) a.lse[row] = top * a.c - win_weight_lift<IN>() + __builtin_amdgcn_logf(den);
-  } else {
-    if (static_cast<int>(threadIdx.x) < a.dv && a.out) store_elem(a.out, row * a.dv + threadIdx.x, IN, 0.f);
-    if (threadIdx.x == 0 && a.lse) a.lse[row] = 0.f;
+  if (i >= prefix_count(a, b, length)) {
+    if (t < a.dv && a.out) store_elem(a.out, row * a.dv + t, IN, 0.f);
+    if (t == 0 && a.lse) a.lse[row] = 0.f;
+    return;
   }
+  const float* part = a.part + row * a.parts * a.pitch + t;
+  const floatx2* stat = reinterpret_cast<const floatx2*>(a.stat) + row * a.parts;
+  const bool column = t < a.dv && a.out;
+  float ahead[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) ahead[j] = column && j < a.parts ? part[j * a.pitch] : 0.f;
+  floatx2 mine[2];
+  float top = -__builtin_inff(), den = 0.f;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    mine[k] = t + 128 * k < a.parts ? stat[t + 128 * k] : floatx2{-__builtin_inff(), 0.f};
+    top = fmaxf(top, mine[k][0]);
+  }
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if ((t & 63) == 0) red[t >> 6] = top;
+  __syncthreads();
+  top = fmaxf(red[0], red[1]);
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float f = mine[k][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f((mine[k][0] - top) * a.c);
+    weight[t + 128 * k] = f;
+    den = fmaf(f, mine[k][1], den);
+  }
+  for (int o = 32; o > 0; o >>= 1) den += __shfl_xor(den, o);
+  if ((t & 63) == 0) red[t >> 6] = den;
+  __syncthreads();
+  den = red[0] + red[1];
+  if (!(den > 0.f)) den = __builtin_nanf("");
+  if (column) {
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) sum = fmaf(weight[j], ahead[j], sum);
+#pragma unroll 8
+    for (int j = AHEAD; j < a.parts; ++j) sum = fmaf(weight[j], part[j * a.pitch], sum);
+    store_elem(a.out, row * a.dv + t, IN, sum / den);
+  }
+  if (t == 0 && a.lse) a.lse[row] = prefix_lse<IN>(top, den, a.c);
 }
 
 struct ReceivedArgs {
   PrefixArgs a;          // q, own k; lse: the rows' statistics
-  int tiles, nsplit;     // tiles of 128 keys, workgroups a tile
+  int few;               // up to RECEIVED_FEW rows: received_few_kernel
+  int tiles, nsplit;     // workgroups of a key head along its keys, and along the rows (few: 1)
   float* sums;           // [nsplit][batch][kv][m], or the weights themselves with one
   float* weights;        // [batch][kv][m]
 };
 
+constexpr int RECEIVED_FEW = 128;
 template <int IN>
 __host__ __device__ constexpr int received_rows() { return IN == F32 ? 32 : 64; }
+// blocks of 32 keys a wave: two share what a wave reads of the rows, which one block's products wait for (LDS reads 128 bytes
+// a cycle; 32 heads of 16384 rows, 128 wide, 1.77 ms with one, 1.32 with two).  fp32 operands leave no room for two.
+template <int IN>
+__host__ __device__ constexpr int received_blocks() { return IN == F32 ? 1 : 2; }
 
-// The weights that keys receive.  A workgroup holds 128 keys of a key head as operands, 32 a wave, and walks over the
-// rows that see one of them, head by head of the group; with X = Q K^T a lane has 16 rows of one key, whose weights
-// it sums: no exchange between lanes until the end.  Sums of 16 go into a compensated total (16384 x 4 rows).
+// A row's statistic as its weights take it.  A row whose sum of weights is not finite has none that are; no row, no weights.
+__device__ __forceinline__ float received_stat(float lse, bool row) {
+  return row ? (win_finite(lse) ? -lse : __builtin_nanf("")) : -__builtin_inff();
+}
+
+// Weights of 32 staged rows from r0 (a multiple of 32) with a wave's keys.  (Products that start from the statistics would
+// save 4 % and round their sums at the statistics' size: errors of 5e-7, so 5e-8.)
+template <int P, int IN, int NB>
+__device__ __forceinline__ void received_weights(floatx16 (&x)[NB], const uint4* qs, const float* stat, int r0,
+                                                 const WinFrag<IN> (&kf)[NB][P / 16], float c, int lane) {
+  const int hh = lane >> 5;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[n][e] = 0.f;
+#pragma unroll
+  for (int s = 0; s < P / 16; ++s) {
+    const WinFrag<IN> q = win_read_row<P, IN>(qs, r0 + (lane & 31), s, hh);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) win_mma<IN>(x[n], q, kf[n][s]);
+  }
+#pragma unroll
+  for (int e = 0; e < 16; e += 4) {
+    const floatx4 y = *reinterpret_cast<const floatx4*>(&stat[r0 + 8 * (e >> 2) + 4 * hh]);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[n][e + j] = __builtin_amdgcn_exp2f(fmaf(x[n][e + j], c, y[j]));
+  }
+}
+__device__ __forceinline__ void received_add(float& total, float& lost, const floatx16& x) {
+  float sum = x[0];
+#pragma unroll
+  for (int e = 1; e < 16; ++e) sum += x[e];
+  const float y = sum - lost, z = total + y;
+  lost = (z - total) - y;
+  total = z;
+}
+
+// The weights that keys receive.  A workgroup holds 32 to 64 keys a wave as operands and walks over its share of the rows
+// that see one of them, head by head of the group; with X = Q K^T a lane has 16 rows of one key, whose weights it sums: no
+// exchange between lanes until the end.  Sums of 16 go into a compensated total (16384 x 4 rows).  32 heads of 16384 rows,
+// 128 wide: 1.32 ms, 830 TFLOP/s (a large matrix product 1200); 64 wide 0.76 ms, bound by the exponentials.
 template <int P, int IN>
 __global__ __launch_bounds__(256, 2) void received_kernel(const ReceivedArgs w) {
-  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BQ = received_rows<IN>(), NSUB = BQ / 32;
+  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BQ = received_rows<IN>(), NB = received_blocks<IN>();
   __shared__ uint4 qs[BQ * CH];
   __shared__ __attribute__((aligned(16))) float stat[BQ];
   const PrefixArgs& a = w.a;
+  // a tile's workgroups, then the tiles of a key head next to each other, those that most rows see first
   int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int tile = id % w.tiles;
-  id /= w.tiles;
-  const int split = id % w.nsplit, unit = id / w.nsplit, b = unit / a.kv, hk = unit - b * a.kv;
+  const int split = id % w.nsplit;
+  id /= w.nsplit;
+  const int tile = id % w.tiles, unit = id / w.tiles, b = unit / a.kv, hk = unit - b * a.kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
   const int length = prefix_length(a, b), count = prefix_count(a, b, length), base = length - count;
-  const int key0 = tile * WIN_ROWS, w0 = key0 + 32 * wave, key = w0 + (lane & 31);
+  const int key0 = tile * 128 * NB, w0 = key0 + 32 * NB * wave;
 
-  float total = 0.f, lost = 0.f;
+  float total[NB], lost[NB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) total[n] = lost[n] = 0.f;
   const int i0 = (key0 > base ? key0 - base : 0) / BQ * BQ;  // the first row that sees one of the keys
   const int row_tiles = key0 < length && i0 < count ? (count - i0 + BQ - 1) / BQ : 0, all = row_tiles * a.group;
   const int share = (all + w.nsplit - 1) / w.nsplit, t0 = split * share, t1 = t0 + share < all ? t0 + share : all;
   if (t0 < t1) {
-    WinFrag<IN> kf[P / 16];
+    WinFrag<IN> kf[NB][P / 16];
     const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
-    const char* krow = rows_at<ES>(a.k, b, hk, key < length ? key : 0);
 #pragma unroll
-    for (int s = 0; s < P / 16; ++s) {
-      kf[s] = win_load_row<IN>(krow, s, hh, a.d, flip);
-      win_keep<IN>(kf[s], key < length);
+    for (int n = 0; n < NB; ++n) {
+      const int key = w0 + 32 * n + (lane & 31);
+      const char* row = rows_at<ES>(a.k, b, hk, key < length ? key : 0);
+#pragma unroll
+      for (int s = 0; s < P / 16; ++s) {
+        kf[n][s] = win_load_row<IN>(row, s, hh, a.d, flip);
+        win_keep<IN>(kf[n][s], key < length);
+      }
     }
     WinStage<P, IN, BQ, 256> stage;
     stage.init(a.q, a.d);
     float next = 0.f;
-    auto load = [&](int it) {
-      const int g = it / row_tiles, i = i0 + (it - g * row_tiles) * BQ, h = hk * a.group + g;
+    int g = t0 / row_tiles, i = i0 + (t0 - g * row_tiles) * BQ;  // of the tile that is loaded next
+    auto load = [&]() {
+      const int h = hk * a.group + g, r = i + static_cast<int>(threadIdx.x % BQ);
       stage.load(rows_at<ES>(a.q, b, h, i), count - i);
-      const int r = i + static_cast<int>(threadIdx.x % BQ);
-      next = a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.n + (r < count ? r : count - 1)];
-      // behind the last row: no weights; a row whose sum of weights is not finite has none that are
-      next = r < count ? (win_finite(next) ? next : __builtin_nanf("")) : __builtin_inff();
+      next = received_stat(a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.n + (r < count ? r : count - 1)], r < count);
     };
-    load(t0);
+    load();
     for (int it = t0; it < t1; ++it) {
-      const int i = i0 + it % row_tiles * BQ;
+      const int row = i;
       __syncthreads();
-      stage.put(qs, count - i);
+      stage.put(qs, count - row);
       if (threadIdx.x < BQ) stat[threadIdx.x] = next;
       __syncthreads();
-      if (it + 1 < t1) load(it + 1);
-      const bool every = base + i >= w0 + 31;
+      i += BQ;
+      if (i >= count) {
+        i = i0;
+        ++g;
+      }
+      if (it + 1 < t1) load();
+      const bool every = base + row >= w0 + 32 * NB - 1;
 #pragma unroll
-      for (int sub = 0; sub < NSUB; ++sub) {
-        floatx16 x;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = 0.f;
-#pragma unroll
-        for (int s = 0; s < P / 16; ++s)
-          win_mma<IN>(x, win_read_row<P, IN>(qs, 32 * sub + (lane & 31), s, hh), kf[s]);
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const floatx4 y = *reinterpret_cast<const floatx4*>(&stat[32 * sub + 8 * (e >> 2) + 4 * hh]);
-          x[e] = __builtin_amdgcn_exp2f(fmaf(x[e], a.c, -y[e & 3]));
-        }
+      for (int sub = 0; sub < BQ / 32; ++sub) {
+        floatx16 x[NB];
+        received_weights<P, IN, NB>(x, qs, stat, 32 * sub, kf, a.c, lane);
         if (!every) {
-          const int from = key - base - i - 32 * sub - 4 * hh;  // the first of the lane's rows that sees its key
 #pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = 8 * (e >> 2) + (e & 3) >= from ? x[e] : 0.f;
+          for (int n = 0; n < NB; ++n) {
+            // the first of the lane's rows that sees its key
+            const int from = w0 + 32 * n + (lane & 31) - base - row - 32 * sub - 4 * hh;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[n][e] = 8 * (e >> 2) + (e & 3) >= from ? x[n][e] : 0.f;
+          }
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) sum += x[e];
-        const float y = sum - lost, z = total + y;
-        lost = (z - total) - y;
-        total = z;
+        for (int n = 0; n < NB; ++n) received_add(total[n], lost[n], x[n]);
       }
     }
   }
-  total += __shfl_xor(total, 32);
-  if (hh == 0 && key < a.m) {
-    float* to = w.nsplit == 1 ? w.weights : w.sums + static_cast<int64_t>(split) * a.batch * a.kv * a.m;
-    to[static_cast<int64_t>(unit) * a.m + key] = key < length ? total : 0.f;
+  float* const to = (w.nsplit == 1 ? w.weights : w.sums + static_cast<int64_t>(split) * a.batch * a.kv * a.m) +
+                    static_cast<int64_t>(unit) * a.m;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    total[n] += __shfl_xor(total[n], 32);
+    const int key = w0 + 32 * n + (lane & 31);
+    if (hh == 0 && key < a.m) to[key] = key < length ? total[n] : 0.f;
+  }
+}
+
+// The same for up to RECEIVED_FEW rows, those of the group's heads together (row i of head g at i group + g): they stay in
+// LDS, and the waves walk over the keys, 32 at a time and the next two blocks on their way, each by itself.  Keys go
+// through LDS too: as operands they are loaded in pieces of 32 bytes a row and instruction.  Bound by reading the keys.
+template <int P, int IN>
+__host__ __device__ constexpr int received_few_bytes(int rows) {  // of LDS
+  return (rows + 4 * 32) * P * (IN == F32 ? 4 : 2) + 8 * rows;
+}
+template <int P, int IN>
+__global__ __launch_bounds__(256, 2) void received_few_kernel(const ReceivedArgs w) {
+  constexpr int ES = IN == F32 ? 4 : 2, E = 16 / ES, CH = win_chunks<ES>(P);
+  extern __shared__ uint4 win_lds[];
+  const PrefixArgs& a = w.a;
+  const int id = xcd_remap(blockIdx.x, gridDim.x), part = id % w.tiles, unit = id / w.tiles;
+  const int b = unit / a.kv, hk = unit - b * a.kv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
+  const int length = prefix_length(a, b), count = prefix_count(a, b, length), base = length - count;
+  const int rows = count * a.group, blocks = (rows + 31) / 32;  // rows, and blocks of 32 of them
+  const int room = (a.n * a.group + 31) / 32 * 32;
+  uint4 *const qs = win_lds, *const ks = qs + room * CH + wave * 32 * CH;
+  float* const stat = reinterpret_cast<float*>(qs + (room + 4 * 32) * CH);
+  int* const seen = reinterpret_cast<int*>(stat + room);  // the last token that a row sees
+  float* const to = w.weights + static_cast<int64_t>(unit) * a.m;
+
+  const int step = 4 * w.tiles, first = 4 * part + wave;  // blocks of keys
+  const int key_blocks = rows > 0 ? (length + 31) / 32 : 0;
+  WinStage<P, IN, 32, 64> even, odd;
+  even.init(a.k, a.d);
+  odd.init(a.k, a.d);
+  auto load = [&](auto& stage, int block) {
+    if (block < key_blocks) stage.load(rows_at<ES>(a.k, b, hk, 32 * block), length - 32 * block);
+  };
+  load(even, first);
+  load(odd, first + step);
+
+  for (int u = threadIdx.x; u < 32 * blocks * CH; u += 256) {
+    const int r = u / CH, c = u - r * CH, i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) - i * a.group;
+    const uint4 x = rows_unit<ES>(rows_at<ES>(a.q, b, h, i), c * E, a.d);
+    qs[r * CH + (c ^ win_swizzle<CH>(r))] = uint4{r < rows ? x.x : 0u, r < rows ? x.y : 0u, r < rows ? x.z : 0u,
+                                                  r < rows ? x.w : 0u};
+  }
+  for (int r = threadIdx.x; r < 32 * blocks; r += 256) {
+    const int i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) - i * a.group;
+    stat[r] = received_stat(a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.n + i], r < rows);
+    seen[r] = base + i;
+  }
+  __syncthreads();
+
+  const uint32_t flip = a.scale < 0.f ? (IN == F32 ? 0x80000000u : 0x80008000u) : 0u;
+  auto take = [&](auto& stage, int block) {
+    const int key = 32 * block + (lane & 31);
+    float total = 0.f, lost = 0.f;
+    if (block < key_blocks) {
+      win_sync<true>();
+      stage.put(ks, length - 32 * block);
+      load(stage, block + 2 * step);
+      win_sync<true>();
+      WinFrag<IN> kf[1][P / 16];
+#pragma unroll
+      for (int s = 0; s < P / 16; ++s) {
+        kf[0][s] = win_read_row<P, IN>(ks, lane & 31, s, hh);
+#pragma unroll
+        for (int j = 0; j < (IN == F32 ? 2 : 1); ++j) {
+          uint4& u = kf[0][s].w[j];
+          u = uint4{u.x ^ flip, u.y ^ flip, u.z ^ flip, u.w ^ flip};
+        }
+      }
+      for (int r0 = 0; r0 < 32 * blocks; r0 += 32) {
+        floatx16 x[1];
+        received_weights<P, IN, 1>(x, qs, stat, r0, kf, a.c, lane);
+        if (32 * block + 31 > base) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) x[0][e] = key <= seen[r0 + 8 * (e >> 2) + 4 * hh + (e & 3)] ? x[0][e] : 0.f;
+        }
+        received_add(total, lost, x[0]);
+      }
+    }
+    total += __shfl_xor(total, 32);
+    if (hh == 0 && key < a.m) to[key] = key < length ? total : 0.f;
+  };
+  const int end = (a.m + 31) / 32;
+  for (int block = first; block < end; block += 2 * step) {
+    take(even, block);
+    if (block + step < end) take(odd, block + step);
   }
 }
 

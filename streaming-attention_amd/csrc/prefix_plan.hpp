@@ -6,11 +6,6 @@
 
 namespace sta_api {
 
-template <int P, int IN>
-int launch_prefix(const sta::PrefixArgs& a, const sta::PrefixWalk& w, int share, int values, hipStream_t s);
-template <int P, int IN>
-int launch_received(const sta::ReceivedArgs& w, hipStream_t s);
-
 constexpr int kMaxPrefixD = 128;
 constexpr int64_t kMaxPrefixRows = int64_t(1) << 30;
 constexpr int kMaxPrefixParts = 256;  // prefix_join_kernel's weights
@@ -26,12 +21,12 @@ struct PrefixPlan {
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // One walk over `keys` keys of units of `rows` rows: the tile and the number of workgroups that share a tile's keys.
-// Up to 32 rows: one tile of 32 whose waves share the keys.  The card holds 512 workgroups at a time (256 compute units,
-// two each of 128 columns); a share has at least 256 keys.
-inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows, int64_t keys) {
+// Up to 32 rows: one tile of 32 whose waves share the keys.  A share has at least 256 keys; room: workgroups that the walk
+// is to fill the card with, which holds 512 at a time (256 compute units, two each of 128 columns).
+inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows, int64_t keys, int64_t room) {
   share = rows <= 32;
   w.tiles = static_cast<int>(ceil_div(rows, share ? 32 : sta::WIN_ROWS));
-  int64_t want = 512 / (units * w.tiles);
+  int64_t want = room / (units * w.tiles);
   const int64_t most = ceil_div(keys, 256);
   if (want > most) want = most;
   if (want > kMaxPrefixParts / 2) want = kMaxPrefixParts / 2;
@@ -39,7 +34,8 @@ inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows
 }
 
 // own: the sequences' own tokens take part.  The sequences of a set lie in one tile for the prefix where each has fewer rows
-// than a tile.
+// than a tile; then one workgroup of the prefix's walk a compute unit leaves room for one of the other's, and half the
+// partials of two (64 x 32 heads of 128 over 32768 shared and 1024 own rows: 107 us, 122 with two).
 inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, bool own) {
   PrefixPlan p{};
   const int64_t rows = static_cast<int64_t>(a.n) * a.group, units = static_cast<int64_t>(a.batch) * a.kv;
@@ -48,13 +44,13 @@ inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, bool own) {
     p.walks = own ? 2 : 1;
     p.walk[0].span = a.per_set;
     p.walk[0].prefix = 1;
-    deal_out(p.walk[0], p.share[0], static_cast<int64_t>(a.sets) * a.kv, rows * a.per_set, a.p);
+    deal_out(p.walk[0], p.share[0], static_cast<int64_t>(a.sets) * a.kv, rows * a.per_set, a.p, own ? 256 : 512);
     p.parts = p.walk[0].nsplit;
     if (own) {
       p.walk[1].span = 1;
       p.walk[1].own = 1;
       p.walk[1].first = p.parts;
-      deal_out(p.walk[1], p.share[1], units, rows, a.m);
+      deal_out(p.walk[1], p.share[1], units, rows, a.m, 512);
       p.parts += p.walk[1].nsplit;
     }
     return p;
@@ -63,13 +59,22 @@ inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, bool own) {
   p.walk[0].span = 1;
   p.walk[0].prefix = a.p > 0;
   p.walk[0].own = 1;
-  deal_out(p.walk[0], p.share[0], units, rows, static_cast<int64_t>(a.p) + a.m);
+  deal_out(p.walk[0], p.share[0], units, rows, static_cast<int64_t>(a.p) + a.m, 512);
   p.parts = p.walk[0].nsplit > 1 ? p.walk[0].nsplit : 0;
   return p;
 }
 
+// the partials: sums, then statistics
+inline int64_t prefix_sum_bytes(const sta::PrefixArgs& a, int parts) {
+  return 4 * static_cast<int64_t>(a.batch) * a.heads * a.n * parts * a.pitch;
+}
 inline int64_t prefix_part_bytes(const sta::PrefixArgs& a, int parts) {
-  return 4 * static_cast<int64_t>(a.batch) * a.heads * a.n * parts * (a.dv + 2);
+  return prefix_sum_bytes(a, parts) + ceil_div(8 * static_cast<int64_t>(a.batch) * a.heads * a.n * parts, 16) * 16;
+}
+inline void set_parts(sta::PrefixArgs& a, void* room, int parts) {
+  a.part = static_cast<float*>(room);
+  a.stat = reinterpret_cast<float*>(static_cast<char*>(room) + prefix_sum_bytes(a, parts));
+  a.parts = parts;
 }
 
 // The shape part of the arguments; d and dv padded are the caller's.
@@ -97,6 +102,7 @@ inline int prefix_shape(sta::PrefixArgs& a, int dtype, int64_t batch, int heads,
   a.p = static_cast<int>(p);
   a.d = d;
   a.dv = dv;
+  a.pitch = (dv + 3) / 4 * 4;
   a.scale = scale;
   const float c = (scale < 0.f ? -scale : scale) * 1.44269504088896340736f;
   a.c = c > 1e-37f ? c : 1e-37f;  // above 0: a hidden pair's logit, -inf, stays one times c
@@ -114,32 +120,6 @@ inline bool prefix_strides_ok(const int64_t* strides, int tensors, int dtype) {
 
 inline sta::Rows prefix_rows_of(const void* p, const int64_t* strides) {
   return sta::Rows{p, strides[0], strides[1], strides[2], 0};
-}
-
-template <typename Call>
-int prefix_by_type(int dtype, int width, Call call) {
-#define STA_PREFIX_CASE(P)                                                                                 \
-  if (width <= P) {                                                                                        \
-    if (dtype == STA_F32) return call(std::integral_constant<int, P>{}, std::integral_constant<int, sta::F32>{});   \
-    if (dtype == STA_BF16) return call(std::integral_constant<int, P>{}, std::integral_constant<int, sta::BF16>{}); \
-    return call(std::integral_constant<int, P>{}, std::integral_constant<int, sta::F16>{});                \
-  }
-  STA_PREFIX_CASE(32)
-  STA_PREFIX_CASE(64)
-  STA_PREFIX_CASE(96)
-  STA_PREFIX_CASE(128)
-#undef STA_PREFIX_CASE
-  return STA_ERR_UNSUPPORTED;
-}
-
-// the walks of a plan
-inline int run_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int dtype, int values, hipStream_t s) {
-  return prefix_by_type(dtype, values && a.dv > a.d ? a.dv : a.d, [&](auto width, auto in) {
-    int st = STA_OK;
-    for (int i = 0; i < p.walks && st == STA_OK; ++i)
-      st = launch_prefix<decltype(width)::value, decltype(in)::value>(a, p.walk[i], p.share[i], values, s);
-    return st;
-  });
 }
 
 }  // namespace sta_api

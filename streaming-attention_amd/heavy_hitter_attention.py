@@ -313,15 +313,18 @@ class HeavyHitterStreamingAttention:
         float32 [S,Hkv,recent + 1 + kept]) as the cache holds them, in the order of its slots; zero, and position -1,
         where no token is."""
         shape = (self.streams, self.kv_heads, self._slots)
+        weights = self._weights.new_empty(shape)
+        positions = self._positions.new_empty(shape)
         keys = self._weights.new_empty((*shape, self.dim), dtype=self.dtype)
         values = self._weights.new_empty((*shape, self.value_dim), dtype=self.dtype)
         with _on(self.device):
             st = _native.lib().sta_heavy_items(
                 self._code, self.streams, self.kv_heads, self.dim, self.value_dim, self.recent, self.kept,
-                self._keys.data_ptr(), self._values.data_ptr(), self._positions.data_ptr(), keys.data_ptr(),
-                values.data_ptr(), _native.stream_handle(self.device))
+                self._keys.data_ptr(), self._values.data_ptr(), self._weights.data_ptr(), self._positions.data_ptr(),
+                keys.data_ptr(), values.data_ptr(), weights.data_ptr(), positions.data_ptr(),
+                _native.stream_handle(self.device))
         _native.check(st, "sta_heavy_items")
-        return keys, values, self.positions.clone(), self.weights.clone()
+        return keys, values, positions, weights
 
     def state_size_bytes(self) -> int:
         """Device bytes of the cache."""

@@ -155,7 +155,7 @@ def test_null_pointers_are_refused():
         assert l.sta_received_attention(*bad) == arg, i
     assert l.sta_received_attention(*received) == _native.STA_ERR_SCRATCH
     state = [some] * 6
-    heavy = [some, some, some, 1, 2, 8, 2, 64, 64, strides, 0.125, 16, 100, None, None, 0, 0, None, None, *state, some, None, 0,
+    heavy = [some, some, some, 1, 2, 8, 2, 64, 64, strides, 0.125, 16, 1 << 20, None, None, 0, 0, None, None, *state, some, None, 0,
              None]
     for i in (0, 2, 9, *range(19, 25), 25):
         bad = list(heavy)
@@ -178,8 +178,8 @@ def test_null_pointers_are_refused():
         assert l.sta_heavy_start(*bad) == arg, i
     assert l.sta_heavy_start(*start) == _native.STA_ERR_SCRATCH
     assert l.sta_heavy_start(*start[:6], 0, *start[7:]) == _native.STA_ERR_SHAPE
-    items = [1, 2, 2, 64, 64, 16, 100, some, some, some, some, some, None]
-    for i in range(7, 12):
+    items = [1, 2, 2, 64, 64, 16, 100, *[some] * 8, None]
+    for i in range(7, 15):
         bad = list(items)
         bad[i] = None
         assert l.sta_heavy_items(*bad) == arg, i
