@@ -72,59 +72,96 @@ __device__ __forceinline__ unsigned long long heavy_least(unsigned long long x, 
   return x;
 }
 
-__device__ __forceinline__ HeavyMove heavy_move(const HeavyArgs& a, int sh, bool append) {
+// What a step of a key head with count n does: its slots, and once the leaving token's weight and the lowest kept ones (of
+// even and of odd counts) are there, where it goes.
+__device__ __forceinline__ HeavyMove heavy_slots(const HeavyArgs& a, bool append, int64_t n) {
   HeavyMove m;
-  const int64_t n = a.counts[sh];
   m.n = n < 0 ? 0 : n;
-  const int64_t after = m.n + (append ? 1 : 0), gone = m.n - a.recent;
-  m.from = m.to = m.slot = m.hole = -1;
+  const int64_t after = m.n + (append ? 1 : 0), older = after - a.recent;
+  m.hole = older > 0 ? static_cast<int>((older - 1) % a.ring) : -1;
+  m.held = older > 0 ? a.ring + static_cast<int>(older < a.kept ? older : a.kept) : static_cast<int>(after);
+  m.slot = append ? static_cast<int>(m.n % a.ring) : -1;
+  m.from = append ? m.hole : -1;
+  m.to = -1;
   m.weight = 0.f;
-  if (append) {
-    m.slot = static_cast<int>(m.n % a.ring);
-    if (gone >= 0) {
-      m.from = static_cast<int>(gone % a.ring);
-      m.weight = a.weights[static_cast<int64_t>(sh) * a.pitch + m.from];
-      if (gone < a.kept) {
-        m.to = a.ring + static_cast<int>(gone);
-      } else {
-        const unsigned long long low = a.lowest[2 * static_cast<int64_t>(sh) + (m.n & 1)];
-        const int slot = static_cast<int>(low & 0xffffffffu);
-        if (heavy_order(m.weight) >= static_cast<uint32_t>(low >> 32) && slot >= a.ring && slot < a.r.slots) m.to = slot;
+  return m;
+}
+__device__ __forceinline__ float heavy_weight(const HeavyArgs& a, int sh, int slot) {
+  return a.weights[static_cast<int64_t>(sh) * a.pitch + (slot < 0 ? 0 : slot)];
+}
+__device__ __forceinline__ void heavy_goes(const HeavyArgs& a, HeavyMove& m, float weight, unsigned long long even,
+                                           unsigned long long odd) {
+  const int64_t gone = m.n - a.recent;
+  const unsigned long long low = m.n & 1 ? odd : even;
+  const int lowest = static_cast<int>(low & 0xffffffffu);
+  const bool free = gone < a.kept;
+  const bool better = heavy_order(weight) >= static_cast<uint32_t>(low >> 32) && lowest >= a.ring && lowest < a.r.slots;
+  if (m.from >= 0) {
+    m.weight = weight;
+    m.to = free ? a.ring + static_cast<int>(gone) : (better ? lowest : -1);
+  }
+}
+
+// A thread's piece of a token's row, of the first 4 nbk threads 8 dimensions of the key, of threads 64 .. 64 + 32 nbv - 1
+// a column of the value: from the call or a slot, into a slot.
+template <int ST>
+struct HeavyPiece {
+  static constexpr int ES = ST == F32 ? 4 : 2;
+  uint4 k[ES / 2];
+  uint32_t v;
+
+  __device__ __forceinline__ static bool key(const RingArgs& a) { return static_cast<int>(threadIdx.x) < 4 * a.nbk; }
+  __device__ __forceinline__ static bool value(const RingArgs& a) {
+    return threadIdx.x >= 64 && static_cast<int>(threadIdx.x) < 64 + 32 * a.nbv;
+  }
+  __device__ __forceinline__ static uint8_t* key_at(const RingArgs& a, int sh, int slot) {
+    return a.keys + (static_cast<int64_t>(sh) * a.tiles + (slot >> 5)) * ring_tile_bytes(a.nbk, ST) +
+           ring_key_at(slot & 31, 8 * threadIdx.x, a.nbk, ST);
+  }
+  __device__ __forceinline__ static uint8_t* value_at(const RingArgs& a, int sh, int slot) {
+    return a.values + (static_cast<int64_t>(sh) * a.tiles + (slot >> 5)) * ring_tile_bytes(a.nbv, ST) +
+           ring_value_at(slot & 31, threadIdx.x - 64, a.nbv, ST);
+  }
+  __device__ __forceinline__ void load_new(const RingArgs& a, int s, int hk) {
+    if (key(a)) {
+      const char* row = rows_at<ES>(a.k, s, hk, 0);
+#pragma unroll
+      for (int i = 0; i < ES / 2; ++i) k[i] = rows_chunk<ES>(row, 8 * threadIdx.x + (16 / ES) * i, a.d);
+    } else if (value(a)) {
+      const char* row = rows_at<ES>(a.v, s, hk, 0);
+      const int col = threadIdx.x - 64;
+      v = 0u;
+      if (col < a.dv) {
+        if constexpr (ES == 4)
+          v = reinterpret_cast<const uint32_t*>(row)[col];
+        else
+          v = reinterpret_cast<const uint16_t*>(row)[col];
       }
     }
   }
-  const int64_t older = after - a.recent;
-  if (older > 0) {
-    m.hole = static_cast<int>((older - 1) % a.ring);
-    m.held = a.ring + static_cast<int>(older < a.kept ? older : a.kept);
-  } else {
-    m.held = static_cast<int>(after);
-  }
-  return m;
-}
-
-// The token that leaves the ring into its kept slot, by a workgroup of at least 64 + 32 nbv threads; the caller's barrier
-// follows.  Its old slot is nobody's to write in this step.
-template <int ST>
-__device__ __forceinline__ void heavy_keep(const RingArgs& a, int sh, int from, int to) {
-  constexpr int ES = ST == F32 ? 4 : 2;
-  const int64_t tile0 = static_cast<int64_t>(sh) * a.tiles;
-  const int t = threadIdx.x;
-  if (t < 4 * a.nbk) {
-    const uint8_t* x = a.keys + (tile0 + (from >> 5)) * ring_tile_bytes(a.nbk, ST) + ring_key_at(from & 31, 8 * t, a.nbk, ST);
-    uint8_t* y = a.keys + (tile0 + (to >> 5)) * ring_tile_bytes(a.nbk, ST) + ring_key_at(to & 31, 8 * t, a.nbk, ST);
+  __device__ __forceinline__ void load(const RingArgs& a, int sh, int slot) {
+    if (key(a)) {
 #pragma unroll
-    for (int i = 0; i < ES / 2; ++i) reinterpret_cast<uint4*>(y)[i] = reinterpret_cast<const uint4*>(x)[i];
-  } else if (t >= 64 && t < 64 + 32 * a.nbv) {
-    const uint8_t* x =
-        a.values + (tile0 + (from >> 5)) * ring_tile_bytes(a.nbv, ST) + ring_value_at(from & 31, t - 64, a.nbv, ST);
-    uint8_t* y = a.values + (tile0 + (to >> 5)) * ring_tile_bytes(a.nbv, ST) + ring_value_at(to & 31, t - 64, a.nbv, ST);
-    if constexpr (ES == 4)
-      *reinterpret_cast<uint32_t*>(y) = *reinterpret_cast<const uint32_t*>(x);
-    else
-      *reinterpret_cast<uint16_t*>(y) = *reinterpret_cast<const uint16_t*>(x);
+      for (int i = 0; i < ES / 2; ++i) k[i] = reinterpret_cast<const uint4*>(key_at(a, sh, slot))[i];
+    } else if (value(a)) {
+      if constexpr (ES == 4)
+        v = *reinterpret_cast<const uint32_t*>(value_at(a, sh, slot));
+      else
+        v = *reinterpret_cast<const uint16_t*>(value_at(a, sh, slot));
+    }
   }
-}
+  __device__ __forceinline__ void store(const RingArgs& a, int sh, int slot) const {
+    if (key(a)) {
+#pragma unroll
+      for (int i = 0; i < ES / 2; ++i) reinterpret_cast<uint4*>(key_at(a, sh, slot))[i] = k[i];
+    } else if (value(a)) {
+      if constexpr (ES == 4)
+        *reinterpret_cast<uint32_t*>(value_at(a, sh, slot)) = v;
+      else
+        *reinterpret_cast<uint16_t*>(value_at(a, sh, slot)) = static_cast<uint16_t>(v);
+    }
+  }
+};
 
 // A slot's weight and position after the step, before its query adds to the weight.
 __device__ __forceinline__ float heavy_base(const HeavyMove& m, int slot, float w) {
@@ -132,15 +169,17 @@ __device__ __forceinline__ float heavy_base(const HeavyMove& m, int slot, float 
   return slot == m.slot || slot == m.hole ? 0.f : w;
 }
 
-// The increments of slots 4 at, .. + 3 from `queries` heads' logits (`pitch` floats each), and what they do to the lowest
-// kept weight; stat: the heads' maxima, and their sums' inverses `stats` behind them.
+// four slots' weights
+__device__ __forceinline__ floatx4* heavy_weights(const HeavyArgs& a, int sh, int at) {
+  return reinterpret_cast<floatx4*>(a.weights + static_cast<int64_t>(sh) * a.pitch + 4 * at);
+}
+// Slots 4 at, .. + 3 of weights w grow by `queries` heads' logits (`pitch` floats each); what that does to the lowest kept
+// weight.  stat: the heads' maxima, and their sums' inverses `stats` behind them.
 template <int ST, typename Logits>
 __device__ __forceinline__ unsigned long long heavy_grow(const HeavyArgs& a, const HeavyMove& m, int sh, int at,
-                                                         Logits logits, int64_t pitch, int queries, const float* stat,
-                                                         int stats) {
+                                                         const floatx4& w, Logits logits, int64_t pitch, int queries,
+                                                         const float* stat, int stats) {
   constexpr float lift = win_weight_lift<ST>();
-  float* row = a.weights + static_cast<int64_t>(sh) * a.pitch + 4 * at;
-  const floatx4 w = *reinterpret_cast<const floatx4*>(row);
   floatx4 grown = floatx4{0.f, 0.f, 0.f, 0.f};
   for (int i = 0; i < queries; ++i) {
     const floatx4 x = *reinterpret_cast<const floatx4*>(logits + i * pitch + 4 * at);
@@ -160,7 +199,7 @@ __device__ __forceinline__ unsigned long long heavy_grow(const HeavyArgs& a, con
     y[j] = in ? heavy_base(m, slot, w[j]) + grown[j] : 0.f;
     if (in && slot >= a.ring) low = heavy_min(low, heavy_key(y[j], slot));
   }
-  *reinterpret_cast<floatx4*>(row) = y;
+  *heavy_weights(a, sh, at) = y;
   return low;
 }
 
@@ -202,7 +241,25 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   float *const red = heavy_lds, *const kept = heavy_lds + 4 * rows * PITCH;
   const int kept_pitch = heavy_kept_pitch(h.pitch);
 
-  const HeavyMove move = heavy_move(h, sh, a.append);
+  // Loads come one after the other only where one needs what another gave: what no count is needed for first, then the
+  // leaving token, the first tile and the weights.
+  const int64_t n = h.counts[sh];
+  const unsigned long long low_even = h.lowest[2 * static_cast<int64_t>(sh)], low_odd = h.lowest[2 * static_cast<int64_t>(sh) + 1];
+  HeavyPiece<ST> fresh{}, old{};
+  if (a.append) fresh.load_new(a, s, hk);
+  const int queries = min(16, a.group - 16 * chunk);
+  const int64_t head0 = static_cast<int64_t>(s) * a.heads + hk * a.group + 16 * chunk;
+  uint4 q_row[NBK][ES / 2];
+  {
+    const char* row = rows_at<ES>(a.q, s, hk * a.group + 16 * chunk + (li < queries ? li : 0), 0);
+#pragma unroll
+    for (int b = 0; b < NBK; ++b)
+#pragma unroll
+      for (int i = 0; i < ES / 2; ++i) q_row[b][i] = rows_chunk<ES>(row, 32 * b + 8 * lg + 16 / ES * i, a.d);
+  }
+  HeavyMove move = heavy_slots(h, a.append, n);
+  const float leaving = heavy_weight(h, sh, move.from);
+  if (move.from >= 0) old.load(a, sh, move.from);
   const bool alone = h.alone;
   const int all = (move.held + 31) >> 5, per = (all + a.nsplit - 1) / a.nsplit;
   const int t0 = split * per, t1 = t0 + per < all ? t0 + per : all, count = t1 - t0;
@@ -215,42 +272,44 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
     const int t = i + turn;
     return t0 + (t < count ? t : t - count);
   };
-  // a wave's first tile, before the new token is in if it does not go there
+  // a wave's first tile, before the new token is in
   RingTile<NBK, NBV, ST> even;
   const int first = wave < count ? tile(wave) : -1;
-  const bool early = first >= 0 && first != move.to >> 5 && first != move.slot >> 5;
-  if (early) even.load(a, tile0 + first, lane);
+  if (first >= 0) even.load(a, tile0 + first, lane);
+  constexpr int HOLD = 4;
+  floatx4 weights[HOLD];
+#pragma unroll
+  for (int j = 0; j < HOLD; ++j) {
+    const int at = threadIdx.x + 256 * j;
+    weights[j] = alone && 4 * at < move.held ? *heavy_weights(h, sh, at) : floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  heavy_goes(h, move, leaving, low_even, low_odd);
   if (a.append) {
-    if (move.to >= 0 && (move.to >> 5) >= t0 && (move.to >> 5) < t1) heavy_keep<ST>(a, sh, move.from, move.to);
-    if ((move.slot >> 5) >= t0 && (move.slot >> 5) < t1) ring_put<ST, ST>(a, s, hk, move.slot);
+    if (move.to >= 0 && (move.to >> 5) >= t0 && (move.to >> 5) < t1) old.store(a, sh, move.to);
+    if ((move.slot >> 5) >= t0 && (move.slot >> 5) < t1) fresh.store(a, sh, move.slot);
     __syncthreads();
+    if (first >= 0 && (first == move.to >> 5 || first == move.slot >> 5)) even.load(a, tile0 + first, lane);  // again
   }
   if (!alone && split == 0 && chunk == 0 && threadIdx.x == 0) {
     h.moves[sh] = move;
     h.lowest[2 * static_cast<int64_t>(sh) + ((move.n + a.append) & 1)] = HEAVY_NONE;
   }
 
-  const int queries = min(16, a.group - 16 * chunk);
-  const int64_t head0 = static_cast<int64_t>(s) * a.heads + hk * a.group + 16 * chunk;
   RingFrag<ST> qf[NBK];
-  {
-    const bool in = li < queries;
-    const char* row = rows_at<ES>(a.q, s, hk * a.group + 16 * chunk + (in ? li : 0), 0);
 #pragma unroll
-    for (int b = 0; b < NBK; ++b) {
-      constexpr int E = 16 / ES;
-      float x[8];
+  for (int b = 0; b < NBK; ++b) {
+    constexpr int E = 16 / ES;
+    float x[8];
 #pragma unroll
-      for (int i = 0; i < 8 / E; ++i) {
-        float y[E];
-        rows_unpack<ST>(rows_chunk<ES>(row, 32 * b + 8 * lg + E * i, a.d), y);
+    for (int i = 0; i < 8 / E; ++i) {
+      float y[E];
+      rows_unpack<ST>(q_row[b][i], y);
 #pragma unroll
-        for (int e = 0; e < E; ++e) x[E * i + e] = in ? (a.scale < 0.f ? -y[e] : y[e]) : 0.f;
-      }
-      RingFrag<ST> planes[1];
-      ring_planes<ST, 1>(x, planes);
-      qf[b] = planes[0];
+      for (int e = 0; e < E; ++e) x[E * i + e] = li < queries ? (a.scale < 0.f ? -y[e] : y[e]) : 0.f;
     }
+    RingFrag<ST> planes[1];
+    ring_planes<ST, 1>(x, planes);
+    qf[b] = planes[0];
   }
 
   floatx4 acc[CT];
@@ -339,7 +398,6 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   {
     RingTile<NBK, NBV, ST> odd;
     int i = wave;
-    if (i < count && !early) even.load(a, tile0 + tile(i), lane);
     while (i < count) {
       if (i + 4 < count) odd.load(a, tile0 + tile(i + 4), lane);
       take(even, tile(i));
@@ -388,13 +446,17 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   if (!alone) return;
   __syncthreads();  // the logits of all waves, too
   unsigned long long low = HEAVY_NONE;
-  for (int at = threadIdx.x; 4 * at < move.held; at += 256) {
-    if (h.local)
-      low = heavy_min(low, heavy_grow<ST>(h, move, sh, at, static_cast<const float*>(kept), kept_pitch, queries, stat, 16));
-    else
-      low = heavy_min(low, heavy_grow<ST>(h, move, sh, at, static_cast<const float*>(h.logits + head0 * h.pitch), h.pitch,
-                                          queries, stat, 16));
-  }
+  auto grow = [&](int at, const floatx4& w) {
+    if (4 * at >= move.held) return;
+    const unsigned long long x =
+        h.local ? heavy_grow<ST>(h, move, sh, at, w, static_cast<const float*>(kept), kept_pitch, queries, stat, 16)
+                : heavy_grow<ST>(h, move, sh, at, w, static_cast<const float*>(h.logits + head0 * h.pitch), h.pitch, queries,
+                                 stat, 16);
+    low = heavy_min(low, x);
+  };
+#pragma unroll
+  for (int j = 0; j < HOLD; ++j) grow(threadIdx.x + 256 * j, weights[j]);
+  for (int at = threadIdx.x + 256 * HOLD; 4 * at < move.held; at += 256) grow(at, *heavy_weights(h, sh, at));
   low = heavy_least<256>(low, red_low);
   if (threadIdx.x == 0) {
     heavy_positions(h, move, sh);
@@ -465,9 +527,11 @@ __global__ __launch_bounds__(512) void heavy_join_kernel(const HeavyArgs h, int 
     return;
   }
   const int id = blockIdx.x - outputs, sh = id / ranges, range = id - sh * ranges;
-  const HeavyMove move = h.moves[sh];
   const int s = sh / a.kv, hk = sh - s * a.kv;
   const int64_t head0 = static_cast<int64_t>(s) * a.heads + hk * a.group;
+  const int at = range * (HEAVY_SLOTS / 4) + t;
+  const floatx4 w = 4 * at < h.pitch ? *heavy_weights(h, sh, at) : floatx4{0.f, 0.f, 0.f, 0.f};
+  const HeavyMove move = h.moves[sh];
   unsigned long long low = HEAVY_NONE;
   if (range * HEAVY_SLOTS < move.held) {
     for (int i = wave; i < a.group; i += 8) {  // a wave a head: its maximum and sum
@@ -489,9 +553,8 @@ __global__ __launch_bounds__(512) void heavy_join_kernel(const HeavyArgs h, int 
       }
     }
     __syncthreads();
-    const int at = range * (HEAVY_SLOTS / 4) + threadIdx.x;
     if (4 * at < move.held)
-      low = heavy_grow<ST>(h, move, sh, at, static_cast<const float*>(h.logits + head0 * h.pitch), h.pitch, a.group, stat,
+      low = heavy_grow<ST>(h, move, sh, at, w, static_cast<const float*>(h.logits + head0 * h.pitch), h.pitch, a.group, stat,
                            HEAVY_HEADS);
   }
   low = heavy_least<512>(low, red_low);
@@ -510,9 +573,14 @@ __global__ __launch_bounds__(256) void heavy_update_kernel(const HeavyArgs h) {
   const RingArgs& a = h.r;
   __shared__ unsigned long long red_low[4];
   const int sh = blockIdx.x, s = sh / a.kv, hk = sh - s * a.kv;
-  const HeavyMove move = heavy_move(h, sh, true);
-  if (move.to >= 0) heavy_keep<ST>(a, sh, move.from, move.to);
-  ring_put<ST, ST>(a, s, hk, move.slot);
+  HeavyPiece<ST> fresh{}, old{};
+  fresh.load_new(a, s, hk);
+  HeavyMove move = heavy_slots(h, true, h.counts[sh]);
+  if (move.from >= 0) old.load(a, sh, move.from);
+  heavy_goes(h, move, heavy_weight(h, sh, move.from), h.lowest[2 * static_cast<int64_t>(sh)],
+             h.lowest[2 * static_cast<int64_t>(sh) + 1]);
+  if (move.to >= 0) old.store(a, sh, move.to);
+  fresh.store(a, sh, move.slot);
   float* row = h.weights + static_cast<int64_t>(sh) * h.pitch;
   unsigned long long low = HEAVY_NONE;
   for (int slot = h.ring + threadIdx.x; slot < move.held; slot += 256)

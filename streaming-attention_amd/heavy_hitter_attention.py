@@ -180,7 +180,6 @@ class HeavyHitterStreamingAttention:
             raise ValueError("prefix_lengths must be on the object's device")
         return _rows(pk), _rows(pv), prefix_lengths
 
-    @torch.no_grad()
     def _attend(self, q: Tensor, k: Optional[Tensor], v: Optional[Tensor], prefix, prefix_lengths) -> Tensor:
         sets = p = 0
         pk = pv = prefix_strides = None
@@ -191,7 +190,7 @@ class HeavyHitterStreamingAttention:
         elif prefix_lengths is not None:
             raise ValueError("prefix_lengths without a prefix")
         nbytes = self._bytes.get((sets, p))
-        if nbytes is None:
+        if nbytes is None:  # another prefix than the last call's
             nbytes = _native.lib().sta_heavy_attention_bytes(
                 self._code, self.streams, self.heads, self.kv_heads, self.dim, self.value_dim, self.recent, self.kept,
                 sets, p)
@@ -199,7 +198,7 @@ class HeavyHitterStreamingAttention:
                 raise _native.NativeError("sta_heavy_attention_bytes refused the shape")
             self._bytes = {(sets, p): nbytes}
         out = q.new_empty((self.streams, self.heads, self.value_dim))
-        ws = q.new_empty(nbytes, dtype=torch.uint8)
+        ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         if q.is_contiguous() and (k is None or (k.is_contiguous() and v.is_contiguous())):
             strides = self._dense
         else:
@@ -210,7 +209,7 @@ class HeavyHitterStreamingAttention:
             st = _native.lib().sta_heavy_attention(
                 q.data_ptr(), _native.ptr(k), _native.ptr(v), self._code, self.streams, self.heads, self.kv_heads,
                 self.dim, self.value_dim, strides, self.scale, self.recent, self.kept, _native.ptr(pk), _native.ptr(pv),
-                sets, p, prefix_strides, _native.ptr(prefix_lengths), *self._state, out.data_ptr(), ws.data_ptr(),
+                sets, p, prefix_strides, _native.ptr(prefix_lengths), *self._state, out.data_ptr(), _native.ptr(ws),
                 nbytes, _native.stream_handle(self.device))
         _native.check(st, "sta_heavy_attention")
         return out
@@ -234,7 +233,6 @@ class HeavyHitterStreamingAttention:
         that holds none."""
         return self._attend(self._rows(query, self._shapes["query"], "query"), None, None, prefix, prefix_lengths)
 
-    @torch.no_grad()
     def update(self, key: Tensor, value: Tensor) -> None:
         """One token of every stream into the cache."""
         k = self._rows(key, self._shapes["key"], "key")

@@ -36,8 +36,10 @@ def _strides(*tensors: Tensor):
 def _refuse_gradients(*tensors: Tensor) -> None:
     """There is no backward pass; a result without one would be taken for a constant."""
     _refuse_tangents(*tensors)
-    if torch.is_grad_enabled() and any(x.requires_grad for x in tensors):
-        raise RuntimeError("there is no backward pass: call under torch.no_grad(), or detach the inputs")
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x.requires_grad:
+                raise RuntimeError("there is no backward pass: call under torch.no_grad(), or detach the inputs")
 
 
 def _check_rows(q: Tensor, k: Tensor, names: str) -> None:
@@ -74,7 +76,21 @@ def _check_prefix(prefix_k: Tensor, prefix_v: Tensor, batch: int, kv_heads: int,
     return prefix_k, prefix_v
 
 
-@torch.no_grad()
+_workspaces: dict = {}  # bytes by shape, of the last few shapes
+
+
+def _workspace(*shape) -> int:
+    nbytes = _workspaces.get(shape)
+    if nbytes is None:
+        nbytes = _native.lib().sta_prefix_attention_bytes(*shape)
+        if nbytes < 0:
+            raise _native.NativeError("sta_prefix_attention_bytes refused the shape")
+        if len(_workspaces) >= 64:
+            _workspaces.clear()
+        _workspaces[shape] = nbytes
+    return nbytes
+
+
 def _attention(q: Tensor, k: Tensor, v: Tensor, pk: Tensor, pv: Tensor, lengths: Optional[Tensor],
                counts: Optional[Tensor], prefix_lengths: Optional[Tensor], scale: float,
                with_lse: bool) -> Tuple[Tensor, Optional[Tensor]]:
@@ -88,13 +104,11 @@ def _attention(q: Tensor, k: Tensor, v: Tensor, pk: Tensor, pv: Tensor, lengths:
         wide = _attention(*(_widen(x) for x in (q, k, v, pk, pv)), lengths, counts, prefix_lengths, scale, with_lse)
         return out.copy_(wide[0][..., :dv]), wide[1]
     q, k, v, pk, pv = _rows(q), _rows(k), _rows(v), _rows(pk), _rows(pv)
-    code, lib = _native.DTYPE_CODES[q.dtype], _native.lib()
+    code = _native.DTYPE_CODES[q.dtype]
+    nbytes = _workspace(code, b, h, hk, sets, n, m, p, d, dv)
     with _on(q.device):
-        nbytes = lib.sta_prefix_attention_bytes(code, b, h, hk, sets, n, m, p, d, dv)
-        if nbytes < 0:
-            raise _native.NativeError("sta_prefix_attention_bytes refused the shape")
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
-        st = lib.sta_prefix_attention(
+        st = _native.lib().sta_prefix_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), pk.data_ptr(), pv.data_ptr(), code, b, h, hk, sets, n, m, p, d,
             dv, _strides(q, k, v, pk, pv), scale, _native.ptr(lengths), _native.ptr(counts),
             _native.ptr(prefix_lengths), out.data_ptr(), _native.ptr(lse), _native.ptr(ws), nbytes,
