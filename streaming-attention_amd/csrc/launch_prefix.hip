@@ -27,21 +27,36 @@ int launch_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int values, hip
     return check_launch();
   };
   constexpr int shared = sta::win_lds_bytes<P, IN, true>(), rows = 4 * sta::win_join_floats<P>();
-  const int stage = sta::win_lds_bytes<P, IN, false>(), wide = a.parts && values && rows > stage ? rows : stage;
+  const int by_rows = a.parts && values ? rows : 0;
+  auto least = [&](int bytes) { return bytes > by_rows ? bytes : by_rows; };
+  const int wide = least(sta::win_lds_bytes<P, IN, false>());
+  const int ga = static_cast<int>(grid[0]), gb = static_cast<int>(grid[1]);
+  if constexpr (IN != sta::F32 && (P == 64 || P == 128)) {
+    if (p.stream && !p.share[0] && a.d == P && (!values || a.dv == P)) {
+      const int lds = values ? least(sta::prefix_stream_bytes<P, true>()) : sta::prefix_stream_bytes<P, false>();
+      if (p.walks == 2) {
+        return p.share[1] ? launch(sta::prefix_walks_kernel<P, IN, false, true, true>, lds > shared ? lds : shared, p.walk[0],
+                                   p.walk[1], ga, gb)
+                          : launch(sta::prefix_walks_kernel<P, IN, false, false, true>, lds, p.walk[0], p.walk[1], ga, gb);
+      }
+      return values ? launch(sta::prefix_attention_kernel<P, IN, false, true, true>, lds, p.walk[0])
+                    : launch(sta::prefix_attention_kernel<P, IN, false, false, true>, lds, p.walk[0]);
+    }
+  }
   if (p.walks == 2) {
-    const int both = wide > shared ? wide : shared;
-    const int ga = static_cast<int>(grid[0]), gb = static_cast<int>(grid[1]);
     if (p.share[0] && p.share[1])
-      return launch(sta::prefix_walks_kernel<P, IN, true, true>, shared, p.walk[0], p.walk[1], ga, gb);
-    if (p.share[1]) return launch(sta::prefix_walks_kernel<P, IN, false, true>, both, p.walk[0], p.walk[1], ga, gb);
-    return launch(sta::prefix_walks_kernel<P, IN, false, false>, wide, p.walk[0], p.walk[1], ga, gb);
+      return launch(sta::prefix_walks_kernel<P, IN, true, true, false>, shared, p.walk[0], p.walk[1], ga, gb);
+    if (p.share[1])
+      return launch(sta::prefix_walks_kernel<P, IN, false, true, false>, wide > shared ? wide : shared, p.walk[0], p.walk[1],
+                    ga, gb);
+    return launch(sta::prefix_walks_kernel<P, IN, false, false, false>, wide, p.walk[0], p.walk[1], ga, gb);
   }
   if (values) {
-    return p.share[0] ? launch(sta::prefix_attention_kernel<P, IN, true, true>, shared, p.walk[0])
-                      : launch(sta::prefix_attention_kernel<P, IN, false, true>, wide, p.walk[0]);
+    return p.share[0] ? launch(sta::prefix_attention_kernel<P, IN, true, true, false>, shared, p.walk[0])
+                      : launch(sta::prefix_attention_kernel<P, IN, false, true, false>, wide, p.walk[0]);
   }
-  return p.share[0] ? launch(sta::prefix_attention_kernel<P, IN, true, false>, shared, p.walk[0])
-                    : launch(sta::prefix_attention_kernel<P, IN, false, false>, wide, p.walk[0]);
+  return p.share[0] ? launch(sta::prefix_attention_kernel<P, IN, true, false, false>, shared, p.walk[0])
+                    : launch(sta::prefix_attention_kernel<P, IN, false, false, false>, wide, p.walk[0]);
 }
 
 template <int P, int IN>

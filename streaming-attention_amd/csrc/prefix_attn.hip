@@ -63,10 +63,10 @@ __device__ __forceinline__ float prefix_lse(float top, float den, float c) {
 }
 
 template <int P, int IN, bool SHARE, bool VALUES, bool CAREFUL>
-__device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk& w, int id, int again) {
+__device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk& w, int id, uint4* key_lds, uint4* value_lds,
+                                           int again) {
   constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BK = win_keys<IN, SHARE>(), NSUB = BK / 32,
                 MT = P / 32, STEP = SHARE ? 4 : 1;
-  extern __shared__ uint4 win_lds[];
   // the tiles of a unit, then the units of a key head next to each other: they read the same keys
   const int tile = w.tiles - 1 - id % w.tiles;
   id /= w.tiles;
@@ -74,7 +74,7 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
   id /= w.nsplit;
   const int units = a.batch / w.span, hk = id / units, b0 = (id - hk * units) * w.span;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
-  uint4 *const ks = win_lds + (SHARE ? wave * 2 * BK * CH : 0), *const vs = ks + BK * CH;
+  uint4 *const ks = key_lds + (SHARE ? wave * 2 * BK * CH : 0), *const vs = value_lds + (SHARE ? wave * 2 * BK * CH : 0);
   const int r0 = tile * win_rows<SHARE>(), w0 = r0 + (SHARE ? 0 : 32 * wave);
   const int per = a.n * a.group;  // rows of a sequence
 
@@ -268,7 +268,7 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
   };
 
   if constexpr (SHARE) {
-    float *red = reinterpret_cast<float*>(win_lds), *red_m = red + win_join_floats<P>(), *red_l = red_m + 4 * 32;
+    float *red = reinterpret_cast<float*>(key_lds), *red_m = red + win_join_floats<P>(), *red_l = red_m + 4 * 32;
     __syncthreads();
     if constexpr (VALUES) win_join_put<P>(red, acc, wave, lane);
     if (hh == 0) {
@@ -331,7 +331,7 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
   if (VALUES && a.parts) {
     // Partials by whole rows, through LDS: stored from the lanes that have them, 16 bytes here and there, they cost as much
     // as eight tiles of keys (64 x 32 heads over 32768 rows, 32 shares: 77 us, so 56)
-    float* red = reinterpret_cast<float*>(win_lds);
+    float* red = reinterpret_cast<float*>(key_lds);
     __syncthreads();
     win_join_put<P>(red, acc, wave, lane);
     win_sync<true>();
@@ -359,38 +359,326 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
   return bad;
 }
 
-template <int P, int IN, bool SHARE, bool VALUES>
-__global__ __launch_bounds__(256, (win_row_waves<P, IN, SHARE>())) void prefix_attention_kernel(const PrefixArgs a,
-                                                                                               const PrefixWalk w) {
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
+// A wave's 32 rows over a tile of staged keys: the running maximum and sum of weights, and the value sums.
+template <int P, int IN, int NSUB>
+struct PrefixRows {
+  floatx16 acc[P / 32];
+  float m, limit, l, room;
+
+  // low: where no logit is below it
+  __device__ __forceinline__ void init(float low, float c) {
+#pragma unroll
+    for (int mt = 0; mt < P / 32; ++mt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
+    m = limit = low;
+    l = 0.f;
+    room = win_weight_room<IN>() / c;
+  }
+  __device__ __forceinline__ static void logits(floatx16 (&x)[NSUB], const uint4* ks, const WinFrag<IN> (&qf)[P / 16], int lane) {
+#pragma unroll
+    for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[sub][i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < P / 16; ++s)
+#pragma unroll
+      for (int sub = 0; sub < NSUB; ++sub)
+        win_mma<IN>(x[sub], win_read_row<P, IN>(ks, 32 * sub + (lane & 31), s, lane >> 5), qf[s]);
+  }
+  // logits to weights; all: every row sees every key, else the lane's row sees key k up to `ahead`
+  template <bool VALUES>
+  __device__ __forceinline__ void weights(floatx16 (&x)[NSUB], bool all, int ahead, float c) {
+    if (!all) {
+#pragma unroll
+      for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool seen = 32 * sub + 8 * (i >> 2) + (i & 3) <= ahead;
+          x[sub][i] = seen ? x[sub][i] : -__builtin_inff();
+        }
+    }
+    float top = m;
+#pragma unroll
+    for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, x[sub][i]);
+    // the maximum moves, for both lanes of a row at once, when a weight would exceed 2^room
+    if (__any(top > limit)) {
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float shrink = __builtin_amdgcn_exp2f((m - top) * c);
+      l *= shrink;
+      if constexpr (VALUES) {
+#pragma unroll
+        for (int mt = 0; mt < P / 32; ++mt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[mt][i] *= shrink;
+      }
+      m = top;
+      limit = m + room;
+    }
+    const float mc = m * c - win_weight_lift<IN>();
+#pragma unroll
+    for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        x[sub][i] = __builtin_amdgcn_exp2f(fmaf(x[sub][i], c, -mc));
+      }
+    // a tile's weights first: long rows' sums lose less
+#pragma unroll
+    for (int sub = 0; sub < NSUB; ++sub) {
+      float sum = x[sub][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) sum += x[sub][i];
+      l += sum;
+    }
+  }
+  __device__ __forceinline__ void values(const floatx16 (&x)[NSUB], const uint4* vs, int lane) {
+#pragma unroll
+    for (int sub = 0; sub < NSUB; ++sub)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const WinFrag<IN> p = win_operand<IN>(x[sub], t);
+#pragma unroll
+        for (int mt = 0; mt < P / 32; ++mt)
+          win_mma<IN>(acc[mt], win_read_columns<P, IN>(vs, 32 * sub + 16 * t, mt, lane), p);
+      }
+  }
+};
+
+// The first pass for 16-bit heads exactly P wide on 16 bytes, wide tiles: that of prefix_pass with tiles that go from memory to LDS
+// directly, keys and values of even and of odd tiles in buffers of their own, so that one barrier a tile is enough and a
+// tile's value products run into the next one's logits.  The buffers are restrict arguments: the compiler then sees that
+// reads of one need not wait for loads to another.  32 x 512 rows of 8 sequences behind 16384, 128 wide, 1.29 -> 1.12 ms
+// (1000 TFLOP/s; a large matrix product 1200), 64 wide 0.38 -> 0.35 ms; 32 heads' statistics of 16384 rows 1.25 -> 1.06 ms.
+typedef const __attribute__((address_space(1))) void* stream_global;
+typedef __attribute__((address_space(3))) void* stream_lds;
+
+// Where a lane's units of a tile lie in memory, from its first row: unit (NJ wave + j) 64 + lane of the tile's order in LDS
+template <int P>
+struct StreamTile {
+  static constexpr int CH = P / 8, NJ = 64 * CH / 256;
+  int pitch, at[NJ];
+
+  __device__ __forceinline__ static int unit(int j) { return static_cast<int>(NJ * (threadIdx.x >> 6) + j) * 64 + (threadIdx.x & 63); }
+  __device__ __forceinline__ void init(int64_t row_elements) {
+    pitch = static_cast<int>(row_elements) * 2;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int u = unit(j), r = u / CH;
+      at[j] = r * pitch + ((u % CH) ^ win_swizzle<CH>(r)) * 16;
+    }
+  }
+  // rows behind the last are read as the last one: their logits are hidden, their weights 0
+  __device__ __forceinline__ void load(const char* row, int left, uint4* lds) const {
+    const int first = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * NJ * 64;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      uint32_t off = at[j];
+      if (left < 64) off -= max(0, unit(j) / CH - left + 1) * pitch;
+      __builtin_amdgcn_global_load_lds((stream_global)(row + off), (stream_lds)(lds + first + 64 * j), 16, 0, 0);
+    }
+  }
+};
+
+// a barrier behind the wave's loads to LDS and its LDS reads
+__device__ __forceinline__ void stream_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0), lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <int P, bool VALUES>
+__host__ __device__ constexpr int prefix_stream_bytes() { return (VALUES ? 4 : 2) * 64 * P * 2; }
+
+template <int P, int IN, bool VALUES>
+__device__ __forceinline__ int prefix_stream_pass(const PrefixArgs& a, const PrefixWalk& w, int id, float* red,
+                                                  uint4* __restrict__ ks0, uint4* __restrict__ ks1,
+                                                  uint4* __restrict__ vs0, uint4* __restrict__ vs1) {
+  constexpr int MT = P / 32, BK = 64, NSUB = 2;
+  const int tile = w.tiles - 1 - id % w.tiles;
+  id /= w.tiles;
+  const int split = id % w.nsplit;
+  id /= w.nsplit;
+  const int units = a.batch / w.span, hk = id / units, b0 = (id - hk * units) * w.span;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hh = lane >> 5;
+  const int r0 = tile * WIN_ROWS, w0 = r0 + 32 * wave, per = a.n * a.group;
+
+  // the lane's row
+  const int row = w0 + (lane & 31);
+  const bool in = row < w.span * per;
+  const int bl = (in ? row : 0) / per, z = (in ? row : 0) - bl * per, b = b0 + bl, i = z / a.group, h = hk * a.group + z - i * a.group;
+  const int64_t at = (static_cast<int64_t>(b) * a.heads + h) * a.n + i;
+  const int my_length = prefix_length(a, b), my_count = prefix_count(a, b, my_length);
+  const bool live = in && i < my_count;
+  const int my_lim = my_length - my_count + i;
+
+  const int set = b0 / a.per_set, rows_p = w.prefix ? prefix_rows(a, set) : 0;
+  int own_end = 0, base = 0, count = a.n;
+  if (w.own) {
+    const int length = prefix_length(a, b0);
+    count = prefix_count(a, b0, length);
+    base = length - count;
+    const int last = (r0 + WIN_ROWS - 1) / a.group;
+    own_end = r0 / a.group < count ? base + (last < count ? last + 1 : count) : 0;
+  }
+  const bool any = w.own ? own_end > 0 : r0 < w.span * per;
+  const int tiles_p = any ? (rows_p + BK - 1) / BK : 0, all_tiles = tiles_p + (own_end + BK - 1) / BK;
+  const int own_first = (split + w.nsplit - tiles_p % w.nsplit) % w.nsplit;
+
+  PrefixRows<P, IN, NSUB> sums;
+  sums.init(-1e30f, a.c);
+  if (split < all_tiles) {
+    WinFrag<IN> qf[P / 16];
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+    const char* qrow = rows_at<2>(a.q, b, h, i);
+#pragma unroll
+    for (int s = 0; s < P / 16; ++s) {
+      qf[s] = win_load_row<IN>(qrow, s, hh, P, flip);
+      win_keep<IN>(qf[s], live);
+    }
+#pragma unroll 1
+    for (int seg = 0; seg < 2; ++seg) {
+      const Rows kr = seg ? a.k : a.pk, vr = seg ? a.v : a.pv;
+      const int rb = seg ? b0 : set, end = seg ? own_end : rows_p;
+      const int lo = seg ? own_first : split, hi = seg ? all_tiles - tiles_p : tiles_p, step = w.nsplit;
+      if (lo >= hi) continue;
+      const int lim = seg ? my_lim : rows_p - 1;
+      const int lim_lo = seg ? base + w0 / a.group : rows_p - 1;
+      const int lim_hi = seg ? base + min((w0 + 31) / a.group, count - 1) : rows_p - 1;
+      StreamTile<P> kt, vt;
+      kt.init(kr.sn);
+      if constexpr (VALUES) vt.init(vr.sn);
+      const char *const kp = rows_at<2>(kr, rb, hk, 0), *const vp = VALUES ? rows_at<2>(vr, rb, hk, 0) : nullptr;
+      // nothing behind the last tile
+      auto keys = [&](int it, uint4* to) {
+        if (it < hi) kt.load(kp + static_cast<int64_t>(it) * BK * kt.pitch, end - it * BK, to);
+      };
+      auto values = [&](int it, uint4* to) {
+        if constexpr (VALUES) {
+          if (it < hi) vt.load(vp + static_cast<int64_t>(it) * BK * vt.pitch, end - it * BK, to);
+        }
+      };
+      // a tile, from keys and values that are there when it begins and when its weights are taken
+      auto turn = [&](int it, uint4* ks, const uint4* vs, uint4* next) {
+        const int key0 = it * BK, active = key0 <= lim_hi;
+        floatx16 x[NSUB];
+        if (active) {
+          sums.logits(x, ks, qf, lane);
+          sums.template weights<VALUES>(x, key0 + BK - 1 <= lim_lo, lim - key0 - 4 * hh, a.c);
+        }
+        // these keys and the values before are done with; the next keys and these values are there
+        stream_barrier();
+        keys(it + 2 * step, ks);
+        values(it + step, next);
+        if (VALUES && active) sums.values(x, vs, lane);
+      };
+      keys(lo, ks0);
+      keys(lo + step, ks1);
+      values(lo, vs0);
+      stream_barrier();
+#pragma unroll 1
+      for (int it = lo; it < hi; it += 2 * step) {
+        turn(it, ks0, vs0, vs1);
+        if (it + step < hi) turn(it + step, ks1, vs1, vs0);
+      }
+      stream_barrier();
+    }
+    sums.l += __shfl_xor(sums.l, 32);
+  }
+
+  int bad = 0;
+  if (live) {
+    const bool sees = split < tiles_p || (split < all_tiles && own_first * BK <= my_lim);
+    bad = !win_finite(sums.l) || (sees && !(sums.l > 0.f));
+    if constexpr (VALUES) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) bad |= !win_finite(sums.acc[mt][e]);
+    }
+  }
+  bad |= __shfl_xor(bad, 32);
+  const bool store = in && !bad;
+  if (a.parts) {
+    const int64_t part = at * a.parts + w.first + split;
+    if constexpr (VALUES) {  // by whole rows, see prefix_pass
+      __syncthreads();
+      win_join_put<P>(red, sums.acc, wave, lane);
+      win_sync<true>();
+      constexpr int UNITS = P / 4;
+#pragma unroll 4
+      for (int u = 0; u < UNITS / 2; ++u) {
+        const int unit = 64 * u + lane, r = unit / UNITS, col = 4 * (unit % UNITS);
+        const int lo = __shfl(static_cast<int>(part), r), hi = __shfl(static_cast<int>(part >> 32), r);
+        const int64_t to = static_cast<int64_t>(hi) << 32 | static_cast<uint32_t>(lo);
+        if (__shfl(static_cast<int>(store), r))
+          *reinterpret_cast<floatx4*>(a.part + to * P + col) = *reinterpret_cast<floatx4*>(&red[(wave * 32 + r) * (P + 4) + col]);
+      }
+    }
+    if (store && hh == 0)
+      *reinterpret_cast<floatx2*>(a.stat + 2 * part) = floatx2{prefix_top(sums.m, sums.l), sums.l};
+  } else if (store) {
+    const float inv = 1.f / sums.l;
+    if constexpr (VALUES) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          win_store4<IN>(a.out, at * P, 32 * mt + 8 * r + 4 * hh, P, live ? sums.acc[mt][4 * r] * inv : 0.f,
+                         live ? sums.acc[mt][4 * r + 1] * inv : 0.f, live ? sums.acc[mt][4 * r + 2] * inv : 0.f,
+                         live ? sums.acc[mt][4 * r + 3] * inv : 0.f);
+    }
+    if (a.lse && hh == 0) a.lse[at] = live ? prefix_lse<IN>(sums.m, sums.l, a.c) : 0.f;
+  }
+  return bad;
+}
+
+// both passes over a walk, see win_passes
+template <int P, int IN, bool SHARE, bool VALUES, bool STREAM>
+__device__ __forceinline__ void prefix_passes(const PrefixArgs& a, const PrefixWalk& w, int id, uint4* lds) {
+  constexpr int VALUE_UNITS = win_keys<IN, SHARE>() * win_chunks<IN == F32 ? 4 : 2>(P);
   win_passes([&](auto second, int again) {
-    return prefix_pass<P, IN, SHARE, VALUES, decltype(second)::value>(a, w, id, again);
+    constexpr bool CAREFUL = decltype(second)::value;
+    if constexpr (STREAM && !CAREFUL) {
+      constexpr int UNITS = 64 * P / 8;
+      return prefix_stream_pass<P, IN, VALUES>(a, w, id, reinterpret_cast<float*>(lds), lds, lds + UNITS, lds + 2 * UNITS,
+                                               lds + 3 * UNITS);
+    } else {
+      return prefix_pass<P, IN, SHARE, VALUES, CAREFUL>(a, w, id, lds, lds + VALUE_UNITS, again);
+    }
   });
+}
+// waves a SIMD
+template <int P, int IN, bool SHARE, bool VALUES, bool STREAM>
+__host__ __device__ constexpr int prefix_waves() {
+  return STREAM ? (VALUES ? (P > 64 ? 2 : 3) : 4) : win_row_waves<P, IN, SHARE>();
+}
+
+template <int P, int IN, bool SHARE, bool VALUES, bool STREAM>
+__global__ __launch_bounds__(256, (prefix_waves<P, IN, SHARE, VALUES, STREAM>())) void prefix_attention_kernel(
+    const PrefixArgs a, const PrefixWalk w) {
+  extern __shared__ uint4 win_lds[];
+  prefix_passes<P, IN, SHARE, VALUES, STREAM>(a, w, xcd_remap(blockIdx.x, gridDim.x), win_lds);
 }
 
 // Both walks of a batch of few rows in one launch: that over the prefix is bound by products and by latency, that over the
 // own tokens by memory.  64 x 32 heads, 128 wide, 32768 shared and up to 1024 own rows: 56 and 32 us one after the other, 78
 // together, with the prefix's workgroups first (98 with the two in turn).
-template <int P, int IN, bool SHARE_A, bool SHARE_B>
-__global__ __launch_bounds__(256, (win_row_waves<P, IN, SHARE_B>() < win_row_waves<P, IN, SHARE_A>()
-                                       ? win_row_waves<P, IN, SHARE_B>()
-                                       : win_row_waves<P, IN, SHARE_A>())) void
+template <int P, int IN, bool SHARE_A, bool SHARE_B, bool STREAM>
+__global__ __launch_bounds__(256, (prefix_waves<P, IN, SHARE_B, true, false>() < prefix_waves<P, IN, SHARE_A, true, STREAM>()
+                                       ? prefix_waves<P, IN, SHARE_B, true, false>()
+                                       : prefix_waves<P, IN, SHARE_A, true, STREAM>())) void
 prefix_walks_kernel(const PrefixArgs a, const PrefixWalk wa, const PrefixWalk wb, int grid_a, int grid_b) {
+  extern __shared__ uint4 win_lds[];
   // each walk's neighbours on one XCD, the first walk's workgroups before the second's
   const int xcds = grid_a % 8 == 0 && grid_b % 8 == 0 ? 8 : 1, xcd = blockIdx.x % xcds, slot = blockIdx.x / xcds;
   const int ga = grid_a / xcds, gb = grid_b / xcds;
-  const bool first = slot < ga;
-  if (first) {
-    const int id = xcd * ga + slot;
-    win_passes([&](auto second, int again) {
-      return prefix_pass<P, IN, SHARE_A, true, decltype(second)::value>(a, wa, id, again);
-    });
-  } else {
-    const int id = xcd * gb + slot - ga;
-    win_passes([&](auto second, int again) {
-      return prefix_pass<P, IN, SHARE_B, true, decltype(second)::value>(a, wb, id, again);
-    });
-  }
+  if (slot < ga)
+    prefix_passes<P, IN, SHARE_A, true, STREAM>(a, wa, xcd * ga + slot, win_lds);
+  else
+    prefix_passes<P, IN, SHARE_B, true, false>(a, wb, xcd * gb + slot - ga, win_lds);
 }
 
 // The partials of a row: a workgroup of 128 threads a row, a thread a column.  Bound by latency, so that the partials' loads

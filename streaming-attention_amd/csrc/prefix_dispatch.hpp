@@ -27,7 +27,16 @@ int prefix_by_type(int dtype, int width, Call call) {
   return STA_ERR_UNSUPPORTED;
 }
 
-inline int run_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int dtype, int values, hipStream_t s) {
+// rows on 16 bytes (of 2-byte elements)
+inline bool on_units(const sta::Rows& t) {
+  return ((reinterpret_cast<uintptr_t>(t.p) | 2 * t.sb | 2 * t.sh | 2 * t.sn) & 15) == 0;
+}
+
+// the walks of a plan
+inline int run_prefix(const sta::PrefixArgs& a, PrefixPlan p, int dtype, int values, hipStream_t s) {
+  const bool prefix = p.walk[0].prefix, own = p.walks == 1 && p.walk[0].own;  // of the first walk
+  p.stream = (!own || on_units(a.k)) && (!prefix || on_units(a.pk)) &&
+             (!values || ((!own || on_units(a.v)) && (!prefix || on_units(a.pv))));
   return prefix_by_type(dtype, values && a.dv > a.d ? a.dv : a.d, [&](auto width, auto in) {
     return launch_prefix<decltype(width)::value, decltype(in)::value>(a, p, values, s);
   });

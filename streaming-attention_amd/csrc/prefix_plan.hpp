@@ -16,6 +16,7 @@ struct PrefixPlan {
   sta::PrefixWalk walk[2];
   int share[2];
   int parts;        // 0: one workgroup finishes a row
+  int stream;       // the first walk's keys and values lie on 16 bytes: prefix_stream_pass where the widths allow it
 };
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
