@@ -122,6 +122,7 @@ int sta_received_attention(const void* q, const void* k, int dtype, int64_t batc
   a.lengths = lengths;
   a.counts = counts;
   plan_received(w, dtype);
+  w.stream = on_units(a.q);
   char* room = static_cast<char*>(workspace);
   w.sums = reinterpret_cast<float*>(room);
   room += received_sum_bytes(w);

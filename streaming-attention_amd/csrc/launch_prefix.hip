@@ -72,9 +72,15 @@ int launch_received(const sta::ReceivedArgs& w, hipStream_t s) {
       if (e != hipSuccess) return hip_status(e);
     }
     hipLaunchKernelGGL((sta::received_few_kernel<P, IN>), g, dim3(256), lds, s, w);
-  } else {
-    hipLaunchKernelGGL((sta::received_kernel<P, IN>), g, dim3(256), 0, s, w);
+    return check_launch();
   }
+  if constexpr (IN != sta::F32 && (P == 64 || P == 128)) {
+    if (w.stream && w.a.d == P) {
+      hipLaunchKernelGGL((sta::received_kernel<P, IN, true>), g, dim3(256), 0, s, w);
+      return check_launch();
+    }
+  }
+  hipLaunchKernelGGL((sta::received_kernel<P, IN, false>), g, dim3(256), 0, s, w);
   return check_launch();
 }
 

@@ -739,6 +739,7 @@ __global__ __launch_bounds__(128) void prefix_join_kernel(const PrefixArgs a) {
 struct ReceivedArgs {
   PrefixArgs a;          // q, own k; lse: the rows' statistics
   int few;               // up to RECEIVED_FEW rows: received_few_kernel
+  int stream;            // rows on 16 bytes
   int tiles, nsplit;     // workgroups of a key head along its keys, and along the rows (few: 1)
   float* sums;           // [nsplit][batch][kv][m], or the weights themselves with one
   float* weights;        // [batch][kv][m]
@@ -794,15 +795,15 @@ __device__ __forceinline__ void received_add(float& total, float& lost, const fl
 // The weights that keys receive.  A workgroup holds 32 to 64 keys a wave as operands and walks over its share of the rows
 // that see one of them, head by head of the group; with X = Q K^T a lane has 16 rows of one key, whose weights it sums: no
 // exchange between lanes until the end.  Sums of 16 go into a compensated total (16384 x 4 rows).  32 heads of 16384 rows,
-// 128 wide: 1.32 ms, 830 TFLOP/s (a large matrix product 1200); 64 wide 0.76 ms, bound by the exponentials.
-template <int P, int IN>
-__global__ __launch_bounds__(256, 2) void received_kernel(const ReceivedArgs w) {
-  constexpr int ES = IN == F32 ? 4 : 2, CH = win_chunks<ES>(P), BQ = received_rows<IN>(), NB = received_blocks<IN>();
-  __shared__ uint4 qs[BQ * CH];
-  __shared__ __attribute__((aligned(16))) float stat[BQ];
+// 128 wide: 1.14 ms, 965 TFLOP/s (a large matrix product 1200); 64 wide 0.75 ms, bound by the exponentials.
+// STREAM: 16-bit rows exactly P wide on 16 bytes go from memory to LDS directly, a tile ahead in two buffers, with one
+// barrier a tile, and leave room for a third wave a SIMD (1.32 -> 1.22 -> 1.14 ms, 965 TFLOP/s).
+template <int P, int IN, bool STREAM>
+__device__ __forceinline__ void received_walk(const ReceivedArgs& w, int id, uint4* __restrict__ qs0, uint4* __restrict__ qs1,
+                                              float* __restrict__ stat0, float* __restrict__ stat1) {
+  constexpr int ES = IN == F32 ? 4 : 2, BQ = received_rows<IN>(), NB = received_blocks<IN>();
   const PrefixArgs& a = w.a;
   // a tile's workgroups, then the tiles of a key head next to each other, those that most rows see first
-  int id = xcd_remap(blockIdx.x, gridDim.x);
   const int split = id % w.nsplit;
   id /= w.nsplit;
   const int tile = id % w.tiles, unit = id / w.tiles, b = unit / a.kv, hk = unit - b * a.kv;
@@ -829,28 +830,26 @@ __global__ __launch_bounds__(256, 2) void received_kernel(const ReceivedArgs w) 
         win_keep<IN>(kf[n][s], key < length);
       }
     }
-    WinStage<P, IN, BQ, 256> stage;
-    stage.init(a.q, a.d);
-    float next = 0.f;
-    int g = t0 / row_tiles, i = i0 + (t0 - g * row_tiles) * BQ;  // of the tile that is loaded next
-    auto load = [&]() {
-      const int h = hk * a.group + g, r = i + static_cast<int>(threadIdx.x % BQ);
-      stage.load(rows_at<ES>(a.q, b, h, i), count - i);
-      next = received_stat(a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.n + (r < count ? r : count - 1)], r < count);
+    // a tile of rows: head g of the group, rows from i on
+    struct At {
+      int g, i;
     };
-    load();
-    for (int it = t0; it < t1; ++it) {
-      const int row = i;
-      __syncthreads();
-      stage.put(qs, count - row);
-      if (threadIdx.x < BQ) stat[threadIdx.x] = next;
-      __syncthreads();
-      i += BQ;
-      if (i >= count) {
-        i = i0;
-        ++g;
+    At next{t0 / row_tiles, i0 + (t0 % row_tiles) * BQ};  // of the tile that is loaded next
+    auto advance = [&]() {
+      const At x = next;
+      next.i += BQ;
+      if (next.i >= count) {
+        next.i = i0;
+        ++next.g;
       }
-      if (it + 1 < t1) load();
+      return x;
+    };
+    auto stat_of = [&](const At& x) {
+      const int h = hk * a.group + x.g, r = x.i + static_cast<int>(threadIdx.x % BQ);
+      return received_stat(a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.n + (r < count ? r : count - 1)], r < count);
+    };
+    auto rows_of = [&](const At& x) { return rows_at<ES>(a.q, b, hk * a.group + x.g, x.i); };
+    auto take = [&](int row, const uint4* qs, const float* stat) {
       const bool every = base + row >= w0 + 32 * NB - 1;
 #pragma unroll
       for (int sub = 0; sub < BQ / 32; ++sub) {
@@ -868,6 +867,55 @@ __global__ __launch_bounds__(256, 2) void received_kernel(const ReceivedArgs w) 
 #pragma unroll
         for (int n = 0; n < NB; ++n) received_add(total[n], lost[n], x[n]);
       }
+    };
+    if constexpr (STREAM) {
+      StreamTile<P> qt;
+      qt.init(a.q.sn);
+      At x = advance();
+      qt.load(rows_of(x), count - x.i, qs0);
+      if (threadIdx.x < BQ) stat0[threadIdx.x] = stat_of(x);
+      int row = x.i, coming = 0;
+      float stat = 0.f;
+      auto load = [&](int it, uint4* qs) {  // the tile behind `it`, if there is one
+        if (it + 1 >= t1) return;
+        x = advance();
+        qt.load(rows_of(x), count - x.i, qs);
+        stat = stat_of(x);
+        coming = x.i;
+      };
+      // a tile; then the next one is there
+      auto turn = [&](int it, const uint4* qs, const float* st, uint4* after, float* after_stat) {
+        load(it, after);
+        take(row, qs, st);
+        if (it + 1 < t1 && threadIdx.x < BQ) after_stat[threadIdx.x] = stat;
+        row = coming;
+        stream_barrier();
+      };
+      stream_barrier();
+#pragma unroll 1
+      for (int it = t0; it < t1; it += 2) {
+        turn(it, qs0, stat0, qs1, stat1);
+        if (it + 1 < t1) turn(it + 1, qs1, stat1, qs0, stat0);
+      }
+    } else {
+      WinStage<P, IN, BQ, 256> stage;
+      stage.init(a.q, a.d);
+      At x = advance();
+      stage.load(rows_of(x), count - x.i);
+      float stat = stat_of(x);
+      for (int it = t0; it < t1; ++it) {
+        const int row = x.i;
+        __syncthreads();
+        stage.put(qs0, count - row);
+        if (threadIdx.x < BQ) stat0[threadIdx.x] = stat;
+        __syncthreads();
+        if (it + 1 < t1) {
+          x = advance();
+          stage.load(rows_of(x), count - x.i);
+          stat = stat_of(x);
+        }
+        take(row, qs0, stat0);
+      }
     }
   }
   float* const to = (w.nsplit == 1 ? w.weights : w.sums + static_cast<int64_t>(split) * a.batch * a.kv * a.m) +
@@ -878,6 +926,14 @@ __global__ __launch_bounds__(256, 2) void received_kernel(const ReceivedArgs w) 
     const int key = w0 + 32 * n + (lane & 31);
     if (hh == 0 && key < a.m) to[key] = key < length ? total[n] : 0.f;
   }
+}
+
+template <int P, int IN, bool STREAM>
+__global__ __launch_bounds__(256, (STREAM ? 3 : 2)) void received_kernel(const ReceivedArgs w) {
+  constexpr int UNITS = received_rows<IN>() * win_chunks<IN == F32 ? 4 : 2>(P), BQ = received_rows<IN>();
+  __shared__ uint4 qs[(STREAM ? 2 : 1) * UNITS];
+  __shared__ __attribute__((aligned(16))) float stat[2 * BQ];
+  received_walk<P, IN, STREAM>(w, xcd_remap(blockIdx.x, gridDim.x), qs, qs + (STREAM ? UNITS : 0), stat, stat + BQ);
 }
 
 // The same for up to RECEIVED_FEW rows, those of the group's heads together (row i of head g at i group + g): they stay in
