@@ -164,7 +164,7 @@ int64_t sta_heavy_attention_bytes(int dtype, int64_t streams, int heads, int kv_
   }
   sta::PrefixArgs x;
   if (prefix_of(x, h.r, dtype, sets, p, 1.f) != STA_OK) return -1;
-  const int parts = plan_prefix(x, false).parts;
+  const int parts = plan_prefix(x, dtype, false).parts;
   plan_heavy(h, parts);
   return workspace_of(h, &x, parts).total();
 }
@@ -197,7 +197,7 @@ int sta_heavy_attention(const void* q, const void* k, const void* v, int dtype, 
   if (p > 0) {
     if (const int st = prefix_of(x, a, dtype, sets, p, scale)) return st;
     if (!prefix_strides_ok(prefix_strides, 2, dtype)) return STA_ERR_UNSUPPORTED;
-    plan = plan_prefix(x, false);
+    plan = plan_prefix(x, dtype, false);
   }
   plan_heavy(h, plan.parts);
   const Workspace w = workspace_of(h, p > 0 ? &x : nullptr, plan.parts);

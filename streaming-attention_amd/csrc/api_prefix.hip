@@ -60,7 +60,7 @@ int64_t sta_prefix_attention_bytes(int dtype, int64_t batch, int heads, int kv_h
                                    int64_t p, int d, int dv) {
   sta::PrefixArgs a;
   if (prefix_shape(a, dtype, batch, heads, kv_heads, sets, n, m, p, d, dv, 1.f) != STA_OK || m < 1 || dv < 1) return -1;
-  return prefix_part_bytes(a, plan_prefix(a, true).parts);
+  return prefix_part_bytes(a, plan_prefix(a, dtype, true).parts);
 }
 
 int sta_prefix_attention(const void* q, const void* k, const void* v, const void* prefix_k, const void* prefix_v, int dtype,
@@ -74,7 +74,7 @@ int sta_prefix_attention(const void* q, const void* k, const void* v, const void
   if (m < 1 || dv < 1) return STA_ERR_SHAPE;
   if (!aligned16(out)) return STA_ERR_ARG;
   if (!prefix_strides_ok(strides, p > 0 ? 5 : 3, dtype)) return STA_ERR_UNSUPPORTED;
-  const PrefixPlan plan = plan_prefix(a, true);
+  const PrefixPlan plan = plan_prefix(a, dtype, true);
   const int64_t need = prefix_part_bytes(a, plan.parts);
   if (need > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < need)) return STA_ERR_SCRATCH;
   a.q = prefix_rows_of(q, strides);
@@ -101,7 +101,7 @@ int64_t sta_received_attention_bytes(int dtype, int64_t batch, int heads, int kv
   if (prefix_shape(w.a, dtype, batch, heads, kv_heads, batch, n, m, 0, d, 0, 1.f) != STA_OK || m < 1) return -1;
   plan_received(w, dtype);
   int64_t bytes = received_sum_bytes(w);
-  if (!with_lse) bytes += received_lse_bytes(w.a) + prefix_part_bytes(w.a, plan_prefix(w.a, true).parts);
+  if (!with_lse) bytes += received_lse_bytes(w.a) + prefix_part_bytes(w.a, plan_prefix(w.a, dtype, true).parts);
   return bytes;
 }
 
@@ -133,7 +133,7 @@ int sta_received_attention(const void* q, const void* k, int dtype, int64_t batc
   } else {
     a.lse = reinterpret_cast<float*>(room);
     room += received_lse_bytes(a);
-    const PrefixPlan plan = plan_prefix(a, true);
+    const PrefixPlan plan = plan_prefix(a, dtype, true);
     set_parts(a, room, plan.parts);
     int st = run_prefix(a, plan, dtype, 0, s);
     if (st == STA_OK && plan.parts) st = join_rows(a, dtype, s);

@@ -615,11 +615,12 @@ __device__ __forceinline__ float heavy_given(float w) { return w == w ? w + 0.f 
 // largest weights, of equal ones the first.  Three passes over the weights find the smallest that stays, 11 bits of its
 // order at a time (the highest first, among those that agree with it so far): the weights of a prompt lie within a few powers
 // of two, so that bins of 8 bits, the sign and 7 of the exponent's, would all be added to in one place.  One more pass puts the
-// rows that stay down in their order.  The first 16384 weights are held in registers.  16 x 8 key heads of 8192 rows: 20 us.
+// rows that stay down in their order.  Bound by its barriers.  The first 8192 weights are held in registers.  16 x 8 key heads of 8192 rows: 16
+// us (the last pass 1024 at a time: 20; 8 x 65536 79 and 111).
 __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFill f) {
   const HeavyArgs& h = f.h;
-  constexpr int HOLD = 16, BINS = 2048;
-  __shared__ int bins[BINS], wave_sum[2][16], chosen[2];
+  constexpr int HOLD = 8, BINS = 2048;
+  __shared__ int bins[BINS], wave_sum[16], chosen[2], cells[16 * HOLD];
   __shared__ unsigned long long red_low[16];
   const int sh = blockIdx.x, s = sh / h.r.kv, n = heavy_take(f, s), t = threadIdx.x, lane = t & 63, wave = t >> 6;
   if (n == 0) return;
@@ -646,8 +647,11 @@ __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFi
         if (low + bits == 32 || u >> (low + bits) == least >> (low + bits)) atomicAdd(&bins[(u >> low) & mask], 1);
       };
 #pragma unroll
-      for (int j = 0; j < HOLD; ++j)
-        if (t + 1024 * j < older) put(hold[j]);
+      for (int j = 0; j < HOLD; ++j) {
+        if (1024 * j < older) {
+          if (t + 1024 * j < older) put(hold[j]);
+        }
+      }
       for (int i = t + 1024 * HOLD; i < older; i += 1024) put(heavy_given(given[i]));
       __syncthreads();
       // the highest bin with `want` at or above it: sums from above, two bins a thread
@@ -657,10 +661,10 @@ __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFi
         const int y = __shfl_up(before, o);
         if (lane >= o) before += y;
       }
-      if (lane == 63) wave_sum[0][wave] = before;
+      if (lane == 63) wave_sum[wave] = before;
       __syncthreads();
       before -= part[0] + part[1];
-      for (int j = 0; j < wave; ++j) before += wave_sum[0][j];
+      for (int j = 0; j < wave; ++j) before += wave_sum[j];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         if (before < want && before + part[j] >= want) {
@@ -676,44 +680,92 @@ __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFi
     }
     equal = want;
   }
-  // the rows that stay, in their order
+  // The rows that stay, in their order, 8192 at a time: counts by 64 rows of those equal to the smallest, then of those that
+  // stay, each summed up by one wave.
   unsigned long long low = HEAVY_NONE;
   int taken = 0, ties = 0;
-  auto place = [&](int i, float w) {
-    const uint32_t u = heavy_order(w);
-    const bool tie = i < older && u == least && equal != 0x7fffffff;
-    const unsigned long long ballot = __ballot(tie), below = (1ull << lane) - 1ull;
-    if (lane == 0) wave_sum[0][wave] = __popcll(ballot);
+  const unsigned long long below = (1ull << lane) - 1ull;
+  auto sum_up = [&](int& total) {  // cells become what is before them, and total's old value with it
     __syncthreads();
-    int rank = ties + __popcll(ballot & below), all = 0;
-    for (int j = 0; j < 16; ++j) {
-      if (j < wave) rank += wave_sum[0][j];
-      all += wave_sum[0][j];
-    }
-    ties += all;
-    const bool stays = i < older && (equal == 0x7fffffff || u > least || (tie && rank < equal));
-    const unsigned long long kept = __ballot(stays);
-    if (lane == 0) wave_sum[1][wave] = __popcll(kept);
-    __syncthreads();
-    int at = taken + __popcll(kept & below);
-    all = 0;
-    for (int j = 0; j < 16; ++j) {
-      if (j < wave) at += wave_sum[1][j];
-      all += wave_sum[1][j];
-    }
-    taken += all;
-    if (stays) {
-      const int slot = h.ring + at;
-      token[slot] = i;
-      weights[slot] = w;
-      positions[slot] = i;
-      low = heavy_min(low, heavy_key(w, slot));
-    }
-  };
+    if (wave == 0) {
+      int part[HOLD / 4], sum = 0;
 #pragma unroll
-  for (int j = 0; j < HOLD; ++j)
-    if (1024 * j < older) place(1024 * j + t, hold[j]);
-  for (int i0 = 1024 * HOLD; i0 < older; i0 += 1024) place(i0 + t, i0 + t < older ? heavy_given(given[i0 + t]) : 0.f);
+      for (int j = 0; j < HOLD / 4; ++j) {
+        part[j] = cells[HOLD / 4 * lane + j];
+        sum += part[j];
+      }
+      int before = sum;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(before, o);
+        if (lane >= o) before += y;
+      }
+      if (lane == 63) chosen[0] = before;
+      before -= sum;
+#pragma unroll
+      for (int j = 0; j < HOLD / 4; ++j) {
+        cells[HOLD / 4 * lane + j] = total + before;
+        before += part[j];
+      }
+    }
+    __syncthreads();
+    total += chosen[0];
+  };
+  for (int i0 = 0; i0 < older; i0 += 1024 * HOLD) {
+    uint32_t stays = 0u;
+    const int live = min(HOLD, (older - i0 + 1023) / 1024);  // of hold
+    if (i0 > 0) {
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j) {
+        const int i = i0 + 1024 * j + t;
+        hold[j] = i < older ? heavy_given(given[i]) : 0.f;
+      }
+    }
+    if (equal != 0x7fffffff) {
+      uint32_t tie = 0u;
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j) {
+        bool in = false;
+        if (j < live) in = i0 + 1024 * j + t < older && heavy_order(hold[j]) == least;
+        const unsigned long long ballot = __ballot(in);
+        if (lane == 0) cells[16 * j + wave] = __popcll(ballot);
+        tie |= static_cast<uint32_t>(in) << j;
+      }
+      sum_up(ties);
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j) {
+        if (j < live) {
+          const bool in = tie >> j & 1u;
+          const int rank = cells[16 * j + wave] + __popcll(__ballot(in) & below);
+          const bool stay = i0 + 1024 * j + t < older && (heavy_order(hold[j]) > least || (in && rank < equal));
+          stays |= static_cast<uint32_t>(stay) << j;
+        }
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int j = 0; j < HOLD; ++j) stays |= static_cast<uint32_t>(i0 + 1024 * j + t < older) << j;
+    }
+#pragma unroll
+    for (int j = 0; j < HOLD; ++j) {
+      const unsigned long long ballot = __ballot(stays >> j & 1u);
+      if (lane == 0) cells[16 * j + wave] = __popcll(ballot);
+    }
+    sum_up(taken);
+#pragma unroll
+    for (int j = 0; j < HOLD; ++j) {
+      if (j < live) {
+        const bool stay = stays >> j & 1u;
+        const int slot = h.ring + cells[16 * j + wave] + __popcll(__ballot(stay) & below);
+        if (stay) {
+          token[slot] = i0 + 1024 * j + t;
+          weights[slot] = hold[j];
+          positions[slot] = i0 + 1024 * j + t;
+          low = heavy_min(low, heavy_key(hold[j], slot));
+        }
+      }
+    }
+    __syncthreads();
+  }
   for (int slot = h.ring + taken + t; slot < h.pitch; slot += 1024) {
     token[slot] = -1;
     weights[slot] = 0.f;

@@ -23,23 +23,26 @@ inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // One walk over `keys` keys of units of `rows` rows: the tile and the number of workgroups that share a tile's keys.
 // Up to 64 rows: tiles of 32 whose waves share the keys (8 key heads of 16384 x 128 and 64 rows: 27 us, 32 with a tile of
-// 128; 96 rows 33 and 33, 128 rows 38 and 34).  A share has at least 256 keys; room: workgroups that the walk is to fill the
-// card with, which holds 512 at a time (256 compute units, two each of 128 columns).
-inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows, int64_t keys, int64_t room) {
+// 128; 96 rows 33 and 33, 128 rows 38 and 34).  A share has at least `least` keys; room: workgroups that the walk is to fill
+// the card with, which holds 512 at a time (256 compute units, two each of 128 columns).
+inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows, int64_t keys, int64_t room, int64_t least) {
   share = rows <= 64;
   w.tiles = static_cast<int>(ceil_div(rows, share ? 32 : sta::WIN_ROWS));
   int64_t want = room / (units * w.tiles);
-  const int64_t most = ceil_div(keys, 256);
+  const int64_t most = ceil_div(keys, least);
   if (want > most) want = most;
   if (want > kMaxPrefixParts / 2) want = kMaxPrefixParts / 2;
   w.nsplit = static_cast<int>(want < 1 ? 1 : want);
 }
 
+// A share of 256 keys is two tiles of 32 a wave (fp32, whose products take 16 times as long: 128; four rows
+// over 8 x 2048 keys 14 -> 11 us).
 // own: the sequences' own tokens take part.  The sequences of a set lie in one tile for the prefix where each has fewer rows
 // than a tile; then one workgroup of the prefix's walk a compute unit leaves room for one of the other's, and has half the
 // partials of two (64 x 32 heads of 128 over 32768 shared and 1024 own rows: 107 us, 122 with two; 64 rows over 8 x 16384
 // alone 27 and 32).
-inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, bool own) {
+inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, int dtype, bool own) {
+  const int64_t least = dtype == STA_F32 ? 128 : 256;
   PrefixPlan p{};
   const int64_t rows = static_cast<int64_t>(a.n) * a.group, units = static_cast<int64_t>(a.batch) * a.kv;
   const bool packed = a.p > 0 && (!own || (a.per_set > 1 && rows < sta::WIN_ROWS));
@@ -47,13 +50,13 @@ inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, bool own) {
     p.walks = own ? 2 : 1;
     p.walk[0].span = a.per_set;
     p.walk[0].prefix = 1;
-    deal_out(p.walk[0], p.share[0], static_cast<int64_t>(a.sets) * a.kv, rows * a.per_set, a.p, 256);
+    deal_out(p.walk[0], p.share[0], static_cast<int64_t>(a.sets) * a.kv, rows * a.per_set, a.p, 256, least);
     p.parts = p.walk[0].nsplit;
     if (own) {
       p.walk[1].span = 1;
       p.walk[1].own = 1;
       p.walk[1].first = p.parts;
-      deal_out(p.walk[1], p.share[1], units, rows, a.m, 512);
+      deal_out(p.walk[1], p.share[1], units, rows, a.m, 512, least);
       p.parts += p.walk[1].nsplit;
     }
     return p;
@@ -62,7 +65,7 @@ inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, bool own) {
   p.walk[0].span = 1;
   p.walk[0].prefix = a.p > 0;
   p.walk[0].own = 1;
-  deal_out(p.walk[0], p.share[0], units, rows, static_cast<int64_t>(a.p) + a.m, 512);
+  deal_out(p.walk[0], p.share[0], units, rows, static_cast<int64_t>(a.p) + a.m, 512, least);
   p.parts = p.walk[0].nsplit > 1 ? p.walk[0].nsplit : 0;
   return p;
 }

@@ -18,9 +18,9 @@ from typing import Optional, Sequence, Tuple, Union
 import torch
 
 import _native
-from shared_prefix_attention import _check_prefix, _check_rows, _refuse_gradients, _strides, shared_prefix_attention
+from shared_prefix_attention import _check_prefix, _check_rows, _refuse_gradients, _walkable, shared_prefix_attention
 from sink_window_attention import (MAX_DIM, MAX_ROWS, _attention_scale, _check_dtype, _check_gpu, _check_lengths, _on,
-                                   _rows, _widen)
+                                   _widen)
 
 Tensor = torch.Tensor
 
@@ -56,7 +56,7 @@ def received_attention(q: Tensor, k: Tensor, *, lengths: Optional[Tensor] = None
     weights = q.new_empty((b, hk, m), dtype=torch.float32)
     if weights.numel() == 0 or n == 0 or h == 0:
         return weights.zero_()
-    q, k = _rows(_widen(q.detach())), _rows(_widen(k.detach()))
+    (q, k), strides = _walkable(_widen(q.detach()), _widen(k.detach()))
     code, lib = _native.DTYPE_CODES[q.dtype], _native.lib()
     with _on(q.device):
         nbytes = lib.sta_received_attention_bytes(code, b, h, hk, n, m, q.shape[3], lse is not None)
@@ -64,7 +64,7 @@ def received_attention(q: Tensor, k: Tensor, *, lengths: Optional[Tensor] = None
             raise _native.NativeError("sta_received_attention_bytes refused the shape")
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         st = lib.sta_received_attention(
-            q.data_ptr(), k.data_ptr(), code, b, h, hk, n, m, q.shape[3], _strides(q, k), s, _native.ptr(lengths),
+            q.data_ptr(), k.data_ptr(), code, b, h, hk, n, m, q.shape[3], strides, s, _native.ptr(lengths),
             _native.ptr(counts), _native.ptr(lse), weights.data_ptr(), _native.ptr(ws), nbytes,
             _native.stream_handle(q.device))
     _native.check(st, "sta_received_attention")
@@ -167,7 +167,7 @@ class HeavyHitterStreamingAttention:
             x = x.detach().to(device=self.device, dtype=self.dtype)
         return x if x.is_contiguous() or x.stride(-1) == 1 or x.shape[-1] == 1 else x.detach().contiguous()
 
-    def _check_shared(self, prefix, prefix_lengths) -> Tuple[Tensor, Tensor, Optional[Tensor]]:
+    def _check_shared(self, prefix, prefix_lengths) -> tuple:
         pk, pv = prefix
         if self.dim * pk.element_size() < 16 or self.value_dim * pk.element_size() < 16:
             raise ValueError("a shared prefix needs keys and values of at least 16 bytes")
@@ -178,15 +178,14 @@ class HeavyHitterStreamingAttention:
         prefix_lengths = _check_lengths(prefix_lengths, pk.shape[0], "prefix_lengths")
         if prefix_lengths is not None and prefix_lengths.device != self.device:
             raise ValueError("prefix_lengths must be on the object's device")
-        return _rows(pk), _rows(pv), prefix_lengths
+        return *_walkable(pk, pv), prefix_lengths
 
     def _attend(self, q: Tensor, k: Optional[Tensor], v: Optional[Tensor], prefix, prefix_lengths) -> Tensor:
         sets = p = 0
         pk = pv = prefix_strides = None
         if prefix is not None:
-            pk, pv, prefix_lengths = self._check_shared(prefix, prefix_lengths)
+            (pk, pv), prefix_strides, prefix_lengths = self._check_shared(prefix, prefix_lengths)
             sets, p = pk.shape[0], pk.shape[2]
-            prefix_strides = _strides(pk, pv)
         elif prefix_lengths is not None:
             raise ValueError("prefix_lengths without a prefix")
         nbytes = self._bytes.get((sets, p))
@@ -263,13 +262,14 @@ class HeavyHitterStreamingAttention:
         if rows == 0:
             return
         weights = weights.detach().contiguous()
+        (k, v), strides = _walkable(k, v)
         lib = _native.lib()
         with _on(self.device):
             nbytes = lib.sta_heavy_start_bytes(self.streams, self.kv_heads, self.recent, self.kept)
             ws = k.new_empty(nbytes, dtype=torch.uint8)
             st = lib.sta_heavy_start(
                 k.data_ptr(), v.data_ptr(), weights.data_ptr(), self._code, self.streams, self.kv_heads, rows, self.dim,
-                self.value_dim, _strides(k, v), self.recent, self.kept, _native.ptr(counts), *self._state,
+                self.value_dim, strides, self.recent, self.kept, _native.ptr(counts), *self._state,
                 ws.data_ptr(), nbytes, _native.stream_handle(self.device))
         _native.check(st, "sta_heavy_start")
 

@@ -22,15 +22,21 @@ Tensor = torch.Tensor
 
 __all__ = ["shared_prefix_attention"]
 
-_STRIDES = {n: _native.ctypes.c_int64 * n for n in (6, 9, 15)}
+_STRIDES = {n: _native.ctypes.c_int64 * 3 * n for n in (2, 5)}
 
 
-def _strides(*tensors: Tensor):
-    """The element strides of batch, head and row of every tensor, for the C ABI."""
-    flat = ()
+def _walkable(*tensors: Tensor):
+    """The tensors, those whose rows the kernels cannot walk as dense copies, and the element strides of batch, head and
+    row of each, for the C ABI."""
+    rows, strides = [], []
     for x in tensors:
-        flat += x.stride()[:3]
-    return _STRIDES[len(flat)](*flat)
+        s = x.stride()
+        if (s[3] != 1 and x.shape[3] != 1) or s[2] * x.element_size() > 1 << 24:
+            x = _rows(x)
+            s = x.stride()
+        rows.append(x)
+        strides.append(s[:3])
+    return rows, _STRIDES[len(rows)](*strides)
 
 
 def _refuse_gradients(*tensors: Tensor) -> None:
@@ -103,14 +109,14 @@ def _attention(q: Tensor, k: Tensor, v: Tensor, pk: Tensor, pv: Tensor, lengths:
     if min(d, dv) * q.element_size() < 16:
         wide = _attention(*(_widen(x) for x in (q, k, v, pk, pv)), lengths, counts, prefix_lengths, scale, with_lse)
         return out.copy_(wide[0][..., :dv]), wide[1]
-    q, k, v, pk, pv = _rows(q), _rows(k), _rows(v), _rows(pk), _rows(pv)
+    (q, k, v, pk, pv), strides = _walkable(q, k, v, pk, pv)
     code = _native.DTYPE_CODES[q.dtype]
     nbytes = _workspace(code, b, h, hk, sets, n, m, p, d, dv)
     with _on(q.device):
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         st = _native.lib().sta_prefix_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), pk.data_ptr(), pv.data_ptr(), code, b, h, hk, sets, n, m, p, d,
-            dv, _strides(q, k, v, pk, pv), scale, _native.ptr(lengths), _native.ptr(counts),
+            dv, strides, scale, _native.ptr(lengths), _native.ptr(counts),
             _native.ptr(prefix_lengths), out.data_ptr(), _native.ptr(lse), _native.ptr(ws), nbytes,
             _native.stream_handle(q.device))
     _native.check(st, "sta_prefix_attention")
