@@ -9,19 +9,22 @@ namespace {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <int IN>
-void join(const sta::PrefixArgs& a, dim3 grid, hipStream_t s) {
-  hipLaunchKernelGGL((sta::prefix_join_kernel<IN>), grid, dim3(128), 0, s, a);
+void join(const sta::PrefixArgs& a, bool few, dim3 grid, hipStream_t s) {
+  if (few) hipLaunchKernelGGL((sta::prefix_join_few_kernel<IN>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((sta::prefix_join_kernel<IN>), grid, dim3(128), 0, s, a);
 }
 
-// The partials of every row; a row is a workgroup, in rows of 2^20 of them.
+// The partials of every row, in rows of 2^20 workgroups.
 int join_rows(const sta::PrefixArgs& a, int dtype, hipStream_t s) {
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.n, x = rows < 1 << 20 ? rows : 1 << 20;
-  const int64_t y = ceil_div(rows, x);
+  const bool few = a.parts <= sta::PREFIX_FEW_PARTS;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.heads * a.n;
+  const int64_t groups = few ? ceil_div(rows, a.out ? 256 / (a.pitch / 4) : 256) : rows;
+  const int64_t x = groups < 1 << 20 ? groups : 1 << 20, y = ceil_div(groups, x);
   if (y > 65535) return STA_ERR_SHAPE;
   const dim3 g(static_cast<unsigned>(x), static_cast<unsigned>(y));
-  if (dtype == STA_F32) join<sta::F32>(a, g, s);
-  else if (dtype == STA_BF16) join<sta::BF16>(a, g, s);
-  else join<sta::F16>(a, g, s);
+  if (dtype == STA_F32) join<sta::F32>(a, few, g, s);
+  else if (dtype == STA_BF16) join<sta::BF16>(a, few, g, s);
+  else join<sta::F16>(a, few, g, s);
   return check_launch();
 }
 

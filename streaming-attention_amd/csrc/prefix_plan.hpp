@@ -37,20 +37,32 @@ inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows
 
 // A share of 256 keys is two tiles of 32 a wave (fp32, whose products take 16 times as long: 128; four rows
 // over 8 x 2048 keys 14 -> 11 us).
-// own: the sequences' own tokens take part.  The sequences of a set lie in one tile for the prefix where each has fewer rows
-// than a tile; then one workgroup of the prefix's walk a compute unit leaves room for one of the other's, and has half the
-// partials of two (64 x 32 heads of 128 over 32768 shared and 1024 own rows: 107 us, 122 with two; 64 rows over 8 x 16384
-// alone 27 and 32).
+// own: the sequences' own tokens take part.  The sequences of a set lie in one tile for the prefix (two walks, whose partials
+// are joined) where each has few rows and there are keys enough:
+// * up to 512 keys a workgroup goes over both for itself, without partials (4 x 8 heads of 64 over 256 and 64 keys 10.3 -> 9.1
+//   us, 64 x 4 of 64 rows 19.7 -> 11.2; over 576 keys 8 x 8 x 4 rows take 10.6 and 10.1, 32 x 32 of one row 18.5 and 20.4);
+//   fp32 up to 128 (64 x 8 x 4 rows of 128 over 128 keys 46 -> 41 us, of 64 23 -> 16, 2 x 2 of 128 19 -> 21; over 256 keys 49
+//   and 56);
+// * above 64 rows its tile of 128 is full enough (64 x 4 of 96 rows of 64 over 16384: 272 -> 176 us, 16 x 8 142 -> 97, 4 x
+//   8 38.6 -> 37.1); not in fp32 (4 x 8 of 96 rows of 128 over 4096: 95 and 109 us).
+// One workgroup of the prefix's walk a compute unit leaves room for one of the other's, and has half the partials of two (64
+// x 32 heads of 128 over 32768 shared and 1024 own rows: 107 us, 122 with two; 64 rows over 8 x 16384 alone 27 and 32); with
+// many tiles and more than 1024 keys a share, two (64 x 4 of 48 rows of 64 over 16384: 134 -> 82 us, 32 rows 73 -> 57, 16
+// x 8 of 32 rows 43 -> 38; of 1024 keys 28 and 27, 30 and 30, of 512 23 and 26).
 inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, int dtype, bool own) {
-  const int64_t least = dtype == STA_F32 ? 128 : 256;
+  const int64_t least = dtype == STA_F32 ? 128 : 256, keys = static_cast<int64_t>(a.p) + a.m;
+  const bool one = keys <= (dtype == STA_F32 ? 128 : 512);
   PrefixPlan p{};
   const int64_t rows = static_cast<int64_t>(a.n) * a.group, units = static_cast<int64_t>(a.batch) * a.kv;
-  const bool packed = a.p > 0 && (!own || (a.per_set > 1 && rows < sta::WIN_ROWS));
+  const bool packed =
+      a.p > 0 && (!own || (!one && a.per_set > 1 && rows < (dtype == STA_F32 ? sta::WIN_ROWS : sta::WIN_ROWS / 2 + 1)));
   if (packed) {
+    const int64_t sets = static_cast<int64_t>(a.sets) * a.kv, together = rows * a.per_set;
+    const int64_t tiles = sets * ceil_div(together, sta::WIN_ROWS);
     p.walks = own ? 2 : 1;
     p.walk[0].span = a.per_set;
     p.walk[0].prefix = 1;
-    deal_out(p.walk[0], p.share[0], static_cast<int64_t>(a.sets) * a.kv, rows * a.per_set, a.p, 256, least);
+    deal_out(p.walk[0], p.share[0], sets, together, a.p, tiles >= 32 && a.p * tiles > 256 * 1024 ? 512 : 256, least);
     p.parts = p.walk[0].nsplit;
     if (own) {
       p.walk[1].span = 1;
@@ -65,7 +77,7 @@ inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, int dtype, bool own) {
   p.walk[0].span = 1;
   p.walk[0].prefix = a.p > 0;
   p.walk[0].own = 1;
-  deal_out(p.walk[0], p.share[0], units, rows, static_cast<int64_t>(a.p) + a.m, 512, least);
+  deal_out(p.walk[0], p.share[0], units, rows, keys, one ? 1 : 512, least);
   p.parts = p.walk[0].nsplit > 1 ? p.walk[0].nsplit : 0;
   return p;
 }
