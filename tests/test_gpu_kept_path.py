@@ -62,7 +62,11 @@ def spread(x):
 SIZES = [  # b h hk n m sets p d dv: one row, few, many; widths with and without tiles straight to LDS
     (3, 4, 2, 1, 40, 1, 300, 64, 64), (16, 16, 4, 40, 70, 2, 130, 128, 128), (9, 12, 12, 150, 150, 3, 100, 64, 64),
     (40, 8, 2, 1, 90, 1, 700, 128, 128), (2, 4, 2, 20, 33, 1, 65, 40, 24), (64, 32, 32, 20, 20, 1, 70, 64, 64),
-    (24, 16, 16, 130, 150, 2, 90, 128, 128), (20, 32, 16, 140, 140, 1, 65, 64, 64)]  # the last: rows that one workgroup finishes
+    (24, 16, 16, 130, 150, 2, 90, 128, 128), (20, 32, 16, 140, 140, 1, 65, 64, 64),  # the last: rows that one workgroup finishes
+    # prefixes and own tokens in walks of their own: tiles of 32 and of 128, many partials and few
+    (3, 4, 2, 1, 40, 1, 5000, 64, 64), (16, 8, 2, 10, 40, 1, 600, 128, 128), (6, 4, 4, 33, 50, 2, 800, 64, 64),
+    (12, 2, 2, 20, 33, 1, 700, 40, 24)]
+WALKS = SIZES[:4] + SIZES[8:]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -136,7 +140,7 @@ def test_what_is_hidden_does_not_count(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("size", SIZES[:4])
+@pytest.mark.parametrize("size", WALKS)
 def test_rows_of_one_key_and_lowest_values(size, dtype):
     """Keys that hide by the type's lowest value, rows whose logits are all -inf (NaN, as a softmax of them), and keys
     of -inf beside others (weights of 0)."""

@@ -63,6 +63,29 @@ def test_outputs_and_statistics(b, h, hk, n, m, sets, p, d, dv, lengths, counts,
     check(attend(x, **kw), ref.prefix_attention(*x, **kw))
 
 
+WALKS = [  # keys enough for the prefix and the own tokens to be walked apart
+    (2, 2, 1, 1, 5, 1, 600, 16, 24, [5, 0], None, None),
+    (4, 1, 1, 2, 5, 2, 700, 5, 3, [5, 1, 0, 2], None, [700, 0]),
+    (6, 6, 2, 9, 40, 3, 600, 93, 77, [40, 17, 3, 40, 0, 1], [9, 5, 9, 1, 0, 1], [600, 1, 333]),
+    (6, 4, 4, 33, 33, 2, 900, 128, 128, [33, 1, 0, 32, 5, 33], [33, 1, 0, 32, 5, 33], None),
+    (8, 64, 32, 60, 70, 1, 500, 32, 32, [70, 66, 1, 0, 33, 64, 65, 70], [60, 60, 1, 0, 33, 60, 60, 2], None),
+    (6, 2, 2, 64, 64, 1, 520, 64, 64, None, None, [519]),
+    (2, 3, 1, 30, 60, 1, 600, 96, 80, [60, 31], [30, 29], None),
+    (3, 1, 1, 1, 1, 1, 9000, 32, 32, None, None, None),
+    (1, 2, 2, 1, 9000, 1, 0, 32, 64, [8999], None, None),
+    (2, 1, 1, 1, 4500, 1, 700, 64, 32, [4500, 1], None, [640]),
+    (16, 8, 8, 32, 40, 1, 8200, 64, 32, None, None, None),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,hk,n,m,sets,p,d,dv,lengths,counts,plens", WALKS)
+def test_walks_that_are_joined(b, h, hk, n, m, sets, p, d, dv, lengths, counts, plens, dtype):
+    x = make(b, h, hk, n, m, sets, p, d, dv, dtype, seed=2)
+    kw = dict(lengths=lengths, counts=counts, prefix_lengths=plens)
+    check(attend(x, **kw), ref.prefix_attention(*x, **kw))
+
+
 MANY = [  # enough rows for tiles of 128, and for workgroups that finish their rows
     (16, 32, 8, 5, 64, 1, 300, 64, 64, None, None, None),
     (24, 16, 16, 130, 130, 2, 90, 64, 32, None, None, [90, 61]),
