@@ -31,8 +31,8 @@ int launch_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int values, hip
   auto least = [&](int bytes) { return bytes > by_rows ? bytes : by_rows; };
   const int wide = least(sta::win_lds_bytes<P, IN, false>());
   const int ga = static_cast<int>(grid[0]), gb = static_cast<int>(grid[1]);
-  if constexpr (IN != sta::F32 && (P == 64 || P == 128)) {
-    if (p.stream && !p.share[0] && a.d == P && (!values || a.dv == P)) {
+  if constexpr (IN != sta::F32) {
+    if (p.stream && !p.share[0] && a.d % 8 == 0 && (!values || a.dv % 8 == 0)) {
       const int lds = values ? least(sta::prefix_stream_bytes<P, true>()) : sta::prefix_stream_bytes<P, false>();
       if (p.walks == 2) {
         return p.share[1] ? launch(sta::prefix_walks_kernel<P, IN, false, true, true>, lds > shared ? lds : shared, p.walk[0],
@@ -74,8 +74,8 @@ int launch_received(const sta::ReceivedArgs& w, hipStream_t s) {
     hipLaunchKernelGGL((sta::received_few_kernel<P, IN>), g, dim3(256), lds, s, w);
     return check_launch();
   }
-  if constexpr (IN != sta::F32 && (P == 64 || P == 128)) {
-    if (w.stream && w.a.d == P) {
+  if constexpr (IN != sta::F32) {
+    if (w.stream && w.a.d % 8 == 0) {
       hipLaunchKernelGGL((sta::received_kernel<P, IN, true>), g, dim3(256), 0, s, w);
       return check_launch();
     }

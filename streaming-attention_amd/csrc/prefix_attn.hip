@@ -120,8 +120,9 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
     const int last = (r0 + win_rows<SHARE>() - 1) / a.group;
     own_end = r0 / a.group < count ? base + (last < count ? last + 1 : count) : 0;
   }
-  const bool any = w.own ? own_end > 0 : r0 < w.span * per;
-  const int tiles_p = any ? (rows_p + BK - 1) / BK : 0, all_tiles = tiles_p + (own_end + BK - 1) / BK;
+  // a wave without a live row (a padded batch has many) leaves its products out; four that share their rows, their loads too
+  const bool awake = __any(mine.live), any = (!SHARE || awake) && (w.own ? own_end > 0 : r0 < w.span * per);
+  const int tiles_p = any ? (rows_p + BK - 1) / BK : 0, all_tiles = any ? tiles_p + (own_end + BK - 1) / BK : 0;
   // Every nsplit-th tile: workgroups that walk in step are at neighbouring rows, and not at round distances, which would
   // ask the same memory channels at a time.
   const int own_first = (split + w.nsplit - tiles_p % w.nsplit) % w.nsplit;  // of the own tokens' tiles
@@ -163,7 +164,7 @@ __device__ __forceinline__ int prefix_pass(const PrefixArgs& a, const PrefixWalk
         if constexpr (VALUES) vst.put(vs, end - key0);
         win_sync<SHARE>();
         if (AHEAD && it + step < hi) load(it + step);
-        if (key0 > lim_hi) continue;
+        if (key0 > lim_hi || !awake) continue;
         const bool all = key0 + BK - 1 <= lim_lo;
         floatx16 x[NSUB];
 #pragma unroll
@@ -446,11 +447,12 @@ struct PrefixRows {
   }
 };
 
-// The first pass for 16-bit heads exactly P wide on 16 bytes, wide tiles: that of prefix_pass with tiles that go from memory to LDS
+// The first pass for 16-bit heads of whole 16 bytes, wide tiles: that of prefix_pass with tiles that go from memory to LDS
 // directly, keys and values of even and of odd tiles in buffers of their own, so that one barrier a tile is enough and a
 // tile's value products run into the next one's logits.  The buffers are restrict arguments: the compiler then sees that
 // reads of one need not wait for loads to another.  32 x 512 rows of 8 sequences behind 16384, 128 wide, 1.29 -> 1.12 ms
 // (1000 TFLOP/s; a large matrix product 1200), 64 wide 0.38 -> 0.35 ms; 32 heads' statistics of 16384 rows 1.25 -> 1.06 ms.
+// Widths between (their tiles padded to P): 8 x 32 heads of 512 rows behind 4096, 80 and 72 wide, 279 -> 249 us, 112 wide 362 -> 310.
 typedef const __attribute__((address_space(1))) void* stream_global;
 typedef __attribute__((address_space(3))) void* stream_lds;
 
@@ -461,12 +463,13 @@ struct StreamTile {
   int pitch, at[NJ];
 
   __device__ __forceinline__ static int unit(int j) { return static_cast<int>(NJ * (threadIdx.x >> 6) + j) * 64 + (threadIdx.x & 63); }
-  __device__ __forceinline__ void init(int64_t row_elements) {
+  // units behind the rows' width are read as the last one: they meet zeros, or give columns that are not stored
+  __device__ __forceinline__ void init(int64_t row_elements, int width) {
     pitch = static_cast<int>(row_elements) * 2;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int u = unit(j), r = u / CH;
-      at[j] = r * pitch + ((u % CH) ^ win_swizzle<CH>(r)) * 16;
+      at[j] = r * pitch + min((u % CH) ^ win_swizzle<CH>(r), width / 8 - 1) * 16;
     }
   }
   // rows behind the last are read as the last one: their logits are hidden, their weights 0
@@ -523,7 +526,7 @@ __device__ __forceinline__ int prefix_stream_pass(const PrefixArgs& a, const Pre
     const int last = (r0 + WIN_ROWS - 1) / a.group;
     own_end = r0 / a.group < count ? base + (last < count ? last + 1 : count) : 0;
   }
-  const bool any = w.own ? own_end > 0 : r0 < w.span * per;
+  const bool awake = __any(live), any = w.own ? own_end > 0 : r0 < w.span * per;  // awake: see prefix_pass
   const int tiles_p = any ? (rows_p + BK - 1) / BK : 0, all_tiles = tiles_p + (own_end + BK - 1) / BK;
   const int own_first = (split + w.nsplit - tiles_p % w.nsplit) % w.nsplit;
 
@@ -535,7 +538,7 @@ __device__ __forceinline__ int prefix_stream_pass(const PrefixArgs& a, const Pre
     const char* qrow = rows_at<2>(a.q, b, h, i);
 #pragma unroll
     for (int s = 0; s < P / 16; ++s) {
-      qf[s] = win_load_row<IN>(qrow, s, hh, P, flip);
+      qf[s] = win_load_row<IN>(qrow, s, hh, a.d, flip);
       win_keep<IN>(qf[s], live);
     }
 #pragma unroll 1
@@ -548,8 +551,8 @@ __device__ __forceinline__ int prefix_stream_pass(const PrefixArgs& a, const Pre
       const int lim_lo = seg ? base + w0 / a.group : rows_p - 1;
       const int lim_hi = seg ? base + min((w0 + 31) / a.group, count - 1) : rows_p - 1;
       StreamTile<P> kt, vt;
-      kt.init(kr.sn);
-      if constexpr (VALUES) vt.init(vr.sn);
+      kt.init(kr.sn, a.d);
+      if constexpr (VALUES) vt.init(vr.sn, a.dv);
       const char *const kp = rows_at<2>(kr, rb, hk, 0), *const vp = VALUES ? rows_at<2>(vr, rb, hk, 0) : nullptr;
       // nothing behind the last tile
       auto keys = [&](int it, uint4* to) {
@@ -562,7 +565,7 @@ __device__ __forceinline__ int prefix_stream_pass(const PrefixArgs& a, const Pre
       };
       // a tile, from keys and values that are there when it begins and when its weights are taken
       auto turn = [&](int it, uint4* ks, const uint4* vs, uint4* next) {
-        const int key0 = it * BK, active = key0 <= lim_hi;
+        const int key0 = it * BK, active = key0 <= lim_hi && awake;
         floatx16 x[NSUB];
         if (active) {
           sums.logits(x, ks, qf, lane);
@@ -613,8 +616,8 @@ __device__ __forceinline__ int prefix_stream_pass(const PrefixArgs& a, const Pre
         const int unit = 64 * u + lane, r = unit / UNITS, col = 4 * (unit % UNITS);
         const int lo = __shfl(static_cast<int>(part), r), hi = __shfl(static_cast<int>(part >> 32), r);
         const int64_t to = static_cast<int64_t>(hi) << 32 | static_cast<uint32_t>(lo);
-        if (__shfl(static_cast<int>(store), r))
-          *reinterpret_cast<floatx4*>(a.part + to * P + col) = *reinterpret_cast<floatx4*>(&red[(wave * 32 + r) * (P + 4) + col]);
+        if (__shfl(static_cast<int>(store), r) && col < a.dv)
+          *reinterpret_cast<floatx4*>(a.part + to * a.pitch + col) = *reinterpret_cast<floatx4*>(&red[(wave * 32 + r) * (P + 4) + col]);
       }
     }
     if (store && hh == 0)
@@ -625,10 +628,13 @@ __device__ __forceinline__ int prefix_stream_pass(const PrefixArgs& a, const Pre
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          win_store4<IN>(a.out, at * P, 32 * mt + 8 * r + 4 * hh, P, live ? sums.acc[mt][4 * r] * inv : 0.f,
-                         live ? sums.acc[mt][4 * r + 1] * inv : 0.f, live ? sums.acc[mt][4 * r + 2] * inv : 0.f,
-                         live ? sums.acc[mt][4 * r + 3] * inv : 0.f);
+        for (int r = 0; r < 4; ++r) {
+          const int col = 32 * mt + 8 * r + 4 * hh;
+          if (col < a.dv)
+            win_store4<IN>(a.out, at * a.dv, col, a.dv, live ? sums.acc[mt][4 * r] * inv : 0.f,
+                           live ? sums.acc[mt][4 * r + 1] * inv : 0.f, live ? sums.acc[mt][4 * r + 2] * inv : 0.f,
+                           live ? sums.acc[mt][4 * r + 3] * inv : 0.f);
+        }
     }
     if (a.lse && hh == 0) a.lse[at] = live ? prefix_lse<IN>(sums.m, sums.l, a.c) : 0.f;
   }
@@ -838,7 +844,7 @@ __device__ __forceinline__ void received_add(float& total, float& lost, const fl
 // that see one of them, head by head of the group; with X = Q K^T a lane has 16 rows of one key, whose weights it sums: no
 // exchange between lanes until the end.  Sums of 16 go into a compensated total (16384 x 4 rows).  32 heads of 16384 rows,
 // 128 wide: 1.14 ms, 965 TFLOP/s (a large matrix product 1200); 64 wide 0.75 ms, bound by the exponentials.
-// STREAM: 16-bit rows exactly P wide on 16 bytes go from memory to LDS directly, a tile ahead in two buffers, with one
+// STREAM: 16-bit rows of whole 16 bytes go from memory to LDS directly, a tile ahead in two buffers, with one
 // barrier a tile, and leave room for a third wave a SIMD (1.32 -> 1.22 -> 1.14 ms, 965 TFLOP/s).
 template <int P, int IN, bool STREAM>
 __device__ __forceinline__ void received_walk(const ReceivedArgs& w, int id, uint4* __restrict__ qs0, uint4* __restrict__ qs1,
@@ -912,7 +918,7 @@ __device__ __forceinline__ void received_walk(const ReceivedArgs& w, int id, uin
     };
     if constexpr (STREAM) {
       StreamTile<P> qt;
-      qt.init(a.q.sn);
+      qt.init(a.q.sn, a.d);
       At x = advance();
       qt.load(rows_of(x), count - x.i, qs0);
       if (threadIdx.x < BQ) stat0[threadIdx.x] = stat_of(x);
