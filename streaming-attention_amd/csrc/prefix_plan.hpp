@@ -46,9 +46,10 @@ inline void deal_out(sta::PrefixWalk& w, int& share, int64_t units, int64_t rows
 // * above 64 rows its tile of 128 is full enough (64 x 4 of 96 rows of 64 over 16384: 272 -> 176 us, 16 x 8 142 -> 97, 4 x
 //   8 38.6 -> 37.1); not in fp32 (4 x 8 of 96 rows of 128 over 4096: 95 and 109 us).
 // One workgroup of the prefix's walk a compute unit leaves room for one of the other's, and has half the partials of two (64
-// x 32 heads of 128 over 32768 shared and 1024 own rows: 107 us, 122 with two; 64 rows over 8 x 16384 alone 27 and 32); with
+// x 32 heads of 128 over 16384 shared and 1024 own rows: 79 us, 92 with two; 64 rows over 8 x 16384 alone 27 and 32); with
 // many tiles and more than 1024 keys a share, two (64 x 4 of 48 rows of 64 over 16384: 134 -> 82 us, 32 rows 73 -> 57, 16
-// x 8 of 32 rows 43 -> 38; of 1024 keys 28 and 27, 30 and 30, of 512 23 and 26).
+// x 8 of 32 rows 43 -> 38; of 1024 keys 28 and 27, 30 and 30, of 512 23 and 26).  Many are 32, or 16 up to 64 columns (64 x
+// 32 heads over 32768 shared and 1024 own rows, 64 wide 57 -> 50 us, 128 wide 108 and 110).
 inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, int dtype, bool own) {
   const int64_t least = dtype == STA_F32 ? 128 : 256, keys = static_cast<int64_t>(a.p) + a.m;
   const bool one = keys <= (dtype == STA_F32 ? 128 : 512);
@@ -62,7 +63,8 @@ inline PrefixPlan plan_prefix(const sta::PrefixArgs& a, int dtype, bool own) {
     p.walks = own ? 2 : 1;
     p.walk[0].span = a.per_set;
     p.walk[0].prefix = 1;
-    deal_out(p.walk[0], p.share[0], sets, together, a.p, tiles >= 32 && a.p * tiles > 256 * 1024 ? 512 : 256, least);
+    const bool two = a.p * tiles > 256 * 1024 && tiles >= (a.d <= 64 && a.dv <= 64 ? 16 : 32);
+    deal_out(p.walk[0], p.share[0], sets, together, a.p, two ? 512 : 256, least);
     p.parts = p.walk[0].nsplit;
     if (own) {
       p.walk[1].span = 1;
