@@ -107,7 +107,7 @@ def lib():
 
 def test_workspaces_refuse_what_the_calls_refuse():
     f = lib().sta_prefix_attention_bytes
-    good = (1, 4, 8, 2, 2, 1, 64, 128, 64, 64)  # type batch heads kv sets n m p d dv
+    good = (1, 4, 8, 2, 2, 1, 64, 1280, 64, 64)  # type batch heads kv sets n m p d dv
     assert f(*good) > 0
     for i, x in ((0, 3), (1, 0), (1, 3), (2, 7), (3, 0), (4, 0), (5, 0), (6, 0), (7, -1), (8, 129), (8, 7), (9, 0), (9, 129),
                  (7, (1 << 30) + 1), (5, 1 << 31)):
@@ -138,7 +138,7 @@ def test_null_pointers_are_refused():
     strides = (_native.ctypes.c_int64 * 15)()
     some = 4096  # never read: the call ends before
     arg = _native.STA_ERR_ARG
-    prefix = [some, some, some, some, some, 1, 4, 8, 2, 2, 1, 64, 128, 64, 64, strides, 0.125, None, None, None, some, None, None,
+    prefix = [some, some, some, some, some, 1, 4, 8, 2, 2, 1, 64, 1280, 64, 64, strides, 0.125, None, None, None, some, None, None,
               0, None]
     for i in (0, 1, 2, 3, 4, 15, 20):
         bad = list(prefix)
