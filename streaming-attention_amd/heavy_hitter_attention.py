@@ -41,7 +41,7 @@ def received_attention(q: Tensor, k: Tensor, *, lengths: Optional[Tensor] = None
     gives them with_lse (a prefix's tokens then have their share of every row), or None: computed here, over the own
     tokens alone.  Zero behind the lengths; NaN for tokens that a row with an infinite or NaN statistic sees.  May be
     captured into a graph; inputs that ask for derivatives are refused (RuntimeError)."""
-    _refuse_gradients(q, k)
+    _refuse_gradients(*((q, k) if lse is None else (q, k, lse)))
     _check_rows(q, k, "q and k")
     b, h, n, d = q.shape
     hk, m = k.shape[1], k.shape[2]

@@ -441,3 +441,35 @@ def test_large_caches():
     mean = torch.cat([v[:, 0], v[:, 0, :3]], 1).double().mean(1)
     assert ref.over(got[:, 0], (mean.cpu(), 2.0 ** -8 * (mean.abs() + v.double().abs().mean()).cpu())) <= 1.0
     assert c.positions[2, 0, :512].ge(0).sum().item() == 511 and c.positions[2, 0].ge(0).sum().item() == 703
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kw", [dict(), dict(kept=2000, recent=9, n=2100), dict(heads=40, kv=1, streams=2)])
+def test_prefixes_of_nothing(kw, dtype):
+    """A prefix without rows, or with none that count, is none: outputs within a rounding, and the same tokens held."""
+    a, b, c = (cache_of(dtype=dtype, **kw) for _ in range(3))
+    none = tuple(t.to(DEV) for t in make(3, dtype, (a.kv_heads, 0, 32), (a.kv_heads, 0, 24)))
+    some = tuple(t.to(DEV) for t in make(4, dtype, (2, a.kv_heads, 77, 32), (2, a.kv_heads, 77, 24)))
+    some[1][:] = math.nan
+    eps = 2 * torch.finfo(dtype).eps + 64 * torch.finfo(torch.float32).eps  # two roundings of an output, fp32 sums
+    for i in range(3):
+        q, k, v = token(a, 20 + i)
+        want = a.step(q, k, v)
+        assert torch.equal(b.step(q, k, v, prefix=none), want)
+        got = c.step(q, k, v, prefix=some, prefix_lengths=ints([0, -3]))
+        assert ((got.double() - want.double()).abs() <= eps * v.abs().max().clamp(min=4.0)).all()
+    assert same(a, b) and torch.equal(a.positions, c.positions)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_of_empty_caches_behind_a_prefix(dtype):
+    """Before a token has come a query sees the prefix alone; without one its output is zero."""
+    c = hha.HeavyHitterStreamingAttention(32, 24, streams=4, heads=8, kv_heads=2, kept=12, recent=5, dtype=dtype)
+    q = token(c, 1)[0]
+    pk, pv = make(2, dtype, (2, 2, 600, 32), (2, 2, 600, 24))
+    got = c.query(q, prefix=(pk.to(DEV), pv.to(DEV)), prefix_lengths=ints([600, 3]))
+    # the prefix's rows as own tokens of each stream, whose newest row is the query's
+    k, v = (t.repeat_interleave(2, 0) for t in (pk, pv))
+    want = ref.prefix_attention(q.cpu()[:, :, None], k, v, pk[:1, :, :0], pv[:1, :, :0], lengths=[600, 600, 3, 3])
+    check({"out": got[:, :, None]}, {"out": want["out"]})
+    assert c.query(q).eq(0).all() and c.weights.eq(0).all() and c.lengths.eq(0).all()

@@ -61,6 +61,8 @@ def test_mixed_types_and_derivatives():
             spa.shared_prefix_attention(*y)
     with pytest.raises(RuntimeError, match="no backward pass"):
         hha.received_attention(x[0].requires_grad_(), x[1])
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        hha.received_attention(x[0].detach(), x[1], lse=torch.zeros(B, H, N, requires_grad=True))
     with torch.autograd.forward_ad.dual_level():
         dual = torch.autograd.forward_ad.make_dual(x[1], torch.ones_like(x[1]))
         with pytest.raises(RuntimeError, match="forward-mode"):
