@@ -19,7 +19,7 @@ import torch
 
 import _native
 from shared_prefix_attention import _check_prefix, _check_rows, _refuse_gradients, _walkable, shared_prefix_attention
-from sink_window_attention import (MAX_DIM, MAX_ROWS, _attention_scale, _check_dtype, _check_gpu, _check_lengths, _on,
+from sink_window_attention import (MAX_DIM, MAX_ROWS, _attention_scale, _check_dtype, _check_gpu, _check_lengths, _like, _on,
                                    _widen)
 
 Tensor = torch.Tensor
@@ -138,10 +138,14 @@ class HeavyHitterStreamingAttention:
                          "positions": self._positions, "lowest": self._lowest}
         self._state = tuple(x.data_ptr() for x in self._tensors.values())
         self._views = self._weights[..., :self._slots], self._positions[..., :self._slots]
+        shape = (streams, kv_heads, self._slots)  # of the items' rows, without memory of their own
+        self._items = tuple(room(1, dtype=t).expand(size) for size, t in (
+            ((*shape, dim), dtype), ((*shape, value_dim), dtype), (shape, torch.int64), (shape, torch.float32)))
         self._shapes = {"query": (streams, heads, dim), "key": (streams, kv_heads, dim),
                         "value": (streams, kv_heads, value_dim)}
         self._dense = _PAIRS[6](heads * dim, dim, kv_heads * dim, dim, kv_heads * value_dim, value_dim)
         self._bytes: dict = {}
+        self._start_bytes = _native.lib().sta_heavy_start_bytes(streams, kv_heads, recent, kept)
 
     @property
     def lengths(self) -> Tensor:
@@ -171,21 +175,20 @@ class HeavyHitterStreamingAttention:
         pk, pv = prefix
         if self.dim * pk.element_size() < 16 or self.value_dim * pk.element_size() < 16:
             raise ValueError("a shared prefix needs keys and values of at least 16 bytes")
-        pk, pv = _check_prefix(pk.detach(), pv.detach(), self.streams, self.kv_heads, self.dim, self.value_dim)
+        sets, p = _check_prefix(pk, pv, self.streams, self.kv_heads, self.dim, self.value_dim)
         for x in (pk, pv):
             if x.dtype != self.dtype or x.device != self.device:
                 raise ValueError("the prefix must have the object's dtype and be on its device")
-        prefix_lengths = _check_lengths(prefix_lengths, pk.shape[0], "prefix_lengths")
+        prefix_lengths = _check_lengths(prefix_lengths, sets, "prefix_lengths")
         if prefix_lengths is not None and prefix_lengths.device != self.device:
             raise ValueError("prefix_lengths must be on the object's device")
-        return *_walkable(pk, pv), prefix_lengths
+        return *_walkable(pk.detach(), pv.detach()), sets, p, prefix_lengths
 
     def _attend(self, q: Tensor, k: Optional[Tensor], v: Optional[Tensor], prefix, prefix_lengths) -> Tensor:
         sets = p = 0
         pk = pv = prefix_strides = None
         if prefix is not None:
-            (pk, pv), prefix_strides, prefix_lengths = self._check_shared(prefix, prefix_lengths)
-            sets, p = pk.shape[0], pk.shape[2]
+            (pk, pv), prefix_strides, sets, p, prefix_lengths = self._check_shared(prefix, prefix_lengths)
         elif prefix_lengths is not None:
             raise ValueError("prefix_lengths without a prefix")
         nbytes = self._bytes.get((sets, p))
@@ -196,7 +199,7 @@ class HeavyHitterStreamingAttention:
             if nbytes < 0:
                 raise _native.NativeError("sta_heavy_attention_bytes refused the shape")
             self._bytes = {(sets, p): nbytes}
-        out = q.new_empty((self.streams, self.heads, self.value_dim))
+        out = _like(q) if self.dim == self.value_dim else q.new_empty((self.streams, self.heads, self.value_dim))
         ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         if q.is_contiguous() and (k is None or (k.is_contiguous() and v.is_contiguous())):
             strides = self._dense
@@ -265,12 +268,11 @@ class HeavyHitterStreamingAttention:
         (k, v), strides = _walkable(k, v)
         lib = _native.lib()
         with _on(self.device):
-            nbytes = lib.sta_heavy_start_bytes(self.streams, self.kv_heads, self.recent, self.kept)
-            ws = k.new_empty(nbytes, dtype=torch.uint8)
+            ws = k.new_empty(self._start_bytes, dtype=torch.uint8)
             st = lib.sta_heavy_start(
                 k.data_ptr(), v.data_ptr(), weights.data_ptr(), self._code, self.streams, self.kv_heads, rows, self.dim,
                 self.value_dim, strides, self.recent, self.kept, _native.ptr(counts), *self._state,
-                ws.data_ptr(), nbytes, _native.stream_handle(self.device))
+                ws.data_ptr(), self._start_bytes, _native.stream_handle(self.device))
         _native.check(st, "sta_heavy_start")
 
     @torch.no_grad()
@@ -310,11 +312,7 @@ class HeavyHitterStreamingAttention:
         """(keys [S,Hkv,recent + 1 + kept,dim], values [S,Hkv,recent + 1 + kept,value_dim], positions int64, weights
         float32 [S,Hkv,recent + 1 + kept]) as the cache holds them, in the order of its slots; zero, and position -1,
         where no token is."""
-        shape = (self.streams, self.kv_heads, self._slots)
-        weights = self._weights.new_empty(shape)
-        positions = self._positions.new_empty(shape)
-        keys = self._weights.new_empty((*shape, self.dim), dtype=self.dtype)
-        values = self._weights.new_empty((*shape, self.value_dim), dtype=self.dtype)
+        keys, values, positions, weights = (_like(x) for x in self._items)
         with _on(self.device):
             st = _native.lib().sta_heavy_items(
                 self._code, self.streams, self.kv_heads, self.dim, self.value_dim, self.recent, self.kept,

@@ -10,32 +10,34 @@ only: results take no part in derivatives, and inputs that ask for one are refus
 
 from __future__ import annotations
 
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
 
 import _native
-from sink_window_attention import (MAX_DIM, MAX_ROWS, _attention_scale, _check_dtype, _check_gpu, _check_lengths, _on,
-                                   _refuse_tangents, _rows, _widen)
+from sink_window_attention import (MAX_DIM, MAX_ROWS, _attention_scale, _check_dtype, _check_gpu, _check_lengths, _like, _on,
+                                   _refuse_tangents, _widen)
 
 Tensor = torch.Tensor
 
 __all__ = ["shared_prefix_attention"]
 
-_STRIDES = {n: _native.ctypes.c_int64 * 3 * n for n in (2, 5)}
+_STRIDES = {n: struct.Struct(f"{3 * n}q").pack for n in (2, 5)}  # a third of a ctypes array's host time
 
 
 def _walkable(*tensors: Tensor):
-    """The tensors, those whose rows the kernels cannot walk as dense copies, and the element strides of batch, head and
-    row of each, for the C ABI."""
-    rows, strides = [], []
+    """The tensors, those whose rows the kernels cannot walk as dense copies, and the element strides of batch (0 for a
+    prefix [Hkv,P,D]), head and row of each, for the C ABI."""
+    rows, strides = [], ()
     for x in tensors:
         s = x.stride()
-        if (s[3] != 1 and x.shape[3] != 1) or s[2] * x.element_size() > 1 << 24:
-            x = _rows(x)
+        # rows of contiguous elements, at most 2^24 bytes apart
+        if (s[-1] != 1 and x.shape[-1] != 1) or (s[-2] > 1 << 22 and s[-2] * x.element_size() > 1 << 24):
+            x = x.clone(memory_format=torch.contiguous_format)  # strides of dimensions of one element too
             s = x.stride()
         rows.append(x)
-        strides.append(s[:3])
+        strides += s[:3] if len(s) == 4 else (0, *s[:2])
     return rows, _STRIDES[len(rows)](*strides)
 
 
@@ -65,21 +67,20 @@ def _check_rows(q: Tensor, k: Tensor, names: str) -> None:
         raise ValueError(f"at most {MAX_ROWS} rows are supported")
 
 
-def _check_prefix(prefix_k: Tensor, prefix_v: Tensor, batch: int, kv_heads: int, d: int, dv: int) -> Tuple[Tensor, Tensor]:
-    """A prefix [Hkv,P,D] as [1,Hkv,P,D]; shapes checked."""
-    if prefix_k.ndim != prefix_v.ndim or prefix_k.ndim not in (3, 4):
+def _check_prefix(prefix_k: Tensor, prefix_v: Tensor, batch: int, kv_heads: int, d: int, dv: int) -> Tuple[int, int]:
+    """(prefixes, rows of each) of [G,Hkv,P,D], or of [Hkv,P,D]; shapes checked."""
+    shape, values = prefix_k.shape, prefix_v.shape
+    if len(shape) != len(values) or len(shape) not in (3, 4):
         raise ValueError("prefix_k and prefix_v must be [Hkv,P,D] or [G,Hkv,P,D]")
-    if prefix_k.ndim == 3:
-        prefix_k, prefix_v = prefix_k[None], prefix_v[None]
-    sets, hk, p, pd = prefix_k.shape
-    if hk != kv_heads or pd != d or tuple(prefix_v.shape) != (sets, hk, p, dv):
+    sets, hk, p, pd = shape if len(shape) == 4 else (1, *shape)
+    if hk != kv_heads or pd != d or values[-1] != dv or values[:-1] != shape[:-1]:
         raise ValueError(f"prefix_k and prefix_v must be [G,{kv_heads},P,{d}] and [G,{kv_heads},P,{dv}], got "
                          f"{tuple(prefix_k.shape)} and {tuple(prefix_v.shape)}")
     if sets == 0 or batch % sets != 0:
         raise ValueError(f"the {batch} sequences must be a multiple of the {sets} prefixes")
     if p > MAX_ROWS:
         raise ValueError(f"at most {MAX_ROWS} rows are supported")
-    return prefix_k, prefix_v
+    return sets, p
 
 
 _workspaces: dict = {}  # bytes by shape, of the last few shapes
@@ -97,17 +98,17 @@ def _workspace(*shape) -> int:
     return nbytes
 
 
-def _attention(q: Tensor, k: Tensor, v: Tensor, pk: Tensor, pv: Tensor, lengths: Optional[Tensor],
+def _attention(q: Tensor, k: Tensor, v: Tensor, pk: Tensor, pv: Tensor, sets: int, p: int, lengths: Optional[Tensor],
                counts: Optional[Tensor], prefix_lengths: Optional[Tensor], scale: float,
                with_lse: bool) -> Tuple[Tensor, Optional[Tensor]]:
     b, h, n, d = q.shape
-    hk, m, dv, sets, p = k.shape[1], k.shape[2], v.shape[3], pk.shape[0], pk.shape[2]
-    out = q.new_empty((b, h, n, dv))
+    hk, m, dv = k.shape[1], k.shape[2], v.shape[3]
+    out = _like(q) if d == dv else q.new_empty((b, h, n, dv))
     lse = q.new_empty((b, h, n), dtype=torch.float32) if with_lse else None
     if out.numel() == 0:
         return out, lse
     if min(d, dv) * q.element_size() < 16:
-        wide = _attention(*(_widen(x) for x in (q, k, v, pk, pv)), lengths, counts, prefix_lengths, scale, with_lse)
+        wide = _attention(*(_widen(x) for x in (q, k, v, pk, pv)), sets, p, lengths, counts, prefix_lengths, scale, with_lse)
         return out.copy_(wide[0][..., :dv]), wide[1]
     (q, k, v, pk, pv), strides = _walkable(q, k, v, pk, pv)
     code = _native.DTYPE_CODES[q.dtype]
@@ -144,15 +145,15 @@ def shared_prefix_attention(q: Tensor, k: Tensor, v: Tensor, prefix_k: Tensor, p
     _refuse_gradients(q, k, v, prefix_k, prefix_v)
     _check_rows(q, k, "q, k and v")
     b, _, _, d = q.shape
-    if v.ndim != 4 or tuple(v.shape[:3]) != tuple(k.shape[:3]):
+    if v.ndim != 4 or v.shape[:3] != k.shape[:3]:
         raise ValueError(f"v must be [B,Hkv,M,Dv] like k, got {tuple(v.shape)} and {tuple(k.shape)}")
     if not 1 <= v.shape[3] <= MAX_DIM:
         raise ValueError(f"key and value widths must be 1 .. {MAX_DIM}, got {v.shape[3]}")
-    prefix_k, prefix_v = _check_prefix(prefix_k, prefix_v, b, k.shape[1], d, v.shape[3])
+    sets, p = _check_prefix(prefix_k, prefix_v, b, k.shape[1], d, v.shape[3])
     _check_dtype(q, k, v, prefix_k, prefix_v)
     lengths, counts = _check_lengths(lengths, b), _check_lengths(counts, b, "counts")
-    prefix_lengths = _check_lengths(prefix_lengths, prefix_k.shape[0], "prefix_lengths")
+    prefix_lengths = _check_lengths(prefix_lengths, sets, "prefix_lengths")
     _check_gpu(q, k, v, prefix_k, prefix_v, lengths, counts, prefix_lengths)
-    out, lse = _attention(q, k, v, prefix_k, prefix_v, lengths, counts, prefix_lengths, _attention_scale(scale, d),
-                          with_lse)
+    out, lse = _attention(q, k, v, prefix_k, prefix_v, sets, p, lengths, counts, prefix_lengths,
+                          _attention_scale(scale, d), with_lse)
     return (out, lse) if with_lse else out

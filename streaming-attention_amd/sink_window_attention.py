@@ -144,7 +144,7 @@ def _on(device: torch.device):
 
 def _widen(x: Tensor) -> Tensor:
     """x with zero columns up to the 16 bytes that the kernels' rows have at least."""
-    short = 16 // x.element_size() - x.shape[3]
+    short = 16 // x.element_size() - x.shape[-1]
     return torch.nn.functional.pad(x, (0, short)) if short > 0 else x
 
 
