@@ -28,16 +28,18 @@ int join_rows(const sta::PrefixArgs& a, int dtype, hipStream_t s) {
   return check_launch();
 }
 
-// How the received weights are dealt out.  Few rows: 2048 workgroups (eight a compute unit), whose waves have four blocks
-// of keys at least.  Many: a workgroup a tile of keys, and where that leaves fewer than 4096 several that share its rows, of
-// which the first tiles have most, 16 row tiles at least.
+// How the received weights are dealt out.  Few rows: as many workgroups as the card holds at a time (two a compute unit, four
+// of up to 64 columns of 16 bits), whose waves have four blocks of keys at least (16 x 8 key heads of 8192 rows, 128 wide, 128
+// rows: 64 us, 77 with 2048; 16 x 16 of 64: 47 with 1024, 54 with 512, 49 with 2048; fp32 175, 180 with 2048).  Many: a
+// workgroup a tile of keys, and where that leaves fewer than 4096 several that share its rows, of which the first tiles have
+// most, 16 row tiles at least.
 void plan_received(sta::ReceivedArgs& w, int dtype) {
   const sta::PrefixArgs& a = w.a;
   const int64_t units = static_cast<int64_t>(a.batch) * a.kv, rows = static_cast<int64_t>(a.n) * a.group;
   w.few = rows <= sta::RECEIVED_FEW;
   w.nsplit = 1;
   if (w.few) {
-    const int64_t want = ceil_div(2048, units), most = ceil_div(a.m, 4 * 4 * 32);
+    const int64_t want = ceil_div(dtype != STA_F32 && a.d <= 64 ? 1024 : 512, units), most = ceil_div(a.m, 4 * 4 * 32);
     w.tiles = static_cast<int>(want < most ? want : most);
     return;
   }
