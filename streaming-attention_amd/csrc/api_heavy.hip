@@ -268,6 +268,14 @@ int sta_heavy_start(const void* k, const void* v, const float* given, int dtype,
   dim3 g, heads;
   if (!tile_grid(f.h.r, g) || !head_grid(f.h.r, 1024, heads)) return STA_ERR_SHAPE;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  // up to a tile a compute unit (3 x 2 key heads of 1025 rows, 66 tiles: 13.2 us in two launches, 12.2 in one; 8 x 2000, 256
+  // tiles 14.0 and 13.0, 512 tiles 14.5 and 23.6)
+  if (static_cast<int64_t>(g.x) * g.y <= 256) {
+    by_type(dtype, [&](auto t) {
+      hipLaunchKernelGGL((sta::heavy_start_kernel<decltype(t)::value>), g, dim3(1024), 0, s, f);
+    });
+    return check_launch();
+  }
   hipLaunchKernelGGL(sta::heavy_select_kernel, heads, dim3(1024), 0, s, f);
   by_type(dtype, [&](auto t) {
     hipLaunchKernelGGL((sta::heavy_fill_kernel<decltype(t)::value>), g, dim3(256), 0, s, f);

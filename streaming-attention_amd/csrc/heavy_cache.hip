@@ -615,19 +615,18 @@ __device__ __forceinline__ float heavy_given(float w) { return w == w ? w + 0.f 
 // largest weights, of equal ones the first.  Three passes over the weights find the smallest that stays, 11 bits of its
 // order at a time (the highest first, among those that agree with it so far): the weights of a prompt lie within a few powers
 // of two, so that bins of 8 bits, the sign and 7 of the exponent's, would all be added to in one place.  One more pass puts the
-// rows that stay down in their order.  Bound by its barriers.  The first 8192 weights are held in registers.  16 x 8 key heads of 8192 rows: 16
-// us (the last pass 1024 at a time: 20; 8 x 65536 79 and 111).
-__global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFill f) {
+// rows that stay down in their order: put(slot, row or -1, weight) once for every slot.  Bound by its barriers.  The first
+// 8192 weights are held in registers.  16 x 8 key heads of 8192 rows: 16 us (the last pass 1024 at a time: 20; 8 x 65536 79
+// and 111).  first_of_head: the workgroup writes what a key
+// head has one of.
+template <typename Put>
+__device__ __forceinline__ void heavy_select(const HeavyFill& f, int sh, int n, bool first_of_head, Put put_row) {
   const HeavyArgs& h = f.h;
   constexpr int HOLD = 8, BINS = 2048;
   __shared__ int bins[BINS], wave_sum[16], chosen[2], cells[16 * HOLD];
   __shared__ unsigned long long red_low[16];
-  const int sh = blockIdx.x, s = sh / h.r.kv, n = heavy_take(f, s), t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  if (n == 0) return;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const float* given = f.given + static_cast<int64_t>(sh) * f.rows;
-  int* token = f.token + static_cast<int64_t>(sh) * h.pitch;
-  float* weights = h.weights + static_cast<int64_t>(sh) * h.pitch;
-  int64_t* positions = h.positions + static_cast<int64_t>(sh) * h.pitch;
   const int older = n > h.recent ? n - h.recent : 0;
   float hold[HOLD];
 #pragma unroll
@@ -757,32 +756,35 @@ __global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFi
         const bool stay = stays >> j & 1u;
         const int slot = h.ring + cells[16 * j + wave] + __popcll(__ballot(stay) & below);
         if (stay) {
-          token[slot] = i0 + 1024 * j + t;
-          weights[slot] = hold[j];
-          positions[slot] = i0 + 1024 * j + t;
+          put_row(slot, i0 + 1024 * j + t, hold[j]);
           low = heavy_min(low, heavy_key(hold[j], slot));
         }
       }
     }
     __syncthreads();
   }
-  for (int slot = h.ring + taken + t; slot < h.pitch; slot += 1024) {
-    token[slot] = -1;
-    weights[slot] = 0.f;
-    positions[slot] = -1;
-  }
+  for (int slot = h.ring + taken + t; slot < h.pitch; slot += 1024) put_row(slot, -1, 0.f);
   for (int slot = t; slot < h.ring; slot += 1024) {
     const int p = n - 1 - static_cast<int>((static_cast<int64_t>(n) - 1 - slot + h.ring) % h.ring);
     const bool in = p >= 0 && p >= older;
-    token[slot] = in ? p : -1;
-    weights[slot] = in ? heavy_given(given[p]) : 0.f;
-    positions[slot] = in ? p : -1;
+    put_row(slot, in ? p : -1, in ? heavy_given(given[p]) : 0.f);
   }
   low = heavy_least<1024>(low, red_low);
-  if (t == 0) {
+  if (t == 0 && first_of_head) {
     h.lowest[2 * static_cast<int64_t>(sh) + (n & 1)] = low;
     h.counts[sh] = n;
   }
+}
+
+__global__ __launch_bounds__(1024) static void heavy_select_kernel(const HeavyFill f) {
+  const int sh = blockIdx.x, n = heavy_take(f, sh / f.h.r.kv);
+  if (n == 0) return;
+  const int64_t at = static_cast<int64_t>(sh) * f.h.pitch;
+  heavy_select(f, sh, n, true, [&](int slot, int row, float weight) {
+    f.token[at + slot] = row;
+    f.h.weights[at + slot] = weight;
+    f.h.positions[at + slot] = row;
+  });
 }
 
 // The rows that stay into their slots: a workgroup a tile.
@@ -797,6 +799,26 @@ __global__ __launch_bounds__(256) void heavy_fill_kernel(const HeavyFill f) {
   if (threadIdx.x < 32) token[threadIdx.x] = f.token[static_cast<int64_t>(sh) * f.h.pitch + 32 * tile + threadIdx.x];
   if (!__syncthreads_or(threadIdx.x < 32 && token[threadIdx.x] >= 0)) return;
   ring_fill<ST, ST>(a, s, hk, tile, token);
+}
+
+// Both in one launch, for few tiles: the workgroup of each selects for itself and keeps what falls into its tile.
+template <int ST>
+__global__ __launch_bounds__(1024) void heavy_start_kernel(const HeavyFill f) {
+  const RingArgs& a = f.h.r;
+  __shared__ int token[32];
+  const int sh = blockIdx.x / a.tiles, tile = blockIdx.x - sh * a.tiles, s = sh / a.kv;
+  const int n = heavy_take(f, s);
+  if (n == 0) return;
+  const int64_t at = static_cast<int64_t>(sh) * f.h.pitch;
+  heavy_select(f, sh, n, tile == 0, [&](int slot, int row, float weight) {
+    if (slot >> 5 != tile) return;
+    token[slot & 31] = row;
+    f.h.weights[at + slot] = weight;
+    f.h.positions[at + slot] = row;
+  });
+  __syncthreads();
+  if (!__syncthreads_or(threadIdx.x < 32 && token[threadIdx.x & 31] >= 0)) return;
+  ring_fill<ST, ST, 1024>(a, s, sh - s * a.kv, tile, token);
 }
 
 // The slots as they are: rows, positions and weights.

@@ -614,8 +614,8 @@ __device__ __forceinline__ int ring_take(const RingFill& f, int s) {
   return t < 0 ? 0 : (t > f.rows ? f.rows : t);
 }
 
-// The rows token[0 .. 31] (-1: none) of a stream's key head into the slots of a tile, by a workgroup of 256 threads.
-template <int ST, int Q>
+// The rows token[0 .. 31] (-1: none) of a stream's key head into the slots of a tile, by a workgroup of THREADS threads.
+template <int ST, int Q, int THREADS = 256>
 __device__ __forceinline__ void ring_fill(const RingArgs& a, int s, int hk, int tile, const int* token) {
   constexpr int ES = Q == F32 ? 4 : 2;
   __shared__ uint32_t vals[32 * 132];  // the tile's values (bits, or codes), 32 nbv + 1 a slot
@@ -625,7 +625,7 @@ __device__ __forceinline__ void ring_fill(const RingArgs& a, int s, int hk, int 
   uint8_t* values = a.values + at * ring_tile_bytes(a.nbv, ST);
   const int pitch = 32 * a.nbv + 1;
   // 8 columns of a slot's key a thread, 4 neighbouring threads a block
-  for (int i = threadIdx.x; i < 32 * 4 * a.nbk; i += 256) {
+  for (int i = threadIdx.x; i < 32 * 4 * a.nbk; i += THREADS) {
     const int r = i / (4 * a.nbk), u = i - r * 4 * a.nbk, col = 8 * u, p = token[r];
     const char* row = rows_at<ES>(a.k, s, hk, p < 0 ? 0 : p);
     uint8_t* to = keys + ring_key_at(r, col, a.nbk, ST);
@@ -658,7 +658,7 @@ __device__ __forceinline__ void ring_fill(const RingArgs& a, int s, int hk, int 
     }
   }
   // values: the rows (codes) of the tile's slots, then 8 slots of a column a thread
-  for (int i = threadIdx.x; i < 32 * 4 * a.nbv; i += 256) {
+  for (int i = threadIdx.x; i < 32 * 4 * a.nbv; i += THREADS) {
     const int r = i / (4 * a.nbv), u = i - r * 4 * a.nbv, col = 8 * u, p = token[r];
     const char* row = rows_at<ES>(a.v, s, hk, p < 0 ? 0 : p);
     constexpr int E = 16 / ES;
@@ -694,7 +694,7 @@ __device__ __forceinline__ void ring_fill(const RingArgs& a, int s, int hk, int 
     }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 64 * (ST == RING_F4 ? a.nbv : 2 * a.nbv); i += 256) {
+  for (int i = threadIdx.x; i < 64 * (ST == RING_F4 ? a.nbv : 2 * a.nbv); i += THREADS) {
     const int lane = i & 63, ct = i >> 6, g = lane >> 4;
     const int col = ST == RING_F4 ? 32 * ct + (lane & 15) : 16 * ct + (lane & 15);
     uint32_t w[8];

@@ -139,7 +139,7 @@ class HeavyHitterStreamingAttention:
         self._state = tuple(x.data_ptr() for x in self._tensors.values())
         self._views = self._weights[..., :self._slots], self._positions[..., :self._slots]
         shape = (streams, kv_heads, self._slots)  # of the items' rows, without memory of their own
-        self._items = tuple(room(1, dtype=t).expand(size) for size, t in (
+        self._items = tuple(torch.empty(1, dtype=t, device=self.device).expand(size) for size, t in (
             ((*shape, dim), dtype), ((*shape, value_dim), dtype), (shape, torch.int64), (shape, torch.float32)))
         self._shapes = {"query": (streams, heads, dim), "key": (streams, kv_heads, dim),
                         "value": (streams, kv_heads, value_dim)}

@@ -117,7 +117,9 @@ def rows(streams, kv, n, d, dv, dtype, seed=0):
 @pytest.mark.parametrize("kind", ["random", "equal", "two", "extreme", "signs"])
 @pytest.mark.parametrize("streams,kv,n,kept,recent,counts", [
     (1, 1, 1, 1, 1, None), (2, 1, 40, 16, 8, None), (3, 2, 100, 37, 5, [100, 0, 41]), (2, 2, 3000, 1000, 77, [2999, 1078]),
-    (1, 2, 2500, 31, 1, None), (4, 1, 64, 100, 20, [64, -1, 1, 99]), (1, 1, 5000, 1500, 3400, None)])
+    (1, 2, 2500, 31, 1, None), (4, 1, 64, 100, 20, [64, -1, 1, 99]), (1, 1, 5000, 1500, 3400, None),
+    # more rows than are held in registers, and caches of more tiles than compute units
+    (1, 1, 9000, 500, 100, None), (40, 4, 60, 40, 9, [60, 0, 3, -1] * 10), (2, 4, 17000, 1000, 200, [17000, 16383])])
 def test_start(streams, kv, n, kept, recent, counts, kind):
     """Which tokens of a prompt stay: random weights, equal ones (the first stay), two values, extremes, both signs."""
     dtype, d, dv = torch.bfloat16, 16, 8
