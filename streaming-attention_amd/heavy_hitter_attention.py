@@ -265,6 +265,8 @@ class HeavyHitterStreamingAttention:
         if rows == 0:
             return
         weights = weights.detach().contiguous()
+        if 0 <= weights.data_ptr() - self._state[3] < 4 * self._weights.numel():  # the state's own, which the call writes
+            weights = weights.clone()
         (k, v), strides = _walkable(k, v)
         lib = _native.lib()
         with _on(self.device):

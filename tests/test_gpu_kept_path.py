@@ -473,3 +473,16 @@ def test_queries_of_empty_caches_behind_a_prefix(dtype):
     want = ref.prefix_attention(q.cpu()[:, :, None], k, v, pk[:1, :, :0], pv[:1, :, :0], lengths=[600, 600, 3, 3])
     check({"out": got[:, :, None]}, {"out": want["out"]})
     assert c.query(q).eq(0).all() and c.weights.eq(0).all() and c.lengths.eq(0).all()
+
+
+@pytest.mark.parametrize("streams,kv,kept,first", [(1, 1, 24, 0), (1, 1, 24, 9), (2, 2, 24, 0), (1, 1, 9000, 0)])
+def test_starts_from_the_state_s_own_weights(streams, kv, kept, first):
+    """`weights` is a view of what start writes."""
+    slots = kept + 8
+    c = cache_of(streams=streams, heads=kv, kv=kv, kept=kept, recent=7, n=slots + 5)
+    own = c.weights[..., first:]
+    k, v = (t.to(DEV) for t in make(6, c.dtype, (streams, kv, slots - first, 32), (streams, kv, slots - first, 24)))
+    want = cache_of(streams=streams, heads=kv, kv=kv, kept=kept, recent=7, n=slots + 5)
+    want.start(k, v, own.clone())
+    c.start(k, v, own)
+    assert same(c, want)
