@@ -615,10 +615,9 @@ __device__ __forceinline__ float heavy_given(float w) { return w == w ? w + 0.f 
 // largest weights, of equal ones the first.  Three passes over the weights find the smallest that stays, 11 bits of its
 // order at a time (the highest first, among those that agree with it so far): the weights of a prompt lie within a few powers
 // of two, so that bins of 8 bits, the sign and 7 of the exponent's, would all be added to in one place.  One more pass puts the
-// rows that stay down in their order: put(slot, row or -1, weight) once for every slot.  Bound by its barriers.  The first
+// rows that stay down in their order: put_row(slot, row or -1, weight) once for every slot.  Bound by its barriers.  The first
 // 8192 weights are held in registers.  16 x 8 key heads of 8192 rows: 16 us (the last pass 1024 at a time: 20; 8 x 65536 79
-// and 111).  first_of_head: the workgroup writes what a key
-// head has one of.
+// and 111).  first_of_head: the workgroup writes what a key head has one of.
 template <typename Put>
 __device__ __forceinline__ void heavy_select(const HeavyFill& f, int sh, int n, bool first_of_head, Put put_row) {
   const HeavyArgs& h = f.h;

@@ -34,11 +34,9 @@ int launch_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int values, hip
   if constexpr (IN != sta::F32) {
     if (p.stream && !p.share[0] && a.d % 8 == 0 && (!values || a.dv % 8 == 0)) {
       const int lds = values ? least(sta::prefix_stream_bytes<P, true>()) : sta::prefix_stream_bytes<P, false>();
-      if (p.walks == 2) {
-        return p.share[1] ? launch(sta::prefix_walks_kernel<P, IN, false, true, true>, lds > shared ? lds : shared, p.walk[0],
-                                   p.walk[1], ga, gb)
-                          : launch(sta::prefix_walks_kernel<P, IN, false, false, true>, lds, p.walk[0], p.walk[1], ga, gb);
-      }
+      if (p.walks == 2)
+        return launch(sta::prefix_walks_kernel<P, IN, false, true, true>, lds > shared ? lds : shared, p.walk[0], p.walk[1], ga,
+                      gb);
       return values ? launch(sta::prefix_attention_kernel<P, IN, false, true, true>, lds, p.walk[0])
                     : launch(sta::prefix_attention_kernel<P, IN, false, false, true>, lds, p.walk[0]);
     }
@@ -46,10 +44,12 @@ int launch_prefix(const sta::PrefixArgs& a, const PrefixPlan& p, int values, hip
   if (p.walks == 2) {
     if (p.share[0] && p.share[1])
       return launch(sta::prefix_walks_kernel<P, IN, true, true, false>, shared, p.walk[0], p.walk[1], ga, gb);
-    if (p.share[1])
-      return launch(sta::prefix_walks_kernel<P, IN, false, true, false>, wide > shared ? wide : shared, p.walk[0], p.walk[1],
-                    ga, gb);
-    return launch(sta::prefix_walks_kernel<P, IN, false, false, false>, wide, p.walk[0], p.walk[1], ga, gb);
+    if constexpr (IN == sta::F32) {  // 16-bit rows that are walked apart are few
+      if (!p.share[1])
+        return launch(sta::prefix_walks_kernel<P, IN, false, false, false>, wide, p.walk[0], p.walk[1], ga, gb);
+    }
+    return launch(sta::prefix_walks_kernel<P, IN, false, true, false>, wide > shared ? wide : shared, p.walk[0], p.walk[1], ga,
+                  gb);
   }
   if (values) {
     return p.share[0] ? launch(sta::prefix_attention_kernel<P, IN, true, true, false>, shared, p.walk[0])

@@ -670,8 +670,8 @@ __global__ __launch_bounds__(256, (prefix_waves<P, IN, SHARE, VALUES, STREAM>())
 }
 
 // Both walks of a batch of few rows in one launch: that over the prefix is bound by products and by latency, that over the
-// own tokens by memory.  64 x 32 heads, 128 wide, 32768 shared and up to 1024 own rows: 56 and 32 us one after the other, 78
-// together, with the prefix's workgroups first (98 with the two in turn).
+// own tokens by memory.  64 x 32 heads, 128 wide, 32768 shared and up to 1024 own rows: 74 us, that over the prefix by itself
+// 63; the prefix's workgroups first (with the two in turn 98 us, 78 then).
 template <int P, int IN, bool SHARE_A, bool SHARE_B, bool STREAM>
 __global__ __launch_bounds__(256, (prefix_waves<P, IN, SHARE_B, true, false>() < prefix_waves<P, IN, SHARE_A, true, STREAM>()
                                        ? prefix_waves<P, IN, SHARE_B, true, false>()

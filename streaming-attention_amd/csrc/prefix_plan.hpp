@@ -14,7 +14,7 @@ constexpr int kMaxPrefixParts = 256;  // prefix_join_kernel's weights
 struct PrefixPlan {
   int walks;
   sta::PrefixWalk walk[2];
-  int share[2];
+  int share[2];     // tiles of 32 rows whose waves share the keys, see deal_out; of two walks of 16-bit rows the second's always
   int parts;        // 0: one workgroup finishes a row
   int stream;       // the first walk's keys and values lie on 16 bytes: prefix_stream_pass where the widths allow it
 };
