@@ -2,6 +2,8 @@
 // checks, plans, launches.
 #include "prefix_dispatch.hpp"
 
+#include <utility>
+
 using namespace sta_api;
 
 namespace {
@@ -32,7 +34,8 @@ int join_rows(const sta::PrefixArgs& a, int dtype, hipStream_t s) {
 // of up to 64 columns of 16 bits), whose waves have four blocks of keys at least (16 x 8 key heads of 8192 rows, 128 wide, 128
 // rows: 64 us, 77 with 2048; 16 x 16 of 64: 47 with 1024, 54 with 512, 49 with 2048; fp32 175, 180 with 2048).  Many: a
 // workgroup a tile of keys, and where that leaves fewer than 4096 several that share its rows, of which the first tiles have
-// most, 16 row tiles at least.
+// most, 8 row tiles of 64 at least (4 x 8 x 4 heads of 1024 rows of 128: 41 us, 45 with 16, 45 with 4), 2 of up to 512
+// workgroups and 1 of up to 256 (8 x 4 heads of 256 rows 9.5 us, 11 with 2, 36 with 16; of 512 rows 15, of 1024 21, and 35).
 void plan_received(sta::ReceivedArgs& w, int dtype) {
   const sta::PrefixArgs& a = w.a;
   const int64_t units = static_cast<int64_t>(a.batch) * a.kv, rows = static_cast<int64_t>(a.n) * a.group;
@@ -44,10 +47,11 @@ void plan_received(sta::ReceivedArgs& w, int dtype) {
     return;
   }
   w.tiles = static_cast<int>(ceil_div(a.m, dtype == STA_F32 ? 128 : 256));
-  int64_t want = 4096 / (units * w.tiles);
-  const int64_t most = ceil_div(a.group * ceil_div(a.n, 64), 16);
-  if (want > most) want = most;
-  w.nsplit = static_cast<int>(want < 1 ? 1 : want);
+  const int64_t row_tiles = a.group * ceil_div(a.n, 64);
+  for (const auto& [groups, least] : {std::pair<int64_t, int64_t>{256, 1}, {512, 2}, {4096, 8}}) {
+    const int64_t want = groups / (units * w.tiles), most = ceil_div(row_tiles, least), split = want < most ? want : most;
+    if (split > w.nsplit) w.nsplit = static_cast<int>(split);
+  }
 }
 
 int64_t received_sum_bytes(const sta::ReceivedArgs& w) {
