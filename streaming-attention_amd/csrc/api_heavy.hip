@@ -51,13 +51,16 @@ int heavy_shape(sta::HeavyArgs& h, int dtype, int64_t streams, int heads, int kv
   return STA_OK;
 }
 
-// Workgroups that share a key head's slots: two a compute unit of the whole launch, each with at least 8 tiles.
-int splits_of(const sta::RingArgs& a) {
+// Workgroups that share a key head's slots: one a compute unit of the whole launch, whose waves have a tile at least (32 x 8
+// key heads of 2048 slots of 128: 49 us, 62 with two a compute unit, 8 of 16000 20 and 20, fp32 39 and 49; 8 of 1024 slots in
+// shares of four tiles 12 us, of eight 13, fp32 15 and 21).  Short caches have one, which finishes their key heads in one
+// launch (64 wide, 800 slots 9.1 us, 9.4 shared, 1050 slots 10.3 and 9.4; 128 wide, 430 slots 9.0 and 9.7, 560 slots 12.4 and
+// 11.8 with four query heads; fp32 128 wide, 170 slots 12.4 and 12.6, 300 slots 15 and 12).
+int splits_of(const sta::RingArgs& a, int dtype) {
   const int64_t work = static_cast<int64_t>(a.streams) * a.kv * a.chunks;
-  int64_t want = 512 / work;
-  const int64_t most = a.tiles / 8 < 512 ? a.tiles / 8 : 512;
-  if (want > most) want = most;
-  return static_cast<int>(want < 1 ? 1 : want);
+  if (static_cast<int64_t>(a.tiles) * (a.nbk + a.nbv) <= (dtype == STA_F32 ? 40 : 104)) return 1;
+  const int64_t want = 256 / work, most = (a.tiles + 3) / 4, split = want < most ? want : most;
+  return static_cast<int>(split < 1 ? 1 : split);
 }
 
 // A shared prefix in front of the cache: one row a head, that of the one own token, which the walk leaves to the cache.
@@ -84,8 +87,8 @@ Workspace workspace_of(const sta::HeavyArgs& h, const sta::PrefixArgs* p, int pr
   if (p) w.prefix = prefix_part_bytes(*p, prefix_parts);
   return w;
 }
-void plan_heavy(sta::HeavyArgs& h, int prefix_parts) {
-  h.r.nsplit = splits_of(h.r);
+void plan_heavy(sta::HeavyArgs& h, int dtype, int prefix_parts) {
+  h.r.nsplit = splits_of(h.r, dtype);
   h.prefix_parts = prefix_parts;
   h.alone = h.r.nsplit == 1 && h.r.chunks == 1 && prefix_parts == 0;
   // two workgroups a compute unit with the logits in LDS, and the kernel's own kilobyte
@@ -159,13 +162,13 @@ int64_t sta_heavy_attention_bytes(int dtype, int64_t streams, int heads, int kv_
   if (heavy_shape(h, dtype, streams, heads, kv_heads, d, dv, recent, kept) != STA_OK) return -1;
   if (p < 0) return -1;
   if (p == 0) {
-    plan_heavy(h, 0);
+    plan_heavy(h, dtype, 0);
     return workspace_of(h, nullptr, 0).total();
   }
   sta::PrefixArgs x;
   if (prefix_of(x, h.r, dtype, sets, p, 1.f) != STA_OK) return -1;
   const int parts = plan_prefix(x, dtype, false).parts;
-  plan_heavy(h, parts);
+  plan_heavy(h, dtype, parts);
   return workspace_of(h, &x, parts).total();
 }
 
@@ -199,7 +202,7 @@ int sta_heavy_attention(const void* q, const void* k, const void* v, int dtype, 
     if (!prefix_strides_ok(prefix_strides, 2, dtype)) return STA_ERR_UNSUPPORTED;
     plan = plan_prefix(x, dtype, false);
   }
-  plan_heavy(h, plan.parts);
+  plan_heavy(h, dtype, plan.parts);
   const Workspace w = workspace_of(h, p > 0 ? &x : nullptr, plan.parts);
   if (w.total() > 0 && (!workspace || !aligned16(workspace) || workspace_bytes < w.total())) return STA_ERR_SCRATCH;
   char* room = static_cast<char*>(workspace);
