@@ -153,7 +153,7 @@ def test_start(streams, kv, n, kept, recent, counts, kind):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("streams,heads,kv,kept,recent,d,dv,p,plen", [
     (1, 1, 1, 4, 2, 8, 8, 1, None), (4, 8, 2, 30, 10, 64, 64, 200, 130), (2, 6, 2, 12, 5, 93, 77, 700, None),
-    (3, 4, 4, 300, 40, 128, 128, 64, 0)])
+    (3, 4, 4, 300, 40, 128, 128, 64, 0), (2, 6, 3, 600, 30, 128, 96, 150, 149)])
 def test_steps_behind_a_prefix(streams, heads, kv, kept, recent, d, dv, p, plen, dtype):
     cache = hha.HeavyHitterStreamingAttention(d, dv, streams=streams, heads=heads, kv_heads=kv, kept=kept, recent=recent,
                                               dtype=dtype)
@@ -180,7 +180,7 @@ def test_prefixes_of_groups(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("heads,kv,kept", [(4, 1, 9000), (32, 1, 3000), (8, 8, 2500)])
+@pytest.mark.parametrize("heads,kv,kept", [(4, 1, 9000), (32, 1, 3000), (8, 8, 2500), (6, 3, 560), (6, 3, 900)])
 def test_caches_split_over_workgroups(heads, kv, kept, dtype):
     recent, d, dv = 100, 40, 64
     cache = hha.HeavyHitterStreamingAttention(d, dv, heads=heads, kv_heads=kv, kept=kept, recent=recent, dtype=dtype)
