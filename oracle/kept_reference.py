@@ -68,8 +68,8 @@ def prefix_attention(q, k, v, pk, pv, *, lengths=None, counts=None, prefix_lengt
     return {name: tuple(x) for name, x in res.items()}
 
 
-def received(q, k, *, lengths=None, counts=None, lse=None, scale=None):
-    """(value, bound) [B,Hkv,M] of the weights that the own tokens receive."""
+def received(q, k, *, lengths=None, counts=None, lse=None, scale=None, hide=None):
+    """(value, bound) [B,Hkv,M] of the weights that the own tokens receive; hide: bool [M], keys with logits of -inf."""
     b, h, n, d = q.shape
     hk, m = k.shape[1], k.shape[2]
     scale = 1 / math.sqrt(d) if scale is None else scale
@@ -80,6 +80,8 @@ def received(q, k, *, lengths=None, counts=None, lse=None, scale=None):
         if c == 0:
             continue
         hidden = torch.ones(c, length, dtype=torch.bool).triu(length - c + 1)
+        if hide is not None:
+            hidden |= hide[:length]
         for j in range(h):
             g = j * hk // h
             p, own, rel, el = _weights(q[i, j, :c].double(), k[i, g, :length].double(), hidden, scale, d)

@@ -898,18 +898,23 @@ __device__ __forceinline__ void received_walk(const ReceivedArgs& w, int id, uin
     };
     auto rows_of = [&](const At& x) { return rows_at<ES>(a.q, b, hk * a.group + x.g, x.i); };
     auto take = [&](int row, const uint4* qs, const float* stat) {
-      const bool every = base + row >= w0 + 32 * NB - 1;
+      // every row sees every key, and there is one in every place: what fills up the last tile may meet an infinite key
+      const bool every = base + row >= w0 + 32 * NB - 1 && row + BQ <= count;
 #pragma unroll
       for (int sub = 0; sub < BQ / 32; ++sub) {
         floatx16 x[NB];
         received_weights<P, IN, NB>(x, qs, stat, 32 * sub, kf, a.c, lane);
         if (!every) {
+          const int end = count - row - 32 * sub - 4 * hh;  // of the lane's rows
 #pragma unroll
           for (int n = 0; n < NB; ++n) {
             // the first of the lane's rows that sees its key
             const int from = w0 + 32 * n + (lane & 31) - base - row - 32 * sub - 4 * hh;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[n][e] = 8 * (e >> 2) + (e & 3) >= from ? x[n][e] : 0.f;
+            for (int e = 0; e < 16; ++e) {
+              const int at = 8 * (e >> 2) + (e & 3);
+              x[n][e] = at >= from && at < end ? x[n][e] : 0.f;
+            }
           }
         }
 #pragma unroll
@@ -1004,7 +1009,7 @@ __global__ __launch_bounds__(256, 2) void received_few_kernel(const ReceivedArgs
   const int room = (a.n * a.group + 31) / 32 * 32;
   uint4 *const qs = win_lds, *const ks = qs + room * CH + wave * 32 * CH;
   float* const stat = reinterpret_cast<float*>(qs + (room + 4 * 32) * CH);
-  int* const seen = reinterpret_cast<int*>(stat + room);  // the last token that a row sees
+  int* const seen = reinterpret_cast<int*>(stat + room);  // the last token that a row sees, -1 in the place of a row
   float* const to = w.weights + static_cast<int64_t>(unit) * a.m;
 
   const int step = 4 * w.tiles, first = 4 * part + wave;  // blocks of keys
@@ -1027,7 +1032,7 @@ __global__ __launch_bounds__(256, 2) void received_few_kernel(const ReceivedArgs
   for (int r = threadIdx.x; r < 32 * blocks; r += 256) {
     const int i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) - i * a.group;
     stat[r] = received_stat(a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.n + i], r < rows);
-    seen[r] = base + i;
+    seen[r] = r < rows ? base + i : -1;
   }
   __syncthreads();
 
@@ -1053,7 +1058,7 @@ __global__ __launch_bounds__(256, 2) void received_few_kernel(const ReceivedArgs
       for (int r0 = 0; r0 < 32 * blocks; r0 += 32) {
         floatx16 x[1];
         received_weights<P, IN, 1>(x, qs, stat, r0, kf, a.c, lane);
-        if (32 * block + 31 > base) {
+        if (32 * block + 31 > base || r0 + 32 > rows) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) x[0][e] = key <= seen[r0 + 8 * (e >> 2) + 4 * hh + (e & 3)] ? x[0][e] : 0.f;
         }
