@@ -898,8 +898,9 @@ __device__ __forceinline__ void received_walk(const ReceivedArgs& w, int id, uin
     };
     auto rows_of = [&](const At& x) { return rows_at<ES>(a.q, b, hk * a.group + x.g, x.i); };
     auto take = [&](int row, const uint4* qs, const float* stat) {
-      // every row sees every key, and there is one in every place: what fills up the last tile may meet an infinite key
-      const bool every = base + row >= w0 + 32 * NB - 1 && row + BQ <= count;
+      // Every row sees every key, and there is one in every place: zeros that fill up the last tile give NaN with an infinite key
+      // (straight to LDS the last row fills it up, whose logits are its own).
+      const bool every = base + row >= w0 + 32 * NB - 1 && (STREAM || row + BQ <= count);
 #pragma unroll
       for (int sub = 0; sub < BQ / 32; ++sub) {
         floatx16 x[NB];
@@ -913,7 +914,7 @@ __device__ __forceinline__ void received_walk(const ReceivedArgs& w, int id, uin
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
               const int at = 8 * (e >> 2) + (e & 3);
-              x[n][e] = at >= from && at < end ? x[n][e] : 0.f;
+              x[n][e] = at >= from && (STREAM || at < end) ? x[n][e] : 0.f;
             }
           }
         }
@@ -1009,7 +1010,7 @@ __global__ __launch_bounds__(256, 2) void received_few_kernel(const ReceivedArgs
   const int room = (a.n * a.group + 31) / 32 * 32;
   uint4 *const qs = win_lds, *const ks = qs + room * CH + wave * 32 * CH;
   float* const stat = reinterpret_cast<float*>(qs + (room + 4 * 32) * CH);
-  int* const seen = reinterpret_cast<int*>(stat + room);  // the last token that a row sees, -1 in the place of a row
+  int* const seen = reinterpret_cast<int*>(stat + room);  // the last token that a row sees
   float* const to = w.weights + static_cast<int64_t>(unit) * a.m;
 
   const int step = 4 * w.tiles, first = 4 * part + wave;  // blocks of keys
@@ -1025,14 +1026,13 @@ __global__ __launch_bounds__(256, 2) void received_few_kernel(const ReceivedArgs
 
   for (int u = threadIdx.x; u < 32 * blocks * CH; u += 256) {
     const int r = u / CH, c = u - r * CH, i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) - i * a.group;
-    const uint4 x = rows_unit<ES>(rows_at<ES>(a.q, b, h, i), c * E, a.d);
-    qs[r * CH + (c ^ win_swizzle<CH>(r))] = uint4{r < rows ? x.x : 0u, r < rows ? x.y : 0u, r < rows ? x.z : 0u,
-                                                  r < rows ? x.w : 0u};
+    // the last row fills up the last block: it sees every key, and zeros would give NaN with an infinite one
+    qs[r * CH + (c ^ win_swizzle<CH>(r))] = rows_unit<ES>(rows_at<ES>(a.q, b, h, i), c * E, a.d);
   }
   for (int r = threadIdx.x; r < 32 * blocks; r += 256) {
     const int i = min(r, rows - 1) / a.group, h = hk * a.group + min(r, rows - 1) - i * a.group;
     stat[r] = received_stat(a.lse[(static_cast<int64_t>(b) * a.heads + h) * a.n + i], r < rows);
-    seen[r] = r < rows ? base + i : -1;
+    seen[r] = base + i;
   }
   __syncthreads();
 
@@ -1058,7 +1058,7 @@ __global__ __launch_bounds__(256, 2) void received_few_kernel(const ReceivedArgs
       for (int r0 = 0; r0 < 32 * blocks; r0 += 32) {
         floatx16 x[1];
         received_weights<P, IN, 1>(x, qs, stat, r0, kf, a.c, lane);
-        if (32 * block + 31 > base || r0 + 32 > rows) {
+        if (32 * block + 31 > base) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) x[0][e] = key <= seen[r0 + 8 * (e >> 2) + 4 * hh + (e & 3)] ? x[0][e] : 0.f;
         }
