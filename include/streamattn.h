@@ -633,9 +633,10 @@ int64_t sta_heavy_attention_bytes(int dtype, int64_t streams, int heads, int kv_
  * out [streams][heads][dv] (dense) = softmax attention of q [streams][heads][d] over the tokens held, after the new tokens k
  * [streams][kv_heads][d], v [..][dv] went in (both NULL: no new token), and over a prefix that the streams of a set share;
  * nothing to see gives 0.  Each token's weight grows by the softmax weights that it gets from the query heads of its key
- * head (increments that are not finite are left out).  strides [3][2] (host memory): element strides of stream and head
- * of q, k and v.  prefix_k [sets][kv_heads][p][d], prefix_v [..][dv], prefix_strides [2][3], prefix_lengths: as
- * sta_prefix_attention (rows of at least 16 bytes then), p 0: none.  workspace: caller-allocated, 16-byte aligned, of
+ * head (increments that are not finite are left out), or falls to -FLT_MAX where its logit with a query below 2^64 is +inf
+ * or NaN.  strides [3][2] (host memory): element strides of stream and head of q, k and v.  prefix_k [sets][kv_heads][p][d],
+ * prefix_v [..][dv], prefix_strides [2][3], prefix_lengths: as sta_prefix_attention (rows of at least 16 bytes then), p 0:
+ * none.  workspace: caller-allocated, 16-byte aligned, of
  * sta_heavy_attention_bytes (contents undefined before and after).
  */
 int sta_heavy_attention(const void* q, const void* k, const void* v, int dtype, int64_t streams, int heads, int kv_heads,

@@ -28,7 +28,7 @@ def small(dtype, values):
 def _weights(q, keys, hidden, scale, d):
     """(weights [rows, keys], log2 of their sums, relative bound of a weight, absolute bound of the log2)."""
     x = (q @ keys.T) * scale
-    size = torch.where(hidden, 0.0, (q.abs() @ keys.abs().T) * abs(scale)).amax(1, keepdim=True)
+    size = torch.where(hidden | ~torch.isfinite(x), 0.0, (q.abs() @ keys.abs().T) * abs(scale)).amax(1, keepdim=True)
     x = torch.where(hidden, -math.inf, x)
     top = x.amax(1, keepdim=True)
     p = torch.exp(x - top)
@@ -94,6 +94,9 @@ def received(q, k, *, lengths=None, counts=None, lse=None, scale=None, hide=None
             # a sum of c weights a head: sixteen at a time, the rest compensated, the heads' and splits' totals
             out[1][i, g, :length] += (p * rel).sum(0) + F24 * 48 * p.sum(0)
     return tuple(out)
+
+
+LEAST = -torch.finfo(torch.float32).max  # weight of a token whose logits are not finite
 
 
 class Cache:
@@ -172,16 +175,25 @@ class Cache:
                 if not keys:
                     continue
                 keys, values = torch.stack(keys).double(), torch.stack(values).double()
-                p, _, rel, _ = _weights(q[s, h * group:(h + 1) * group].double(), keys,
-                                        torch.zeros(group, keys.shape[0], dtype=torch.bool), scale, d)
+                rows = q[s, h * group:(h + 1) * group].double()
+                p, _, rel, _ = _weights(rows, keys, torch.zeros(group, keys.shape[0], dtype=torch.bool), scale, d)
+                # logits of +inf (beyond float32) or NaN: the row has no weights, the token the least, if the query is sane
+                logits = rows @ keys.T * (-1.0 if scale < 0 else 1.0)
+                lost = ~(logits <= -LEAST)
+                p = torch.where(lost.any(1, keepdim=True), math.nan, p)
+                lost = (lost & (rows.abs() < 2.0 ** 64).all(1, keepdim=True)).any(0)
                 o, a = p @ values, p @ values.abs()
                 out[0][s, h * group:(h + 1) * group] = o
                 out[1][s, h * group:(h + 1) * group] = (u * o.abs() + (w16 + 2 * rel + F24 * keys.shape[0]) * a
                                                         + small(q.dtype, values))
                 for i, x in enumerate(held):
-                    x[1] += float(p[:, i].sum())
+                    if lost[i]:
+                        x[1:] = [min(x[1], LEAST), x[2], x[3], 0.0]
+                        continue
+                    fine = torch.isfinite(p[:, i])
+                    x[1] += float(p[fine, i].sum())
                     # the weights' own errors, their sum over the heads, its addition
-                    grown = float((p[:, i] * (2 * rel[:, 0] + F24 * (group + 8))).sum()) + F24 * abs(x[1])
+                    grown = float((p[:, i] * (2 * rel[:, 0] + F24 * (group + 8)))[fine].sum()) + F24 * abs(x[1])
                     if len(x) == 4:
                         x.append(0.0)
                     x[4] += grown

@@ -9,7 +9,10 @@
 //   p_hj = exp(s q_h.k_j - L_h), L_h = log of the sum over the tokens held (and the rows of a shared prefix),
 //   o_h = sum_j p_hj v_j,   W_j += sum over the query heads of the key head of p_hj
 // Increments that are not finite are left out, so that a token held with an infinity or NaN does not make its
-// neighbours' weights NaN, and itself leaves in the end.
+// neighbours' weights NaN.  A token whose logit is +inf or NaN with a finite query makes that row's weights NaN, all of them,
+// as long as it is held: its own weight becomes the lowest finite one, so that of the kept tokens it leaves first (its
+// increments left out alone, tokens that come after it have weights of 0 and take each other's place, the first slot of equal
+// ones, beside it).
 //
 // Keys and values lie as in the token cache of windowed attention (ring_cache.hip).  The slot of the lowest W is part of
 // the state: whoever changes weights looks for it, in the pass that it makes over them anyway, so that a step knows it
@@ -169,6 +172,10 @@ __device__ __forceinline__ float heavy_base(const HeavyMove& m, int slot, float 
   return slot == m.slot || slot == m.hole ? 0.f : w;
 }
 
+constexpr float HEAVY_LEAST = -3.4028235e38f;  // of a token whose logits are not finite
+// A query beyond it, infinite or NaN is itself what makes a logit so.  (Keys of 128 columns up to 2^57 give finite logits below.)
+constexpr float HEAVY_QUERY = 0x1p64f;
+
 // four slots' weights
 __device__ __forceinline__ floatx4* heavy_weights(const HeavyArgs& a, int sh, int at) {
   return reinterpret_cast<floatx4*>(a.weights + static_cast<int64_t>(sh) * a.pitch + 4 * at);
@@ -181,13 +188,24 @@ __device__ __forceinline__ unsigned long long heavy_grow(const HeavyArgs& a, con
                                                          const float* stat, int stats) {
   constexpr float lift = win_weight_lift<ST>();
   floatx4 grown = floatx4{0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < queries; ++i) {
-    const floatx4 x = *reinterpret_cast<const floatx4*>(logits + i * pitch + 4 * at);
-    const float top = stat[i], inv = stat[stats + i];
+  bool wrong = false, lost[4] = {};
+  auto add = [&](const floatx4& x, float top, float inv) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(x[j] - top, a.r.c, lift)) * inv;
-      grown[j] += win_finite(p) ? p : 0.f;
+    for (int j = 0; j < 4; ++j) grown[j] += __builtin_amdgcn_exp2f(fmaf(x[j] - top, a.r.c, lift)) * inv;
+  };
+  for (int i = 0; i < queries; ++i) {
+    const float inv = stat[stats + i];
+    wrong |= !win_finite(inv);
+    add(*reinterpret_cast<const floatx4*>(logits + i * pitch + 4 * at), stat[i], inv);
+  }
+  if (wrong) {  // a row's sum is 0, or not finite: once more with the others, and is it by one of these tokens
+    grown = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < queries; ++i) {
+      const floatx4 x = *reinterpret_cast<const floatx4*>(logits + i * pitch + 4 * at);
+      const float inv = stat[stats + i];
+      if (win_finite(inv)) add(x, stat[i], inv);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) lost[j] |= !(x[j] < __builtin_inff());
     }
   }
   unsigned long long low = HEAVY_NONE;
@@ -196,7 +214,8 @@ __device__ __forceinline__ unsigned long long heavy_grow(const HeavyArgs& a, con
   for (int j = 0; j < 4; ++j) {
     const int slot = 4 * at + j;
     const bool in = slot < m.held && slot != m.hole;
-    y[j] = in ? heavy_base(m, slot, w[j]) + grown[j] : 0.f;
+    const float base = heavy_base(m, slot, w[j]);
+    y[j] = in ? (lost[j] ? fminf(base, HEAVY_LEAST) : base + grown[j]) : 0.f;
     if (in && slot >= a.ring) low = heavy_min(low, heavy_key(y[j], slot));
   }
   *heavy_weights(a, sh, at) = y;
@@ -410,6 +429,33 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   }
   l += __shfl_xor(l, 16);
   l += __shfl_xor(l, 32);
+  // A row with a logit of +inf or NaN: where the query is at fault no token is, and the wave puts what it has put down of such
+  // a query down once more.
+  if (__any(!win_finite(l))) {
+    constexpr int E = 16 / ES;
+    const char* row = rows_at<ES>(a.q, s, hk * a.group + 16 * chunk + (li < queries ? li : 0), 0);
+    bool sane = true;
+#pragma unroll 1
+    for (int i = 0; i < NBK * ES / 2; ++i) {
+      float y[E];
+      rows_unpack<ST>(rows_chunk<ES>(row, 32 * (i / (ES / 2)) + 8 * lg + E * (i % (ES / 2)), a.d), y);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sane &= fabsf(y[e]) < HEAVY_QUERY;
+    }
+    const unsigned long long odd = __ballot(!sane && li < queries);
+    if (odd >> li & 0x1000100010001ull) {
+      for (int i = wave; i < count; i += 4) {
+        float* const to = h.local ? kept + li * kept_pitch + 4 * lg + 32 * tile(i) : logits + 32 * tile(i);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          floatx4 x = *reinterpret_cast<floatx4*>(to + 16 * half);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x[j] = win_finite(x[j]) ? x[j] : -__builtin_inff();
+          *reinterpret_cast<floatx4*>(to + 16 * half) = x;
+        }
+      }
+    }
+  }
 
   // the four waves' sums
 #pragma unroll

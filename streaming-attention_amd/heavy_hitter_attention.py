@@ -86,8 +86,10 @@ class HeavyHitterStreamingAttention:
     also see keys and values that the streams share and that never leave; their share counts in every weight.
 
     dtype (float32, bfloat16, float16) is that of inputs, outputs and the cache; weights, sums and softmax statistics are
-    fp32.  Increments that are infinite or NaN are left out of the weights, so a token held with such a value, which
-    makes the outputs that it reaches NaN or infinite, is forgotten like others.
+    fp32.  Increments that are infinite or NaN are left out of the weights.  A token whose key gives a logit of +infinity
+    (or beyond fp32) or NaN with a finite query makes the outputs that it reaches NaN while it is held; its weight is the
+    lowest finite one from then on, whatever it was, so it is the first that another token takes the place of.  One whose
+    value alone is infinite or NaN is forgotten like others.
 
     Calls run on the device's current stream and may be captured into graphs (replays advance the state like
     calls); calls on one object have to be ordered, by one stream or by events.  Results take no part in derivatives."""
@@ -249,10 +251,10 @@ class HeavyHitterStreamingAttention:
     @torch.no_grad()
     def start(self, keys: Tensor, values: Tensor, weights: Tensor, *, counts: Optional[Tensor] = None) -> None:
         """Streams begin anew from prompts: keys [S,Hkv,P,dim], values [S,Hkv,P,value_dim] and the weights that their
-        tokens have received, float32 [S,Hkv,P] (received_attention's; an infinite one keeps a token for good, NaN counts
-        as 0).  The last `recent` tokens stay, and of the others the `kept` of the largest weights (of equal ones the first), in
-        the order of their positions.  counts: int32 [S] on the device, the rows of every stream that are tokens (None: all P;
-        values above P are taken as P); a stream with none, 0 or less, keeps what it holds."""
+        tokens have received, float32 [S,Hkv,P] (received_attention's; an infinite one keeps a token with a finite key
+        for good, NaN counts as 0).  The last `recent` tokens stay, and of the others the `kept` of the largest weights (of
+        equal ones the first), in the order of their positions.  counts: int32 [S] on the device, the rows of every stream
+        that are tokens (None: all P; values above P are taken as P); a stream with none, 0 or less, keeps what it holds."""
         rows = keys.shape[2] if keys.ndim == 4 else 0
         if rows > MAX_ROWS:
             raise ValueError(f"at most {MAX_ROWS} rows at a time are supported")

@@ -57,3 +57,124 @@ def test_received_weights_of_keys_that_hide(b, h, hk, n, m, d, counts, dtype):
         assert ref.over(got, want) <= 1.0
         got = hha.received_attention(view(q.to(DEV)), view(k.to(DEV)), counts=ints(counts), lse=lse)
         assert ref.over(got, given) <= 1.0
+
+
+def cache_of(dtype, streams=2, heads=4, kv=2, kept=12, recent=5, d=32, dv=24):
+    c = hha.HeavyHitterStreamingAttention(d, dv, streams=streams, heads=heads, kv_heads=kv, kept=kept, recent=recent, dtype=dtype,
+                                          device=DEV)
+    return c, ref.Cache(streams, kv, kept, recent)
+
+
+def token(c, seed):
+    return make(seed, c.dtype, (c.streams, c.heads, c.dim), (c.streams, c.kv_heads, c.dim), (c.streams, c.kv_heads, c.value_dim))
+
+
+def follow(c, want, q, k=None, v=None, prefix=None):
+    """A step or query of both, the statement from the cache's own weights: the same tokens, and weights within their bounds."""
+    want.adopt(c.weights.cpu())
+    kw = {} if prefix is None else dict(prefix=[x.to(DEV) for x in prefix])
+    if k is None:
+        got = c.query(q.to(DEV), **kw)
+    else:
+        got = c.step(q.to(DEV), k.to(DEV), v.to(DEV), **kw)
+        want.update(k, v)
+    want.query(q, 1 / math.sqrt(c.dim), prefix, None if prefix is None else prefix[0].shape[1])
+    weights, bound, positions = want.state()
+    torch.cuda.synchronize()
+    assert torch.equal(c.positions.cpu(), positions)
+    assert ref.over(c.weights, (weights, bound)) <= 1.0
+    return got
+
+
+PATHS = [dict(), dict(heads=40, kv=1, streams=1), dict(heads=16, kv=1, streams=1, kept=1400, recent=9),
+         dict(kept=3000, recent=9, streams=1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, 3e38])
+@pytest.mark.parametrize("prefix", [False, True])
+@pytest.mark.parametrize("kw", PATHS)
+def test_tokens_with_keys_that_are_not_finite_leave_first(kw, prefix, bad, dtype):
+    """Two of the tokens that a full cache holds for their weights, in slots that are not the first."""
+    if bad == 3e38 and dtype == torch.float16:
+        pytest.skip("no such key in fp16")
+    c, want = cache_of(dtype, **kw)
+    n = c.kept + c.recent + 40
+    k, v = make(1, dtype, (c.streams, c.kv_heads, n, c.dim), (c.streams, c.kv_heads, n, c.value_dim))
+    w = torch.rand(c.streams, c.kv_heads, n, generator=torch.Generator().manual_seed(2)) + 1.0
+    k[0, 0, [20, 33], 0], w[0, 0, [20, 33]] = bad, 9.0
+    c.start(k.to(DEV), v.to(DEV), w.to(DEV))
+    want.start(k, v, w)
+    pk, pv = make(3, dtype, (c.kv_heads, 60, c.dim), (c.kv_heads, 60, c.value_dim))
+    for t in range(5):
+        q, k, v = token(c, 10 + t)
+        q[..., 0] = 3.0
+        out = follow(c, want, q, k, v, (pk, pv) if prefix else None)
+        group = c.heads // c.kv_heads
+        # the first step finds them out; the next two send one away each, before their queries
+        assert torch.isfinite(out).all() if t > 1 else out[0, :group].isnan().all()
+        assert torch.isfinite(out[0, group:]).all() and torch.isfinite(out[1:]).all() and torch.isfinite(c.weights).all()
+    assert not {20, 33} & set(c.positions[0, 0].tolist())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tokens_that_come_with_such_keys(dtype):
+    """Two while the cache fills: they hold their slots until it is full, and leave then."""
+    c, want = cache_of(dtype)
+    for t in range(30):
+        q, k, v = token(c, 50 + t)
+        if t in (3, 6):
+            k[1, 0, 5] = math.nan
+        out = follow(c, want, q, k, v)
+        assert torch.isfinite(out[0]).all()
+    assert torch.isfinite(out).all() and not {3, 6} & set(c.positions[1, 0].tolist())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_prompts_with_such_keys(dtype):
+    """All rows that see the key have weights of NaN, so no token a weight; the streams get rid of it all the same."""
+    c, _ = cache_of(dtype)
+    q, k, v = make(4, dtype, (c.streams, c.heads, 40, c.dim), (c.streams, c.kv_heads, 40, c.dim), (c.streams, c.kv_heads, 40, c.value_dim))
+    k[0, 1, 3, 7] = math.nan
+    c.prefill(q.to(DEV), k.to(DEV), v.to(DEV))
+    assert torch.isfinite(c.weights).all() and 3 in c.positions[0, 1].tolist()
+    for t in range(3):
+        out = c.step(*(x.to(DEV) for x in token(c, 80 + t)))
+    assert torch.isfinite(out).all() and 3 not in c.positions[0, 1].tolist()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tokens_without_queries(dtype):
+    """Weights of 0 all over: the first query finds the tokens out."""
+    c, want = cache_of(dtype)
+    for t in range(40):
+        q, k, v = token(c, 200 + t)
+        if t in (2, 9):
+            k[0, 0] = -math.inf
+        c.update(k.to(DEV), v.to(DEV))
+        want.update(k, v)
+    assert torch.equal(c.positions.cpu(), want.state()[2]) and {2, 9} <= set(c.positions[0, 0].tolist())
+    for t in range(4):
+        q, k, v = token(c, 300 + t)
+        out = follow(c, want, q, k, v)
+    assert torch.isfinite(out).all() and not {2, 9} & set(c.positions[0, 0].tolist())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf, 3e38])
+@pytest.mark.parametrize("kw", PATHS)
+def test_queries_that_are_not_finite_blame_no_token(kw, bad, dtype):
+    if bad == 3e38 and dtype == torch.float16:
+        pytest.skip("no such query in fp16")
+    c, want = cache_of(dtype, **kw)
+    n = c.kept + c.recent + 10
+    k, v = make(5, dtype, (c.streams, c.kv_heads, n, c.dim), (c.streams, c.kv_heads, n, c.value_dim))
+    k[:, :, ::3] *= 16.0
+    w = torch.rand(c.streams, c.kv_heads, n, generator=torch.Generator().manual_seed(6))
+    c.start(k.to(DEV), v.to(DEV), w.to(DEV))
+    want.start(k, v, w)
+    for t in range(3):
+        q, k, v = token(c, 400 + t)
+        q[0, 1, 2] = bad
+        follow(c, want, q, k, v)
+        assert c.weights.ge(0).all()
