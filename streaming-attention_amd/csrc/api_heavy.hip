@@ -219,6 +219,9 @@ int sta_heavy_attention(const void* q, const void* k, const void* v, int dtype, 
     set_parts(x, room + w.logits + w.moves + w.part, plan.parts);
     h.prefix = x.part;
     h.prefix_stat = x.stat;
+    h.prefix_lengths = prefix_lengths;
+    h.prefix_rows = x.p;
+    h.per_set = x.per_set;
     if (const int st = run_prefix(x, plan, dtype, 1, s)) return st;
   }
   int st = STA_OK;

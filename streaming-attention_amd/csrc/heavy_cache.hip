@@ -37,6 +37,8 @@ struct HeavyArgs {
   float* stat;
   const float *prefix, *prefix_stat;
   int prefix_parts, part_pitch;
+  const int* prefix_lengths;  // [sets] or null: rows of the prefix that count, of prefix_rows
+  int prefix_rows, per_set;   // per_set: streams that share one
   int alone;             // a workgroup has a key head to itself and finishes it: one split, up to 16 query heads, no prefix
   int local;             // such a workgroup keeps the logits in LDS
 };
@@ -511,6 +513,10 @@ __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel
   }
 }
 
+__device__ __forceinline__ int heavy_prefix_rows(const HeavyArgs& a, int s) {
+  return a.prefix_lengths ? prefix_clamp(a.prefix_lengths[s / a.per_set], a.prefix_rows) : a.prefix_rows;
+}
+
 // Steps that several workgroups share: outputs, 4 groups of 128 threads (a column each) over the partials of a query head,
 // then in workgroups of their own the weights, 2048 slots of a key head each.
 constexpr int HEAVY_SPLITS = 1024, HEAVY_SLOTS = 2048, HEAVY_HEADS = 512;
@@ -568,7 +574,8 @@ __global__ __launch_bounds__(512) void heavy_join_kernel(const HeavyArgs h, int 
       den = 0.f;
       for (int i = 0; i < 8; ++i) den += wave_red[i];
       sum = red[t] + red[128 + t] + red[256 + t] + red[384 + t];
-      store_elem(a.out, head * a.dv + t, ST, held || den != 0.f ? sum / den : 0.f);
+      const bool sees = held || den != 0.f || (h.prefix_parts && heavy_prefix_rows(h, s));
+      store_elem(a.out, head * a.dv + t, ST, sees ? sum / den : 0.f);  // logits of -inf alone: NaN
     }
     return;
   }

@@ -234,7 +234,7 @@ class HeavyHitterStreamingAttention:
     def query(self, query: Tensor, *, prefix: Optional[Tuple[Tensor, Tensor]] = None,
               prefix_lengths: Optional[Tensor] = None) -> Tensor:
         """Attention of one query a head over the tokens held (and the prefix), whose weights grow by it; zero for a stream
-        that holds none."""
+        that has nothing to see."""
         return self._attend(self._rows(query, self._shapes["query"], "query"), None, None, prefix, prefix_lengths)
 
     def update(self, key: Tensor, value: Tensor) -> None:

@@ -178,3 +178,17 @@ def test_queries_that_are_not_finite_blame_no_token(kw, bad, dtype):
         q[0, 1, 2] = bad
         follow(c, want, q, k, v)
         assert c.weights.ge(0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_of_empty_streams_behind_a_prefix_that_hides(dtype):
+    """Rows that are there with logits of -inf alone give NaN, as a softmax of them; no rows at all zero."""
+    c, _ = cache_of(dtype, streams=4)
+    q = token(c, 1)[0]
+    q[..., 0] = 1.0
+    pk, pv = make(2, dtype, (2, c.kv_heads, 60, c.dim), (2, c.kv_heads, 60, c.value_dim))
+    pk[..., 0] = -math.inf
+    got = c.query(q.to(DEV), prefix=(pk.to(DEV), pv.to(DEV)), prefix_lengths=ints([60, 0]))
+    assert got[:2].isnan().all() and got[2:].eq(0).all()
+    got = c.query(q.to(DEV), prefix=(pk.to(DEV), pv.to(DEV)))
+    assert got.isnan().all() and c.weights.eq(0).all()
