@@ -55,11 +55,16 @@ int heavy_shape(sta::HeavyArgs& h, int dtype, int64_t streams, int heads, int kv
 // key heads of 2048 slots of 128: 49 us, 62 with two a compute unit, 8 of 16000 20 and 20, fp32 39 and 49; 8 of 1024 slots in
 // shares of four tiles 12 us, of eight 13, fp32 15 and 21).  Short caches have one, which finishes their key heads in one
 // launch (64 wide, 800 slots 9.1 us, 9.4 shared, 1050 slots 10.3 and 9.4; 128 wide, 430 slots 9.0 and 9.7, 560 slots 12.4 and
-// 11.8 with four query heads; fp32 128 wide, 170 slots 12.4 and 12.6, 300 slots 15 and 12).
+// 11.8 with four query heads; fp32 128 wide, 170 slots 12.4 and 12.6, 300 slots 15 and 12).  Above 128 key heads two shares
+// would leave a second turn half empty, and one is best (17 x 8 key heads of 16000 slots of 128: 193 us, two 253, three 198;
+// 25 x 8: 255, 296 and 307; 31 x 8: 328, 358 and 358).  fp32 has a workgroup a compute unit at a time: three shares of up to
+// 170 key heads take two turns of a third each (17 x 8 of 4096 slots of 128: 178 -> 142 us, 20 x 8 183 -> 150; of 2048 95 ->
+// 83, 64 wide 47 -> 44; of 1024 54 and 53, 64 wide 27 and 29).
 int splits_of(const sta::RingArgs& a, int dtype) {
-  const int64_t work = static_cast<int64_t>(a.streams) * a.kv * a.chunks;
-  if (static_cast<int64_t>(a.tiles) * (a.nbk + a.nbv) <= (dtype == STA_F32 ? 40 : 104)) return 1;
-  const int64_t want = 256 / work, most = (a.tiles + 3) / 4, split = want < most ? want : most;
+  const int64_t work = static_cast<int64_t>(a.streams) * a.kv * a.chunks, blocks = static_cast<int64_t>(a.tiles) * (a.nbk + a.nbv);
+  if (blocks <= (dtype == STA_F32 ? 40 : 104)) return 1;
+  const bool thirds = dtype == STA_F32 && work > 128 && 3 * work <= 512 && blocks >= 256;
+  const int64_t want = thirds ? 3 : 256 / work, most = (a.tiles + 3) / 4, split = want < most ? want : most;
   return static_cast<int>(split < 1 ? 1 : split);
 }
 

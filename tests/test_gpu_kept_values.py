@@ -70,7 +70,8 @@ def token(c, seed):
 
 
 def follow(c, want, q, k=None, v=None, prefix=None):
-    """A step or query of both, the statement from the cache's own weights: the same tokens, and weights within their bounds."""
+    """A step or query of both, the statement from the cache's own weights: the same tokens, outputs and weights within their
+    bounds."""
     want.adopt(c.weights.cpu())
     kw = {} if prefix is None else dict(prefix=[x.to(DEV) for x in prefix])
     if k is None:
@@ -78,7 +79,9 @@ def follow(c, want, q, k=None, v=None, prefix=None):
     else:
         got = c.step(q.to(DEV), k.to(DEV), v.to(DEV), **kw)
         want.update(k, v)
-    want.query(q, 1 / math.sqrt(c.dim), prefix, None if prefix is None else prefix[0].shape[1])
+    value, near = want.query(q, 1 / math.sqrt(c.dim), prefix, None if prefix is None else prefix[0].shape[1])
+    fine = torch.isfinite(value).all(-1)
+    assert ref.over(got.cpu()[fine], (value[fine], near[fine])) <= 1.0 and not torch.isfinite(got.cpu()[~fine]).any()
     weights, bound, positions = want.state()
     torch.cuda.synchronize()
     assert torch.equal(c.positions.cpu(), positions)
@@ -192,3 +195,16 @@ def test_queries_of_empty_streams_behind_a_prefix_that_hides(dtype):
     assert got[:2].isnan().all() and got[2:].eq(0).all()
     got = c.query(q.to(DEV), prefix=(pk.to(DEV), pv.to(DEV)))
     assert got.isnan().all() and c.weights.eq(0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kv", [129, 171])
+def test_more_key_heads_than_half_the_compute_units(kv, dtype):
+    c, want = cache_of(dtype, streams=1, heads=kv, kv=kv, kept=1190, recent=9, d=96, dv=100)
+    k, v = make(7, dtype, (1, kv, 1230, c.dim), (1, kv, 1230, c.value_dim))
+    w = torch.rand(1, kv, 1230, generator=torch.Generator().manual_seed(8))
+    c.start(k.to(DEV), v.to(DEV), w.to(DEV))
+    want.start(k, v, w)
+    for t in range(2):
+        q, k, v = token(c, 500 + t)
+        follow(c, want, q, k, v)

@@ -47,3 +47,16 @@ def test_a_query_that_is_not_finite_is_not_theirs():
     before = cache.state()[0]
     assert cache.query(torch.full((1, 1, 8), math.nan), 1.0)[0].isnan().all()
     assert torch.equal(cache.state()[0], before)
+
+
+def test_shares_of_more_key_heads_than_half_the_compute_units():
+    """float32 key heads of long caches are shared by three workgroups up to 170 of them; a workspace for partials says so."""
+    import _native
+
+    def shared(dtype, streams, kept):
+        pitch = (kept + 33 + 31) // 32 * 32
+        return _native.load_library().sta_heavy_attention_bytes(dtype, streams, 8, 8, 128, 128, 32, kept, 0, 0) > 4 * streams * 8 * pitch
+
+    assert shared(0, 16, 2015) and shared(0, 17, 2015) and shared(0, 21, 2015)
+    assert not shared(0, 22, 2015) and not shared(0, 32, 2015) and not shared(0, 17, 700)
+    assert shared(1, 16, 2015) and not shared(1, 17, 2015) and not shared(2, 17, 16000)
