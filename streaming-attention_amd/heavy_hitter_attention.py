@@ -86,7 +86,9 @@ class HeavyHitterStreamingAttention:
     also see keys and values that the streams share and that never leave; their share counts in every weight.
 
     dtype (float32, bfloat16, float16) is that of inputs, outputs and the cache; weights, sums and softmax statistics are
-    fp32.  Increments that are infinite or NaN are left out of the weights.  A token whose key gives a logit of +infinity
+    fp32.  A weight is a plain fp32 sum: what a query adds to it is rounded at 2^-24 of the weight, so that weights order what
+    differs by more than n 2^-24 of them after n queries, and one does not grow past 2^24 times what each query adds.
+    Increments that are infinite or NaN are left out of the weights.  A token whose key gives a logit of +infinity
     (or beyond fp32) or NaN with a finite query makes the outputs that it reaches NaN while it is held; its weight is the
     lowest finite one from then on, whatever it was, so it is the first that another token takes the place of.  One whose
     value alone is infinite or NaN is forgotten like others.

@@ -208,3 +208,32 @@ def test_more_key_heads_than_half_the_compute_units(kv, dtype):
     for t in range(2):
         q, k, v = token(c, 500 + t)
         follow(c, want, q, k, v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("first", [0.0, 1000.0, 3.0e5])
+@pytest.mark.parametrize("kw", PATHS[:1] + PATHS[3:])
+def test_weights_are_fp32_sums(kw, first, dtype):
+    """Many queries without tokens between them: every addition rounds at 2^-24 of the weight that comes out, and what a query
+    adds is as near as a step's is."""
+    c, _ = cache_of(dtype, **kw)
+    n, queries, scale = c.recent + c.kept, 300, 1 / math.sqrt(c.dim)
+    k, v = make(9, dtype, (c.streams, c.kv_heads, n, c.dim), (c.streams, c.kv_heads, n, c.value_dim))
+    c.start(k.to(DEV), v.to(DEV), torch.full((c.streams, c.kv_heads, n), first, device=DEV))
+    q = make(10, dtype, (queries, c.streams, c.heads, c.dim))[0]
+    for t in range(queries):
+        c.query(q[t].to(DEV))
+    group = c.heads // c.kv_heads
+    rows = q.double().view(queries, c.streams, c.kv_heads, group, c.dim).permute(1, 2, 0, 3, 4).flatten(2, 3)
+    p, _, rel, _ = zip(*(ref._weights(rows[s, h], k[s, h].double(), torch.zeros(rows.shape[2], n, dtype=torch.bool), scale, c.dim)
+                         for s in range(c.streams) for h in range(c.kv_heads)))
+    p, rel = torch.stack(p), torch.stack(rel)
+    want = (first + p.sum(1)).view(c.streams, c.kv_heads, n)
+    near = ((p * (2 * rel + ref.F24 * (group + 8))).sum(1)).view(want.shape) + queries * ref.F24 * want
+    at = c.positions.cpu()
+    assert (at >= 0).sum(-1).eq(n).all()
+    for s in range(c.streams):
+        for h in range(c.kv_heads):
+            held = at[s, h] >= 0
+            got = c.weights[s, h].cpu()[held]
+            assert ref.over(got, (want[s, h][at[s, h][held]], near[s, h][at[s, h][held]])) <= 1.0
