@@ -246,7 +246,7 @@ __host__ __device__ constexpr int64_t heavy_lds_bytes(int group, int nbv, int pi
 template <int NBK, int NBV, int ST>
 __global__ __launch_bounds__(256, ST == F32 ? 1 : 2) void heavy_attention_kernel(const HeavyArgs h) {
   const RingArgs& a = h.r;
-  constexpr int PP = ST == F32 ? 1 : 2;  // planes of the weights, see ring_cache.hip
+  constexpr int PP = ST == F32 ? 1 : 2;  // planes of the weights, see ring_cache.hip (a prefix has one, see prefix_attn.hip)
   constexpr int ES = ST == F32 ? 4 : 2, CT = 2 * NBV, W = RingTile<NBK, NBV, ST>::W;
   constexpr int PITCH = heavy_red_pitch(NBV);
   extern __shared__ float heavy_lds[];  // [4][queries][PITCH] for the waves' sums, then the logits if they are kept here

@@ -10,7 +10,10 @@
 // The rows of a "unit" of `span` sequences and one key head lie in the order (sequence, row, query head of the group): the
 // query heads of a key head, and with span > 1 the sequences of a set, are rows of one product with the keys that
 // they share.  A workgroup takes 128 (shared tiles: 32) rows and a share of the unit's key tiles; its walk is the one of
-// window_forward_kernel, whose tiles, layouts and second pass for results that are not finite it uses.
+// window_forward_kernel, whose tiles, layouts and second pass for results that are not finite it uses.  Weights of 16-bit rows
+// are rounded to their type for the value product (half a step each; sums of weights and received weights are not): outputs
+// are off by 0.0023 of their deviation in bf16, 0.0017 with fp32 weights, which is the output's own rounding; fp16 2.9e-4 and
+// 2.1e-4.  A second plane of the weights would make three products of two, and products are what bounds large calls.
 #pragma once
 #include "window_attn.hip"
 
@@ -843,9 +846,10 @@ __device__ __forceinline__ void received_add(float& total, float& lost, const fl
 // The weights that keys receive.  A workgroup holds 32 to 64 keys a wave as operands and walks over its share of the rows
 // that see one of them, head by head of the group; with X = Q K^T a lane has 16 rows of one key, whose weights it sums: no
 // exchange between lanes until the end.  Sums of 16 go into a compensated total (16384 x 4 rows).  32 heads of 16384 rows,
-// 128 wide: 1.14 ms, 965 TFLOP/s (a large matrix product 1200); 64 wide 0.75 ms, bound by the exponentials.
+// 128 wide: 1.04 to 1.10 ms by card, 1000 to 1060 TFLOP/s (a large matrix product 1200 to 1390); 64 wide 0.75 ms, bound by the
+// exponentials.
 // STREAM: 16-bit rows of whole 16 bytes go from memory to LDS directly, a tile ahead in two buffers, with one
-// barrier a tile, and leave room for a third wave a SIMD (1.32 -> 1.22 -> 1.14 ms, 965 TFLOP/s).
+// barrier a tile, and leave room for a third wave a SIMD (on one card 1.32 -> 1.22 -> 1.14 ms).
 template <int P, int IN, bool STREAM>
 __device__ __forceinline__ void received_walk(const ReceivedArgs& w, int id, uint4* __restrict__ qs0, uint4* __restrict__ qs1,
                                               float* __restrict__ stat0, float* __restrict__ stat1) {
